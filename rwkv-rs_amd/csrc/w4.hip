@@ -1,0 +1,309 @@
+// Products with 4-bit weights, and quantising and restoring them
+// (include/rwkv_w4.h).
+//
+// linear: y[m, n] = sum over groups G of s[n, G] * sum over k in G of x[m, k] v[n, k].
+// The values v are small bf16 numbers, so the inner sums are matrix
+// instructions on bf16 operands whose products are exact; a group's sum is
+// multiplied by its scale in fp32 and added to the total.
+#include <algorithm>
+
+#include "w4_device.hpp"
+
+namespace rwkv_w4 {
+namespace {
+
+constexpr int kWave = 64;
+
+// Elements i .. i + 7 of a row of n, those past its end zero. kVector: n and i
+// are multiples of 8 and the row begins on 16 bytes.
+template <bool BF, bool kVector>
+__device__ __forceinline__ void load8(const void* row, int64_t i, int64_t n, float (&v)[8]) {
+  if (kVector) {
+    if (i >= n) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    } else if constexpr (BF) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(row) + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[2 * e] = __builtin_bit_cast(float, w[e] << 16);
+        v[2 * e + 1] = __builtin_bit_cast(float, w[e] & 0xffff0000u);
+      }
+    } else {
+      const f32x4* const p = reinterpret_cast<const f32x4*>(static_cast<const float*>(row) + i);
+      const f32x4 a = p[0], b = p[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = a[e];
+        v[4 + e] = b[e];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (i + e >= n) v[e] = 0.f;
+      else if constexpr (BF) v[e] = bf_bits(static_cast<const uint16_t*>(row)[i + e]);
+      else v[e] = static_cast<const float*>(row)[i + e];
+    }
+  }
+}
+
+template <bool BF, bool kVector>
+__device__ __forceinline__ void store8(void* row, int64_t i, int64_t n, const float (&v)[8]) {
+  if (kVector) {
+    if (i >= n) return;
+    if constexpr (BF) {
+      bf16x8 w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = static_cast<__bf16>(v[e]);
+      *reinterpret_cast<bf16x8*>(static_cast<uint16_t*>(row) + i) = w;
+    } else {
+      f32x4* const p = reinterpret_cast<f32x4*>(static_cast<float*>(row) + i);
+      p[0] = f32x4{v[0], v[1], v[2], v[3]};
+      p[1] = f32x4{v[4], v[5], v[6], v[7]};
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (i + e >= n) return;
+      if constexpr (BF) static_cast<__bf16*>(row)[i + e] = static_cast<__bf16>(v[e]);
+      else static_cast<float*>(row)[i + e] = v[e];
+    }
+  }
+}
+
+__device__ __forceinline__ char* row_at(void* base, int64_t row, int64_t n, bool bf) {
+  return static_cast<char*>(base) + row * n * (bf ? 2 : 4);
+}
+
+// ---------------------------------------------------------- quantise, restore
+// A wave takes a block of 16 outputs and 128 inputs, lane l the output l % 16
+// at the inputs 32 j + 8 (l / 16) .. + 7 of each j, which are its 16 bytes of
+// the packed block; four lanes hold 32 consecutive inputs of an output.
+constexpr int kBlockWaves = 4;
+
+// Nearest magnitude, ties to the even mantissa: the midpoints times the scale
+// are exact in fp32 (three significant bits by eight), so no quotient is rounded.
+__device__ __forceinline__ uint32_t code_of(float w, float s) {
+  const float a = fabsf(w);
+  const uint32_t c = (a > 0.25f * s) + (a >= 0.75f * s) + (a > 1.25f * s) + (a >= 1.75f * s) + (a > 2.5f * s) +
+                     (a >= 3.5f * s) + (a > 5.f * s);
+  return c | (c && w < 0.f ? 8u : 0u);
+}
+
+constexpr uint32_t kMaxScale = 0x7e2a;   // the largest bf16 number six times which is an fp32 number
+
+template <bool BF, bool kVector, int kGroup>
+__global__ __launch_bounds__(kBlockWaves* kWave) void quantize_kernel(const WeightCall c) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int64_t ib = blocks_in(c.in), blocks = blocks_out(c.out) * ib;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kBlockWaves;
+  for (int64_t b = static_cast<int64_t>(blockIdx.x) * kBlockWaves + (threadIdx.x >> 6); b < blocks; b += stride) {
+    const int64_t n = b / ib, k = b % ib, row = n * kRows + r;
+    float w[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (row < c.out) {
+        load8<BF, kVector>(row_at(c.weight, row, c.in, BF), k * kInputs + 32 * j + 8 * g, c.in, w[j]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[j][e] = 0.f;
+      }
+    }
+    // the largest magnitude as an integer: infinities and NaN are above all numbers
+    uint32_t top[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      top[j] = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top[j] = max(top[j], __builtin_bit_cast(uint32_t, w[j][e]) & 0x7fffffffu);
+    }
+    constexpr int kGroups = kInputs / kGroup, kSteps = kGroup / 32;
+    uint16_t scale[kGroups];
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) {
+      uint32_t t = top[q * kSteps];
+#pragma unroll
+      for (int j = 1; j < kSteps; ++j) t = max(t, top[q * kSteps + j]);
+      t = max(t, static_cast<uint32_t>(__shfl_xor(static_cast<int>(t), 16)));
+      t = max(t, static_cast<uint32_t>(__shfl_xor(static_cast<int>(t), 32)));
+      const float s = __builtin_bit_cast(float, t) * (1.f / 6.f);
+      const uint32_t rounded = __builtin_bit_cast(uint16_t, static_cast<__bf16>(s));
+      scale[q] = static_cast<uint16_t>(t >= 0x7f800000u ? 0x7fc0u : min(rounded, kMaxScale));
+    }
+    u32x4 word;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float s = bf_bits(scale[j / kSteps]);
+      word[j] = 0;
+      if (s > 0.f)   // not 0, and not NaN
+#pragma unroll
+        for (int e = 0; e < 8; ++e) word[j] |= code_of(w[j][e], s) << (4 * e);
+    }
+    reinterpret_cast<u32x4*>(c.packed)[b * kWave + lane] = word;
+    if (g == 0)
+#pragma unroll
+      for (int q = 0; q < kGroups; ++q) static_cast<uint16_t*>(c.scales)[(b * kRows + r) * kGroups + q] = scale[q];
+  }
+}
+
+template <bool BF, bool kVector, int kGroup>
+__global__ __launch_bounds__(kBlockWaves* kWave) void dequantize_kernel(const WeightCall c) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int64_t ib = blocks_in(c.in), blocks = blocks_out(c.out) * ib;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kBlockWaves;
+  for (int64_t b = static_cast<int64_t>(blockIdx.x) * kBlockWaves + (threadIdx.x >> 6); b < blocks; b += stride) {
+    const int64_t n = b / ib, k = b % ib, row = n * kRows + r;
+    if (row >= c.out) continue;
+    const u32x4 word = reinterpret_cast<const u32x4*>(c.packed)[b * kWave + lane];
+    float s[kInputs / kGroup];
+    load_scales<kGroup>(c.scales, b * kRows + r, s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bf16x8 v = weights8(word[j]);
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = kShrink * static_cast<float>(v[e]) * s[32 * j / kGroup];
+      store8<BF, kVector>(row_at(c.weight, row, c.in, BF), k * kInputs + 32 * j + 8 * g, c.in, w);
+    }
+  }
+}
+
+// --------------------------------------------------------------------- linear
+// A workgroup forms 16 outputs of up to 16 MT rows; its eight waves split the
+// inputs in blocks of 128 (one 16-byte load of weights a lane, four matrix
+// instructions a row tile) and add up through LDS in wave order.
+// v_mfma_f32_16x16x32_bf16: lane l holds A[row l % 16] and B[column l % 16] at
+// k = 8 (l / 16) .. + 7, the result D[row 4 (l / 16) + r][column l % 16].
+constexpr int kLinearWaves = 8;
+
+template <bool BF, bool kVector>
+__device__ __forceinline__ auto load_x(const void* row, int64_t i, int64_t n) {
+  if constexpr (BF && kVector) {
+    Parts<1> p;
+    if (i < n) {
+      p.p[0] = *reinterpret_cast<const bf16x8*>(static_cast<const uint16_t*>(row) + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p.p[0][e] = static_cast<__bf16>(0.f);
+    }
+    return p;
+  } else {
+    float v[8];
+    load8<BF, kVector>(row, i, n, v);
+    if constexpr (BF) {
+      Parts<1> p;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p.p[0][e] = static_cast<__bf16>(v[e]);
+      return p;
+    } else {
+      return split(v);
+    }
+  }
+}
+
+template <bool BF, bool kVector, int kGroup, int MT>
+__global__ __launch_bounds__(kLinearWaves* kWave) void linear_kernel(const LinearCall c) {
+  __shared__ float part[kLinearWaves][MT * 256];
+  constexpr int kParts = BF ? 1 : 3, kSteps = kGroup / 32;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = lane & 15, g = lane >> 4;
+  const int64_t n = blockIdx.x, ib = blocks_in(c.in);
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.y) * 16 * MT; row0 < c.rows;
+       row0 += static_cast<int64_t>(gridDim.y) * 16 * MT) {
+    f32x4 acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int64_t k = wave; k < ib; k += kLinearWaves) {
+      const int64_t b = n * ib + k;
+      const u32x4 word = reinterpret_cast<const u32x4*>(c.packed)[b * kWave + lane];
+      float s[kInputs / kGroup];
+      load_scales<kGroup>(c.scales, b * kRows + t, s);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int64_t row = min(row0 + 16 * m + t, c.rows - 1);
+        const void* const x = row_at(const_cast<void*>(c.x), row, c.in, BF);
+        f32x4 sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const Parts<kParts> xs = load_x<BF, kVector>(x, k * kInputs + 32 * j + 8 * g, c.in);
+          const bf16x8 w = weights8(word[j]);
+          if (j % kSteps == 0) sum = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = kParts - 1; i >= 0; --i) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xs.p[i], w, sum, 0, 0, 0);
+          if (j % kSteps == kSteps - 1) acc[m] += sum * s[32 * j / kGroup];
+        }
+      }
+    }
+    __syncthreads();   // the sums of the rows before are read
+#pragma unroll
+    for (int m = 0; m < MT; ++m) *reinterpret_cast<f32x4*>(&part[wave][m * 256 + 4 * lane]) = acc[m];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * 256; i += kLinearWaves * kWave) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < kLinearWaves; ++w) v += part[w][i];
+      v *= kShrink;
+      const int l = (i >> 2) & 63;
+      const int64_t row = row0 + 16 * (i >> 8) + 4 * (l >> 4) + (i & 3), col = n * kRows + (l & 15);
+      if (row >= c.rows || col >= c.out) continue;
+      if constexpr (BF) static_cast<__bf16*>(c.y)[row * c.out + col] = static_cast<__bf16>(v);
+      else static_cast<float*>(c.y)[row * c.out + col] = v;
+    }
+  }
+}
+
+// ----------------------------------------------------------------- dispatch
+template <typename F>
+hipError_t by_group(int group, F&& f) {
+  if (group == 32) f(std::integral_constant<int, 32>());
+  else if (group == 64) f(std::integral_constant<int, 64>());
+  else f(std::integral_constant<int, 128>());
+  return hipGetLastError();
+}
+template <typename F>
+hipError_t by_form(bool bf16, bool vector, int group, F&& f) {
+  return by_group(group, [&](auto g) {
+    if (bf16) vector ? f(std::true_type(), std::true_type(), g) : f(std::true_type(), std::false_type(), g);
+    else vector ? f(std::false_type(), std::true_type(), g) : f(std::false_type(), std::false_type(), g);
+  });
+}
+
+bool vector_rows(const void* p, int64_t n) { return n % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// enough workgroups for every compute unit's waves; each takes several blocks beyond that
+unsigned block_grid(const WeightCall& c) {
+  const int64_t blocks = blocks_out(c.out) * blocks_in(c.in);
+  return static_cast<unsigned>(std::min<int64_t>((blocks + kBlockWaves - 1) / kBlockWaves, 1 << 20));
+}
+
+}  // namespace
+
+hipError_t launch_quantize(const WeightCall& c, hipStream_t stream) {
+  return by_form(c.bf16, vector_rows(c.weight, c.in), c.group, [&](auto bf, auto vec, auto group) {
+    hipLaunchKernelGGL((quantize_kernel<bf(), vec(), group()>), dim3(block_grid(c)), dim3(kBlockWaves * kWave), 0,
+                       stream, c);
+  });
+}
+
+hipError_t launch_dequantize(const WeightCall& c, hipStream_t stream) {
+  return by_form(c.bf16, vector_rows(c.weight, c.in), c.group, [&](auto bf, auto vec, auto group) {
+    hipLaunchKernelGGL((dequantize_kernel<bf(), vec(), group()>), dim3(block_grid(c)), dim3(kBlockWaves * kWave), 0,
+                       stream, c);
+  });
+}
+
+hipError_t launch_linear(const LinearCall& c, hipStream_t stream) {
+  return by_form(c.bf16, vector_rows(c.x, c.in), c.group, [&](auto bf, auto vec, auto group) {
+    auto go = [&](auto mt) {
+      const int64_t tiles = (c.rows + 16 * mt() - 1) / (16 * mt());
+      const dim3 grid(static_cast<unsigned>(blocks_out(c.out)), static_cast<unsigned>(std::min<int64_t>(tiles, 65535)));
+      hipLaunchKernelGGL((linear_kernel<bf(), vec(), group(), mt()>), grid, dim3(kLinearWaves * kWave), 0, stream, c);
+    };
+    if (c.rows <= 16) go(std::integral_constant<int, 1>());
+    else if (c.rows <= 32) go(std::integral_constant<int, 2>());
+    else go(std::integral_constant<int, 4>());
+  });
+}
+
+}  // namespace rwkv_w4

@@ -1,0 +1,283 @@
+"""4-bit weights on the GPU against plain float64 restatements: quantising and
+restoring bit for bit, products within the rounding of fp32 sums."""
+
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+from conftest import announce, load_pkg
+
+pytestmark = pytest.mark.gpu
+pkg = load_pkg()
+w4 = pkg.w4
+MAGNITUDES = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
+GROUPS = (32, 64, 128)
+
+
+def ref_quantize(w, group):
+    """Scales [out, groups] (fp32 of bf16) and codes [out, in padded to 128], on the CPU."""
+    out, d_in = w.shape
+    w = torch.nn.functional.pad(w.float().cpu(), (0, -d_in % 128)).view(out, -1, group)
+    top = w.abs().amax(2)
+    scale = (top * (1.0 / 6.0)).to(torch.bfloat16).float()
+    limit = torch.finfo(torch.float32).max / 6                         # of a scale whose weights fp32 holds
+    scale = torch.where(scale > limit, torch.tensor(0x7e2a, dtype=torch.int16).view(torch.bfloat16).float(), scale)
+    bad = ~torch.isfinite(w).all(2)
+    scale[bad] = math.nan
+    s, a = scale.double().unsqueeze(2), w.abs().double()
+    ratio = torch.where(s > 0, a / s, torch.zeros_like(a)).clamp(max=7.0)
+    dist = (ratio.unsqueeze(3) - MAGNITUDES).abs()
+    # nearest; of two equally near the one with an even mantissa bit (an even code)
+    near = dist == dist.min(3, keepdim=True).values
+    even = near & (torch.arange(8) % 2 == 0)
+    pick = torch.where(even.any(3, keepdim=True), even, near)
+    code = pick.int().argmax(3)
+    code[~(s > 0).expand_as(code)] = 0
+    code = torch.where((w < 0) & (code > 0), code + 8, code)
+    return scale, code.reshape(out, -1)
+
+
+def ref_values(scale, code, d_in):
+    out = code.shape[0]
+    v = MAGNITUDES[code & 7] * torch.where(code > 7, -1.0, 1.0)
+    return (v.view(out, scale.shape[1], -1) * scale.double().unsqueeze(2)).view(out, -1)[:, :d_in]
+
+
+def ref_pack(code):
+    """include/rwkv_w4.h's layout, byte by byte."""
+    out, d_in = code.shape
+    n, k = -(-out // 16), d_in // 128
+    full = torch.zeros(16 * n, d_in, dtype=torch.int64)
+    full[:out] = code
+    N, K, g, r, j, b = (torch.arange(x).view([-1 if i == a else 1 for i in range(6)])
+                        for a, x in enumerate((n, k, 4, 16, 4, 4)))
+    low = full[16 * N + r, 128 * K + 32 * j + 8 * g + 2 * b]
+    high = full[16 * N + r, 128 * K + 32 * j + 8 * g + 2 * b + 1]
+    return (low | high << 4).view(n, k, 4, 16, 16).to(torch.uint8)
+
+
+def rand(*shape, seed, dtype=torch.float32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 1), (16, 128), (17, 129), (5, 4), (33, 96), (129, 1000), (256, 768), (40, 72)])
+def test_quantize_and_restore(shape, dtype, group):
+    announce("w4 quantize", shape, dtype, group)
+    w = rand(*shape, seed=1, dtype=dtype, scale=0.02)
+    q = w4.quantize(w, group)
+    scale, code = ref_quantize(w, group)
+    assert torch.equal(q.packed.cpu(), ref_pack(code))
+    n, k = q.packed.shape[:2]
+    got = q.scales.cpu().float().transpose(1, 2).reshape(16 * n, -1)
+    assert torch.equal(got[:shape[0]], scale) and not got[shape[0]:].any()
+    want = ref_values(scale, code, shape[1])
+    assert torch.equal(w4.dequantize(q).cpu().double(), want)          # exact in fp32
+    assert torch.equal(w4.dequantize(q, torch.bfloat16).cpu(), want.float().to(torch.bfloat16))
+
+
+def test_quantize_edges():
+    """Midpoints, saturation, signed zeros, empty and denormal groups, infinities and NaN."""
+    announce("w4 quantize edges")
+    w = torch.zeros(8, 64)
+    mids = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    w[0, :7], w[0, 7:14], w[0, 20] = mids, -mids, 6.0                  # scale exactly 1
+    w[1, :14] = torch.nextafter(torch.cat([mids, mids]), torch.tensor([9.0] * 7 + [0.0] * 7))
+    w[1, 20] = -6.0
+    w[2, 3] = -0.0
+    w[3, :4] = torch.tensor([1e-38, -1e-39, 1e-45, 3e-39])
+    w[4, 1], w[4, 40] = math.inf, 1.0
+    w[5, 33], w[5, 2] = math.nan, 1.0
+    w[6, 0], w[6, 1] = 3.4e38, -1e38
+    w[7, 0] = 1e-45                                                     # its scale rounds to zero
+    q = w4.quantize(w.cuda(), 32)
+    scale, code = ref_quantize(w, 32)
+    assert torch.equal(q.packed.cpu(), ref_pack(code))
+    got, want = w4.dequantize(q).cpu().double(), ref_values(scale, code, 64)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(), want.nan_to_num())
+    assert got[4, :32].isnan().all() and got[4, 40] == 6 * float(torch.tensor(1 / 6).bfloat16()) and got[5, 33:].isnan().all()
+    assert got[0, :7].tolist() == [0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0]
+    assert got[1, :7].tolist() == [0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+    assert got[1, 7:14].tolist() == [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0]
+
+
+def check_linear(x, q, d_out, d_in):
+    """Against float64 products of the same values. A sum of K products in fp32,
+    in any order and however a matrix instruction rounds inside (one unit in the
+    last place, 2^-23, for each addition), is off by at most (K + 8) 2^-23 sum
+    |x w|; fp32 parts lose 2^-23 |x w| more; the result is rounded once."""
+    y = w4.linear(x, q)
+    assert y.dtype == x.dtype and y.shape == (*x.shape[:-1], d_out)
+    w = w4.dequantize(q).cpu().double()
+    xd = x.cpu().double()
+    want, mass = xd @ w.t(), xd.abs() @ w.abs().t()
+    last = 2.0 ** -8 if x.dtype == torch.bfloat16 else 2.0 ** -23
+    err = (y.cpu().double() - want).abs()
+    bound = (d_in + 9) * 2.0 ** -23 * mass + last * want.abs() + 1e-37
+    assert (err <= bound).all(), float((err / bound).max())
+    # and as a whole far nearer than that bound
+    rel = float(err.norm() / want.norm().clamp(min=1e-300))
+    assert rel <= (2.0 ** -8 if x.dtype == torch.bfloat16 else 2e-6), rel
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,d_out,d_in,group", [
+    (1, 16, 128, 32), (1, 1, 1, 64), (1, 768, 768, 64), (2, 100, 300, 128), (3, 777, 1000, 32),
+    (7, 64, 64, 64), (8, 48, 1024, 128), (16, 33, 129, 64), (17, 256, 768, 128), (31, 80, 416, 32),
+    (33, 130, 2048, 64), (64, 512, 256, 32), (65, 96, 640, 64), (100, 300, 333, 128),
+    (129, 128, 512, 64), (257, 200, 1152, 32), (300, 1000, 200, 128), (1, 40, 9000, 64)])
+def test_linear(rows, d_out, d_in, group, dtype):
+    announce("w4 linear", rows, d_out, d_in, group, dtype)
+    q = w4.quantize(rand(d_out, d_in, seed=2, scale=0.05), group)
+    check_linear(rand(rows, d_in, seed=3, dtype=dtype), q, d_out, d_in)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 20, 200])
+def test_linear_hears_every_element(rows, dtype):
+    """One activation at a time: the outputs are the weights of its input, exactly."""
+    announce("w4 linear one-hot", rows, dtype)
+    d_out, d_in = 50, 200
+    q = w4.quantize(rand(d_out, d_in, seed=4), 32)
+    w = w4.dequantize(q, dtype)
+    for k0 in range(0, d_in, rows):
+        ks = torch.arange(k0, k0 + rows, device="cuda") % d_in
+        x = torch.zeros(rows, d_in, device="cuda", dtype=dtype)
+        x[torch.arange(rows), ks] = 1.0
+        assert torch.equal(w4.linear(x, q), w.t()[ks])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 19, 150])
+@pytest.mark.parametrize("d_in", [256, 203])
+def test_linear_infinities_and_nan_stay_in_their_rows(rows, d_in, dtype):
+    announce("w4 linear non-finite", rows, d_in, dtype)
+    d_out = 70
+    q = w4.quantize(rand(d_out, d_in, seed=5), 64)
+    w = w4.dequantize(q).cpu().double()
+    x = rand(rows, d_in, seed=6, dtype=dtype)
+    x[0, 3] = math.inf
+    if rows > 1:
+        x[1, 5], x[1, 9], x[2, 7], x[3, d_in - 1] = math.inf, -math.inf, math.nan, -math.inf
+        x[4, 0] = torch.finfo(dtype).max
+    y, want = w4.linear(x, q).cpu().double(), x.cpu().double() @ w.t()
+    assert torch.equal(y.isnan(), want.isnan())
+    assert torch.equal(y == math.inf, want.to(dtype) == math.inf)
+    assert torch.equal(y == -math.inf, want.to(dtype) == -math.inf)
+    fine = y.isfinite()
+    assert torch.allclose(y[fine], want[fine], rtol=2.0 ** -7, atol=1e-3)
+
+
+def test_a_nan_group_reaches_its_output_only():
+    announce("w4 linear NaN weight")
+    w = rand(40, 300, seed=7)
+    w[11, 170] = math.nan
+    q = w4.quantize(w, 64)
+    y = w4.linear(rand(3, 300, seed=8), q)
+    assert y[:, 11].isnan().all() and y.isnan().sum() == 3
+
+
+def test_fp32_activations_of_every_size():
+    """x is cut into three bf16 parts: nothing is lost from 2^-100 to 2^120."""
+    announce("w4 linear fp32 range")
+    q = w4.quantize(torch.eye(64, device="cuda") * 6.0, 32)          # 6 on the diagonal, scale 1
+    x = rand(1, 64, seed=9) * torch.exp2(torch.linspace(-100, 120, 64, device="cuda"))
+    y = w4.linear(x, q)
+    assert torch.allclose(y, 6.0 * x, rtol=2.0 ** -22, atol=0.0)
+
+
+def test_linear_results_do_not_depend_on_the_call():
+    """The same row, alone and among others of the same launch, again and again."""
+    announce("w4 linear repeat")
+    q = w4.quantize(rand(512, 768, seed=10), 64)
+    x = rand(13, 768, seed=11, dtype=torch.bfloat16)
+    y = w4.linear(x, q)
+    for _ in range(3):
+        assert torch.equal(w4.linear(x, q), y)
+    assert torch.equal(w4.linear(x[4:5], q), y[4:5])
+
+
+def test_linear_shapes_strides_and_empty_calls():
+    announce("w4 linear shapes")
+    q = w4.quantize(rand(24, 136, seed=12), 64)
+    x = rand(2, 3, 136, seed=13, dtype=torch.bfloat16)
+    y = w4.linear(x, q)
+    assert y.shape == (2, 3, 24) and torch.equal(y.view(6, 24), w4.linear(x.view(6, 136), q))
+    assert torch.equal(w4.linear(x[:, -1], q), y[:, -1])                       # strided rows
+    wide = rand(3, 272, seed=14, dtype=torch.bfloat16)
+    assert torch.equal(w4.linear(wide[:, ::2], q), w4.linear(wide[:, ::2].contiguous(), q))
+    flat = rand(137, seed=15, dtype=torch.bfloat16)
+    assert torch.equal(w4.linear(flat[1:], q), w4.linear(flat[1:].clone(), q))  # begins anywhere
+    assert w4.linear(x[:0], q).shape == (0, 3, 24)
+    w = rand(24 * 136 + 1, seed=16)[1:].view(24, 136)
+    assert torch.equal(w4.quantize(w).packed, w4.quantize(w.clone()).packed)
+    wt = rand(136, 24, seed=17).t()
+    assert torch.equal(w4.quantize(wt).packed, w4.quantize(wt.contiguous()).packed)
+
+
+def test_linear_on_another_stream_and_in_a_graph():
+    announce("w4 linear stream and graph")
+    q = w4.quantize(rand(256, 512, seed=18), 128)
+    xs = [rand(4, 512, seed=19 + i, dtype=torch.bfloat16) for i in range(3)]
+    want = [w4.linear(x, q) for x in xs]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = w4.linear(xs[0], q)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want[0])
+    held = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = w4.linear(held, q)
+    for x, w in zip(xs + xs, want + want):
+        held.copy_(x)
+        graph.replay()
+        assert torch.equal(out, w)
+        torch.cuda.synchronize()
+
+
+def test_refusals():
+    announce("w4 refusals")
+    q = w4.quantize(rand(24, 136, seed=20), 64)
+    x = rand(2, 136, seed=21)
+    for bad, exc in [(lambda: w4.quantize(x, 48), ValueError), (lambda: w4.quantize(x.cpu()), ValueError),
+                     (lambda: w4.quantize(x[0]), ValueError), (lambda: w4.quantize(x.half()), TypeError),
+                     (lambda: w4.quantize(x[:0]), ValueError), (lambda: w4.linear(x.half(), q), TypeError),
+                     (lambda: w4.linear(x[:, 1:], q), ValueError), (lambda: w4.linear(x.cpu(), q), ValueError),
+                     (lambda: w4.linear(x.clone().requires_grad_(), q), RuntimeError),
+                     (lambda: w4.dequantize(q, torch.float16), TypeError),
+                     (lambda: w4.W4Weight(q.packed, q.scales, 24, 136, 32), ValueError),
+                     (lambda: w4.W4Weight(q.packed[:1], q.scales, 24, 136, 64), ValueError),
+                     (lambda: w4.W4Weight(q.packed.int(), q.scales, 24, 136, 64), ValueError),
+                     (lambda: w4.W4Weight(q.packed, q.scales.cpu(), 24, 136, 64), ValueError),
+                     (lambda: w4.W4Linear.from_linear(nn.Linear(8, 8).cuda()), ValueError)]:
+        with pytest.raises(exc):
+            bad()
+    with torch.no_grad():
+        w4.linear(x.clone().requires_grad_(), q)
+
+
+def test_module_and_model():
+    announce("w4 module")
+    lin = nn.Linear(192, 80, bias=False).cuda()
+    mod = w4.W4Linear.from_linear(lin, 32)
+    x = rand(5, 192, seed=22)
+    with torch.no_grad():
+        assert torch.equal(mod(x), w4.linear(x, w4.quantize(lin.weight, 32)))
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            y = mod(x)
+        assert y.dtype == torch.bfloat16 and torch.equal(y, w4.linear(x.bfloat16(), mod.weight))
+    again = w4.W4Linear(w4.quantize(torch.zeros(80, 192, device="cuda"), 32))
+    again.load_state_dict(mod.state_dict())
+    with torch.no_grad():
+        assert torch.equal(again(x), mod(x))
+    model = pkg.model.AutoRegressiveModel(100, 2, 128, 2).init_random().cuda()
+    w4.quantize_model(model, 64)
+    kinds = [type(m) for m in model.modules()]
+    assert kinds.count(w4.W4Linear) == 2 * 6 + 1 and nn.Linear not in kinds

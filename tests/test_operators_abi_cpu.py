@@ -1,0 +1,126 @@
+"""The C ABI of the 4-bit products and of the token scores without a GPU: what
+the headers declare is exported, and bad calls are refused on the host."""
+
+import os
+
+import pytest
+import torch
+
+from conftest import REPO, load_pkg
+from test_abi_cpu import declared_functions
+
+FAKE = 1 << 20        # a pointer that is never followed
+
+
+@pytest.fixture(scope="module")
+def native():
+    n = load_pkg()._native
+    n.lib()
+    return n
+
+
+@pytest.mark.parametrize("header,exports", [("rwkv_w4.h", "W4_EXPORTS"),
+                                            ("rwkv_token_scores.h", "SCORES_EXPORTS")])
+def test_exports(native, header, exports):
+    declared = declared_functions(os.path.join(REPO, "include", header), "rwkv_")
+    assert set(declared) == set(getattr(native, exports))
+    for name in declared:
+        assert hasattr(native.lib(), name) and name in native._SIGNATURES
+
+
+def test_w4_sizes(native):
+    lib = native.lib()
+    assert lib.rwkv_w4_packed_bytes(1, 1) == 1024 and lib.rwkv_w4_packed_bytes(17, 129) == 4096
+    assert lib.rwkv_w4_packed_bytes(768, 768) == 768 * 768 // 2
+    assert lib.rwkv_w4_scales_bytes(768, 768, 64) == 768 * 12 * 2
+    assert lib.rwkv_w4_scales_bytes(17, 129, 32) == 32 * 8 * 2
+    for bad in ((0, 1), (1, 0), (-1, 5), ((1 << 26) + 1, 8), (8, (1 << 26) + 1)):
+        assert lib.rwkv_w4_packed_bytes(*bad) == -1 and lib.rwkv_w4_scales_bytes(*bad, 64) == -1
+    assert lib.rwkv_w4_scales_bytes(8, 8, 16) == -1
+
+
+def test_w4_refusals(native):
+    lib = native.lib()
+    w, p, s, x, y = (FAKE * i for i in (1, 10, 20, 30, 40))
+
+    def quantize(weight=w, out=32, d_in=256, group=64, dtype=0, packed=p, scales=s):
+        return lib.rwkv_w4_quantize(weight, out, d_in, group, dtype, packed, scales, None)
+
+    def restore(packed=p, scales=s, out=32, d_in=256, group=64, dtype=0, weight=w):
+        return lib.rwkv_w4_dequantize(packed, scales, out, d_in, group, dtype, weight, None)
+
+    def linear(x=x, packed=p, scales=s, rows=4, out=32, d_in=256, group=64, dtype=0, y=y):
+        return lib.rwkv_w4_linear(x, packed, scales, rows, out, d_in, group, dtype, y, None)
+    for call in (quantize, restore, linear):
+        assert call(dtype=2) == 5
+        for bad in (dict(out=0), dict(d_in=-1), dict(group=48), dict(out=(1 << 26) + 1)):
+            assert call(**bad) == 2, bad
+        assert call(packed=None) == 1 and call(scales=None) == 1
+        assert call(packed=p + 8) == 6 and call(scales=s + 2) == 6
+    for call in (quantize, restore):
+        assert call(weight=None) == 1 and call(weight=w + 2) == 6
+        assert call(weight=p) == 7 and call(weight=s) == 7
+    assert quantize(packed=s) == 7
+    assert linear(rows=-1) == 2 and linear(rows=(1 << 26) + 1) == 2
+    assert linear(x=None) == 1 and linear(y=None) == 1
+    assert linear(x=x + 2) == 6 and linear(y=y + 1) == 6 and linear(y=y + 1, dtype=1) == 6
+    for other in (x, p, s):
+        assert linear(y=other) == 7
+    assert linear(y=x + 4 * 256 * 4 - 4) == 7
+    assert linear(rows=0, x=None, y=None) == 0
+
+
+def test_token_scores_refusals(native):
+    lib = native.lib()
+    x, t, lp, en, mx, ls, tl, ti, ws = (FAKE * i for i in (1, 100, 101, 102, 103, 104, 105, 106, 107))
+
+    def forward(logits=x, tokens=t, rows=4, vocab=1000, top=5, dtype=0, log_prob=lp, entropy=en,
+                row_max=mx, log_sum=ls, top_lp=tl, ids=ti, workspace=ws, nbytes=1 << 19):
+        return lib.rwkv_token_scores_forward(logits, tokens, rows, vocab, top, dtype, log_prob, entropy,
+                                             row_max, log_sum, top_lp, ids, workspace, nbytes, None)
+
+    def backward(logits=x, tokens=t, row_max=mx, log_sum=ls, entropy=en, ids=ti, g=lp, h=tl, tg=ws,
+                 rows=4, vocab=1000, top=5, dtype=0, grad=FAKE * 200):
+        return lib.rwkv_token_scores_backward(logits, tokens, row_max, log_sum, entropy, ids, g, h, tg,
+                                              rows, vocab, top, dtype, grad, None)
+    for call in (forward, backward):
+        assert call(dtype=3) == 5
+        for bad in (dict(rows=-1), dict(vocab=0), dict(top=-1), dict(top=65), dict(vocab=4), dict(vocab=1 << 31),
+                    dict(rows=1 << 31)):
+            assert call(**bad) == 2, bad
+        for name in ("logits", "tokens", "entropy", "row_max", "log_sum", "ids"):
+            assert call(**{name: None}) == 1, name
+        assert call(logits=x + 2) == 6 and call(logits=x + 1, dtype=1) == 6 and call(tokens=t + 4) == 6
+        assert call(rows=0, logits=None) == 0
+    assert forward(log_prob=None) == 1 and forward(top_lp=None) == 1
+    assert forward(log_prob=lp + 2) == 6 and forward(ids=ti + 4) == 6
+    assert forward(entropy=lp) == 7 and forward(row_max=x) == 7 and forward(ids=t) == 7
+    assert backward(grad=None) == 1
+    assert backward(grad=x) == 7 and backward(grad=FAKE * 100 - 8) == 7 and backward(g=FAKE * 200) == 7
+    assert backward(g=lp + 2) == 6 and backward(tg=ws + 1) == 6
+    for rows, vocab, top in ((1, 65536, 5), (64, 1000, 0), (8192, 65536, 64), (0, 10, 0)):
+        assert lib.rwkv_token_scores_workspace_bytes(rows, vocab, top) >= 0
+    assert lib.rwkv_token_scores_workspace_bytes(1, 10, 11) == -1
+    needed = lib.rwkv_token_scores_workspace_bytes(1, 1 << 20, 64)
+    if needed > 0:
+        assert forward(rows=1, vocab=1 << 20, top=64, nbytes=needed - 1) == 2
+        assert forward(rows=1, vocab=1 << 20, top=64, workspace=None) == 1
+        assert forward(rows=1, vocab=1 << 20, top=64, workspace=ws + 8) == 6
+
+
+def test_python_refuses_host_tensors():
+    pkg = load_pkg()
+    with pytest.raises(ValueError):
+        pkg.w4.quantize(torch.zeros(16, 64))
+    with pytest.raises(ValueError):
+        pkg.token_scores.token_scores(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64))
+    # a weight can be described without a GPU, and is checked
+    packed = torch.zeros(1, 1, 4, 16, 16, dtype=torch.uint8)
+    scales = torch.zeros(1, 1, 16, 2, dtype=torch.bfloat16)
+    w = pkg.w4.W4Weight(packed, scales, 3, 5, 64)
+    with pytest.raises(ValueError):
+        pkg.w4.linear(torch.zeros(2, 5), w)
+    for bad in ((packed, scales, 3, 5, 32), (packed, scales, 17, 5, 64), (packed, scales, 3, 129, 64),
+                (packed, scales.float(), 3, 5, 64), (packed, scales, 0, 5, 64), (packed, scales, 3, 5, 16)):
+        with pytest.raises(ValueError):
+            pkg.w4.W4Weight(*bad)
