@@ -30,7 +30,7 @@
  * Conventions are those of wkv7.h: status codes (checked on the host before
  * any launch), WKV7_DTYPE_* codes, work enqueued on `stream` without
  * synchronising, nothing allocated, outputs that overlap no other operand.
- * Every operand is aligned to its element, the workspace to 16 bytes.
+ * Every operand is aligned to its element.
  */
 #ifndef RWKV_RS_AMD_TOKEN_SCORES_H
 #define RWKV_RS_AMD_TOKEN_SCORES_H
@@ -44,19 +44,14 @@ extern "C" {
 /* The most alternatives of a row. */
 #define RWKV_TOKEN_SCORES_MAX_TOP 64
 
-/* Device memory a forward call of these sizes asks for (16-byte aligned, no
- * initialisation; 0: none), or -1 for sizes that are not supported: 0 <= rows,
- * 0 < vocab, both below 2^31, 0 <= top <= min(vocab, the most). */
-int64_t rwkv_token_scores_workspace_bytes(int64_t rows, int64_t vocab, int64_t top);
-
 /* log_prob, entropy, row_max, row_log_sum [rows], top_log_probs [rows, top]
- * fp32, top_ids [rows, top] int64 (the last two NULL when top is 0). The maxima
- * and log sums are kept for the backward. */
+ * fp32, top_ids [rows, top] int64. The maxima and log sums are for the backward,
+ * and may be NULL; so are the last two when top is 0. Sizes: 0 <= rows, 0 <
+ * vocab, both below 2^31, 0 <= top <= min(vocab, the most). */
 int rwkv_token_scores_forward(const void *logits, const int64_t *tokens, int64_t rows,
                               int64_t vocab, int64_t top, int dtype, float *log_prob,
                               float *entropy, float *row_max, float *row_log_sum,
-                              float *top_log_probs, int64_t *top_ids, void *workspace,
-                              int64_t workspace_bytes, void *stream);
+                              float *top_log_probs, int64_t *top_ids, void *stream);
 
 /* row_max, row_log_sum, entropy and top_ids are the forward's. */
 int rwkv_token_scores_backward(const void *logits, const int64_t *tokens, const float *row_max,

@@ -47,30 +47,21 @@ int64_t size_of(int dtype) { return dtype == WKV7_DTYPE_BF16 ? 2 : 4; }
 
 extern "C" {
 
-int64_t rwkv_token_scores_workspace_bytes(int64_t rows, int64_t vocab, int64_t top) {
-  return sizes_ok(rows, vocab, top) ? rwkv_scores::workspace_bytes(rows, vocab, top) : -1;
-}
-
 int rwkv_token_scores_forward(const void* logits, const int64_t* tokens, int64_t rows, int64_t vocab,
                               int64_t top, int dtype, float* log_prob, float* entropy, float* row_max,
-                              float* row_log_sum, float* top_log_probs, int64_t* top_ids, void* workspace,
-                              int64_t workspace_bytes, void* stream) {
+                              float* row_log_sum, float* top_log_probs, int64_t* top_ids, void* stream) {
   if (dtype != WKV7_DTYPE_F32 && dtype != WKV7_DTYPE_BF16) return WKV7_ERR_DTYPE;
   if (!sizes_ok(rows, vocab, top)) return WKV7_ERR_SHAPE;
   if (rows == 0) return WKV7_OK;
-  if (!logits || !tokens || !log_prob || !entropy || !row_max || !row_log_sum ||
+  if (!logits || !tokens || !log_prob || !entropy ||
       (top > 0 && (!top_log_probs || !top_ids)))
     return WKV7_ERR_NULL_POINTER;
-  const int64_t needed = rwkv_scores::workspace_bytes(rows, vocab, top);
-  if (workspace_bytes < needed) return WKV7_ERR_SHAPE;
-  if (needed > 0 && !workspace) return WKV7_ERR_NULL_POINTER;
   if (!aligned(logits, size_of(dtype)) || !aligned(tokens, 8) || !aligned(log_prob, 4) || !aligned(entropy, 4) ||
-      !aligned(row_max, 4) || !aligned(row_log_sum, 4) || (top > 0 && (!aligned(top_log_probs, 4) || !aligned(top_ids, 8))) ||
-      (needed > 0 && !aligned(workspace, 16)))
+      !aligned(row_max, 4) || !aligned(row_log_sum, 4) || (top > 0 && (!aligned(top_log_probs, 4) || !aligned(top_ids, 8))))
     return WKV7_ERR_ALIGNMENT;
   const int64_t rb = rows * 4;
   if (any_overlap({{log_prob, rb}, {entropy, rb}, {row_max, rb}, {row_log_sum, rb}, {top_log_probs, rb * top},
-                   {top_ids, 2 * rb * top}, {workspace, needed}},
+                   {top_ids, 2 * rb * top}},
                   {{logits, rows * vocab * size_of(dtype)}, {tokens, rows * 8}}))
     return WKV7_ERR_OVERLAP;
   rwkv_scores::ForwardCall c{};
@@ -86,7 +77,6 @@ int rwkv_token_scores_forward(const void* logits, const int64_t* tokens, int64_t
   c.log_sum = row_log_sum;
   c.top_log_probs = top_log_probs;
   c.top_ids = top_ids;
-  c.workspace = workspace;
   return wkv7::hip_status(rwkv_scores::launch_forward(c, static_cast<hipStream_t>(stream)));
 }
 

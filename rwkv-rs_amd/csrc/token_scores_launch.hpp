@@ -14,9 +14,8 @@ struct ForwardCall {
   int64_t rows, vocab;
   int top;
   bool bf16;
-  float *log_prob, *entropy, *row_max, *log_sum, *top_log_probs;
+  float *log_prob, *entropy, *row_max, *log_sum, *top_log_probs;   // row_max, log_sum: may be null
   int64_t* top_ids;
-  void* workspace;
 };
 struct BackwardCall {
   const void* logits;
@@ -30,7 +29,6 @@ struct BackwardCall {
   void* logits_grad;
 };
 
-int64_t workspace_bytes(int64_t rows, int64_t vocab, int64_t top);
 hipError_t launch_forward(const ForwardCall& c, hipStream_t s);
 hipError_t launch_backward(const BackwardCall& c, hipStream_t s);
 

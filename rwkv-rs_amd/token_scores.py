@@ -31,23 +31,29 @@ class TokenScores(NamedTuple):
     top_ids: torch.Tensor
 
 
+def _forward(logits, tokens, top, keep):
+    """The four outputs and, with ``keep``, what the backward needs of each row."""
+    rows, vocab = logits.shape
+    dev = logits.device
+    code = _code(logits.dtype)
+
+    def row():
+        return torch.empty(rows, dtype=torch.float32, device=dev)
+    log_prob, entropy = row(), row()
+    row_max, log_sum = (row(), row()) if keep else (None, None)
+    top_lp = torch.empty(rows, top, dtype=torch.float32, device=dev)
+    top_ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
+    _native.check(_native.lib().rwkv_token_scores_forward(
+        logits.data_ptr(), tokens.data_ptr(), rows, vocab, top, code, log_prob.data_ptr(),
+        entropy.data_ptr(), _ptr(row_max), _ptr(log_sum), top_lp.data_ptr(), top_ids.data_ptr(),
+        _stream(dev)))
+    return log_prob, entropy, top_lp, top_ids, row_max, log_sum
+
+
 class _TokenScores(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top):
-        rows, vocab = logits.shape
-        dev = logits.device
-        code = _code(logits.dtype)
-        lib = _native.lib()
-        log_prob, entropy, row_max, log_sum = (torch.empty(rows, dtype=torch.float32, device=dev)
-                                               for _ in range(4))
-        top_lp = torch.empty(rows, top, dtype=torch.float32, device=dev)
-        top_ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
-        nbytes = lib.rwkv_token_scores_workspace_bytes(rows, vocab, top)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
-        _native.check(lib.rwkv_token_scores_forward(
-            logits.data_ptr(), tokens.data_ptr(), rows, vocab, top, code, log_prob.data_ptr(),
-            entropy.data_ptr(), row_max.data_ptr(), log_sum.data_ptr(), top_lp.data_ptr(),
-            top_ids.data_ptr(), _ptr(ws), nbytes, _stream(dev)))
+        log_prob, entropy, top_lp, top_ids, row_max, log_sum = _forward(logits, tokens, top, True)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_ids)
         ctx.save_for_backward(logits, tokens, row_max, log_sum, entropy, top_ids)
@@ -90,7 +96,12 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> To
     if vocab == 0:
         raise ValueError("the vocabulary is empty")
     lead = logits.shape[:-1]
-    out = _TokenScores.apply(logits.reshape(-1, vocab).contiguous(),
-                             tokens.reshape(-1).to(torch.int64).contiguous(), int(top))
-    return TokenScores(out[0].reshape(lead), out[1].reshape(lead), out[2].reshape(*lead, top),
-                       out[3].reshape(*lead, top))
+    flat = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
+    tokens = tokens.reshape(-1).to(torch.int64).contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        out = _TokenScores.apply(flat.contiguous(), tokens, int(top))
+    else:
+        out = _forward(flat.contiguous(), tokens, int(top), False)[:4]
+    if len(lead) != 1:
+        out = [t.reshape(lead + t.shape[1:]) for t in out]
+    return TokenScores(*out)

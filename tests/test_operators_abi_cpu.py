@@ -72,14 +72,14 @@ def test_w4_refusals(native):
 
 def test_token_scores_refusals(native):
     lib = native.lib()
-    x, t, lp, en, mx, ls, tl, ti, ws = (FAKE * i for i in (1, 100, 101, 102, 103, 104, 105, 106, 107))
+    x, t, lp, en, mx, ls, tl, ti, tg = (FAKE * i for i in (1, 100, 101, 102, 103, 104, 105, 106, 107))
 
     def forward(logits=x, tokens=t, rows=4, vocab=1000, top=5, dtype=0, log_prob=lp, entropy=en,
-                row_max=mx, log_sum=ls, top_lp=tl, ids=ti, workspace=ws, nbytes=1 << 19):
+                row_max=mx, log_sum=ls, top_lp=tl, ids=ti):
         return lib.rwkv_token_scores_forward(logits, tokens, rows, vocab, top, dtype, log_prob, entropy,
-                                             row_max, log_sum, top_lp, ids, workspace, nbytes, None)
+                                             row_max, log_sum, top_lp, ids, None)
 
-    def backward(logits=x, tokens=t, row_max=mx, log_sum=ls, entropy=en, ids=ti, g=lp, h=tl, tg=ws,
+    def backward(logits=x, tokens=t, row_max=mx, log_sum=ls, entropy=en, ids=ti, g=lp, h=tl, tg=tg,
                  rows=4, vocab=1000, top=5, dtype=0, grad=FAKE * 200):
         return lib.rwkv_token_scores_backward(logits, tokens, row_max, log_sum, entropy, ids, g, h, tg,
                                               rows, vocab, top, dtype, grad, None)
@@ -88,24 +88,17 @@ def test_token_scores_refusals(native):
         for bad in (dict(rows=-1), dict(vocab=0), dict(top=-1), dict(top=65), dict(vocab=4), dict(vocab=1 << 31),
                     dict(rows=1 << 31)):
             assert call(**bad) == 2, bad
-        for name in ("logits", "tokens", "entropy", "row_max", "log_sum", "ids"):
+        for name in ("logits", "tokens", "entropy", "ids"):
             assert call(**{name: None}) == 1, name
         assert call(logits=x + 2) == 6 and call(logits=x + 1, dtype=1) == 6 and call(tokens=t + 4) == 6
         assert call(rows=0, logits=None) == 0
     assert forward(log_prob=None) == 1 and forward(top_lp=None) == 1
     assert forward(log_prob=lp + 2) == 6 and forward(ids=ti + 4) == 6
     assert forward(entropy=lp) == 7 and forward(row_max=x) == 7 and forward(ids=t) == 7
-    assert backward(grad=None) == 1
+    assert forward(log_sum=ls + 1) == 6
+    assert backward(grad=None) == 1 and backward(row_max=None) == 1 and backward(log_sum=None) == 1
     assert backward(grad=x) == 7 and backward(grad=FAKE * 100 - 8) == 7 and backward(g=FAKE * 200) == 7
-    assert backward(g=lp + 2) == 6 and backward(tg=ws + 1) == 6
-    for rows, vocab, top in ((1, 65536, 5), (64, 1000, 0), (8192, 65536, 64), (0, 10, 0)):
-        assert lib.rwkv_token_scores_workspace_bytes(rows, vocab, top) >= 0
-    assert lib.rwkv_token_scores_workspace_bytes(1, 10, 11) == -1
-    needed = lib.rwkv_token_scores_workspace_bytes(1, 1 << 20, 64)
-    if needed > 0:
-        assert forward(rows=1, vocab=1 << 20, top=64, nbytes=needed - 1) == 2
-        assert forward(rows=1, vocab=1 << 20, top=64, workspace=None) == 1
-        assert forward(rows=1, vocab=1 << 20, top=64, workspace=ws + 8) == 6
+    assert backward(g=lp + 2) == 6 and backward(tg=tg + 1) == 6
 
 
 def test_python_refuses_host_tensors():
