@@ -31,8 +31,9 @@
 extern "C" {
 #endif
 
-/* The most outputs, inputs and rows that a call takes. */
+/* The most outputs and inputs, and the most rows, that a call takes. */
 #define RWKV_W4_MAX_DIM (1 << 26)
+#define RWKV_W4_MAX_ROWS (1 << 20)
 
 /* Bytes of `packed` and of `scales`, or -1 for sizes or a group that are not
  * supported. */

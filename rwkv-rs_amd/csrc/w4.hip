@@ -170,18 +170,17 @@ __global__ __launch_bounds__(kBlockWaves* kWave) void dequantize_kernel(const We
 }
 
 // --------------------------------------------------------------------- linear
-// A workgroup forms 16 outputs of up to 16 MT rows; its eight waves split the
-// inputs in blocks of 128 (one 16-byte load of weights a lane, four matrix
-// instructions a row tile) and add up through LDS in wave order.
+// How rows of activations are read: every one is whole blocks of 128 inputs, or
+// pieces of eight, from a 16-byte boundary on; or element by element.
+enum Form { kBlocks, kPieces, kElements };
+
 // v_mfma_f32_16x16x32_bf16: lane l holds A[row l % 16] and B[column l % 16] at
 // k = 8 (l / 16) .. + 7, the result D[row 4 (l / 16) + r][column l % 16].
-constexpr int kLinearWaves = 8;
-
-template <bool BF, bool kVector>
+template <bool BF, Form kForm>
 __device__ __forceinline__ auto load_x(const void* row, int64_t i, int64_t n) {
-  if constexpr (BF && kVector) {
+  if constexpr (BF && kForm != kElements) {
     Parts<1> p;
-    if (i < n) {
+    if (kForm == kBlocks || i < n) {
       p.p[0] = *reinterpret_cast<const bf16x8*>(static_cast<const uint16_t*>(row) + i);
     } else {
 #pragma unroll
@@ -190,7 +189,7 @@ __device__ __forceinline__ auto load_x(const void* row, int64_t i, int64_t n) {
     return p;
   } else {
     float v[8];
-    load8<BF, kVector>(row, i, n, v);
+    load8<BF, kForm != kElements>(row, i, kForm == kBlocks ? INT64_MAX : n, v);
     if constexpr (BF) {
       Parts<1> p;
 #pragma unroll
@@ -202,55 +201,184 @@ __device__ __forceinline__ auto load_x(const void* row, int64_t i, int64_t n) {
   }
 }
 
-template <bool BF, bool kVector, int kGroup, int MT>
-__global__ __launch_bounds__(kLinearWaves* kWave) void linear_kernel(const LinearCall c) {
-  __shared__ float part[kLinearWaves][MT * 256];
+template <int kParts>
+__device__ __forceinline__ f32x4 multiply(const Parts<kParts>& x, const bf16x8& w, f32x4 sum) {
+#pragma unroll
+  for (int i = kParts - 1; i >= 0; --i) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.p[i], w, sum, 0, 0, 0);
+  return sum;
+}
+
+template <bool BF>
+__device__ __forceinline__ void store_y(const LinearCall& c, int64_t row, int64_t col, float v) {
+  if (row >= c.rows || col >= c.out) return;
+  v *= kShrink;
+  if constexpr (BF) static_cast<__bf16*>(c.y)[row * c.out + col] = static_cast<__bf16>(v);
+  else static_cast<float*>(c.y)[row * c.out + col] = v;
+}
+
+// Few rows. A workgroup forms 16 NT outputs of up to 16 MT rows; its waves split
+// the inputs in blocks of 128 (one 16-byte load of weights a lane and 16 outputs,
+// four matrix instructions a tile) and add up through LDS in wave order. A wave
+// has kDepth blocks' loads in flight.
+template <bool BF, Form kForm, int kGroup, int MT, int NT, int kWaves, int kDepth>
+__global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) {
+  __shared__ float part[kWaves][MT * NT * 256];
   constexpr int kParts = BF ? 1 : 3, kSteps = kGroup / 32;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = lane & 15, g = lane >> 4;
-  const int64_t n = blockIdx.x, ib = blocks_in(c.in);
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.y) * 16 * MT; row0 < c.rows;
-       row0 += static_cast<int64_t>(gridDim.y) * 16 * MT) {
-    f32x4 acc[MT];
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * NT, ib = blocks_in(c.in), ob = blocks_out(c.out);
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * 16 * MT;
+  const void* x[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int64_t k = wave; k < ib; k += kLinearWaves) {
-      const int64_t b = n * ib + k;
-      const u32x4 word = reinterpret_cast<const u32x4*>(c.packed)[b * kWave + lane];
-      float s[kInputs / kGroup];
-      load_scales<kGroup>(c.scales, b * kRows + t, s);
+  for (int m = 0; m < MT; ++m) x[m] = row_at(const_cast<void*>(c.x), min(row0 + 16 * m + t, c.rows - 1), c.in, BF);
+  f32x4 acc[MT][NT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int64_t row = min(row0 + 16 * m + t, c.rows - 1);
-        const void* const x = row_at(const_cast<void*>(c.x), row, c.in, BF);
-        f32x4 sum;
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const Parts<kParts> xs = load_x<BF, kVector>(x, k * kInputs + 32 * j + 8 * g, c.in);
-          const bf16x8 w = weights8(word[j]);
-          if (j % kSteps == 0) sum = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int64_t k0 = wave; k0 < ib; k0 += kWaves * kDepth) {
+    u32x4 word[kDepth][NT];
+    float s[kDepth][NT][kInputs / kGroup];
 #pragma unroll
-          for (int i = kParts - 1; i >= 0; --i) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xs.p[i], w, sum, 0, 0, 0);
-          if (j % kSteps == kSteps - 1) acc[m] += sum * s[32 * j / kGroup];
+    for (int d = 0; d < kDepth; ++d) {
+      const int64_t k = k0 + d * kWaves;
+      if (k < ib) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int64_t b = min(n0 + n, ob - 1) * ib + k;   // past the end: the last outputs, not stored
+          word[d][n] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(c.packed) + b * kWave + lane);
+          load_scales<kGroup>(c.scales, b * kRows + t, s[d][n]);
         }
       }
     }
-    __syncthreads();   // the sums of the rows before are read
+    Parts<kParts> xs[kDepth][MT][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) *reinterpret_cast<f32x4*>(&part[wave][m * 256 + 4 * lane]) = acc[m];
-    __syncthreads();
-    for (int i = threadIdx.x; i < MT * 256; i += kLinearWaves * kWave) {
-      float v = 0.f;
+    for (int d = 0; d < kDepth; ++d) {
+      const int64_t k = k0 + d * kWaves;
+      if (k < ib) {
 #pragma unroll
-      for (int w = 0; w < kLinearWaves; ++w) v += part[w][i];
-      v *= kShrink;
-      const int l = (i >> 2) & 63;
-      const int64_t row = row0 + 16 * (i >> 8) + 4 * (l >> 4) + (i & 3), col = n * kRows + (l & 15);
-      if (row >= c.rows || col >= c.out) continue;
-      if constexpr (BF) static_cast<__bf16*>(c.y)[row * c.out + col] = static_cast<__bf16>(v);
-      else static_cast<float*>(c.y)[row * c.out + col] = v;
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) xs[d][m][j] = load_x<BF, kForm>(x[m], k * kInputs + 32 * j + 8 * g, c.in);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      if (k0 + d * kWaves < ib) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          f32x4 sum[MT];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bf16x8 w = weights8(word[d][n][j]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              sum[m] = multiply(xs[d][m][j], w, j % kSteps == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[m]);
+              if (j % kSteps == kSteps - 1) acc[m][n] += sum[m] * s[d][n][32 * j / kGroup];
+            }
+          }
+        }
+      }
     }
   }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) *reinterpret_cast<f32x4*>(&part[wave][(m * NT + n) * 256 + 4 * lane]) = acc[m][n];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MT * NT * 256; i += kWaves * kWave) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v += part[w][i];
+    const int l = (i >> 2) & 63, m = i / (NT * 256), n = i / 256 % NT;
+    store_y<BF>(c, row0 + 16 * m + 4 * (l >> 4) + (i & 3), (n0 + n) * kRows + (l & 15), v);
+  }
+}
+
+// Many rows. A workgroup forms 16 MT rows by 64 NT outputs, its four waves 16 NT
+// outputs each. The rows' activations of 128 inputs go through LDS, one block
+// ahead, in the order in which the waves' matrix instructions read them: piece
+// (row 16 m + t, inputs 32 j + 8 g ..) of 16 bytes at place 16 g + (t ^ (4 g + j))
+// of 64 for (m, j). The exclusive or spreads a row's 16 pieces, which neighbouring
+// threads bring, over all banks. Weights go to registers, one block ahead too.
+constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave;
+template <bool BF, Form kForm, int kGroup, int MT, int NT>
+__global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall c) {
+  constexpr int kParts = BF ? 1 : 3, kSteps = kGroup / 32, kPiecesOfRow = kInputs / 8;
+  constexpr int kLoads = 16 * MT * kPiecesOfRow / kTileThreads;   // pieces a thread brings
+  __shared__ bf16x8 xs[2][kParts][MT * 4 * kWave];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int t = lane & 15, g = lane >> 4;
+  const int64_t ib = blocks_in(c.in), ob = blocks_out(c.out);
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * 16 * MT;
+  const int64_t n0 = (static_cast<int64_t>(blockIdx.x) * kTileWaves + wave) * NT;
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Parts<kParts> bring[kLoads];
+  u32x4 word[NT];
+  float s[NT][kInputs / kGroup];
+  const int piece = tid % kPiecesOfRow;
+  auto load = [&](int64_t k) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int64_t row = min(row0 + tid / kPiecesOfRow + i * (kTileThreads / kPiecesOfRow), c.rows - 1);
+      bring[i] = load_x<BF, kForm>(row_at(const_cast<void*>(c.x), row, c.in, BF), k * kInputs + 8 * piece, c.in);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int64_t b = min(n0 + n, ob - 1) * ib + k;   // past the end: the last outputs, not stored
+      word[n] = reinterpret_cast<const u32x4*>(c.packed)[b * kWave + lane];
+      load_scales<kGroup>(c.scales, b * kRows + t, s[n]);
+    }
+  };
+  load(0);
+  for (int64_t k = 0; k < ib; ++k) {
+    bf16x8(*const at)[MT * 4 * kWave] = xs[k & 1];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = tid / kPiecesOfRow + i * (kTileThreads / kPiecesOfRow), j = piece >> 2, q = piece & 3;
+      const int place = (row / 16 * 4 + j) * kWave + 16 * q + ((row & 15) ^ (4 * q + j));
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) at[p][place] = bring[i].p[p];
+    }
+    u32x4 w[NT];
+    float scale[NT][kInputs / kGroup];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      w[n] = word[n];
+#pragma unroll
+      for (int q = 0; q < kInputs / kGroup; ++q) scale[n][q] = s[n][q];
+    }
+    __syncthreads();   // the block before is read: its place is written only after the next of these
+    if (k + 1 < ib) load(k + 1);
+    f32x4 sum[MT][NT];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      Parts<kParts> a[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) a[m].p[p] = at[p][(m * 4 + j) * kWave + 16 * g + (t ^ (4 * g + j))];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const bf16x8 v = weights8(w[n][j]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          sum[m][n] = multiply(a[m], v, j % kSteps == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[m][n]);
+          if (j % kSteps == kSteps - 1) acc[m][n] += sum[m][n] * scale[n][32 * j / kGroup];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) store_y<BF>(c, row0 + 16 * m + 4 * g + r, (n0 + n) * kRows + t, acc[m][n][r]);
 }
 
 // ----------------------------------------------------------------- dispatch
@@ -293,16 +421,46 @@ hipError_t launch_dequantize(const WeightCall& c, hipStream_t stream) {
   });
 }
 
+namespace {
+
+template <bool BF, Form kForm, int kGroup, int MT, int NT, int kWaves, int kDepth>
+void few(const LinearCall& c, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + NT - 1) / NT), static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)));
+  hipLaunchKernelGGL((few_kernel<BF, kForm, kGroup, MT, NT, kWaves, kDepth>), grid, dim3(kWaves * kWave), 0, s, c);
+}
+template <bool BF, Form kForm, int kGroup, int MT, int NT>
+void tiles(const LinearCall& c, hipStream_t s) {
+  constexpr int cols = kTileWaves * NT;
+  const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + cols - 1) / cols), static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)));
+  hipLaunchKernelGGL((tile_kernel<BF, kForm, kGroup, MT, NT>), grid, dim3(kTileThreads), 0, s, c);
+}
+
+template <bool BF, Form kForm, int kGroup>
+void linear(const LinearCall& c, hipStream_t s) {
+  const int64_t ob = blocks_out(c.out), ib = blocks_in(c.in);
+  if (c.rows <= 16) {
+    if (ob >= 1024) few<BF, kForm, kGroup, 1, BF ? 4 : 2, 8, 1>(c, s);
+    else if (ob >= 512) few<BF, kForm, kGroup, 1, 2, 8, BF ? 2 : 1>(c, s);
+    else if (ib >= 64) few<BF, kForm, kGroup, 1, 1, 16, BF ? 4 : 1>(c, s);
+    else few<BF, kForm, kGroup, 1, 1, 8, BF ? 4 : 2>(c, s);
+  } else if (c.rows <= 32) {
+    if (ob >= 512) few<BF, kForm, kGroup, 2, 2, 8, 1>(c, s);
+    else few<BF, kForm, kGroup, 2, 1, 8, BF ? 2 : 1>(c, s);
+  } else {
+    const int64_t rt = (c.rows + 63) / 64;
+    if (rt * ob >= 16 * 256) tiles<BF, kForm, kGroup, 4, BF ? 4 : 2>(c, s);
+    else if (rt * ob >= 8 * 256) tiles<BF, kForm, kGroup, 4, 2>(c, s);
+    else tiles<BF, kForm, kGroup, 2, 1>(c, s);
+  }
+}
+
+}  // namespace
+
 hipError_t launch_linear(const LinearCall& c, hipStream_t stream) {
   return by_form(c.bf16, vector_rows(c.x, c.in), c.group, [&](auto bf, auto vec, auto group) {
-    auto go = [&](auto mt) {
-      const int64_t tiles = (c.rows + 16 * mt() - 1) / (16 * mt());
-      const dim3 grid(static_cast<unsigned>(blocks_out(c.out)), static_cast<unsigned>(std::min<int64_t>(tiles, 65535)));
-      hipLaunchKernelGGL((linear_kernel<bf(), vec(), group(), mt()>), grid, dim3(kLinearWaves * kWave), 0, stream, c);
-    };
-    if (c.rows <= 16) go(std::integral_constant<int, 1>());
-    else if (c.rows <= 32) go(std::integral_constant<int, 2>());
-    else go(std::integral_constant<int, 4>());
+    if constexpr (!vec()) linear<bf(), kElements, group()>(c, stream);
+    else if (c.in % kInputs == 0) linear<bf(), kBlocks, group()>(c, stream);
+    else linear<bf(), kPieces, group()>(c, stream);
   });
 }
 

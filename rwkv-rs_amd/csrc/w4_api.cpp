@@ -99,7 +99,7 @@ int rwkv_w4_dequantize(const void* packed, const void* scales, int64_t out, int6
 int rwkv_w4_linear(const void* x, const void* packed, const void* scales, int64_t rows, int64_t out,
                    int64_t in, int64_t group, int dtype, void* y, void* stream) {
   if (dtype != WKV7_DTYPE_F32 && dtype != WKV7_DTYPE_BF16) return WKV7_ERR_DTYPE;
-  if (!dims_ok(out, in) || !group_ok(group) || rows < 0 || rows > RWKV_W4_MAX_DIM) return WKV7_ERR_SHAPE;
+  if (!dims_ok(out, in) || !group_ok(group) || rows < 0 || rows > RWKV_W4_MAX_ROWS) return WKV7_ERR_SHAPE;
   if (!packed || !scales || (rows > 0 && (!x || !y))) return WKV7_ERR_NULL_POINTER;
   if (!aligned(packed, 16) || !aligned(scales, 16) || !aligned(x, size_of(dtype)) ||
       !aligned(y, size_of(dtype)))

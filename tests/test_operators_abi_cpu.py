@@ -61,7 +61,7 @@ def test_w4_refusals(native):
         assert call(weight=None) == 1 and call(weight=w + 2) == 6
         assert call(weight=p) == 7 and call(weight=s) == 7
     assert quantize(packed=s) == 7
-    assert linear(rows=-1) == 2 and linear(rows=(1 << 26) + 1) == 2
+    assert linear(rows=-1) == 2 and linear(rows=(1 << 20) + 1) == 2
     assert linear(x=None) == 1 and linear(y=None) == 1
     assert linear(x=x + 2) == 6 and linear(y=y + 1) == 6 and linear(y=y + 1, dtype=1) == 6
     for other in (x, p, s):
