@@ -55,13 +55,21 @@ int rwkv_w4_dequantize(const void *packed, const void *scales, int64_t out,
                        int64_t in, int64_t group, int dtype, void *weight,
                        void *stream);
 
+/* Device memory that rwkv_w4_linear asks for (16-byte aligned, no
+ * initialisation), 0 for none (always up to 16 rows), or -1 for sizes or a dtype
+ * that are not supported: with few outputs and many inputs, workgroups share
+ * the inputs and leave their sums there. */
+int64_t rwkv_w4_linear_workspace_bytes(int64_t rows, int64_t out, int64_t in,
+                                       int dtype);
+
 /* y [rows, out] = x [rows, in] W^T, x and y in dtype. Products are exact in
  * fp32 (bf16 x) or formed from x's three bf16 parts, which hold it whole (fp32
  * x; parts below 2^-126 are lost); sums are fp32, the scale is applied to a
  * group's sum in fp32, and y is rounded once. */
 int rwkv_w4_linear(const void *x, const void *packed, const void *scales,
                    int64_t rows, int64_t out, int64_t in, int64_t group,
-                   int dtype, void *y, void *stream);
+                   int dtype, void *y, void *workspace, int64_t workspace_bytes,
+                   void *stream);
 
 #ifdef __cplusplus
 }

@@ -76,7 +76,7 @@ DECODE_EXPORTS = ("rwkv_decode_workspace_bytes", "rwkv_decode_cell", "rwkv_decod
 
 # and of include/rwkv_w4.h and include/rwkv_token_scores.h
 W4_EXPORTS = ("rwkv_w4_packed_bytes", "rwkv_w4_scales_bytes", "rwkv_w4_quantize",
-              "rwkv_w4_dequantize", "rwkv_w4_linear")
+              "rwkv_w4_dequantize", "rwkv_w4_linear_workspace_bytes", "rwkv_w4_linear")
 SCORES_EXPORTS = ("rwkv_token_scores_forward", "rwkv_token_scores_backward")
 
 _P = ctypes.c_void_p
@@ -130,7 +130,8 @@ _SIGNATURES = {
     "rwkv_w4_scales_bytes": ([_I64] * 3, _I64),
     "rwkv_w4_quantize": ([_P] + [_I64] * 3 + [_INT] + [_P] * 3, _INT),
     "rwkv_w4_dequantize": ([_P] * 2 + [_I64] * 3 + [_INT] + [_P] * 2, _INT),
-    "rwkv_w4_linear": ([_P] * 3 + [_I64] * 4 + [_INT] + [_P] * 2, _INT),
+    "rwkv_w4_linear_workspace_bytes": ([_I64] * 3 + [_INT], _I64),
+    "rwkv_w4_linear": ([_P] * 3 + [_I64] * 4 + [_INT] + [_P] * 2 + [_I64, _P], _INT),
     "rwkv_token_scores_forward": ([_P] * 2 + [_I64] * 3 + [_INT] + [_P] * 7, _INT),
     "rwkv_token_scores_backward": ([_P] * 9 + [_I64] * 3 + [_INT] + [_P] * 2, _INT),
 }

@@ -408,14 +408,18 @@ __global__ __launch_bounds__(kWaves * 64, 4) void forward_kernel(const ForwardCa
       most_at = Q + lane;
     }
     float chunk_max, bound_x = 0.f;
+    int bound_q = 0;
     if constexpr (kTop) {
       find_bound(sh, key_of(most, most_at), k);
       chunk_max = sh.max;
       bound_x = key_x(sh.bound);
+      bound_q = key_j(sh.bound);
       uint32_t reached = 0;   // the pieces that may hold an alternative
 #pragma unroll
       for (int i = 0; i < kPieces; ++i)
-        if (piece_max[i] >= bound_x && i * kThreads + lane < left) reached |= 1u << i;
+        if ((piece_max[i] > bound_x || (piece_max[i] == bound_x && q0 + i * kThreads + lane <= bound_q)) &&
+            i * kThreads + lane < left)
+          reached |= 1u << i;
       if (reached) {
         int n = atomicAdd(&sh.pieces, __popc(reached));
 #pragma unroll
@@ -462,7 +466,7 @@ __global__ __launch_bounds__(kWaves * 64, 4) void forward_kernel(const ForwardCa
     }
     if constexpr (kTop) {
       __syncthreads();
-      const int bound_q = key_j(sh.bound), pieces = min(sh.pieces, max_pieces(kWaves));
+      const int pieces = min(sh.pieces, max_pieces(kWaves));
       auto list = [&](float v, int q, int j) {
         if (v > bound_x || (v == bound_x && q <= bound_q)) {
           const int n = atomicAdd(&sh.listed, 1);

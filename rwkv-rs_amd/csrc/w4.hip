@@ -295,15 +295,16 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
   }
 }
 
-// Many rows. A workgroup forms 16 MT rows by 64 NT outputs, its four waves 16 NT
-// outputs each. The rows' activations of 128 inputs go through LDS, one block
+// Many rows. A workgroup forms 16 MT rows by 64 NT outputs of `share` blocks of
+// inputs, its four waves 16 NT outputs each; where the inputs are shared among
+// workgroups, join_kernel adds up what they leave. The rows' activations of 128 inputs go through LDS, one block
 // ahead, in the order in which the waves' matrix instructions read them: piece
 // (row 16 m + t, inputs 32 j + 8 g ..) of 16 bytes at place 16 g + (t ^ (4 g + j))
 // of 64 for (m, j). The exclusive or spreads a row's 16 pieces, which neighbouring
 // threads bring, over all banks. Weights go to registers, one block ahead too.
 constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave;
 template <bool BF, Form kForm, int kGroup, int MT, int NT>
-__global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall c) {
+__global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall c, const int64_t share) {
   constexpr int kParts = BF ? 1 : 3, kSteps = kGroup / 32, kPiecesOfRow = kInputs / 8;
   constexpr int kLoads = 16 * MT * kPiecesOfRow / kTileThreads;   // pieces a thread brings
   __shared__ bf16x8 xs[2][kParts][MT * 4 * kWave];
@@ -334,9 +335,11 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall 
       load_scales<kGroup>(c.scales, b * kRows + t, s[n]);
     }
   };
-  load(0);
-  for (int64_t k = 0; k < ib; ++k) {
-    bf16x8(*const at)[MT * 4 * kWave] = xs[k & 1];
+  const int64_t k1 = min(blockIdx.z * share + share, ib);
+  int buffer = 0;
+  if (blockIdx.z * share < k1) load(blockIdx.z * share);
+  for (int64_t k = blockIdx.z * share; k < k1; ++k, buffer ^= 1) {
+    bf16x8(*const at)[MT * 4 * kWave] = xs[buffer];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = tid / kPiecesOfRow + i * (kTileThreads / kPiecesOfRow), j = piece >> 2, q = piece & 3;
@@ -353,7 +356,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall 
       for (int q = 0; q < kInputs / kGroup; ++q) scale[n][q] = s[n][q];
     }
     __syncthreads();   // the block before is read: its place is written only after the next of these
-    if (k + 1 < ib) load(k + 1);
+    if (k + 1 < k1) load(k + 1);
     f32x4 sum[MT][NT];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -378,7 +381,24 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall 
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) store_y<BF>(c, row0 + 16 * m + 4 * g + r, (n0 + n) * kRows + t, acc[m][n][r]);
+      for (int r = 0; r < 4; ++r) {
+        const int64_t row = row0 + 16 * m + 4 * g + r, col = (n0 + n) * kRows + t;
+        if (gridDim.z == 1) store_y<BF>(c, row, col, acc[m][n][r]);
+        else if (row < c.rows && col < c.out) c.partial[(blockIdx.z * c.rows + row) * c.out + col] = acc[m][n][r];
+      }
+}
+
+// The parts that tile_kernel's workgroups left of each output, in order.
+template <bool BF>
+__global__ __launch_bounds__(256) void join_kernel(const LinearCall c, const int splits) {
+  const int64_t n = c.rows * c.out, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n) return;
+  float v = 0.f;
+#pragma unroll 4
+  for (int z = 0; z < splits; ++z) v += c.partial[z * n + i];
+  v *= kShrink;
+  if constexpr (BF) static_cast<__bf16*>(c.y)[i] = static_cast<__bf16>(v);
+  else static_cast<float*>(c.y)[i] = v;
 }
 
 // ----------------------------------------------------------------- dispatch
@@ -428,33 +448,88 @@ void few(const LinearCall& c, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + NT - 1) / NT), static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)));
   hipLaunchKernelGGL((few_kernel<BF, kForm, kGroup, MT, NT, kWaves, kDepth>), grid, dim3(kWaves * kWave), 0, s, c);
 }
+constexpr int64_t kMinTiles = 32, kEnoughTiles = 256, kFillTiles = 512, kMinShare = 4;
+
+// Tiles of 16 MT rows and 64 NT outputs, and how many workgroups share the
+// inputs of each.
+struct Tiles {
+  int MT, NT, splits;
+  int64_t share;   // blocks of inputs of a workgroup
+};
+Tiles plan(int64_t rows, int64_t out, int64_t in, bool bf16) {
+  const int64_t ob = blocks_out(out), ib = blocks_in(in);
+  Tiles t{rows <= 32 ? 2 : 4, bf16 ? 4 : 2, 1, ib};
+  auto count = [&] { return (rows + 16 * t.MT - 1) / (16 * t.MT) * ((ob + 4 * t.NT - 1) / (4 * t.NT)); };
+  while (t.NT > 1 && count() < kMinTiles) t.NT /= 2;
+  const int64_t splits = count() >= kEnoughTiles ? 1 : std::max<int64_t>(1, std::min<int64_t>(kFillTiles / count(), ib / kMinShare));
+  t.share = (ib + splits - 1) / splits;
+  t.splits = static_cast<int>((ib + t.share - 1) / t.share);
+  return t;
+}
+// Whether a call runs on few_kernel, whose workgroups read the rows' activations
+// whole, each for few outputs, but in one launch without a barrier: always up to 16
+// rows; up to 32 while what they read together is small and the chip holds them at
+// once; up to 64 with few inputs and outputs.
+constexpr int64_t kFewRows = 16, kFewBytes = int64_t(64) << 20, kFewOutBlocks = 1024;
+constexpr int64_t kWideFewInBlocks = 8, kWideFewOutBlocks = 256;
+int few_columns(int64_t rows, int64_t ob) {   // NT
+  if (rows > 32) return 1;
+  if (rows > 16) return ob >= 1024 ? 4 : ob >= 512 ? 2 : 1;
+  return ob >= 2048 ? 4 : ob >= 512 ? 2 : 1;
+}
+bool runs_few(int64_t rows, int64_t out, int64_t in, bool bf16) {
+  if (rows <= kFewRows) return true;
+  if (rows > 64) return false;
+  const int64_t ob = blocks_out(out), NT = few_columns(rows, ob);
+  if (rows > 32) return ob <= kWideFewOutBlocks && blocks_in(in) <= kWideFewInBlocks;
+  return ob <= kFewOutBlocks && (ob + NT - 1) / NT * 32 * in * (bf16 ? 2 : 4) <= kFewBytes;
+}
+
 template <bool BF, Form kForm, int kGroup, int MT, int NT>
-void tiles(const LinearCall& c, hipStream_t s) {
+void tiles(const LinearCall& c, const Tiles& t, hipStream_t s) {
   constexpr int cols = kTileWaves * NT;
-  const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + cols - 1) / cols), static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)));
-  hipLaunchKernelGGL((tile_kernel<BF, kForm, kGroup, MT, NT>), grid, dim3(kTileThreads), 0, s, c);
+  const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + cols - 1) / cols), static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)), t.splits);
+  hipLaunchKernelGGL((tile_kernel<BF, kForm, kGroup, MT, NT>), grid, dim3(kTileThreads), 0, s, c, t.share);
+  if (t.splits > 1)
+    hipLaunchKernelGGL(join_kernel<BF>, dim3(static_cast<unsigned>((c.rows * c.out + 255) / 256)), dim3(256), 0, s, c, t.splits);
 }
 
 template <bool BF, Form kForm, int kGroup>
 void linear(const LinearCall& c, hipStream_t s) {
-  const int64_t ob = blocks_out(c.out), ib = blocks_in(c.in);
-  if (c.rows <= 16) {
-    if (ob >= 1024) few<BF, kForm, kGroup, 1, BF ? 4 : 2, 8, 1>(c, s);
-    else if (ob >= 512) few<BF, kForm, kGroup, 1, 2, 8, BF ? 2 : 1>(c, s);
-    else if (ib >= 64) few<BF, kForm, kGroup, 1, 1, 16, BF ? 4 : 1>(c, s);
-    else few<BF, kForm, kGroup, 1, 1, 8, BF ? 4 : 2>(c, s);
-  } else if (c.rows <= 32) {
-    if (ob >= 512) few<BF, kForm, kGroup, 2, 2, 8, 1>(c, s);
-    else few<BF, kForm, kGroup, 2, 1, 8, BF ? 2 : 1>(c, s);
+  if (runs_few(c.rows, c.out, c.in, BF)) {
+    const int NT = few_columns(c.rows, blocks_out(c.out));
+    if (c.rows > 32) {
+      few<BF, kForm, kGroup, 4, 1, 8, 1>(c, s);
+    } else if (c.rows > 16) {
+      if (NT == 4) few<BF, kForm, kGroup, 2, 4, 8, 1>(c, s);
+      else if (NT == 2) few<BF, kForm, kGroup, 2, 2, 8, 1>(c, s);
+      else few<BF, kForm, kGroup, 2, 1, 8, BF ? 2 : 1>(c, s);
+    } else {
+      if (NT == 4) few<BF, kForm, kGroup, 1, 4, 8, BF ? 2 : 1>(c, s);
+      else if (NT == 2) few<BF, kForm, kGroup, 1, 2, BF ? 16 : 8, 1>(c, s);
+      else few<BF, kForm, kGroup, 1, 1, 16, BF ? 2 : 1>(c, s);
+    }
+    return;
+  }
+  const Tiles t = plan(c.rows, c.out, c.in, BF);
+  if (t.MT == 2) {
+    if (t.NT == 1) tiles<BF, kForm, kGroup, 2, 1>(c, t, s);
+    else if (t.NT == 2) tiles<BF, kForm, kGroup, 2, 2>(c, t, s);
+    else if constexpr (BF) tiles<BF, kForm, kGroup, 2, 4>(c, t, s);
   } else {
-    const int64_t rt = (c.rows + 63) / 64;
-    if (rt * ob >= 16 * 256) tiles<BF, kForm, kGroup, 4, BF ? 4 : 2>(c, s);
-    else if (rt * ob >= 8 * 256) tiles<BF, kForm, kGroup, 4, 2>(c, s);
-    else tiles<BF, kForm, kGroup, 2, 1>(c, s);
+    if (t.NT == 1) tiles<BF, kForm, kGroup, 4, 1>(c, t, s);
+    else if (t.NT == 2) tiles<BF, kForm, kGroup, 4, 2>(c, t, s);
+    else if constexpr (BF) tiles<BF, kForm, kGroup, 4, 4>(c, t, s);
   }
 }
 
 }  // namespace
+
+int64_t workspace_bytes(int64_t rows, int64_t out, int64_t in, bool bf16) {
+  if (runs_few(rows, out, in, bf16)) return 0;
+  const int splits = plan(rows, out, in, bf16).splits;
+  return splits == 1 ? 0 : splits * rows * out * 4;
+}
 
 hipError_t launch_linear(const LinearCall& c, hipStream_t stream) {
   return by_form(c.bf16, vector_rows(c.x, c.in), c.group, [&](auto bf, auto vec, auto group) {

@@ -76,6 +76,12 @@ int64_t rwkv_w4_scales_bytes(int64_t out, int64_t in, int64_t group) {
   return dims_ok(out, in) && group_ok(group) ? rwkv_w4::scales_bytes(out, in, group) : -1;
 }
 
+int64_t rwkv_w4_linear_workspace_bytes(int64_t rows, int64_t out, int64_t in, int dtype) {
+  if (rows < 0 || rows > RWKV_W4_MAX_ROWS || !dims_ok(out, in)) return -1;
+  if (dtype != WKV7_DTYPE_F32 && dtype != WKV7_DTYPE_BF16) return -1;
+  return rwkv_w4::workspace_bytes(rows, out, in, dtype == WKV7_DTYPE_BF16);
+}
+
 int rwkv_w4_quantize(const void* weight, int64_t out, int64_t in, int64_t group, int dtype, void* packed,
                      void* scales, void* stream) {
   if (int rc = check_weight(weight, packed, scales, out, in, group, dtype)) return rc;
@@ -97,7 +103,8 @@ int rwkv_w4_dequantize(const void* packed, const void* scales, int64_t out, int6
 }
 
 int rwkv_w4_linear(const void* x, const void* packed, const void* scales, int64_t rows, int64_t out,
-                   int64_t in, int64_t group, int dtype, void* y, void* stream) {
+                   int64_t in, int64_t group, int dtype, void* y, void* workspace, int64_t workspace_bytes,
+                   void* stream) {
   if (dtype != WKV7_DTYPE_F32 && dtype != WKV7_DTYPE_BF16) return WKV7_ERR_DTYPE;
   if (!dims_ok(out, in) || !group_ok(group) || rows < 0 || rows > RWKV_W4_MAX_ROWS) return WKV7_ERR_SHAPE;
   if (!packed || !scales || (rows > 0 && (!x || !y))) return WKV7_ERR_NULL_POINTER;
@@ -105,7 +112,11 @@ int rwkv_w4_linear(const void* x, const void* packed, const void* scales, int64_
       !aligned(y, size_of(dtype)))
     return WKV7_ERR_ALIGNMENT;
   if (rows == 0) return WKV7_OK;
-  if (any_overlap({{y, rows * out * size_of(dtype)}},
+  const int64_t needed = rwkv_w4::workspace_bytes(rows, out, in, dtype == WKV7_DTYPE_BF16);
+  if (workspace_bytes < needed) return WKV7_ERR_SHAPE;
+  if (needed > 0 && !workspace) return WKV7_ERR_NULL_POINTER;
+  if (needed > 0 && !aligned(workspace, 16)) return WKV7_ERR_ALIGNMENT;
+  if (any_overlap({{y, rows * out * size_of(dtype)}, {workspace, needed}},
                   {{x, rows * in * size_of(dtype)}, {packed, rwkv_w4::packed_bytes(out, in)},
                    {scales, rwkv_w4::scales_bytes(out, in, group)}}))
     return WKV7_ERR_OVERLAP;
@@ -119,6 +130,7 @@ int rwkv_w4_linear(const void* x, const void* packed, const void* scales, int64_
   c.in = in;
   c.group = static_cast<int>(group);
   c.bf16 = dtype == WKV7_DTYPE_BF16;
+  c.partial = static_cast<float*>(workspace);
   return wkv7::hip_status(rwkv_w4::launch_linear(c, static_cast<hipStream_t>(stream)));
 }
 

@@ -31,10 +31,13 @@ struct LinearCall {
   int64_t rows, out, in;
   int group;
   bool bf16;
+  float* partial;             // workspace of workspace_bytes, or null where that is 0
 };
 
 hipError_t launch_quantize(const WeightCall& c, hipStream_t s);
 hipError_t launch_dequantize(const WeightCall& c, hipStream_t s);
+// What a product of these sizes asks for.
+int64_t workspace_bytes(int64_t rows, int64_t out, int64_t in, bool bf16);
 hipError_t launch_linear(const LinearCall& c, hipStream_t s);
 
 }  // namespace rwkv_w4

@@ -22,10 +22,11 @@ import torch
 import torch.nn as nn
 
 from . import _native
-from .neighbors import _code, _stream
+from .neighbors import _code, _ptr, _stream
 
 GROUPS = (32, 64, 128)
 MAX_DIM = 1 << 26        # RWKV_W4_MAX_DIM
+FEW_ROWS = 16            # up to as many rows no workspace is asked for
 
 
 @dataclass(frozen=True)
@@ -106,9 +107,16 @@ def linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
     x = x.contiguous()
     y = torch.empty(*x.shape[:-1], weight.out_features, dtype=x.dtype, device=dev)
     rows = x.numel() // weight.in_features
-    _native.check(_native.lib().rwkv_w4_linear(
+    lib = _native.lib()
+    nbytes = 0
+    ws = None
+    if rows > FEW_ROWS:
+        nbytes = lib.rwkv_w4_linear_workspace_bytes(rows, weight.out_features, weight.in_features, code)
+        if nbytes > 0:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _native.check(lib.rwkv_w4_linear(
         x.data_ptr(), weight.packed.data_ptr(), weight.scales.data_ptr(), rows, weight.out_features,
-        weight.in_features, weight.group_size, code, y.data_ptr(), _stream(dev)))
+        weight.in_features, weight.group_size, code, y.data_ptr(), _ptr(ws), nbytes, _stream(dev)))
     return y
 
 

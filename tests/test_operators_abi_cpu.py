@@ -49,8 +49,8 @@ def test_w4_refusals(native):
     def restore(packed=p, scales=s, out=32, d_in=256, group=64, dtype=0, weight=w):
         return lib.rwkv_w4_dequantize(packed, scales, out, d_in, group, dtype, weight, None)
 
-    def linear(x=x, packed=p, scales=s, rows=4, out=32, d_in=256, group=64, dtype=0, y=y):
-        return lib.rwkv_w4_linear(x, packed, scales, rows, out, d_in, group, dtype, y, None)
+    def linear(x=x, packed=p, scales=s, rows=4, out=32, d_in=256, group=64, dtype=0, y=y, ws=None, nbytes=0):
+        return lib.rwkv_w4_linear(x, packed, scales, rows, out, d_in, group, dtype, y, ws, nbytes, None)
     for call in (quantize, restore, linear):
         assert call(dtype=2) == 5
         for bad in (dict(out=0), dict(d_in=-1), dict(group=48), dict(out=(1 << 26) + 1)):
@@ -68,6 +68,16 @@ def test_w4_refusals(native):
         assert linear(y=other) == 7
     assert linear(y=x + 4 * 256 * 4 - 4) == 7
     assert linear(rows=0, x=None, y=None) == 0
+    # a call whose inputs are shared needs its workspace
+    size = lib.rwkv_w4_linear_workspace_bytes
+    assert size(16, 768, 1 << 14, 1) == 0 and size(0, 8, 8, 0) == 0
+    assert size(-1, 8, 8, 0) == size(1, 0, 8, 0) == size(1, 8, 8, 2) == size((1 << 20) + 1, 8, 8, 0) == -1
+    needed = size(20, 32, 1 << 14, 1)
+    big = dict(rows=20, d_in=1 << 14, dtype=1, x=FAKE * 50, y=FAKE * 60, packed=FAKE * 70, scales=FAKE * 80)
+    assert needed > 0
+    assert linear(**big) == 2 and linear(**big, ws=FAKE * 90, nbytes=needed - 1) == 2
+    assert linear(**big, nbytes=needed) == 1 and linear(**big, ws=FAKE * 90 + 8, nbytes=needed) == 6
+    assert linear(**big, ws=FAKE * 50, nbytes=needed) == 7 and linear(**big, ws=FAKE * 60, nbytes=needed) == 7
 
 
 def test_token_scores_refusals(native):
