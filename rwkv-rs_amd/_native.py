@@ -46,6 +46,17 @@ class DecodeCellParams(ctypes.Structure):
         + [(n, ctypes.c_float) for n in ("norm_time_eps", "norm_channel_eps", "group_norm_eps")])
 
 
+class W4Matrix(ctypes.Structure):
+    """struct rwkv_w4_matrix (include/rwkv_decode_w4.h)."""
+    _fields_ = [("packed", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
+
+
+class DecodeW4Weights(ctypes.Structure):
+    """struct rwkv_decode_w4_weights (include/rwkv_decode_w4.h)."""
+    _fields_ = ([(n, W4Matrix) for n in ("receptance", "key", "value", "output", "channel_key",
+                                         "channel_value")] + [("group", ctypes.c_int64)])
+
+
 def options_ref(opts):
     """A pointer argument for an optional wkv7_options (None -> NULL)."""
     return None if opts is None else ctypes.cast(ctypes.pointer(opts), ctypes.c_void_p)
@@ -74,9 +85,10 @@ SEGMENT_EXPORTS = ("wkv7_forward_workspace_bytes", "wkv7_backward_workspace_byte
 # and of include/rwkv_decode.h
 DECODE_EXPORTS = ("rwkv_decode_workspace_bytes", "rwkv_decode_cell", "rwkv_decode_head")
 
-# and of include/rwkv_w4.h and include/rwkv_token_scores.h
+# and of include/rwkv_w4.h, rwkv_decode_w4.h and rwkv_token_scores.h
 W4_EXPORTS = ("rwkv_w4_packed_bytes", "rwkv_w4_scales_bytes", "rwkv_w4_quantize",
               "rwkv_w4_dequantize", "rwkv_w4_linear_workspace_bytes", "rwkv_w4_linear")
+DECODE_W4_EXPORTS = ("rwkv_decode_cell_w4", "rwkv_decode_head_w4")
 SCORES_EXPORTS = ("rwkv_token_scores_forward", "rwkv_token_scores_backward")
 
 _P = ctypes.c_void_p
@@ -123,6 +135,8 @@ _SIGNATURES = {
     "rwkv_decode_workspace_bytes": ([_I64] * 2, _I64),
     "rwkv_decode_cell": ([_P] * 9 + [_I64] * 3 + [_INT] * 2 + [_P, _I64, _P], _INT),
     "rwkv_decode_head": ([_P] * 3 + [ctypes.c_float, _P] + [_I64] * 3 + [_P] * 2 + [_I64, _P], _INT),
+    "rwkv_decode_cell_w4": ([_P] * 10 + [_I64] * 3 + [_INT] * 2 + [_P, _I64, _P], _INT),
+    "rwkv_decode_head_w4": ([_P] * 3 + [ctypes.c_float, _P] + [_I64] * 4 + [_P] * 2 + [_I64, _P], _INT),
     "rwkv_cross_entropy_l2wrap_forward": ([_P] * 2 + [_I64] * 2 + [_INT] + [_P] * 5, _INT),
     "rwkv_cross_entropy_l2wrap_backward": ([_P] * 6 + [ctypes.c_float] + [_I64] * 2 + [_INT]
                                            + [_P] * 2, _INT),

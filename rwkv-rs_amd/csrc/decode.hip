@@ -11,7 +11,8 @@
 //   output product + residual
 //   norm + token shift + mix, key product + relu^2, value product + residual
 // The weights are read as they are stored, fp32, and rounded to bf16 in
-// registers, so no bf16 copy of them is made or kept. At 12 cells, C = 768, 8
+// registers, so no bf16 copy of them is made or kept; 4-bit ones
+// (include/rwkv_decode_w4.h) are taken apart there. At 12 cells, C = 768, 8
 // sequences, vocabulary 65536, a step took 9,150 us through the modules and
 // takes 835 so. Its kernels sum to 684 us, of which the head's 201 MB of
 // weights are 49; the rest is each launch's own latency, 3-9 us. The host, which
@@ -20,6 +21,7 @@
 
 #include "neighbors_device.hpp"
 #include "neighbors_launch.hpp"
+#include "w4_device.hpp"
 #include "wkv7_launch.hpp"
 
 namespace rwkv_decode {
@@ -136,13 +138,15 @@ hipError_t norm_mix(const NormArgs& a, hipStream_t s) {
 // (a LoRA factor's), rounded to bf16 as it is read.
 enum Act { kNone, kTanh, kSigmoid, kSquaredRelu, kResidual };
 struct Job {
-  const float* w;
+  const float* w;     // or 4-bit weights, when there are scales
   const bf16_t* x;
   void* out;          // bf16, or (kResidual) the fp32 rows the result is added to
   int K, N;
   int tile0;          // first 16-column tile of this job in the launch
   int act;
   bool in_out;        // W is [K, N]
+  const uint16_t* scales;
+  int group;
 };
 constexpr int kMaxJobs = 7;
 struct GemmArgs {
@@ -171,7 +175,56 @@ __device__ __forceinline__ bf16x8 weights8(const Job& j, int n, int k) {
 // 16] and B[column l % 16] at k = 8 (l / 16) .. + 7, the result D[row 4 (l /
 // 16) + r][column l % 16] (any order of k serves, the same for A and B).
 constexpr int kGemmWaves = 8, kDepth = 4;
+
+// The same from 4-bit weights, in steps of 128 inputs: four MFMAs, each one's
+// sum times its group's scale; what it returns is kShrink times too small.
 template <int MT>
+__device__ __forceinline__ void w4_steps(const Job& j, int tile, int wave, int rows, f32x4 (&acc)[MT]) {
+  constexpr int kW4Depth = MT == 1 ? 2 : 1;
+  const int lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
+  const int blocks = (j.K + rwkv_w4::kInputs - 1) / rwkv_w4::kInputs, groups = rwkv_w4::kInputs / j.group;
+  const rwkv_w4::u32x4* const words = reinterpret_cast<const rwkv_w4::u32x4*>(j.w);
+  for (int s0 = wave; s0 < blocks; s0 += kGemmWaves * kW4Depth) {
+    rwkv_w4::u32x4 word[kW4Depth];
+    uint16_t scale[kW4Depth][4];
+    bf16x8 x[kW4Depth][MT][4];
+#pragma unroll
+    for (int d = 0; d < kW4Depth; ++d) {
+      const int s = s0 + d * kGemmWaves;
+      if (s < blocks) {
+        const int64_t b = (int64_t)tile * blocks + s;
+        word[d] = __builtin_nontemporal_load(words + b * 64 + lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) scale[d][i] = j.scales[(b * rwkv_w4::kRows + t) * groups + i * groups / 4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const bf16_t* const row = j.x + (int64_t)min(16 * m + t, rows - 1) * j.K;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = rwkv_w4::kInputs * s + 32 * i + 8 * g;   // K is a multiple of 64
+            if (k < j.K) x[d][m][i] = *reinterpret_cast<const bf16x8*>(row + k);
+            else x[d][m][i] = bf16x8{};
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < kW4Depth; ++d)
+      if (s0 + d * kGemmWaves < blocks) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bf16x8 w = rwkv_w4::weights8(word[d][i]);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            acc[m] += __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[d][m][i], w, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0) *
+                      bf(scale[d][i]);
+        }
+      }
+  }
+}
+
+// kW4: some of the launch's jobs have 4-bit weights.
+template <int MT, bool kW4>
 __global__ __launch_bounds__(64 * kGemmWaves) void rows_gemm_kernel(const GemmArgs a) {
   __shared__ float part[kGemmWaves][MT * 256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -184,7 +237,9 @@ __global__ __launch_bounds__(64 * kGemmWaves) void rows_gemm_kernel(const GemmAr
   f32x4 acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s0 = wave; s0 < steps; s0 += kGemmWaves * kDepth) {
+  const bool w4 = kW4 && j.scales;
+  if (w4) w4_steps<MT>(j, blockIdx.x - j.tile0, wave, a.rows, acc);
+  for (int s0 = w4 ? steps : wave; s0 < steps; s0 += kGemmWaves * kDepth) {
     bf16x8 w[kDepth], x[kDepth][MT];
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
@@ -215,6 +270,7 @@ __global__ __launch_bounds__(64 * kGemmWaves) void rows_gemm_kernel(const GemmAr
     const int l = (i >> 2) & 63, row = 16 * (i >> 8) + 4 * (l >> 4) + (i & 3), col = n0 + (l & 15);
     if (row >= a.rows || col >= j.N) continue;
     const int64_t at = (int64_t)row * j.N + col;
+    if (w4) v *= rwkv_w4::kShrink;
     v = rbf(v);
     if (j.act == kResidual) {
       static_cast<float*>(j.out)[at] += v;
@@ -306,17 +362,23 @@ __global__ __launch_bounds__(1024) void lora_prepare_kernel(const PrepareArgs a)
   }
 }
 
+template <bool kW4>
+hipError_t gemm(const GemmArgs& a, int tiles, hipStream_t s) {
+  const dim3 grid(tiles), block(64 * kGemmWaves);
+  if (a.rows <= 16) hipLaunchKernelGGL((rows_gemm_kernel<1, kW4>), grid, block, 0, s, a);
+  else if (a.rows <= 32) hipLaunchKernelGGL((rows_gemm_kernel<2, kW4>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((rows_gemm_kernel<4, kW4>), grid, block, 0, s, a);
+  return hipGetLastError();
+}
 hipError_t gemm(GemmArgs& a, hipStream_t s) {
   int tiles = 0;
+  bool w4 = false;
   for (int i = 0; i < a.jobs; ++i) {
     a.job[i].tile0 = tiles;
     tiles += (a.job[i].N + 15) / 16;
+    w4 |= a.job[i].scales != nullptr;
   }
-  const dim3 grid(tiles), block(64 * kGemmWaves);
-  if (a.rows <= 16) hipLaunchKernelGGL(rows_gemm_kernel<1>, grid, block, 0, s, a);
-  else if (a.rows <= 32) hipLaunchKernelGGL(rows_gemm_kernel<2>, grid, block, 0, s, a);
-  else hipLaunchKernelGGL(rows_gemm_kernel<4>, grid, block, 0, s, a);
-  return hipGetLastError();
+  return w4 ? gemm<true>(a, tiles, s) : gemm<false>(a, tiles, s);
 }
 
 template <bool kFirst>
@@ -366,11 +428,20 @@ hipError_t launch_cell(const CellCall& c, hipStream_t stream) {
   GemmArgs g{};
   g.rows = R;
   auto add = [&](const float* w, const bf16_t* x, void* out, int64_t K, int64_t N, int act, bool in_out) {
-    g.job[g.jobs++] = Job{w, x, out, (int)K, (int)N, 0, act, in_out};
+    g.job[g.jobs++] = Job{w, x, out, (int)K, (int)N, 0, act, in_out, nullptr, 0};
   };
-  add(p.receptance, mix, rec, C, C, kNone, false);
-  add(p.key, mix + 2 * RC, key, C, C, kNone, false);
-  add(p.value, mix + 3 * RC, val, C, C, kNone, false);
+  // a large matrix: p's, or the 4-bit one in its place
+  auto add_matrix = [&](const float* w, rwkv_w4_matrix rwkv_decode_w4_weights::*q, const bf16_t* x, void* out,
+                        int64_t K, int64_t N, int act) {
+    add(c.w4 ? static_cast<const float*>((c.w4->*q).packed) : w, x, out, K, N, act, false);
+    if (!c.w4) return;
+    g.job[g.jobs - 1].scales = static_cast<const uint16_t*>((c.w4->*q).scales);
+    g.job[g.jobs - 1].group = (int)c.w4->group;
+  };
+  typedef rwkv_decode_w4_weights W4;
+  add_matrix(p.receptance, &W4::receptance, mix, rec, C, C, kNone);
+  add_matrix(p.key, &W4::key, mix + 2 * RC, key, C, C, kNone);
+  add_matrix(p.value, &W4::value, mix + 3 * RC, val, C, C, kNone);
   add(p.rate_a, mix + 4 * RC, h_rate, C, p.rate_rank, kNone, true);
   add(p.decay_a, mix + RC, h_decay, C, p.decay_rank, kTanh, true);
   add(p.gate_a, mix + 5 * RC, h_gate, C, p.gate_rank, kSigmoid, true);
@@ -447,7 +518,7 @@ hipError_t launch_cell(const CellCall& c, hipStream_t stream) {
 
   g = GemmArgs{};
   g.rows = R;
-  add(p.output, read, c.x, C, C, kResidual, false);
+  add_matrix(p.output, &W4::output, read, c.x, C, C, kResidual);
   if ((e = gemm(g, stream)) != hipSuccess) return e;
 
   // channel mixer
@@ -462,11 +533,11 @@ hipError_t launch_cell(const CellCall& c, hipStream_t stream) {
   bf16_t* const hidden = mix + RC;   // [rows, 4 C]
   g = GemmArgs{};
   g.rows = R;
-  add(p.channel_key, mix, hidden, C, 4 * (int64_t)C, kSquaredRelu, false);
+  add_matrix(p.channel_key, &W4::channel_key, mix, hidden, C, 4 * (int64_t)C, kSquaredRelu);
   if ((e = gemm(g, stream)) != hipSuccess) return e;
   g = GemmArgs{};
   g.rows = R;
-  add(p.channel_value, hidden, c.x, 4 * (int64_t)C, C, kResidual, false);
+  add_matrix(p.channel_value, &W4::channel_value, hidden, c.x, 4 * (int64_t)C, C, kResidual);
   return gemm(g, stream);
 }
 
@@ -484,7 +555,12 @@ hipError_t launch_head(const HeadCall& c, hipStream_t stream) {
   GemmArgs g{};
   g.rows = c.rows;
   g.jobs = 1;
-  g.job[0] = Job{c.unembed, n.out[0], c.logits, C, (int)c.vocab, 0, kNone, false};
+  g.job[0] = Job{c.unembed, n.out[0], c.logits, C, (int)c.vocab, 0, kNone, false, nullptr, 0};
+  if (c.unembed_w4) {
+    g.job[0].w = static_cast<const float*>(c.unembed_w4->packed);
+    g.job[0].scales = static_cast<const uint16_t*>(c.unembed_w4->scales);
+    g.job[0].group = c.group;
+  }
   return gemm(g, stream);
 }
 

@@ -5,6 +5,7 @@
 #include <cmath>
 #include <initializer_list>
 
+#include "w4_launch.hpp"
 #include "wkv7_launch.hpp"
 
 namespace {
@@ -24,6 +25,7 @@ bool ranks_fit(const rwkv_decode_cell_params& p, int64_t C) {
   return p.decay_rank > 0 && p.rate_rank > 0 && p.gate_rank > 0 && (!p.residual_a || p.residual_rank > 0) &&
          sum <= 4 * C;
 }
+bool group_ok(int64_t group) { return group == 32 || group == 64 || group == 128; }
 bool eps_ok(float e) { return e >= 0.f && std::isfinite(e); }
 
 struct Range {
@@ -60,19 +62,12 @@ bool any_overlap(Ranges outs) {
   return false;
 }
 
-}  // namespace
-
-extern "C" {
-
-int64_t rwkv_decode_workspace_bytes(int64_t rows, int64_t num_heads) {
-  return supported(rows, num_heads) ? rwkv_decode::workspace_bytes(rows, num_heads) : -1;
-}
-
-int rwkv_decode_cell(const rwkv_decode_cell_params* params, float* x, const int32_t* batch_ids, void* state,
-                     const float* shift_time_in, float* shift_time_out, const float* shift_channel_in,
-                     float* shift_channel_out, const int32_t* elapsed_t, int64_t rows, int64_t num_heads,
-                     int64_t full_batch, int state_dtype, int use_dither, void* workspace,
-                     int64_t workspace_bytes, void* stream) {
+// w4: the six large matrices, in the place of params'; null: params'
+int cell(const rwkv_decode_cell_params* params, const rwkv_decode_w4_weights* w4, float* x,
+         const int32_t* batch_ids, void* state, const float* shift_time_in, float* shift_time_out,
+         const float* shift_channel_in, float* shift_channel_out, const int32_t* elapsed_t, int64_t rows,
+         int64_t num_heads, int64_t full_batch, int state_dtype, int use_dither, void* workspace,
+         int64_t workspace_bytes, void* stream) {
   if (state_dtype != WKV7_DTYPE_F32 && state_dtype != WKV7_DTYPE_BF16) return WKV7_ERR_DTYPE;
   // distinct ids need as many slots, as in wkv7_infer_forward
   if (!supported(rows, num_heads) || full_batch < rows || full_batch > INT32_MAX - RWKV_DECODE_MAX_ROWS)
@@ -80,6 +75,7 @@ int rwkv_decode_cell(const rwkv_decode_cell_params* params, float* x, const int3
   if (use_dither != 0 && use_dither != 1) return WKV7_ERR_FLAGS;
   if (use_dither && state_dtype == WKV7_DTYPE_F32) return WKV7_ERR_FLAGS;
   if (!params) return WKV7_ERR_NULL_POINTER;
+  if (w4 && !group_ok(w4->group)) return WKV7_ERR_SHAPE;
   const rwkv_decode_cell_params& p = *params;
   const int64_t C = num_heads * 64;
   if (!ranks_fit(p, C)) return WKV7_ERR_SHAPE;
@@ -87,15 +83,27 @@ int rwkv_decode_cell(const rwkv_decode_cell_params* params, float* x, const int3
   const int64_t row = C * 4, matrix = C * row;   // bytes
   const Ranges weights = {{p.norm_time_weight, row}, {p.norm_time_bias, row}, {p.norm_channel_weight, row},
                           {p.norm_channel_bias, row}, {p.mix[0], row}, {p.mix[1], row}, {p.mix[2], row},
-                          {p.mix[3], row}, {p.mix[4], row}, {p.mix[5], row}, {p.receptance, matrix},
-                          {p.key, matrix}, {p.value, matrix}, {p.output, matrix},
+                          {p.mix[3], row}, {p.mix[4], row}, {p.mix[5], row},
                           {p.decay_a, p.decay_rank * row}, {p.decay_b, p.decay_rank * row}, {p.decay_bias, row},
                           {p.rate_a, p.rate_rank * row}, {p.rate_b, p.rate_rank * row}, {p.rate_bias, row},
                           {p.gate_a, p.gate_rank * row}, {p.gate_b, p.gate_rank * row}, {p.key_removal, row},
                           {p.key_replacement, row}, {p.bonus, row}, {p.group_norm_weight, row},
-                          {p.group_norm_bias, row}, {p.channel_mix, row}, {p.channel_key, 4 * matrix},
-                          {p.channel_value, 4 * matrix}};
+                          {p.group_norm_bias, row}, {p.channel_mix, row}};
+  const Ranges plain = {{p.receptance, matrix}, {p.key, matrix}, {p.value, matrix}, {p.output, matrix},
+                        {p.channel_key, 4 * matrix}, {p.channel_value, 4 * matrix}};
+  const rwkv_decode_w4_weights q = w4 ? *w4 : rwkv_decode_w4_weights{};
+  const int64_t square = rwkv_w4::packed_bytes(C, C), up = rwkv_w4::packed_bytes(4 * C, C),
+                down = rwkv_w4::packed_bytes(C, 4 * C), group = w4 ? q.group : 128;
+  const int64_t square_s = rwkv_w4::scales_bytes(C, C, group), up_s = rwkv_w4::scales_bytes(4 * C, C, group),
+                down_s = rwkv_w4::scales_bytes(C, 4 * C, group);
+  const Ranges packed = {{q.receptance.packed, square}, {q.receptance.scales, square_s}, {q.key.packed, square},
+                         {q.key.scales, square_s}, {q.value.packed, square}, {q.value.scales, square_s},
+                         {q.output.packed, square}, {q.output.scales, square_s}, {q.channel_key.packed, up},
+                         {q.channel_key.scales, up_s}, {q.channel_value.packed, down},
+                         {q.channel_value.scales, down_s}};
+  const Ranges& matrices = w4 ? packed : plain;
   if (int rc = check_pointers(weights)) return rc;
+  if (int rc = check_pointers(matrices)) return rc;
   const int64_t res = p.residual_a ? p.residual_rank * row : 0;
   const Ranges residual = {{p.residual_a, res}, {p.residual_b, res}, {p.residual_bias, row}};
   if (p.residual_a)
@@ -112,11 +120,12 @@ int rwkv_decode_cell(const rwkv_decode_cell_params* params, float* x, const int3
   if (!aligned(batch_ids, 4) || !aligned(elapsed_t, 4)) return WKV7_ERR_ALIGNMENT;
   if (workspace_bytes < needed) return WKV7_ERR_SHAPE;
   if (any_overlap(outs) || any_overlap(outs, shifts) || any_overlap(outs, weights) ||
-      (p.residual_a && any_overlap(outs, residual)) ||
+      any_overlap(outs, matrices) || (p.residual_a && any_overlap(outs, residual)) ||
       any_overlap(outs, {{batch_ids, rows * 4}, {elapsed_t, full_batch * 4}}))
     return WKV7_ERR_OVERLAP;
   rwkv_decode::CellCall c{};
   c.p = params;
+  c.w4 = w4;
   c.x = x;
   c.batch_ids = batch_ids;
   c.state = state;
@@ -134,20 +143,28 @@ int rwkv_decode_cell(const rwkv_decode_cell_params* params, float* x, const int3
   return wkv7::hip_status(rwkv_decode::launch_cell(c, static_cast<hipStream_t>(stream)));
 }
 
-int rwkv_decode_head(const float* x, const float* norm_weight, const float* norm_bias, float norm_eps,
-                     const float* unembed, int64_t rows, int64_t num_heads, int64_t vocab, void* logits,
-                     void* workspace, int64_t workspace_bytes, void* stream) {
+int head(const float* x, const float* norm_weight, const float* norm_bias, float norm_eps, const float* unembed,
+         const rwkv_w4_matrix* unembed_w4, int64_t group, int64_t rows, int64_t num_heads, int64_t vocab,
+         void* logits, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!supported(rows, num_heads) || vocab <= 0 || vocab > INT32_MAX - 16) return WKV7_ERR_SHAPE;
   if (!eps_ok(norm_eps)) return WKV7_ERR_SHAPE;
+  const bool plain = !unembed_w4;
+  if (!plain && (!group_ok(group) || vocab > RWKV_W4_MAX_DIM)) return WKV7_ERR_SHAPE;
+  const rwkv_w4_matrix q = plain ? rwkv_w4_matrix{} : *unembed_w4;
   const int64_t C = num_heads * 64, needed = rwkv_decode::workspace_bytes(rows, num_heads);
-  const Ranges weights = {{norm_weight, C * 4}, {norm_bias, C * 4}, {unembed, vocab * C * 4}};
+  const Ranges weights = {{norm_weight, C * 4}, {norm_bias, C * 4},
+                          {plain ? unembed : q.packed, plain ? vocab * C * 4 : rwkv_w4::packed_bytes(vocab, C)}};
+  const Ranges scales = {{q.scales, plain ? 0 : rwkv_w4::scales_bytes(vocab, C, group)}};
   if (int rc = check_pointers(weights)) return rc;
+  if (!plain)
+    if (int rc = check_pointers(scales)) return rc;
   if (rows == 0) return WKV7_OK;
   const Ranges rows_in = {{x, rows * C * 4}}, outs = {{logits, rows * vocab * 2}, {workspace, needed}};
   if (int rc = check_pointers(rows_in)) return rc;
   if (int rc = check_pointers(outs)) return rc;
   if (workspace_bytes < needed) return WKV7_ERR_SHAPE;
-  if (any_overlap(outs) || any_overlap(outs, weights) || any_overlap(outs, rows_in)) return WKV7_ERR_OVERLAP;
+  if (any_overlap(outs) || any_overlap(outs, weights) || any_overlap(outs, scales) || any_overlap(outs, rows_in))
+    return WKV7_ERR_OVERLAP;
   rwkv_decode::HeadCall c{};
   c.x = x;
   c.norm_weight = norm_weight;
@@ -157,9 +174,55 @@ int rwkv_decode_head(const float* x, const float* norm_weight, const float* norm
   c.rows = static_cast<int>(rows);
   c.H = static_cast<int>(num_heads);
   c.vocab = vocab;
+  c.unembed_w4 = unembed_w4;
+  c.group = static_cast<int>(group);
   c.logits = static_cast<rwkv_decode::bf16_t*>(logits);
   c.workspace = workspace;
   return wkv7::hip_status(rwkv_decode::launch_head(c, static_cast<hipStream_t>(stream)));
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t rwkv_decode_workspace_bytes(int64_t rows, int64_t num_heads) {
+  return supported(rows, num_heads) ? rwkv_decode::workspace_bytes(rows, num_heads) : -1;
+}
+
+int rwkv_decode_cell(const rwkv_decode_cell_params* params, float* x, const int32_t* batch_ids, void* state,
+                     const float* shift_time_in, float* shift_time_out, const float* shift_channel_in,
+                     float* shift_channel_out, const int32_t* elapsed_t, int64_t rows, int64_t num_heads,
+                     int64_t full_batch, int state_dtype, int use_dither, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+  return cell(params, nullptr, x, batch_ids, state, shift_time_in, shift_time_out, shift_channel_in,
+              shift_channel_out, elapsed_t, rows, num_heads, full_batch, state_dtype, use_dither, workspace,
+              workspace_bytes, stream);
+}
+
+int rwkv_decode_head(const float* x, const float* norm_weight, const float* norm_bias, float norm_eps,
+                     const float* unembed, int64_t rows, int64_t num_heads, int64_t vocab, void* logits,
+                     void* workspace, int64_t workspace_bytes, void* stream) {
+  return head(x, norm_weight, norm_bias, norm_eps, unembed, nullptr, 0, rows, num_heads, vocab, logits, workspace,
+              workspace_bytes, stream);
+}
+
+int rwkv_decode_cell_w4(const rwkv_decode_cell_params* params, const rwkv_decode_w4_weights* weights, float* x,
+                        const int32_t* batch_ids, void* state, const float* shift_time_in, float* shift_time_out,
+                        const float* shift_channel_in, float* shift_channel_out, const int32_t* elapsed_t,
+                        int64_t rows, int64_t num_heads, int64_t full_batch, int state_dtype, int use_dither,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!weights) return WKV7_ERR_NULL_POINTER;
+  return cell(params, weights, x, batch_ids, state, shift_time_in, shift_time_out, shift_channel_in,
+              shift_channel_out, elapsed_t, rows, num_heads, full_batch, state_dtype, use_dither, workspace,
+              workspace_bytes, stream);
+}
+
+int rwkv_decode_head_w4(const float* x, const float* norm_weight, const float* norm_bias, float norm_eps,
+                        const rwkv_w4_matrix* unembed, int64_t group, int64_t rows, int64_t num_heads,
+                        int64_t vocab, void* logits, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!unembed) return WKV7_ERR_NULL_POINTER;
+  return head(x, norm_weight, norm_bias, norm_eps, nullptr, unembed, group, rows, num_heads, vocab, logits,
+              workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

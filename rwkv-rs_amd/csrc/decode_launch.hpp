@@ -6,7 +6,7 @@
 
 #include <cstdint>
 
-#include "../../include/rwkv_decode.h"
+#include "../../include/rwkv_decode_w4.h"
 
 namespace rwkv_decode {
 
@@ -14,6 +14,7 @@ typedef uint16_t bf16_t;
 
 struct CellCall {
   const rwkv_decode_cell_params* p;
+  const rwkv_decode_w4_weights* w4;   // null: the matrices are p's
   float* x;
   const int32_t* batch_ids;
   void* state;
@@ -30,6 +31,8 @@ struct HeadCall {
   float eps;
   int rows, H;
   int64_t vocab;
+  const rwkv_w4_matrix* unembed_w4;   // null: unembed
+  int group;
   bf16_t* logits;
   void* workspace;
 };

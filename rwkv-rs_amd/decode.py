@@ -1,4 +1,5 @@
-"""One decode step of the model on the kernels of include/rwkv_decode.h.
+"""One decode step of the model on the kernels of include/rwkv_decode.h and, for
+a model with 4-bit weights (``w4.quantize_model``), include/rwkv_decode_w4.h.
 
 ``AutoRegressiveModel.infer`` uses it for a step of up to 64 sequences under
 bf16 autocast with fp32 parameters (``step`` says when), in place of the
@@ -20,7 +21,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 
-from . import _native
+from . import _native, w4
 
 MAX_ROWS = 64        # RWKV_DECODE_MAX_ROWS
 # The kernels take C up to RWKV_DECODE_MAX_DIM (8192), but they read the fp32
@@ -74,6 +75,16 @@ class _Reader:
             raise _Unsupported
         return self.param(module, "weight", (d_out, d_in))
 
+    def packed(self, module, d_in, d_out):
+        """(packed, scales, group size) of a linear layer with a 4-bit weight."""
+        if (not _plain(module, w4.W4Linear) or module.in_features != d_in
+                or module.out_features != d_out or module.group_size not in w4.GROUPS):
+            raise _Unsupported
+        blocks, b = (-(-d_out // 16), -(-d_in // 128)), module._buffers
+        return (self.tensor(b["packed"], (*blocks, 4, 16, 16), torch.uint8),
+                self.tensor(b["scales"], (*blocks, 16, 128 // module.group_size), torch.bfloat16),
+                module.group_size)
+
     def norm(self, module, dim):
         if (not _plain(module, nn.LayerNorm) or module.normalized_shape != (dim,)
                 or not 0.0 <= module.eps < float("inf")):
@@ -82,8 +93,32 @@ class _Reader:
                 float(module.eps))
 
 
+def _matrices(p, wp, gr, cm, rd: _Reader, C: int):
+    """A cell's six large matrices, into ``p``, or as rwkv_decode_w4_weights
+    where they are 4-bit ones of one group size."""
+    of = (("receptance", wp._modules["projection_receptance"], C, C),
+          ("key", wp._modules["projection_key"], C, C),
+          ("value", wp._modules["projection_value"], C, C),
+          ("output", gr._modules["projection_output"], C, C),
+          ("channel_key", cm._modules["key"], C, 4 * C),
+          ("channel_value", cm._modules["value"], 4 * C, C))
+    if type(of[0][1]) is not w4.W4Linear:
+        for name, module, d_in, d_out in of:
+            setattr(p, name, rd.linear(module, d_in, d_out))
+        return None
+    q = _native.DecodeW4Weights()
+    for name, module, d_in, d_out in of:
+        packed, scales, group = rd.packed(module, d_in, d_out)
+        if q.group not in (0, group):
+            raise _Unsupported
+        q.group = group
+        setattr(q, name, _native.W4Matrix(packed, scales))
+    return q
+
+
 def _cell_params(m, cell, rd: _Reader, C: int, H: int):
-    """The rwkv_decode_cell_params of one CausalCell."""
+    """The rwkv_decode_cell_params of one CausalCell, and its 4-bit matrices or
+    None."""
     if not _plain(cell, m.CausalCell):
         raise _Unsupported
     sub = cell._modules
@@ -107,10 +142,7 @@ def _cell_params(m, cell, rd: _Reader, C: int, H: int):
         p.mix[i] = rd.param(wp, "param_" + name, row)
     p.mix[5] = rd.param(gr, "param_gate", row)
     wsub, gsub = wp._modules, gr._modules
-    p.receptance = rd.linear(wsub["projection_receptance"], C, C)
-    p.key = rd.linear(wsub["projection_key"], C, C)
-    p.value = rd.linear(wsub["projection_value"], C, C)
-    p.output = rd.linear(gsub["projection_output"], C, C)
+    matrices = _matrices(p, wp, gr, cm, rd, C)
 
     def lora(module, activation, bias):
         # the modules call the LoRA's product, or its forward, which does
@@ -147,14 +179,12 @@ def _cell_params(m, cell, rd: _Reader, C: int, H: int):
     p.group_norm_bias = rd.param(gn, "bias", (C,))
     p.group_norm_eps = m.GROUP_NORM_EPS
     p.channel_mix = rd.param(cm, "token_shift_diff_scale", row)
-    p.channel_key = rd.linear(cm._modules["key"], C, 4 * C)
-    p.channel_value = rd.linear(cm._modules["value"], 4 * C, C)
     for rank in (p.decay_rank, p.rate_rank, p.gate_rank, p.residual_rank or 32):
         if rank % 32 or not 0 < rank <= C:
             raise _Unsupported
     if p.decay_rank + p.rate_rank + p.gate_rank + (p.residual_rank or 0) > 4 * C:
         raise _Unsupported
-    return p
+    return p, matrices
 
 
 def step(model, contexts, batch_ids, infer_state, context_mask,
@@ -162,7 +192,8 @@ def step(model, contexts, batch_ids, infer_state, context_mask,
     """``(logits or None,)`` of one decode step, its slots of ``infer_state``
     updated, or None where the step is not one these kernels take: one token of
     at most 64 sequences, no mask, bf16 autocast over fp32 parameters on the
-    GPU, and a model made of the framework's own modules."""
+    GPU, and a model made of the framework's own modules (the large matrices of
+    a cell all fp32 or all 4-bit)."""
     from . import model as m
     rows, T = contexts.shape
     if not infer_state.state or infer_state.elapsed_t is None:
@@ -193,12 +224,14 @@ def step(model, contexts, batch_ids, infer_state, context_mask,
                   rd.tensor(t, (slots, C)), rd.tensor(ch, (slots, C)))
                  for c, s, t, ch in zip(cells, infer_state.state, infer_state.shift_time,
                                         infer_state.shift_channel)]
-        if calls[0][0].residual_a or not all(c[0].residual_a for c in calls[1:]):
+        if calls[0][0][0].residual_a or not all(c[0][0].residual_a for c in calls[1:]):
             return None   # the first cell is the one without a value residual
         head = None
         if unembed_mode != "skip":
+            unembed = model._modules["unembed"]
+            read = rd.packed if type(unembed) is w4.W4Linear else rd.linear
             head = (rd.norm(model._modules["layer_norm_for_unembed"], C),
-                    rd.linear(model._modules["unembed"], C, model.vocab_size))
+                    read(unembed, C, model.vocab_size))
     except LookupError:
         return None
     ids = batch_ids.to(device=dev, dtype=torch.int32).contiguous()
@@ -217,18 +250,27 @@ def step(model, contexts, batch_ids, infer_state, context_mask,
     code = _native.DTYPE_BF16 if bf16_state else _native.DTYPE_F32
     next_time = [torch.empty_like(t) for t in infer_state.shift_time]
     next_channel = [torch.empty_like(t) for t in infer_state.shift_channel]
-    for (p, state, time_in, channel_in), time_out, channel_out in zip(calls, next_time, next_channel):
-        _native.check(lib.rwkv_decode_cell(
-            ctypes.addressof(p), x.data_ptr(), ids.data_ptr(), state, time_in, time_out.data_ptr(),
-            channel_in, channel_out.data_ptr(), elapsed.data_ptr(), rows, H, slots, code,
-            int(bf16_state), ws.data_ptr(), nbytes, stream))
+    for ((p, q), state, time_in, channel_in), time_out, channel_out in zip(calls, next_time,
+                                                                            next_channel):
+        rest = (x.data_ptr(), ids.data_ptr(), state, time_in, time_out.data_ptr(), channel_in,
+                channel_out.data_ptr(), elapsed.data_ptr(), rows, H, slots, code, int(bf16_state),
+                ws.data_ptr(), nbytes, stream)
+        if q is None:
+            _native.check(lib.rwkv_decode_cell(ctypes.addressof(p), *rest))
+        else:
+            _native.check(lib.rwkv_decode_cell_w4(ctypes.addressof(p), ctypes.addressof(q), *rest))
     infer_state.shift_time[:] = next_time
     infer_state.shift_channel[:] = next_channel
     if head is None:
         return (None,)
     (weight, bias, eps), unembed = head
     logits = torch.empty((rows, 1, model.vocab_size), dtype=torch.bfloat16, device=dev)
-    _native.check(lib.rwkv_decode_head(x.data_ptr(), weight, bias, eps, unembed, rows, H,
-                                       model.vocab_size, logits.data_ptr(), ws.data_ptr(), nbytes,
-                                       stream))
+    rest = (rows, H, model.vocab_size, logits.data_ptr(), ws.data_ptr(), nbytes, stream)
+    if isinstance(unembed, tuple):
+        packed, scales, group = unembed
+        matrix = _native.W4Matrix(packed, scales)
+        _native.check(lib.rwkv_decode_head_w4(x.data_ptr(), weight, bias, eps,
+                                              ctypes.addressof(matrix), group, *rest))
+    else:
+        _native.check(lib.rwkv_decode_head(x.data_ptr(), weight, bias, eps, unembed, *rest))
     return (logits,)

@@ -50,6 +50,7 @@ import torch.nn.functional as F
 from . import decode as _decode
 from . import lm_loss as _loss
 from . import neighbors as _nb
+from . import token_scores as _scores
 from . import wkv7 as _wkv7
 
 CHUNK_LEN = 16                 # time_mixer/mod.rs:190
@@ -629,6 +630,20 @@ class AutoRegressiveModel(nn.Module):
             return fused[0]
         x = self.layer_norm_for_first_cell(self.embed(contexts))
         return self._infer_cells(x, T, batch_ids, infer_state, context_mask, unembed_mode)
+
+    @torch.no_grad()
+    def score(self, contexts: torch.Tensor, batch_ids: torch.Tensor, infer_state: "InferState",
+              context_mask: Optional[torch.Tensor] = None, top: int = 0) -> "_scores.TokenScores":
+        """How likely the model finds a given text: ``infer`` over ``contexts``
+        ([batch, T]), and of every token but a row's first the log probability,
+        the entropy it was taken from and the ``top`` most likely alternatives,
+        [batch, T - 1, ..] (``token_scores.token_scores``). The slots advance as
+        in ``infer``. Where ``context_mask`` is 0 at a token or at the one before
+        it, its scores mean nothing."""
+        logits = self.infer(contexts, batch_ids, infer_state, context_mask, "full")
+        # a row's last logits have no token yet; scored like the others, they are cut off
+        tokens = torch.cat([contexts[:, 1:], contexts[:, :1]], dim=1)
+        return _scores.TokenScores(*(s[:, :-1] for s in _scores.token_scores(logits, tokens, top)))
 
     def _infer_cells(self, x, T, batch_ids, infer_state, context_mask, unembed_mode):
         """``infer`` of T steps from the first cell on."""

@@ -19,7 +19,7 @@ def native():
     return n
 
 
-@pytest.mark.parametrize("header,exports", [("rwkv_w4.h", "W4_EXPORTS"),
+@pytest.mark.parametrize("header,exports", [("rwkv_w4.h", "W4_EXPORTS"), ("rwkv_decode_w4.h", "DECODE_W4_EXPORTS"),
                                             ("rwkv_token_scores.h", "SCORES_EXPORTS")])
 def test_exports(native, header, exports):
     declared = declared_functions(os.path.join(REPO, "include", header), "rwkv_")
@@ -72,12 +72,61 @@ def test_w4_refusals(native):
     size = lib.rwkv_w4_linear_workspace_bytes
     assert size(16, 768, 1 << 14, 1) == 0 and size(0, 8, 8, 0) == 0
     assert size(-1, 8, 8, 0) == size(1, 0, 8, 0) == size(1, 8, 8, 2) == size((1 << 20) + 1, 8, 8, 0) == -1
-    needed = size(20, 32, 1 << 14, 1)
-    big = dict(rows=20, d_in=1 << 14, dtype=1, x=FAKE * 50, y=FAKE * 60, packed=FAKE * 70, scales=FAKE * 80)
+    needed = size(100, 32, 1 << 14, 1)
+    big = dict(rows=100, d_in=1 << 14, dtype=1, x=FAKE * 50, y=FAKE * 60, packed=FAKE * 70, scales=FAKE * 80)
     assert needed > 0
     assert linear(**big) == 2 and linear(**big, ws=FAKE * 90, nbytes=needed - 1) == 2
     assert linear(**big, nbytes=needed) == 1 and linear(**big, ws=FAKE * 90 + 8, nbytes=needed) == 6
     assert linear(**big, ws=FAKE * 50, nbytes=needed) == 7 and linear(**big, ws=FAKE * 60, nbytes=needed) == 7
+
+
+def test_decode_w4_refusals():
+    import ctypes
+    if torch.cuda.is_available():
+        pytest.skip("an accepted call would launch on addresses that are not memory")
+    from test_decode_step_cpu import GIB, HIP, NULL, SHAPE, ALIGNMENT, OVERLAP, _params
+    native = load_pkg()._native
+    lib = native.lib()
+    rows, heads, C = 3, 3, 192
+    need = lib.rwkv_decode_workspace_bytes(rows, heads)
+
+    def weights(group=64, **over):
+        q = native.DecodeW4Weights()
+        q.group = group
+        for i, (name, kind) in enumerate(q._fields_[:-1]):
+            setattr(q, name, native.W4Matrix((2000 + 2 * i) * GIB, (2001 + 2 * i) * GIB))
+        for name, at in over.items():
+            setattr(q, name, native.W4Matrix(*at))
+        return q
+
+    def cell(q, p=None, **over):
+        p = p or _params(native, True)
+        for name in ("receptance", "key", "value", "output", "channel_key", "channel_value"):
+            setattr(p, name, None)                                  # not looked at
+        a = dict(x=GIB, ws=9 * GIB, nbytes=need)
+        a.update(over)
+        return lib.rwkv_decode_cell_w4(
+            ctypes.addressof(p), ctypes.addressof(q) if q else None, a["x"], 2 * GIB, 3 * GIB, 4 * GIB, 5 * GIB,
+            6 * GIB, 7 * GIB, 8 * GIB, rows, heads, 4, 1, 1, a["ws"], a["nbytes"], None)
+    assert cell(weights()) == HIP and cell(None) == NULL            # nothing to refuse but the missing GPU
+    for group in (0, 16, 48, 256):
+        assert cell(weights(group)) == SHAPE
+    assert cell(weights(key=(None, GIB * 99))) == NULL and cell(weights(output=(GIB * 99, None))) == NULL
+    assert cell(weights(value=(GIB * 99 + 8, GIB * 98))) == ALIGNMENT
+    last = weights().channel_value
+    size, scales = lib.rwkv_w4_packed_bytes(C, 4 * C), lib.rwkv_w4_scales_bytes(C, 4 * C, 64)
+    assert cell(weights(), x=last.packed + size - 16) == OVERLAP and cell(weights(), x=last.packed + size) == HIP
+    assert cell(weights(), ws=last.scales + scales - 16) == OVERLAP and cell(weights(), ws=last.scales + scales) == HIP
+    assert cell(weights(), nbytes=need - 1) == SHAPE
+
+    def head(q=(4 * GIB, 5 * GIB), group=32, vocab=50, logits=6 * GIB, ws=7 * GIB):
+        m = native.W4Matrix(*q) if q else None
+        return lib.rwkv_decode_head_w4(GIB, 2 * GIB, 3 * GIB, 1e-5, ctypes.addressof(m) if m else None, group, rows,
+                                       heads, vocab, logits, ws, need, None)
+    assert head() == HIP and head(None) == NULL and head((None, GIB)) == NULL and head((GIB * 4, None)) == NULL
+    assert head(group=8) == SHAPE and head(vocab=0) == SHAPE and head(vocab=(1 << 26) + 1) == SHAPE
+    assert head((4 * GIB + 4, 5 * GIB)) == ALIGNMENT
+    assert head(logits=4 * GIB) == OVERLAP and head(logits=5 * GIB) == OVERLAP and head(ws=5 * GIB) == OVERLAP
 
 
 def test_token_scores_refusals(native):
