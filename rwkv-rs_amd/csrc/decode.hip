@@ -176,26 +176,31 @@ __device__ __forceinline__ bf16x8 weights8(const Job& j, int n, int k) {
 // 16) + r][column l % 16] (any order of k serves, the same for A and B).
 constexpr int kGemmWaves = 8, kDepth = 4;
 
-// The same from 4-bit weights, in steps of 128 inputs: four MFMAs, each one's
-// sum times its group's scale; what it returns is kShrink times too small.
-template <int MT>
-__device__ __forceinline__ void w4_steps(const Job& j, int tile, int wave, int rows, f32x4 (&acc)[MT]) {
-  constexpr int kW4Depth = MT == 1 ? 2 : 1;
+// The same from 4-bit weights, 16 NT columns in steps of 128 inputs: four MFMAs a
+// tile, each one's sum times its group's scale; what it returns is kShrink times
+// too small.
+template <int MT, int NT>
+__device__ __forceinline__ void w4_steps(const Job& j, int tile, int wave, int rows, f32x4 (&acc)[MT][NT]) {
+  constexpr int kW4Depth = MT * NT == 1 ? 2 : 1;
   const int lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
   const int blocks = (j.K + rwkv_w4::kInputs - 1) / rwkv_w4::kInputs, groups = rwkv_w4::kInputs / j.group;
+  const int last = (j.N + rwkv_w4::kRows - 1) / rwkv_w4::kRows - 1;
   const rwkv_w4::u32x4* const words = reinterpret_cast<const rwkv_w4::u32x4*>(j.w);
   for (int s0 = wave; s0 < blocks; s0 += kGemmWaves * kW4Depth) {
-    rwkv_w4::u32x4 word[kW4Depth];
-    uint16_t scale[kW4Depth][4];
+    rwkv_w4::u32x4 word[kW4Depth][NT];
+    uint16_t scale[kW4Depth][NT][4];
     bf16x8 x[kW4Depth][MT][4];
 #pragma unroll
     for (int d = 0; d < kW4Depth; ++d) {
       const int s = s0 + d * kGemmWaves;
       if (s < blocks) {
-        const int64_t b = (int64_t)tile * blocks + s;
-        word[d] = __builtin_nontemporal_load(words + b * 64 + lane);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) scale[d][i] = j.scales[(b * rwkv_w4::kRows + t) * groups + i * groups / 4];
+        for (int n = 0; n < NT; ++n) {
+          const int64_t b = (int64_t)min(tile * NT + n, last) * blocks + s;   // past the end: not stored
+          word[d][n] = __builtin_nontemporal_load(words + b * 64 + lane);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) scale[d][n][i] = j.scales[(b * rwkv_w4::kRows + t) * groups + i * groups / 4];
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           const bf16_t* const row = j.x + (int64_t)min(16 * m + t, rows - 1) * j.K;
@@ -212,33 +217,38 @@ __device__ __forceinline__ void w4_steps(const Job& j, int tile, int wave, int r
     for (int d = 0; d < kW4Depth; ++d)
       if (s0 + d * kGemmWaves < blocks) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bf16x8 w = rwkv_w4::weights8(word[d][i]);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
-            acc[m] += __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[d][m][i], w, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0) *
-                      bf(scale[d][i]);
-        }
+          for (int i = 0; i < 4; ++i) {
+            const bf16x8 w = rwkv_w4::weights8(word[d][n][i]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              acc[m][n] += __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[d][m][i], w, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0) *
+                           bf(scale[d][n][i]);
+          }
       }
   }
 }
 
-// kW4: some of the launch's jobs have 4-bit weights.
-template <int MT, bool kW4>
+// Jobs with 4-bit weights take 16 NT columns a workgroup; NT = 0: there are none.
+template <int MT, int NT>
 __global__ __launch_bounds__(64 * kGemmWaves) void rows_gemm_kernel(const GemmArgs a) {
-  __shared__ float part[kGemmWaves][MT * 256];
+  constexpr int kCols = NT > 0 ? NT : 1;
+  __shared__ float part[kGemmWaves][MT * kCols * 256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int ji = 0;
   while (ji + 1 < a.jobs && (int)blockIdx.x >= a.job[ji + 1].tile0) ++ji;
   const Job& j = a.job[ji];
-  const int n0 = 16 * (blockIdx.x - j.tile0);
+  const bool w4 = NT > 0 && j.scales;
+  const int n0 = 16 * (w4 ? kCols : 1) * (blockIdx.x - j.tile0);
   const int n = min(n0 + (lane & 15), j.N - 1), k0 = 8 * (lane >> 4);
   const int steps = j.K / 32;
-  f32x4 acc[MT];
+  f32x4 acc[MT][kCols];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const bool w4 = kW4 && j.scales;
-  if (w4) w4_steps<MT>(j, blockIdx.x - j.tile0, wave, a.rows, acc);
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[m][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (w4) w4_steps<MT, kCols>(j, blockIdx.x - j.tile0, wave, a.rows, acc);
   for (int s0 = w4 ? steps : wave; s0 < steps; s0 += kGemmWaves * kDepth) {
     bf16x8 w[kDepth], x[kDepth][MT];
 #pragma unroll
@@ -257,17 +267,21 @@ __global__ __launch_bounds__(64 * kGemmWaves) void rows_gemm_kernel(const GemmAr
     for (int d = 0; d < kDepth; ++d)
       if (s0 + d * kGemmWaves < steps) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[d][m], w[d], acc[m], 0, 0, 0);
+        for (int m = 0; m < MT; ++m) acc[m][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[d][m], w[d], acc[m][0], 0, 0, 0);
       }
   }
 #pragma unroll
-  for (int m = 0; m < MT; ++m) *reinterpret_cast<f32x4*>(&part[wave][m * 256 + 4 * lane]) = acc[m];
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+      if (c == 0 || w4) *reinterpret_cast<f32x4*>(&part[wave][(c * MT + m) * 256 + 4 * lane]) = acc[m][c];
   __syncthreads();
-  for (int i = threadIdx.x; i < MT * 256; i += 64 * kGemmWaves) {
+  for (int i = threadIdx.x; i < MT * 256 * (w4 ? kCols : 1); i += 64 * kGemmWaves) {
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < kGemmWaves; ++w) v += part[w][i];
-    const int l = (i >> 2) & 63, row = 16 * (i >> 8) + 4 * (l >> 4) + (i & 3), col = n0 + (l & 15);
+    const int l = (i >> 2) & 63, row = 16 * (i / 256 % MT) + 4 * (l >> 4) + (i & 3);
+    const int col = n0 + 16 * (i / (256 * MT)) + (l & 15);
     if (row >= a.rows || col >= j.N) continue;
     const int64_t at = (int64_t)row * j.N + col;
     if (w4) v *= rwkv_w4::kShrink;
@@ -362,23 +376,32 @@ __global__ __launch_bounds__(1024) void lora_prepare_kernel(const PrepareArgs a)
   }
 }
 
-template <bool kW4>
-hipError_t gemm(const GemmArgs& a, int tiles, hipStream_t s) {
+template <int NT>
+hipError_t gemm(GemmArgs& a, hipStream_t s) {
+  int tiles = 0;
+  for (int i = 0; i < a.jobs; ++i) {
+    const int cols = a.job[i].scales ? 16 * NT : 16;
+    a.job[i].tile0 = tiles;
+    tiles += (a.job[i].N + cols - 1) / cols;
+  }
   const dim3 grid(tiles), block(64 * kGemmWaves);
-  if (a.rows <= 16) hipLaunchKernelGGL((rows_gemm_kernel<1, kW4>), grid, block, 0, s, a);
-  else if (a.rows <= 32) hipLaunchKernelGGL((rows_gemm_kernel<2, kW4>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((rows_gemm_kernel<4, kW4>), grid, block, 0, s, a);
+  if (a.rows <= 16) hipLaunchKernelGGL((rows_gemm_kernel<1, NT>), grid, block, 0, s, a);
+  else if (a.rows <= 32) hipLaunchKernelGGL((rows_gemm_kernel<2, NT>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((rows_gemm_kernel<4, NT < 2 ? NT : 2>), grid, block, 0, s, a);
   return hipGetLastError();
 }
 hipError_t gemm(GemmArgs& a, hipStream_t s) {
-  int tiles = 0;
-  bool w4 = false;
-  for (int i = 0; i < a.jobs; ++i) {
-    a.job[i].tile0 = tiles;
-    tiles += (a.job[i].N + 15) / 16;
-    w4 |= a.job[i].scales != nullptr;
-  }
-  return w4 ? gemm<true>(a, tiles, s) : gemm<false>(a, tiles, s);
+  int64_t w4 = 0;   // tiles of 16 columns
+  for (int i = 0; i < a.jobs; ++i)
+    if (a.job[i].scales) w4 += (a.job[i].N + 15) / 16;
+  if (w4 == 0) return gemm<0>(a, s);
+  // What more columns a workgroup save is reading the rows again; fewer keep more
+  // workgroups. us a step at C = 4096, 3 cells, 1 / 8 / 64 sequences, one tile
+  // everywhere 324, 366, 1189, so 297, 317, 771 (the head on few_kernel or
+  // tile_kernel of w4.hip included).
+  const bool wide = a.rows > 32;   // two column tiles at most: 64 KB of sums
+  if (w4 >= 1024 && !wide) return gemm<4>(a, s);
+  return w4 >= 512 ? gemm<2>(a, s) : gemm<1>(a, s);
 }
 
 template <bool kFirst>
@@ -552,6 +575,19 @@ hipError_t launch_head(const HeadCall& c, hipStream_t stream) {
   n.C = C;
   n.out[0] = static_cast<bf16_t*>(c.workspace);
   if (hipError_t e = norm_mix<0>(n, stream)) return e;
+  if (c.unembed_w4 && rwkv_w4::workspace_bytes(c.rows, c.vocab, C, true) == 0) {
+    rwkv_w4::LinearCall y{};
+    y.x = n.out[0];
+    y.packed = c.unembed_w4->packed;
+    y.scales = c.unembed_w4->scales;
+    y.y = c.logits;
+    y.rows = c.rows;
+    y.out = c.vocab;
+    y.in = C;
+    y.group = c.group;
+    y.bf16 = true;
+    return rwkv_w4::launch_linear(y, stream);
+  }
   GemmArgs g{};
   g.rows = c.rows;
   g.jobs = 1;

@@ -34,6 +34,9 @@ MAX_ROWS = 64        # RWKV_DECODE_MAX_ROWS
 # 1124 at C = 4096 and 64 sequences against 1252, elsewhere up to 4096 they are
 # slower; with a context a step, 2157 and more at C = 4096.)
 MAX_DIM = 4096
+# 4-bit weights are an eighth of that. C = 8192, 2 cells, 1 / 8 / 32 / 64 sequences:
+# through the modules 1322, 1332, 1406, 1436, here 418, 433, 695, 1289.
+MAX_DIM_W4 = 8192    # RWKV_DECODE_MAX_DIM
 
 
 def _plain(module, cls) -> bool:
@@ -75,15 +78,16 @@ class _Reader:
             raise _Unsupported
         return self.param(module, "weight", (d_out, d_in))
 
-    def packed(self, module, d_in, d_out):
-        """(packed, scales, group size) of a linear layer with a 4-bit weight."""
-        if (not _plain(module, w4.W4Linear) or module.in_features != d_in
-                or module.out_features != d_out or module.group_size not in w4.GROUPS):
+    def packed(self, module, d_in, d_out, group):
+        """(packed, scales) of a linear layer with a 4-bit weight."""
+        if not _plain(module, w4.W4Linear):
             raise _Unsupported
-        blocks, b = (-(-d_out // 16), -(-d_in // 128)), module._buffers
-        return (self.tensor(b["packed"], (*blocks, 4, 16, 16), torch.uint8),
-                self.tensor(b["scales"], (*blocks, 16, 128 // module.group_size), torch.bfloat16),
-                module.group_size)
+        d = module.__dict__
+        if d["in_features"] != d_in or d["out_features"] != d_out or d["group_size"] != group:
+            raise _Unsupported
+        n, k, b = -(-d_out // 16), -(-d_in // 128), d["_buffers"]
+        return (self.tensor(b["packed"], (n, k, 4, 16, 16), torch.uint8),
+                self.tensor(b["scales"], (n, k, 16, 128 // group), torch.bfloat16))
 
     def norm(self, module, dim):
         if (not _plain(module, nn.LayerNorm) or module.normalized_shape != (dim,)
@@ -106,14 +110,9 @@ def _matrices(p, wp, gr, cm, rd: _Reader, C: int):
         for name, module, d_in, d_out in of:
             setattr(p, name, rd.linear(module, d_in, d_out))
         return None
-    q = _native.DecodeW4Weights()
-    for name, module, d_in, d_out in of:
-        packed, scales, group = rd.packed(module, d_in, d_out)
-        if q.group not in (0, group):
-            raise _Unsupported
-        q.group = group
-        setattr(q, name, _native.W4Matrix(packed, scales))
-    return q
+    group = of[0][1].group_size
+    return _native.DecodeW4Weights(*(rd.packed(module, d_in, d_out, group)
+                                     for _, module, d_in, d_out in of), group)
 
 
 def _cell_params(m, cell, rd: _Reader, C: int, H: int):
@@ -211,7 +210,7 @@ def step(model, contexts, batch_ids, infer_state, context_mask,
     cells = list(stack._modules["cells"])
     slots, H = infer_state.state[0].shape[:2]
     C = 64 * H
-    if (not 0 < C <= MAX_DIM or batch_ids.shape != (rows,) or infer_state.elapsed_t.shape != (slots,)
+    if (not 0 < C <= MAX_DIM_W4 or batch_ids.shape != (rows,) or infer_state.elapsed_t.shape != (slots,)
             or not len(infer_state.state) == len(infer_state.shift_time)
             == len(infer_state.shift_channel) == len(cells)):
         return None
@@ -224,14 +223,19 @@ def step(model, contexts, batch_ids, infer_state, context_mask,
                   rd.tensor(t, (slots, C)), rd.tensor(ch, (slots, C)))
                  for c, s, t, ch in zip(cells, infer_state.state, infer_state.shift_time,
                                         infer_state.shift_channel)]
+        if C > MAX_DIM and not all(c[0][1] for c in calls):
+            return None
         if calls[0][0][0].residual_a or not all(c[0][0].residual_a for c in calls[1:]):
             return None   # the first cell is the one without a value residual
         head = None
         if unembed_mode != "skip":
             unembed = model._modules["unembed"]
-            read = rd.packed if type(unembed) is w4.W4Linear else rd.linear
-            head = (rd.norm(model._modules["layer_norm_for_unembed"], C),
-                    read(unembed, C, model.vocab_size))
+            norm = rd.norm(model._modules["layer_norm_for_unembed"], C)
+            if type(unembed) is w4.W4Linear:
+                head_group = unembed.group_size
+                head = norm, rd.packed(unembed, C, model.vocab_size, head_group)
+            else:
+                head = norm, rd.linear(unembed, C, model.vocab_size)
     except LookupError:
         return None
     ids = batch_ids.to(device=dev, dtype=torch.int32).contiguous()
@@ -267,10 +271,9 @@ def step(model, contexts, batch_ids, infer_state, context_mask,
     logits = torch.empty((rows, 1, model.vocab_size), dtype=torch.bfloat16, device=dev)
     rest = (rows, H, model.vocab_size, logits.data_ptr(), ws.data_ptr(), nbytes, stream)
     if isinstance(unembed, tuple):
-        packed, scales, group = unembed
-        matrix = _native.W4Matrix(packed, scales)
+        matrix = _native.W4Matrix(*unembed)
         _native.check(lib.rwkv_decode_head_w4(x.data_ptr(), weight, bias, eps,
-                                              ctypes.addressof(matrix), group, *rest))
+                                              ctypes.addressof(matrix), head_group, *rest))
     else:
         _native.check(lib.rwkv_decode_head(x.data_ptr(), weight, bias, eps, unembed, *rest))
     return (logits,)
