@@ -7,14 +7,23 @@
 // Forward: a workgroup loads a row (or a chunk of a long one) into registers
 // once, eight logits a piece, all loads in flight together, and everything else
 // works on those: the maximum, the sums, and the alternatives. These are found
-// through a bound: each of 64 groups of pieces has a largest logit, and the k-th
-// largest of those is no larger than the k-th largest logit, so what reaches it
-// (a few more than k logits, where large ones do not crowd into few groups) goes
-// to a list in LDS, whose items are then ranked against each other. A list that
-// overflows is replaced by k rounds of taking the largest that is left.
+// through a bound: each of 64 groups of pieces (128 for more than 32 alternatives)
+// has a largest logit, and the k-th largest of those is no larger than the k-th
+// largest logit, so what reaches it goes to a list in LDS, whose items are then
+// ranked against each other. Where large logits do not crowd into few groups that
+// is a few more than k (of 64 groups for k = 20 about 24, for 32 44; of 128 for 64
+// 89; of 64 they would be some 300). A list that overflows is replaced by k rounds
+// of taking the largest that is left.
+//
+// us and what bounds it: 4096 x 65536 bf16 without alternatives 92 (5.8 TB/s, HBM),
+// with 20 117, with 64 142 (vector instructions, some 13 for a logit, and the
+// waits between the steps of the selection); with one of eight rows masked 119
+// and 142. 1024 x 65536 fp32 with 20 47 (5.7 TB/s). Backward of 4096 x 65536 bf16
+// 214 (5.0 TB/s, HBM).
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "token_scores_launch.hpp"
 
@@ -22,7 +31,7 @@ namespace rwkv_scores {
 namespace {
 
 constexpr int kPiece = 8;    // logits of a load (bf16: 16 bytes) or of two (fp32)
-constexpr int kGroups = 64;  // also the most alternatives
+constexpr int kTopStep = 32;  // alternatives: up to two steps of these, for each of which there are 64 groups
 constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // 2^kFloor is 0: what lies below adds nothing, and 0 times it is 0
 constexpr float kFloor = -256.f;
@@ -35,6 +44,14 @@ struct __attribute__((packed, aligned(2))) Raw16 {
 struct __attribute__((packed, aligned(4))) Raw32 {
   float v[8];
 };
+// The largest of three; fmaxf would have each operand's NaN made quiet first, an
+// instruction for each logit.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 template <bool BF>
 struct Piece;   // as loaded
 template <>
@@ -46,7 +63,7 @@ struct alignas(16) Piece<true> {
   }
   __device__ __forceinline__ float largest() const {
     const Piece& p = *this;
-    return fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+    return max3(max3(p[0], p[1], p[2]), max3(p[3], p[4], p[5]), max3(p[6], p[7], p[7]));
   }
   __device__ __forceinline__ void clear() { raw = Raw16{{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}}; }
   // The values are taken out of the words again from here on, so that a pass
@@ -62,7 +79,7 @@ struct alignas(16) Piece<false> {
   __device__ __forceinline__ float operator[](int e) const { return raw.v[e]; }
   __device__ __forceinline__ float largest() const {
     const Piece& p = *this;
-    return fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+    return max3(max3(p[0], p[1], p[2]), max3(p[3], p[4], p[5]), max3(p[6], p[7], p[7]));
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -94,7 +111,7 @@ __device__ __forceinline__ Piece<BF> load_piece(const char* chunk, uint32_t q) {
 
 // A logit with its index (or a piece's largest with the piece's number) as one
 // number: of two, the larger logit is larger, then the lower index. Zeros of
-// both signs are equal. No key is below kGroups.
+// both signs are equal. No key is 0.
 typedef unsigned long long Key;
 __device__ __forceinline__ Key key_of(float x, int j) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
@@ -136,12 +153,6 @@ __device__ __forceinline__ Key largest_of(Key k) {
   if constexpr (kLanes > 8) k = larger(k, swapped<8>(k));
   return k;
 }
-__device__ __forceinline__ Key wave_largest(Key k) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) k = larger(k, __shfl_xor(k, o));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(k >> 32));
-  return static_cast<Key>(hi) << 32 | static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(k)));
-}
 // Of all lanes, in every lane: the row's shifts, then its last lane to the rows
 // behind; lane 63 has it all.
 template <int kCtrl, int kRowMask>
@@ -167,55 +178,72 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 // Pieces and candidates that the lists hold; a chunk that has more goes the
-// other way.
-constexpr int max_pieces(int waves) { return waves == 1 ? 64 : waves <= 4 ? 128 : 256; }
-constexpr int max_listed(int waves) { return waves == 1 ? 512 : 4 * max_pieces(waves); }
-constexpr int kRanked = 128;   // more than these are cut to the most before they are ranked
-template <bool BF, int kWaves>
+// other way. A row that a mask leaves fewer than k tokens has up to k pieces of
+// minus infinity in them.
+template <bool BF, int kWaves, int kTop>
 struct Shared {
-  Piece<BF> piece[max_pieces(kWaves)];
-  int piece_at[max_pieces(kWaves)];
-  Key key[kWaves][kGroups + 1];
+  static constexpr int kGroups = 64 * kTop, kMost = kTopStep * kTop;
+  static constexpr int kPieces = 128 * kTop, kListed = 512 * kTop;
+  Piece<BF> piece[kPieces];
+  int piece_at[kPieces];
+  Key key[kWaves][65];
   Key group[kGroups];
-  Key list[max_listed(kWaves)];
-  Key best[2][kGroups];        // the alternatives so far, in order
+  Key list[kListed];
+  Key best[2][kMost];        // the alternatives so far, in order
   Key bound;
-  float max, part_max[kWaves], part_s[kWaves], part_u[kWaves];
+  float max;
   int pieces, listed;
 };
+constexpr int kRanked = 128;   // more than these are cut to the most before they are ranked
 
-// The largest of every thread's keys (`mine`; lane l of every wave belongs to
-// group l) and the k-th largest of the groups' largest, into sh.max and
-// sh.bound. Every group's largest is another item, so the bound is one of the 64.
-template <bool BF, int kWaves>
-__device__ __forceinline__ void find_bound(Shared<BF, kWaves>& sh, Key mine, int k) {
-  const int tid = threadIdx.x, group = tid / kWaves, sub = tid % kWaves;
+// The largest of every thread's keys (`mine`; a group is a lane of kWaves / kTop
+// waves) and the k-th largest of the groups' largest, into sh.max and sh.bound.
+// Every group's largest is another item, so the bound is one of them. Where it is
+// minus infinity (a mask has left fewer than k groups anything), the whole pieces
+// of it count as the eight logits that they are: few of them are needed.
+template <bool BF, int kWaves, int kTop>
+__device__ __forceinline__ void find_bound(Shared<BF, kWaves, kTop>& sh, Key mine, int k, int Q) {
+  static_assert(kWaves % kTop == 0 && kTop <= 2, "a thread's key is in one group");
+  constexpr int kShare = kWaves / kTop, kCompared = 64 * kTop / kShare;
+  const int tid = threadIdx.x, group = tid / kShare, sub = tid % kShare;
   Key key = mine;
-  if constexpr (kWaves > 1) {
+  if constexpr (kShare > 1) {
     sh.key[tid >> 6][tid & 63] = mine;
     __syncthreads();
-    key = largest_of<kWaves>(sh.key[sub][group]);
+    key = largest_of<kShare>(sh.key[group / 64 * kShare + sub][group & 63]);
   }
   if (sub == 0) sh.group[group] = key;
   __syncthreads();
   int rank = 0;
-#pragma unroll
-  for (int i = 0; i < kGroups / kWaves; ++i) rank += sh.group[sub * (kGroups / kWaves) + i] > key;
-  rank = sum_of<kWaves>(rank);
+#pragma unroll 16
+  for (int i = 0; i < kCompared; ++i) rank += sh.group[sub * kCompared + i] > key;
+  rank = sum_of<kShare>(rank);
   if (sub == 0) {
     if (rank == 0) sh.max = key_x(key);
     if (rank == k - 1) sh.bound = key;
   }
   if (tid == 0) sh.pieces = sh.listed = 0;
   __syncthreads();
+  constexpr Key kSome = Key{0x00800000u} << 32;   // the least key of more than minus infinity
+  const Key bound = sh.bound;
+  if (bound >= kSome) return;
+  int some = 0;
+#pragma unroll 16
+  for (int i = 0; i < kCompared; ++i) some += sh.group[sub * kCompared + i] >= kSome;
+  some = sum_of<kShare>(some);
+  __syncthreads();   // every thread has the bound that is replaced
+  if (sub == 0 && rank == some + (k - some + kPiece - 1) / kPiece - 1 && key_j(key) < Q) sh.bound = key;
+  __syncthreads();
 }
 
 // The list's n keys, more than k of them, cut to their k largest by the first
-// wave: a number that k keys reach, by bisection (they are all different, so there
-// is one). Ranking n keys against each other is n^2 / 2 comparisons; this is n for
-// a step, of which there are some twenty.
-template <bool BF, int kWaves>
-__device__ __forceinline__ void cut_list(Shared<BF, kWaves>& sh, int n, int k) {
+// wave: a key that k keys reach (they are all different, so there is one) is
+// looked for among those that still can be it. Ranking n keys against each other
+// is n^2 comparisons, this n for each of the about 2 ln n keys tried. (By halving
+// the distance between the numbers, 54 steps where minus infinities differ in
+// their index alone, a masked row took 9 us.)
+template <bool BF, int kWaves, int kTop>
+__device__ __forceinline__ void cut_list(Shared<BF, kWaves, kTop>& sh, int n, int k) {
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
     auto each = [&](auto f) {   // of four keys a lane at a time, 0 for none
@@ -228,26 +256,29 @@ __device__ __forceinline__ void cut_list(Shared<BF, kWaves>& sh, int n, int k) {
         for (int i = 0; i < 4; ++i) f(v[i]);
       }
     };
-    Key low = ~Key{0}, high = 0;
-    each([&](Key v) {
-      if (v != 0 && v < low) low = v;
-      high = larger(high, v);
-    });
-    low = ~wave_largest(~low);
-    high = wave_largest(high) + 1;
-    Key mid;
-    while (true) {   // n keys reach low and none reaches high: what is between halves every time
-      mid = low + (high - low) / 2;
+    Key low = 0, high = ~Key{0}, tried = sh.list[n / 2];
+    while (true) {
       int count = 0;
-      each([&](Key v) { count += __popcll(__ballot(v >= mid)); });
-      if (count == k || mid == low) break;
-      (count > k ? low : high) = mid;
+      Key above = 0, below = 0;   // one of the lane's that can be it, on either side
+      each([&](Key v) {
+        count += __popcll(__ballot(v >= tried));
+        if (v > tried && v < high) above = v;
+        if (v < tried && v > low) below = v;
+      });
+      if (count == k) break;
+      (count > k ? low : high) = tried;
+      const Key next = count > k ? above : below;
+      const unsigned long long have = __ballot(next != 0);
+      if (have == 0) break;
+      const int from = __ffsll(have) - 1;
+      tried = static_cast<Key>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(next >> 32), from))) << 32 |
+              static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(next), from));
     }
     int to = 0;   // a key's place is never behind its own
     each([&](Key v) {
-      const unsigned long long hit = __ballot(v >= mid);
+      const unsigned long long hit = __ballot(v >= tried);
       const int place = to + __popcll(hit & ((1ull << lane) - 1));
-      if (v >= mid && place < k) sh.list[place] = v;
+      if (v >= tried && place < k) sh.list[place] = v;
       to += __popcll(hit);
     });
   }
@@ -271,8 +302,8 @@ __device__ __forceinline__ int count_above(const Key* keys, int n, Key mine) {
 
 // Ranks the list's n keys together with the `held` best so far, and gives those
 // before the k-th to keep(rank, key). Sixteen lanes count for a key.
-template <bool BF, int kWaves, typename F>
-__device__ __forceinline__ void rank_keys(const Shared<BF, kWaves>& sh, int n, const Key* best, int held, int k, F&& keep) {
+template <bool BF, int kWaves, int kTop, typename F>
+__device__ __forceinline__ void rank_keys(const Shared<BF, kWaves, kTop>& sh, int n, const Key* best, int held, int k, F&& keep) {
   const int sub = threadIdx.x & 15;
 #pragma nounroll
   for (int i = threadIdx.x >> 4; i < n + held; i += kWaves * 4) {
@@ -285,8 +316,8 @@ __device__ __forceinline__ void rank_keys(const Shared<BF, kWaves>& sh, int n, c
 
 // The list by another way: sh.list becomes the k largest of what next(last)
 // gives, each thread's largest key below `last`. Ends with a barrier.
-template <bool BF, int kWaves, typename F>
-__device__ __forceinline__ void take_largest(Shared<BF, kWaves>& sh, int k, F&& next) {
+template <bool BF, int kWaves, int kTop, typename F>
+__device__ __forceinline__ void take_largest(Shared<BF, kWaves, kTop>& sh, int k, F&& next) {
   Key last = ~Key{0};
   __syncthreads();
 #pragma nounroll
@@ -350,14 +381,18 @@ __device__ __forceinline__ void write_top(const ForwardCall& c, int64_t row, int
   c.top_ids[row * c.top + rank] = t.valid() ? key_j(v) : -1;
 }
 
-// The largest key below `last` of a thread's share of the row, which is read again.
-template <bool BF>
-__device__ __forceinline__ Key next_of(const void* row, int64_t begin, int64_t end, int stride, Key last) {
+// The largest key below `last` of a thread's pieces of a chunk, which are read again.
+template <bool BF, int kThreads>
+__device__ __forceinline__ Key next_of(const void* row, int q0, int pieces, Key last) {
   Key v = 0;
-#pragma nounroll
-  for (int64_t j = begin + threadIdx.x; j < end; j += stride) {
-    const Key y = key_of(load_one<BF>(row, j), static_cast<int>(j));
-    if (y < last) v = larger(v, y);
+#pragma unroll 2
+  for (int q = threadIdx.x; q < pieces; q += kThreads) {
+    const Piece<BF> p = load_piece<BF>(at<BF>(row, static_cast<int64_t>(q0) * kPiece), q);
+#pragma unroll
+    for (int e = 0; e < kPiece; ++e) {
+      const Key y = key_of(p[e], (q0 + q) * kPiece + e);
+      if (y < last) v = larger(v, y);
+    }
   }
   return v;
 }
@@ -365,10 +400,13 @@ __device__ __forceinline__ Key next_of(const void* row, int64_t begin, int64_t e
 // The row is Q pieces and, after them, up to seven single logits, one to a
 // thread, which are numbered like pieces (Q, Q + 1, ..). A chunk is kPieces of
 // them a thread.
-template <bool BF, int kWaves, int kPieces, bool kTop>
+// kTop: steps of alternatives, 0 for none.
+template <bool BF, int kWaves, int kPieces, int kTop>
 __global__ __launch_bounds__(kWaves * 64, 4) void forward_kernel(const ForwardCall c) {
   constexpr int kThreads = kWaves * 64, kChunk = kThreads * kPieces;
-  __shared__ Shared<BF, kWaves> sh;
+  typedef Shared<BF, kWaves, kTop> Lists;
+  __shared__ std::conditional_t<kTop != 0, Lists, int> sh;
+  __shared__ float part_max[kWaves], part_s[kWaves], part_u[kWaves];
   const int64_t row = blockIdx.x, V = c.vocab;
   const void* const x = at<BF>(c.logits, row * V);
   const int tid = threadIdx.x, wave = tid >> 6, k = c.top;
@@ -409,36 +447,31 @@ __global__ __launch_bounds__(kWaves * 64, 4) void forward_kernel(const ForwardCa
     }
     float chunk_max, bound_x = 0.f;
     int bound_q = 0;
-    if constexpr (kTop) {
-      find_bound(sh, key_of(most, most_at), k);
+    if constexpr (kTop != 0) {
+      find_bound(sh, key_of(most, most_at), k, Q);
       chunk_max = sh.max;
       bound_x = key_x(sh.bound);
       bound_q = key_j(sh.bound);
-      uint32_t reached = 0;   // the pieces that may hold an alternative
+      // the pieces that may hold an alternative; few of a wave's do
 #pragma unroll
       for (int i = 0; i < kPieces; ++i)
-        if ((piece_max[i] > bound_x || (piece_max[i] == bound_x && q0 + i * kThreads + lane <= bound_q)) &&
-            i * kThreads + lane < left)
-          reached |= 1u << i;
-      if (reached) {
-        int n = atomicAdd(&sh.pieces, __popc(reached));
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i)
-          if (reached >> i & 1) {
-            if (n < max_pieces(kWaves)) {
+        if (piece_max[i] >= bound_x) {
+          const int q = q0 + i * kThreads + lane;
+          if ((piece_max[i] > bound_x || q <= bound_q) && i * kThreads + lane < left) {
+            const int n = atomicAdd(&sh.pieces, 1);
+            if (n < Lists::kPieces) {
               sh.piece[n] = p[i];
-              sh.piece_at[n] = q0 + i * kThreads + lane;
+              sh.piece_at[n] = q;
             }
-            ++n;
           }
-      }
+        }
     } else {
       const float v = wave_max(most);
-      if ((tid & 63) == 0) sh.part_max[wave] = v;
+      if ((tid & 63) == 0) part_max[wave] = v;
       __syncthreads();
-      chunk_max = sh.part_max[0];
+      chunk_max = part_max[0];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) chunk_max = fmaxf(chunk_max, sh.part_max[w]);
+      for (int w = 1; w < kWaves; ++w) chunk_max = fmaxf(chunk_max, part_max[w]);
     }
     const Origin before = o;
     o = origin(fmaxf(o.m, chunk_max));
@@ -464,13 +497,13 @@ __global__ __launch_bounds__(kWaves * 64, 4) void forward_kernel(const ForwardCa
       const float base = o.m == -INFINITY ? 0.f : o.m;   // nothing but minus infinity so far: the terms are 0
       add_all([&](float v) { return (v - base) * kLog2E; });
     }
-    if constexpr (kTop) {
+    if constexpr (kTop != 0) {
       __syncthreads();
-      const int pieces = min(sh.pieces, max_pieces(kWaves));
+      const int pieces = min(sh.pieces, Lists::kPieces);
       auto list = [&](float v, int q, int j) {
         if (v > bound_x || (v == bound_x && q <= bound_q)) {
           const int n = atomicAdd(&sh.listed, 1);
-          if (n < max_listed(kWaves)) sh.list[n] = key_of(v, j);
+          if (n < Lists::kListed) sh.list[n] = key_of(v, j);
         }
       };
 #pragma nounroll
@@ -481,10 +514,13 @@ __global__ __launch_bounds__(kWaves * 64, 4) void forward_kernel(const ForwardCa
       if (has_single) list(single, Q + lane, Q * kPiece + lane);
       __syncthreads();
       int n = sh.listed;
-      if (n > max_listed(kWaves) || sh.pieces > max_pieces(kWaves)) {
-        const int64_t begin = static_cast<int64_t>(q0) * kPiece, end = final ? V : begin + kChunk * kPiece;
-        n = static_cast<int>(min(static_cast<int64_t>(k), end - begin));
-        take_largest(sh, n, [&](Key last) { return next_of<BF>(x, begin, end, kThreads, last); });
+      if (n > Lists::kListed || sh.pieces > Lists::kPieces) {
+        const int singles = final ? rest : 0;
+        n = static_cast<int>(min(static_cast<int64_t>(k), static_cast<int64_t>(left) * kPiece + singles));
+        take_largest(sh, n, [&](Key last) {
+          const Key v = next_of<BF, kThreads>(x, q0, left, last), y = key_of(single, Q * kPiece + tid);
+          return has_single && y < last ? larger(v, y) : v;
+        });
       }
       if (n > kRanked) {
         cut_list(sh, n, k);
@@ -500,19 +536,19 @@ __global__ __launch_bounds__(kWaves * 64, 4) void forward_kernel(const ForwardCa
   s = wave_sum(s);
   u = wave_sum(u);
   if ((tid & 63) == 0) {
-    sh.part_s[wave] = s;
-    sh.part_u[wave] = u;
+    part_s[wave] = s;
+    part_u[wave] = u;
   }
   __syncthreads();
   Sums t{o, 0.f, 0.f};
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    t.s += sh.part_s[w];
-    t.u += sh.part_u[w];
+    t.s += part_s[w];
+    t.u += part_u[w];
   }
   const float log_sum = t.log_sum();
   if (tid == 0) write_row<BF>(c, row, t, log_sum);
-  if constexpr (kTop)
+  if constexpr (kTop != 0)
     if (tid < k) write_top(c, row, tid, sh.best[now][tid], t, log_sum);
 }
 
@@ -542,6 +578,9 @@ __device__ __forceinline__ void store_piece(void* row, int64_t q, const float (&
   }
 }
 
+// The last rows first: the forward has read them last, and what of them is still
+// in the cache need not come from memory (us, forward and backward, 8192 x 65536
+// bf16 611 / 596, 1024 x 65536 fp32 173 / 168).
 // Blocks (row, y) take `share` pieces of a row each, the last one its single
 // logits too. The elements with a term of their own are written again, whole, by
 // the block that holds them.
@@ -549,7 +588,7 @@ constexpr int kThreads = 256;
 
 template <bool BF>
 __global__ __launch_bounds__(kThreads) void backward_kernel(const BackwardCall c, const int64_t share) {
-  const int64_t row = blockIdx.x, V = c.vocab, Q = V / kPiece;
+  const int64_t row = c.rows - 1 - blockIdx.x, V = c.vocab, Q = V / kPiece;
   const int64_t begin = blockIdx.y * share, end = min(begin + share, Q);
   const void* const x = at<BF>(c.logits, row * V);
   void* const dx = const_cast<char*>(at<BF>(c.logits_grad, row * V));
@@ -579,36 +618,52 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(const BackwardCall c
   if (!__any(j == t) && lane == 0 && t >= from && t < to) store_one<BF>(dx, t, r.of(load_one<BF>(x, t)) + g);
 }
 
-template <bool BF, int kWaves, int kPieces>
+template <bool BF, int kTop, int kWaves, int kPieces>
 void forward(const ForwardCall& c, hipStream_t s) {
-  auto* const kernel = c.top > 0 ? forward_kernel<BF, kWaves, kPieces, true> : forward_kernel<BF, kWaves, kPieces, false>;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(c.rows)), dim3(kWaves * 64), 0, s, c);
+  hipLaunchKernelGGL((forward_kernel<BF, kWaves, kPieces, kTop>), dim3(static_cast<unsigned>(c.rows)), dim3(kWaves * 64),
+                     0, s, c);
 }
 
 // The smallest workgroup whose registers hold a row, up to 128 of a thread's: what
 // the selection costs does not grow with the pieces a thread holds. us, bf16, 20
-// alternatives (waves, pieces a thread): 8192 x 4096 (2, 4) 26.5, (4, 2) 30.8, (1,
-// 8) 27.6; 8192 x 8192 (4, 4) 39.2, (2, 8) 40.3, (4, 8) 45.2; 2048 x 32768 (4, 16)
-// 33.8, (8, 8) 36.4, (8, 16) 42; 4096 x 65536 (8, 16) 132, (8, 8) in two chunks 147,
-// (4, 16) 137, (16, 8) 171. fp32 pieces are twice the registers: 1024 x 65536 (8, 8)
-// 48, (16, 8) 58; with a workgroup a compute unit or fewer the row's own time
-// counts, 256 x 65529 (16, 8) 17.5, (8, 8) 20.6.
-template <bool BF>
+// alternatives (waves, pieces a thread): 8192 x 4096 (2, 4) 25, (4, 2) 31, (1, 8)
+// 28; 8192 x 8192 (4, 4) 37, (2, 8) 40, (4, 8) 45; 2048 x 32768 (4, 16) 30, (8, 8)
+// 36, (8, 16) 42. Longer bf16 rows: 4096 x 65536 (4, 16), two chunks in smaller
+// workgroups that wait for each other less, 117, (8, 16) 121, (8, 8) 147, (16, 8)
+// 171; with 64 alternatives, whose second list is longer, (4, 16) 160, (8, 16) 142;
+// without any there is little to wait for, (4, 16) 95.9, (8, 16) 91.8, and with few
+// rows the row's own time counts, 8 x 65536 (8, 16) 9.3, (4, 16) 15. fp32 pieces
+// are twice the registers: 1024 x 65536 (8, 8) 47, (16, 8) 58; 256 x 65529 (16, 8)
+// 17.4, (8, 8) 20.6.
+constexpr int64_t kManyRows = 512, kOwnTimeRows = 256;
+template <bool BF, int kTop>
 hipError_t forward(const ForwardCall& c, hipStream_t s) {
-  if (c.vocab <= 64 * 1 * kPiece) forward<BF, 1, 1>(c, s);
-  else if (c.vocab <= 64 * 2 * kPiece) forward<BF, 1, 2>(c, s);
-  else if (c.vocab <= 64 * 4 * kPiece) forward<BF, 1, 4>(c, s);
-  else if (c.vocab <= 128 * 4 * kPiece) forward<BF, 2, 4>(c, s);
-  else if (c.vocab <= 256 * 4 * kPiece) forward<BF, 4, 4>(c, s);
-  else if (c.vocab <= 256 * 8 * kPiece) forward<BF, 4, 8>(c, s);
-  else if constexpr (BF) {
-    if (c.vocab <= 256 * 16 * kPiece) forward<BF, 4, 16>(c, s);
-    else forward<BF, 8, 16>(c, s);
+  auto holds = [&](int waves, int pieces) { return c.vocab <= waves * 64 * pieces * kPiece; };
+  if constexpr (kTop <= 1) {   // a wave is 64 groups
+    if (holds(1, 1)) forward<BF, kTop, 1, 1>(c, s);
+    else if (holds(1, 2)) forward<BF, kTop, 1, 2>(c, s);
+    else if (holds(1, 4)) forward<BF, kTop, 1, 4>(c, s);
   } else {
-    if (c.rows <= 256) forward<BF, 16, 8>(c, s);
-    else forward<BF, 8, 8>(c, s);
+    if (holds(2, 1)) forward<BF, kTop, 2, 1>(c, s);
+  }
+  if (holds(kTop <= 1 ? 1 : 2, kTop <= 1 ? 4 : 1)) return hipGetLastError();
+  if (holds(2, 4)) forward<BF, kTop, 2, 4>(c, s);
+  else if (holds(4, 4)) forward<BF, kTop, 4, 4>(c, s);
+  else if (holds(4, 8)) forward<BF, kTop, 4, 8>(c, s);
+  else if constexpr (BF) {
+    if (holds(4, 16) || (kTop == 1 && c.rows > kManyRows)) forward<BF, kTop, 4, 16>(c, s);
+    else forward<BF, kTop, 8, 16>(c, s);
+  } else {
+    if (c.rows <= kOwnTimeRows) forward<BF, kTop, 16, 8>(c, s);
+    else forward<BF, kTop, 8, 8>(c, s);
   }
   return hipGetLastError();
+}
+
+template <bool BF>
+hipError_t forward(const ForwardCall& c, hipStream_t s) {
+  if (c.top == 0) return forward<BF, 0>(c, s);
+  return c.top <= kTopStep ? forward<BF, 1>(c, s) : forward<BF, 2>(c, s);
 }
 
 }  // namespace

@@ -4,7 +4,15 @@
 // linear: y[m, n] = sum over groups G of s[n, G] * sum over k in G of x[m, k] v[n, k].
 // The values v are small bf16 numbers, so the inner sums are matrix
 // instructions on bf16 operands whose products are exact; a group's sum is
-// multiplied by its scale in fp32 and added to the total.
+// multiplied by its scale in fp32 and added to the total. (Weights times scale
+// rounded to bf16 would be one operation less for each four products and 2^-9
+// off each.) An fp32 activation is three bf16 parts that hold all of it.
+//
+// Up to about 64 rows the weights' bytes bound it: few_kernel, 1 x 4096 x 16384
+// (34 MB) 8.8 us, 8 x 4096 x 65536 28 us (4.8 TB/s, what a copy reaches). Many
+// rows are matrix products: tile_kernel, 512 x 2048 x 8192 26.7 us (644 TFLOP/s),
+// 2048 x 4096 x 4096 74 us (927), a library product of bf16 matrices of 8192^3
+// 1130.
 #include <algorithm>
 
 #include "w4_device.hpp"
@@ -79,7 +87,8 @@ __device__ __forceinline__ char* row_at(void* base, int64_t row, int64_t n, bool
 // ---------------------------------------------------------- quantise, restore
 // A wave takes a block of 16 outputs and 128 inputs, lane l the output l % 16
 // at the inputs 32 j + 8 (l / 16) .. + 7 of each j, which are its 16 bytes of
-// the packed block; four lanes hold 32 consecutive inputs of an output.
+// the packed block; four lanes hold 32 consecutive inputs of an output. HBM bounds
+// both: 65536 x 768 fp32 quantised and restored 93 us for 453 MB (4.9 TB/s).
 constexpr int kBlockWaves = 4;
 
 // Nearest magnitude, ties to the even mantissa: the midpoints times the scale
@@ -219,7 +228,12 @@ __device__ __forceinline__ void store_y(const LinearCall& c, int64_t row, int64_
 // Few rows. A workgroup forms 16 NT outputs of up to 16 MT rows; its waves split
 // the inputs in blocks of 128 (one 16-byte load of weights a lane and 16 outputs,
 // four matrix instructions a tile) and add up through LDS in wave order. A wave
-// has kDepth blocks' loads in flight.
+// has kDepth blocks' loads in flight: what the weights' stream needs is bytes in
+// flight on every compute unit, from many waves, or several tiles or blocks a wave.
+// us, 1 row, (NT, waves, depth): 4096 x 16384 one tile at a time 11.4, (1, 8, 4)
+// 12.8, (4, 8, 1) 11.1, (2, 16, 1) 8.9; 768 x 65536, 8 rows, (1, 8, 4) 17.0, (2,
+// 16, 1) 11.5, (4, 8, 2) 9.5; 4096 x 4096 (1, 8, 4) 5.2, (1, 16, 2) 4.7; 16384 x
+// 4096 one tile at a time 23.9, (1, 16, 2) 11.4, (2, 16, 1) 14.
 template <bool BF, Form kForm, int kGroup, int MT, int NT, int kWaves, int kDepth>
 __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) {
   __shared__ float part[kWaves][MT * NT * 256];
@@ -297,11 +311,13 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
 
 // Many rows. A workgroup forms 16 MT rows by 64 NT outputs of `share` blocks of
 // inputs, its four waves 16 NT outputs each; where the inputs are shared among
-// workgroups, join_kernel adds up what they leave. The rows' activations of 128 inputs go through LDS, one block
-// ahead, in the order in which the waves' matrix instructions read them: piece
-// (row 16 m + t, inputs 32 j + 8 g ..) of 16 bytes at place 16 g + (t ^ (4 g + j))
-// of 64 for (m, j). The exclusive or spreads a row's 16 pieces, which neighbouring
-// threads bring, over all banks. Weights go to registers, one block ahead too.
+// workgroups, join_kernel adds up what they leave. The rows' activations of 128
+// inputs go through LDS, one block ahead, in the order in which the waves' matrix
+// instructions read them: piece (row 16 m + t, inputs 32 j + 8 g ..) of 16 bytes
+// at place 16 g + (t ^ (4 g + j)) of 64 for (m, j). The exclusive or spreads a
+// row's 16 pieces, which neighbouring threads bring, over all banks. Weights go to
+// registers, one block ahead too. With few_kernel's way of reading activations
+// 512 x 2048 x 8192 took 124 us.
 constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave;
 template <bool BF, Form kForm, int kGroup, int MT, int NT>
 __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall c, const int64_t share) {
@@ -445,13 +461,19 @@ namespace {
 
 template <bool BF, Form kForm, int kGroup, int MT, int NT, int kWaves, int kDepth>
 void few(const LinearCall& c, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + NT - 1) / NT), static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)));
+  const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + NT - 1) / NT),
+                  static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)));
   hipLaunchKernelGGL((few_kernel<BF, kForm, kGroup, MT, NT, kWaves, kDepth>), grid, dim3(kWaves * kWave), 0, s, c);
 }
-constexpr int64_t kMinTiles = 32, kEnoughTiles = 256, kFillTiles = 512, kMinShare = 4;
-
 // Tiles of 16 MT rows and 64 NT outputs, and how many workgroups share the
 // inputs of each.
+// Wide tiles read the activations less often, narrow ones are more workgroups;
+// workgroups that share inputs are a second launch. us: 64 x 10240 x 2560 in 80
+// workgroups of (2, 1) tiles that share nothing 64, 40 (4, 1) tiles shared by 12
+// 18, by 6 22; 64 x 2560 x 10240 40 (4, 4) tiles shared by 5 17.8, 80 (4, 2)
+// tiles by 5 21.9; 512 x 2048 x 8192 512 (4, 2) tiles 26.7, 256 (4, 4) tiles 28.3,
+// shared by 2 37.
+constexpr int64_t kMinTiles = 32, kEnoughTiles = 256, kFillTiles = 512, kMinShare = 4;
 struct Tiles {
   int MT, NT, splits;
   int64_t share;   // blocks of inputs of a workgroup
@@ -461,7 +483,9 @@ Tiles plan(int64_t rows, int64_t out, int64_t in, bool bf16) {
   Tiles t{rows <= 32 ? 2 : 4, bf16 ? 4 : 2, 1, ib};
   auto count = [&] { return (rows + 16 * t.MT - 1) / (16 * t.MT) * ((ob + 4 * t.NT - 1) / (4 * t.NT)); };
   while (t.NT > 1 && count() < kMinTiles) t.NT /= 2;
-  const int64_t splits = count() >= kEnoughTiles ? 1 : std::max<int64_t>(1, std::min<int64_t>(kFillTiles / count(), ib / kMinShare));
+  if (t.NT == 4 && count() >= kEnoughTiles && count() < kFillTiles) t.NT = 2;
+  const int64_t splits =
+      count() >= kEnoughTiles ? 1 : std::max<int64_t>(1, std::min<int64_t>(kFillTiles / count(), ib / kMinShare));
   t.share = (ib + splits - 1) / splits;
   t.splits = static_cast<int>((ib + t.share - 1) / t.share);
   return t;
@@ -469,7 +493,10 @@ Tiles plan(int64_t rows, int64_t out, int64_t in, bool bf16) {
 // Whether a call runs on few_kernel, whose workgroups read the rows' activations
 // whole, each for few outputs, but in one launch without a barrier: always up to 16
 // rows; up to 32 while what they read together is small and the chip holds them at
-// once; up to 64 with few inputs and outputs.
+// once; up to 64 with few inputs and outputs. us, few_kernel / tile_kernel: 17 x 768
+// x 768 3.2 / 5.4, 17 x 2560 x 10240 9.5 / 12.2 (52 MB), 32 x 10240 x 2560 22 / 13.7
+// (105 MB), 32 x 768 x 65536 16.2 / 13.3; 64 x 768 x 3072 5.4 / 8.1, 64 x 3072 x 768
+// 13.2 / 9.5, 64 x 2048 x 2048 9.8 / 9.4, 64 x 768 x 65536 54 / 17.
 constexpr int64_t kFewRows = 16, kFewBytes = int64_t(64) << 20, kFewOutBlocks = 1024;
 constexpr int64_t kWideFewInBlocks = 8, kWideFewOutBlocks = 256;
 int few_columns(int64_t rows, int64_t ob) {   // NT
@@ -488,10 +515,12 @@ bool runs_few(int64_t rows, int64_t out, int64_t in, bool bf16) {
 template <bool BF, Form kForm, int kGroup, int MT, int NT>
 void tiles(const LinearCall& c, const Tiles& t, hipStream_t s) {
   constexpr int cols = kTileWaves * NT;
-  const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + cols - 1) / cols), static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)), t.splits);
+  const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + cols - 1) / cols),
+                  static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)), t.splits);
   hipLaunchKernelGGL((tile_kernel<BF, kForm, kGroup, MT, NT>), grid, dim3(kTileThreads), 0, s, c, t.share);
   if (t.splits > 1)
-    hipLaunchKernelGGL(join_kernel<BF>, dim3(static_cast<unsigned>((c.rows * c.out + 255) / 256)), dim3(256), 0, s, c, t.splits);
+    hipLaunchKernelGGL(join_kernel<BF>, dim3(static_cast<unsigned>((c.rows * c.out + 255) / 256)), dim3(256), 0, s, c,
+                       t.splits);
 }
 
 template <bool BF, Form kForm, int kGroup>

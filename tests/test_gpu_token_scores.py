@@ -80,7 +80,9 @@ def test_forward(vocab, dtype):
 
 @pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("rows,vocab,top", [(64, 1000, 20), (300, 4096, 3), (700, 256, 64), (1100, 97, 10),
-                                            (2100, 33, 2), (40, 65536, 20), (300, 20011, 7)])
+                                            (2100, 33, 2), (40, 65536, 20), (300, 20011, 7), (40, 65536, 32),
+                                            (40, 65536, 33), (600, 65536, 64), (300, 300, 33), (64, 2000, 33),
+                                            (500, 640, 64), (90, 1024, 64), (64, 4096, 48), (700, 8000, 40)])
 def test_forward_many_rows(rows, vocab, top, dtype):
     announce("token scores rows", rows, vocab, top, dtype)
     check(*make(rows, vocab, dtype, seed=7), top)
@@ -109,7 +111,7 @@ def test_masks_and_ties(vocab, dtype):
     x[13] = -0.0
     x[13, ::2] = 0.0                                     # zeros of both signs are equal
     tokens[14], tokens[15] = -1, vocab
-    for top in (0, 1, 20, 64):
+    for top in (0, 1, 20, 32, 33, 64):
         check(x, tokens, top)
 
 
