@@ -18,9 +18,8 @@
  * Code c stands for the magnitude number c & 7, negative when c & 8. A lane of
  * a matrix instruction reads its 32 weights as 16 consecutive bytes.
  *
- * packed and scales are aligned to 16 bytes, other operands to their elements
- * (rows that all begin on 16 bytes are read in pieces of 16). What a call
- * writes may not overlap anything else that it is given.
+ * packed and scales are aligned to 16 bytes, other operands to their elements.
+ * What a call writes may not overlap anything else that it is given.
  */
 #ifndef RWKV_RS_AMD_RWKV_W4_H
 #define RWKV_RS_AMD_RWKV_W4_H
@@ -31,7 +30,8 @@
 extern "C" {
 #endif
 
-/* The most outputs and inputs, and the most rows, that a call takes. */
+/* The most outputs and inputs, and the most rows, that a call takes. A weight
+ * has at most 2^31 - 1 blocks. */
 #define RWKV_W4_MAX_DIM (1 << 26)
 #define RWKV_W4_MAX_ROWS (1 << 20)
 

@@ -22,53 +22,53 @@ namespace {
 
 constexpr int kWave = 64;
 
-// Elements i .. i + 7 of a row of n, those past its end zero. kVector: n and i
-// are multiples of 8 and the row begins on 16 bytes.
-template <bool BF, bool kVector>
+// Rows of inputs that are no multiple of eight begin anywhere; the hardware takes
+// such addresses in one access.
+struct __attribute__((packed, aligned(2))) Half8 {
+  bf16x8 v;
+};
+struct __attribute__((packed, aligned(4))) Float8 {
+  float v[8];
+};
+
+// Elements i .. i + 7 of a row of n, those past its end zero (kWhole: there are none).
+template <bool BF, bool kWhole>
 __device__ __forceinline__ void load8(const void* row, int64_t i, int64_t n, float (&v)[8]) {
-  if (kVector) {
-    if (i >= n) {
+  if (kWhole || i + 8 <= n) {
+    if constexpr (BF) {
+      const bf16x8 w = reinterpret_cast<const Half8*>(static_cast<const uint16_t*>(row) + i)->v;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    } else if constexpr (BF) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(row) + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[2 * e] = __builtin_bit_cast(float, w[e] << 16);
-        v[2 * e + 1] = __builtin_bit_cast(float, w[e] & 0xffff0000u);
-      }
+      for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(w[e]);
     } else {
-      const f32x4* const p = reinterpret_cast<const f32x4*>(static_cast<const float*>(row) + i);
-      const f32x4 a = p[0], b = p[1];
+      const Float8 w = *reinterpret_cast<const Float8*>(static_cast<const float*>(row) + i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = a[e];
-        v[4 + e] = b[e];
-      }
+      for (int e = 0; e < 8; ++e) v[e] = w.v[e];
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (i + e >= n) v[e] = 0.f;
-      else if constexpr (BF) v[e] = bf_bits(static_cast<const uint16_t*>(row)[i + e]);
-      else v[e] = static_cast<const float*>(row)[i + e];
+      v[e] = 0.f;
+      if (i + e < n) {
+        if constexpr (BF) v[e] = bf_bits(static_cast<const uint16_t*>(row)[i + e]);
+        else v[e] = static_cast<const float*>(row)[i + e];
+      }
     }
   }
 }
 
-template <bool BF, bool kVector>
+template <bool BF>
 __device__ __forceinline__ void store8(void* row, int64_t i, int64_t n, const float (&v)[8]) {
-  if (kVector) {
-    if (i >= n) return;
+  if (i + 8 <= n) {
     if constexpr (BF) {
-      bf16x8 w;
+      Half8 w;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = static_cast<__bf16>(v[e]);
-      *reinterpret_cast<bf16x8*>(static_cast<uint16_t*>(row) + i) = w;
+      for (int e = 0; e < 8; ++e) w.v[e] = static_cast<__bf16>(v[e]);
+      *reinterpret_cast<Half8*>(static_cast<uint16_t*>(row) + i) = w;
     } else {
-      f32x4* const p = reinterpret_cast<f32x4*>(static_cast<float*>(row) + i);
-      p[0] = f32x4{v[0], v[1], v[2], v[3]};
-      p[1] = f32x4{v[4], v[5], v[6], v[7]};
+      Float8 w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w.v[e] = v[e];
+      *reinterpret_cast<Float8*>(static_cast<float*>(row) + i) = w;
     }
   } else {
 #pragma unroll
@@ -91,29 +91,53 @@ __device__ __forceinline__ char* row_at(void* base, int64_t row, int64_t n, bool
 // both: 65536 x 768 fp32 quantised and restored 93 us for 453 MB (4.9 TB/s).
 constexpr int kBlockWaves = 4;
 
-// Nearest magnitude, ties to the even mantissa: the midpoints times the scale
-// are exact in fp32 (three significant bits by eight), so no quotient is rounded.
-__device__ __forceinline__ uint32_t code_of(float w, float s) {
-  const float a = fabsf(w);
-  const uint32_t c = (a > 0.25f * s) + (a >= 0.75f * s) + (a > 1.25f * s) + (a >= 1.75f * s) + (a > 2.5f * s) +
-                     (a >= 3.5f * s) + (a > 5.f * s);
-  return c | (c && w < 0.f ? 8u : 0u);
+// Eight weights' codes: the nearest magnitude to |w| / s, ties to the even
+// mantissa, as the hardware's conversion rounds the quotient. The quotient is the
+// correctly rounded one (a product with the rounded reciprocal, corrected by its
+// residual, which is exact), and that is on a midpoint m only where w / s is: m s
+// has at most eleven significant bits, so another w is at least a unit in its own
+// last place away from it, and its quotient more than half of one in m's. Numbers
+// near the ends of fp32's range are moved to its middle first. What rounds to zero
+// has no sign. By comparisons with the seven midpoints it was twice the
+// instructions: 65536 x 768 bf16 42 us, so 29.
+struct Scale {
+  float shift, s, inverse;
+  __device__ __forceinline__ explicit Scale(float scale) {
+    shift = scale < 0x1p-64f ? 0x1p100f : scale > 0x1p64f ? 0x1p-100f : 1.f;
+    s = scale * shift;
+    inverse = 1.f / s;
+  }
+  __device__ __forceinline__ float quotient(float w) const {
+    w *= shift;
+    const float q = w * inverse;
+    return fmaf(fmaf(-q, s, w), inverse, q);
+  }
+};
+__device__ __forceinline__ uint32_t codes_of(const float (&w)[8], const Scale& s) {
+  uint32_t word = 0;
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, s.quotient(w[0]), s.quotient(w[1]), 1.f, 0);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, s.quotient(w[2]), s.quotient(w[3]), 1.f, 1);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, s.quotient(w[4]), s.quotient(w[5]), 1.f, 2);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, s.quotient(w[6]), s.quotient(w[7]), 1.f, 3);
+  const uint32_t some = (word & 0x77777777u) + 0x77777777u;   // bit 3 of each code whose magnitude is not 0
+  return word & (some | 0x77777777u);
 }
 
 constexpr uint32_t kMaxScale = 0x7e2a;   // the largest bf16 number six times which is an fp32 number
 
-template <bool BF, bool kVector, int kGroup>
+template <bool BF, int kGroup>
 __global__ __launch_bounds__(kBlockWaves* kWave) void quantize_kernel(const WeightCall c) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int64_t ib = blocks_in(c.in), blocks = blocks_out(c.out) * ib;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kBlockWaves;
-  for (int64_t b = static_cast<int64_t>(blockIdx.x) * kBlockWaves + (threadIdx.x >> 6); b < blocks; b += stride) {
-    const int64_t n = b / ib, k = b % ib, row = n * kRows + r;
+  const uint32_t ib = static_cast<uint32_t>(blocks_in(c.in)), blocks = static_cast<uint32_t>(blocks_out(c.out)) * ib;
+  const uint32_t first = blockIdx.x * kBlockWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (uint32_t i = first; i < blocks; i += gridDim.x * kBlockWaves) {
+    const uint32_t out = i / ib;
+    const int64_t b = i, n = out, k = i - out * ib, row = n * kRows + r;
     float w[4][8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (row < c.out) {
-        load8<BF, kVector>(row_at(c.weight, row, c.in, BF), k * kInputs + 32 * j + 8 * g, c.in, w[j]);
+        load8<BF, false>(row_at(c.weight, row, c.in, BF), k * kInputs + 32 * j + 8 * g, c.in, w[j]);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[j][e] = 0.f;
@@ -145,9 +169,8 @@ __global__ __launch_bounds__(kBlockWaves* kWave) void quantize_kernel(const Weig
     for (int j = 0; j < 4; ++j) {
       const float s = bf_bits(scale[j / kSteps]);
       word[j] = 0;
-      if (s > 0.f)   // not 0, and not NaN
-#pragma unroll
-        for (int e = 0; e < 8; ++e) word[j] |= code_of(w[j][e], s) << (4 * e);
+      const uint32_t codes = codes_of(w[j], Scale(s));
+      if (s > 0.f) word[j] = codes;   // not 0, and not NaN
     }
     reinterpret_cast<u32x4*>(c.packed)[b * kWave + lane] = word;
     if (g == 0)
@@ -156,13 +179,14 @@ __global__ __launch_bounds__(kBlockWaves* kWave) void quantize_kernel(const Weig
   }
 }
 
-template <bool BF, bool kVector, int kGroup>
+template <bool BF, int kGroup>
 __global__ __launch_bounds__(kBlockWaves* kWave) void dequantize_kernel(const WeightCall c) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int64_t ib = blocks_in(c.in), blocks = blocks_out(c.out) * ib;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kBlockWaves;
-  for (int64_t b = static_cast<int64_t>(blockIdx.x) * kBlockWaves + (threadIdx.x >> 6); b < blocks; b += stride) {
-    const int64_t n = b / ib, k = b % ib, row = n * kRows + r;
+  const uint32_t ib = static_cast<uint32_t>(blocks_in(c.in)), blocks = static_cast<uint32_t>(blocks_out(c.out)) * ib;
+  const uint32_t first = blockIdx.x * kBlockWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (uint32_t i = first; i < blocks; i += gridDim.x * kBlockWaves) {
+    const uint32_t out = i / ib;
+    const int64_t b = i, n = out, k = i - out * ib, row = n * kRows + r;
     if (row >= c.out) continue;
     const u32x4 word = reinterpret_cast<const u32x4*>(c.packed)[b * kWave + lane];
     float s[kInputs / kGroup];
@@ -173,40 +197,26 @@ __global__ __launch_bounds__(kBlockWaves* kWave) void dequantize_kernel(const We
       float w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = kShrink * static_cast<float>(v[e]) * s[32 * j / kGroup];
-      store8<BF, kVector>(row_at(c.weight, row, c.in, BF), k * kInputs + 32 * j + 8 * g, c.in, w);
+      store8<BF>(row_at(c.weight, row, c.in, BF), k * kInputs + 32 * j + 8 * g, c.in, w);
     }
   }
 }
 
 // --------------------------------------------------------------------- linear
-// How rows of activations are read: every one is whole blocks of 128 inputs, or
-// pieces of eight, from a 16-byte boundary on; or element by element.
-enum Form { kBlocks, kPieces, kElements };
-
+// Activations i .. i + 7 of a row of n. kWhole: it is whole blocks of 128 inputs.
 // v_mfma_f32_16x16x32_bf16: lane l holds A[row l % 16] and B[column l % 16] at
 // k = 8 (l / 16) .. + 7, the result D[row 4 (l / 16) + r][column l % 16].
-template <bool BF, Form kForm>
+template <bool BF, bool kWhole>
 __device__ __forceinline__ auto load_x(const void* row, int64_t i, int64_t n) {
-  if constexpr (BF && kForm != kElements) {
+  float v[8];
+  load8<BF, kWhole>(row, i, n, v);
+  if constexpr (BF) {
     Parts<1> p;
-    if (kForm == kBlocks || i < n) {
-      p.p[0] = *reinterpret_cast<const bf16x8*>(static_cast<const uint16_t*>(row) + i);
-    } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p.p[0][e] = static_cast<__bf16>(0.f);
-    }
+    for (int e = 0; e < 8; ++e) p.p[0][e] = static_cast<__bf16>(v[e]);
     return p;
   } else {
-    float v[8];
-    load8<BF, kForm != kElements>(row, i, kForm == kBlocks ? INT64_MAX : n, v);
-    if constexpr (BF) {
-      Parts<1> p;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) p.p[0][e] = static_cast<__bf16>(v[e]);
-      return p;
-    } else {
-      return split(v);
-    }
+    return split(v);
   }
 }
 
@@ -234,7 +244,7 @@ __device__ __forceinline__ void store_y(const LinearCall& c, int64_t row, int64_
 // 12.8, (4, 8, 1) 11.1, (2, 16, 1) 8.9; 768 x 65536, 8 rows, (1, 8, 4) 17.0, (2,
 // 16, 1) 11.5, (4, 8, 2) 9.5; 4096 x 4096 (1, 8, 4) 5.2, (1, 16, 2) 4.7; 16384 x
 // 4096 one tile at a time 23.9, (1, 16, 2) 11.4, (2, 16, 1) 14.
-template <bool BF, Form kForm, int kGroup, int MT, int NT, int kWaves, int kDepth>
+template <bool BF, bool kWhole, int kGroup, int MT, int NT, int kWaves, int kDepth>
 __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) {
   __shared__ float part[kWaves][MT * NT * 256];
   constexpr int kParts = BF ? 1 : 3, kSteps = kGroup / 32;
@@ -273,7 +283,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) xs[d][m][j] = load_x<BF, kForm>(x[m], k * kInputs + 32 * j + 8 * g, c.in);
+          for (int j = 0; j < 4; ++j) xs[d][m][j] = load_x<BF, kWhole>(x[m], k * kInputs + 32 * j + 8 * g, c.in);
       }
     }
 #pragma unroll
@@ -319,7 +329,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
 // registers, one block ahead too. With few_kernel's way of reading activations
 // 512 x 2048 x 8192 took 124 us.
 constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave;
-template <bool BF, Form kForm, int kGroup, int MT, int NT>
+template <bool BF, bool kWhole, int kGroup, int MT, int NT>
 __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall c, const int64_t share) {
   constexpr int kParts = BF ? 1 : 3, kSteps = kGroup / 32, kPiecesOfRow = kInputs / 8;
   constexpr int kLoads = 16 * MT * kPiecesOfRow / kTileThreads;   // pieces a thread brings
@@ -342,7 +352,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall 
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int64_t row = min(row0 + tid / kPiecesOfRow + i * (kTileThreads / kPiecesOfRow), c.rows - 1);
-      bring[i] = load_x<BF, kForm>(row_at(const_cast<void*>(c.x), row, c.in, BF), k * kInputs + 8 * piece, c.in);
+      bring[i] = load_x<BF, kWhole>(row_at(const_cast<void*>(c.x), row, c.in, BF), k * kInputs + 8 * piece, c.in);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -426,44 +436,39 @@ hipError_t by_group(int group, F&& f) {
   return hipGetLastError();
 }
 template <typename F>
-hipError_t by_form(bool bf16, bool vector, int group, F&& f) {
-  return by_group(group, [&](auto g) {
-    if (bf16) vector ? f(std::true_type(), std::true_type(), g) : f(std::true_type(), std::false_type(), g);
-    else vector ? f(std::false_type(), std::true_type(), g) : f(std::false_type(), std::false_type(), g);
-  });
+hipError_t by_type(bool bf16, int group, F&& f) {
+  return by_group(group, [&](auto g) { bf16 ? f(std::true_type(), g) : f(std::false_type(), g); });
 }
 
-bool vector_rows(const void* p, int64_t n) { return n % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-// enough workgroups for every compute unit's waves; each takes several blocks beyond that
-unsigned block_grid(const WeightCall& c) {
+// a block of weights a wave; beyond what a launch holds, several
+dim3 block_grid(const WeightCall& c) {
   const int64_t blocks = blocks_out(c.out) * blocks_in(c.in);
-  return static_cast<unsigned>(std::min<int64_t>((blocks + kBlockWaves - 1) / kBlockWaves, 1 << 20));
+  return dim3(static_cast<unsigned>(std::min<int64_t>((blocks + kBlockWaves - 1) / kBlockWaves, 1 << 20)));
 }
 
 }  // namespace
 
 hipError_t launch_quantize(const WeightCall& c, hipStream_t stream) {
-  return by_form(c.bf16, vector_rows(c.weight, c.in), c.group, [&](auto bf, auto vec, auto group) {
-    hipLaunchKernelGGL((quantize_kernel<bf(), vec(), group()>), dim3(block_grid(c)), dim3(kBlockWaves * kWave), 0,
+  return by_type(c.bf16, c.group, [&](auto bf, auto group) {
+    hipLaunchKernelGGL((quantize_kernel<bf(), group()>), block_grid(c), dim3(kBlockWaves * kWave), 0,
                        stream, c);
   });
 }
 
 hipError_t launch_dequantize(const WeightCall& c, hipStream_t stream) {
-  return by_form(c.bf16, vector_rows(c.weight, c.in), c.group, [&](auto bf, auto vec, auto group) {
-    hipLaunchKernelGGL((dequantize_kernel<bf(), vec(), group()>), dim3(block_grid(c)), dim3(kBlockWaves * kWave), 0,
+  return by_type(c.bf16, c.group, [&](auto bf, auto group) {
+    hipLaunchKernelGGL((dequantize_kernel<bf(), group()>), block_grid(c), dim3(kBlockWaves * kWave), 0,
                        stream, c);
   });
 }
 
 namespace {
 
-template <bool BF, Form kForm, int kGroup, int MT, int NT, int kWaves, int kDepth>
+template <bool BF, bool kWhole, int kGroup, int MT, int NT, int kWaves, int kDepth>
 void few(const LinearCall& c, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + NT - 1) / NT),
                   static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)));
-  hipLaunchKernelGGL((few_kernel<BF, kForm, kGroup, MT, NT, kWaves, kDepth>), grid, dim3(kWaves * kWave), 0, s, c);
+  hipLaunchKernelGGL((few_kernel<BF, kWhole, kGroup, MT, NT, kWaves, kDepth>), grid, dim3(kWaves * kWave), 0, s, c);
 }
 // Tiles of 16 MT rows and 64 NT outputs, and how many workgroups share the
 // inputs of each.
@@ -512,43 +517,43 @@ bool runs_few(int64_t rows, int64_t out, int64_t in, bool bf16) {
   return ob <= kFewOutBlocks && (ob + NT - 1) / NT * 32 * in * (bf16 ? 2 : 4) <= kFewBytes;
 }
 
-template <bool BF, Form kForm, int kGroup, int MT, int NT>
+template <bool BF, bool kWhole, int kGroup, int MT, int NT>
 void tiles(const LinearCall& c, const Tiles& t, hipStream_t s) {
   constexpr int cols = kTileWaves * NT;
   const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + cols - 1) / cols),
                   static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)), t.splits);
-  hipLaunchKernelGGL((tile_kernel<BF, kForm, kGroup, MT, NT>), grid, dim3(kTileThreads), 0, s, c, t.share);
+  hipLaunchKernelGGL((tile_kernel<BF, kWhole, kGroup, MT, NT>), grid, dim3(kTileThreads), 0, s, c, t.share);
   if (t.splits > 1)
     hipLaunchKernelGGL(join_kernel<BF>, dim3(static_cast<unsigned>((c.rows * c.out + 255) / 256)), dim3(256), 0, s, c,
                        t.splits);
 }
 
-template <bool BF, Form kForm, int kGroup>
+template <bool BF, bool kWhole, int kGroup>
 void linear(const LinearCall& c, hipStream_t s) {
   if (runs_few(c.rows, c.out, c.in, BF)) {
     const int NT = few_columns(c.rows, blocks_out(c.out));
     if (c.rows > 32) {
-      few<BF, kForm, kGroup, 4, 1, 8, 1>(c, s);
+      few<BF, kWhole, kGroup, 4, 1, 8, 1>(c, s);
     } else if (c.rows > 16) {
-      if (NT == 4) few<BF, kForm, kGroup, 2, 4, 8, 1>(c, s);
-      else if (NT == 2) few<BF, kForm, kGroup, 2, 2, 8, 1>(c, s);
-      else few<BF, kForm, kGroup, 2, 1, 8, BF ? 2 : 1>(c, s);
+      if (NT == 4) few<BF, kWhole, kGroup, 2, 4, 8, 1>(c, s);
+      else if (NT == 2) few<BF, kWhole, kGroup, 2, 2, 8, 1>(c, s);
+      else few<BF, kWhole, kGroup, 2, 1, 8, BF ? 2 : 1>(c, s);
     } else {
-      if (NT == 4) few<BF, kForm, kGroup, 1, 4, 8, BF ? 2 : 1>(c, s);
-      else if (NT == 2) few<BF, kForm, kGroup, 1, 2, BF ? 16 : 8, 1>(c, s);
-      else few<BF, kForm, kGroup, 1, 1, 16, BF ? 2 : 1>(c, s);
+      if (NT == 4) few<BF, kWhole, kGroup, 1, 4, 8, BF ? 2 : 1>(c, s);
+      else if (NT == 2) few<BF, kWhole, kGroup, 1, 2, BF ? 16 : 8, 1>(c, s);
+      else few<BF, kWhole, kGroup, 1, 1, 16, BF ? 2 : 1>(c, s);
     }
     return;
   }
   const Tiles t = plan(c.rows, c.out, c.in, BF);
   if (t.MT == 2) {
-    if (t.NT == 1) tiles<BF, kForm, kGroup, 2, 1>(c, t, s);
-    else if (t.NT == 2) tiles<BF, kForm, kGroup, 2, 2>(c, t, s);
-    else if constexpr (BF) tiles<BF, kForm, kGroup, 2, 4>(c, t, s);
+    if (t.NT == 1) tiles<BF, kWhole, kGroup, 2, 1>(c, t, s);
+    else if (t.NT == 2) tiles<BF, kWhole, kGroup, 2, 2>(c, t, s);
+    else if constexpr (BF) tiles<BF, kWhole, kGroup, 2, 4>(c, t, s);
   } else {
-    if (t.NT == 1) tiles<BF, kForm, kGroup, 4, 1>(c, t, s);
-    else if (t.NT == 2) tiles<BF, kForm, kGroup, 4, 2>(c, t, s);
-    else if constexpr (BF) tiles<BF, kForm, kGroup, 4, 4>(c, t, s);
+    if (t.NT == 1) tiles<BF, kWhole, kGroup, 4, 1>(c, t, s);
+    else if (t.NT == 2) tiles<BF, kWhole, kGroup, 4, 2>(c, t, s);
+    else if constexpr (BF) tiles<BF, kWhole, kGroup, 4, 4>(c, t, s);
   }
 }
 
@@ -561,10 +566,9 @@ int64_t workspace_bytes(int64_t rows, int64_t out, int64_t in, bool bf16) {
 }
 
 hipError_t launch_linear(const LinearCall& c, hipStream_t stream) {
-  return by_form(c.bf16, vector_rows(c.x, c.in), c.group, [&](auto bf, auto vec, auto group) {
-    if constexpr (!vec()) linear<bf(), kElements, group()>(c, stream);
-    else if (c.in % kInputs == 0) linear<bf(), kBlocks, group()>(c, stream);
-    else linear<bf(), kPieces, group()>(c, stream);
+  return by_type(c.bf16, c.group, [&](auto bf, auto group) {
+    if (c.in % kInputs == 0) linear<bf(), true, group()>(c, stream);
+    else linear<bf(), false, group()>(c, stream);
   });
 }
 

@@ -37,7 +37,8 @@ bool any_overlap(Ranges outs, Ranges ins) {
 }
 
 bool dims_ok(int64_t out, int64_t in) {
-  return out > 0 && out <= RWKV_W4_MAX_DIM && in > 0 && in <= RWKV_W4_MAX_DIM;
+  return out > 0 && out <= RWKV_W4_MAX_DIM && in > 0 && in <= RWKV_W4_MAX_DIM &&
+         rwkv_w4::blocks_out(out) * rwkv_w4::blocks_in(in) <= INT32_MAX;
 }
 bool group_ok(int64_t group) { return group == 32 || group == 64 || group == 128; }
 int64_t size_of(int dtype) { return dtype == WKV7_DTYPE_BF16 ? 2 : 4; }

@@ -34,7 +34,8 @@ def test_w4_sizes(native):
     assert lib.rwkv_w4_packed_bytes(768, 768) == 768 * 768 // 2
     assert lib.rwkv_w4_scales_bytes(768, 768, 64) == 768 * 12 * 2
     assert lib.rwkv_w4_scales_bytes(17, 129, 32) == 32 * 8 * 2
-    for bad in ((0, 1), (1, 0), (-1, 5), ((1 << 26) + 1, 8), (8, (1 << 26) + 1)):
+    assert lib.rwkv_w4_packed_bytes(1 << 26, 512 * 128 - 128) == (1 << 22) * 511 * 1024
+    for bad in ((0, 1), (1, 0), (-1, 5), ((1 << 26) + 1, 8), (8, (1 << 26) + 1), (1 << 26, 512 * 128)):
         assert lib.rwkv_w4_packed_bytes(*bad) == -1 and lib.rwkv_w4_scales_bytes(*bad, 64) == -1
     assert lib.rwkv_w4_scales_bytes(8, 8, 16) == -1
 
