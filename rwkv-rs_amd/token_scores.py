@@ -15,6 +15,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
 from .neighbors import _code, _ptr, _stream
@@ -60,6 +61,7 @@ class _TokenScores(torch.autograd.Function):
         return log_prob, entropy, top_lp, top_ids
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_log_prob, d_entropy, d_top, _):
         if d_log_prob is None and d_entropy is None and d_top is None:
             return None, None, None

@@ -292,6 +292,37 @@ def test_replays(rows, vocab):
             assert torch.equal(got, b)
 
 
+def test_more_rows_than_a_launch_holds():
+    announce("token scores, 2^21 + 5 rows")
+    rows, vocab = (1 << 21) + 5, 8
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(rows, vocab, generator=g, device="cuda").requires_grad_()
+    tokens = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    out = ts.token_scores(x, tokens, 2)
+    w = torch.randn(rows, generator=g, device="cuda")
+    grad, = torch.autograd.grad((out.log_prob, out.entropy, out.top_log_probs), x,
+                                (w, 2 * w, torch.stack([w, -w], 1)))
+    for part in (slice(0, 9), slice((1 << 21) - 4, None)):       # around the cut, alone
+        y = x.detach()[part].requires_grad_()
+        few = ts.token_scores(y, tokens[part], 2)
+        for a, b in zip(out, few):
+            assert torch.equal(a[part], b)
+        alone, = torch.autograd.grad((few.log_prob, few.entropy, few.top_log_probs), y,
+                                     (w[part], 2 * w[part], torch.stack([w[part], -w[part]], 1)))
+        assert torch.equal(grad[part], alone)
+    want = torch.log_softmax(x.detach().double(), 1).gather(1, tokens[:, None])[:, 0]
+    assert (out.log_prob.double() - want).abs().max() < 1e-5
+
+
+def test_there_is_no_second_derivative():
+    announce("token scores, second derivative")
+    x, tokens = make(3, 40, torch.float32)
+    x = x.cuda().requires_grad_()
+    grad, = torch.autograd.grad(ts.token_scores(x, tokens.cuda()).log_prob.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()
+
+
 def test_refusals():
     announce("token scores refusals")
     x, tokens = make(4, 30, torch.float32)
