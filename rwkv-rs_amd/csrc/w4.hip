@@ -330,7 +330,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
 // 512 x 2048 x 8192 took 124 us.
 constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave;
 template <bool BF, bool kWhole, int kGroup, int MT, int NT>
-__global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall c, const int64_t share) {
+__global__ __launch_bounds__(kTileThreads, BF ? 2 : 1) void tile_kernel(const LinearCall c, const int64_t share) {
   constexpr int kParts = BF ? 1 : 3, kSteps = kGroup / 32, kPiecesOfRow = kInputs / 8;
   constexpr int kLoads = 16 * MT * kPiecesOfRow / kTileThreads;   // pieces a thread brings
   __shared__ bf16x8 xs[2][kParts][MT * 4 * kWave];
