@@ -10,10 +10,11 @@
 //
 // Up to about 64 rows the weights' bytes bound it: few_kernel, 1 x 4096 x 16384
 // (34 MB) 8.8 us, 8 x 4096 x 65536 28 us (4.8 TB/s, what a copy reaches). Many
-// rows are matrix products: tile_kernel, 512 x 2048 x 8192 26.7 us (644 TFLOP/s),
-// 2048 x 4096 x 4096 74 us (927), a library product of bf16 matrices of 8192^3
+// rows are matrix products: tile_kernel, 512 x 2048 x 8192 24.5 us (700 TFLOP/s),
+// 2048 x 4096 x 4096 75 us (916), a library product of bf16 matrices of 8192^3
 // 1130.
 #include <algorithm>
+#include <iterator>
 
 #include "w4_device.hpp"
 
@@ -31,29 +32,33 @@ struct __attribute__((packed, aligned(4))) Float8 {
   float v[8];
 };
 
-// Elements i .. i + 7 of a row of n, those past its end zero (kWhole: there are none).
+// Elements i .. i + 7 of a row of n in its type, those past its end zero (kWhole:
+// there are none).
+template <bool BF>
+struct Eight {
+  std::conditional_t<BF, bf16x8, float[8]> v;
+};
 template <bool BF, bool kWhole>
-__device__ __forceinline__ void load8(const void* row, int64_t i, int64_t n, float (&v)[8]) {
+__device__ __forceinline__ Eight<BF> load8(const void* row, int64_t i, int64_t n) {
+  using T = std::conditional_t<BF, __bf16, float>;
+  const T* const p = static_cast<const T*>(row) + i;
+  Eight<BF> x;
   if (kWhole || i + 8 <= n) {
     if constexpr (BF) {
-      const bf16x8 w = reinterpret_cast<const Half8*>(static_cast<const uint16_t*>(row) + i)->v;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(w[e]);
+      x.v = reinterpret_cast<const Half8*>(p)->v;
     } else {
-      const Float8 w = *reinterpret_cast<const Float8*>(static_cast<const float*>(row) + i);
+      const Float8 w = *reinterpret_cast<const Float8*>(p);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = w.v[e];
+      for (int e = 0; e < 8; ++e) x.v[e] = w.v[e];
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[e] = 0.f;
-      if (i + e < n) {
-        if constexpr (BF) v[e] = bf_bits(static_cast<const uint16_t*>(row)[i + e]);
-        else v[e] = static_cast<const float*>(row)[i + e];
-      }
+      x.v[e] = T(0.f);
+      if (i + e < n) x.v[e] = p[e];
     }
   }
+  return x;
 }
 
 template <bool BF>
@@ -133,16 +138,14 @@ __global__ __launch_bounds__(kBlockWaves* kWave) void quantize_kernel(const Weig
   for (uint32_t i = first; i < blocks; i += gridDim.x * kBlockWaves) {
     const uint32_t out = i / ib;
     const int64_t b = i, n = out, k = i - out * ib, row = n * kRows + r;
+    Eight<BF> x[4];
     float w[4][8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (row < c.out) {
-        load8<BF, false>(row_at(c.weight, row, c.in, BF), k * kInputs + 32 * j + 8 * g, c.in, w[j]);
-      } else {
+    for (int j = 0; j < 4; ++j) x[j] = load8<BF, false>(row_at(c.weight, min(row, c.out - 1), c.in, BF), k * kInputs + 32 * j + 8 * g, c.in);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[j][e] = 0.f;
-      }
-    }
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[j][e] = row < c.out ? static_cast<float>(x[j].v[e]) : 0.f;
     // the largest magnitude as an integer: infinities and NaN are above all numbers
     uint32_t top[4];
 #pragma unroll
@@ -189,8 +192,7 @@ __global__ __launch_bounds__(kBlockWaves* kWave) void dequantize_kernel(const We
     const int64_t b = i, n = out, k = i - out * ib, row = n * kRows + r;
     if (row >= c.out) continue;
     const u32x4 word = reinterpret_cast<const u32x4*>(c.packed)[b * kWave + lane];
-    float s[kInputs / kGroup];
-    load_scales<kGroup>(c.scales, b * kRows + r, s);
+    const Scales<kGroup> s = load_scales<kGroup>(c.scales, b * kRows + r);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const bf16x8 v = weights8(word[j]);
@@ -203,21 +205,12 @@ __global__ __launch_bounds__(kBlockWaves* kWave) void dequantize_kernel(const We
 }
 
 // --------------------------------------------------------------------- linear
-// Activations i .. i + 7 of a row of n. kWhole: it is whole blocks of 128 inputs.
 // v_mfma_f32_16x16x32_bf16: lane l holds A[row l % 16] and B[column l % 16] at
 // k = 8 (l / 16) .. + 7, the result D[row 4 (l / 16) + r][column l % 16].
-template <bool BF, bool kWhole>
-__device__ __forceinline__ auto load_x(const void* row, int64_t i, int64_t n) {
-  float v[8];
-  load8<BF, kWhole>(row, i, n, v);
-  if constexpr (BF) {
-    Parts<1> p;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) p.p[0][e] = static_cast<__bf16>(v[e]);
-    return p;
-  } else {
-    return split(v);
-  }
+template <bool BF>
+__device__ __forceinline__ auto parts(const Eight<BF>& x) {
+  if constexpr (BF) return Parts<1>{{x.v}};
+  else return split(x.v);
 }
 
 template <int kParts>
@@ -262,7 +255,7 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
     for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int64_t k0 = wave; k0 < ib; k0 += kWaves * kDepth) {
     u32x4 word[kDepth][NT];
-    float s[kDepth][NT][kInputs / kGroup];
+    Scales<kGroup> s[kDepth][NT];
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       const int64_t k = k0 + d * kWaves;
@@ -271,11 +264,11 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
         for (int n = 0; n < NT; ++n) {
           const int64_t b = min(n0 + n, ob - 1) * ib + k;   // past the end: the last outputs, not stored
           word[d][n] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(c.packed) + b * kWave + lane);
-          load_scales<kGroup>(c.scales, b * kRows + t, s[d][n]);
+          s[d][n] = load_scales<kGroup>(c.scales, b * kRows + t);
         }
       }
     }
-    Parts<kParts> xs[kDepth][MT][4];
+    Eight<BF> xs[kDepth][MT][4];
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       const int64_t k = k0 + d * kWaves;
@@ -283,22 +276,22 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) xs[d][m][j] = load_x<BF, kWhole>(x[m], k * kInputs + 32 * j + 8 * g, c.in);
+          for (int j = 0; j < 4; ++j) xs[d][m][j] = load8<BF, kWhole>(x[m], k * kInputs + 32 * j + 8 * g, c.in);
       }
     }
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       if (k0 + d * kWaves < ib) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          f32x4 sum[MT];
+        for (int m = 0; m < MT; ++m) {
+          f32x4 sum[NT];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const bf16x8 w = weights8(word[d][n][j]);
+            const Parts<kParts> a = parts<BF>(xs[d][m][j]);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              sum[m] = multiply(xs[d][m][j], w, j % kSteps == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[m]);
-              if (j % kSteps == kSteps - 1) acc[m][n] += sum[m] * s[d][n][32 * j / kGroup];
+            for (int n = 0; n < NT; ++n) {
+              sum[n] = multiply(a, weights8(word[d][n][j]), j % kSteps == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[n]);
+              if (j % kSteps == kSteps - 1) acc[m][n] += sum[n] * s[d][n][32 * j / kGroup];
             }
           }
         }
@@ -322,17 +315,24 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
 // Many rows. A workgroup forms 16 MT rows by 64 NT outputs of `share` blocks of
 // inputs, its four waves 16 NT outputs each; where the inputs are shared among
 // workgroups, join_kernel adds up what they leave. The rows' activations of 128
-// inputs go through LDS, one block ahead, in the order in which the waves' matrix
-// instructions read them: piece (row 16 m + t, inputs 32 j + 8 g ..) of 16 bytes
-// at place 16 g + (t ^ (4 g + j)) of 64 for (m, j). The exclusive or spreads a
-// row's 16 pieces, which neighbouring threads bring, over all banks. Weights go to
-// registers, one block ahead too. With few_kernel's way of reading activations
-// 512 x 2048 x 8192 took 124 us.
+// inputs go through LDS in the order in which the waves' matrix instructions read
+// them: piece (row 16 m + t, inputs 32 j + 8 g ..) of 16 bytes at place 16 g + (t ^
+// (4 g + j)) of 64 for (m, j). The exclusive or spreads a row's 16 pieces, which
+// neighbouring threads bring, over all banks. With few_kernel's way of reading
+// activations 512 x 2048 x 8192 took 124 us.
+//
+// Loads are two blocks ahead, in registers of their own for odd and even blocks, as
+// they come from memory: activations are asked for once LDS has the ones before,
+// weights once the products have. A condition around a load, a conversion at it or a
+// copy of what it brings made the compiler wait for all of them in each block: 512 x
+// 2048 x 8192 fp32 81 us, now 50; 512 x 8192 x 2048 40, now 31. The last blocks ask
+// for the last one again instead. (4, 4) tiles have registers for one block ahead.
 constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave;
 template <bool BF, bool kWhole, int kGroup, int MT, int NT>
-__global__ __launch_bounds__(kTileThreads, BF ? 2 : 1) void tile_kernel(const LinearCall c, const int64_t share) {
+__global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall c, const int64_t share) {
   constexpr int kParts = BF ? 1 : 3, kSteps = kGroup / 32, kPiecesOfRow = kInputs / 8;
   constexpr int kLoads = 16 * MT * kPiecesOfRow / kTileThreads;   // pieces a thread brings
+  constexpr int kAhead = MT * NT > 8 ? 1 : 2;
   __shared__ bf16x8 xs[2][kParts][MT * 4 * kWave];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int t = lane & 15, g = lane >> 4;
@@ -344,45 +344,45 @@ __global__ __launch_bounds__(kTileThreads, BF ? 2 : 1) void tile_kernel(const Li
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Parts<kParts> bring[kLoads];
-  u32x4 word[NT];
-  float s[NT][kInputs / kGroup];
+  Eight<BF> bring[kAhead][kLoads];
+  u32x4 word[kAhead][NT];
+  Scales<kGroup> s[kAhead][NT];
   const int piece = tid % kPiecesOfRow;
-  auto load = [&](int64_t k) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int64_t row = min(row0 + tid / kPiecesOfRow + i * (kTileThreads / kPiecesOfRow), c.rows - 1);
-      bring[i] = load_x<BF, kWhole>(row_at(const_cast<void*>(c.x), row, c.in, BF), k * kInputs + 8 * piece, c.in);
-    }
+  auto load_w = [&](int d, int64_t k) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int64_t b = min(n0 + n, ob - 1) * ib + k;   // past the end: the last outputs, not stored
-      word[n] = reinterpret_cast<const u32x4*>(c.packed)[b * kWave + lane];
-      load_scales<kGroup>(c.scales, b * kRows + t, s[n]);
+      word[d][n] = reinterpret_cast<const u32x4*>(c.packed)[b * kWave + lane];
+      s[d][n] = load_scales<kGroup>(c.scales, b * kRows + t);
     }
   };
-  const int64_t k1 = min(blockIdx.z * share + share, ib);
-  int buffer = 0;
-  if (blockIdx.z * share < k1) load(blockIdx.z * share);
-  for (int64_t k = blockIdx.z * share; k < k1; ++k, buffer ^= 1) {
+  auto load_x = [&](int d, int64_t k) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int64_t row = min(row0 + tid / kPiecesOfRow + i * (kTileThreads / kPiecesOfRow), c.rows - 1);
+      bring[d][i] = load8<BF, kWhole>(row_at(const_cast<void*>(c.x), row, c.in, BF), k * kInputs + 8 * piece, c.in);
+    }
+  };
+  const int64_t first = blockIdx.z * share, k1 = min(first + share, ib);
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d) {
+    load_x(d, min(first + d, k1 - 1));
+    load_w(d, min(first + d, k1 - 1));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  auto step = [&](int d, int buffer, int64_t k) {
     bf16x8(*const at)[MT * 4 * kWave] = xs[buffer];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = tid / kPiecesOfRow + i * (kTileThreads / kPiecesOfRow), j = piece >> 2, q = piece & 3;
       const int place = (row / 16 * 4 + j) * kWave + 16 * q + ((row & 15) ^ (4 * q + j));
+      const Parts<kParts> x = parts<BF>(bring[d][i]);
 #pragma unroll
-      for (int p = 0; p < kParts; ++p) at[p][place] = bring[i].p[p];
-    }
-    u32x4 w[NT];
-    float scale[NT][kInputs / kGroup];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      w[n] = word[n];
-#pragma unroll
-      for (int q = 0; q < kInputs / kGroup; ++q) scale[n][q] = s[n][q];
+      for (int p = 0; p < kParts; ++p) at[p][place] = x.p[p];
     }
     __syncthreads();   // the block before is read: its place is written only after the next of these
-    if (k + 1 < k1) load(k + 1);
+    load_x(d, min(k + kAhead, k1 - 1));
+    __builtin_amdgcn_sched_barrier(0);
     f32x4 sum[MT][NT];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -393,25 +393,42 @@ __global__ __launch_bounds__(kTileThreads, BF ? 2 : 1) void tile_kernel(const Li
         for (int p = 0; p < kParts; ++p) a[m].p[p] = at[p][(m * 4 + j) * kWave + 16 * g + (t ^ (4 * g + j))];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const bf16x8 v = weights8(w[n][j]);
+        const bf16x8 v = weights8(word[d][n][j]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           sum[m][n] = multiply(a[m], v, j % kSteps == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[m][n]);
-          if (j % kSteps == kSteps - 1) acc[m][n] += sum[m][n] * scale[n][32 * j / kGroup];
+          if (j % kSteps == kSteps - 1) acc[m][n] += sum[m][n] * s[d][n][32 * j / kGroup];
         }
       }
     }
+    load_w(d, min(k + kAhead, k1 - 1));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  int64_t k = first;
+  if constexpr (kAhead == 1) {
+    for (int buffer = 0; k < k1; ++k, buffer ^= 1) step(0, buffer, k);
+  } else {
+    for (; k + 1 < k1; k += 2) {
+      step(0, 0, k);
+      step(1, 1, k + 1);
+    }
+    if (k < k1) step(0, 0, k);
   }
+  const bool shared = gridDim.z > 1;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int n = 0; n < NT; ++n) {
+    const int64_t col = (n0 + n) * kRows + t;
+    if (col >= c.out) continue;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int64_t row = row0 + 16 * m + 4 * g + r, col = (n0 + n) * kRows + t;
-        if (gridDim.z == 1) store_y<BF>(c, row, col, acc[m][n][r]);
-        else if (row < c.rows && col < c.out) c.partial[(blockIdx.z * c.rows + row) * c.out + col] = acc[m][n][r];
+        const int64_t row = row0 + 16 * m + 4 * g + r;
+        if (row >= c.rows) continue;
+        if (shared) c.partial[(blockIdx.z * c.rows + row) * c.out + col] = acc[m][n][r];
+        else store_y<BF>(c, row, col, acc[m][n][r]);
       }
+  }
 }
 
 // The parts that tile_kernel's workgroups left of each output, in order.
@@ -470,55 +487,80 @@ void few(const LinearCall& c, hipStream_t s) {
                   static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)));
   hipLaunchKernelGGL((few_kernel<BF, kWhole, kGroup, MT, NT, kWaves, kDepth>), grid, dim3(kWaves * kWave), 0, s, c);
 }
-// Tiles of 16 MT rows and 64 NT outputs, and how many workgroups share the
-// inputs of each.
-// Wide tiles read the activations less often, narrow ones are more workgroups;
-// workgroups that share inputs are a second launch. us: 64 x 10240 x 2560 in 80
-// workgroups of (2, 1) tiles that share nothing 64, 40 (4, 1) tiles shared by 12
-// 18, by 6 22; 64 x 2560 x 10240 40 (4, 4) tiles shared by 5 17.8, 80 (4, 2)
-// tiles by 5 21.9; 512 x 2048 x 8192 512 (4, 2) tiles 26.7, 256 (4, 4) tiles 28.3,
-// shared by 2 37.
-constexpr int64_t kMinTiles = 32, kEnoughTiles = 256, kFillTiles = 512, kMinShare = 4;
-struct Tiles {
+// Up to 16 rows run on few_kernel; more on it or on tile_kernel's tiles of 16 MT rows
+// and 64 NT outputs, with the inputs of each shared among several workgroups or not,
+// whichever a linear model of the time, in ns, holds to be fastest. A block of inputs
+// (few_kernel: a wave's) takes `block` and `each` for every workgroup that a compute
+// unit has of the launch; shared inputs a launch more and the parts' way through
+// memory, and the host's second launch and workspace, which kFewLaunch is 1000 lower
+// than its fit for. The numbers are fitted to 1400 timings of 17 to 2048 rows by 768 x 768 to
+// 4096 x 16384 and 768 x 65536 (rms 8% bf16, 7% fp32; few_kernel's 7 to 11%); what
+// the model picks is on average 2.5% (bf16) and 1.3% (fp32) slower than the fastest
+// that was timed. us, model's pick / one tile of (4, 4), fp32 (4, 2), for all, shared
+// among up to 512 workgroups: 256 x 2048 x 8192 15.3 / 25.9, 64 x 2560 x 10240 13.0 /
+// 18.9, 512 x 2048 x 8192 fp32 54 / 70; few_kernel / tiles: 17 x 768 x 768 2.9 / 4.6,
+// 32 x 4096 x 16384 14.8 / 16.4, 64 x 2048 x 2048 9.7 / 7.4.
+struct Tile {
+  int MT, NT;
+  int64_t block, each;
+};
+constexpr Tile kBf16Tiles[] = {{2, 1, 150, 180}, {2, 2, 130, 320}, {2, 4, 350, 460},
+                               {4, 1, 170, 330}, {4, 2, 110, 570}, {4, 4, 840, 740}};
+constexpr Tile kF32Tiles[] = {{2, 1, 240, 560}, {2, 2, 290, 740}, {2, 4, 460, 1280}};
+// few_kernel's `each` is for 16 MT rows; fewer, which are fewer lines to read, take
+// (rows + 20) / (16 MT + 20) of it.
+constexpr Tile kBf16Few[] = {{2, 1, 0, 1860}, {2, 2, 960, 1280}, {2, 4, 0, 3700}, {4, 1, 210, 3390}};
+constexpr Tile kF32Few[] = {{2, 1, 2080, 1920}, {2, 2, 3350, 1700}, {2, 4, 0, 6850}, {4, 1, 340, 7850}};
+constexpr int64_t kFewRows = 16, kFewMost = 64, kFewWaves = 8;
+constexpr int64_t kUnits = 256, kFewLaunch = 1000, kLaunch = 4000, kJoin = 2000, kJoinBytesPerNs = 2400, kMaxSplits = 64;
+struct Plan {
+  bool few;
   int MT, NT, splits;
   int64_t share;   // blocks of inputs of a workgroup
 };
-Tiles plan(int64_t rows, int64_t out, int64_t in, bool bf16) {
-  const int64_t ob = blocks_out(out), ib = blocks_in(in);
-  Tiles t{rows <= 32 ? 2 : 4, bf16 ? 4 : 2, 1, ib};
-  auto count = [&] { return (rows + 16 * t.MT - 1) / (16 * t.MT) * ((ob + 4 * t.NT - 1) / (4 * t.NT)); };
-  while (t.NT > 1 && count() < kMinTiles) t.NT /= 2;
-  if (t.NT == 4 && count() >= kEnoughTiles && count() < kFillTiles) t.NT = 2;
-  const int64_t splits =
-      count() >= kEnoughTiles ? 1 : std::max<int64_t>(1, std::min<int64_t>(kFillTiles / count(), ib / kMinShare));
-  t.share = (ib + splits - 1) / splits;
-  t.splits = static_cast<int>((ib + t.share - 1) / t.share);
-  return t;
-}
-// Whether a call runs on few_kernel, whose workgroups read the rows' activations
-// whole, each for few outputs, but in one launch without a barrier: always up to 16
-// rows; up to 32 while what they read together is small and the chip holds them at
-// once; up to 64 with few inputs and outputs. us, few_kernel / tile_kernel: 17 x 768
-// x 768 3.2 / 5.4, 17 x 2560 x 10240 9.5 / 12.2 (52 MB), 32 x 10240 x 2560 22 / 13.7
-// (105 MB), 32 x 768 x 65536 16.2 / 13.3; 64 x 768 x 3072 5.4 / 8.1, 64 x 3072 x 768
-// 13.2 / 9.5, 64 x 2048 x 2048 9.8 / 9.4, 64 x 768 x 65536 54 / 17.
-constexpr int64_t kFewRows = 16, kFewBytes = int64_t(64) << 20, kFewOutBlocks = 1024;
-constexpr int64_t kWideFewInBlocks = 8, kWideFewOutBlocks = 256;
-int few_columns(int64_t rows, int64_t ob) {   // NT
+int few_columns(int64_t rows, int64_t ob) {   // few_kernel's NT
   if (rows > 32) return 1;
   if (rows > 16) return ob >= 1024 ? 4 : ob >= 512 ? 2 : 1;
   return ob >= 2048 ? 4 : ob >= 512 ? 2 : 1;
 }
-bool runs_few(int64_t rows, int64_t out, int64_t in, bool bf16) {
-  if (rows <= kFewRows) return true;
-  if (rows > 64) return false;
-  const int64_t ob = blocks_out(out), NT = few_columns(rows, ob);
-  if (rows > 32) return ob <= kWideFewOutBlocks && blocks_in(in) <= kWideFewInBlocks;
-  return ob <= kFewOutBlocks && (ob + NT - 1) / NT * 32 * in * (bf16 ? 2 : 4) <= kFewBytes;
+int64_t blocks_ns(const Tile& t, int64_t groups, int64_t blocks) {
+  const int64_t all = groups <= 4 * kUnits ? (groups + kUnits - 1) / kUnits * t.each : groups * t.each / kUnits;
+  return blocks * (t.block + all);
+}
+Plan plan(int64_t rows, int64_t out, int64_t in, bool bf16) {
+  const int64_t ob = blocks_out(out), ib = blocks_in(in);
+  const int NT = few_columns(rows, ob);
+  Plan best{true, rows <= 16 ? 1 : rows <= 32 ? 2 : 4, NT, 1, ib};
+  if (rows <= kFewRows) return best;
+  int64_t least = INT64_MAX;
+  if (rows <= kFewMost) {
+    Tile t = (bf16 ? kBf16Few : kF32Few)[rows > 32 ? 3 : NT / 2];
+    t.each = t.each * (rows + 20) / (16 * t.MT + 20);
+    least = kFewLaunch + blocks_ns(t, (ob + NT - 1) / NT, (ib + kFewWaves - 1) / kFewWaves);
+  }
+  auto consider = [&](const Tile& t, int64_t count, int64_t splits) {
+    const int64_t share = (ib + splits - 1) / splits;
+    splits = (ib + share - 1) / share;
+    int64_t ns = kLaunch + blocks_ns(t, count * splits, share);
+    if (splits > 1) ns += kJoin + splits * rows * out * 4 / kJoinBytesPerNs;
+    if (ns >= least) return;
+    least = ns;
+    best = Plan{false, t.MT, t.NT, static_cast<int>(splits), share};
+  };
+  const Tile* const tiles = bf16 ? kBf16Tiles : kF32Tiles;
+  const int n = bf16 ? std::size(kBf16Tiles) : std::size(kF32Tiles);
+  for (int i = 0; i < n; ++i) {
+    const Tile& t = tiles[i];
+    const int64_t count = (rows + 16 * t.MT - 1) / (16 * t.MT) * ((ob + 4 * t.NT - 1) / (4 * t.NT));
+    consider(t, count, 1);
+    for (int64_t units = kUnits; units <= 4 * kUnits; units += kUnits)   // one to four workgroups a compute unit
+      if (const int64_t splits = std::min({units / count, ib, kMaxSplits}); splits > 1) consider(t, count, splits);
+  }
+  return best;
 }
 
 template <bool BF, bool kWhole, int kGroup, int MT, int NT>
-void tiles(const LinearCall& c, const Tiles& t, hipStream_t s) {
+void tiles(const LinearCall& c, const Plan& t, hipStream_t s) {
   constexpr int cols = kTileWaves * NT;
   const dim3 grid(static_cast<unsigned>((blocks_out(c.out) + cols - 1) / cols),
                   static_cast<unsigned>((c.rows + 16 * MT - 1) / (16 * MT)), t.splits);
@@ -530,37 +572,33 @@ void tiles(const LinearCall& c, const Tiles& t, hipStream_t s) {
 
 template <bool BF, bool kWhole, int kGroup>
 void linear(const LinearCall& c, hipStream_t s) {
-  if (runs_few(c.rows, c.out, c.in, BF)) {
-    const int NT = few_columns(c.rows, blocks_out(c.out));
-    if (c.rows > 32) {
-      few<BF, kWhole, kGroup, 4, 1, 8, 1>(c, s);
-    } else if (c.rows > 16) {
-      if (NT == 4) few<BF, kWhole, kGroup, 2, 4, 8, 1>(c, s);
-      else if (NT == 2) few<BF, kWhole, kGroup, 2, 2, 8, 1>(c, s);
-      else few<BF, kWhole, kGroup, 2, 1, 8, BF ? 2 : 1>(c, s);
-    } else {
-      if (NT == 4) few<BF, kWhole, kGroup, 1, 4, 8, BF ? 2 : 1>(c, s);
-      else if (NT == 2) few<BF, kWhole, kGroup, 1, 2, BF ? 16 : 8, 1>(c, s);
-      else few<BF, kWhole, kGroup, 1, 1, 16, BF ? 2 : 1>(c, s);
+  const Plan t = plan(c.rows, c.out, c.in, BF);
+  if (t.few) {
+    if (t.MT == 4) return few<BF, kWhole, kGroup, 4, 1, 8, 1>(c, s);
+    if (t.MT == 2) {
+      if (t.NT == 4) return few<BF, kWhole, kGroup, 2, 4, 8, 1>(c, s);
+      if (t.NT == 2) return few<BF, kWhole, kGroup, 2, 2, 8, 1>(c, s);
+      return few<BF, kWhole, kGroup, 2, 1, 8, BF ? 2 : 1>(c, s);
     }
-    return;
+    if (t.NT == 4) return few<BF, kWhole, kGroup, 1, 4, 8, BF ? 2 : 1>(c, s);
+    if (t.NT == 2) return few<BF, kWhole, kGroup, 1, 2, BF ? 16 : 8, 1>(c, s);
+    return few<BF, kWhole, kGroup, 1, 1, 16, BF ? 2 : 1>(c, s);
   }
-  const Tiles t = plan(c.rows, c.out, c.in, BF);
-  if (t.MT == 2) {
-    if (t.NT == 1) tiles<BF, kWhole, kGroup, 2, 1>(c, t, s);
-    else if (t.NT == 2) tiles<BF, kWhole, kGroup, 2, 2>(c, t, s);
-    else if constexpr (BF) tiles<BF, kWhole, kGroup, 2, 4>(c, t, s);
-  } else {
-    if (t.NT == 1) tiles<BF, kWhole, kGroup, 4, 1>(c, t, s);
-    else if (t.NT == 2) tiles<BF, kWhole, kGroup, 4, 2>(c, t, s);
-    else if constexpr (BF) tiles<BF, kWhole, kGroup, 4, 4>(c, t, s);
+  if constexpr (BF) {
+    if (t.MT == 4) {
+      if (t.NT == 4) return tiles<BF, kWhole, kGroup, 4, 4>(c, t, s);
+      if (t.NT == 2) return tiles<BF, kWhole, kGroup, 4, 2>(c, t, s);
+      return tiles<BF, kWhole, kGroup, 4, 1>(c, t, s);
+    }
   }
+  if (t.NT == 4) return tiles<BF, kWhole, kGroup, 2, 4>(c, t, s);
+  if (t.NT == 2) return tiles<BF, kWhole, kGroup, 2, 2>(c, t, s);
+  tiles<BF, kWhole, kGroup, 2, 1>(c, t, s);
 }
 
 }  // namespace
 
 int64_t workspace_bytes(int64_t rows, int64_t out, int64_t in, bool bf16) {
-  if (runs_few(rows, out, in, bf16)) return 0;
   const int splits = plan(rows, out, in, bf16).splits;
   return splits == 1 ? 0 : splits * rows * out * 4;
 }

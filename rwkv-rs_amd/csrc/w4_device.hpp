@@ -52,24 +52,31 @@ __device__ __forceinline__ Parts<3> split(const float (&x)[8]) {
   return r;
 }
 
-// the scales of an output's inputs 128 k .., as floats
+// The scales of an output's inputs 128 k .. as they are stored, and one of them as
+// a float. They are loaded apart from their use: a conversion where the load stands
+// waits there, before the loads after it are on their way.
 template <int kGroup>
-__device__ __forceinline__ void load_scales(const void* scales, int64_t at, float (&s)[kInputs / kGroup]) {
-  constexpr int n = kInputs / kGroup;
-  const uint16_t* const p = static_cast<const uint16_t*>(scales) + at * n;
-  if constexpr (n == 1) {
-    s[0] = bf_bits(*p);
-  } else if constexpr (n == 2) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-    s[0] = bf_bits(w & 0xffffu);
-    s[1] = bf_bits(w >> 16);
+struct Scales {
+  static constexpr int kCount = kInputs / kGroup, kWords = (kCount + 1) / 2;
+  uint32_t w[kWords];
+  __device__ __forceinline__ float operator[](int i) const {
+    return __builtin_bit_cast(float, i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+};
+template <int kGroup>
+__device__ __forceinline__ Scales<kGroup> load_scales(const void* scales, int64_t at) {
+  Scales<kGroup> s;
+  const uint16_t* const p = static_cast<const uint16_t*>(scales) + at * Scales<kGroup>::kCount;
+  if constexpr (kGroup == 128) {
+    s.w[0] = *p;
+  } else if constexpr (kGroup == 64) {
+    s.w[0] = *reinterpret_cast<const uint32_t*>(p);
   } else {
     const uint2 w = *reinterpret_cast<const uint2*>(p);
-    s[0] = bf_bits(w.x & 0xffffu);
-    s[1] = bf_bits(w.x >> 16);
-    s[2] = bf_bits(w.y & 0xffffu);
-    s[3] = bf_bits(w.y >> 16);
+    s.w[0] = w.x;
+    s.w[1] = w.y;
   }
+  return s;
 }
 
 }  // namespace rwkv_w4
