@@ -97,9 +97,11 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> To
         raise ValueError(f"top must be 0 to {min(MAX_TOP, vocab)}, got {top}")
     if vocab == 0:
         raise ValueError("the vocabulary is empty")
-    lead = logits.shape[:-1]
+    lead = tokens.shape
     flat = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
-    tokens = tokens.reshape(-1).to(torch.int64).contiguous()
+    if len(lead) != 1:
+        tokens = tokens.reshape(-1)
+    tokens = tokens.to(torch.int64).contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
         out = _TokenScores.apply(flat.contiguous(), tokens, int(top))
     else:
