@@ -38,6 +38,8 @@ MAX_DIM = 4096
 # through the modules 1322, 1332, 1406, 1436, here 418, 433, 695, 1289.
 MAX_DIM_W4 = 8192    # RWKV_DECODE_MAX_DIM
 
+_W4Fields = ctypes.c_int64 * (ctypes.sizeof(_native.DecodeW4Weights) // 8)
+
 
 def _plain(module, cls) -> bool:
     """Exactly ``cls`` (a missing module, None, is not), calling nothing but
@@ -100,19 +102,24 @@ class _Reader:
 def _matrices(p, wp, gr, cm, rd: _Reader, C: int):
     """A cell's six large matrices, into ``p``, or as rwkv_decode_w4_weights
     where they are 4-bit ones of one group size."""
-    of = (("receptance", wp._modules["projection_receptance"], C, C),
-          ("key", wp._modules["projection_key"], C, C),
-          ("value", wp._modules["projection_value"], C, C),
-          ("output", gr._modules["projection_output"], C, C),
-          ("channel_key", cm._modules["key"], C, 4 * C),
-          ("channel_value", cm._modules["value"], 4 * C, C))
-    if type(of[0][1]) is not w4.W4Linear:
-        for name, module, d_in, d_out in of:
-            setattr(p, name, rd.linear(module, d_in, d_out))
+    wsub, csub = wp._modules, cm._modules
+    receptance, output = wsub["projection_receptance"], gr._modules["projection_output"]
+    if type(receptance) is not w4.W4Linear:
+        p.receptance = rd.linear(receptance, C, C)
+        p.key = rd.linear(wsub["projection_key"], C, C)
+        p.value = rd.linear(wsub["projection_value"], C, C)
+        p.output = rd.linear(output, C, C)
+        p.channel_key = rd.linear(csub["key"], C, 4 * C)
+        p.channel_value = rd.linear(csub["value"], 4 * C, C)
         return None
-    group = of[0][1].group_size
-    return _native.DecodeW4Weights(*(rd.packed(module, d_in, d_out, group)
-                                     for _, module, d_in, d_out in of), group)
+    group = receptance.group_size
+    # filled as the thirteen 8-byte fields it is: the structures in it take ctypes longer
+    return _W4Fields(*rd.packed(receptance, C, C, group),
+                     *rd.packed(wsub["projection_key"], C, C, group),
+                     *rd.packed(wsub["projection_value"], C, C, group),
+                     *rd.packed(output, C, C, group),
+                     *rd.packed(csub["key"], C, 4 * C, group),
+                     *rd.packed(csub["value"], 4 * C, C, group), group)
 
 
 def _cell_params(m, cell, rd: _Reader, C: int, H: int):
