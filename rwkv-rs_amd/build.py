@@ -1,5 +1,5 @@
-"""Build libwkv7_hip.so (the gfx950 kernels and their C ABI: include/wkv7.h
-and include/rwkv_neighbors.h) in-tree.
+"""Build libwkv7_hip.so (the gfx950 kernels and their C ABI: the headers in
+include/) in-tree.
 
     python rwkv-rs_amd/build.py          # or __graft_entry__.build()
 
