@@ -317,9 +317,8 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
 // workgroups, join_kernel adds up what they leave. The rows' activations of 128
 // inputs go through LDS in the order in which the waves' matrix instructions read
 // them: piece (row 16 m + t, inputs 32 j + 8 g ..) of 16 bytes at place 16 g + (t ^
-// (4 g + j)) of 64 for (m, j). The exclusive or spreads a row's 16 pieces, which
-// neighbouring threads bring, over all banks. With few_kernel's way of reading
-// activations 512 x 2048 x 8192 took 124 us.
+// spread(g, j)) of 64 for (m, j). With few_kernel's way of reading activations 512 x
+// 2048 x 8192 took 124 us.
 //
 // Loads are two blocks ahead, in registers of their own for odd and even blocks, as
 // they come from memory: activations are asked for once LDS has the ones before,
@@ -328,6 +327,12 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
 // 2048 x 8192 fp32 81 us, now 50; 512 x 8192 x 2048 40, now 31. The last blocks ask
 // for the last one again instead. (4, 4) tiles have registers for one block ahead.
 constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave;
+// Eight neighbouring threads bring pieces (g, j) of one row with all g and two j:
+// their places are to differ modulo 8 (128 bytes a cycle). A read takes 16 lanes a
+// cycle, places 0 to 3 and 12 to 15 of a g and 4 to 11 of the next or the other way
+// round: g and g + 1 are to agree in whether bits 2 and 3 of it differ. (4 g + j gave
+// two-way conflicts in both, half of the LDS's busy cycles.)
+__device__ __forceinline__ int spread(int g, int j) { return 2 * g + (j & 1) + (j >> 1) * 8; }
 template <bool BF, bool kWhole, int kGroup, int MT, int NT>
 __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall c, const int64_t share) {
   constexpr int kParts = BF ? 1 : 3, kSteps = kGroup / 32, kPiecesOfRow = kInputs / 8;
@@ -375,7 +380,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall 
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = tid / kPiecesOfRow + i * (kTileThreads / kPiecesOfRow), j = piece >> 2, q = piece & 3;
-      const int place = (row / 16 * 4 + j) * kWave + 16 * q + ((row & 15) ^ (4 * q + j));
+      const int place = (row / 16 * 4 + j) * kWave + 16 * q + ((row & 15) ^ spread(q, j));
       const Parts<kParts> x = parts<BF>(bring[d][i]);
 #pragma unroll
       for (int p = 0; p < kParts; ++p) at[p][place] = x.p[p];
@@ -390,7 +395,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall 
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int p = 0; p < kParts; ++p) a[m].p[p] = at[p][(m * 4 + j) * kWave + 16 * g + (t ^ (4 * g + j))];
+        for (int p = 0; p < kParts; ++p) a[m].p[p] = at[p][(m * 4 + j) * kWave + 16 * g + (t ^ spread(g, j))];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const bf16x8 v = weights8(word[d][n][j]);
