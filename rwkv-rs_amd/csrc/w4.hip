@@ -10,8 +10,8 @@
 //
 // Up to about 64 rows the weights' bytes bound it: few_kernel, 1 x 4096 x 16384
 // (34 MB) 8.8 us, 8 x 4096 x 65536 28 us (4.8 TB/s, what a copy reaches). Many
-// rows are matrix products: tile_kernel, 512 x 2048 x 8192 24.5 us (700 TFLOP/s),
-// 2048 x 4096 x 4096 75 us (916), a library product of bf16 matrices of 8192^3
+// rows are matrix products: tile_kernel, 512 x 2048 x 8192 22.9 us (750 TFLOP/s),
+// 2048 x 4096 x 4096 62 us (1105), a library product of bf16 matrices of 8192^3
 // 1130.
 #include <algorithm>
 #include <iterator>
@@ -324,8 +324,15 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
 // they come from memory: activations are asked for once LDS has the ones before,
 // weights once the products have. A condition around a load, a conversion at it or a
 // copy of what it brings made the compiler wait for all of them in each block: 512 x
-// 2048 x 8192 fp32 81 us, now 50; 512 x 8192 x 2048 40, now 31. The last blocks ask
+// 2048 x 8192 fp32 81 us, then 50; 512 x 8192 x 2048 40, then 32. The last blocks ask
 // for the last one again instead. (4, 4) tiles have registers for one block ahead.
+// A tile's sums are added to the total while the next tile's products run, which
+// hides the wait for them (128 x 4096 x 4096 15.3, then 13.0; 512 x 2048 x 8192 in
+// groups of 32 29.8, then 27.2), and results are stored by way of LDS, eight outputs
+// a lane (512 x 2048 x 8192 26.4, then 25.0; 2048 x 4096 x 4096 71.5, then 67.4).
+// What is left there is the loop: 1.15 us a block of (4, 2) tiles on two workgroups a
+// compute unit, of which the matrix units are busy for 45%, as in a large library
+// product.
 constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave;
 // Eight neighbouring threads bring pieces (g, j) of one row with all g and two j:
 // their places are to differ modulo 8 (128 bytes a cycle). A read takes 16 lanes a
@@ -335,10 +342,14 @@ constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave;
 __device__ __forceinline__ int spread(int g, int j) { return 2 * g + (j & 1) + (j >> 1) * 8; }
 template <bool BF, bool kWhole, int kGroup, int MT, int NT>
 __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall c, const int64_t share) {
-  constexpr int kParts = BF ? 1 : 3, kSteps = kGroup / 32, kPiecesOfRow = kInputs / 8;
+  constexpr int kParts = BF ? 1 : 3, kSteps = kGroup / 32, kGroups = kInputs / kGroup, kPiecesOfRow = kInputs / 8;
   constexpr int kLoads = 16 * MT * kPiecesOfRow / kTileThreads;   // pieces a thread brings
   constexpr int kAhead = MT * NT > 8 ? 1 : 2;
-  __shared__ bf16x8 xs[2][kParts][MT * 4 * kWave];
+  constexpr int kPitch = 16 * NT + 4;   // of a wave's 16 rows of results: the four that a store writes apart in banks
+  using Blocks = bf16x8[2][kParts][MT * 4 * kWave];
+  using Results = float[kTileWaves][16 * kPitch];
+  __shared__ __attribute__((aligned(16))) char lds[std::max(sizeof(Blocks), sizeof(Results))];
+  Blocks& xs = *reinterpret_cast<Blocks*>(lds);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int t = lane & 15, g = lane >> 4;
   const int64_t ib = blocks_in(c.in), ob = blocks_out(c.out);
@@ -388,24 +399,37 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall 
     __syncthreads();   // the block before is read: its place is written only after the next of these
     load_x(d, min(k + kAhead, k1 - 1));
     __builtin_amdgcn_sched_barrier(0);
-    f32x4 sum[MT][NT];
+    Parts<kParts> a[kSteps][MT];
+    f32x4 before[MT];   // the sums of the tiles and group before, not yet in acc
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      Parts<kParts> a[MT];
+    for (int i = 0; i < kGroups * NT; ++i) {
+      const int q = i / NT, n = i % NT;
+      if (n == 0) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+        for (int e = 0; e < kSteps; ++e)
 #pragma unroll
-        for (int p = 0; p < kParts; ++p) a[m].p[p] = at[p][(m * 4 + j) * kWave + 16 * g + (t ^ spread(g, j))];
+          for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const bf16x8 v = weights8(word[d][n][j]);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          sum[m][n] = multiply(a[m], v, j % kSteps == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[m][n]);
-          if (j % kSteps == kSteps - 1) acc[m][n] += sum[m][n] * s[d][n][32 * j / kGroup];
-        }
+            for (int p = 0; p < kParts; ++p)
+              a[e][m].p[p] = at[p][(m * 4 + q * kSteps + e) * kWave + 16 * g + (t ^ spread(g, q * kSteps + e))];
       }
+      f32x4 sum[MT];
+#pragma unroll
+      for (int e = 0; e < kSteps; ++e) {
+        const bf16x8 v = weights8(word[d][n][q * kSteps + e]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) sum[m] = multiply(a[e][m], v, e == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[m]);
+      }
+      if (i > 0) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m][(i - 1) % NT] += before[m] * s[d][(i - 1) % NT][(i - 1) / NT];
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) before[m] = sum[m];
+      __builtin_amdgcn_sched_barrier(0);
     }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m][NT - 1] += before[m] * s[d][NT - 1][kGroups - 1];
     load_w(d, min(k + kAhead, k1 - 1));
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -419,20 +443,35 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall 
     }
     if (k < k1) step(0, 0, k);
   }
+  // 16 rows of the wave's results at a time go through LDS to be stored in pieces of
+  // eight outputs
   const bool shared = gridDim.z > 1;
+  float* const out = (*reinterpret_cast<Results*>(lds))[wave];
+  __syncthreads();   // all have read the last block
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int64_t col = (n0 + n) * kRows + t;
-    if (col >= c.out) continue;
+  for (int m = 0; m < MT; ++m) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t row = row0 + 16 * m + 4 * g + r;
-        if (row >= c.rows) continue;
-        if (shared) c.partial[(blockIdx.z * c.rows + row) * c.out + col] = acc[m][n][r];
-        else store_y<BF>(c, row, col, acc[m][n][r]);
+      for (int r = 0; r < 4; ++r) out[(4 * g + r) * kPitch + 16 * n + t] = acc[m][n][r];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = lane; i < 32 * NT; i += kWave) {
+      const int at = i % (2 * NT) * 8;
+      const int64_t row = row0 + 16 * m + i / (2 * NT), col = n0 * kRows + at;
+      if (row >= c.rows || col >= c.out) continue;
+      const f32x4* const from = reinterpret_cast<const f32x4*>(out + i / (2 * NT) * kPitch + at);
+      const f32x4 lo = from[0], hi = from[1];
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      if (shared) {
+        store8<false>(c.partial + (blockIdx.z * c.rows + row) * c.out, col, c.out, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= kShrink;
+        store8<BF>(row_at(c.y, row, c.out, BF), col, c.out, v);
       }
+    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -497,21 +536,22 @@ void few(const LinearCall& c, hipStream_t s) {
 // whichever a linear model of the time, in ns, holds to be fastest. A block of inputs
 // (few_kernel: a wave's) takes `block` and `each` for every workgroup that a compute
 // unit has of the launch; shared inputs a launch more and the parts' way through
-// memory, and the host's second launch and workspace, which kFewLaunch is 1000 lower
-// than its fit for. The numbers are fitted to 1400 timings of 17 to 2048 rows by 768 x 768 to
-// 4096 x 16384 and 768 x 65536 (rms 8% bf16, 7% fp32; few_kernel's 7 to 11%); what
-// the model picks is on average 2.5% (bf16) and 1.3% (fp32) slower than the fastest
-// that was timed. us, model's pick / one tile of (4, 4), fp32 (4, 2), for all, shared
-// among up to 512 workgroups: 256 x 2048 x 8192 15.3 / 25.9, 64 x 2560 x 10240 13.0 /
-// 18.9, 512 x 2048 x 8192 fp32 54 / 70; few_kernel / tiles: 17 x 768 x 768 2.9 / 4.6,
-// 32 x 4096 x 16384 14.8 / 16.4, 64 x 2048 x 2048 9.7 / 7.4.
+// memory. The numbers are fitted to 7100 timings of 17 to 2048 rows by 768 x 768 to
+// 4096 x 16384 and 768 x 65536 (rms 9% bf16, 8% fp32; few_kernel's 7 to 11%); the
+// tiles picked are on average 0.9% (bf16) and 1.4% (fp32) slower than the fastest
+// that was timed. kFewLaunch is 1000 lower than its fit, for the second launch and
+// the workspace that few_kernel does not ask the host for. us, model's pick / one
+// tile of (4, 4), fp32 (4, 2), for all, shared among up to 512 workgroups: 256 x 2048
+// x 8192 15 / 26, 64 x 2560 x 10240 12 / 19, 512 x 2048 x 8192 fp32 51 / 70;
+// few_kernel / tiles: 17 x 768 x 768 2.9 / 4.6, 32 x 4096 x 16384 14.8 / 16.4, 64 x
+// 2048 x 2048 9.7 / 7.4.
 struct Tile {
   int MT, NT;
   int64_t block, each;
 };
-constexpr Tile kBf16Tiles[] = {{2, 1, 150, 180}, {2, 2, 130, 320}, {2, 4, 350, 460},
-                               {4, 1, 170, 330}, {4, 2, 110, 570}, {4, 4, 840, 740}};
-constexpr Tile kF32Tiles[] = {{2, 1, 240, 560}, {2, 2, 290, 740}, {2, 4, 460, 1280}};
+constexpr Tile kBf16Tiles[] = {{2, 1, 89, 153}, {2, 2, 136, 259}, {2, 4, 154, 514},
+                               {4, 1, 78, 317}, {4, 2, 86, 537},  {4, 4, 536, 701}};
+constexpr Tile kF32Tiles[] = {{2, 1, 232, 470}, {2, 2, 252, 698}, {2, 4, 373, 1016}};
 // few_kernel's `each` is for 16 MT rows; fewer, which are fewer lines to read, take
 // (rows + 20) / (16 MT + 20) of it.
 constexpr Tile kBf16Few[] = {{2, 1, 0, 1860}, {2, 2, 960, 1280}, {2, 4, 0, 3700}, {4, 1, 210, 3390}};
