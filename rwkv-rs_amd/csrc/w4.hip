@@ -538,24 +538,23 @@ void few(const LinearCall& c, hipStream_t s) {
 // unit has of the launch; shared inputs a launch more and the parts' way through
 // memory. The numbers are fitted to 7100 timings of 17 to 2048 rows by 768 x 768 to
 // 4096 x 16384 and 768 x 65536 (rms 9% bf16, 8% fp32; few_kernel's 7 to 11%); the
-// tiles picked are on average 0.9% (bf16) and 1.4% (fp32) slower than the fastest
-// that was timed. kFewLaunch is 1000 lower than its fit, for the second launch and
-// the workspace that few_kernel does not ask the host for. us, model's pick / one
-// tile of (4, 4), fp32 (4, 2), for all, shared among up to 512 workgroups: 256 x 2048
-// x 8192 15 / 26, 64 x 2560 x 10240 12 / 19, 512 x 2048 x 8192 fp32 51 / 70;
-// few_kernel / tiles: 17 x 768 x 768 2.9 / 4.6, 32 x 4096 x 16384 14.8 / 16.4, 64 x
-// 2048 x 2048 9.7 / 7.4.
+// tiles picked are on average 0.9% (bf16) and 1.4% (fp32) slower than the fastest that
+// was timed, bf16 tiles of (2, 4) and (4, 1) among them. kFewLaunch is 1000 lower than
+// its fit, for the second launch and the workspace that few_kernel does not ask the
+// host for. us, model's pick / one tile of (4, 4), fp32 (4, 2), for all, shared among
+// up to 512 workgroups: 256 x 2048 x 8192 15 / 26, 64 x 2560 x 10240 12 / 19, 512 x
+// 2048 x 8192 fp32 50 / 70; few_kernel / tiles: 17 x 768 x 768 2.9 / 4.6, 17 x 2048 x
+// 8192 5.5 / 9.2, 64 x 2048 x 2048 9.7 / 7.4.
 struct Tile {
   int MT, NT;
   int64_t block, each;
 };
-constexpr Tile kBf16Tiles[] = {{2, 1, 89, 153}, {2, 2, 136, 259}, {2, 4, 154, 514},
-                               {4, 1, 78, 317}, {4, 2, 86, 537},  {4, 4, 536, 701}};
+constexpr Tile kBf16Tiles[] = {{2, 1, 89, 153}, {2, 2, 136, 259}, {4, 2, 86, 537}, {4, 4, 536, 701}};
 constexpr Tile kF32Tiles[] = {{2, 1, 232, 470}, {2, 2, 252, 698}, {2, 4, 373, 1016}};
 // few_kernel's `each` is for 16 MT rows; fewer, which are fewer lines to read, take
 // (rows + 20) / (16 MT + 20) of it.
-constexpr Tile kBf16Few[] = {{2, 1, 0, 1860}, {2, 2, 960, 1280}, {2, 4, 0, 3700}, {4, 1, 210, 3390}};
-constexpr Tile kF32Few[] = {{2, 1, 2080, 1920}, {2, 2, 3350, 1700}, {2, 4, 0, 6850}, {4, 1, 340, 7850}};
+constexpr Tile kBf16Few[] = {{2, 1, 0, 1860}, {2, 2, 960, 1280}, {4, 1, 210, 3390}};
+constexpr Tile kF32Few[] = {{2, 1, 2080, 1920}, {2, 2, 3350, 1700}, {4, 1, 340, 7850}};
 constexpr int64_t kFewRows = 16, kFewMost = 64, kFewWaves = 8;
 constexpr int64_t kUnits = 256, kFewLaunch = 1000, kLaunch = 4000, kJoin = 2000, kJoinBytesPerNs = 2400, kMaxSplits = 64;
 struct Plan {
@@ -565,7 +564,7 @@ struct Plan {
 };
 int few_columns(int64_t rows, int64_t ob) {   // few_kernel's NT
   if (rows > 32) return 1;
-  if (rows > 16) return ob >= 1024 ? 4 : ob >= 512 ? 2 : 1;
+  if (rows > 16) return ob >= 512 ? 2 : 1;
   return ob >= 2048 ? 4 : ob >= 512 ? 2 : 1;
 }
 int64_t blocks_ns(const Tile& t, int64_t groups, int64_t blocks) {
@@ -579,7 +578,7 @@ Plan plan(int64_t rows, int64_t out, int64_t in, bool bf16) {
   if (rows <= kFewRows) return best;
   int64_t least = INT64_MAX;
   if (rows <= kFewMost) {
-    Tile t = (bf16 ? kBf16Few : kF32Few)[rows > 32 ? 3 : NT / 2];
+    Tile t = (bf16 ? kBf16Few : kF32Few)[rows > 32 ? 2 : NT - 1];
     t.each = t.each * (rows + 20) / (16 * t.MT + 20);
     least = kFewLaunch + blocks_ns(t, (ob + NT - 1) / NT, (ib + kFewWaves - 1) / kFewWaves);
   }
@@ -621,7 +620,6 @@ void linear(const LinearCall& c, hipStream_t s) {
   if (t.few) {
     if (t.MT == 4) return few<BF, kWhole, kGroup, 4, 1, 8, 1>(c, s);
     if (t.MT == 2) {
-      if (t.NT == 4) return few<BF, kWhole, kGroup, 2, 4, 8, 1>(c, s);
       if (t.NT == 2) return few<BF, kWhole, kGroup, 2, 2, 8, 1>(c, s);
       return few<BF, kWhole, kGroup, 2, 1, 8, BF ? 2 : 1>(c, s);
     }
@@ -630,13 +628,11 @@ void linear(const LinearCall& c, hipStream_t s) {
     return few<BF, kWhole, kGroup, 1, 1, 16, BF ? 2 : 1>(c, s);
   }
   if constexpr (BF) {
-    if (t.MT == 4) {
-      if (t.NT == 4) return tiles<BF, kWhole, kGroup, 4, 4>(c, t, s);
-      if (t.NT == 2) return tiles<BF, kWhole, kGroup, 4, 2>(c, t, s);
-      return tiles<BF, kWhole, kGroup, 4, 1>(c, t, s);
-    }
+    if (t.NT == 4) return tiles<BF, kWhole, kGroup, 4, 4>(c, t, s);
+    if (t.MT == 4) return tiles<BF, kWhole, kGroup, 4, 2>(c, t, s);
+  } else {
+    if (t.NT == 4) return tiles<BF, kWhole, kGroup, 2, 4>(c, t, s);
   }
-  if (t.NT == 4) return tiles<BF, kWhole, kGroup, 2, 4>(c, t, s);
   if (t.NT == 2) return tiles<BF, kWhole, kGroup, 2, 2>(c, t, s);
   tiles<BF, kWhole, kGroup, 2, 1>(c, t, s);
 }

@@ -106,18 +106,18 @@ def test_quantize_edges():
     assert got[1, 7:14].tolist() == [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0]
 
 
-def check_linear(x, q, d_out, d_in):
+def check_linear(x, q, d_out, d_in, on="cpu"):
     """Against float64 products of the same values. A sum of K products in fp32,
     in any order and however a matrix instruction rounds inside (one unit in the
     last place, 2^-23, for each addition), is off by at most (K + 8) 2^-23 sum
     |x w|; fp32 parts lose 2^-23 |x w| more; the result is rounded once."""
     y = w4.linear(x, q)
     assert y.dtype == x.dtype and y.shape == (*x.shape[:-1], d_out)
-    w = w4.dequantize(q).cpu().double()
-    xd = x.cpu().double()
+    w = w4.dequantize(q).to(on).double()
+    xd = x.to(on).double()
     want, mass = xd @ w.t(), xd.abs() @ w.abs().t()
     last = 2.0 ** -8 if x.dtype == torch.bfloat16 else 2.0 ** -23
-    err = (y.cpu().double() - want).abs()
+    err = (y.to(on).double() - want).abs()
     bound = (d_in + 9) * 2.0 ** -23 * mass + last * want.abs() + 1e-37
     assert (err <= bound).all(), float((err / bound).max())
     # and as a whole far nearer than that bound
@@ -135,6 +135,25 @@ def test_linear(rows, d_out, d_in, group, dtype):
     announce("w4 linear", rows, d_out, d_in, group, dtype)
     q = w4.quantize(rand(d_out, d_in, seed=2, scale=0.05), group)
     check_linear(rand(rows, d_in, seed=3, dtype=dtype), q, d_out, d_in)
+
+
+@pytest.mark.parametrize("dtype,rows,d_out,d_in,group", [
+    # up to 16 rows with one, two and four tiles of outputs a workgroup; up to 64 without a share
+    (torch.bfloat16, 5, 8200, 140, 64), (torch.bfloat16, 3, 32800, 130, 128), (torch.float32, 9, 8200, 140, 32),
+    (torch.float32, 2, 32800, 130, 64), (torch.bfloat16, 18, 8523, 131, 32), (torch.float32, 17, 8828, 543, 64),
+    (torch.float32, 33, 16, 429, 128),
+    # each tile, with an odd and an even number of blocks of inputs, one workgroup a tile or several
+    (torch.bfloat16, 66, 16, 130, 64), (torch.bfloat16, 40, 17, 1256, 128), (torch.bfloat16, 165, 16, 5510, 32),
+    (torch.bfloat16, 65, 18481, 132, 32), (torch.bfloat16, 96, 20443, 128, 64), (torch.bfloat16, 18, 8851, 3844, 64),
+    (torch.bfloat16, 33, 24702, 137, 128), (torch.bfloat16, 52, 25785, 128, 32), (torch.bfloat16, 34, 2906, 4608, 64),
+    (torch.bfloat16, 264, 25527, 130, 64), (torch.bfloat16, 339, 28674, 128, 128), (torch.bfloat16, 339, 28671, 256, 32),
+    (torch.float32, 1474, 32, 648, 64), (torch.float32, 34, 8474, 133, 128), (torch.float32, 19, 23877, 128, 32),
+    (torch.float32, 162, 67, 5532, 32), (torch.float32, 69, 67, 5683, 64), (torch.float32, 17, 33985, 129, 64),
+    (torch.float32, 20, 34947, 128, 128), (torch.float32, 1064, 129, 1325, 128), (torch.float32, 33, 333, 5426, 32)])
+def test_linear_every_form(dtype, rows, d_out, d_in, group):
+    announce("w4 linear form", dtype, rows, d_out, d_in, group)
+    q = w4.quantize(rand(d_out, d_in, seed=31, scale=0.05), group)
+    check_linear(rand(rows, d_in, seed=32, dtype=dtype), q, d_out, d_in, on="cuda")
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
