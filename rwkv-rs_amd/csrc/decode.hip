@@ -397,11 +397,33 @@ hipError_t gemm(GemmArgs& a, hipStream_t s) {
   if (w4 == 0) return gemm<0>(a, s);
   // What more columns a workgroup save is reading the rows again; fewer keep more
   // workgroups. us a step at C = 4096, 3 cells, 1 / 8 / 64 sequences, one tile
-  // everywhere 324, 366, 1189, so 297, 317, 771 (the head on few_kernel or
-  // tile_kernel of w4.hip included).
+  // everywhere 324, 366, 1189, so 297, 317, 771 (before w4_linear took most of the
+  // last).
   const bool wide = a.rows > 32;   // two column tiles at most: 64 KB of sums
   if (w4 >= 1024 && !wide) return gemm<4>(a, s);
   return w4 >= 512 ? gemm<2>(a, s) : gemm<1>(a, s);
+}
+
+// A product with a 4-bit matrix on w4.hip's kernels. Beyond kGemmW4Rows rows, whose
+// activations rows_gemm_kernel's workgroups each read whole, it is the faster way for
+// one in a launch of its own: us a step, 64 sequences, C = 768, 12 cells 907, so 808;
+// C = 2560, 4 cells 739, so 598; C = 8192, 2 cells 1289, so 903. The three that share
+// a launch with the LoRAs stay there: launches of their own took 999, 636 and 826.
+constexpr int kGemmW4Rows = 16;
+hipError_t w4_linear(const rwkv_w4_matrix& w, int64_t group, const void* x, void* y, int rows, int64_t in, int64_t out,
+                     rwkv_w4::Finish finish, hipStream_t s) {
+  rwkv_w4::LinearCall c{};
+  c.x = x;
+  c.packed = w.packed;
+  c.scales = w.scales;
+  c.y = y;
+  c.rows = rows;
+  c.out = out;
+  c.in = in;
+  c.group = static_cast<int>(group);
+  c.bf16 = true;
+  c.finish = finish;
+  return rwkv_w4::launch_linear(c, s);
 }
 
 template <bool kFirst>
@@ -460,6 +482,17 @@ hipError_t launch_cell(const CellCall& c, hipStream_t stream) {
     if (!c.w4) return;
     g.job[g.jobs - 1].scales = static_cast<const uint16_t*>((c.w4->*q).scales);
     g.job[g.jobs - 1].group = (int)c.w4->group;
+  };
+  // one in a launch of its own
+  auto alone = [&](const float* w, rwkv_w4_matrix rwkv_decode_w4_weights::*q, const bf16_t* x, void* out, int64_t K,
+                   int64_t N, int act) {
+    if (c.w4 && R > kGemmW4Rows)
+      return w4_linear(c.w4->*q, c.w4->group, x, out, R, K, N,
+                       act == kResidual ? rwkv_w4::kAddTo : rwkv_w4::kSquaredRelu, stream);
+    g = GemmArgs{};
+    g.rows = R;
+    add_matrix(w, q, x, out, K, N, act);
+    return gemm(g, stream);
   };
   typedef rwkv_decode_w4_weights W4;
   add_matrix(p.receptance, &W4::receptance, mix, rec, C, C, kNone);
@@ -539,10 +572,7 @@ hipError_t launch_cell(const CellCall& c, hipStream_t stream) {
   o.out = read;
   if ((e = rwkv_nb::launch_readout_forward(o, stream)) != hipSuccess) return e;
 
-  g = GemmArgs{};
-  g.rows = R;
-  add_matrix(p.output, &W4::output, read, c.x, C, C, kResidual);
-  if ((e = gemm(g, stream)) != hipSuccess) return e;
+  if ((e = alone(p.output, &W4::output, read, c.x, C, C, kResidual)) != hipSuccess) return e;
 
   // channel mixer
   n.weight = p.norm_channel_weight;
@@ -554,14 +584,8 @@ hipError_t launch_cell(const CellCall& c, hipStream_t stream) {
   n.out[0] = mix;
   if ((e = norm_mix<1>(n, stream)) != hipSuccess) return e;
   bf16_t* const hidden = mix + RC;   // [rows, 4 C]
-  g = GemmArgs{};
-  g.rows = R;
-  add_matrix(p.channel_key, &W4::channel_key, mix, hidden, C, 4 * (int64_t)C, kSquaredRelu);
-  if ((e = gemm(g, stream)) != hipSuccess) return e;
-  g = GemmArgs{};
-  g.rows = R;
-  add_matrix(p.channel_value, &W4::channel_value, hidden, c.x, 4 * (int64_t)C, C, kResidual);
-  return gemm(g, stream);
+  if ((e = alone(p.channel_key, &W4::channel_key, mix, hidden, C, 4 * (int64_t)C, kSquaredRelu)) != hipSuccess) return e;
+  return alone(p.channel_value, &W4::channel_value, hidden, c.x, 4 * (int64_t)C, C, kResidual);
 }
 
 hipError_t launch_head(const HeadCall& c, hipStream_t stream) {
@@ -575,28 +599,12 @@ hipError_t launch_head(const HeadCall& c, hipStream_t stream) {
   n.C = C;
   n.out[0] = static_cast<bf16_t*>(c.workspace);
   if (hipError_t e = norm_mix<0>(n, stream)) return e;
-  if (c.unembed_w4 && rwkv_w4::workspace_bytes(c.rows, c.vocab, C, true) == 0) {
-    rwkv_w4::LinearCall y{};
-    y.x = n.out[0];
-    y.packed = c.unembed_w4->packed;
-    y.scales = c.unembed_w4->scales;
-    y.y = c.logits;
-    y.rows = c.rows;
-    y.out = c.vocab;
-    y.in = C;
-    y.group = c.group;
-    y.bf16 = true;
-    return rwkv_w4::launch_linear(y, stream);
-  }
+  if (c.unembed_w4)
+    return w4_linear(*c.unembed_w4, c.group, n.out[0], c.logits, c.rows, C, c.vocab, rwkv_w4::kStore, stream);
   GemmArgs g{};
   g.rows = c.rows;
   g.jobs = 1;
   g.job[0] = Job{c.unembed, n.out[0], c.logits, C, (int)c.vocab, 0, kNone, false, nullptr, 0};
-  if (c.unembed_w4) {
-    g.job[0].w = static_cast<const float*>(c.unembed_w4->packed);
-    g.job[0].scales = static_cast<const uint16_t*>(c.unembed_w4->scales);
-    g.job[0].group = c.group;
-  }
   return gemm(g, stream);
 }
 

@@ -220,12 +220,43 @@ __device__ __forceinline__ f32x4 multiply(const Parts<kParts>& x, const bf16x8& 
   return sum;
 }
 
+__device__ __forceinline__ float rounded(float v) { return static_cast<float>(static_cast<__bf16>(v)); }
+__device__ __forceinline__ float squared_relu(float v) {
+  v = rounded(v);
+  return v > 0.f ? v * v : v == v ? 0.f : v;   // NaN stays
+}
 template <bool BF>
 __device__ __forceinline__ void store_y(const LinearCall& c, int64_t row, int64_t col, float v) {
   if (row >= c.rows || col >= c.out) return;
   v *= kShrink;
-  if constexpr (BF) static_cast<__bf16*>(c.y)[row * c.out + col] = static_cast<__bf16>(v);
-  else static_cast<float*>(c.y)[row * c.out + col] = v;
+  if constexpr (BF) {
+    if (c.finish == kAddTo) static_cast<float*>(c.y)[row * c.out + col] += rounded(v);
+    else static_cast<__bf16*>(c.y)[row * c.out + col] = static_cast<__bf16>(c.finish == kSquaredRelu ? squared_relu(v) : v);
+  } else {
+    static_cast<float*>(c.y)[row * c.out + col] = v;
+  }
+}
+
+// eight outputs of a row, from the sums before the last multiplication
+template <bool BF>
+__device__ __forceinline__ void store_y8(const LinearCall& c, int64_t row, int64_t col, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= kShrink;
+  if constexpr (BF) {
+    if (c.finish == kAddTo) {
+      void* const to = row_at(c.y, row, c.out, false);
+      const Eight<false> x = load8<false, false>(to, col, c.out);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = x.v[e] + rounded(v[e]);
+      store8<false>(to, col, c.out, v);
+      return;
+    }
+    if (c.finish == kSquaredRelu) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = squared_relu(v[e]);
+    }
+  }
+  store8<BF>(row_at(c.y, row, c.out, BF), col, c.out, v);
 }
 
 // Few rows. A workgroup forms 16 NT outputs of up to 16 MT rows; its waves split
@@ -463,13 +494,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall 
       const f32x4* const from = reinterpret_cast<const f32x4*>(out + i / (2 * NT) * kPitch + at);
       const f32x4 lo = from[0], hi = from[1];
       float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      if (shared) {
-        store8<false>(c.partial + (blockIdx.z * c.rows + row) * c.out, col, c.out, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= kShrink;
-        store8<BF>(row_at(c.y, row, c.out, BF), col, c.out, v);
-      }
+      if (shared) store8<false>(c.partial + (blockIdx.z * c.rows + row) * c.out, col, c.out, v);
+      else store_y8<BF>(c, row, col, v);
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -571,7 +597,7 @@ int64_t blocks_ns(const Tile& t, int64_t groups, int64_t blocks) {
   const int64_t all = groups <= 4 * kUnits ? (groups + kUnits - 1) / kUnits * t.each : groups * t.each / kUnits;
   return blocks * (t.block + all);
 }
-Plan plan(int64_t rows, int64_t out, int64_t in, bool bf16) {
+Plan plan(int64_t rows, int64_t out, int64_t in, bool bf16, bool may_share) {
   const int64_t ob = blocks_out(out), ib = blocks_in(in);
   const int NT = few_columns(rows, ob);
   Plan best{true, rows <= 16 ? 1 : rows <= 32 ? 2 : 4, NT, 1, ib};
@@ -597,6 +623,7 @@ Plan plan(int64_t rows, int64_t out, int64_t in, bool bf16) {
     const Tile& t = tiles[i];
     const int64_t count = (rows + 16 * t.MT - 1) / (16 * t.MT) * ((ob + 4 * t.NT - 1) / (4 * t.NT));
     consider(t, count, 1);
+    if (!may_share) continue;
     for (int64_t units = kUnits; units <= 4 * kUnits; units += kUnits)   // one to four workgroups a compute unit
       if (const int64_t splits = std::min({units / count, ib, kMaxSplits}); splits > 1) consider(t, count, splits);
   }
@@ -616,7 +643,7 @@ void tiles(const LinearCall& c, const Plan& t, hipStream_t s) {
 
 template <bool BF, bool kWhole, int kGroup>
 void linear(const LinearCall& c, hipStream_t s) {
-  const Plan t = plan(c.rows, c.out, c.in, BF);
+  const Plan t = plan(c.rows, c.out, c.in, BF, c.partial != nullptr);
   if (t.few) {
     if (t.MT == 4) return few<BF, kWhole, kGroup, 4, 1, 8, 1>(c, s);
     if (t.MT == 2) {
@@ -640,7 +667,7 @@ void linear(const LinearCall& c, hipStream_t s) {
 }  // namespace
 
 int64_t workspace_bytes(int64_t rows, int64_t out, int64_t in, bool bf16) {
-  const int splits = plan(rows, out, in, bf16).splits;
+  const int splits = plan(rows, out, in, bf16, true).splits;
   return splits == 1 ? 0 : splits * rows * out * 4;
 }
 

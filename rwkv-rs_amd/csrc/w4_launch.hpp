@@ -24,6 +24,9 @@ struct WeightCall {           // quantize: weight to packed and scales; dequanti
   int group;
   bool bf16;
 };
+// What becomes of a product's results, rounded to y's type. The last two take bf16
+// activations; kAddTo's y is the fp32 rows that the results are added to.
+enum Finish { kStore, kSquaredRelu, kAddTo };
 struct LinearCall {
   const void* x;              // [rows, in]
   const void *packed, *scales;
@@ -31,7 +34,8 @@ struct LinearCall {
   int64_t rows, out, in;
   int group;
   bool bf16;
-  float* partial;             // workspace of workspace_bytes, or null where that is 0
+  float* partial;             // workspace of workspace_bytes, or null: no inputs are shared among workgroups
+  Finish finish;              // kStore with a workspace
 };
 
 hipError_t launch_quantize(const WeightCall& c, hipStream_t s);

@@ -35,7 +35,7 @@ MAX_ROWS = 64        # RWKV_DECODE_MAX_ROWS
 # slower; with a context a step, 2157 and more at C = 4096.)
 MAX_DIM = 4096
 # 4-bit weights are an eighth of that. C = 8192, 2 cells, 1 / 8 / 32 / 64 sequences:
-# through the modules 1322, 1332, 1406, 1436, here 418, 433, 695, 1289.
+# through the modules 1322, 1332, 1406, 1436, here 418, 432, 624, 903.
 MAX_DIM_W4 = 8192    # RWKV_DECODE_MAX_DIM
 
 _W4Fields = ctypes.c_int64 * (ctypes.sizeof(_native.DecodeW4Weights) // 8)

@@ -39,6 +39,14 @@ def test_a_fused_step_matches_the_modules(monkeypatch, rows, slots, heads, vocab
         assert x.dtype == y.dtype and _err(x, y) < 1e-2
 
 
+@pytest.mark.parametrize("rows,slots,heads,vocab,group,state_dtype", [
+    (17, 17, 12, 200, 64, torch.bfloat16), (64, 64, 12, 97, 32, torch.bfloat16), (40, 41, 33, 130, 128, torch.bfloat16),
+    (64, 64, 32, 50, 64, torch.float32)])
+def test_a_step_of_wide_cells_matches_the_modules(monkeypatch, rows, slots, heads, vocab, group, state_dtype):
+    # wide enough that the products of more than 16 rows take w4.hip's tiles, with either finish
+    test_a_fused_step_matches_the_modules(monkeypatch, rows, slots, heads, vocab, group, state_dtype)
+
+
 def test_it_is_the_model_whose_weights_they_stand_for():
     # the same weights as fp32 parameters, which the products round to bf16: 2^-9 of
     # each, as much again as the activations' own rounding
