@@ -64,8 +64,10 @@ int64_t rwkv_w4_linear_workspace_bytes(int64_t rows, int64_t out, int64_t in,
 
 /* y [rows, out] = x [rows, in] W^T, x and y in dtype. Products are exact in
  * fp32 (bf16 x) or formed from x's three bf16 parts, which hold it whole (fp32
- * x; parts below 2^-126 are lost); sums are fp32, the scale is applied to a
- * group's sum in fp32, and y is rounded once. */
+ * x; what of it is below 2^-133 is lost); sums are fp32, the scale is applied to
+ * a group's sum in fp32, and y is rounded once. Sums are kept 1024 times too
+ * small, so that none overflows where y does not; a group adds up to 2^-140 to
+ * the error of a y near the least numbers. */
 int rwkv_w4_linear(const void *x, const void *packed, const void *scales,
                    int64_t rows, int64_t out, int64_t in, int64_t group,
                    int dtype, void *y, void *workspace, int64_t workspace_bytes,

@@ -300,3 +300,47 @@ def test_module_and_model():
     w4.quantize_model(model, 64)
     kinds = [type(m) for m in model.modules()]
     assert kinds.count(w4.W4Linear) == 2 * 6 + 1 and nn.Linear not in kinds
+
+
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 20, 100])
+def test_sums_overflow_only_where_the_result_does(rows, dtype, group):
+    """Activations near the largest number, weights so small that the results are
+    ordinary: a group's sum before its scale, and the sum of some groups, are not."""
+    announce("w4 linear near the largest number", rows, dtype, group)
+    d_out, d_in = 40, 512
+    small = w4.quantize(torch.full((d_out, d_in), 1e-3, device="cuda"), group)
+    check_linear(torch.full((rows, d_in), 3e38, device="cuda", dtype=dtype), small, d_out, d_in)
+    two = torch.zeros(rows, d_in, device="cuda", dtype=dtype)
+    two[:, :2] = 3e38
+    check_linear(two, w4.quantize(torch.full((d_out, d_in), 0.06, device="cuda"), group), d_out, d_in)
+    # 256 inputs of either sign: the sum is 0, that of the first half 256 * 0.1 * 3e38;
+    # check_linear's bound on the rounding of sums
+    x = torch.full((rows, d_in), 3e38, device="cuda", dtype=dtype)
+    x[:, d_in // 2:] = -3e38
+    y = w4.linear(x, w4.quantize(torch.full((d_out, d_in), 0.1, device="cuda"), group))
+    assert float(y.double().abs().max()) <= (d_in + 9) * 2.0 ** -23 * d_in * 0.101 * 3e38
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 20, 100])
+def test_the_smallest_activations(rows, dtype):
+    """Scale 1, one activation a row and weight: bf16 ones are exact down to 2^-133,
+    fp32 ones lose what is below that, and a result is a multiple of 2^-139."""
+    announce("w4 linear near the smallest number", rows, dtype)
+    w = torch.zeros(16, 64)
+    w[:, :8] = MAGNITUDES.float()
+    w[:, 40] = 6.0                                                     # of the other group
+    q = w4.quantize(w.cuda(), 32)
+    g = torch.Generator().manual_seed(33)
+    for power in range(-149, -90):
+        x = torch.zeros(rows, 64, dtype=torch.float64)
+        x[torch.arange(rows), torch.arange(rows) % 8] = torch.exp2(torch.rand(rows, generator=g, dtype=torch.float64) + power)
+        x = x.to(dtype)
+        y = w4.linear(x.cuda(), q).cpu().double()
+        want = x.double() @ w.double().t()
+        if dtype == torch.bfloat16:
+            assert torch.equal(y, want.to(dtype).double()), power
+        else:
+            assert ((y - want).abs() <= 6 * 2.0 ** -133 + 2.0 ** -139 + 2.0 ** -23 * want.abs()).all(), power
