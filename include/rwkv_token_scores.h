@@ -17,7 +17,8 @@
  * infinity. A row without a distribution -- every logit minus infinity, or one
  * of them NaN or plus infinity -- gets NaN throughout, and -1 for its ids. A
  * token outside [0, vocab) gets a NaN log probability; the rest of its row is
- * as ever.
+ * as ever. No log probability is above 0 and no entropy below it, by rounding
+ * either.
  *
  * Backward, with g = log_prob_grad[r], h = entropy_grad[r], t_i =
  * top_grad[r][i] (each of the three arrays may be NULL: zeros):

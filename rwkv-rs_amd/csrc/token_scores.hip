@@ -357,7 +357,10 @@ struct Sums {
   Origin o;
   float s, u;
   __device__ __forceinline__ bool valid() const { return fabsf(o.m) < INFINITY && s == s; }
-  __device__ __forceinline__ float log_sum() const { return logf(s) - kLn2 * o.off; }
+  // Neither the log of a sum that holds 1 nor an entropy is negative; what the
+  // exponential and the logarithm round (about 2^-24) may be.
+  __device__ __forceinline__ float log_sum() const { return fmaxf(logf(s) - kLn2 * o.off, 0.f); }
+  __device__ __forceinline__ float entropy() const { return valid() ? fmaxf(logf(s) - kLn2 * (u / s), 0.f) : NAN; }
   __device__ __forceinline__ float log_p(float x, float log_sum) const { return valid() ? (x - o.m) - log_sum : NAN; }
 };
 // terms measured from `from`, from then on from `to`, whose m is no smaller
@@ -372,7 +375,7 @@ template <bool BF>
 __device__ __forceinline__ void write_row(const ForwardCall& c, int64_t row, const Sums& t, float log_sum) {
   const int64_t token = c.tokens[row];
   c.log_prob[row] = token >= 0 && token < c.vocab ? t.log_p(load_one<BF>(c.logits, row * c.vocab + token), log_sum) : NAN;
-  c.entropy[row] = t.valid() ? logf(t.s) - kLn2 * (t.u / t.s) : NAN;
+  c.entropy[row] = t.entropy();
   if (c.row_max) c.row_max[row] = t.o.m;
   if (c.log_sum) c.log_sum[row] = t.valid() ? log_sum : NAN;
 }

@@ -338,3 +338,20 @@ def test_refusals():
                      (lambda: ts.token_scores(x[:, :0], tokens), ValueError)]:
         with pytest.raises(exc):
             bad()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("vocab", [1, 100, 700, 5000, 30000, 65536, 140000])
+def test_signs_of_certain_rows(vocab, dtype):
+    """A token that has all of the probability, or all but a rounding: no log
+    probability above zero, no entropy below it."""
+    announce("token scores of certain rows", vocab, dtype)
+    x, tokens = make(64, vocab, dtype, seed=21)
+    top = torch.linspace(0, 90, 64).to(dtype)
+    x[:, vocab // 2] += top
+    x[:32, :vocab // 2] = -math.inf
+    x[:32, vocab // 2 + 1:] = -math.inf
+    tokens[:] = vocab // 2
+    for k in (0, 1, min(vocab, 33)):
+        out = check(x, tokens, k)
+        assert (out.log_prob <= 0).all() and (out.top_log_probs <= 0).all() and (out.entropy >= 0).all()
