@@ -27,6 +27,7 @@ import ctypes
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -57,6 +58,13 @@ def _stream(device: torch.device) -> int:
     # 1.9 us a call, an eighth of a small launch from Python
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def _no_tangent(t: torch.Tensor, what: str) -> None:
+    """Refuses a dual tensor, for the ways around ``autograd.Function.apply``,
+    which does: its tangent would be dropped, and read as zero."""
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{what} have no forward-mode derivative")
 
 
 def _gpu(t: torch.Tensor, what: str) -> torch.Tensor:

@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .neighbors import _code, _ptr, _stream
+from .neighbors import _code, _no_tangent, _ptr, _stream
 
 MAX_TOP = 64     # RWKV_TOKEN_SCORES_MAX_TOP
 
@@ -97,6 +97,7 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> To
         raise ValueError(f"top must be 0 to {min(MAX_TOP, vocab)}, got {top}")
     if vocab == 0:
         raise ValueError("the vocabulary is empty")
+    _no_tangent(logits, "token scores")
     lead = tokens.shape
     flat = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
     if len(lead) != 1:

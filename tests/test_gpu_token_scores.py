@@ -355,3 +355,25 @@ def test_signs_of_certain_rows(vocab, dtype):
     for k in (0, 1, min(vocab, 33)):
         out = check(x, tokens, k)
         assert (out.log_prob <= 0).all() and (out.top_log_probs <= 0).all() and (out.entropy >= 0).all()
+
+
+def test_forward_mode_is_refused():
+    """Outputs without a tangent would be read as constants."""
+    announce("token scores, forward mode")
+    fw = torch.autograd.forward_ad
+    x, tokens = make(3, 40, torch.float32)
+    x, tokens = x.cuda(), tokens.cuda()
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                ts.token_scores(dual, tokens, 2)
+        with pytest.raises(NotImplementedError):
+            ts.token_scores(dual[0], tokens[0])
+        with pytest.raises(NotImplementedError):
+            ts.token_scores(fw.make_dual(x.clone().requires_grad_(), torch.ones_like(x)), tokens)
+        want = ts.token_scores(x, tokens, 2)                  # no tangent: nothing is lost
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda z: ts.token_scores(z, tokens).log_prob, (x,), (torch.ones_like(x),))
+    for a, b in zip(ts.token_scores(x, tokens, 2), want):
+        assert torch.equal(a, b)
