@@ -11,7 +11,7 @@ as long as their bytes do.
 * ``quantize_model`` a model's projections and unembedding, in place
 
 There are no gradients: the products are for serving, and refuse operands that
-ask for one. Operands live on the GPU; there is no CPU path.
+ask for one or carry a forward-mode tangent. Operands live on the GPU; there is no CPU path.
 """
 
 from __future__ import annotations
@@ -22,7 +22,7 @@ import torch
 import torch.nn as nn
 
 from . import _native
-from .neighbors import _code, _ptr, _stream
+from .neighbors import _code, _no_tangent, _ptr, _stream
 
 GROUPS = (32, 64, 128)
 MAX_DIM = 1 << 26        # RWKV_W4_MAX_DIM
@@ -104,6 +104,7 @@ def linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("products with 4-bit weights have no gradient (use torch.no_grad)")
     code = _code(x.dtype)
+    _no_tangent(x, "products with 4-bit weights")
     x = x.contiguous()
     y = torch.empty(*x.shape[:-1], weight.out_features, dtype=x.dtype, device=dev)
     rows = x.numel() // weight.in_features

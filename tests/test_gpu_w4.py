@@ -344,3 +344,22 @@ def test_the_smallest_activations(rows, dtype):
             assert torch.equal(y, want.to(dtype).double()), power
         else:
             assert ((y - want).abs() <= 6 * 2.0 ** -133 + 2.0 ** -139 + 2.0 ** -23 * want.abs()).all(), power
+
+
+def test_forward_mode_is_refused():
+    """A result without a tangent would be read as a constant."""
+    announce("w4 linear, forward mode")
+    fw = torch.autograd.forward_ad
+    q = w4.quantize(rand(24, 136, seed=34), 64)
+    mod = w4.W4Linear(q)
+    x = rand(2, 136, seed=35)
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda z: w4.linear(z, q), mod):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    call(dual)
+        with torch.autocast("cuda", dtype=torch.bfloat16), pytest.raises(NotImplementedError):
+            mod(dual)
+        want = w4.linear(x, q)                                # no tangent: nothing is lost
+    assert torch.equal(w4.linear(x, q), want)
