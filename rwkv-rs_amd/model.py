@@ -639,8 +639,13 @@ class AutoRegressiveModel(nn.Module):
         the entropy it was taken from and the ``top`` most likely alternatives,
         [batch, T - 1, ..] (``token_scores.token_scores``). The slots advance as
         in ``infer``. Where ``context_mask`` is 0 at a token or at the one before
-        it, its scores mean nothing."""
+        it, its scores mean nothing. Logits of another type than float32 and
+        bfloat16 are scored in float32. What is refused leaves the slots as they
+        were."""
+        _scores.check_top(top, self.vocab_size)      # before the slots advance
         logits = self.infer(contexts, batch_ids, infer_state, context_mask, "full")
+        if logits.dtype not in (torch.float32, torch.bfloat16):
+            logits = logits.float()
         # a row's last logits have no token yet; scored like the others, they are cut off
         tokens = torch.cat([contexts[:, 1:], contexts[:, :1]], dim=1)
         return _scores.TokenScores(*(s[:, :-1] for s in _scores.token_scores(logits, tokens, top)))

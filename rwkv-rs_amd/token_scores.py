@@ -32,6 +32,11 @@ class TokenScores(NamedTuple):
     top_ids: torch.Tensor
 
 
+def check_top(top: int, vocab: int) -> None:
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"top must be 0 to {min(MAX_TOP, vocab)}, got {top}")
+
+
 def _forward(logits, tokens, top, keep):
     """The four outputs and, with ``keep``, what the backward needs of each row."""
     rows, vocab = logits.shape
@@ -93,8 +98,7 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> To
     if tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:
         raise TypeError(f"tokens must be integers, got {tokens.dtype}")
     vocab = logits.shape[-1]
-    if not 0 <= top <= min(MAX_TOP, vocab):
-        raise ValueError(f"top must be 0 to {min(MAX_TOP, vocab)}, got {top}")
+    check_top(top, vocab)
     if vocab == 0:
         raise ValueError("the vocabulary is empty")
     _no_tangent(logits, "token scores")

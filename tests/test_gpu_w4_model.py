@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from conftest import announce, load_pkg
+from model_helpers import tiny_model
 from test_gpu_decode_step import DEV, _err, _infer, _model, _state
 
 pytestmark = pytest.mark.gpu
@@ -146,3 +147,36 @@ def test_scoring_a_text(bits):
         step = model.infer(text[:, -1:], ids, a)
     s = pkg.token_scores.token_scores(step[:, 0], step[:, 0].argmax(1), 3)
     assert torch.equal(s.log_prob, s.top_log_probs[:, 0]) and (s.entropy > 0).all()
+
+
+def _slots(st):
+    return [t.clone() for t in st.state + st.shift_time + st.shift_channel + [st.elapsed_t]]
+
+
+@pytest.mark.parametrize("top", [-1, 65, 98])
+def test_a_refused_score_leaves_the_slots(top):
+    announce("refused score", top)
+    model = _model()
+    st = _state(model, 3, torch.bfloat16, 4)
+    before = _slots(st)
+    text, ids = torch.zeros(2, 5, dtype=torch.long, device=DEV), torch.tensor([2, 0], device=DEV)
+    with torch.autocast("cuda", dtype=torch.bfloat16), pytest.raises(ValueError):
+        model.score(text, ids, st, top=top)
+    assert all(torch.equal(x, y) for x, y in zip(_slots(st), before))
+
+
+def test_scores_under_fp16_autocast():
+    """Logits that the scores do not read are not refused once the slots are advanced."""
+    announce("score, fp16 autocast")
+    model = tiny_model(seed=1, cells=2, heads=2, vocab=97, std=0.2, wkv7_dtype=torch.bfloat16,
+                       neighbor_ops="torch").to(DEV)
+    text = torch.randint(0, 97, (2, 5), generator=torch.Generator().manual_seed(6)).to(DEV)
+    ids = torch.tensor([2, 0], device=DEV)
+    a, b = _state(model, 3, torch.bfloat16, 4), _state(model, 3, torch.bfloat16, 4)
+    with torch.autocast("cuda", dtype=torch.float16):
+        logits = model.infer(text, ids, b, unembed_mode="full")
+        got = model.score(text, ids, a, top=3)
+    assert logits.dtype == torch.float16
+    at = torch.log_softmax(logits.double(), -1)[:, :-1].gather(2, text[:, 1:, None])[..., 0]
+    assert (got.log_prob.double() - at).abs().max() < 1e-5           # log p of up to 8 in fp32, as above
+    assert all(torch.equal(x, y) for x, y in zip(_slots(a), _slots(b)))
