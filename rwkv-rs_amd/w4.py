@@ -162,7 +162,7 @@ def quantize_model(model: nn.Module, group_size: int = 64) -> nn.Module:
         raise ValueError("model must hold the linear layers, not be one")
     done = {}
     for parent in list(model.modules()):
-        for name, child in list(parent.named_children()):
+        for name, child in list(parent._modules.items()):   # named_children() leaves out a child's second name
             if type(child) is nn.Linear and child.bias is None:
                 if child not in done:
                     done[child] = W4Linear.from_linear(child, group_size)

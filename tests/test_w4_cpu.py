@@ -1,0 +1,35 @@
+"""Modules with 4-bit weights without a GPU: what replacing a model's layers and
+moving them between types leaves."""
+
+import pytest
+import torch
+import torch.nn as nn
+
+from conftest import load_pkg
+
+w4 = load_pkg().w4
+
+
+def host_weight(out, d_in, group=64):
+    n, k = -(-out // 16), -(-d_in // 128)
+    g = torch.Generator().manual_seed(out)
+    packed = torch.randint(0, 256, (n, k, 4, 16, 16), generator=g).to(torch.uint8)
+    scales = torch.rand(n, k, 16, 128 // group, generator=g).to(torch.bfloat16)
+    return w4.W4Weight(packed, scales, out, d_in, group)
+
+
+@pytest.fixture
+def quantize_on_the_host(monkeypatch):
+    """Codes and scales that have nothing to do with the weight; nothing computes with them."""
+    monkeypatch.setattr(w4, "quantize", lambda weight, group: host_weight(*weight.shape, group))
+
+
+def test_every_name_of_a_layer_is_replaced(quantize_on_the_host):
+    a, b = nn.Linear(8, 8, bias=False), nn.Linear(8, 4, bias=False)
+    model = nn.Sequential(a, b, a)
+    model.inner = nn.Module()
+    model.inner.first, model.inner.second = b, b
+    w4.quantize_model(model, 64)
+    assert type(model[0]) is type(model[1]) is w4.W4Linear
+    assert model[2] is model[0] and model.inner.first is model.inner.second is model[1]
+    assert not any(isinstance(m, nn.Linear) for m in model.modules())
