@@ -157,14 +157,18 @@ def quantize_model(model: nn.Module, group_size: int = 64) -> nn.Module:
     """Replace every bias-free ``nn.Linear`` of ``model`` (an
     ``AutoRegressiveModel``'s projections, channel mixers and unembedding) by a
     ``W4Linear`` of its weight, in place; the embedding, the LoRAs and the norms
-    stay as they are. Returns the model, which is then for serving only."""
+    stay as they are. Returns the model, which is then for serving only; where a
+    layer is refused (its type, its device), none is replaced."""
     if isinstance(model, nn.Linear):
         raise ValueError("model must hold the linear layers, not be one")
+    places = [(parent, name, child) for parent in list(model.modules())
+              # named_children() leaves out a child's second name
+              for name, child in parent._modules.items()
+              if type(child) is nn.Linear and child.bias is None]
     done = {}
-    for parent in list(model.modules()):
-        for name, child in list(parent._modules.items()):   # named_children() leaves out a child's second name
-            if type(child) is nn.Linear and child.bias is None:
-                if child not in done:
-                    done[child] = W4Linear.from_linear(child, group_size)
-                setattr(parent, name, done[child])
+    for _, _, child in places:   # all of them before the model changes: one may be refused
+        if child not in done:
+            done[child] = W4Linear.from_linear(child, group_size)
+    for parent, name, child in places:
+        setattr(parent, name, done[child])
     return model

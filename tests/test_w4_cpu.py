@@ -33,3 +33,16 @@ def test_every_name_of_a_layer_is_replaced(quantize_on_the_host):
     assert type(model[0]) is type(model[1]) is w4.W4Linear
     assert model[2] is model[0] and model.inner.first is model.inner.second is model[1]
     assert not any(isinstance(m, nn.Linear) for m in model.modules())
+
+
+def test_a_layer_that_cannot_be_quantised_leaves_the_model_whole(monkeypatch):
+    def quantize(weight, group):
+        if weight.dtype != torch.float32:
+            raise TypeError("expected float32 or bfloat16")
+        return host_weight(*weight.shape, group)
+    monkeypatch.setattr(w4, "quantize", quantize)
+    model = nn.Sequential(nn.Linear(8, 8, bias=False), nn.Linear(8, 8, bias=False).half())
+    kept = list(model)
+    with pytest.raises(TypeError):
+        w4.quantize_model(model, 64)
+    assert list(model) == kept
