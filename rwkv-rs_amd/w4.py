@@ -124,7 +124,7 @@ def linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
 class W4Linear(nn.Module):
     """A bias-free linear layer with a 4-bit weight, in the place of an
     ``nn.Linear`` of a model that is served. Under autocast x is cast to
-    autocast's dtype, as ``nn.Linear`` does."""
+    autocast's dtype, as ``nn.Linear`` does. Casting the module leaves its weight."""
 
     def __init__(self, weight: W4Weight):
         super().__init__()
@@ -142,6 +142,17 @@ class W4Linear(nn.Module):
     @property
     def weight(self) -> W4Weight:
         return W4Weight(self.packed, self.scales, self.out_features, self.in_features, self.group_size)
+
+    def _apply(self, fn, recurse=True):
+        # a cast of the model (.float(), .half()) moves the buffers but leaves their
+        # types, which are the format's
+        before = self.packed, self.scales
+        super()._apply(fn, recurse)
+        for name, old in zip(("packed", "scales"), before):
+            new = getattr(self, name)
+            if new.dtype != old.dtype:
+                setattr(self, name, old.to(new.device))
+        return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if torch.is_autocast_enabled(x.device.type):

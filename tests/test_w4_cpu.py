@@ -46,3 +46,27 @@ def test_a_layer_that_cannot_be_quantised_leaves_the_model_whole(monkeypatch):
     with pytest.raises(TypeError):
         w4.quantize_model(model, 64)
     assert list(model) == kept
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.float(), lambda m: m.half(), lambda m: m.double(),
+                                  lambda m: m.bfloat16(), lambda m: m.to(torch.float32), lambda m: m.type(torch.float32),
+                                  lambda m: m.half().float(), lambda m: m.to("cpu")])
+def test_casting_a_model_leaves_the_format(cast):
+    """Scales of up to the largest bf16 number, which fp16 does not hold."""
+    w = host_weight(20, 130, 32)
+    w.scales[0, 0, 0, 0], w.scales[0, 0, 1, 0] = 3e38, 1e-38
+    model = nn.Sequential(nn.Linear(4, 130), w4.W4Linear(w))
+    packed, scales = w.packed.clone(), w.scales.clone()
+    cast(model)
+    got = model[1].weight                                            # W4Weight checks the types
+    assert torch.equal(got.packed, packed) and torch.equal(got.scales, scales)
+    assert set(dict(model[1].named_buffers())) == {"packed", "scales"}
+    assert got.packed.data_ptr() == model[1].packed.data_ptr()
+
+
+def test_a_moved_model_keeps_the_format():
+    model = nn.Sequential(w4.W4Linear(host_weight(20, 130, 32)))
+    model.to("meta", torch.float16)
+    assert model[0].scales.device.type == "meta" and model[0].scales.dtype == torch.bfloat16
+    model.to_empty(device="cpu")
+    assert model[0].weight.scales.shape == (2, 2, 16, 4)
