@@ -343,6 +343,15 @@ __global__ __launch_bounds__(kWaves* kWave) void few_kernel(const LinearCall c) 
   }
 }
 
+// Between a wave's writes to its part of LDS and its lanes' reads of each other's,
+// and before that part is written again. The LDS takes a wave's accesses in order;
+// this keeps the compiler's order.
+__device__ __forceinline__ void wave_exchange() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // Many rows. A workgroup forms 16 MT rows by 64 NT outputs of `share` blocks of
 // inputs, its four waves 16 NT outputs each; where the inputs are shared among
 // workgroups, join_kernel adds up what they leave. The rows' activations of 128
@@ -485,7 +494,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall 
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int r = 0; r < 4; ++r) out[(4 * g + r) * kPitch + 16 * n + t] = acc[m][n][r];
-    __builtin_amdgcn_wave_barrier();
+    wave_exchange();
 #pragma unroll
     for (int i = lane; i < 32 * NT; i += kWave) {
       const int at = i % (2 * NT) * 8;
@@ -497,7 +506,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const LinearCall 
       if (shared) store8<false>(c.partial + (blockIdx.z * c.rows + row) * c.out, col, c.out, v);
       else store_y8<BF>(c, row, col, v);
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_exchange();
   }
 }
 
