@@ -363,3 +363,58 @@ def test_forward_mode_is_refused():
             mod(dual)
         want = w4.linear(x, q)                                # no tangent: nothing is lost
     assert torch.equal(w4.linear(x, q), want)
+
+
+@pytest.mark.parametrize("dtype,rows,d_out,d_in,group", [
+    # five blocks of inputs a workgroup and more, in which LDS and the registers ahead
+    # are used again: an odd and an even number, the inputs shared or not, the last
+    # share as long or shorter, inputs of whole blocks and not
+    (torch.bfloat16, 231, 28672, 640, 64), (torch.bfloat16, 257, 25705, 658, 32), (torch.bfloat16, 2048, 4096, 700, 128),
+    (torch.bfloat16, 34, 16924, 4480, 128), (torch.bfloat16, 33, 16971, 4351, 64), (torch.bfloat16, 36, 16414, 5252, 32),
+    (torch.bfloat16, 33, 16499, 5248, 64), (torch.bfloat16, 35, 26025, 640, 128), (torch.bfloat16, 33, 27730, 642, 32),
+    (torch.bfloat16, 33, 3531, 4736, 64), (torch.bfloat16, 34, 2691, 7379, 128), (torch.bfloat16, 65, 19285, 520, 64),
+    (torch.bfloat16, 17, 8346, 4096, 32), (torch.bfloat16, 17, 5475, 7300, 128), (torch.bfloat16, 1930, 22, 2827, 64),
+    (torch.float32, 38, 16591, 640, 64), (torch.float32, 36, 17074, 658, 128), (torch.float32, 33, 1315, 11285, 32),
+    (torch.float32, 33, 8215, 2048, 128), (torch.float32, 35, 1539, 9600, 64), (torch.float32, 33, 8406, 2204, 32),
+    (torch.float32, 33, 8654, 533, 32), (torch.float32, 34, 8518, 768, 64), (torch.float32, 609, 66, 6413, 128),
+    (torch.float32, 566, 67, 9088, 64), (torch.float32, 489, 65, 8320, 32), (torch.float32, 478, 296, 2069, 64),
+    (torch.float32, 1770, 43, 640, 128)])
+def test_linear_tiles_of_many_blocks(dtype, rows, d_out, d_in, group):
+    announce("w4 linear tiles", dtype, rows, d_out, d_in, group)
+    q = w4.quantize(rand(d_out, d_in, seed=41, scale=0.05), group)
+    check_linear(rand(rows, d_in, seed=42, dtype=dtype), q, d_out, d_in, on="cuda")
+
+
+@pytest.mark.parametrize("dtype,rows,d_out,d_in", [(torch.bfloat16, 575, 17, 7434), (torch.bfloat16, 33, 3531, 4736),
+                                                   (torch.float32, 361, 16, 11520)])
+def test_shared_inputs_on_two_streams_and_in_a_graph(dtype, rows, d_out, d_in):
+    """Products with a workspace: two streams at a time do not share it, and a graph keeps its own."""
+    announce("w4 linear with a workspace, streams and graph", dtype, rows, d_out, d_in)
+    native = pkg._native
+    code = native.DTYPE_BF16 if dtype == torch.bfloat16 else native.DTYPE_F32
+    assert native.lib().rwkv_w4_linear_workspace_bytes(rows, d_out, d_in, code) > 0
+    q = w4.quantize(rand(d_out, d_in, seed=43), 64)
+    xs = [rand(rows, d_in, seed=44 + i, dtype=dtype) for i in range(3)]
+    want = [w4.linear(x, q) for x in xs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(8):
+        for s, x, out in zip(streams, xs, got):
+            with torch.cuda.stream(s):
+                out.append(w4.linear(x, q))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for out, w in zip(got, want):
+        assert all(torch.equal(y, w) for y in out)
+    held = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = w4.linear(held, q)
+    for x, w in zip(xs + xs, want + want):
+        held.copy_(x)
+        assert torch.equal(w4.linear(x, q), w)                        # eager work between the replays
+        graph.replay()
+        assert torch.equal(out, w)
+        torch.cuda.synchronize()
