@@ -138,6 +138,8 @@ def _cell_params(m, cell, rd: _Reader, C: int, H: int):
             or tm.wkv7_dtype != torch.bfloat16 or tm.num_heads != H or tm.head_size != 64
             or wp.num_heads != H):
         raise _Unsupported
+    if C > MAX_DIM and type(wp._modules["projection_receptance"]) is not w4.W4Linear:
+        raise _Unsupported   # fp32 matrices (_matrices): before anything is read and checked in vain
     p = _native.DecodeCellParams()
     p.norm_time_weight, p.norm_time_bias, p.norm_time_eps = rd.norm(
         sub["pre_layer_norm_for_time_mix"], C)
@@ -230,8 +232,6 @@ def step(model, contexts, batch_ids, infer_state, context_mask,
                   rd.tensor(t, (slots, C)), rd.tensor(ch, (slots, C)))
                  for c, s, t, ch in zip(cells, infer_state.state, infer_state.shift_time,
                                         infer_state.shift_channel)]
-        if C > MAX_DIM and not all(c[0][1] for c in calls):
-            return None
         if calls[0][0][0].residual_a or not all(c[0][0].residual_a for c in calls[1:]):
             return None   # the first cell is the one without a value residual
         head = None

@@ -368,3 +368,26 @@ def test_a_captured_step_replays_and_streams_do_not_share():
                 got[i].append(_infer(model, toks, ids, sts[i]))
     torch.cuda.synchronize()
     assert all(torch.equal(x, want) for g in got for x in g)
+
+
+def test_a_model_too_wide_is_left_before_its_parameters_are_read(monkeypatch):
+    """It runs through the modules; what a step reads and checks of it first is lost."""
+    announce("decode step, too wide a model")
+    pkg = load_pkg()
+    read = []
+    real = pkg.decode._Reader.tensor
+    monkeypatch.setattr(pkg.decode._Reader, "tensor", lambda *a: read.append(1) or real(*a))
+    monkeypatch.setattr(pkg.decode, "MAX_DIM", 64)
+    model = _model()
+    st = _state(model, 2, torch.bfloat16, 1)
+    ids, toks = torch.arange(2, device=DEV), torch.zeros(2, 1, dtype=torch.long, device=DEV)
+
+    def taken():
+        read.clear()
+        with torch.autocast("cuda", dtype=torch.bfloat16), torch.no_grad():
+            return pkg.decode.step(model, toks, ids, st, None, "last") is not None
+    assert not taken() and not read
+    pkg.w4.quantize_model(model)
+    assert taken() and read                                   # 4-bit cells go further
+    model.cells.cells[1] = _model().cells.cells[1]
+    assert not taken()                                        # one cell of fp32 weights
