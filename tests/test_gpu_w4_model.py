@@ -6,7 +6,7 @@ import torch
 
 from conftest import announce, load_pkg
 from model_helpers import tiny_model
-from test_gpu_decode_step import DEV, _err, _infer, _model, _state
+from test_gpu_decode_step import DEV, _err, _infer, _model, _state, _wide_model
 
 pytestmark = pytest.mark.gpu
 
@@ -180,3 +180,32 @@ def test_scores_under_fp16_autocast():
     at = torch.log_softmax(logits.double(), -1)[:, :-1].gather(2, text[:, 1:, None])[..., 0]
     assert (got.log_prob.double() - at).abs().max() < 1e-5           # log p of up to 8 in fp32, as above
     assert all(torch.equal(x, y) for x, y in zip(_slots(a), _slots(b)))
+
+
+@pytest.mark.parametrize("rows,heads,group,state_dtype", [
+    # (row tiles, column tiles) of the launch that receptance, key and value share: from
+    # C = 2752 on two column tiles, from 5504 four, beyond 32 rows two; up to 16
+    # sequences the channel mixer's key has two from C = 2048 on and four from 4096
+    (1, 32, 64, torch.bfloat16), (8, 43, 32, torch.bfloat16), (16, 64, 128, torch.float32), (1, 85, 64, torch.bfloat16),
+    (16, 86, 32, torch.bfloat16), (8, 87, 128, torch.bfloat16), (1, 128, 64, torch.bfloat16),
+    (17, 43, 128, torch.bfloat16), (32, 64, 32, torch.float32), (17, 86, 64, torch.bfloat16), (32, 87, 32, torch.bfloat16),
+    (33, 43, 64, torch.bfloat16), (40, 64, 128, torch.bfloat16), (64, 87, 32, torch.bfloat16),
+    # the other products on w4.hip's two column tiles of up to 32 rows, and its tiles of 64 rows
+    (17, 128, 32, torch.bfloat16), (64, 128, 128, torch.bfloat16)])
+def test_a_step_with_several_column_tiles_matches_the_modules(monkeypatch, rows, heads, group, state_dtype):
+    announce("4-bit decode step, column tiles", rows, heads, group, str(state_dtype))
+    tiles = 3 * heads * 64 // 16, 4 * heads * 64 // 16
+    assert tiles[0] >= 512 or rows <= 16 and tiles[1] >= 512      # what a launch has to have for two of them
+    pkg = load_pkg()
+    model = pkg.w4.quantize_model(_wide_model(heads), group)
+    ids, toks = torch.arange(rows, device=DEV), torch.arange(rows, device=DEV).reshape(rows, 1) % 33
+    a, b = _state(model, rows, state_dtype, 7), _state(model, rows, state_dtype, 7)
+    taken = []
+    real = pkg.decode.step
+    monkeypatch.setattr(pkg.decode, "step", lambda *x: taken.append(real(*x)) or taken[-1])
+    got = _infer(model, toks, ids, a)
+    monkeypatch.setattr(pkg.decode, "step", lambda *x: None)
+    want = _infer(model, toks, ids, b)
+    assert taken[0] is not None and _err(got, want) < 1e-2
+    for x, y in zip(a.state + a.shift_time + a.shift_channel, b.state + b.shift_time + b.shift_channel):
+        assert _err(x, y) < 1e-2
