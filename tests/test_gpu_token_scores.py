@@ -377,3 +377,32 @@ def test_forward_mode_is_refused():
         torch.func.jvp(lambda z: ts.token_scores(z, tokens).log_prob, (x,), (torch.ones_like(x),))
     for a, b in zip(ts.token_scores(x, tokens, 2), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("rows,vocab,top", [(513, 65536, 20), (520, 33000, 32), (513, 70001, 5), (300, 70001, 0)])
+def test_many_long_rows(rows, vocab, top, dtype):
+    """Rows of several chunks of 32768 (bf16, more than 512 rows, up to 32
+    alternatives) or other sizes, masked in one chunk, in all but one and in all."""
+    announce("token scores, many long rows", rows, vocab, top, dtype)
+    x, tokens = make(rows, vocab, dtype, seed=23)
+    chunk, left = 32768, max(top // 2, 1)
+    last = (vocab - 1) // chunk * chunk
+    x[0, :chunk - left] = -math.inf                      # the first chunk has fewer than `top`
+    x[1, :chunk] = -math.inf                             # or none
+    x[2, last + left:] = -math.inf                       # so has the last
+    x[3, last:] = -math.inf
+    x[4, left:] = -math.inf                              # the row has, in its first chunk
+    x[5, :vocab - left] = -math.inf                      # in its last
+    x[6, 1:vocab - 1] = -math.inf                        # one at each end
+    x[7] = -math.inf
+    x[8, :chunk] = LOWEST[dtype]                         # far below what follows
+    x[9, last:] += 300.0                                 # all of the mass is in the last chunk
+    x[10, :chunk] += 300.0                               # in the first
+    x[11] = 0.75
+    x[12, chunk - 1], x[12, chunk] = 50.0, 50.0          # equal ones on both sides
+    x[13, vocab - 1] = math.nan
+    x[14, 0] = math.inf
+    x[rows - 1] = torch.sort(x[rows - 1].float()).values.to(dtype)
+    tokens[2], tokens[4], tokens[5] = vocab - 1, 0, vocab - 1
+    check(x, tokens, top)
