@@ -8,11 +8,13 @@
 // rounded to bf16 would be one operation less for each four products and 2^-9
 // off each.) An fp32 activation is three bf16 parts that hold all of it.
 //
-// Up to about 64 rows the weights' bytes bound it: few_kernel, 1 x 4096 x 16384
-// (34 MB) 8.8 us, 8 x 4096 x 65536 28 us (4.8 TB/s, what a copy reaches). Many
-// rows are matrix products: tile_kernel, 512 x 2048 x 8192 22.9 us (750 TFLOP/s),
-// 2048 x 4096 x 4096 62 us (1105), a library product of bf16 matrices of 8192^3
-// 1130.
+// The weights' bytes bound it for up to 8 rows of a wide matrix: few_kernel, 1 x 4096
+// x 16384 (34 MB) 8.6 us, 8 x 4096 x 65536 28 us (4.8 TB/s, what a copy reaches). More
+// rows, up to 64, wait for their activations, which every workgroup reads: 12 x 10240 x
+// 2560 11.0 us (1.3 TB/s of weights), 64 x 4096 x 16384 17.1 (2.1). Many rows are
+// matrix products: tile_kernel, 512 x 2048 x 8192 22.9 us (750 TFLOP/s), 2048 x 4096 x
+// 4096 62 to 69 us (1105 to 1000; groups of 64), a library product of bf16 matrices of
+// 8192^3 1130 to 1400.
 #include <algorithm>
 #include <iterator>
 

@@ -3,7 +3,8 @@ include/rwkv_token_scores.h: the log probability of given tokens, the entropy
 and the most likely alternatives of each row of logits, as one torch autograd
 Function. All three have a gradient: of the log probability for training on
 sampled answers, of the entropy for keeping them varied, of the alternatives'
-log probabilities for learning from a teacher's.
+log probabilities for learning from a teacher's. There is no second derivative and
+no forward mode.
 
 The forward reads the logits once, in their dtype, and keeps three numbers a row;
 the backward reads them once more and writes their gradient once. Operands live
