@@ -1,0 +1,77 @@
+/*
+ * rwkv_linear_loss.h -- C ABI of the language model's training loss straight
+ * from its last hidden states and its unembedding, on gfx950: the cross entropy
+ * with l2wrap's gradient term of rwkv_lm_loss.h, of logits that are formed in
+ * tiles and never stored. Statuses, dtype codes and threading rules are wkv7.h's.
+ * No counterpart in the reference, which forms the logits (model.rs:150-169).
+ *
+ * hidden [rows, c], weight [vocab, c] row-major in dtype, targets int64 [rows].
+ *
+ * Forward:
+ *   z_rj   = sum_k hidden_rk weight_jk      (exact products, fp32 sums)
+ *   lse_r  = log sum_j exp(z_rj)
+ *   loss_r = lse_r - z_r,t_r
+ * to row_loss, row_lse, row_max (fp32 [rows]) and row_argmax (int32 [rows], the
+ * first index of the row's maximum); the last three are kept for the backward. A
+ * row whose target is ignore_index has loss 0; one whose target is otherwise
+ * outside [0, vocab) a NaN loss. A row with a NaN or an infinite logit has a NaN
+ * loss too.
+ *
+ * Backward, with g_r = row_loss_grad[r] (fp32 [rows]):
+ *   D_rj = g_r (exp(z_rj - lse_r) - [j == t_r]) + [j == argmax_r] l2wrap_scale max_r
+ *   hidden_grad = D weight,   weight_grad = D^T hidden
+ * in dtype, each rounded once; either pointer may be NULL (not wanted). A row
+ * whose target is ignore_index has D = 0; a target otherwise outside [0, vocab)
+ * no target term. z is formed again, a piece of the vocabulary at a time. D over
+ * the call's largest |g_r| or |l2wrap_scale max_r| is rounded to bf16 for bf16
+ * operands (half a step, 2^-9, of each D_rj) and held in two fp16 numbers (22 bits)
+ * for fp32 ones.
+ *
+ * fp32 operands are multiplied as two fp16 numbers each, after a power of two that
+ * brings the operand's largest magnitude to 2^13 .. 2^14: 22 bits of each element, but
+ * never finer than 2^-38 of that largest magnitude, three products, fp32 sums.
+ *
+ * Operands are aligned to their elements, and where c is a multiple of 8, hidden,
+ * weight and their gradients to 16 bytes. What a call writes may not overlap
+ * anything else that it is given.
+ */
+#ifndef RWKV_RS_AMD_LINEAR_LOSS_H
+#define RWKV_RS_AMD_LINEAR_LOSS_H
+
+#include "wkv7.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* The most of each size. */
+#define RWKV_LINEAR_LOSS_MAX_ROWS (1 << 22)
+#define RWKV_LINEAR_LOSS_MAX_VOCAB (1 << 22)
+#define RWKV_LINEAR_LOSS_MAX_C (1 << 16)
+
+/* Device memory that a call asks for (16-byte aligned, no initialisation; calls
+ * that may overlap in time need one each), or -1 for sizes or a dtype that are not
+ * supported. */
+int64_t rwkv_linear_loss_forward_workspace_bytes(int64_t rows, int64_t vocab, int64_t c, int dtype);
+int64_t rwkv_linear_loss_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t c, int dtype);
+
+int rwkv_linear_loss_forward(const void *hidden, const void *weight, const int64_t *targets,
+                             int64_t rows, int64_t vocab, int64_t c, int dtype,
+                             int64_t ignore_index, float *row_loss, float *row_lse,
+                             float *row_max, int32_t *row_argmax, void *workspace,
+                             int64_t workspace_bytes, void *stream);
+
+/* row_lse, row_max and row_argmax are the forward's of the same operands. */
+int rwkv_linear_loss_backward(const void *hidden, const void *weight, const int64_t *targets,
+                              const float *row_lse, const float *row_max,
+                              const int32_t *row_argmax, const float *row_loss_grad,
+                              float l2wrap_scale, int64_t rows, int64_t vocab, int64_t c,
+                              int dtype, int64_t ignore_index, void *hidden_grad,
+                              void *weight_grad, void *workspace, int64_t workspace_bytes,
+                              void *stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* RWKV_RS_AMD_LINEAR_LOSS_H */

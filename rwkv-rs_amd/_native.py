@@ -91,6 +91,11 @@ W4_EXPORTS = ("rwkv_w4_packed_bytes", "rwkv_w4_scales_bytes", "rwkv_w4_quantize"
 DECODE_W4_EXPORTS = ("rwkv_decode_cell_w4", "rwkv_decode_head_w4")
 SCORES_EXPORTS = ("rwkv_token_scores_forward", "rwkv_token_scores_backward")
 
+# and of include/rwkv_linear_loss.h
+LINEAR_LOSS_EXPORTS = ("rwkv_linear_loss_forward_workspace_bytes",
+                       "rwkv_linear_loss_backward_workspace_bytes",
+                       "rwkv_linear_loss_forward", "rwkv_linear_loss_backward")
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
@@ -148,6 +153,11 @@ _SIGNATURES = {
     "rwkv_w4_linear": ([_P] * 3 + [_I64] * 4 + [_INT] + [_P] * 2 + [_I64, _P], _INT),
     "rwkv_token_scores_forward": ([_P] * 2 + [_I64] * 3 + [_INT] + [_P] * 7, _INT),
     "rwkv_token_scores_backward": ([_P] * 9 + [_I64] * 3 + [_INT] + [_P] * 2, _INT),
+    "rwkv_linear_loss_forward_workspace_bytes": ([_I64] * 3 + [_INT], _I64),
+    "rwkv_linear_loss_backward_workspace_bytes": ([_I64] * 3 + [_INT], _I64),
+    "rwkv_linear_loss_forward": ([_P] * 3 + [_I64] * 3 + [_INT, _I64] + [_P] * 5 + [_I64, _P], _INT),
+    "rwkv_linear_loss_backward": ([_P] * 7 + [ctypes.c_float] + [_I64] * 3 + [_INT, _I64]
+                                  + [_P] * 3 + [_I64, _P], _INT),
 }
 
 _lib = None

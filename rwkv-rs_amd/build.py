@@ -23,7 +23,8 @@ SOURCES = ["wkv7_api.cpp", "wkv7_forward.hip", "wkv7_backward.hip", "wkv7_infer.
            "wkv7_chunk_forward.hip", "wkv7_chunk_backward.hip", "wkv7_f32_chunk.hip", "wkv7_segment.hip",
            "wkv7_selftest.hip",
            "neighbors_api.cpp", "neighbors.hip", "lm_loss_api.cpp", "lm_loss.hip",
-           "decode_api.cpp", "decode.hip", "w4_api.cpp", "w4.hip", "token_scores_api.cpp", "token_scores.hip"]
+           "decode_api.cpp", "decode.hip", "w4_api.cpp", "w4.hip", "token_scores_api.cpp", "token_scores.hip",
+           "linear_loss_api.cpp", "linear_loss.hip"]
 ARCH = "gfx950"
 
 

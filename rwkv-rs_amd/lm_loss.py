@@ -9,16 +9,22 @@ writes the logits' gradient once, with l2wrap's term (kernels/l2wrap/mod.rs:
 38-66: 1e-4 / num_tokens * max(logits) at each row's argmax) folded in. The
 logits stay in their dtype (bf16 under autocast) instead of being cast to
 fp32. Operands live on the GPU; there is no CPU path.
+
+``linear_cross_entropy_l2wrap`` is the same loss straight from the last hidden
+states and the unembedding (include/rwkv_linear_loss.h): the logits are formed in
+tiles, twice, and neither they nor their gradient are ever whole in memory.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
-from .neighbors import _code, _ptr, _stream
+from .neighbors import _code, _no_tangent, _ptr, _stream
 
 L2WRAP_FACTOR = 1e-4     # kernels/l2wrap/mod.rs:61-62
+IGNORE_INDEX = -100      # a target that is not learned, as torch's cross entropy has it
 
 
 class _CrossEntropyL2Wrap(torch.autograd.Function):
@@ -64,3 +70,91 @@ def cross_entropy_l2wrap(logits: torch.Tensor, targets: torch.Tensor) -> torch.T
     """``F.cross_entropy(l2wrap(logits, rows), targets)``: the mean over the
     rows, l2wrap counting every row as a token (model.rs:161-169)."""
     return cross_entropy_l2wrap_rows(logits, targets, logits.shape[0]).mean()
+
+
+# ------------------------------------------- from hidden states and unembedding
+def _workspace(which: str, rows: int, vocab: int, c: int, code: int, device) -> tuple:
+    nbytes = getattr(_native.lib(), f"rwkv_linear_loss_{which}_workspace_bytes")(rows, vocab, c, code)
+    if nbytes < 0:
+        raise ValueError(f"hidden [{rows}, {c}] and weight [{vocab}, {c}] are not supported")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+
+
+def _linear_forward(hidden, weight, targets, ignore_index):
+    """Loss, log-sum-exp, maximum and argmax of every row."""
+    (rows, c), vocab, dev = hidden.shape, weight.shape[0], hidden.device
+    code = _code(hidden.dtype)
+    loss, lse, mx = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(3))
+    arg = torch.empty(rows, dtype=torch.int32, device=dev)
+    ws, nbytes = _workspace("forward", rows, vocab, c, code, dev)
+    _native.call("rwkv_linear_loss_forward", _ptr(hidden), _ptr(weight), _ptr(targets), rows, vocab, c,
+                 code, ignore_index, _ptr(loss), _ptr(lse), _ptr(mx), _ptr(arg), _ptr(ws), nbytes,
+                 _stream(dev))
+    return loss, lse, mx, arg
+
+
+class _LinearCrossEntropyL2Wrap(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, num_tokens, ignore_index):
+        loss, lse, mx, arg = _linear_forward(hidden, weight, targets, ignore_index)
+        ctx.save_for_backward(hidden, weight, targets, lse, mx, arg)
+        ctx.scale = L2WRAP_FACTOR / num_tokens if num_tokens > 0 else 0.0
+        ctx.ignore_index = ignore_index
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        hidden, weight, targets, lse, mx, arg = ctx.saved_tensors
+        (rows, c), vocab, dev = hidden.shape, weight.shape[0], hidden.device
+        code = _code(hidden.dtype)
+        g = dloss.to(torch.float32).contiguous()
+        dhidden, dweight = (torch.empty_like(t) if need else None
+                            for t, need in zip((hidden, weight), ctx.needs_input_grad))
+        ws, nbytes = _workspace("backward", rows, vocab, c, code, dev)
+        _native.call("rwkv_linear_loss_backward", _ptr(hidden), _ptr(weight), _ptr(targets), _ptr(lse),
+                     _ptr(mx), _ptr(arg), _ptr(g), ctx.scale, rows, vocab, c, code, ctx.ignore_index,
+                     _ptr(dhidden), _ptr(dweight), _ptr(ws), nbytes, _stream(dev))
+        return dhidden, dweight, None, None, None
+
+
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def linear_cross_entropy_l2wrap_rows(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                                     num_tokens: int, ignore_index: int = IGNORE_INDEX) -> torch.Tensor:
+    """``cross_entropy_l2wrap_rows(hidden @ weight.T, targets, num_tokens)`` without
+    the logits: ``hidden`` [rows, c] and ``weight`` [vocab, c] are both float32 or both
+    bfloat16, and differentiable once, in reverse mode. Logits are not rounded on the
+    way. A row whose target is ``ignore_index`` has loss 0 and no gradient; one whose target is
+    otherwise outside [0, vocab) a NaN loss."""
+    if not hidden.is_cuda or weight.device != hidden.device or targets.device != hidden.device:
+        raise ValueError("hidden, weight and targets must be on the same GPU")
+    if hidden.dim() != 2 or weight.dim() != 2 or weight.shape[1] != hidden.shape[1] \
+            or targets.shape != hidden.shape[:1]:
+        raise ValueError("hidden must be [rows, c], weight [vocab, c] and targets [rows]")
+    if 0 in weight.shape:
+        raise ValueError("the vocabulary or the hidden states are empty")
+    if weight.dtype != hidden.dtype:
+        raise TypeError(f"hidden and weight must have one dtype, got {hidden.dtype} and {weight.dtype}")
+    if targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool:
+        raise TypeError(f"targets must be integers, got {targets.dtype}")
+    _code(hidden.dtype)
+    for t in (hidden, weight):
+        _no_tangent(t, "losses from hidden states")
+    hidden, weight = _operand(hidden), _operand(weight)
+    targets = targets.to(torch.int64).contiguous()
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _LinearCrossEntropyL2Wrap.apply(hidden, weight, targets, int(num_tokens), int(ignore_index))
+    return _linear_forward(hidden, weight, targets, int(ignore_index))[0]
+
+
+def linear_cross_entropy_l2wrap(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                                ignore_index: int = IGNORE_INDEX) -> torch.Tensor:
+    """``cross_entropy_l2wrap(hidden @ weight.T, targets)`` without the logits: the
+    mean over the rows that are not ignored (0 when all are), l2wrap counting every
+    row as a token."""
+    rows = linear_cross_entropy_l2wrap_rows(hidden, weight, targets, hidden.shape[0], ignore_index)
+    return rows.sum() / (targets != ignore_index).sum().clamp(min=1)
