@@ -27,8 +27,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWords = 256, kRowsTile = 128;   // a tile of logits
-constexpr int kWavesP = 2, kWavesQ = 2, kThreads = 256;
+constexpr int kWords = 256, kRowsTile = 256;   // a tile of logits
+constexpr int kWavesP = 2, kWavesQ = 4, kThreads = 512;
 constexpr int kUnits = 256;                    // compute units
 constexpr int kXcds = 8;
 constexpr int kMaxBlocks = 256;                // of a maximum over an operand
@@ -52,9 +52,9 @@ struct Scalars {
 
 // Consecutive workgroups go to the eight XCDs in turn: give each XCD a run of
 // consecutive tiles, which read the same operands, for its L2.
-__device__ __forceinline__ int64_t tile_of_block(int64_t blocks, int64_t block) {
-  const int64_t whole = blocks / kXcds, rest = blocks % kXcds, x = block % kXcds;
-  return x * whole + min(x, rest) + block / kXcds;
+__device__ __forceinline__ int tile_of_block() {
+  const int blocks = gridDim.x, block = blockIdx.x, x = block % kXcds;
+  return x * (blocks / kXcds) + min(x, blocks % kXcds) + block / kXcds;
 }
 
 // ------------------------------------------------------------- operands as planes
@@ -121,8 +121,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
 // ------------------------------------------------------------------------- logits
 struct LogitsCall {
   Matrix x, w;
-  int64_t rows, vocab, steps;    // steps: c up to a whole step
-  int64_t first, words;          // the piece of the vocabulary, whole tiles
+  int rows, vocab, steps;        // steps: c up to a whole step
+  int first, words;              // the piece of the vocabulary, whole tiles
   const Scalars* scalars;
   const int64_t* targets;
   int64_t ignore_index;
@@ -138,27 +138,27 @@ struct LogitsCall {
 };
 
 // A run of words whose rows of w stay in an XCD's L2 while the rows of x pass by.
-constexpr int64_t kWordTiles = 8;
+constexpr int kWordTiles = 8;
 template <bool BF>
-using LogitsTile = Tile<kRows, kRows, kWords, kRowsTile, kWavesP, kWavesQ, true, BF ? 1 : 2>;
+using LogitsTile = Tile<kRows, kRows, kWords, kRowsTile, kWavesP, kWavesQ, true, true, BF ? 1 : 2>;
 
 template <bool BF, bool kBackward>
 __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c) {
   using T = LogitsTile<BF>;
   __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
-  const int64_t row_tiles = ceil_div(c.rows, kRowsTile), word_tiles = c.words / kWords;
-  const int64_t at = tile_of_block(gridDim.x, blockIdx.x);
-  const int64_t run = at / (kWordTiles * row_tiles), in_run = at % (kWordTiles * row_tiles);
-  const int64_t run_words = min(kWordTiles, word_tiles - run * kWordTiles);
-  const int64_t word_tile = run * kWordTiles + in_run % run_words, row_tile = in_run / run_words;
-  const int64_t v0 = c.first + word_tile * kWords, r0 = row_tile * kRowsTile;
+  const int row_tiles = (c.rows + kRowsTile - 1) / kRowsTile, word_tiles = c.words / kWords;
+  const int at = tile_of_block();
+  const int run = at / (kWordTiles * row_tiles), in_run = at % (kWordTiles * row_tiles);
+  const int run_words = min(kWordTiles, word_tiles - run * kWordTiles);
+  const int word_tile = run * kWordTiles + in_run % run_words, row_tile = in_run / run_words;
+  const int v0 = c.first + word_tile * kWords, r0 = row_tile * kRowsTile;
   T t;
-  t.sum(lds, Operand{c.w.data + v0 * c.w.pitch, c.w.pitch, c.vocab - v0, c.steps},
-        Operand{c.x.data + r0 * c.x.pitch, c.x.pitch, c.rows - r0, c.steps}, c.w.plane, c.x.plane, 0, c.steps);
+  t.sum(lds, Operand{c.w.data + int64_t{v0} * c.w.pitch, c.w.pitch, c.vocab - v0, c.steps},
+        Operand{c.x.data + int64_t{r0} * c.x.pitch, c.x.pitch, c.rows - r0, c.steps}, c.w.plane, c.x.plane, 0, c.steps);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
   // lane's words: this + 64 (i / 4) + 4 (i % 4) + element
-  const int64_t word0 = v0 + wp * T::kWaveP + 16 * g;
+  const int word0 = v0 + wp * T::kWaveP + 16 * g;
   if constexpr (!BF) {
     const int exponent = -(c.scalars->exponent[0] + c.scalars->exponent[1]);
 #pragma unroll
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
 #pragma unroll
     for (int j = 0; j < T::kTilesQ; ++j) {
       const int in_tile = wq * T::kWaveQ + 16 * j + m;
-      const int64_t row = r0 + in_tile;
+      const int row = r0 + in_tile;
       float most = t.acc[0][j][0];
 #pragma unroll
       for (int i = 0; i < T::kTilesP; ++i)
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
       const int q = threadIdx.x;
       const float a = maxima[q], b = maxima[kRowsTile + q];
       const float most = fmaxf(a, b), sa = sums[q], sb = sums[kRowsTile + q];
-      const int64_t to = v0 / kWords * c.rows + r0 + q;
+      const int64_t to = int64_t{v0 / kWords} * c.rows + r0 + q;
       const int fa = firsts[q], fb = firsts[kRowsTile + q];
       c.part_max[to] = most;
       // a half without a word (or all of minus infinity) has a NaN for a sum
@@ -241,12 +241,13 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
     const float reference = c.scalars->reference;
 #pragma unroll
     for (int j = 0; j < T::kTilesQ; ++j) {
-      const int64_t row = r0 + wq * T::kWaveQ + 16 * j + m;
-      const int64_t known = min(row, c.rows - 1), target = c.targets[known];
+      const int row = r0 + wq * T::kWaveQ + 16 * j + m, known = min(row, c.rows - 1);
+      const int64_t target = c.targets[known];
       const bool dead = row >= c.rows || target == c.ignore_index;
       const float lse = c.row_lse[known], h = c.row_grad[known] / reference;
       const float wrap = c.l2wrap_scale * c.row_max[known] / reference;
-      const int64_t own = target - word0, top = c.row_argmax[known] - word0;
+      const int64_t own = target - word0;
+      const int top = c.row_argmax[known] - word0;
 #pragma unroll
       for (int half = 0; half < T::kTilesP / 4; ++half) {
         float v[16];
@@ -266,13 +267,13 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
 #pragma unroll
           for (int n = 0; n < 16; ++n) v[n] = 0.f;
         }
-        const int64_t word = word0 + 64 * half;
+        const int word = word0 + 64 * half;
         if (word + 16 > c.vocab) {
 #pragma unroll
           for (int n = 0; n < 16; ++n)
             if (word + n >= c.vocab) v[n] = 0.f;
         }
-        char* const to = c.d + (row * c.words + word - c.first) * 2;
+        char* const to = c.d + (static_cast<int64_t>(row) * c.words + word - c.first) * 2;
         if constexpr (BF) {
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
@@ -410,23 +411,23 @@ __device__ __forceinline__ void store4(void* base, int64_t at, f32x4 v, int64_t 
 struct WeightGradCall {
   Matrix x;
   const char* d;
-  int64_t d_plane, words, padded_rows;
-  int64_t rows, vocab, c, first;
+  int64_t d_plane;
+  int words, padded_rows, rows, vocab, c, first;
   const Scalars* scalars;
   void* grad;
 };
 // dw of the piece's words: steps are rows; those past the last have D = 0.
 template <bool BF, int kChannels>
 __global__ __launch_bounds__(kThreads, 2) void weight_grad_kernel(const WeightGradCall c) {
-  using T = Tile<kSteps, kSteps, kChannels, 128, kWavesP, kWavesQ, false, BF ? 1 : 2>;
+  using T = Tile<kSteps, kSteps, kChannels, 256, kWavesP, kWavesQ, false, false, BF ? 1 : 2>;
   __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
-  const int64_t channel_tiles = ceil_div(c.c, kChannels);
-  const int64_t at = tile_of_block(gridDim.x, blockIdx.x);
-  const int64_t c0 = at % channel_tiles * kChannels, w0 = at / channel_tiles * 128;
-  const int64_t steps = ceil_div(c.rows, kStep) * kStep;
+  const int channel_tiles = (c.c + kChannels - 1) / kChannels;
+  const int at = tile_of_block();
+  const int c0 = at % channel_tiles * kChannels, w0 = at / channel_tiles * 256;
+  const int steps = (c.rows + kStep - 1) / kStep * kStep;
   T t;
   t.sum(lds, Operand{c.x.data + c0 * 2, c.x.pitch, c.c - c0, c.rows},
-        Operand{c.d + w0 * 2, c.words * 2, c.words - w0, c.padded_rows}, c.x.plane, c.d_plane, 0, steps);
+        Operand{c.d + w0 * 2, int64_t{c.words} * 2, c.words - w0, c.padded_rows}, c.x.plane, c.d_plane, 0, steps);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
   const float reference = c.scalars->reference;
@@ -434,16 +435,16 @@ __global__ __launch_bounds__(kThreads, 2) void weight_grad_kernel(const WeightGr
   const bool whole = c.c % 4 == 0;
 #pragma unroll
   for (int j = 0; j < T::kTilesQ; ++j) {
-    const int64_t word = c.first + w0 + wq * T::kWaveQ + 16 * j + m;
+    const int word = c.first + w0 + wq * T::kWaveQ + 16 * j + m;
     if (word >= c.vocab) continue;
 #pragma unroll
     for (int i = 0; i < T::kTilesP; ++i) {
-      const int64_t channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
+      const int channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
       if (channel >= c.c) continue;
       f32x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = unscaled<BF>(t.acc[i][j][e], reference, exponent);
-      store4<BF>(c.grad, word * c.c + channel, v, c.c - channel, whole);
+      store4<BF>(c.grad, int64_t{word} * c.c + channel, v, c.c - channel, whole);
     }
   }
 }
@@ -451,36 +452,36 @@ __global__ __launch_bounds__(kThreads, 2) void weight_grad_kernel(const WeightGr
 struct HiddenGradCall {
   Matrix w;
   const char* d;
-  int64_t d_plane, words;
-  int64_t rows, vocab, c, first;
-  int64_t share;             // words of a workgroup
+  int64_t d_plane;
+  int words, rows, vocab, c, first;
+  int share;                 // words of a workgroup
   bool begin;                // the first piece: nothing to add to
   float* sums;               // [splits, rows, pitch]
-  int64_t pitch;
+  int pitch;
 };
 template <bool BF, int kChannels>
 __global__ __launch_bounds__(kThreads, 2) void hidden_grad_kernel(const HiddenGradCall c) {
-  using T = Tile<kSteps, kRows, kChannels, 128, kWavesP, kWavesQ, false, BF ? 1 : 2>;
+  using T = Tile<kSteps, kRows, kChannels, 256, kWavesP, kWavesQ, false, true, BF ? 1 : 2>;
   __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
-  const int64_t channel_tiles = ceil_div(c.c, kChannels), row_tiles = ceil_div(c.rows, 128);
-  const int64_t at = tile_of_block(gridDim.x, blockIdx.x);
-  const int64_t c0 = at % channel_tiles * kChannels, r0 = at / channel_tiles % row_tiles * 128;
-  const int64_t split = at / channel_tiles / row_tiles;
-  const int64_t k0 = split * c.share, k1 = min(k0 + c.share, c.words);
+  const int channel_tiles = (c.c + kChannels - 1) / kChannels, row_tiles = (c.rows + 255) / 256;
+  const int at = tile_of_block();
+  const int c0 = at % channel_tiles * kChannels, r0 = at / channel_tiles % row_tiles * 256;
+  const int split = at / channel_tiles / row_tiles;
+  const int k0 = split * c.share, k1 = min(k0 + c.share, c.words);
   T t;
-  t.sum(lds, Operand{c.w.data + c.first * c.w.pitch + c0 * 2, c.w.pitch, c.c - c0, c.vocab - c.first},
-        Operand{c.d + r0 * c.words * 2, c.words * 2, 128, c.words}, c.w.plane, c.d_plane, k0, k1);
+  t.sum(lds, Operand{c.w.data + int64_t{c.first} * c.w.pitch + c0 * 2, c.w.pitch, c.c - c0, c.vocab - c.first},
+        Operand{c.d + int64_t{r0} * c.words * 2, int64_t{c.words} * 2, 256, c.words}, c.w.plane, c.d_plane, k0, k1);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
 #pragma unroll
   for (int j = 0; j < T::kTilesQ; ++j) {
-    const int64_t row = r0 + wq * T::kWaveQ + 16 * j + m;
+    const int row = r0 + wq * T::kWaveQ + 16 * j + m;
     if (row >= c.rows) continue;
 #pragma unroll
     for (int i = 0; i < T::kTilesP; ++i) {
-      const int64_t channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
+      const int channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
       if (channel >= c.pitch) continue;
-      f32x4* const to = reinterpret_cast<f32x4*>(c.sums + (split * c.rows + row) * c.pitch + channel);
+      f32x4* const to = reinterpret_cast<f32x4*>(c.sums + (int64_t{split} * c.rows + row) * c.pitch + channel);
       *to = c.begin ? t.acc[i][j] : *to + t.acc[i][j];
     }
   }
@@ -545,7 +546,7 @@ Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
 }
 
 // Two workgroups of a tile fill a compute unit.
-constexpr int64_t kSlots = 2 * kUnits;
+constexpr int64_t kSlots = kUnits;
 constexpr int64_t kMaxD = int64_t{512} << 20;   // bytes of D of a piece
 struct Plan {
   int channels;                     // of a gradient's tile
@@ -561,12 +562,12 @@ Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   const int64_t all = up(vocab, kWords);
   const int64_t most = std::max<int64_t>(kWords, kMaxD / (p.padded_rows * 2 * planes) / kWords * kWords);
   // pieces of whole rounds of the weight gradient's tiles of 128 words
-  const int64_t round = std::max<int64_t>(kSlots / channel_tiles, 2) / 2 * 256;
+  const int64_t round = std::max<int64_t>(kSlots / channel_tiles, 1) * 256;
   p.words = std::min(all, most >= round ? most / round * round : most);
   p.pieces = ceil_div(all, p.words);
   p.words = std::min(p.words, up(ceil_div(all, p.pieces), kWords) );
-  const int64_t tiles = channel_tiles * ceil_div(rows, 128);
-  p.splits = std::max<int64_t>(1, std::min<int64_t>(ceil_div(kSlots, tiles), p.words / 512));
+  const int64_t tiles = channel_tiles * ceil_div(rows, 256);
+  p.splits = std::max<int64_t>(1, std::min<int64_t>(kSlots * 4 / tiles, p.words / 512));
   p.share = up(ceil_div(p.words, p.splits), kStep);
   p.splits = ceil_div(p.words, p.share);
   return p;
@@ -637,10 +638,10 @@ void forward(const ForwardCall& c, hipStream_t s) {
   const ForwardPlaces f = forward_places(c.rows, c.vocab, c.c, BF);
   LogitsCall l{};
   prepare<BF>(c, f.operands, &l.x, &l.w, s);
-  l.rows = c.rows;
-  l.vocab = c.vocab;
-  l.steps = up(c.c, kStep);
-  l.words = up(c.vocab, kWords);
+  l.rows = static_cast<int>(c.rows);
+  l.vocab = static_cast<int>(c.vocab);
+  l.steps = static_cast<int>(up(c.c, kStep));
+  l.words = static_cast<int>(up(c.vocab, kWords));
   l.scalars = reinterpret_cast<const Scalars*>(c.workspace + f.operands.scalars);
   l.targets = c.targets;
   l.part_max = reinterpret_cast<float*>(c.workspace + f.part_max);
@@ -655,20 +656,22 @@ void forward(const ForwardCall& c, hipStream_t s) {
 }
 
 template <bool BF, int kChannels>
-void gradients(const BackwardCall& c, const Plan& p, const BackwardPlaces& b, const LogitsCall& l, hipStream_t s) {
+void gradients(const BackwardCall& c, const Plan& p, const BackwardPlaces& b, const LogitsCall& l, bool first, hipStream_t s) {
   const int64_t channel_tiles = ceil_div(c.c, kChannels);
   if (c.weight_grad) {
-    const WeightGradCall w{l.x, l.d, l.d_plane, l.words, p.padded_rows, c.rows, c.vocab, c.c, l.first, l.scalars, c.weight_grad};
-    const int64_t words = std::min(l.words, c.vocab - l.first);
-    hipLaunchKernelGGL((weight_grad_kernel<BF, kChannels>), dim3(static_cast<unsigned>(channel_tiles * ceil_div(words, 128))),
+    const WeightGradCall w{l.x, l.d, l.d_plane, l.words, static_cast<int>(p.padded_rows), l.rows, l.vocab, static_cast<int>(c.c),
+                           l.first, l.scalars, c.weight_grad};
+    const int words = std::min(l.words, l.vocab - l.first);
+    hipLaunchKernelGGL((weight_grad_kernel<BF, kChannels>), dim3(static_cast<unsigned>(channel_tiles * ceil_div(words, 256))),
                        dim3(kThreads), 0, s, w);
   }
   if (c.hidden_grad) {
     const int64_t splits = ceil_div(l.words, p.share);
-    const HiddenGradCall h{l.w, l.d, l.d_plane, l.words, c.rows, c.vocab, c.c, l.first, p.share, l.first == 0,
-                           reinterpret_cast<float*>(c.workspace + b.sums), p.pitch};
+    const HiddenGradCall h{l.w, l.d, l.d_plane, l.words, l.rows, l.vocab, static_cast<int>(c.c), l.first,
+                           static_cast<int>(p.share), first, reinterpret_cast<float*>(c.workspace + b.sums),
+                           static_cast<int>(p.pitch)};
     hipLaunchKernelGGL((hidden_grad_kernel<BF, kChannels>),
-                       dim3(static_cast<unsigned>(channel_tiles * ceil_div(c.rows, 128) * splits)), dim3(kThreads), 0, s, h);
+                       dim3(static_cast<unsigned>(channel_tiles * ceil_div(c.rows, 256) * splits)), dim3(kThreads), 0, s, h);
   }
 }
 
@@ -681,9 +684,9 @@ void backward(const BackwardCall& c, hipStream_t s) {
   Scalars* const scalars = reinterpret_cast<Scalars*>(c.workspace + b.operands.scalars);
   const ReferenceCall r{c.row_grad, c.row_max, c.targets, c.rows, c.ignore_index, c.l2wrap_scale, scalars};
   hipLaunchKernelGGL(reference_kernel, dim3(1), dim3(1024), 0, s, r);
-  l.rows = c.rows;
-  l.vocab = c.vocab;
-  l.steps = up(c.c, kStep);
+  l.rows = static_cast<int>(c.rows);
+  l.vocab = static_cast<int>(c.vocab);
+  l.steps = static_cast<int>(up(c.c, kStep));
   l.scalars = scalars;
   l.targets = c.targets;
   l.ignore_index = c.ignore_index;
@@ -694,12 +697,13 @@ void backward(const BackwardCall& c, hipStream_t s) {
   l.l2wrap_scale = c.l2wrap_scale;
   l.d = c.workspace + b.d;
   l.d_plane = b.d_plane;
-  for (l.first = 0; l.first < c.vocab; l.first += p.words) {
-    l.words = std::min(p.words, up(c.vocab - l.first, kWords));
+  for (int64_t first = 0; first < c.vocab; first += p.words) {
+    l.first = static_cast<int>(first);
+    l.words = static_cast<int>(std::min(p.words, up(c.vocab - first, kWords)));
     const int64_t tiles = l.words / kWords * ceil_div(c.rows, kRowsTile);
     hipLaunchKernelGGL((logits_kernel<BF, true>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), 0, s, l);
-    if (p.channels == 128) gradients<BF, 128>(c, p, b, l, s);
-    else gradients<BF, 256>(c, p, b, l, s);
+    if (p.channels == 128) gradients<BF, 128>(c, p, b, l, first == 0, s);
+    else gradients<BF, 256>(c, p, b, l, first == 0, s);
   }
   if (c.hidden_grad) {
     const HiddenSumCall h{reinterpret_cast<const float*>(c.workspace + b.sums), c.rows, c.c, p.pitch,

@@ -8,8 +8,8 @@
 // that transpose 4 x 16 elements.
 //
 // A workgroup of kWavesP x kWavesQ waves brings kStep steps of both operands at a
-// time to LDS (16 bytes a lane, without a stop in registers), kStages - 1 of them
-// ahead of the products, behind one barrier each. Instruction 16x16x32: lane l has
+// time to LDS (16 bytes a lane, without a stop in registers), a stage or two ahead of
+// the products, behind one barrier each. Instruction 16x16x32: lane l has
 // element l % 16 of p or q and the steps 8 (l / 16) .. + 7; of the sums, lane l has
 // q = l % 16 and p = 4 (l / 16) .. + 3.
 #pragma once
@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace rwkv_tile {
 
@@ -26,7 +27,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kStep = 32;              // steps of k a stage
+constexpr int kStep = 64;              // steps of k a stage: whole cache lines of an operand that lies by rows
 constexpr int kStepBytes = kStep * 2;
 constexpr int kPieces = kStepBytes / 16;
 
@@ -38,11 +39,21 @@ __device__ __forceinline__ f32x4 multiply(s16x8 p, s16x8 q, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
 }
 
-// 16 bytes from each lane's address to consecutive places from `to` on.
-__device__ __forceinline__ void bring(const char* from, char* to) {
-  typedef const void __attribute__((address_space(1))) * Global;
+// 16 bytes from each lane's offset to consecutive places from `to` on. A buffer load:
+// the compiler takes a global one to LDS for one that LDS may answer too, and waits for
+// every LDS read behind it.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+// A value that is the same in all lanes, where the compiler cannot see that it is.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return static_cast<int64_t>(uniform(static_cast<int>(v >> 32))) << 32 | static_cast<uint32_t>(uniform(static_cast<int>(v)));
+}
+__device__ __forceinline__ Buffer buffer(const char* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, -1, 0x00020000);
+}
+__device__ __forceinline__ void bring(Buffer from, uint32_t offset, int shift, char* to) {
   typedef void __attribute__((address_space(3))) * Local;
-  __builtin_amdgcn_global_load_lds((Global)(uintptr_t)from, (Local)to, 16, 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (Local)to, 16, offset, shift, 0, 0);
 }
 
 // An operand of a tile: element (i, k) at base + i * pitch + 2 k (rows) or base + k *
@@ -53,7 +64,7 @@ __device__ __forceinline__ void bring(const char* from, char* to) {
 struct Operand {
   const char* base;
   int64_t pitch;
-  int64_t items, steps;
+  int items, steps;
 };
 
 enum Layout { kRows, kSteps };
@@ -61,7 +72,7 @@ enum Layout { kRows, kSteps };
 // banks. kSpread: tile i's lane m reads row 64 (i / 4) + 16 (m / 4) + 4 (i % 4) + m %
 // 4 instead of 16 i + m, which leaves a lane with 16 consecutive p.
 template <bool kSpread>
-__device__ __forceinline__ int row_swizzle(int row) { return (-(row >> (kSpread ? 4 : 2))) & 3; }
+__device__ __forceinline__ int row_swizzle(int row) { return ((-(row >> (kSpread ? 4 : 2))) & 3) + 2 * (row & 2); }
 __device__ __forceinline__ int step_swizzle(int k) { return (k & 3) | ((k >> 1) & 4); }
 
 // How a workgroup's lanes bring an operand of kItems to LDS and read it back.
@@ -74,7 +85,8 @@ struct Side {
   static constexpr int kPerStep = kItems / 8;               // pieces of a step (steps' form)
   uint32_t at[kLoads];     // byte offset of a lane's piece from the stage's first element
   const char* base;
-  int64_t pitch, steps;
+  int64_t pitch;
+  int steps;
 
   // the step (steps' form) or row that load j of this lane brings
   __device__ __forceinline__ int line(int j, int wave, int lane) const {
@@ -89,48 +101,44 @@ struct Side {
     return 16 * (c ^ (2 * step_swizzle(l)));
   }
   __device__ __forceinline__ void init(const Operand& o, int wave, int lane) {
-    base = o.base;
+    base = reinterpret_cast<const char*>(uniform(reinterpret_cast<int64_t>(o.base)));
     pitch = o.pitch;
-    steps = o.steps;
+    steps = uniform(o.steps);
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int l = line(j, wave, lane);
       if constexpr (kLayout == kRows) {
-        at[j] = static_cast<uint32_t>(min(static_cast<int64_t>(l), o.items - 1) * pitch) + within(j, wave, lane);
+        at[j] = static_cast<uint32_t>(min(l, o.items - 1) * pitch) + within(j, wave, lane);
       } else {
-        const int last = static_cast<int>(min(o.items - 1, static_cast<int64_t>(kItems - 1)) / 8 * 16);
+        const int last = min(o.items - 1, kItems - 1) / 8 * 16;
         at[j] = static_cast<uint32_t>(l * pitch) + min(within(j, wave, lane), last);
       }
     }
   }
-  // steps k .. k + kStep - 1 of the operand's array at `offset` bytes from the first one
-  __device__ __forceinline__ void load(char* lds, int64_t offset, int64_t k, int wave, int lane) const {
-    if constexpr (kLayout == kRows) {
-      const char* from = base + offset + 2 * k;
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) bring(from + at[j], lds + (j * kWaves + wave) * 1024);
-    } else {
-      const char* from = base + offset + k * pitch;
-      if (k + kStep <= steps) {
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) bring(from + at[j], lds + (j * kWaves + wave) * 1024);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-          const int64_t beyond = max(k + line(j, wave, lane) - (steps - 1), static_cast<int64_t>(0));
-          bring(from + at[j] - beyond * pitch, lds + (j * kWaves + wave) * 1024);
-        }
+  // The buffer of the steps k .. k + kStep - 1 of the operand's array at `offset` bytes
+  // from the first one, and its load j.
+  __device__ __forceinline__ Buffer stage(int64_t offset, int k) const {
+    return buffer(base + offset + (kLayout == kRows ? 2 * k : min(k, steps - 1) * pitch));
+  }
+  __device__ __forceinline__ void load(int j, char* lds, Buffer from, int k, int wave, int lane) const {
+    uint32_t offset = at[j];
+    if constexpr (kLayout == kSteps) {
+      if (k + kStep > steps) {
+        const int last = max(steps - 1 - k, 0);
+        offset -= static_cast<uint32_t>(max(line(j, wave, lane) - last, 0)) * static_cast<uint32_t>(pitch);
       }
     }
+    bring(from, offset, 0, lds + (j * kWaves + wave) * 1024);
   }
   // what lane (m, g) of a wave whose items begin at `first` gives to tile i's instruction
-  __device__ __forceinline__ s16x8 read(const char* lds, int first, int i, int m, int g) const {
+  // over half a stage's steps
+  __device__ __forceinline__ s16x8 read(const char* lds, int half, int first, int i, int m, int g) const {
     if constexpr (kLayout == kRows) {
       const int row = first + (kSpread ? 64 * (i / 4) + 16 * (m >> 2) + 4 * (i % 4) + (m & 3) : 16 * i + m);
-      return *reinterpret_cast<const s16x8*>(lds + row * kStepBytes + 16 * (g ^ row_swizzle<kSpread>(row)));
+      return *reinterpret_cast<const s16x8*>(lds + row * kStepBytes + 16 * ((4 * half + g) ^ row_swizzle<kSpread>(row)));
     } else {
       typedef __attribute__((address_space(3))) s16x4* Local;
-      const int k = 8 * g + (m >> 2);          // and k + 4, whose pieces lie alike
+      const int k = 32 * half + 8 * g + (m >> 2);          // and k + 4, whose pieces lie alike
       const int piece = (first / 8 + 2 * i + ((m & 3) >> 1)) ^ (2 * step_swizzle(k));
       const char* from = lds + k * (kItems * 2) + 16 * piece + 8 * (m & 1);
       const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Local)(from));
@@ -143,79 +151,193 @@ struct Side {
 // kPlanes 1: bf16 operands. 2: each operand is two fp16 arrays, the second (`plane`
 // bytes behind the first) holding what rounding took from the first: the product is
 // hi hi + hi lo + lo hi.
-template <Layout kLayoutP, Layout kLayoutQ, int kP, int kQ, int kWavesP, int kWavesQ, bool kSpread, int kPlanes>
+//
+// LDS holds three stages of one operand and two of the other (kDeepP: three of P). The
+// loop's barrier lies kTail groups of products before a stage's end, when all of the
+// stage has been read: behind it the next stage's first reads and the loads that
+// overwrite this one are issued under the products that are left.
+template <Layout kLayoutP, Layout kLayoutQ, int kP, int kQ, int kWavesP, int kWavesQ, bool kSpread, bool kDeepP, int kPlanes>
 struct Tile {
   static constexpr int kWaves = kWavesP * kWavesQ, kThreads = 64 * kWaves;
-  static constexpr int kStages = 3;
   static constexpr int kWaveP = kP / kWavesP, kWaveQ = kQ / kWavesQ;
   static constexpr int kTilesP = kWaveP / 16, kTilesQ = kWaveQ / 16;
   static_assert(!kSpread || kWaveP % 64 == 0);
   using SideP = Side<kLayoutP, kP, kWaves, kSpread>;
   using SideQ = Side<kLayoutQ, kQ, kWaves, false>;
-  static constexpr int kStageBytes = SideP::kBytes + SideQ::kBytes;
-  static constexpr int kLdsBytes = kStages * kStageBytes;
-  static constexpr int kLoads = SideP::kLoads + SideQ::kLoads;
+  static constexpr int kSlotsP = kDeepP ? 3 : 2, kSlotsQ = kDeepP ? 2 : 3;
+  static constexpr int kPlaceQ = kSlotsP * SideP::kBytes;
+  static constexpr int kLdsBytes = kPlaceQ + kSlotsQ * SideQ::kBytes;
+  static constexpr int kDeepLoads = kDeepP ? SideP::kLoads : SideQ::kLoads;
   static constexpr int kParts = kPlanes == 1 ? 1 : 3;
+  static constexpr int kTail = kTilesP / 2, kBody = 2 * kTilesP - kTail;   // groups of kTilesQ products
+  static constexpr int kHeldP = 2;
 
   f32x4 acc[kTilesP][kTilesQ];
 
-  // Sums over the steps [k0, k1), whole stages. The workgroup may use `lds` again
-  // once all of its waves have come back.
-  __device__ __forceinline__ void sum(char* lds, const Operand& p, const Operand& q, int64_t plane_p, int64_t plane_q,
-                                      int64_t k0, int64_t k1) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int m = lane & 15, g = lane >> 4;
-    const int wave_p = wave % kWavesP * kWaveP, wave_q = wave / kWavesP * kWaveQ;
-#pragma unroll
-    for (int i = 0; i < kTilesP; ++i)
-#pragma unroll
-      for (int j = 0; j < kTilesQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    SideP sp;
-    SideQ sq;
-    sp.init(p, wave, lane);
-    sq.init(q, wave, lane);
-    int64_t k = k0;      // the next stage's steps
-    int part = 0;        // and which product of planes it belongs to
-    auto load = [&](int stage) {
-      char* const at = lds + stage * kStageBytes;
-      sp.load(at, kPlanes > 1 && part == 2 ? plane_p : 0, k, wave, lane);
-      sq.load(at + SideP::kBytes, kPlanes > 1 && part == 1 ? plane_q : 0, k, wave, lane);
-      // past the last stage, that one is brought again, so that a wait always finds as
-      // many loads behind it
+  // The next stage of an operand to be brought: its first step, which product of planes
+  // it belongs to, and its slot. Past the last stage that one is brought again, so that
+  // a wait always finds as many loads behind it.
+  template <int kSlots>
+  struct Next {
+    int k, part, slot;
+    __device__ __forceinline__ void advance(int k0, int k1) {
+      slot = slot == kSlots - 1 ? 0 : slot + 1;
       if (k + kStep < k1) {
         k += kStep;
       } else if (part + 1 < kParts) {
         ++part;
         k = k0;
       }
-    };
-    const int64_t stages = (k1 - k0) / kStep * kParts;
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) load(s);
-    int now = 0, next = kStages - 1;
-    for (int64_t s = 0; s < stages; ++s) {
-      // this wave's loads of stage s are here, and behind the barrier everyone's; and
-      // everyone has read the stage that is overwritten next
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kLoads) : "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      load(next);
-      const char* const at = lds + now * kStageBytes;
-      s16x8 b[kTilesQ];
-#pragma unroll
-      for (int j = 0; j < kTilesQ; ++j) b[j] = sq.read(at + SideP::kBytes, wave_q, j, m, g);
-#pragma unroll
-      for (int i = 0; i < kTilesP; ++i) {
-        const s16x8 a = sp.read(at, wave_p, i, m, g);
-#pragma unroll
-        for (int j = 0; j < kTilesQ; ++j) acc[i][j] = multiply<(kPlanes > 1)>(a, b[j], acc[i][j]);
-      }
-      now = now == kStages - 1 ? 0 : now + 1;
-      next = next == kStages - 1 ? 0 : next + 1;
     }
+  };
+  // What a wave has of a stage before its products begin, and of the stage before it:
+  // the factors of the products that are left there.
+  struct Held {
+    s16x8 q[kTilesQ], p[kHeldP];
+    s16x8 last_q[kTilesQ], last_p[kTail];
+  };
+  struct Place {
+    SideP p;
+    SideQ q;
+    int64_t plane_p, plane_q;
+    int wave, lane;
+    __device__ __forceinline__ Buffer from(const Next<kSlotsP>& n) const { return p.stage(kPlanes > 1 && n.part == 2 ? plane_p : 0, n.k); }
+    __device__ __forceinline__ Buffer from(const Next<kSlotsQ>& n, int) const { return q.stage(kPlanes > 1 && n.part == 1 ? plane_q : 0, n.k); }
+    __device__ __forceinline__ s16x8 read_p(const char* lds, int half, int i) const {
+      return p.read(lds, half, wave % kWavesP * kWaveP, i, lane & 15, lane >> 4);
+    }
+    __device__ __forceinline__ s16x8 read_q(const char* lds, int half, int j) const {
+      return q.read(lds, half, wave / kWavesP * kWaveQ, j, lane & 15, lane >> 4);
+    }
+  };
+  __device__ __forceinline__ static void bring_p(int n, char* lds, const Place& a, Buffer from, const Next<kSlotsP>& next) {
+    a.p.load(n, lds + next.slot * SideP::kBytes, from, next.k, a.wave, a.lane);
+  }
+  __device__ __forceinline__ static void bring_q(int n, char* lds, const Place& a, Buffer from, const Next<kSlotsQ>& next) {
+    a.q.load(n, lds + kPlaceQ + next.slot * SideQ::kBytes, from, next.k, a.wave, a.lane);
+  }
+  __device__ __forceinline__ void products(int i, s16x8 p, const s16x8 (&q)[kTilesQ]) {
+#pragma unroll
+    for (int j = 0; j < kTilesQ; ++j) acc[i][j] = multiply<(kPlanes > 1)>(p, q[j], acc[i][j]);
+  }
+
+  // From one barrier to the next: the products that are left of the stage before, and
+  // this one's but for the last kTail groups. `to_p`, `to_q` are where the loads go and
+  // `p`, `q` what is read, apart from one another, which is said here for the compiler:
+  // it otherwise waits for all loads before a transposing read. Left to itself it also
+  // puts each read right before its products and waits there; the groups fix the order,
+  // with reads two groups ahead or more and none in the last.
+  template <bool kFirst>
+  __device__ __forceinline__ void step(char* __restrict to_p, char* __restrict to_q, const char* __restrict p,
+                                       const char* __restrict q, Held& held, const Place& a, const Next<kSlotsP>& next_p,
+                                       const Next<kSlotsQ>& next_q) {
+    constexpr int kHolds = kTilesQ + kHeldP, kHoldsPerGroup = (kHolds + kTail - 1) / kTail;
+    constexpr int kReads = 2 * kTilesP - kHeldP + kTilesQ, kReadsPerGroup = (kReads + kBody - 3) / (kBody - 2);
+    constexpr int kNear = kDeepP ? SideQ::kLoads : SideP::kLoads;       // of the operand with two slots: first
+    constexpr int kNearPerGroup = (kNear + kTail - 1) / kTail, kDeepPerGroup = (kDeepLoads + kBody - 1) / kBody;
+    const Buffer from_p = a.from(next_p), from_q = a.from(next_q, 0);
+    auto load_near = [&](int n) {
+      if (n >= kNear) return;
+      if constexpr (kDeepP) a.q.load(n, to_q, from_q, next_q.k, a.wave, a.lane);
+      else a.p.load(n, to_p, from_p, next_p.k, a.wave, a.lane);
+    };
+    auto load_deep = [&](int n) {
+      if (n >= kDeepLoads) return;
+      if constexpr (kDeepP) a.p.load(n, to_p, from_p, next_p.k, a.wave, a.lane);
+      else a.q.load(n, to_q, from_q, next_q.k, a.wave, a.lane);
+    };
+#pragma unroll
+    for (int i = 0; i < kTail; ++i) {
+#pragma unroll
+      for (int n = i * kNearPerGroup; n < (i + 1) * kNearPerGroup; ++n) load_near(n);
+#pragma unroll
+      for (int n = i * kHoldsPerGroup; n < (i + 1) * kHoldsPerGroup; ++n) {
+        if (n < kTilesQ) held.q[n] = a.read_q(q, 0, n);
+        else if (n < kHolds) held.p[n - kTilesQ] = a.read_p(p, 0, n - kTilesQ);
+      }
+      if constexpr (!kFirst) products(kTilesP - kTail + i, held.last_p[i], held.last_q);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    s16x8 at[2][kTilesP];
+#pragma unroll
+    for (int i = 0; i < kHeldP; ++i) at[0][i] = held.p[i];
+#pragma unroll
+    for (int i = 0; i < kBody; ++i) {
+#pragma unroll
+      for (int n = i * kDeepPerGroup; n < (i + 1) * kDeepPerGroup; ++n) load_deep(n);
+#pragma unroll
+      for (int n = i * kReadsPerGroup; n < (i + 1) * kReadsPerGroup; ++n) {
+        if (n < kTilesP - kHeldP) at[0][n + kHeldP] = a.read_p(p, 0, n + kHeldP);
+        else if (n < kTilesP - kHeldP + kTilesQ) held.last_q[n - (kTilesP - kHeldP)] = a.read_q(q, 1, n - (kTilesP - kHeldP));
+        else if (n < kReads) at[1][n - (kTilesP - kHeldP + kTilesQ)] = a.read_p(p, 1, n - (kTilesP - kHeldP + kTilesQ));
+      }
+      if (i < kTilesP) products(i, at[0][i % kTilesP], held.q);
+      else products(i - kTilesP, at[1][i % kTilesP], held.last_q);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < kTail; ++i) held.last_p[i] = at[1][kTilesP - kTail + i];
+  }
+
+  // Behind it this stage is everyone's, and the stage before has been read by everyone.
+  // kBehind: this wave's loads that may still be on their way.
+  template <int kBehind>
+  __device__ __forceinline__ static void arrive() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kBehind) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+
+  // Sums over the steps [k0, k1), whole stages. The workgroup may use `lds` again
+  // once all of its waves have come back.
+  __device__ __forceinline__ void sum(char* lds, const Operand& p, const Operand& q, int64_t plane_p, int64_t plane_q,
+                                      int k0, int k1) {
+    Place a;
+    a.lane = threadIdx.x & 63;
+    a.wave = uniform(static_cast<int>(threadIdx.x >> 6));
+    a.p.init(p, a.wave, a.lane);
+    a.q.init(q, a.wave, a.lane);
+    a.plane_p = plane_p;
+    a.plane_q = plane_q;
+#pragma unroll
+    for (int i = 0; i < kTilesP; ++i)
+#pragma unroll
+      for (int j = 0; j < kTilesQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Next<kSlotsP> next_p{k0, 0, 0};
+    Next<kSlotsQ> next_q{k0, 0, 0};
+    auto all_p = [&] {
+      const Buffer from = a.from(next_p);
+#pragma unroll
+      for (int n = 0; n < SideP::kLoads; ++n) bring_p(n, lds, a, from, next_p);
+      next_p.advance(k0, k1);
+    };
+    auto all_q = [&] {
+      const Buffer from = a.from(next_q, 0);
+#pragma unroll
+      for (int n = 0; n < SideQ::kLoads; ++n) bring_q(n, lds, a, from, next_q);
+      next_q.advance(k0, k1);
+    };
+    all_p();
+    all_q();
+    kDeepP ? all_p() : all_q();
+    const int stages = (k1 - k0) / kStep * kParts;
+    int slot_p = 0, slot_q = 0;
+    Held held;
+    auto one = [&](auto first) {
+      arrive<kDeepLoads>();
+      step<decltype(first)::value>(lds + next_p.slot * SideP::kBytes, lds + kPlaceQ + next_q.slot * SideQ::kBytes,
+                                   lds + slot_p * SideP::kBytes, lds + kPlaceQ + slot_q * SideQ::kBytes, held, a, next_p, next_q);
+      next_p.advance(k0, k1);
+      next_q.advance(k0, k1);
+      slot_p = slot_p == kSlotsP - 1 ? 0 : slot_p + 1;
+      slot_q = slot_q == kSlotsQ - 1 ? 0 : slot_q + 1;
+    };
+    one(std::true_type());
+    for (int s = 1; s < stages; ++s) one(std::false_type());
+#pragma unroll
+    for (int i = 0; i < kTail; ++i) products(kTilesP - kTail + i, held.last_p[i], held.last_q);
     // the loads that were brought for no product, and everyone's reads
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    arrive<0>();
   }
 };
 
