@@ -29,91 +29,186 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWords = 256, kRowsTile = 256;   // a tile of logits
 constexpr int kWavesP = 2, kWavesQ = 4, kThreads = 512;
-constexpr int kUnits = 256;                    // compute units
+constexpr int kUnits = 256;                    // compute units; a tile's LDS leaves room for one workgroup on each
 constexpr int kXcds = 8;
 constexpr int kMaxBlocks = 256;                // of a maximum over an operand
 constexpr int kHalfExponent = 13;              // fp16 arrays hold up to 2^14
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-__host__ __device__ int64_t ceil_div(int64_t n, int64_t by) { return (n + by - 1) / by; }
+int64_t ceil_div(int64_t n, int64_t by) { return (n + by - 1) / by; }
 
-// An operand as the tiles read it: rows of `pitch` bytes, a multiple of kStep
-// elements each; two arrays `plane` bytes apart for fp32.
+// An operand as the tiles read it: rows of `pitch` bytes, whole steps; two arrays `plane`
+// bytes apart for fp32.
 struct Matrix {
   const char* data;
   int64_t pitch, plane;
 };
 
-// Numbers that a call's kernels leave to one another.
+// What a call's kernels leave to one another.
 struct Scalars {
-  float reference;             // the backward's: D is held over this
-  int exponent[2];             // fp32 operands' fp16 arrays are 2^exponent as large: x, w
+  float reference;     // D is held over this
+  int exponent[2];     // the fp16 arrays of x and w are 2^exponent as large
 };
 
-// Consecutive workgroups go to the eight XCDs in turn: give each XCD a run of
-// consecutive tiles, which read the same operands, for its L2.
-__device__ __forceinline__ int tile_of_block() {
-  const int blocks = gridDim.x, block = blockIdx.x, x = block % kXcds;
+// Workgroups go to the eight XCDs in turn. Each XCD gets a run of consecutive tiles,
+// which read the same operands, for its L2: the tile of workgroup `block` of `blocks`.
+__device__ __forceinline__ int tile_of_block(int block, int blocks) {
+  const int x = block % kXcds;
   return x * (blocks / kXcds) + min(x, blocks % kXcds) + block / kXcds;
 }
 
-// ------------------------------------------------------------- operands as planes
-__device__ __forceinline__ bool finite_bits(uint32_t magnitude) { return magnitude < 0x7f800000u; }
-
-__global__ __launch_bounds__(256) void largest_kernel(const float* x, int64_t nx, const float* w, int64_t nw, float* out) {
-  const float* const from = blockIdx.y ? w : x;
-  const int64_t n = blockIdx.y ? nw : nx;
-  uint32_t most = 0;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += kMaxBlocks * 256) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, from[i]) & 0x7fffffffu;
-    if (finite_bits(b)) most = max(most, b);
-  }
+// ------------------------------------------------------------- operands as fp16 arrays
+__device__ __forceinline__ uint32_t finite_magnitude(float v) {   // as an integer of the same order; 0 for the others
+  const uint32_t b = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), off)));
+  for (int off = 32; off > 0; off >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), off)));
+  return v;
+}
+__device__ __forceinline__ uint32_t block_max(uint32_t v) {   // of 256 threads
   __shared__ uint32_t part[4];
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
+  v = wave_max(v);
   __syncthreads();
-  if (threadIdx.x == 0)
-    out[blockIdx.y * kMaxBlocks + blockIdx.x] = __builtin_bit_cast(float, max(max(part[0], part[1]), max(part[2], part[3])));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return max(max(part[0], part[1]), max(part[2], part[3]));
 }
 
+// The largest magnitudes: of x, of w, and of the rows' factors of D. Row y of the grid
+// takes array y; each workgroup leaves one number.
+struct SurveyCall {
+  const void* from[2];       // null: not wanted
+  int64_t n[2];
+  const float *row_grad, *row_max;   // null: no backward
+  const int64_t* targets;
+  int64_t rows, ignore_index;
+  float l2wrap_scale;
+  float* residuals;          // [2, rows], cleared; may be null
+  uint32_t* largest;         // [3, kMaxBlocks]
+};
+template <bool BF>
+__global__ __launch_bounds__(256) void survey_kernel(const SurveyCall c) {
+  const int which = blockIdx.y;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, all = kMaxBlocks * 256;
+  uint32_t most = 0;
+  if (which < 2) {
+    if (!c.from[which]) return;
+    constexpr int kPer = BF ? 8 : 4;       // elements of 16 bytes
+    const int64_t n = c.n[which];
+    const bool whole = (reinterpret_cast<uintptr_t>(c.from[which]) & 15) == 0;
+    const int64_t pieces = whole ? n / kPer : 0;
+    const u32x4* const v = static_cast<const u32x4*>(c.from[which]);
+#pragma unroll 4
+    for (int64_t i = first; i < pieces; i += all) {
+      const u32x4 p = v[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (BF) {
+          most = max(most, finite_magnitude(__builtin_bit_cast(float, p[e] << 16)));
+          most = max(most, finite_magnitude(__builtin_bit_cast(float, p[e] & 0xffff0000u)));
+        } else {
+          most = max(most, finite_magnitude(__builtin_bit_cast(float, static_cast<uint32_t>(p[e]))));
+        }
+      }
+    }
+    for (int64_t i = pieces * kPer + first; i < n; i += all) {
+      if constexpr (BF) most = max(most, finite_magnitude(static_cast<float>(static_cast<const __bf16*>(c.from[which])[i])));
+      else most = max(most, finite_magnitude(static_cast<const float*>(c.from[which])[i]));
+    }
+  } else {
+    for (int64_t r = first; r < c.rows; r += all) {
+      if (c.residuals) c.residuals[r] = c.residuals[c.rows + r] = 0.f;
+      if (c.targets[r] == c.ignore_index) continue;
+      most = max(most, max(finite_magnitude(c.row_grad[r]), finite_magnitude(c.l2wrap_scale * c.row_max[r])));
+    }
+  }
+  most = block_max(most);
+  if (threadIdx.x == 0) c.largest[which * kMaxBlocks + blockIdx.x] = most;
+}
+
+// One array made of another: rows of `padded` elements, zeros behind the c there are.
+enum PackKind { kCopy, kToHalf, kToHalves };   // bf16 as it is; bf16 to fp16; fp32 to two of fp16
+struct PackJob {
+  const void* from;
+  char* to;
+  int64_t rows;
+  int kind, which;           // which: of the largest magnitudes
+};
 struct PackCall {
-  const void* from[2];
-  char* to[2];
-  int64_t rows[2];
-  int64_t c, padded;        // elements of a row, there and here
-  const float* largest;     // fp32: kMaxBlocks of each
+  PackJob job[3];
+  int jobs, c, padded;
+  bool factors;              // the backward's reference is wanted
+  const uint32_t* largest;
   Scalars* scalars;
 };
-// Rows of bf16 with zeros up to a whole step, or of fp32 as two fp16 arrays: x s = hi +
-// lo with s the power of two that brings the largest magnitude to 2^13 .. 2^14, lo
-// rounded to 11 bits or to a multiple of 2^-24.
-template <bool BF>
+// fp16 arrays are of x s, s the power of two that brings the largest magnitude to 2^13
+// .. 2^14: bf16 numbers of 2^-27 of it and more are held whole, smaller ones to 2^-38 of
+// it; of fp32 ones the second array holds what is left, rounded to 11 bits or likewise.
+__device__ __forceinline__ int exponent_of(uint32_t largest) {
+  return largest ? min(kHalfExponent - ilogbf(__builtin_bit_cast(float, largest)), 120) : 0;
+}
 __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
-  const int which = blockIdx.y;
-  const int64_t n = c.rows[which] * c.padded, plane = n;
+  const PackJob job = c.job[blockIdx.y];
+  const bool writes = blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0;
   int exponent = 0;
-  if constexpr (!BF) {
-    float most = c.largest[which * kMaxBlocks + threadIdx.x];
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off));
-    __shared__ float part[4];
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
-    __syncthreads();
-    most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    exponent = most > 0.f ? min(kHalfExponent - ilogbf(most), 120) : 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0) c.scalars->exponent[which] = exponent;
+  if (c.factors && blockIdx.x == 0 && blockIdx.y == 0) {
+    const uint32_t most = block_max(c.largest[2 * kMaxBlocks + threadIdx.x]);
+    // a gradient that is the same for all rows leaves exactly one, and so its own rounding out of D
+    if (writes) c.scalars->reference = most ? __builtin_bit_cast(float, most) : 1.f;
   }
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = i / c.padded, k = i % c.padded;
-    if constexpr (BF) {
-      reinterpret_cast<uint16_t*>(c.to[which])[i] = k < c.c ? static_cast<const uint16_t*>(c.from[which])[row * c.c + k] : 0;
-    } else {
-      const float v = k < c.c ? ldexpf(static_cast<const float*>(c.from[which])[row * c.c + k], exponent) : 0.f;
-      const _Float16 hi = static_cast<_Float16>(v);
-      _Float16* const to = reinterpret_cast<_Float16*>(c.to[which]);
-      to[i] = hi;
-      to[plane + i] = static_cast<_Float16>(v - static_cast<float>(hi));
+  if (static_cast<int>(blockIdx.y) >= c.jobs) return;
+  if (job.kind != kCopy) {
+    exponent = exponent_of(block_max(c.largest[job.which * kMaxBlocks + threadIdx.x]));
+    if (blockIdx.x == 0 && threadIdx.x == 0) c.scalars->exponent[job.which] = exponent;
+  }
+  const int lane = threadIdx.x & 63, pieces = c.padded / 8;
+  const int64_t plane = job.rows * c.padded;
+  const bool whole = c.c % 8 == 0;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); row < job.rows; row += gridDim.x * int64_t{4}) {
+    for (int i = lane; i < pieces; i += 64) {
+      float v[8];
+      const int64_t at = row * c.c + 8 * i;
+      if (job.kind == kToHalves) {
+        const float* const from = static_cast<const float*>(job.from) + at;
+        if (whole && 8 * i < c.c) {
+          const f32x4 a = reinterpret_cast<const f32x4*>(from)[0], b = reinterpret_cast<const f32x4*>(from)[1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = 8 * i + e < c.c ? from[e] : 0.f;
+        }
+        f16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float s = ldexpf(v[e], exponent);
+          hi[e] = static_cast<_Float16>(s);
+          lo[e] = static_cast<_Float16>(s - static_cast<float>(hi[e]));
+        }
+        _Float16* const to = reinterpret_cast<_Float16*>(job.to) + row * c.padded + 8 * i;
+        *reinterpret_cast<f16x8*>(to) = hi;
+        *reinterpret_cast<f16x8*>(to + plane) = lo;
+      } else {
+        const __bf16* const from = static_cast<const __bf16*>(job.from) + at;
+        bf16x8 raw;
+        if (whole && 8 * i < c.c) {
+          raw = *reinterpret_cast<const bf16x8*>(from);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) raw[e] = 8 * i + e < c.c ? from[e] : static_cast<__bf16>(0.f);
+        }
+        char* const to = job.to + (row * c.padded + 8 * i) * 2;
+        if (job.kind == kCopy) {
+          *reinterpret_cast<bf16x8*>(to) = raw;
+        } else {
+          f16x8 h;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h[e] = static_cast<_Float16>(ldexpf(static_cast<float>(raw[e]), exponent));
+          *reinterpret_cast<f16x8*>(to) = h;
+        }
+      }
     }
   }
 }
@@ -123,177 +218,185 @@ struct LogitsCall {
   Matrix x, w;
   int rows, vocab, steps;        // steps: c up to a whole step
   int first, words;              // the piece of the vocabulary, whole tiles
+  int tiles;
   const Scalars* scalars;
   const int64_t* targets;
   int64_t ignore_index;
-  // forward: [tiles, rows] each, and the targets' logits
+  // forward: [tiles of words, rows] each, and the targets' logits
   float *part_max, *part_sum, *row_target;
   int* part_argmax;
   // backward
   const float *row_lse, *row_max, *row_grad;
   const int32_t* row_argmax;
   float l2wrap_scale;
-  char* d;                       // [rows up to whole tiles, words] bf16, or two of fp16
+  char* d;                       // [rows up to whole tiles, words] fp16; for fp32 two of them
   int64_t d_plane;
+  float* residuals;              // [2, rows], bf16 operands: what rounding took from D at the target and at the argmax
 };
+
+// D as hidden_grad's products see it: rounded to fp16 and then to bf16.
+__device__ __forceinline__ float as_read(float v) {
+  return static_cast<float>(static_cast<__bf16>(static_cast<float>(static_cast<_Float16>(v))));
+}
 
 // A run of words whose rows of w stay in an XCD's L2 while the rows of x pass by.
 constexpr int kWordTiles = 8;
-template <bool BF>
-using LogitsTile = Tile<kRows, kRows, kWords, kRowsTile, kWavesP, kWavesQ, true, true, BF ? 1 : 2>;
-
 template <bool BF, bool kBackward>
 __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c) {
-  using T = LogitsTile<BF>;
+  using T = Tile<kRows, kRows, kWords, kRowsTile, kWavesP, kWavesQ, true, true, BF ? kBf16 : kHalves>;
   __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
   const int row_tiles = (c.rows + kRowsTile - 1) / kRowsTile, word_tiles = c.words / kWords;
-  const int at = tile_of_block();
-  const int run = at / (kWordTiles * row_tiles), in_run = at % (kWordTiles * row_tiles);
-  const int run_words = min(kWordTiles, word_tiles - run * kWordTiles);
-  const int word_tile = run * kWordTiles + in_run % run_words, row_tile = in_run / run_words;
-  const int v0 = c.first + word_tile * kWords, r0 = row_tile * kRowsTile;
+  // each XCD has a run of tiles, and its workgroups take them in turn
+  const int xcd = blockIdx.x % kXcds, local = blockIdx.x / kXcds, locals = (static_cast<int>(gridDim.x) - xcd + kXcds - 1) / kXcds;
+  const int each = c.tiles / kXcds, rest = c.tiles % kXcds;
+  const int last = (xcd + 1) * each + min(xcd + 1, rest);
+  int at = xcd * each + min(xcd, rest) + local;
   T t;
-  t.sum(lds, Operand{c.w.data + int64_t{v0} * c.w.pitch, c.w.pitch, c.vocab - v0, c.steps},
-        Operand{c.x.data + int64_t{r0} * c.x.pitch, c.x.pitch, c.rows - r0, c.steps}, c.w.plane, c.x.plane, 0, c.steps);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
-  // lane's words: this + 64 (i / 4) + 4 (i % 4) + element
-  const int word0 = v0 + wp * T::kWaveP + 16 * g;
-  if constexpr (!BF) {
-    const int exponent = -(c.scalars->exponent[0] + c.scalars->exponent[1]);
-#pragma unroll
-    for (int i = 0; i < T::kTilesP; ++i)
-#pragma unroll
-      for (int j = 0; j < T::kTilesQ; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t.acc[i][j][e] = ldexpf(t.acc[i][j][e], exponent);
-  }
-  if constexpr (!kBackward) {
-    if (v0 + kWords > c.vocab) {
-#pragma unroll
-      for (int i = 0; i < T::kTilesP; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (word0 + 64 * (i / 4) + 4 * (i % 4) + e >= c.vocab) {
-#pragma unroll
-            for (int j = 0; j < T::kTilesQ; ++j) t.acc[i][j][e] = -INFINITY;
-          }
-    }
-    float* const maxima = reinterpret_cast<float*>(lds);      // [kWavesP][kRowsTile] each
-    float* const sums = maxima + kWavesP * kRowsTile;
-    int* const firsts = reinterpret_cast<int*>(sums + kWavesP * kRowsTile);
-#pragma unroll
-    for (int j = 0; j < T::kTilesQ; ++j) {
-      const int in_tile = wq * T::kWaveQ + 16 * j + m;
-      const int row = r0 + in_tile;
-      float most = t.acc[0][j][0];
+  typename T::Work work;
+  int v0, r0;
+  auto begin = [&](int tile) {
+    const int run = tile / (kWordTiles * row_tiles), in_run = tile % (kWordTiles * row_tiles);
+    const int run_words = min(kWordTiles, word_tiles - run * kWordTiles);
+    v0 = c.first + (run * kWordTiles + in_run % run_words) * kWords;
+    r0 = in_run / run_words * kRowsTile;
+    T::begin(work, lds, Operand{c.w.data + int64_t{v0} * c.w.pitch, c.w.pitch, c.vocab - v0, c.steps},
+             Operand{c.x.data + int64_t{r0} * c.x.pitch, c.x.pitch, c.rows - r0, c.steps}, c.w.plane, c.x.plane, 0, c.steps);
+  };
+  if (at < last) begin(at);
+  for (; at < last; at += locals) {
+    t.run(work, lds);
+    const int v = v0, r = r0;
+    if (at + locals < last) begin(at + locals);   // its loads run under what follows
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
+    // lane's words: this + 64 (i / 4) + 4 (i % 4) + element
+    const int word0 = v + wp * T::kWaveP + 16 * g;
+    if constexpr (!BF) {
+      const int exponent = -(c.scalars->exponent[0] + c.scalars->exponent[1]);
 #pragma unroll
       for (int i = 0; i < T::kTilesP; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) most = fmaxf(most, t.acc[i][j][e]);
-      most = fmaxf(most, __shfl_xor(most, 16));
-      most = fmaxf(most, __shfl_xor(most, 32));
-      float sum = 0.f;
-      int first = INT_MAX;
+        for (int j = 0; j < T::kTilesQ; ++j)
 #pragma unroll
-      for (int i = T::kTilesP - 1; i >= 0; --i)
-#pragma unroll
-        for (int e = 3; e >= 0; --e) {
-          const float z = t.acc[i][j][e];
-          sum += __expf(z - most);
-          first = z == most ? 64 * (i / 4) + 4 * (i % 4) + e : first;
-        }
-      if (first != INT_MAX) first += wp * T::kWaveP + 16 * g;
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
-      first = min(first, __shfl_xor(first, 16));
-      first = min(first, __shfl_xor(first, 32));
-      if (g == 0) {
-        maxima[wp * kRowsTile + in_tile] = most;
-        sums[wp * kRowsTile + in_tile] = sum;
-        firsts[wp * kRowsTile + in_tile] = first;
-      }
-      if (row < c.rows) {
-        const int64_t own = c.targets[row] - word0;
-        if (own >= 0 && own < T::kWaveP && (own & 63) < 16) {
-#pragma unroll
-          for (int i = 0; i < T::kTilesP; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (own == 64 * (i / 4) + 4 * (i % 4) + e) c.row_target[row] = t.acc[i][j][e];
-        }
-      }
+          for (int e = 0; e < 4; ++e) t.acc[i][j][e] = ldexpf(t.acc[i][j][e], exponent);
     }
-    __syncthreads();
-    if (threadIdx.x < kRowsTile && r0 + threadIdx.x < c.rows) {
-      const int q = threadIdx.x;
-      const float a = maxima[q], b = maxima[kRowsTile + q];
-      const float most = fmaxf(a, b), sa = sums[q], sb = sums[kRowsTile + q];
-      const int64_t to = int64_t{v0 / kWords} * c.rows + r0 + q;
-      const int fa = firsts[q], fb = firsts[kRowsTile + q];
-      c.part_max[to] = most;
-      // a half without a word (or all of minus infinity) has a NaN for a sum
-      c.part_sum[to] = (a == -INFINITY ? 0.f : sa * __expf(a - most)) + (b == -INFINITY ? 0.f : sb * __expf(b - most));
-      const int f = a >= b ? fa : fb;
-      c.part_argmax[to] = f == INT_MAX ? INT_MAX : static_cast<int>(v0) + f;
-    }
-  } else {
-    const float reference = c.scalars->reference;
+    if constexpr (!kBackward) {
+      if (v + kWords > c.vocab) {
 #pragma unroll
-    for (int j = 0; j < T::kTilesQ; ++j) {
-      const int row = r0 + wq * T::kWaveQ + 16 * j + m, known = min(row, c.rows - 1);
-      const int64_t target = c.targets[known];
-      const bool dead = row >= c.rows || target == c.ignore_index;
-      const float lse = c.row_lse[known], h = c.row_grad[known] / reference;
-      const float wrap = c.l2wrap_scale * c.row_max[known] / reference;
-      const int64_t own = target - word0;
-      const int top = c.row_argmax[known] - word0;
+        for (int i = 0; i < T::kTilesP; ++i)
 #pragma unroll
-      for (int half = 0; half < T::kTilesP / 4; ++half) {
-        float v[16];
+          for (int e = 0; e < 4; ++e)
+            if (word0 + 64 * (i / 4) + 4 * (i % 4) + e >= c.vocab) {
 #pragma unroll
-        for (int n = 0; n < 16; ++n) v[n] = h * __expf(t.acc[4 * half + n / 4][j][n % 4] - lse);
-        if (own >= 64 * half && own < 64 * half + 16) {
-#pragma unroll
-          for (int n = 0; n < 16; ++n)
-            if (own == 64 * half + n) v[n] -= h;
-        }
-        if (top >= 64 * half && top < 64 * half + 16) {
-#pragma unroll
-          for (int n = 0; n < 16; ++n)
-            if (top == 64 * half + n) v[n] += wrap;
-        }
-        if (dead) {
-#pragma unroll
-          for (int n = 0; n < 16; ++n) v[n] = 0.f;
-        }
-        const int word = word0 + 64 * half;
-        if (word + 16 > c.vocab) {
-#pragma unroll
-          for (int n = 0; n < 16; ++n)
-            if (word + n >= c.vocab) v[n] = 0.f;
-        }
-        char* const to = c.d + (static_cast<int64_t>(row) * c.words + word - c.first) * 2;
-        if constexpr (BF) {
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            bf16x8 o;
-#pragma unroll
-            for (int n = 0; n < 8; ++n) o[n] = static_cast<__bf16>(v[8 * q + n]);
-            reinterpret_cast<bf16x8*>(to)[q] = o;
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            f16x8 hi, lo;
-#pragma unroll
-            for (int n = 0; n < 8; ++n) {
-              const float s = ldexpf(v[8 * q + n], kHalfExponent);
-              hi[n] = static_cast<_Float16>(s);
-              lo[n] = static_cast<_Float16>(s - static_cast<float>(hi[n]));
+              for (int j = 0; j < T::kTilesQ; ++j) t.acc[i][j][e] = -INFINITY;
             }
+      }
+      float* const maxima = reinterpret_cast<float*>(lds + T::kFree);      // [kWavesP][kRowsTile] each
+      float* const sums = maxima + kWavesP * kRowsTile;
+      int* const firsts = reinterpret_cast<int*>(sums + kWavesP * kRowsTile);
+#pragma unroll
+      for (int j = 0; j < T::kTilesQ; ++j) {
+        const int in_tile = wq * T::kWaveQ + 16 * j + m;
+        const int row = r + in_tile;
+        float most = t.acc[0][j][0];
+#pragma unroll
+        for (int i = 0; i < T::kTilesP; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) most = fmaxf(most, t.acc[i][j][e]);
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        float sum = 0.f;
+        int first = INT_MAX;
+#pragma unroll
+        for (int i = T::kTilesP - 1; i >= 0; --i)
+#pragma unroll
+          for (int e = 3; e >= 0; --e) {
+            const float z = t.acc[i][j][e];
+            sum += __expf(z - most);
+            first = z == most ? 64 * (i / 4) + 4 * (i % 4) + e : first;
+          }
+        if (first != INT_MAX) first += wp * T::kWaveP + 16 * g;
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        first = min(first, __shfl_xor(first, 16));
+        first = min(first, __shfl_xor(first, 32));
+        if (g == 0) {
+          maxima[wp * kRowsTile + in_tile] = most;
+          sums[wp * kRowsTile + in_tile] = sum;
+          firsts[wp * kRowsTile + in_tile] = first;
+        }
+        if (row < c.rows) {
+          const int64_t own = c.targets[row] - word0;
+          if (own >= 0 && own < T::kWaveP && (own & 63) < 16) {
+#pragma unroll
+            for (int i = 0; i < T::kTilesP; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (own == 64 * (i / 4) + 4 * (i % 4) + e) c.row_target[row] = t.acc[i][j][e];
+          }
+        }
+      }
+      __syncthreads();
+      if (threadIdx.x < kRowsTile && r + static_cast<int>(threadIdx.x) < c.rows) {
+        const int q = threadIdx.x;
+        const float a = maxima[q], b = maxima[kRowsTile + q];
+        const float most = fmaxf(a, b), sa = sums[q], sb = sums[kRowsTile + q];
+        const int64_t to = int64_t{v / kWords} * c.rows + r + q;
+        const int fa = firsts[q], fb = firsts[kRowsTile + q];
+        c.part_max[to] = most;
+        // a half without a word (or all of minus infinity) has a NaN for a sum
+        c.part_sum[to] = (a == -INFINITY ? 0.f : sa * __expf(a - most)) + (b == -INFINITY ? 0.f : sb * __expf(b - most));
+        const int f = a >= b ? fa : fb;
+        c.part_argmax[to] = f == INT_MAX ? INT_MAX : v + f;
+      }
+    } else {
+      const float reference = c.scalars->reference;
+#pragma unroll
+      for (int j = 0; j < T::kTilesQ; ++j) {
+        const int row = r + wq * T::kWaveQ + 16 * j + m, known = min(row, c.rows - 1);
+        const int64_t target = c.targets[known];
+        const bool dead = row >= c.rows || target == c.ignore_index;
+        const float lse = c.row_lse[known], h = ldexpf(c.row_grad[known] / reference, kHalfExponent);
+        const float wrap = ldexpf(c.l2wrap_scale * c.row_max[known] / reference, kHalfExponent);
+        const int64_t own = target < c.vocab ? target - word0 : -1;
+        const int top = c.row_argmax[known] - word0;
+#pragma unroll
+        for (int half = 0; half < T::kTilesP / 4; ++half) {
+          float d[16];
+#pragma unroll
+          for (int n = 0; n < 16; ++n) d[n] = h * __expf(t.acc[4 * half + n / 4][j][n % 4] - lse);
+          const bool has_own = own >= 64 * half && own < 64 * half + 16, has_top = top >= 64 * half && top < 64 * half + 16;
+          if (has_own || has_top) {
+#pragma unroll
+            for (int n = 0; n < 16; ++n) {
+              const bool is_own = own == 64 * half + n, is_top = top == 64 * half + n;
+              if (is_own) d[n] -= h;
+              if (is_top) d[n] += wrap;
+              if constexpr (BF) {
+                if (!dead && is_own) c.residuals[row] = d[n] - as_read(d[n]);
+                else if (!dead && is_top) c.residuals[c.rows + row] = d[n] - as_read(d[n]);
+              }
+            }
+          }
+          const int word = word0 + 64 * half;
+          if (dead || word + 16 > c.vocab) {
+#pragma unroll
+            for (int n = 0; n < 16; ++n)
+              if (dead || word + n >= c.vocab) d[n] = 0.f;
+          }
+          char* const to = c.d + (static_cast<int64_t>(row) * c.words + word - c.first) * 2;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            f16x8 hi;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) hi[n] = static_cast<_Float16>(d[8 * q + n]);
             reinterpret_cast<f16x8*>(to)[q] = hi;
-            reinterpret_cast<f16x8*>(to + c.d_plane)[q] = lo;
+            if constexpr (!BF) {
+              f16x8 lo;
+#pragma unroll
+              for (int n = 0; n < 8; ++n) lo[n] = static_cast<_Float16>(d[8 * q + n] - static_cast<float>(hi[n]));
+              reinterpret_cast<f16x8*>(to + c.d_plane)[q] = lo;
+            }
           }
         }
       }
@@ -325,7 +428,7 @@ __device__ __forceinline__ Run combine(const Run& a, const Run& b) {
 __global__ __launch_bounds__(256) void join_kernel(const JoinCall c) {
   __shared__ Run part[16][17];
   const int own = threadIdx.x & 15, share = threadIdx.x >> 4;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + own, tiles = ceil_div(c.vocab, kWords);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + own, tiles = (c.vocab + kWords - 1) / kWords;
   Run run{-INFINITY, 0.f, INT_MAX};
   if (row < c.rows) {
 #pragma unroll 4
@@ -352,41 +455,6 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinCall c) {
 }
 
 // ---------------------------------------------------------------------- gradients
-// What D is held over: the largest of the rows' factors. A gradient that is the same
-// for all rows leaves exactly one, and so its own rounding out of D.
-struct ReferenceCall {
-  const float *row_grad, *row_max;
-  const int64_t* targets;
-  int64_t rows, ignore_index;
-  float l2wrap_scale;
-  Scalars* scalars;
-};
-__global__ __launch_bounds__(1024) void reference_kernel(const ReferenceCall c) {
-  uint32_t most = 0;
-  for (int64_t r = threadIdx.x; r < c.rows; r += 1024) {
-    if (c.targets[r] == c.ignore_index) continue;
-    const uint32_t g = __builtin_bit_cast(uint32_t, c.row_grad[r]) & 0x7fffffffu;
-    const uint32_t w = __builtin_bit_cast(uint32_t, c.l2wrap_scale * c.row_max[r]) & 0x7fffffffu;
-    if (finite_bits(g)) most = max(most, g);
-    if (finite_bits(w)) most = max(most, w);
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), off)));
-  __shared__ uint32_t part[16];
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-#pragma unroll
-    for (int w = 1; w < 16; ++w) most = max(most, part[w]);
-    c.scalars->reference = most == 0 ? 1.f : __builtin_bit_cast(float, most);
-  }
-}
-
-template <bool BF>
-__device__ __forceinline__ float unscaled(float sum, float reference, int exponent) {
-  return BF ? sum * reference : ldexpf(sum, -(kHalfExponent + exponent)) * reference;
-}
-
 template <bool BF>
 __device__ __forceinline__ void store4(void* base, int64_t at, f32x4 v, int64_t left, bool whole) {
   if (whole) {
@@ -408,30 +476,37 @@ __device__ __forceinline__ void store4(void* base, int64_t at, f32x4 v, int64_t 
     }
 }
 
-struct WeightGradCall {
-  Matrix x;
+constexpr int kGradTile = 256;   // words or rows of a gradient's tile
+struct GradientsCall {
+  Matrix x, w;               // x: fp16; w: bf16, or fp16 for fp32
   const char* d;
   int64_t d_plane;
-  int words, padded_rows, rows, vocab, c, first;
+  int first, words, padded_rows, rows, vocab, c;
   const Scalars* scalars;
-  void* grad;
+  int weight_tiles, weight_blocks;   // workgroups of dw's tiles, up to whole rounds of the XCDs; then dx's
+  void* weight_grad;
+  int share;                 // words of a workgroup of dx
+  bool begin;                // the first piece: no sums to add to
+  float* sums;               // [splits, rows, pitch]
+  int pitch;
 };
-// dw of the piece's words: steps are rows; those past the last have D = 0.
+
+// A tile of dw, of the piece's words: steps are rows; those past the last have D = 0.
 template <bool BF, int kChannels>
-__global__ __launch_bounds__(kThreads, 2) void weight_grad_kernel(const WeightGradCall c) {
-  using T = Tile<kSteps, kSteps, kChannels, 256, kWavesP, kWavesQ, false, false, BF ? 1 : 2>;
-  __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
+__device__ __forceinline__ void weight_tile(const GradientsCall& c, char* lds, int at) {
+  using T = Tile<kSteps, kSteps, kChannels, kGradTile, kWavesP, kWavesQ, false, false, BF ? kHalf : kHalves>;
   const int channel_tiles = (c.c + kChannels - 1) / kChannels;
-  const int at = tile_of_block();
-  const int c0 = at % channel_tiles * kChannels, w0 = at / channel_tiles * 256;
-  const int steps = (c.rows + kStep - 1) / kStep * kStep;
+  const int c0 = at % channel_tiles * kChannels, w0 = at / channel_tiles * kGradTile;
   T t;
-  t.sum(lds, Operand{c.x.data + c0 * 2, c.x.pitch, c.c - c0, c.rows},
-        Operand{c.d + w0 * 2, int64_t{c.words} * 2, c.words - w0, c.padded_rows}, c.x.plane, c.d_plane, 0, steps);
+  typename T::Work work;
+  T::begin(work, lds, Operand{c.x.data + c0 * 2, c.x.pitch, c.c - c0, c.rows},
+           Operand{c.d + w0 * 2, int64_t{c.words} * 2, c.words - w0, c.padded_rows}, c.x.plane, c.d_plane, 0,
+           (c.rows + kStep - 1) / kStep * kStep);
+  t.run(work, lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
   const float reference = c.scalars->reference;
-  const int exponent = BF ? 0 : c.scalars->exponent[0];
+  const int exponent = -(kHalfExponent + c.scalars->exponent[0]);
   const bool whole = c.c % 4 == 0;
 #pragma unroll
   for (int j = 0; j < T::kTilesQ; ++j) {
@@ -443,34 +518,25 @@ __global__ __launch_bounds__(kThreads, 2) void weight_grad_kernel(const WeightGr
       if (channel >= c.c) continue;
       f32x4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = unscaled<BF>(t.acc[i][j][e], reference, exponent);
-      store4<BF>(c.grad, int64_t{word} * c.c + channel, v, c.c - channel, whole);
+      for (int e = 0; e < 4; ++e) v[e] = ldexpf(t.acc[i][j][e], exponent) * reference;
+      store4<BF>(c.weight_grad, int64_t{word} * c.c + channel, v, c.c - channel, whole);
     }
   }
 }
 
-struct HiddenGradCall {
-  Matrix w;
-  const char* d;
-  int64_t d_plane;
-  int words, rows, vocab, c, first;
-  int share;                 // words of a workgroup
-  bool begin;                // the first piece: nothing to add to
-  float* sums;               // [splits, rows, pitch]
-  int pitch;
-};
+// A tile of dx, over a share of the piece's words; the words past the vocabulary have D = 0.
 template <bool BF, int kChannels>
-__global__ __launch_bounds__(kThreads, 2) void hidden_grad_kernel(const HiddenGradCall c) {
-  using T = Tile<kSteps, kRows, kChannels, 256, kWavesP, kWavesQ, false, true, BF ? 1 : 2>;
-  __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
-  const int channel_tiles = (c.c + kChannels - 1) / kChannels, row_tiles = (c.rows + 255) / 256;
-  const int at = tile_of_block();
-  const int c0 = at % channel_tiles * kChannels, r0 = at / channel_tiles % row_tiles * 256;
+__device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, int at) {
+  using T = Tile<kSteps, kRows, kChannels, kGradTile, kWavesP, kWavesQ, false, true, BF ? kHalfQ : kHalves>;
+  const int channel_tiles = (c.c + kChannels - 1) / kChannels, row_tiles = c.padded_rows / kGradTile;
+  const int c0 = at % channel_tiles * kChannels, r0 = at / channel_tiles % row_tiles * kGradTile;
   const int split = at / channel_tiles / row_tiles;
   const int k0 = split * c.share, k1 = min(k0 + c.share, c.words);
   T t;
-  t.sum(lds, Operand{c.w.data + int64_t{c.first} * c.w.pitch + c0 * 2, c.w.pitch, c.c - c0, c.vocab - c.first},
-        Operand{c.d + int64_t{r0} * c.words * 2, int64_t{c.words} * 2, 256, c.words}, c.w.plane, c.d_plane, k0, k1);
+  typename T::Work work;
+  T::begin(work, lds, Operand{c.w.data + int64_t{c.first} * c.w.pitch + c0 * 2, c.w.pitch, c.c - c0, c.vocab - c.first},
+           Operand{c.d + int64_t{r0} * c.words * 2, int64_t{c.words} * 2, kGradTile, c.words}, c.w.plane, c.d_plane, k0, k1);
+  t.run(work, lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
 #pragma unroll
@@ -487,29 +553,68 @@ __global__ __launch_bounds__(kThreads, 2) void hidden_grad_kernel(const HiddenGr
   }
 }
 
-// The splits' sums of dx in order, in the operands' type.
+// Both gradients of a piece side by side: dw's tiles, then the shorter ones of dx, which
+// fill the compute units that have none of the last of dw's.
+template <bool BF, int kChannels>
+__global__ __launch_bounds__(kThreads, 2) void gradients_kernel(const GradientsCall c) {
+  using T = Tile<kSteps, kRows, kChannels, kGradTile, kWavesP, kWavesQ, false, true, kHalves>;
+  using U = Tile<kSteps, kSteps, kChannels, kGradTile, kWavesP, kWavesQ, false, false, kHalves>;
+  __shared__ __attribute__((aligned(16))) char lds[std::max(T::kLdsBytes, U::kLdsBytes)];
+  const int block = blockIdx.x, blocks = gridDim.x;
+  if (block < c.weight_blocks) {
+    const int at = tile_of_block(block, c.weight_blocks);
+    if (at < c.weight_tiles) weight_tile<BF, kChannels>(c, lds, at);
+  } else {
+    hidden_tile<BF, kChannels>(c, lds, tile_of_block(block - c.weight_blocks, blocks - c.weight_blocks));
+  }
+}
+
+// The splits' sums of dx in order, in the operands' type. For bf16 operands, what D's
+// rounding took at the target and at the argmax is put back: mostly that is nearly all
+// of a row's D, and its error would be as large as the result's own rounding.
 struct HiddenSumCall {
   const float* sums;
   int64_t rows, c, pitch;
   int splits;
   const Scalars* scalars;
   void* grad;
+  const float* residuals;
+  const int64_t* targets;
+  const int32_t* row_argmax;
+  const __bf16* weight;
 };
 template <bool BF>
 __global__ __launch_bounds__(256) void hidden_sum_kernel(const HiddenSumCall c) {
   const float reference = c.scalars->reference;
-  const int exponent = BF ? 0 : c.scalars->exponent[1];
+  const int exponent = -(kHalfExponent + (BF ? 0 : c.scalars->exponent[1]));
   const int64_t fours = c.pitch / 4, n = c.rows * fours;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= n) return;
   const int64_t row = i / fours, channel = i % fours * 4;
-  if (channel >= c.c) return;
   f32x4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = 0; s < c.splits; ++s) v += reinterpret_cast<const f32x4*>(c.sums)[s * n + i];
+  const bool whole = c.c % 4 == 0;
+  if constexpr (BF) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = unscaled<BF>(v[e], reference, exponent);
-  store4<BF>(c.grad, row * c.c + channel, v, c.c - channel, c.c % 4 == 0);
+    for (int k = 0; k < 2; ++k) {
+      const float r = c.residuals[k * c.rows + row];
+      if (r == 0.f) continue;                      // and so where there is no such word
+      const __bf16* const w = c.weight + (k ? c.row_argmax[row] : c.targets[row]) * c.c + channel;
+      if (whole) {
+        const bf16x4 b = *reinterpret_cast<const bf16x4*>(w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += r * static_cast<float>(b[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (channel + e < c.c) v[e] += r * static_cast<float>(w[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], exponent) * reference;
+  store4<BF>(c.grad, row * c.c + channel, v, c.c - channel, whole);
 }
 
 __global__ __launch_bounds__(256) void clear_kernel(uint32_t* to, int64_t words, int64_t bytes) {
@@ -522,37 +627,48 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t* to, int64_t words,
 // The bf16 operands whose rows are whole steps are read where they are.
 bool packed(int64_t c, bool bf16) { return !bf16 || c % kStep != 0; }
 
-struct Places {
-  int64_t scalars, largest, x, w, x_plane, w_plane;   // byte offsets; planes' sizes
-  int64_t end;
-};
 int64_t take(int64_t& end, int64_t bytes) {
   const int64_t at = end;
   end += up(bytes, 256);
   return at;
 }
-Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
+// Byte offsets of the operands in the workspace.
+struct Places {
+  int64_t scalars, largest, x, w, x_half, x_plane, w_plane;
+  int64_t end;
+};
+Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward) {
   Places p{};
   const int64_t pitch = up(c, kStep) * 2, planes = bf16 ? 1 : 2;
   p.scalars = take(p.end, sizeof(Scalars));
+  p.largest = take(p.end, 3 * kMaxBlocks * 4);
+  p.x_plane = rows * pitch;
+  p.w_plane = vocab * pitch;
   if (packed(c, bf16)) {
-    p.largest = take(p.end, 2 * kMaxBlocks * 4);
-    p.x_plane = rows * pitch;
-    p.w_plane = vocab * pitch;
     p.x = take(p.end, planes * p.x_plane);
     p.w = take(p.end, planes * p.w_plane);
   }
+  if (bf16 && backward) p.x_half = take(p.end, p.x_plane);
   return p;
 }
 
-// Two workgroups of a tile fill a compute unit.
-constexpr int64_t kSlots = kUnits;
-constexpr int64_t kMaxD = int64_t{512} << 20;   // bytes of D of a piece
+// D of a piece takes at most kMaxD bytes, of which the least is a tile of words. dx's
+// shares: those with which the two gradients' tiles, handed to the compute units in turn,
+// are done first, in stages; a tile's first loads and its stores count as kOverhead
+// stages, and the sums' way to memory and back as kBytesPerStage has it.
+constexpr int64_t kMaxD = int64_t{512} << 20, kOverhead = 4, kMaxSplits = 16, kBytesPerStage = int64_t{4} << 20;
 struct Plan {
   int channels;                     // of a gradient's tile
   int64_t words, pieces;            // of a piece
   int64_t padded_rows, splits, share, pitch;
 };
+int64_t finish(int64_t tiles, int64_t each, int64_t more, int64_t more_each) {
+  const int64_t whole = tiles / kUnits * each, late = tiles % kUnits;
+  for (int64_t at = whole + (late ? each : 0), k = (at - whole) / more_each;; ++k) {
+    const int64_t t = std::max(at, whole + k * more_each);
+    if ((kUnits - late) * ((t - whole) / more_each) + late * ((t - at) / more_each) >= more) return t;
+  }
+}
 Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   Plan p{};
   p.channels = (c - 1) % 256 < 128 ? 128 : 256;
@@ -561,29 +677,36 @@ Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   const int64_t channel_tiles = ceil_div(c, p.channels), planes = bf16 ? 1 : 2;
   const int64_t all = up(vocab, kWords);
   const int64_t most = std::max<int64_t>(kWords, kMaxD / (p.padded_rows * 2 * planes) / kWords * kWords);
-  // pieces of whole rounds of the weight gradient's tiles of 128 words
-  const int64_t round = std::max<int64_t>(kSlots / channel_tiles, 1) * 256;
-  p.words = std::min(all, most >= round ? most / round * round : most);
+  p.pieces = ceil_div(all, most);
+  p.words = up(ceil_div(all, p.pieces), kWords);
   p.pieces = ceil_div(all, p.words);
-  p.words = std::min(p.words, up(ceil_div(all, p.pieces), kWords) );
-  const int64_t tiles = channel_tiles * ceil_div(rows, 256);
-  p.splits = std::max<int64_t>(1, std::min<int64_t>(kSlots * 4 / tiles, p.words / 512));
-  p.share = up(ceil_div(p.words, p.splits), kStep);
-  p.splits = ceil_div(p.words, p.share);
+  const int64_t weight_tiles = channel_tiles * ceil_div(p.words, kGradTile), hidden_tiles = channel_tiles * p.padded_rows / kGradTile;
+  int64_t least = INT64_MAX;
+  for (int64_t s = 1; s <= kMaxSplits; ++s) {
+    const int64_t share = up(ceil_div(p.words, s), kStep), splits = ceil_div(p.words, share);
+    if (splits < s) continue;
+    const int64_t time = finish(weight_tiles, ceil_div(rows, kStep) + kOverhead, hidden_tiles * splits, share / kStep + kOverhead) +
+                         splits * rows * p.pitch * 8 / kBytesPerStage;
+    if (time >= least) continue;
+    least = time;
+    p.splits = splits;
+    p.share = share;
+  }
   return p;
 }
 
 struct BackwardPlaces {
   Places operands;
-  int64_t d, d_plane, sums, end;
+  int64_t d, d_plane, sums, residuals, end;
 };
 BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   BackwardPlaces b{};
-  b.operands = operands(rows, vocab, c, bf16);
+  b.operands = operands(rows, vocab, c, bf16, true);
   b.end = b.operands.end;
   b.d_plane = p.padded_rows * p.words * 2;
   b.d = take(b.end, b.d_plane * (bf16 ? 1 : 2));
   b.sums = take(b.end, p.splits * rows * p.pitch * 4);
+  b.residuals = take(b.end, 2 * rows * 4);
   return b;
 }
 
@@ -593,7 +716,7 @@ struct ForwardPlaces {
 };
 ForwardPlaces forward_places(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   ForwardPlaces f{};
-  f.operands = operands(rows, vocab, c, bf16);
+  f.operands = operands(rows, vocab, c, bf16, false);
   f.end = f.operands.end;
   const int64_t parts = ceil_div(vocab, kWords) * rows * 4;
   f.part_max = take(f.end, parts);
@@ -603,41 +726,71 @@ ForwardPlaces forward_places(int64_t rows, int64_t vocab, int64_t c, bool bf16) 
   return f;
 }
 
-// x and w as the tiles read them, made first where they are not so in memory.
+// x and w as the tiles read them (and x in fp16 for bf16 operands' weight gradient), made
+// first where they are not so in memory; the backward's factors.
+struct Operands {
+  Matrix x, w, x_half;
+};
 template <bool BF>
-void prepare(const Call& c, const Places& p, Matrix* x, Matrix* w, hipStream_t s) {
+Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* residuals, hipStream_t s) {
   const int64_t padded = up(c.c, kStep);
-  if (!packed(c.c, BF)) {
-    *x = Matrix{static_cast<const char*>(c.hidden), c.c * 2, 0};
-    *w = Matrix{static_cast<const char*>(c.weight), c.c * 2, 0};
-    return;
-  }
-  float* const largest = reinterpret_cast<float*>(c.workspace + p.largest);
-  if (!BF)
-    hipLaunchKernelGGL(largest_kernel, dim3(kMaxBlocks, 2), dim3(256), 0, s, static_cast<const float*>(c.hidden),
-                       c.rows * c.c, static_cast<const float*>(c.weight), c.vocab * c.c, largest);
+  Operands o;
+  o.x = Matrix{static_cast<const char*>(c.hidden), c.c * 2, 0};
+  o.w = Matrix{static_cast<const char*>(c.weight), c.c * 2, 0};
   PackCall k{};
-  k.from[0] = c.hidden;
-  k.from[1] = c.weight;
-  k.to[0] = c.workspace + p.x;
-  k.to[1] = c.workspace + p.w;
-  k.rows[0] = c.rows;
-  k.rows[1] = c.vocab;
-  k.c = c.c;
-  k.padded = padded;
+  auto pack = [&](const void* from, int64_t to, int64_t rows, int kind, int which, int64_t plane) {
+    k.job[k.jobs++] = PackJob{from, c.workspace + to, rows, kind, which};
+    return Matrix{c.workspace + to, padded * 2, plane};
+  };
+  if (packed(c.c, BF)) {
+    o.x = pack(c.hidden, p.x, c.rows, BF ? kCopy : kToHalves, 0, p.x_plane);
+    o.w = pack(c.weight, p.w, c.vocab, BF ? kCopy : kToHalves, 1, p.w_plane);
+  }
+  o.x_half = o.x;
+  if (BF && b && b->weight_grad) o.x_half = pack(c.hidden, p.x_half, c.rows, kToHalf, 0, 0);
+  if (k.jobs == 0 && !b) return o;
+  k.c = static_cast<int>(c.c);
+  k.padded = static_cast<int>(padded);
+  k.factors = b != nullptr;
+  uint32_t* const largest = reinterpret_cast<uint32_t*>(c.workspace + p.largest);
   k.largest = largest;
   k.scalars = reinterpret_cast<Scalars*>(c.workspace + p.scalars);
-  const int64_t blocks = std::min<int64_t>(ceil_div(std::max(c.rows, c.vocab) * padded, 1024), 4096);
-  hipLaunchKernelGGL(pack_kernel<BF>, dim3(static_cast<unsigned>(blocks), 2), dim3(256), 0, s, k);
-  *x = Matrix{k.to[0], padded * 2, p.x_plane};
-  *w = Matrix{k.to[1], padded * 2, p.w_plane};
+  SurveyCall v{};
+  if (!BF || (b && b->weight_grad)) v.from[0] = c.hidden;
+  if (!BF) v.from[1] = c.weight;
+  v.n[0] = c.rows * c.c;
+  v.n[1] = c.vocab * c.c;
+  v.largest = largest;
+  if (b) {
+    v.row_grad = b->row_grad;
+    v.row_max = b->row_max;
+    v.targets = c.targets;
+    v.rows = c.rows;
+    v.ignore_index = c.ignore_index;
+    v.l2wrap_scale = b->l2wrap_scale;
+    v.residuals = residuals;
+  }
+  if (v.from[0] || b) hipLaunchKernelGGL(survey_kernel<BF>, dim3(kMaxBlocks, b ? 3 : 2), dim3(256), 0, s, v);
+  int64_t rows = 1;
+  for (int i = 0; i < k.jobs; ++i) rows = std::max(rows, k.job[i].rows);
+  hipLaunchKernelGGL(pack_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(rows, 4), 2048)), std::max(k.jobs, 1)),
+                     dim3(256), 0, s, k);
+  return o;
+}
+
+template <bool BF, bool kBackward>
+void logits(LogitsCall& l, hipStream_t s) {
+  l.tiles = static_cast<int>(l.words / kWords * ceil_div(l.rows, kRowsTile));
+  hipLaunchKernelGGL((logits_kernel<BF, kBackward>), dim3(static_cast<unsigned>(std::min(l.tiles, kUnits))), dim3(kThreads), 0, s, l);
 }
 
 template <bool BF>
 void forward(const ForwardCall& c, hipStream_t s) {
   const ForwardPlaces f = forward_places(c.rows, c.vocab, c.c, BF);
+  const Operands o = prepare<BF>(c, f.operands, nullptr, nullptr, s);
   LogitsCall l{};
-  prepare<BF>(c, f.operands, &l.x, &l.w, s);
+  l.x = o.x;
+  l.w = o.w;
   l.rows = static_cast<int>(c.rows);
   l.vocab = static_cast<int>(c.vocab);
   l.steps = static_cast<int>(up(c.c, kStep));
@@ -648,42 +801,22 @@ void forward(const ForwardCall& c, hipStream_t s) {
   l.part_sum = reinterpret_cast<float*>(c.workspace + f.part_sum);
   l.part_argmax = reinterpret_cast<int*>(c.workspace + f.part_argmax);
   l.row_target = reinterpret_cast<float*>(c.workspace + f.row_target);
-  const int64_t tiles = l.words / kWords * ceil_div(c.rows, kRowsTile);
-  hipLaunchKernelGGL((logits_kernel<BF, false>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), 0, s, l);
+  logits<BF, false>(l, s);
   const JoinCall j{l.part_max, l.part_sum, l.row_target, l.part_argmax, c.targets, c.rows, c.vocab, c.ignore_index,
                    c.row_loss, c.row_lse, c.row_max, c.row_argmax};
   hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>(ceil_div(c.rows, 16))), dim3(256), 0, s, j);
-}
-
-template <bool BF, int kChannels>
-void gradients(const BackwardCall& c, const Plan& p, const BackwardPlaces& b, const LogitsCall& l, bool first, hipStream_t s) {
-  const int64_t channel_tiles = ceil_div(c.c, kChannels);
-  if (c.weight_grad) {
-    const WeightGradCall w{l.x, l.d, l.d_plane, l.words, static_cast<int>(p.padded_rows), l.rows, l.vocab, static_cast<int>(c.c),
-                           l.first, l.scalars, c.weight_grad};
-    const int words = std::min(l.words, l.vocab - l.first);
-    hipLaunchKernelGGL((weight_grad_kernel<BF, kChannels>), dim3(static_cast<unsigned>(channel_tiles * ceil_div(words, 256))),
-                       dim3(kThreads), 0, s, w);
-  }
-  if (c.hidden_grad) {
-    const int64_t splits = ceil_div(l.words, p.share);
-    const HiddenGradCall h{l.w, l.d, l.d_plane, l.words, l.rows, l.vocab, static_cast<int>(c.c), l.first,
-                           static_cast<int>(p.share), first, reinterpret_cast<float*>(c.workspace + b.sums),
-                           static_cast<int>(p.pitch)};
-    hipLaunchKernelGGL((hidden_grad_kernel<BF, kChannels>),
-                       dim3(static_cast<unsigned>(channel_tiles * ceil_div(c.rows, 256) * splits)), dim3(kThreads), 0, s, h);
-  }
 }
 
 template <bool BF>
 void backward(const BackwardCall& c, hipStream_t s) {
   const Plan p = plan(c.rows, c.vocab, c.c, BF);
   const BackwardPlaces b = backward_places(p, c.rows, c.vocab, c.c, BF);
+  float* const residuals = BF ? reinterpret_cast<float*>(c.workspace + b.residuals) : nullptr;
+  const Operands o = prepare<BF>(c, b.operands, &c, residuals, s);
+  const Scalars* const scalars = reinterpret_cast<const Scalars*>(c.workspace + b.operands.scalars);
   LogitsCall l{};
-  prepare<BF>(c, b.operands, &l.x, &l.w, s);
-  Scalars* const scalars = reinterpret_cast<Scalars*>(c.workspace + b.operands.scalars);
-  const ReferenceCall r{c.row_grad, c.row_max, c.targets, c.rows, c.ignore_index, c.l2wrap_scale, scalars};
-  hipLaunchKernelGGL(reference_kernel, dim3(1), dim3(1024), 0, s, r);
+  l.x = o.x;
+  l.w = o.w;
   l.rows = static_cast<int>(c.rows);
   l.vocab = static_cast<int>(c.vocab);
   l.steps = static_cast<int>(up(c.c, kStep));
@@ -697,17 +830,37 @@ void backward(const BackwardCall& c, hipStream_t s) {
   l.l2wrap_scale = c.l2wrap_scale;
   l.d = c.workspace + b.d;
   l.d_plane = b.d_plane;
+  l.residuals = residuals;
+  GradientsCall g{};
+  g.x = o.x_half;
+  g.w = o.w;
+  g.d = l.d;
+  g.d_plane = l.d_plane;
+  g.padded_rows = static_cast<int>(p.padded_rows);
+  g.rows = l.rows;
+  g.vocab = l.vocab;
+  g.c = static_cast<int>(c.c);
+  g.scalars = scalars;
+  g.weight_grad = c.weight_grad;
+  g.share = static_cast<int>(p.share);
+  g.sums = reinterpret_cast<float*>(c.workspace + b.sums);
+  g.pitch = static_cast<int>(p.pitch);
+  const int64_t channel_tiles = ceil_div(c.c, p.channels);
   for (int64_t first = 0; first < c.vocab; first += p.words) {
-    l.first = static_cast<int>(first);
-    l.words = static_cast<int>(std::min(p.words, up(c.vocab - first, kWords)));
-    const int64_t tiles = l.words / kWords * ceil_div(c.rows, kRowsTile);
-    hipLaunchKernelGGL((logits_kernel<BF, true>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), 0, s, l);
-    if (p.channels == 128) gradients<BF, 128>(c, p, b, l, first == 0, s);
-    else gradients<BF, 256>(c, p, b, l, first == 0, s);
+    g.first = l.first = static_cast<int>(first);
+    g.words = l.words = static_cast<int>(std::min(p.words, up(c.vocab - first, kWords)));
+    logits<BF, true>(l, s);
+    g.begin = first == 0;
+    g.weight_tiles = c.weight_grad ? static_cast<int>(channel_tiles * (l.words / kGradTile)) : 0;
+    g.weight_blocks = static_cast<int>(up(g.weight_tiles, kXcds));
+    const int64_t hidden_blocks = c.hidden_grad ? channel_tiles * (p.padded_rows / kGradTile) * ceil_div(l.words, p.share) : 0;
+    const dim3 grid(static_cast<unsigned>(g.weight_blocks + hidden_blocks));
+    if (p.channels == 128) hipLaunchKernelGGL((gradients_kernel<BF, 128>), grid, dim3(kThreads), 0, s, g);
+    else hipLaunchKernelGGL((gradients_kernel<BF, 256>), grid, dim3(kThreads), 0, s, g);
   }
   if (c.hidden_grad) {
-    const HiddenSumCall h{reinterpret_cast<const float*>(c.workspace + b.sums), c.rows, c.c, p.pitch,
-                          static_cast<int>(p.splits), scalars, c.hidden_grad};
+    const HiddenSumCall h{g.sums, c.rows, c.c, p.pitch, static_cast<int>(p.splits), scalars, c.hidden_grad,
+                          residuals, c.targets, c.row_argmax, BF ? static_cast<const __bf16*>(c.weight) : nullptr};
     hipLaunchKernelGGL(hidden_sum_kernel<BF>, dim3(static_cast<unsigned>(ceil_div(c.rows * p.pitch / 4, 256))), dim3(256),
                        0, s, h);
   }

@@ -31,12 +31,20 @@ constexpr int kStep = 64;              // steps of k a stage: whole cache lines 
 constexpr int kStepBytes = kStep * 2;
 constexpr int kPieces = kStepBytes / 16;
 
-template <bool kHalf>   // fp16 operands, or bf16
+template <bool kFp16>   // or bf16
 __device__ __forceinline__ f32x4 multiply(s16x8 p, s16x8 q, f32x4 c) {
-  if constexpr (kHalf)
+  if constexpr (kFp16)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ s16x8 half_to_bf16(s16x8 v) {
+  const f16x8 h = __builtin_bit_cast(f16x8, v);
+  bf16x8 b;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) b[e] = static_cast<__bf16>(static_cast<float>(h[e]));
+  return __builtin_bit_cast(s16x8, b);
 }
 
 // 16 bytes from each lane's offset to consecutive places from `to` on. A buffer load:
@@ -148,15 +156,17 @@ struct Side {
   }
 };
 
-// kPlanes 1: bf16 operands. 2: each operand is two fp16 arrays, the second (`plane`
-// bytes behind the first) holding what rounding took from the first: the product is
-// hi hi + hi lo + lo hi.
-//
+// What the operands are: kBf16; kHalf, both fp16; kHalfQ, P bf16 and Q fp16, which is
+// rounded to bf16 on its way to the products; kHalves, each two fp16 arrays, the second
+// (`plane` bytes behind the first) holding what rounding took from the first: the
+// product is hi hi + hi lo + lo hi.
+enum Kind { kBf16, kHalf, kHalfQ, kHalves };
+
 // LDS holds three stages of one operand and two of the other (kDeepP: three of P). The
 // loop's barrier lies kTail groups of products before a stage's end, when all of the
 // stage has been read: behind it the next stage's first reads and the loads that
 // overwrite this one are issued under the products that are left.
-template <Layout kLayoutP, Layout kLayoutQ, int kP, int kQ, int kWavesP, int kWavesQ, bool kSpread, bool kDeepP, int kPlanes>
+template <Layout kLayoutP, Layout kLayoutQ, int kP, int kQ, int kWavesP, int kWavesQ, bool kSpread, bool kDeepP, Kind kKind>
 struct Tile {
   static constexpr int kWaves = kWavesP * kWavesQ, kThreads = 64 * kWaves;
   static constexpr int kWaveP = kP / kWavesP, kWaveQ = kQ / kWavesQ;
@@ -168,7 +178,7 @@ struct Tile {
   static constexpr int kPlaceQ = kSlotsP * SideP::kBytes;
   static constexpr int kLdsBytes = kPlaceQ + kSlotsQ * SideQ::kBytes;
   static constexpr int kDeepLoads = kDeepP ? SideP::kLoads : SideQ::kLoads;
-  static constexpr int kParts = kPlanes == 1 ? 1 : 3;
+  static constexpr int kParts = kKind == kHalves ? 3 : 1;
   static constexpr int kTail = kTilesP / 2, kBody = 2 * kTilesP - kTail;   // groups of kTilesQ products
   static constexpr int kHeldP = 2;
 
@@ -201,8 +211,8 @@ struct Tile {
     SideQ q;
     int64_t plane_p, plane_q;
     int wave, lane;
-    __device__ __forceinline__ Buffer from(const Next<kSlotsP>& n) const { return p.stage(kPlanes > 1 && n.part == 2 ? plane_p : 0, n.k); }
-    __device__ __forceinline__ Buffer from(const Next<kSlotsQ>& n, int) const { return q.stage(kPlanes > 1 && n.part == 1 ? plane_q : 0, n.k); }
+    __device__ __forceinline__ Buffer from(const Next<kSlotsP>& n) const { return p.stage(kKind == kHalves && n.part == 2 ? plane_p : 0, n.k); }
+    __device__ __forceinline__ Buffer from(const Next<kSlotsQ>& n, int) const { return q.stage(kKind == kHalves && n.part == 1 ? plane_q : 0, n.k); }
     __device__ __forceinline__ s16x8 read_p(const char* lds, int half, int i) const {
       return p.read(lds, half, wave % kWavesP * kWaveP, i, lane & 15, lane >> 4);
     }
@@ -218,7 +228,7 @@ struct Tile {
   }
   __device__ __forceinline__ void products(int i, s16x8 p, const s16x8 (&q)[kTilesQ]) {
 #pragma unroll
-    for (int j = 0; j < kTilesQ; ++j) acc[i][j] = multiply<(kPlanes > 1)>(p, q[j], acc[i][j]);
+    for (int j = 0; j < kTilesQ; ++j) acc[i][j] = multiply<(kKind == kHalf || kKind == kHalves)>(p, q[j], acc[i][j]);
   }
 
   // From one barrier to the next: the products that are left of the stage before, and
@@ -256,6 +266,12 @@ struct Tile {
         else if (n < kHolds) held.p[n - kTilesQ] = a.read_p(p, 0, n - kTilesQ);
       }
       if constexpr (!kFirst) products(kTilesP - kTail + i, held.last_p[i], held.last_q);
+      if constexpr (kKind == kHalfQ) {
+        // two groups behind the reads; what the tail cannot hold, before the products
+#pragma unroll
+        for (int n = (i - 2) * kHoldsPerGroup; n < (i == kTail - 1 ? kTilesQ : (i - 1) * kHoldsPerGroup); ++n)
+          if (n >= 0 && n < kTilesQ) held.q[n] = half_to_bf16(held.q[n]);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     s16x8 at[2][kTilesP];
@@ -270,6 +286,13 @@ struct Tile {
         if (n < kTilesP - kHeldP) at[0][n + kHeldP] = a.read_p(p, 0, n + kHeldP);
         else if (n < kTilesP - kHeldP + kTilesQ) held.last_q[n - (kTilesP - kHeldP)] = a.read_q(q, 1, n - (kTilesP - kHeldP));
         else if (n < kReads) at[1][n - (kTilesP - kHeldP + kTilesQ)] = a.read_p(p, 1, n - (kTilesP - kHeldP + kTilesQ));
+      }
+      if constexpr (kKind == kHalfQ) {
+        // a part of them before each group of products, none left before their own
+        constexpr int kEach = (kTilesQ + kTilesP / 2 - 1) / (kTilesP / 2);
+#pragma unroll
+        for (int n = (i - (kTilesP - kTilesP / 2)) * kEach; n < (i - (kTilesP - kTilesP / 2) + 1) * kEach; ++n)
+          if (i < kTilesP && n >= 0 && n < kTilesQ) held.last_q[n] = half_to_bf16(held.last_q[n]);
       }
       if (i < kTilesP) products(i, at[0][i % kTilesP], held.q);
       else products(i - kTilesP, at[1][i % kTilesP], held.last_q);
@@ -288,47 +311,59 @@ struct Tile {
     asm volatile("" ::: "memory");
   }
 
-  // Sums over the steps [k0, k1), whole stages. The workgroup may use `lds` again
-  // once all of its waves have come back.
-  __device__ __forceinline__ void sum(char* lds, const Operand& p, const Operand& q, int64_t plane_p, int64_t plane_q,
-                                      int k0, int k1) {
+  // A sum over the steps [k0, k1), whole stages: begin() asks for the first ones, run()
+  // forms it in acc. Between the two, `lds` is free from kFree on.
+  static constexpr int kFree = kDeepP ? 2 * SideP::kBytes : SideP::kBytes;   // a slot that begin() leaves
+  struct Work {
     Place a;
-    a.lane = threadIdx.x & 63;
-    a.wave = uniform(static_cast<int>(threadIdx.x >> 6));
-    a.p.init(p, a.wave, a.lane);
-    a.q.init(q, a.wave, a.lane);
-    a.plane_p = plane_p;
-    a.plane_q = plane_q;
-#pragma unroll
-    for (int i = 0; i < kTilesP; ++i)
-#pragma unroll
-      for (int j = 0; j < kTilesQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Next<kSlotsP> next_p{k0, 0, 0};
-    Next<kSlotsQ> next_q{k0, 0, 0};
+    int k0, k1;
+    Next<kSlotsP> next_p;
+    Next<kSlotsQ> next_q;
+  };
+  __device__ __forceinline__ static void begin(Work& w, char* lds, const Operand& p, const Operand& q, int64_t plane_p,
+                                               int64_t plane_q, int k0, int k1) {
+    w.a.lane = threadIdx.x & 63;
+    w.a.wave = uniform(static_cast<int>(threadIdx.x >> 6));
+    w.a.p.init(p, w.a.wave, w.a.lane);
+    w.a.q.init(q, w.a.wave, w.a.lane);
+    w.a.plane_p = plane_p;
+    w.a.plane_q = plane_q;
+    w.k0 = k0;
+    w.k1 = k1;
+    w.next_p = {k0, 0, 0};
+    w.next_q = {k0, 0, 0};
     auto all_p = [&] {
-      const Buffer from = a.from(next_p);
+      const Buffer from = w.a.from(w.next_p);
 #pragma unroll
-      for (int n = 0; n < SideP::kLoads; ++n) bring_p(n, lds, a, from, next_p);
-      next_p.advance(k0, k1);
+      for (int n = 0; n < SideP::kLoads; ++n) bring_p(n, lds, w.a, from, w.next_p);
+      w.next_p.advance(k0, k1);
     };
     auto all_q = [&] {
-      const Buffer from = a.from(next_q, 0);
+      const Buffer from = w.a.from(w.next_q, 0);
 #pragma unroll
-      for (int n = 0; n < SideQ::kLoads; ++n) bring_q(n, lds, a, from, next_q);
-      next_q.advance(k0, k1);
+      for (int n = 0; n < SideQ::kLoads; ++n) bring_q(n, lds, w.a, from, w.next_q);
+      w.next_q.advance(k0, k1);
     };
     all_p();
     all_q();
     kDeepP ? all_p() : all_q();
-    const int stages = (k1 - k0) / kStep * kParts;
+  }
+  // The workgroup may use `lds` again once all of its waves have come back.
+  __device__ __forceinline__ void run(Work& w, char* lds) {
+#pragma unroll
+    for (int i = 0; i < kTilesP; ++i)
+#pragma unroll
+      for (int j = 0; j < kTilesQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int stages = (w.k1 - w.k0) / kStep * kParts;
     int slot_p = 0, slot_q = 0;
     Held held;
     auto one = [&](auto first) {
       arrive<kDeepLoads>();
-      step<decltype(first)::value>(lds + next_p.slot * SideP::kBytes, lds + kPlaceQ + next_q.slot * SideQ::kBytes,
-                                   lds + slot_p * SideP::kBytes, lds + kPlaceQ + slot_q * SideQ::kBytes, held, a, next_p, next_q);
-      next_p.advance(k0, k1);
-      next_q.advance(k0, k1);
+      step<decltype(first)::value>(lds + w.next_p.slot * SideP::kBytes, lds + kPlaceQ + w.next_q.slot * SideQ::kBytes,
+                                   lds + slot_p * SideP::kBytes, lds + kPlaceQ + slot_q * SideQ::kBytes, held, w.a, w.next_p,
+                                   w.next_q);
+      w.next_p.advance(w.k0, w.k1);
+      w.next_q.advance(w.k0, w.k1);
       slot_p = slot_p == kSlotsP - 1 ? 0 : slot_p + 1;
       slot_q = slot_q == kSlotsQ - 1 ? 0 : slot_q + 1;
     };
