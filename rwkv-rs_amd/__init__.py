@@ -10,6 +10,8 @@ C ABI (include/wkv7.h) that mirrors rwkv-nn's Burn WKV7 operator traits.
 * ``w4``        -- linear layers with 4-bit weights, for serving
 * ``token_scores`` -- log probability of given tokens, entropy and top
   alternatives of logits, with their gradient
+* ``lm_loss``   -- the training loss, of logits or straight from hidden states
+* ``dropout``   -- dropout whose mask is drawn again instead of being stored
 * ``weights``   -- RWKV-7 release checkpoints (.pth) mapped onto ``model``
 """
 
@@ -20,6 +22,6 @@ from . import synthetic  # noqa: F401
 
 def __getattr__(name):
     if name in ("wkv7", "_native", "build", "model", "neighbors", "weights", "lm_loss", "decode",
-                "w4", "token_scores"):
+                "w4", "token_scores", "dropout"):
         return importlib.import_module(f"{__name__}.{name}")
     raise AttributeError(name)

@@ -96,6 +96,9 @@ LINEAR_LOSS_EXPORTS = ("rwkv_linear_loss_forward_workspace_bytes",
                        "rwkv_linear_loss_backward_workspace_bytes",
                        "rwkv_linear_loss_forward", "rwkv_linear_loss_backward")
 
+# and of include/rwkv_dropout.h
+DROPOUT_EXPORTS = ("rwkv_dropout",)
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
@@ -158,6 +161,7 @@ _SIGNATURES = {
     "rwkv_linear_loss_forward": ([_P] * 3 + [_I64] * 3 + [_INT, _I64] + [_P] * 5 + [_I64, _P], _INT),
     "rwkv_linear_loss_backward": ([_P] * 7 + [ctypes.c_float] + [_I64] * 3 + [_INT, _I64]
                                   + [_P] * 3 + [_I64, _P], _INT),
+    "rwkv_dropout": ([_P] * 3 + [_I64, ctypes.c_double, _I64] + [_INT] * 2 + [_P] * 2, _INT),
 }
 
 _lib = None

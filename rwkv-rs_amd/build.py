@@ -24,7 +24,7 @@ SOURCES = ["wkv7_api.cpp", "wkv7_forward.hip", "wkv7_backward.hip", "wkv7_infer.
            "wkv7_selftest.hip",
            "neighbors_api.cpp", "neighbors.hip", "lm_loss_api.cpp", "lm_loss.hip",
            "decode_api.cpp", "decode.hip", "w4_api.cpp", "w4.hip", "token_scores_api.cpp", "token_scores.hip",
-           "linear_loss_api.cpp", "linear_loss.hip"]
+           "linear_loss_api.cpp", "linear_loss.hip", "dropout_api.cpp", "dropout.hip"]
 ARCH = "gfx950"
 
 
