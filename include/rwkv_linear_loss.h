@@ -13,19 +13,24 @@
  *   loss_r = lse_r - z_r,t_r
  * to row_loss, row_lse, row_max (fp32 [rows]) and row_argmax (int32 [rows], the
  * first index of the row's maximum); the last three are kept for the backward. A
- * row whose target is ignore_index has loss 0; one whose target is otherwise
- * outside [0, vocab) a NaN loss. A row with a NaN or an infinite logit has a NaN
- * loss too.
+ * row whose target is ignore_index has loss 0, and nothing depends on its hidden
+ * state; one whose target is otherwise outside [0, vocab) has a NaN loss. A row with a NaN or
+ * plus infinity among its logits has a NaN loss; minus infinity is a probability of
+ * 0 (bf16 operands; fp32 ones' products make it NaN).
  *
  * Backward, with g_r = row_loss_grad[r] (fp32 [rows]):
  *   D_rj = g_r (exp(z_rj - lse_r) - [j == t_r]) + [j == argmax_r] l2wrap_scale max_r
  *   hidden_grad = D weight,   weight_grad = D^T hidden
  * in dtype, each rounded once; either pointer may be NULL (not wanted). A row
  * whose target is ignore_index has D = 0; a target otherwise outside [0, vocab)
- * no target term. z is formed again, a piece of the vocabulary at a time. D over
- * the call's largest |g_r| or |l2wrap_scale max_r| is rounded to bf16 for bf16
- * operands (half a step, 2^-9, of each D_rj) and held in two fp16 numbers (22 bits)
- * for fp32 ones.
+ * no target term. z is formed again, a piece of the vocabulary at a time, with at
+ * most 512 MiB of D in memory (or a tile of 256 words). D is held in fp16, over the
+ * call's largest |g_r| or |l2wrap_scale max_r| and with what the power of two 2^13
+ * makes of it: 11 bits of each element, but never finer than 2^-38 of that largest
+ * factor; for fp32 operands in two such numbers, 22 bits. The hidden gradient's
+ * products round it to bf16 for bf16 operands, but for the target and the argmax,
+ * whose error is put back; the weight gradient's are fp16, of hidden states scaled by
+ * a power of two (exact but below 2^-27 of the largest magnitude).
  *
  * fp32 operands are multiplied as two fp16 numbers each, after a power of two that
  * brings the operand's largest magnitude to 2^13 .. 2^14: 22 bits of each element, but
@@ -44,10 +49,11 @@
 extern "C" {
 #endif
 
-/* The most of each size. */
+/* The most of each size, and of an operand's elements. */
 #define RWKV_LINEAR_LOSS_MAX_ROWS (1 << 22)
 #define RWKV_LINEAR_LOSS_MAX_VOCAB (1 << 22)
 #define RWKV_LINEAR_LOSS_MAX_C (1 << 16)
+#define RWKV_LINEAR_LOSS_MAX_ELEMENTS ((int64_t)1 << 33)
 
 /* Device memory that a call asks for (16-byte aligned, no initialisation; calls
  * that may overlap in time need one each), or -1 for sizes or a dtype that are not

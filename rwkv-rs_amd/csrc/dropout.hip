@@ -4,6 +4,8 @@
 // A thread draws one Philox4x32-10 block, eight 16-bit numbers, for eight consecutive
 // elements: sixteen bits decide as well as 32 do (p is a multiple of 2^-16, and what
 // is kept is scaled by the probability in use), for half the multiplications.
+#include <algorithm>
+
 #include "dropout_launch.hpp"
 
 namespace rwkv_drop {
@@ -68,44 +70,50 @@ __device__ __forceinline__ void store_eight(void* base, int64_t i, const float (
 // kWhole: all operands begin on a 16-byte boundary, and so does every eight of them.
 template <bool BF, bool OBF, bool kAdd, bool kWhole>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(const Call c) {
-  const int64_t q = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, i = q * kEach;
-  if (i >= c.n) return;
-  const bool full = kWhole && i + kEach <= c.n;
-  float x[kEach], r[kEach];
-  if (full) {
-    load_eight<BF>(c.x, i, x);
-    if constexpr (kAdd) load_eight<OBF>(c.residual, i, r);
-  } else {
+  const uint64_t seed = static_cast<uint64_t>(c.rng[0]);
+  const uint32_t step = static_cast<uint32_t>(c.rng[1]);
+  const float scale = c.threshold ? 65536.f / static_cast<float>(c.threshold) : 0.f;
+  const int64_t groups = (c.n + kEach - 1) / kEach;
+  for (int64_t q = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; q < groups; q += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t i = q * kEach;
+    const bool full = kWhole && i + kEach <= c.n;
+    float x[kEach], r[kEach];
+    if (full) {
+      load_eight<BF>(c.x, i, x);
+      if constexpr (kAdd) load_eight<OBF>(c.residual, i, r);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        x[e] = i + e < c.n ? load_one<BF>(c.x, i + e) : 0.f;
+        if constexpr (kAdd) r[e] = i + e < c.n ? load_one<OBF>(c.residual, i + e) : 0.f;
+      }
+    }
+    const Words u = philox(static_cast<uint64_t>(q), c.site, step, seed);
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      x[e] = i + e < c.n ? load_one<BF>(c.x, i + e) : 0.f;
-      if constexpr (kAdd) r[e] = i + e < c.n ? load_one<OBF>(c.residual, i + e) : 0.f;
+      const uint32_t number = e % 2 ? u.w[e / 2] >> 16 : u.w[e / 2] & 0xffffu;
+      x[e] = number < c.threshold ? x[e] * scale : 0.f;
+      if constexpr (kAdd) x[e] += r[e];
+    }
+    if (full) {
+      store_eight<OBF>(c.out, i, x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (i + e < c.n) {
+          if constexpr (OBF) static_cast<__bf16*>(c.out)[i + e] = static_cast<__bf16>(x[e]);
+          else static_cast<float*>(c.out)[i + e] = x[e];
+        }
     }
   }
-  const Words u = philox(static_cast<uint64_t>(q), c.site, static_cast<uint32_t>(c.rng[1]), static_cast<uint64_t>(c.rng[0]));
-  const float scale = c.threshold ? 65536.f / static_cast<float>(c.threshold) : 0.f;
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const uint32_t number = e % 2 ? u.w[e / 2] >> 16 : u.w[e / 2] & 0xffffu;
-    x[e] = number < c.threshold ? x[e] * scale : 0.f;
-    if constexpr (kAdd) x[e] += r[e];
-  }
-  if (full) {
-    store_eight<OBF>(c.out, i, x);
-  } else {
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      if (i + e < c.n) {
-        if constexpr (OBF) static_cast<__bf16*>(c.out)[i + e] = static_cast<__bf16>(x[e]);
-        else static_cast<float*>(c.out)[i + e] = x[e];
-      }
-  }
 }
+
+constexpr int64_t kMostBlocks = 1 << 22;   // a launch has fewer than 2^32 threads; beyond, a thread takes several eights
 
 template <bool BF, bool OBF, bool kAdd>
 void launch(const Call& c, hipStream_t s) {
   const uintptr_t places = reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.residual) | reinterpret_cast<uintptr_t>(c.out);
-  const dim3 grid(static_cast<unsigned>((c.n + kThreads * kEach - 1) / (kThreads * kEach)));
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((c.n + kThreads * kEach - 1) / (kThreads * kEach), kMostBlocks)));
   if ((places & 15) == 0) hipLaunchKernelGGL((dropout_kernel<BF, OBF, kAdd, true>), grid, dim3(kThreads), 0, s, c);
   else hipLaunchKernelGGL((dropout_kernel<BF, OBF, kAdd, false>), grid, dim3(kThreads), 0, s, c);
 }

@@ -76,11 +76,13 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v) {   // of 256 threads
   return max(max(part[0], part[1]), max(part[2], part[3]));
 }
 
-// The largest magnitudes: of x, of w, and of the rows' factors of D. Row y of the grid
-// takes array y; each workgroup leaves one number.
+// The largest magnitudes: of x but for the rows that are ignored (whatever stands there
+// is nobody's measure), of w, and of the rows' factors of D. Row y of the grid takes
+// array y; each workgroup leaves one number.
 struct SurveyCall {
   const void* from[2];       // null: not wanted
-  int64_t n[2];
+  int64_t n[2];              // rows
+  int64_t c;
   const float *row_grad, *row_max;   // null: no backward
   const int64_t* targets;
   int64_t rows, ignore_index;
@@ -91,34 +93,37 @@ struct SurveyCall {
 template <bool BF>
 __global__ __launch_bounds__(256) void survey_kernel(const SurveyCall c) {
   const int which = blockIdx.y;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, all = kMaxBlocks * 256;
   uint32_t most = 0;
   if (which < 2) {
     if (!c.from[which]) return;
     constexpr int kPer = BF ? 8 : 4;       // elements of 16 bytes
-    const int64_t n = c.n[which];
-    const bool whole = (reinterpret_cast<uintptr_t>(c.from[which]) & 15) == 0;
-    const int64_t pieces = whole ? n / kPer : 0;
-    const u32x4* const v = static_cast<const u32x4*>(c.from[which]);
+    const int lane = threadIdx.x & 63;
+    const int pieces = (reinterpret_cast<uintptr_t>(c.from[which]) & 15) == 0 && c.c % kPer == 0 ? static_cast<int>(c.c / kPer) : 0;
+    for (int64_t row = blockIdx.x * 4 + (threadIdx.x >> 6); row < c.n[which]; row += kMaxBlocks * 4) {
+      if (which == 0 && c.targets[row] == c.ignore_index) continue;
+      const u32x4* const v = reinterpret_cast<const u32x4*>(static_cast<const char*>(c.from[which]) + row * c.c * (BF ? 2 : 4));
 #pragma unroll 4
-    for (int64_t i = first; i < pieces; i += all) {
-      const u32x4 p = v[i];
+      for (int i = lane; i < pieces; i += 64) {
+        const u32x4 p = v[i];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (BF) {
-          most = max(most, finite_magnitude(__builtin_bit_cast(float, p[e] << 16)));
-          most = max(most, finite_magnitude(__builtin_bit_cast(float, p[e] & 0xffff0000u)));
-        } else {
-          most = max(most, finite_magnitude(__builtin_bit_cast(float, static_cast<uint32_t>(p[e]))));
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (BF) {
+            most = max(most, finite_magnitude(__builtin_bit_cast(float, p[e] << 16)));
+            most = max(most, finite_magnitude(__builtin_bit_cast(float, p[e] & 0xffff0000u)));
+          } else {
+            most = max(most, finite_magnitude(__builtin_bit_cast(float, static_cast<uint32_t>(p[e]))));
+          }
+        }
+      }
+      if (pieces == 0) {
+        for (int64_t i = row * c.c + lane; i < (row + 1) * c.c; i += 64) {
+          if constexpr (BF) most = max(most, finite_magnitude(static_cast<float>(static_cast<const __bf16*>(c.from[which])[i])));
+          else most = max(most, finite_magnitude(static_cast<const float*>(c.from[which])[i]));
         }
       }
     }
-    for (int64_t i = pieces * kPer + first; i < n; i += all) {
-      if constexpr (BF) most = max(most, finite_magnitude(static_cast<float>(static_cast<const __bf16*>(c.from[which])[i])));
-      else most = max(most, finite_magnitude(static_cast<const float*>(c.from[which])[i]));
-    }
   } else {
-    for (int64_t r = first; r < c.rows; r += all) {
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; r < c.rows; r += kMaxBlocks * 256) {
       if (c.residuals) c.residuals[r] = c.residuals[c.rows + r] = 0.f;
       if (c.targets[r] == c.ignore_index) continue;
       most = max(most, max(finite_magnitude(c.row_grad[r]), finite_magnitude(c.l2wrap_scale * c.row_max[r])));
@@ -140,12 +145,15 @@ struct PackCall {
   PackJob job[3];
   int jobs, c, padded;
   bool factors;              // the backward's reference is wanted
+  const int64_t* targets;
+  int64_t ignore_index;
   const uint32_t* largest;
   Scalars* scalars;
 };
 // fp16 arrays are of x s, s the power of two that brings the largest magnitude to 2^13
 // .. 2^14: bf16 numbers of 2^-27 of it and more are held whole, smaller ones to 2^-38 of
 // it; of fp32 ones the second array holds what is left, rounded to 11 bits or likewise.
+// Ignored rows of x become zeros: a NaN there does not reach the weight's gradient.
 __device__ __forceinline__ int exponent_of(uint32_t largest) {
   return largest ? min(kHalfExponent - ilogbf(__builtin_bit_cast(float, largest)), 120) : 0;
 }
@@ -167,10 +175,15 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
   const int64_t plane = job.rows * c.padded;
   const bool whole = c.c % 8 == 0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); row < job.rows; row += gridDim.x * int64_t{4}) {
+    const bool ignored = job.kind != kCopy && job.which == 0 && c.targets[row] == c.ignore_index;
     for (int i = lane; i < pieces; i += 64) {
-      float v[8];
       const int64_t at = row * c.c + 8 * i;
-      if (job.kind == kToHalves) {
+      if (ignored) {
+        char* const to = job.to + (row * c.padded + 8 * i) * 2;
+        *reinterpret_cast<u32x4*>(to) = u32x4{0, 0, 0, 0};
+        if (job.kind == kToHalves) *reinterpret_cast<u32x4*>(to + plane * 2) = u32x4{0, 0, 0, 0};
+      } else if (job.kind == kToHalves) {
+        float v[8];
         const float* const from = static_cast<const float*>(job.from) + at;
         if (whole && 8 * i < c.c) {
           const f32x4 a = reinterpret_cast<const f32x4*>(from)[0], b = reinterpret_cast<const f32x4*>(from)[1];
@@ -326,7 +339,8 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
           firsts[wp * kRowsTile + in_tile] = first;
         }
         if (row < c.rows) {
-          const int64_t own = c.targets[row] - word0;
+          const int64_t target = c.targets[row];
+          const int own = target >= 0 && target < c.vocab ? static_cast<int>(target) - word0 : -1;
           if (own >= 0 && own < T::kWaveP && (own & 63) < 16) {
 #pragma unroll
             for (int i = 0; i < T::kTilesP; ++i)
@@ -351,15 +365,28 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
       }
     } else {
       const float reference = c.scalars->reference;
+      struct Row {
+        float lse, h, wrap;
+        int own, top;
+        bool dead;
+      } of[T::kTilesQ];
 #pragma unroll
-      for (int j = 0; j < T::kTilesQ; ++j) {
+      for (int j = 0; j < T::kTilesQ; ++j) {      // all rows' numbers are asked for at once
         const int row = r + wq * T::kWaveQ + 16 * j + m, known = min(row, c.rows - 1);
         const int64_t target = c.targets[known];
-        const bool dead = row >= c.rows || target == c.ignore_index;
-        const float lse = c.row_lse[known], h = ldexpf(c.row_grad[known] / reference, kHalfExponent);
-        const float wrap = ldexpf(c.l2wrap_scale * c.row_max[known] / reference, kHalfExponent);
-        const int64_t own = target < c.vocab ? target - word0 : -1;
-        const int top = c.row_argmax[known] - word0;
+        of[j].dead = row >= c.rows || target == c.ignore_index;
+        of[j].own = target >= 0 && target < c.vocab ? static_cast<int>(target) - word0 : -1;
+        of[j].top = c.row_argmax[known] - word0;
+        of[j].lse = c.row_lse[known];
+        of[j].h = c.row_grad[known];
+        of[j].wrap = c.l2wrap_scale * c.row_max[known];
+      }
+#pragma unroll
+      for (int j = 0; j < T::kTilesQ; ++j) {
+        const int row = r + wq * T::kWaveQ + 16 * j + m;
+        const float lse = of[j].lse, h = ldexpf(of[j].h / reference, kHalfExponent), wrap = ldexpf(of[j].wrap / reference, kHalfExponent);
+        const int own = of[j].own, top = of[j].top;
+        const bool dead = of[j].dead;
 #pragma unroll
         for (int half = 0; half < T::kTilesP / 4; ++half) {
           float d[16];
@@ -476,6 +503,44 @@ __device__ __forceinline__ void store4(void* base, int64_t at, f32x4 v, int64_t 
     }
 }
 
+// dx of four channels from its sum, in the operands' type. For bf16 operands, what D's
+// rounding took at the target and at the argmax is put back: mostly that is nearly all
+// of a row's D, and its error would be as large as the result's own rounding.
+struct HiddenCall {
+  void* grad;
+  int64_t c, rows;
+  const float* residuals;
+  const int64_t* targets;
+  const int32_t* row_argmax;
+  const __bf16* weight;
+};
+template <bool BF>
+__device__ __forceinline__ void finish_hidden(const HiddenCall& c, const Scalars* scalars, int64_t row, int64_t channel, f32x4 v) {
+  const float reference = scalars->reference;
+  const int exponent = -(kHalfExponent + (BF ? 0 : scalars->exponent[1]));
+  const bool whole = c.c % 4 == 0;
+  if constexpr (BF) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float r = c.residuals[k * c.rows + row];
+      if (r == 0.f) continue;                      // and so where there is no such word
+      const __bf16* const w = c.weight + (k ? c.row_argmax[row] : c.targets[row]) * c.c + channel;
+      if (whole) {
+        const bf16x4 b = *reinterpret_cast<const bf16x4*>(w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += r * static_cast<float>(b[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (channel + e < c.c) v[e] += r * static_cast<float>(w[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], exponent) * reference;
+  store4<BF>(c.grad, row * c.c + channel, v, c.c - channel, whole);
+}
+
 constexpr int kGradTile = 256;   // words or rows of a gradient's tile
 struct GradientsCall {
   Matrix x, w;               // x: fp16; w: bf16, or fp16 for fp32
@@ -487,8 +552,9 @@ struct GradientsCall {
   void* weight_grad;
   int share;                 // words of a workgroup of dx
   bool begin;                // the first piece: no sums to add to
-  float* sums;               // [splits, rows, pitch]
+  float* sums;               // [splits, rows, pitch]; null: one share and one piece, dx itself is stored
   int pitch;
+  HiddenCall hidden;
 };
 
 // A tile of dw, of the piece's words: steps are rows; those past the last have D = 0.
@@ -547,6 +613,10 @@ __device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, i
     for (int i = 0; i < T::kTilesP; ++i) {
       const int channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
       if (channel >= c.pitch) continue;
+      if (!c.sums) {
+        finish_hidden<BF>(c.hidden, c.scalars, row, channel, t.acc[i][j]);
+        continue;
+      }
       f32x4* const to = reinterpret_cast<f32x4*>(c.sums + (int64_t{split} * c.rows + row) * c.pitch + channel);
       *to = c.begin ? t.acc[i][j] : *to + t.acc[i][j];
     }
@@ -569,58 +639,28 @@ __global__ __launch_bounds__(kThreads, 2) void gradients_kernel(const GradientsC
   }
 }
 
-// The splits' sums of dx in order, in the operands' type. For bf16 operands, what D's
-// rounding took at the target and at the argmax is put back: mostly that is nearly all
-// of a row's D, and its error would be as large as the result's own rounding.
+// The splits' sums of dx in order.
 struct HiddenSumCall {
   const float* sums;
-  int64_t rows, c, pitch;
+  int64_t rows, pitch;
   int splits;
   const Scalars* scalars;
-  void* grad;
-  const float* residuals;
-  const int64_t* targets;
-  const int32_t* row_argmax;
-  const __bf16* weight;
+  HiddenCall hidden;
 };
 template <bool BF>
 __global__ __launch_bounds__(256) void hidden_sum_kernel(const HiddenSumCall c) {
-  const float reference = c.scalars->reference;
-  const int exponent = -(kHalfExponent + (BF ? 0 : c.scalars->exponent[1]));
   const int64_t fours = c.pitch / 4, n = c.rows * fours;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int64_t row = i / fours, channel = i % fours * 4;
-  f32x4 v{0.f, 0.f, 0.f, 0.f};
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+    f32x4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = 0; s < c.splits; ++s) v += reinterpret_cast<const f32x4*>(c.sums)[s * n + i];
-  const bool whole = c.c % 4 == 0;
-  if constexpr (BF) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float r = c.residuals[k * c.rows + row];
-      if (r == 0.f) continue;                      // and so where there is no such word
-      const __bf16* const w = c.weight + (k ? c.row_argmax[row] : c.targets[row]) * c.c + channel;
-      if (whole) {
-        const bf16x4 b = *reinterpret_cast<const bf16x4*>(w);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += r * static_cast<float>(b[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (channel + e < c.c) v[e] += r * static_cast<float>(w[e]);
-      }
-    }
+    for (int s = 0; s < c.splits; ++s) v += reinterpret_cast<const f32x4*>(c.sums)[s * n + i];
+    finish_hidden<BF>(c.hidden, c.scalars, i / fours, i % fours * 4, v);
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], exponent) * reference;
-  store4<BF>(c.grad, row * c.c + channel, v, c.c - channel, whole);
 }
 
 __global__ __launch_bounds__(256) void clear_kernel(uint32_t* to, int64_t words, int64_t bytes) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i < words) to[i] = 0;
-  else if (i == words && bytes % 4) *reinterpret_cast<uint16_t*>(to + words) = 0;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < words; i += static_cast<int64_t>(gridDim.x) * 256) to[i] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && bytes % 4) *reinterpret_cast<uint16_t*>(to + words) = 0;
 }
 
 // ------------------------------------------------------------------ plan, workspace
@@ -705,7 +745,7 @@ BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64
   b.end = b.operands.end;
   b.d_plane = p.padded_rows * p.words * 2;
   b.d = take(b.end, b.d_plane * (bf16 ? 1 : 2));
-  b.sums = take(b.end, p.splits * rows * p.pitch * 4);
+  b.sums = p.splits == 1 && p.pieces == 1 ? 0 : take(b.end, p.splits * rows * p.pitch * 4);
   b.residuals = take(b.end, 2 * rows * 4);
   return b;
 }
@@ -758,15 +798,16 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
   SurveyCall v{};
   if (!BF || (b && b->weight_grad)) v.from[0] = c.hidden;
   if (!BF) v.from[1] = c.weight;
-  v.n[0] = c.rows * c.c;
-  v.n[1] = c.vocab * c.c;
+  v.n[0] = c.rows;
+  v.n[1] = c.vocab;
+  v.c = c.c;
   v.largest = largest;
+  k.targets = v.targets = c.targets;
+  k.ignore_index = v.ignore_index = c.ignore_index;
   if (b) {
     v.row_grad = b->row_grad;
     v.row_max = b->row_max;
-    v.targets = c.targets;
     v.rows = c.rows;
-    v.ignore_index = c.ignore_index;
     v.l2wrap_scale = b->l2wrap_scale;
     v.residuals = residuals;
   }
@@ -777,6 +818,9 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
                      dim3(256), 0, s, k);
   return o;
 }
+
+// workgroups of 256 for n threads; a launch has fewer than 2^32 of these
+dim3 grid_of(int64_t n) { return dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n, 256), 1 << 22))); }
 
 template <bool BF, bool kBackward>
 void logits(LogitsCall& l, hipStream_t s) {
@@ -843,7 +887,10 @@ void backward(const BackwardCall& c, hipStream_t s) {
   g.scalars = scalars;
   g.weight_grad = c.weight_grad;
   g.share = static_cast<int>(p.share);
-  g.sums = reinterpret_cast<float*>(c.workspace + b.sums);
+  const bool direct = p.splits == 1 && p.pieces == 1;
+  g.sums = direct ? nullptr : reinterpret_cast<float*>(c.workspace + b.sums);
+  g.hidden = HiddenCall{c.hidden_grad, c.c, c.rows, residuals, c.targets, c.row_argmax,
+                        BF ? static_cast<const __bf16*>(c.weight) : nullptr};
   g.pitch = static_cast<int>(p.pitch);
   const int64_t channel_tiles = ceil_div(c.c, p.channels);
   for (int64_t first = 0; first < c.vocab; first += p.words) {
@@ -858,11 +905,9 @@ void backward(const BackwardCall& c, hipStream_t s) {
     if (p.channels == 128) hipLaunchKernelGGL((gradients_kernel<BF, 128>), grid, dim3(kThreads), 0, s, g);
     else hipLaunchKernelGGL((gradients_kernel<BF, 256>), grid, dim3(kThreads), 0, s, g);
   }
-  if (c.hidden_grad) {
-    const HiddenSumCall h{g.sums, c.rows, c.c, p.pitch, static_cast<int>(p.splits), scalars, c.hidden_grad,
-                          residuals, c.targets, c.row_argmax, BF ? static_cast<const __bf16*>(c.weight) : nullptr};
-    hipLaunchKernelGGL(hidden_sum_kernel<BF>, dim3(static_cast<unsigned>(ceil_div(c.rows * p.pitch / 4, 256))), dim3(256),
-                       0, s, h);
+  if (c.hidden_grad && !direct) {
+    const HiddenSumCall h{g.sums, c.rows, p.pitch, static_cast<int>(p.splits), scalars, g.hidden};
+    hipLaunchKernelGGL(hidden_sum_kernel<BF>, grid_of(c.rows * p.pitch / 4), dim3(256), 0, s, h);
   }
 }
 
@@ -884,7 +929,7 @@ hipError_t launch_forward(const ForwardCall& c, hipStream_t s) {
 hipError_t launch_backward(const BackwardCall& c, hipStream_t s) {
   if (c.rows == 0) {   // no row: no gradient of the weight
     const int64_t bytes = c.vocab * c.c * (c.bf16 ? 2 : 4);
-    hipLaunchKernelGGL(clear_kernel, dim3(static_cast<unsigned>(ceil_div(bytes / 4 + 1, 256))), dim3(256), 0, s,
+    hipLaunchKernelGGL(clear_kernel, grid_of(bytes / 4 + 1), dim3(256), 0, s,
                        static_cast<uint32_t*>(c.weight_grad), bytes / 4, bytes);
   } else {
     c.bf16 ? backward<true>(c, s) : backward<false>(c, s);

@@ -40,7 +40,8 @@ bool any_overlap(Ranges outs, Ranges ins) {
 
 bool sizes_ok(int64_t rows, int64_t vocab, int64_t c) {
   return rows >= 0 && rows <= RWKV_LINEAR_LOSS_MAX_ROWS && vocab > 0 && vocab <= RWKV_LINEAR_LOSS_MAX_VOCAB &&
-         c > 0 && c <= RWKV_LINEAR_LOSS_MAX_C;
+         c > 0 && c <= RWKV_LINEAR_LOSS_MAX_C && rows * c <= RWKV_LINEAR_LOSS_MAX_ELEMENTS &&
+         vocab * c <= RWKV_LINEAR_LOSS_MAX_ELEMENTS;
 }
 bool dtype_ok(int dtype) { return dtype == WKV7_DTYPE_F32 || dtype == WKV7_DTYPE_BF16; }
 int64_t size_of(int dtype) { return dtype == WKV7_DTYPE_BF16 ? 2 : 4; }

@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .neighbors import _code, _ptr, _stream
+from .neighbors import _code, _on, _ptr, _stream
 
 LOW32 = 0xFFFFFFFF
 
@@ -31,9 +31,10 @@ def _check(x: torch.Tensor, p: float, rng: torch.Tensor, site: int) -> None:
 
 def _run(x, residual, rng, site, p, out_dtype):
     out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    _native.check(_native.lib().rwkv_dropout(
-        x.data_ptr(), _ptr(residual), rng.data_ptr(), site, p, x.numel(), _code(x.dtype),
-        _code(out_dtype), out.data_ptr(), _stream(x.device)))
+    with _on(x.device):
+        _native.check(_native.lib().rwkv_dropout(
+            x.data_ptr(), _ptr(residual), rng.data_ptr(), site, p, x.numel(), _code(x.dtype),
+            _code(out_dtype), out.data_ptr(), _stream(x.device)))
     return out
 
 
@@ -48,8 +49,15 @@ class _Dropout(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
-        rng, = ctx.saved_tensors
-        return _Dropout.apply(grad, rng, *ctx.args), None, None, None, None
+        return _backward(ctx, grad), None, None, None, None
+
+
+def _backward(ctx, grad):
+    rng, = ctx.saved_tensors
+    if torch.is_grad_enabled():        # a gradient of the gradient is wanted
+        return _Dropout.apply(grad, rng, *ctx.args)
+    site, p, dtype = ctx.args
+    return _run(grad.contiguous(), None, rng, site, p, dtype)
 
 
 class _DropoutAdd(torch.autograd.Function):
@@ -61,9 +69,7 @@ class _DropoutAdd(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
-        rng, = ctx.saved_tensors
-        dx = _Dropout.apply(grad, rng, *ctx.args) if ctx.needs_input_grad[1] else None
-        return grad, dx, None, None, None
+        return grad, _backward(ctx, grad) if ctx.needs_input_grad[1] else None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, site: int = 0) -> torch.Tensor:
@@ -96,18 +102,24 @@ def keep_probability(p: float) -> float:
     return round((1.0 - p) * 65536) / 65536
 
 
-def keep_mask(shape, p: float, rng: torch.Tensor, site: int = 0) -> torch.Tensor:
-    """The elements that ``dropout`` of a tensor of this shape keeps, as a bool tensor
-    on ``rng``'s device, in plain torch (Philox4x32-10 in int64 arithmetic)."""
-    n = torch.Size(shape).numel()
-    q = torch.arange(-(-n // 8), device=rng.device)
-    seed, step = rng[0], rng[1] & LOW32
-    c = [q & LOW32, q >> 32, torch.full_like(q, site), step.expand_as(q)]
+def _philox(c0, c1, c2, c3, seed):
+    """Philox4x32-10 of the counters c0 .. c3 and the key ``seed`` (int64 tensors, the
+    former below 2^32): four words."""
+    c = [c0, c1, c2, c3]
     k = [seed & LOW32, (seed >> 32) & LOW32]
     for _ in range(10):
         a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57     # modulo 2^64: the shift's sign bits are masked off
         c = [((b >> 32) & LOW32) ^ c[1] ^ k[0], b & LOW32, ((a >> 32) & LOW32) ^ c[3] ^ k[1], a & LOW32]
         k = [(k[0] + 0x9E3779B9) & LOW32, (k[1] + 0xBB67AE85) & LOW32]
-    words = torch.stack(c, dim=1)
+    return c
+
+
+def keep_mask(shape, p: float, rng: torch.Tensor, site: int = 0) -> torch.Tensor:
+    """The elements that ``dropout`` of a tensor of this shape keeps, as a bool tensor
+    on ``rng``'s device, in plain torch."""
+    n = torch.Size(shape).numel()
+    q = torch.arange(-(-n // 8), device=rng.device)
+    step = (rng[1] & LOW32).expand_as(q)
+    words = torch.stack(_philox(q & LOW32, q >> 32, torch.full_like(q, site), step, rng[0]), dim=1)
     numbers = torch.stack([words & 0xFFFF, words >> 16], dim=2).reshape(-1)[:n].reshape(shape)
     return numbers < round((1.0 - p) * 65536)

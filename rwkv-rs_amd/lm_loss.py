@@ -21,7 +21,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .neighbors import _code, _no_tangent, _ptr, _stream
+from .neighbors import _code, _no_tangent, _on, _ptr, _stream
 
 L2WRAP_FACTOR = 1e-4     # kernels/l2wrap/mod.rs:61-62
 IGNORE_INDEX = -100      # a target that is not learned, as torch's cross entropy has it
@@ -81,23 +81,26 @@ def _workspace(which: str, rows: int, vocab: int, c: int, code: int, device) -> 
 
 
 def _linear_forward(hidden, weight, targets, ignore_index):
-    """Loss, log-sum-exp, maximum and argmax of every row."""
+    """Every row's loss, and what the backward needs of it: a [3, rows] tensor of its
+    log-sum-exp, its maximum and (as int32) its argmax."""
     (rows, c), vocab, dev = hidden.shape, weight.shape[0], hidden.device
     code = _code(hidden.dtype)
-    loss, lse, mx = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(3))
-    arg = torch.empty(rows, dtype=torch.int32, device=dev)
+    loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    kept = torch.empty(3, rows, dtype=torch.float32, device=dev)
+    at = kept.data_ptr()
     ws, nbytes = _workspace("forward", rows, vocab, c, code, dev)
-    _native.call("rwkv_linear_loss_forward", _ptr(hidden), _ptr(weight), _ptr(targets), rows, vocab, c,
-                 code, ignore_index, _ptr(loss), _ptr(lse), _ptr(mx), _ptr(arg), _ptr(ws), nbytes,
-                 _stream(dev))
-    return loss, lse, mx, arg
+    with _on(dev):
+        _native.check(_native.lib().rwkv_linear_loss_forward(
+            hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), rows, vocab, c, code, ignore_index,
+            loss.data_ptr(), at, at + 4 * rows, at + 8 * rows, ws.data_ptr(), nbytes, _stream(dev)))
+    return loss, kept
 
 
 class _LinearCrossEntropyL2Wrap(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, num_tokens, ignore_index):
-        loss, lse, mx, arg = _linear_forward(hidden, weight, targets, ignore_index)
-        ctx.save_for_backward(hidden, weight, targets, lse, mx, arg)
+        loss, kept = _linear_forward(hidden, weight, targets, ignore_index)
+        ctx.save_for_backward(hidden, weight, targets, kept)
         ctx.scale = L2WRAP_FACTOR / num_tokens if num_tokens > 0 else 0.0
         ctx.ignore_index = ignore_index
         return loss
@@ -105,16 +108,18 @@ class _LinearCrossEntropyL2Wrap(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        hidden, weight, targets, lse, mx, arg = ctx.saved_tensors
+        hidden, weight, targets, kept = ctx.saved_tensors
         (rows, c), vocab, dev = hidden.shape, weight.shape[0], hidden.device
-        code = _code(hidden.dtype)
+        code, at = _code(hidden.dtype), kept.data_ptr()
         g = dloss.to(torch.float32).contiguous()
         dhidden, dweight = (torch.empty_like(t) if need else None
                             for t, need in zip((hidden, weight), ctx.needs_input_grad))
         ws, nbytes = _workspace("backward", rows, vocab, c, code, dev)
-        _native.call("rwkv_linear_loss_backward", _ptr(hidden), _ptr(weight), _ptr(targets), _ptr(lse),
-                     _ptr(mx), _ptr(arg), _ptr(g), ctx.scale, rows, vocab, c, code, ctx.ignore_index,
-                     _ptr(dhidden), _ptr(dweight), _ptr(ws), nbytes, _stream(dev))
+        with _on(dev):
+            _native.check(_native.lib().rwkv_linear_loss_backward(
+                hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), at, at + 4 * rows, at + 8 * rows,
+                g.data_ptr(), ctx.scale, rows, vocab, c, code, ctx.ignore_index, _ptr(dhidden), _ptr(dweight),
+                ws.data_ptr(), nbytes, _stream(dev)))
         return dhidden, dweight, None, None, None
 
 
@@ -128,8 +133,8 @@ def linear_cross_entropy_l2wrap_rows(hidden: torch.Tensor, weight: torch.Tensor,
     """``cross_entropy_l2wrap_rows(hidden @ weight.T, targets, num_tokens)`` without
     the logits: ``hidden`` [rows, c] and ``weight`` [vocab, c] are both float32 or both
     bfloat16, and differentiable once, in reverse mode. Logits are not rounded on the
-    way. A row whose target is ``ignore_index`` has loss 0 and no gradient; one whose target is
-    otherwise outside [0, vocab) a NaN loss."""
+    way. A row whose target is ``ignore_index`` has loss 0 and no gradient, whatever its
+    hidden state is; one whose target is otherwise outside [0, vocab) a NaN loss."""
     if not hidden.is_cuda or weight.device != hidden.device or targets.device != hidden.device:
         raise ValueError("hidden, weight and targets must be on the same GPU")
     if hidden.dim() != 2 or weight.dim() != 2 or weight.shape[1] != hidden.shape[1] \

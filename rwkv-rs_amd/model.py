@@ -31,6 +31,12 @@ param_gate, moves from GatedReadout into that first pass). With
 the readable mirror of the reference and as the reference the fused kernels
 are tested against.
 
+Two things of a training step that the reference does not have: dropout of each
+mixer's output where it joins the residual stream (``dropout``; off by default), and
+the loss straight from the last hidden states, without the logits in memory
+(``loss="pieces"``). Both draw or form again in the backward what they would otherwise
+have stored.
+
 Weights are random N(0, 0.02) (normalisation layers start at one and zero);
 the reference's shape-aware initialiser is not needed to time or check a step.
 Matrix products run in bfloat16 under autocast with float32 master weights;
@@ -48,6 +54,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import decode as _decode
+from . import dropout as _dropout
 from . import lm_loss as _loss
 from . import neighbors as _nb
 from . import token_scores as _scores
@@ -484,23 +491,39 @@ class CausalCell(nn.Module):
     added to the residual stream."""
 
     def __init__(self, num_cells, embedded_dim, num_heads, head_size, cell_id: int,
-                 wkv7_dtype: torch.dtype = torch.bfloat16, neighbor_ops: str = "hip"):
+                 wkv7_dtype: torch.dtype = torch.bfloat16, neighbor_ops: str = "hip",
+                 dropout: float = 0.0):
         super().__init__()
+        self.dropout, self.cell_id = dropout, cell_id
+        self.neighbor_ops = _check_neighbor_ops(neighbor_ops)
         self.pre_layer_norm_for_time_mix = nn.LayerNorm(embedded_dim)
         self.pre_layer_norm_for_channel_mix = nn.LayerNorm(embedded_dim)
         self.time_mixer = TimeMixer(num_cells, embedded_dim, num_heads, head_size, cell_id,
                                     wkv7_dtype, neighbor_ops)
         self.channel_mixer = ChannelMixer(num_cells, embedded_dim, cell_id, neighbor_ops)
 
+    def add(self, x, mixed, dropout_rng, mixer: int):
+        """``x + mixed``, in training with dropout of ``mixed``; the two mixers of
+        each cell have sites of their own."""
+        if dropout_rng is None or self.dropout == 0.0 or not self.training:
+            return x + mixed
+        site = 2 * self.cell_id + mixer
+        if self.neighbor_ops == "hip":
+            return _dropout.dropout_add(x, mixed, self.dropout, dropout_rng, site)
+        keep = _dropout.keep_mask(mixed.shape, self.dropout, dropout_rng, site)
+        kept = _dropout.keep_probability(self.dropout)
+        scale = 1.0 / kept if kept else 0.0
+        return x + torch.where(keep, mixed.to(x.dtype) * scale, 0.0)
+
     def forward(self, x, batch_ids, elapsed_t, value_from_first_cell, state, shift_time,
-                shift_channel, context_mask, kernel):
+                shift_channel, context_mask, kernel, dropout_rng=None):
         tm = self.time_mixer(TimeMixerIO(self.pre_layer_norm_for_time_mix(x), batch_ids,
                                          elapsed_t, context_mask, value_from_first_cell,
                                          shift_time, state), kernel)
-        x = x + tm.embedded_context
+        x = self.add(x, tm.embedded_context, dropout_rng, 0)
         cm, next_shift_channel = self.channel_mixer(self.pre_layer_norm_for_channel_mix(x),
                                                     shift_channel, context_mask, batch_ids)
-        x = x + cm
+        x = self.add(x, cm, dropout_rng, 1)
         return x, tm.value_from_first_cell, tm.state, tm.embedded_token_shift, next_shift_channel
 
 
@@ -509,16 +532,19 @@ class MultiCausalCells(nn.Module):
     precursor feeds every later cell's value residual."""
 
     def __init__(self, num_cells, embedded_dim, num_heads, head_size,
-                 wkv7_dtype: torch.dtype = torch.bfloat16, neighbor_ops: str = "hip"):
+                 wkv7_dtype: torch.dtype = torch.bfloat16, neighbor_ops: str = "hip",
+                 dropout: float = 0.0):
         super().__init__()
         self.cells = nn.ModuleList(
-            CausalCell(num_cells, embedded_dim, num_heads, head_size, i, wkv7_dtype, neighbor_ops)
+            CausalCell(num_cells, embedded_dim, num_heads, head_size, i, wkv7_dtype, neighbor_ops,
+                       dropout)
             for i in range(num_cells))
 
     def forward(self, x, batch_ids, kernel, elapsed_t=None, context_mask=None,
                 shift_time: Optional[List[torch.Tensor]] = None,
                 state: Optional[List[torch.Tensor]] = None,
-                shift_channel: Optional[List[torch.Tensor]] = None):
+                shift_channel: Optional[List[torch.Tensor]] = None,
+                dropout_rng: Optional[torch.Tensor] = None):
         x = apply_context_mask(x, context_mask)
         v_first = torch.zeros_like(x)
         shift_time = list(shift_time) if shift_time is not None else None
@@ -530,7 +556,7 @@ class MultiCausalCells(nn.Module):
                 state[i] if state is not None else None,
                 shift_time[i] if shift_time is not None else None,
                 shift_channel[i] if shift_channel is not None else None,
-                context_mask, kernel)
+                context_mask, kernel, dropout_rng)
             if shift_time is not None:
                 shift_time[i] = st
             if state is not None:
@@ -540,24 +566,58 @@ class MultiCausalCells(nn.Module):
         return x, shift_time, state, shift_channel
 
 
+LOSSES = ("logits", "pieces")
+
+
 class AutoRegressiveModel(nn.Module):
     """examples/rwkv-lm/src/model.rs:50-176: embedding, layer norm, the
-    cells, layer norm, unembedding, l2wrap and mean cross entropy."""
+    cells, layer norm, unembedding, l2wrap and mean cross entropy.
+
+    ``dropout``: in training mode each mixer's output is dropped with this
+    probability where it joins the residual stream (``dropout.dropout_add``). The
+    masks follow from ``dropout_rng``, an int64 buffer [seed, step] that is no part of the
+    state dict: each forward that draws takes the step it finds and counts it up.
+
+    ``loss``: "logits" forms them for the loss; "pieces" does not keep them
+    (``lm_loss.linear_cross_entropy_l2wrap``), needs the "hip" neighbour ops, and
+    leaves out targets of ``lm_loss.IGNORE_INDEX``. An unembedding that is no plain
+    linear layer any more (4-bit weights) has its logits formed all the same."""
 
     def __init__(self, vocab_size: int, num_cells: int, embedded_dim: int, num_heads: int,
                  head_size: int = 64, wkv7_dtype: torch.dtype = torch.bfloat16,
-                 neighbor_ops: str = "hip"):
+                 neighbor_ops: str = "hip", dropout: float = 0.0, loss: str = "logits"):
         super().__init__()
         if embedded_dim != num_heads * head_size:
             raise ValueError("embedded_dim must equal num_heads * head_size")
+        if not 0.0 <= dropout <= 1.0:
+            raise ValueError(f"dropout must be 0 to 1, got {dropout}")
+        if loss not in LOSSES:
+            raise ValueError(f"loss must be one of {LOSSES}, got {loss!r}")
+        if loss == "pieces" and neighbor_ops != "hip":
+            raise ValueError('loss "pieces" needs neighbor_ops "hip"')
         self.embed = nn.Embedding(vocab_size, embedded_dim)
         self.layer_norm_for_first_cell = nn.LayerNorm(embedded_dim)
         self.cells = MultiCausalCells(num_cells, embedded_dim, num_heads, head_size, wkv7_dtype,
-                                      neighbor_ops)
+                                      neighbor_ops, dropout)
         self.layer_norm_for_unembed = nn.LayerNorm(embedded_dim)
         self.unembed = _linear(embedded_dim, vocab_size)
         self.vocab_size = vocab_size
         self.neighbor_ops = _check_neighbor_ops(neighbor_ops)
+        self.dropout, self.loss = dropout, loss
+        self.register_buffer("dropout_rng", torch.zeros(2, dtype=torch.int64), persistent=False)
+
+    def seed_dropout(self, seed: int, step: int = 0):
+        """The masks of the forwards to come: those of ``seed`` from ``step`` on."""
+        self.dropout_rng.copy_(torch.tensor([seed, step], dtype=torch.int64))
+        return self
+
+    def _draw(self) -> Optional[torch.Tensor]:
+        """[seed, step] of a forward that drops, or None."""
+        if self.dropout == 0.0 or not self.training:
+            return None
+        rng = self.dropout_rng.clone()      # the forward's own: the backward reads it again
+        self.dropout_rng[1] += 1
+        return rng
 
     def init_random(self, std: float = 0.02, generator: Optional[torch.Generator] = None):
         """Every weight N(0, std); LayerNorm and GroupNorm weights one and biases zero."""
@@ -670,9 +730,15 @@ class AutoRegressiveModel(nn.Module):
         B, T = inputs.shape
         batch_ids = torch.arange(B, device=inputs.device)
         x = self.layer_norm_for_first_cell(self.embed(inputs))
-        x, _, _, _ = self.cells(x, batch_ids, kernel)
-        logits = self.unembed(self.layer_norm_for_unembed(x))
+        x, _, _, _ = self.cells(x, batch_ids, kernel, dropout_rng=self._draw())
         n = B * T
+        x = self.layer_norm_for_unembed(x)
+        if self.loss == "pieces" and type(self.unembed) is nn.Linear:
+            weight = self.unembed.weight
+            dtype = _matmul_dtype(weight)
+            hidden = x.reshape(n, x.shape[-1]).to(dtype)
+            return _loss.linear_cross_entropy_l2wrap(hidden, weight.to(dtype), targets.reshape(n))
+        logits = self.unembed(x)
         if self.neighbor_ops == "hip":
             return _loss.cross_entropy_l2wrap(logits.reshape(n, self.vocab_size), targets.reshape(n))
         logits = l2wrap(logits.reshape(n, self.vocab_size), n)

@@ -60,6 +60,25 @@ def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
+class _on:
+    """The device of a call's tensors, current while it launches."""
+
+    __slots__ = ("index", "guard")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        here = self.index is None or self.index == torch.cuda.current_device()
+        self.guard = None if here else torch.cuda.device(self.index)
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
 def _no_tangent(t: torch.Tensor, what: str) -> None:
     """Refuses a dual tensor, for the ways around ``autograd.Function.apply``,
     which does: its tangent would be dropped, and read as zero."""
