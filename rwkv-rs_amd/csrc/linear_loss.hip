@@ -67,18 +67,60 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   for (int off = 32; off > 0; off >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), off)));
   return v;
 }
-__device__ __forceinline__ uint32_t block_max(uint32_t v) {   // of 256 threads
-  __shared__ uint32_t part[4];
+template <int kWaves>
+__device__ __forceinline__ uint32_t block_max(uint32_t v) {
+  __shared__ uint32_t part[kWaves];
   v = wave_max(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
-  return max(max(part[0], part[1]), max(part[2], part[3]));
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) v = max(v, part[w]);
+  return v;
 }
+
+// The rows that are not ignored, in order, and where each row is among them (-1: not).
+// The products are formed of these alone: fine-tuning leaves out prompts and padding. One
+// workgroup of kWide threads: each wave takes a run of rows, counts them, then numbers them.
+constexpr int kWide = 1024;
+struct RowsCall {
+  const int64_t* targets;
+  int64_t ignore_index;
+  int rows;
+  int *index, *place, *count;   // null: the rows as they are
+};
+__device__ __forceinline__ void number_rows(const RowsCall& c) {
+  __shared__ int counts[kWide / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int each = (c.rows + kWide - 1) / kWide * 64, first = wave * each, last = min(first + each, c.rows);
+  int n = 0;
+#pragma unroll 8
+  for (int r = first + lane; r - lane < last; r += 64)
+    n += __popcll(__ballot(r < last && c.targets[min(r, c.rows - 1)] != c.ignore_index));
+  if (lane == 0) counts[wave] = n;
+  __syncthreads();
+  int at = 0;
+#pragma unroll
+  for (int w = 0; w < kWide / 64; ++w) {
+    if (w == wave) n = at;
+    at += counts[w];
+  }
+  if (threadIdx.x == 0) *c.count = at;
+#pragma unroll 4
+  for (int r = first + lane; r - lane < last; r += 64) {
+    const bool kept = r < last && c.targets[min(r, c.rows - 1)] != c.ignore_index;
+    const uint64_t all = __ballot(kept);
+    const int own = n + __popcll(all & ((uint64_t{1} << lane) - 1));
+    if (kept) c.index[own] = r;
+    if (r < last) c.place[r] = kept ? own : -1;
+    n += __popcll(all);
+  }
+}
+__global__ __launch_bounds__(kWide) void rows_kernel(const RowsCall c) { number_rows(c); }
 
 // The largest magnitudes: of x but for the rows that are ignored (whatever stands there
 // is nobody's measure), of w, and of the rows' factors of D. Row y of the grid takes
-// array y; each workgroup leaves one number.
+// array y; each workgroup leaves one number. A fourth row numbers the rows.
 struct SurveyCall {
   const void* from[2];       // null: not wanted
   int64_t n[2];              // rows
@@ -89,17 +131,22 @@ struct SurveyCall {
   float l2wrap_scale;
   float* residuals;          // [2, rows], cleared; may be null
   uint32_t* largest;         // [3, kMaxBlocks]
+  RowsCall numbered;
 };
 template <bool BF>
-__global__ __launch_bounds__(256) void survey_kernel(const SurveyCall c) {
+__global__ __launch_bounds__(kWide) void survey_kernel(const SurveyCall c) {
   const int which = blockIdx.y;
   uint32_t most = 0;
+  if (which == 3) {
+    if (blockIdx.x == 0) number_rows(c.numbered);
+    return;
+  }
   if (which < 2) {
     if (!c.from[which]) return;
     constexpr int kPer = BF ? 8 : 4;       // elements of 16 bytes
     const int lane = threadIdx.x & 63;
     const int pieces = (reinterpret_cast<uintptr_t>(c.from[which]) & 15) == 0 && c.c % kPer == 0 ? static_cast<int>(c.c / kPer) : 0;
-    for (int64_t row = blockIdx.x * 4 + (threadIdx.x >> 6); row < c.n[which]; row += kMaxBlocks * 4) {
+    for (int64_t row = blockIdx.x * (kWide / 64) + (threadIdx.x >> 6); row < c.n[which]; row += kMaxBlocks * (kWide / 64)) {
       if (which == 0 && c.targets[row] == c.ignore_index) continue;
       const u32x4* const v = reinterpret_cast<const u32x4*>(static_cast<const char*>(c.from[which]) + row * c.c * (BF ? 2 : 4));
 #pragma unroll 4
@@ -123,13 +170,14 @@ __global__ __launch_bounds__(256) void survey_kernel(const SurveyCall c) {
       }
     }
   } else {
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; r < c.rows; r += kMaxBlocks * 256) {
+    if (!c.row_grad) return;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWide + threadIdx.x; r < c.rows; r += kMaxBlocks * kWide) {
       if (c.residuals) c.residuals[r] = c.residuals[c.rows + r] = 0.f;
       if (c.targets[r] == c.ignore_index) continue;
       most = max(most, max(finite_magnitude(c.row_grad[r]), finite_magnitude(c.l2wrap_scale * c.row_max[r])));
     }
   }
-  most = block_max(most);
+  most = block_max<kWide / 64>(most);
   if (threadIdx.x == 0) c.largest[which * kMaxBlocks + blockIdx.x] = most;
 }
 
@@ -147,13 +195,15 @@ struct PackCall {
   bool factors;              // the backward's reference is wanted
   const int64_t* targets;
   int64_t ignore_index;
+  const int *index, *count;  // of x's rows that are taken; null: all
   const uint32_t* largest;
   Scalars* scalars;
 };
 // fp16 arrays are of x s, s the power of two that brings the largest magnitude to 2^13
 // .. 2^14: bf16 numbers of 2^-27 of it and more are held whole, smaller ones to 2^-38 of
 // it; of fp32 ones the second array holds what is left, rounded to 11 bits or likewise.
-// Ignored rows of x become zeros: a NaN there does not reach the weight's gradient.
+// Ignored rows of x are left out or become zeros: a NaN there does not reach the weight's
+// gradient.
 __device__ __forceinline__ int exponent_of(uint32_t largest) {
   return largest ? min(kHalfExponent - ilogbf(__builtin_bit_cast(float, largest)), 120) : 0;
 }
@@ -162,22 +212,25 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
   const bool writes = blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0;
   int exponent = 0;
   if (c.factors && blockIdx.x == 0 && blockIdx.y == 0) {
-    const uint32_t most = block_max(c.largest[2 * kMaxBlocks + threadIdx.x]);
+    const uint32_t most = block_max<4>(c.largest[2 * kMaxBlocks + threadIdx.x]);
     // a gradient that is the same for all rows leaves exactly one, and so its own rounding out of D
     if (writes) c.scalars->reference = most ? __builtin_bit_cast(float, most) : 1.f;
   }
   if (static_cast<int>(blockIdx.y) >= c.jobs) return;
   if (job.kind != kCopy) {
-    exponent = exponent_of(block_max(c.largest[job.which * kMaxBlocks + threadIdx.x]));
+    exponent = exponent_of(block_max<4>(c.largest[job.which * kMaxBlocks + threadIdx.x]));
     if (blockIdx.x == 0 && threadIdx.x == 0) c.scalars->exponent[job.which] = exponent;
   }
   const int lane = threadIdx.x & 63, pieces = c.padded / 8;
   const int64_t plane = job.rows * c.padded;
   const bool whole = c.c % 8 == 0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); row < job.rows; row += gridDim.x * int64_t{4}) {
-    const bool ignored = job.kind != kCopy && job.which == 0 && c.targets[row] == c.ignore_index;
+  const bool some = c.index && job.which == 0;
+  const int64_t rows = some ? *c.count : job.rows;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); row < rows; row += gridDim.x * int64_t{4}) {
+    const int64_t source = some ? c.index[row] : row;
+    const bool ignored = !some && job.kind != kCopy && job.which == 0 && c.targets[row] == c.ignore_index;
     for (int i = lane; i < pieces; i += 64) {
-      const int64_t at = row * c.c + 8 * i;
+      const int64_t at = source * c.c + 8 * i;
       if (ignored) {
         char* const to = job.to + (row * c.padded + 8 * i) * 2;
         *reinterpret_cast<u32x4*>(to) = u32x4{0, 0, 0, 0};
@@ -231,7 +284,7 @@ struct LogitsCall {
   Matrix x, w;
   int rows, vocab, steps;        // steps: c up to a whole step
   int first, words;              // the piece of the vocabulary, whole tiles
-  int tiles;
+  const int *index, *count;      // the rows that x's are, and how many; null: all as they are
   const Scalars* scalars;
   const int64_t* targets;
   int64_t ignore_index;
@@ -258,10 +311,11 @@ template <bool BF, bool kBackward>
 __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c) {
   using T = Tile<kRows, kRows, kWords, kRowsTile, kWavesP, kWavesQ, true, true, BF ? kBf16 : kHalves>;
   __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
-  const int row_tiles = (c.rows + kRowsTile - 1) / kRowsTile, word_tiles = c.words / kWords;
+  const int rows = c.count ? *c.count : c.rows;
+  const int row_tiles = (rows + kRowsTile - 1) / kRowsTile, word_tiles = c.words / kWords, tiles = row_tiles * word_tiles;
   // each XCD has a run of tiles, and its workgroups take them in turn
   const int xcd = blockIdx.x % kXcds, local = blockIdx.x / kXcds, locals = (static_cast<int>(gridDim.x) - xcd + kXcds - 1) / kXcds;
-  const int each = c.tiles / kXcds, rest = c.tiles % kXcds;
+  const int each = tiles / kXcds, rest = tiles % kXcds;
   const int last = (xcd + 1) * each + min(xcd + 1, rest);
   int at = xcd * each + min(xcd, rest) + local;
   T t;
@@ -273,7 +327,7 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
     v0 = c.first + (run * kWordTiles + in_run % run_words) * kWords;
     r0 = in_run / run_words * kRowsTile;
     T::begin(work, lds, Operand{c.w.data + int64_t{v0} * c.w.pitch, c.w.pitch, c.vocab - v0, c.steps},
-             Operand{c.x.data + int64_t{r0} * c.x.pitch, c.x.pitch, c.rows - r0, c.steps}, c.w.plane, c.x.plane, 0, c.steps);
+             Operand{c.x.data + int64_t{r0} * c.x.pitch, c.x.pitch, rows - r0, c.steps}, c.w.plane, c.x.plane, 0, c.steps);
   };
   if (at < last) begin(at);
   for (; at < last; at += locals) {
@@ -338,8 +392,8 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
           sums[wp * kRowsTile + in_tile] = sum;
           firsts[wp * kRowsTile + in_tile] = first;
         }
-        if (row < c.rows) {
-          const int64_t target = c.targets[row];
+        if (row < rows) {
+          const int64_t target = c.targets[c.index ? c.index[row] : row];
           const int own = target >= 0 && target < c.vocab ? static_cast<int>(target) - word0 : -1;
           if (own >= 0 && own < T::kWaveP && (own & 63) < 16) {
 #pragma unroll
@@ -351,7 +405,7 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
         }
       }
       __syncthreads();
-      if (threadIdx.x < kRowsTile && r + static_cast<int>(threadIdx.x) < c.rows) {
+      if (threadIdx.x < kRowsTile && r + static_cast<int>(threadIdx.x) < rows) {
         const int q = threadIdx.x;
         const float a = maxima[q], b = maxima[kRowsTile + q];
         const float most = fmaxf(a, b), sa = sums[q], sb = sums[kRowsTile + q];
@@ -372,9 +426,9 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
       } of[T::kTilesQ];
 #pragma unroll
       for (int j = 0; j < T::kTilesQ; ++j) {      // all rows' numbers are asked for at once
-        const int row = r + wq * T::kWaveQ + 16 * j + m, known = min(row, c.rows - 1);
+        const int row = r + wq * T::kWaveQ + 16 * j + m, some = min(row, rows - 1), known = c.index ? c.index[some] : some;
         const int64_t target = c.targets[known];
-        of[j].dead = row >= c.rows || target == c.ignore_index;
+        of[j].dead = row >= rows || target == c.ignore_index;
         of[j].own = target >= 0 && target < c.vocab ? static_cast<int>(target) - word0 : -1;
         of[j].top = c.row_argmax[known] - word0;
         of[j].lse = c.row_lse[known];
@@ -436,6 +490,7 @@ struct JoinCall {
   const float *part_max, *part_sum, *row_target;
   const int* part_argmax;
   const int64_t* targets;
+  const int* place;          // of each row among the parts' rows; null: as it is
   int64_t rows, vocab, ignore_index;
   float *row_loss, *row_lse, *row_max;
   int32_t* row_argmax;
@@ -457,10 +512,11 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinCall c) {
   const int own = threadIdx.x & 15, share = threadIdx.x >> 4;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + own, tiles = (c.vocab + kWords - 1) / kWords;
   Run run{-INFINITY, 0.f, INT_MAX};
-  if (row < c.rows) {
+  const int64_t part_row = row >= c.rows ? -1 : c.place ? c.place[row] : row;
+  if (part_row >= 0) {
 #pragma unroll 4
     for (int64_t t = share; t < tiles; t += 16) {
-      const int64_t at = t * c.rows + row;
+      const int64_t at = t * c.rows + part_row;
       run = combine(run, Run{c.part_max[at], c.part_sum[at], c.part_argmax[at]});
     }
   }
@@ -478,7 +534,7 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinCall c) {
   c.row_loss[row] = target == c.ignore_index ? 0.f
                     : target < 0 || target >= c.vocab ? NAN
                     : lse != lse ? NAN
-                                 : fmaxf(lse - c.row_target[row], 0.f);
+                                 : fmaxf(lse - c.row_target[part_row], 0.f);
 }
 
 // ---------------------------------------------------------------------- gradients
@@ -515,14 +571,14 @@ struct HiddenCall {
   const __bf16* weight;
 };
 template <bool BF>
-__device__ __forceinline__ void finish_hidden(const HiddenCall& c, const Scalars* scalars, int64_t row, int64_t channel, f32x4 v) {
+__device__ __forceinline__ void finish_hidden(const HiddenCall& c, const Scalars* scalars, int64_t row, int64_t part_row, int64_t channel, f32x4 v) {
   const float reference = scalars->reference;
   const int exponent = -(kHalfExponent + (BF ? 0 : scalars->exponent[1]));
   const bool whole = c.c % 4 == 0;
   if constexpr (BF) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const float r = c.residuals[k * c.rows + row];
+      const float r = c.residuals[k * c.rows + part_row];
       if (r == 0.f) continue;                      // and so where there is no such word
       const __bf16* const w = c.weight + (k ? c.row_argmax[row] : c.targets[row]) * c.c + channel;
       if (whole) {
@@ -547,28 +603,45 @@ struct GradientsCall {
   const char* d;
   int64_t d_plane;
   int first, words, padded_rows, rows, vocab, c;
+  const int* count;          // of x's and D's rows; null: all
   const Scalars* scalars;
   int weight_tiles, weight_blocks;   // workgroups of dw's tiles, up to whole rounds of the XCDs; then dx's
   void* weight_grad;
   int share;                 // words of a workgroup of dx
   bool begin;                // the first piece: no sums to add to
-  float* sums;               // [splits, rows, pitch]; null: one share and one piece, dx itself is stored
+  float* sums;               // [splits, rows, pitch]; null: dx itself is stored
   int pitch;
   HiddenCall hidden;
 };
+
+// The tiles of a gradient in an order in which those that an XCD has at a time share
+// both operands: runs of up to five tiles of channels, in each the other tiles.
+constexpr int kMaxRun = 5;
+__device__ __forceinline__ void place(int at, int channel_tiles, int others, int& channel_tile, int& other) {
+  const int runs = (channel_tiles + kMaxRun - 1) / kMaxRun, run = (channel_tiles + runs - 1) / runs;
+  const int first = at / (run * others) * run, in_run = at % (run * others), width = min(run, channel_tiles - first);
+  channel_tile = first + in_run % width;
+  other = in_run / width;
+}
 
 // A tile of dw, of the piece's words: steps are rows; those past the last have D = 0.
 template <bool BF, int kChannels>
 __device__ __forceinline__ void weight_tile(const GradientsCall& c, char* lds, int at) {
   using T = Tile<kSteps, kSteps, kChannels, kGradTile, kWavesP, kWavesQ, false, false, BF ? kHalf : kHalves>;
-  const int channel_tiles = (c.c + kChannels - 1) / kChannels;
-  const int c0 = at % channel_tiles * kChannels, w0 = at / channel_tiles * kGradTile;
+  int channel_tile, word_tile;
+  place(at, (c.c + kChannels - 1) / kChannels, c.words / kGradTile, channel_tile, word_tile);
+  const int c0 = channel_tile * kChannels, w0 = word_tile * kGradTile;
+  const int rows = c.count ? *c.count : c.rows;
   T t;
-  typename T::Work work;
-  T::begin(work, lds, Operand{c.x.data + c0 * 2, c.x.pitch, c.c - c0, c.rows},
-           Operand{c.d + w0 * 2, int64_t{c.words} * 2, c.words - w0, c.padded_rows}, c.x.plane, c.d_plane, 0,
-           (c.rows + kStep - 1) / kStep * kStep);
-  t.run(work, lds);
+  if (rows == 0) {
+    t.clear();
+  } else {
+    typename T::Work work;
+    T::begin(work, lds, Operand{c.x.data + c0 * 2, c.x.pitch, c.c - c0, rows},
+             Operand{c.d + w0 * 2, int64_t{c.words} * 2, c.words - w0, c.padded_rows}, c.x.plane, c.d_plane, 0,
+             (rows + kStep - 1) / kStep * kStep);
+    t.run(work, lds);
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
   const float reference = c.scalars->reference;
@@ -590,13 +663,19 @@ __device__ __forceinline__ void weight_tile(const GradientsCall& c, char* lds, i
   }
 }
 
-// A tile of dx, over a share of the piece's words; the words past the vocabulary have D = 0.
+// A tile of dx, over a share of the piece's words; the words past the vocabulary have D =
+// 0. There are as many workgroups as all rows would need.
 template <bool BF, int kChannels>
-__device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, int at) {
+__device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, int block) {
   using T = Tile<kSteps, kRows, kChannels, kGradTile, kWavesP, kWavesQ, false, true, BF ? kHalfQ : kHalves>;
-  const int channel_tiles = (c.c + kChannels - 1) / kChannels, row_tiles = c.padded_rows / kGradTile;
-  const int c0 = at % channel_tiles * kChannels, r0 = at / channel_tiles % row_tiles * kGradTile;
-  const int split = at / channel_tiles / row_tiles;
+  const int rows = c.count ? *c.count : c.rows;
+  const int channel_tiles = (c.c + kChannels - 1) / kChannels, row_tiles = (rows + kGradTile - 1) / kGradTile;
+  const int each = channel_tiles * row_tiles, all = each * ((c.words + c.share - 1) / c.share);
+  if (block >= all) return;
+  const int at = tile_of_block(block, all), split = at / each;
+  int channel_tile, row_tile;
+  place(at % each, channel_tiles, row_tiles, channel_tile, row_tile);
+  const int c0 = channel_tile * kChannels, r0 = row_tile * kGradTile;
   const int k0 = split * c.share, k1 = min(k0 + c.share, c.words);
   T t;
   typename T::Work work;
@@ -608,13 +687,13 @@ __device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, i
 #pragma unroll
   for (int j = 0; j < T::kTilesQ; ++j) {
     const int row = r0 + wq * T::kWaveQ + 16 * j + m;
-    if (row >= c.rows) continue;
+    if (row >= rows) continue;
 #pragma unroll
     for (int i = 0; i < T::kTilesP; ++i) {
       const int channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
       if (channel >= c.pitch) continue;
       if (!c.sums) {
-        finish_hidden<BF>(c.hidden, c.scalars, row, channel, t.acc[i][j]);
+        finish_hidden<BF>(c.hidden, c.scalars, row, row, channel, t.acc[i][j]);
         continue;
       }
       f32x4* const to = reinterpret_cast<f32x4*>(c.sums + (int64_t{split} * c.rows + row) * c.pitch + channel);
@@ -630,12 +709,12 @@ __global__ __launch_bounds__(kThreads, 2) void gradients_kernel(const GradientsC
   using T = Tile<kSteps, kRows, kChannels, kGradTile, kWavesP, kWavesQ, false, true, kHalves>;
   using U = Tile<kSteps, kSteps, kChannels, kGradTile, kWavesP, kWavesQ, false, false, kHalves>;
   __shared__ __attribute__((aligned(16))) char lds[std::max(T::kLdsBytes, U::kLdsBytes)];
-  const int block = blockIdx.x, blocks = gridDim.x;
+  const int block = blockIdx.x;
   if (block < c.weight_blocks) {
     const int at = tile_of_block(block, c.weight_blocks);
     if (at < c.weight_tiles) weight_tile<BF, kChannels>(c, lds, at);
   } else {
-    hidden_tile<BF, kChannels>(c, lds, tile_of_block(block - c.weight_blocks, blocks - c.weight_blocks));
+    hidden_tile<BF, kChannels>(c, lds, block - c.weight_blocks);
   }
 }
 
@@ -644,6 +723,7 @@ struct HiddenSumCall {
   const float* sums;
   int64_t rows, pitch;
   int splits;
+  const int* place;          // of each row among the sums' rows; null: as it is
   const Scalars* scalars;
   HiddenCall hidden;
 };
@@ -651,10 +731,15 @@ template <bool BF>
 __global__ __launch_bounds__(256) void hidden_sum_kernel(const HiddenSumCall c) {
   const int64_t fours = c.pitch / 4, n = c.rows * fours;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / fours, four = i % fours, part_row = c.place ? c.place[row] : row;
     f32x4 v{0.f, 0.f, 0.f, 0.f};
+    if (part_row < 0) {
+      store4<BF>(c.hidden.grad, row * c.hidden.c + 4 * four, v, c.hidden.c - 4 * four, c.hidden.c % 4 == 0);
+      continue;
+    }
 #pragma unroll 4
-    for (int s = 0; s < c.splits; ++s) v += reinterpret_cast<const f32x4*>(c.sums)[s * n + i];
-    finish_hidden<BF>(c.hidden, c.scalars, i / fours, i % fours * 4, v);
+    for (int s = 0; s < c.splits; ++s) v += reinterpret_cast<const f32x4*>(c.sums)[s * n + part_row * fours + four];
+    finish_hidden<BF>(c.hidden, c.scalars, row, part_row, 4 * four, v);
   }
 }
 
@@ -664,7 +749,11 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t* to, int64_t words,
 }
 
 // ------------------------------------------------------------------ plan, workspace
-// The bf16 operands whose rows are whole steps are read where they are.
+// The rows that are not ignored are numbered, and x's brought together, where that is a
+// small part of the work.
+constexpr int64_t kManyRows = 1024;
+bool numbered(int64_t rows) { return rows >= kManyRows; }
+// bf16 operands whose rows are whole steps are read where they are.
 bool packed(int64_t c, bool bf16) { return !bf16 || c % kStep != 0; }
 
 int64_t take(int64_t& end, int64_t bytes) {
@@ -674,7 +763,7 @@ int64_t take(int64_t& end, int64_t bytes) {
 }
 // Byte offsets of the operands in the workspace.
 struct Places {
-  int64_t scalars, largest, x, w, x_half, x_plane, w_plane;
+  int64_t scalars, largest, index, place, count, x, w, x_half, x_plane, w_plane;
   int64_t end;
 };
 Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward) {
@@ -684,10 +773,13 @@ Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward
   p.largest = take(p.end, 3 * kMaxBlocks * 4);
   p.x_plane = rows * pitch;
   p.w_plane = vocab * pitch;
-  if (packed(c, bf16)) {
-    p.x = take(p.end, planes * p.x_plane);
-    p.w = take(p.end, planes * p.w_plane);
+  if (numbered(rows)) {
+    p.index = take(p.end, rows * 4);
+    p.place = take(p.end, rows * 4);
+    p.count = take(p.end, 4);
   }
+  if (packed(c, bf16) || numbered(rows)) p.x = take(p.end, planes * p.x_plane);
+  if (packed(c, bf16)) p.w = take(p.end, planes * p.w_plane);
   if (bf16 && backward) p.x_half = take(p.end, p.x_plane);
   return p;
 }
@@ -735,6 +827,8 @@ Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   return p;
 }
 
+// dx goes by way of sums, unless one workgroup has the whole of a row's and no row is left out.
+bool needs_sums(const Plan& p, int64_t rows) { return p.splits > 1 || p.pieces > 1 || numbered(rows); }
 struct BackwardPlaces {
   Places operands;
   int64_t d, d_plane, sums, residuals, end;
@@ -745,7 +839,7 @@ BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64
   b.end = b.operands.end;
   b.d_plane = p.padded_rows * p.words * 2;
   b.d = take(b.end, b.d_plane * (bf16 ? 1 : 2));
-  b.sums = p.splits == 1 && p.pieces == 1 ? 0 : take(b.end, p.splits * rows * p.pitch * 4);
+  b.sums = !needs_sums(p, rows) ? 0 : take(b.end, p.splits * rows * p.pitch * 4);
   b.residuals = take(b.end, 2 * rows * 4);
   return b;
 }
@@ -767,31 +861,38 @@ ForwardPlaces forward_places(int64_t rows, int64_t vocab, int64_t c, bool bf16) 
 }
 
 // x and w as the tiles read them (and x in fp16 for bf16 operands' weight gradient), made
-// first where they are not so in memory; the backward's factors.
+// first where they are not so in memory; the rows' numbers; the backward's factors.
 struct Operands {
   Matrix x, w, x_half;
+  const int *index, *place, *count;
 };
 template <bool BF>
 Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* residuals, hipStream_t s) {
   const int64_t padded = up(c.c, kStep);
-  Operands o;
+  Operands o{};
   o.x = Matrix{static_cast<const char*>(c.hidden), c.c * 2, 0};
   o.w = Matrix{static_cast<const char*>(c.weight), c.c * 2, 0};
+  RowsCall r{c.targets, c.ignore_index, static_cast<int>(c.rows), nullptr, nullptr, nullptr};
+  if (numbered(c.rows)) {
+    o.index = r.index = reinterpret_cast<int*>(c.workspace + p.index);
+    o.place = r.place = reinterpret_cast<int*>(c.workspace + p.place);
+    o.count = r.count = reinterpret_cast<int*>(c.workspace + p.count);
+  }
   PackCall k{};
   auto pack = [&](const void* from, int64_t to, int64_t rows, int kind, int which, int64_t plane) {
     k.job[k.jobs++] = PackJob{from, c.workspace + to, rows, kind, which};
     return Matrix{c.workspace + to, padded * 2, plane};
   };
-  if (packed(c.c, BF)) {
-    o.x = pack(c.hidden, p.x, c.rows, BF ? kCopy : kToHalves, 0, p.x_plane);
-    o.w = pack(c.weight, p.w, c.vocab, BF ? kCopy : kToHalves, 1, p.w_plane);
-  }
+  if (packed(c.c, BF) || r.index) o.x = pack(c.hidden, p.x, c.rows, BF ? kCopy : kToHalves, 0, p.x_plane);
+  if (packed(c.c, BF)) o.w = pack(c.weight, p.w, c.vocab, BF ? kCopy : kToHalves, 1, p.w_plane);
   o.x_half = o.x;
   if (BF && b && b->weight_grad) o.x_half = pack(c.hidden, p.x_half, c.rows, kToHalf, 0, 0);
   if (k.jobs == 0 && !b) return o;
   k.c = static_cast<int>(c.c);
   k.padded = static_cast<int>(padded);
   k.factors = b != nullptr;
+  k.index = o.index;
+  k.count = o.count;
   uint32_t* const largest = reinterpret_cast<uint32_t*>(c.workspace + p.largest);
   k.largest = largest;
   k.scalars = reinterpret_cast<Scalars*>(c.workspace + p.scalars);
@@ -802,6 +903,7 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
   v.n[1] = c.vocab;
   v.c = c.c;
   v.largest = largest;
+  v.numbered = r;
   k.targets = v.targets = c.targets;
   k.ignore_index = v.ignore_index = c.ignore_index;
   if (b) {
@@ -811,7 +913,8 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
     v.l2wrap_scale = b->l2wrap_scale;
     v.residuals = residuals;
   }
-  if (v.from[0] || b) hipLaunchKernelGGL(survey_kernel<BF>, dim3(kMaxBlocks, b ? 3 : 2), dim3(256), 0, s, v);
+  if (v.from[0] || b) hipLaunchKernelGGL(survey_kernel<BF>, dim3(kMaxBlocks, r.index ? 4 : b ? 3 : 2), dim3(kWide), 0, s, v);
+  else if (r.index) hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(kWide), 0, s, r);
   int64_t rows = 1;
   for (int i = 0; i < k.jobs; ++i) rows = std::max(rows, k.job[i].rows);
   hipLaunchKernelGGL(pack_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(rows, 4), 2048)), std::max(k.jobs, 1)),
@@ -824,8 +927,8 @@ dim3 grid_of(int64_t n) { return dim3(static_cast<unsigned>(std::min<int64_t>(ce
 
 template <bool BF, bool kBackward>
 void logits(LogitsCall& l, hipStream_t s) {
-  l.tiles = static_cast<int>(l.words / kWords * ceil_div(l.rows, kRowsTile));
-  hipLaunchKernelGGL((logits_kernel<BF, kBackward>), dim3(static_cast<unsigned>(std::min(l.tiles, kUnits))), dim3(kThreads), 0, s, l);
+  const int64_t tiles = l.words / kWords * ceil_div(l.rows, kRowsTile);
+  hipLaunchKernelGGL((logits_kernel<BF, kBackward>), dim3(static_cast<unsigned>(std::min<int64_t>(tiles, kUnits))), dim3(kThreads), 0, s, l);
 }
 
 template <bool BF>
@@ -835,6 +938,8 @@ void forward(const ForwardCall& c, hipStream_t s) {
   LogitsCall l{};
   l.x = o.x;
   l.w = o.w;
+  l.index = o.index;
+  l.count = o.count;
   l.rows = static_cast<int>(c.rows);
   l.vocab = static_cast<int>(c.vocab);
   l.steps = static_cast<int>(up(c.c, kStep));
@@ -846,7 +951,7 @@ void forward(const ForwardCall& c, hipStream_t s) {
   l.part_argmax = reinterpret_cast<int*>(c.workspace + f.part_argmax);
   l.row_target = reinterpret_cast<float*>(c.workspace + f.row_target);
   logits<BF, false>(l, s);
-  const JoinCall j{l.part_max, l.part_sum, l.row_target, l.part_argmax, c.targets, c.rows, c.vocab, c.ignore_index,
+  const JoinCall j{l.part_max, l.part_sum, l.row_target, l.part_argmax, c.targets, o.place, c.rows, c.vocab, c.ignore_index,
                    c.row_loss, c.row_lse, c.row_max, c.row_argmax};
   hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>(ceil_div(c.rows, 16))), dim3(256), 0, s, j);
 }
@@ -861,6 +966,8 @@ void backward(const BackwardCall& c, hipStream_t s) {
   LogitsCall l{};
   l.x = o.x;
   l.w = o.w;
+  l.index = o.index;
+  l.count = o.count;
   l.rows = static_cast<int>(c.rows);
   l.vocab = static_cast<int>(c.vocab);
   l.steps = static_cast<int>(up(c.c, kStep));
@@ -878,6 +985,7 @@ void backward(const BackwardCall& c, hipStream_t s) {
   GradientsCall g{};
   g.x = o.x_half;
   g.w = o.w;
+  g.count = o.count;
   g.d = l.d;
   g.d_plane = l.d_plane;
   g.padded_rows = static_cast<int>(p.padded_rows);
@@ -887,7 +995,7 @@ void backward(const BackwardCall& c, hipStream_t s) {
   g.scalars = scalars;
   g.weight_grad = c.weight_grad;
   g.share = static_cast<int>(p.share);
-  const bool direct = p.splits == 1 && p.pieces == 1;
+  const bool direct = !needs_sums(p, c.rows);
   g.sums = direct ? nullptr : reinterpret_cast<float*>(c.workspace + b.sums);
   g.hidden = HiddenCall{c.hidden_grad, c.c, c.rows, residuals, c.targets, c.row_argmax,
                         BF ? static_cast<const __bf16*>(c.weight) : nullptr};
@@ -906,7 +1014,7 @@ void backward(const BackwardCall& c, hipStream_t s) {
     else hipLaunchKernelGGL((gradients_kernel<BF, 256>), grid, dim3(kThreads), 0, s, g);
   }
   if (c.hidden_grad && !direct) {
-    const HiddenSumCall h{g.sums, c.rows, p.pitch, static_cast<int>(p.splits), scalars, g.hidden};
+    const HiddenSumCall h{g.sums, c.rows, p.pitch, static_cast<int>(p.splits), o.place, scalars, g.hidden};
     hipLaunchKernelGGL(hidden_sum_kernel<BF>, grid_of(c.rows * p.pitch / 4), dim3(256), 0, s, h);
   }
 }

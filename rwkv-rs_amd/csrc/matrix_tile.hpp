@@ -348,12 +348,15 @@ struct Tile {
     all_q();
     kDeepP ? all_p() : all_q();
   }
-  // The workgroup may use `lds` again once all of its waves have come back.
-  __device__ __forceinline__ void run(Work& w, char* lds) {
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < kTilesP; ++i)
 #pragma unroll
       for (int j = 0; j < kTilesQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // The workgroup may use `lds` again once all of its waves have come back.
+  __device__ __forceinline__ void run(Work& w, char* lds) {
+    clear();
     const int stages = (w.k1 - w.k0) / kStep * kParts;
     int slot_p = 0, slot_q = 0;
     Held held;

@@ -197,6 +197,25 @@ def test_ignored_and_invalid_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("rows,c", [(1023, 64), (1024, 64), (1025, 100), (4000, 192)])
+def test_many_rows_of_which_some_are_ignored(rows, c, dtype):
+    """From 1024 rows on, those that are learned are brought together first."""
+    announce("linear loss, many rows, some ignored", rows, c, dtype)
+    vocab = 700
+    x, w, t = make(rows, vocab, c, dtype, seed=12)
+    full = t.clone()
+    g = torch.rand(rows, device=DEV) + 0.1
+    r = torch.arange(rows, device=DEV)
+    for dead in (r % 3 != 1, r < rows - 1, r > 0, r < 0, (r // 70) % 2 == 0, r % 64 == 63, r >= 512, r >= 0):
+        t = full.masked_fill(dead, -100)
+        t[2] = -7 if rows == 1025 and not dead[2] else t[2]
+        y = torch.where(dead[:, None], torch.full_like(x, math.nan), x)
+        loss, dx, dw = check(y, w, t, g, rows)
+        assert not dx[dead].any()
+    assert not dw.any()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
 def test_nan_and_infinite_numbers(dtype):
     """A row's own NaN or infinity costs that row's loss and hidden gradient, and every
     word's weight gradient. A word's costs the rows whose logit is NaN or plus infinity;
