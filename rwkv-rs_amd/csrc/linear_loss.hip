@@ -605,7 +605,9 @@ struct GradientsCall {
   int first, words, padded_rows, rows, vocab, c;
   const int* count;          // of x's and D's rows; null: all
   const Scalars* scalars;
-  int weight_tiles, weight_blocks;   // workgroups of dw's tiles, up to whole rounds of the XCDs; then dx's
+  int weight_tiles, weight_blocks;   // dw's workgroups: its tiles, up to whole rounds of the XCDs
+  int hidden_blocks;                 // dx's, likewise
+  bool hidden_first;
   void* weight_grad;
   int share;                 // words of a workgroup of dx
   bool begin;                // the first piece: no sums to add to
@@ -702,19 +704,19 @@ __device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, i
   }
 }
 
-// Both gradients of a piece side by side: dw's tiles, then the shorter ones of dx, which
-// fill the compute units that have none of the last of dw's.
+// Both gradients of a piece side by side: first the longer tiles, then the shorter ones,
+// which fill the compute units that have none of the last of those.
 template <bool BF, int kChannels>
 __global__ __launch_bounds__(kThreads, 2) void gradients_kernel(const GradientsCall c) {
   using T = Tile<kSteps, kRows, kChannels, kGradTile, kWavesP, kWavesQ, false, true, kHalves>;
   using U = Tile<kSteps, kSteps, kChannels, kGradTile, kWavesP, kWavesQ, false, false, kHalves>;
   __shared__ __attribute__((aligned(16))) char lds[std::max(T::kLdsBytes, U::kLdsBytes)];
-  const int block = blockIdx.x;
-  if (block < c.weight_blocks) {
-    const int at = tile_of_block(block, c.weight_blocks);
+  const int weight = static_cast<int>(blockIdx.x) - (c.hidden_first ? c.hidden_blocks : 0);
+  if (weight >= 0 && weight < c.weight_blocks) {
+    const int at = tile_of_block(weight, c.weight_blocks);
     if (at < c.weight_tiles) weight_tile<BF, kChannels>(c, lds, at);
   } else {
-    hidden_tile<BF, kChannels>(c, lds, block - c.weight_blocks);
+    hidden_tile<BF, kChannels>(c, lds, c.hidden_first ? static_cast<int>(blockIdx.x) : weight - c.weight_blocks);
   }
 }
 
@@ -786,17 +788,19 @@ Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward
 
 // D of a piece takes at most kMaxD bytes, of which the least is a tile of words. dx's
 // shares: those with which the two gradients' tiles, handed to the compute units in turn,
-// are done first, in stages; a tile's first loads and its stores count as kOverhead
-// stages, and the sums' way to memory and back as kBytesPerStage has it.
-constexpr int64_t kMaxD = int64_t{512} << 20, kOverhead = 4, kMaxSplits = 16, kBytesPerStage = int64_t{4} << 20;
+// the longer ones first, are done first, in stages; a tile's first loads and its stores
+// count as kOverhead stages, and the sums' way to memory and back as kBytesPerStage has it.
+constexpr int64_t kMaxD = int64_t{512} << 20, kOverhead = 4, kMaxSplits = 64, kBytesPerStage = int64_t{4} << 20;
 struct Plan {
   int channels;                     // of a gradient's tile
   int64_t words, pieces;            // of a piece
   int64_t padded_rows, splits, share, pitch;
+  bool hidden_first;
 };
+// when `more` tiles of `more_each` are done behind `tiles` longer ones of `each`
 int64_t finish(int64_t tiles, int64_t each, int64_t more, int64_t more_each) {
-  const int64_t whole = tiles / kUnits * each, late = tiles % kUnits;
-  for (int64_t at = whole + (late ? each : 0), k = (at - whole) / more_each;; ++k) {
+  const int64_t whole = tiles / kUnits * each, late = tiles % kUnits, at = whole + (late ? each : 0);
+  for (int64_t k = (at - whole) / more_each;; ++k) {
     const int64_t t = std::max(at, whole + k * more_each);
     if ((kUnits - late) * ((t - whole) / more_each) + late * ((t - at) / more_each) >= more) return t;
   }
@@ -813,16 +817,20 @@ Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   p.words = up(ceil_div(all, p.pieces), kWords);
   p.pieces = ceil_div(all, p.words);
   const int64_t weight_tiles = channel_tiles * ceil_div(p.words, kGradTile), hidden_tiles = channel_tiles * p.padded_rows / kGradTile;
+  const int64_t parts = bf16 ? 1 : 3, weight_time = ceil_div(rows, kStep) * parts + kOverhead;
   int64_t least = INT64_MAX;
   for (int64_t s = 1; s <= kMaxSplits; ++s) {
     const int64_t share = up(ceil_div(p.words, s), kStep), splits = ceil_div(p.words, share);
     if (splits < s) continue;
-    const int64_t time = finish(weight_tiles, ceil_div(rows, kStep) + kOverhead, hidden_tiles * splits, share / kStep + kOverhead) +
-                         splits * rows * p.pitch * 8 / kBytesPerStage;
+    const int64_t hidden_time = share / kStep * parts + kOverhead, moved = splits * rows * p.pitch * 8 / kBytesPerStage;
+    if (moved >= least) break;
+    const int64_t time = moved + (hidden_time > weight_time ? finish(hidden_tiles * splits, hidden_time, weight_tiles, weight_time)
+                                                            : finish(weight_tiles, weight_time, hidden_tiles * splits, hidden_time));
     if (time >= least) continue;
     least = time;
     p.splits = splits;
     p.share = share;
+    p.hidden_first = hidden_time > weight_time;
   }
   return p;
 }
@@ -1008,8 +1016,9 @@ void backward(const BackwardCall& c, hipStream_t s) {
     g.begin = first == 0;
     g.weight_tiles = c.weight_grad ? static_cast<int>(channel_tiles * (l.words / kGradTile)) : 0;
     g.weight_blocks = static_cast<int>(up(g.weight_tiles, kXcds));
-    const int64_t hidden_blocks = c.hidden_grad ? channel_tiles * (p.padded_rows / kGradTile) * ceil_div(l.words, p.share) : 0;
-    const dim3 grid(static_cast<unsigned>(g.weight_blocks + hidden_blocks));
+    g.hidden_blocks = c.hidden_grad ? static_cast<int>(up(channel_tiles * (p.padded_rows / kGradTile) * ceil_div(l.words, p.share), kXcds)) : 0;
+    g.hidden_first = p.hidden_first;
+    const dim3 grid(static_cast<unsigned>(g.weight_blocks + g.hidden_blocks));
     if (p.channels == 128) hipLaunchKernelGGL((gradients_kernel<BF, 128>), grid, dim3(kThreads), 0, s, g);
     else hipLaunchKernelGGL((gradients_kernel<BF, 256>), grid, dim3(kThreads), 0, s, g);
   }
