@@ -789,8 +789,9 @@ Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward
 // D of a piece takes at most kMaxD bytes, of which the least is a tile of words. dx's
 // shares: those with which the two gradients' tiles, handed to the compute units in turn,
 // the longer ones first, are done first, in stages; a tile's first loads and its stores
-// count as kOverhead stages, and the sums' way to memory and back as kBytesPerStage has it.
-constexpr int64_t kMaxD = int64_t{512} << 20, kOverhead = 4, kMaxSplits = 64, kBytesPerStage = int64_t{4} << 20;
+// count as kOverhead stages, the launch that adds shares up as kLaunch, and the sums' way
+// to memory and back as kBytesPerStage has it.
+constexpr int64_t kMaxD = int64_t{512} << 20, kOverhead = 4, kLaunch = 4, kMaxSplits = 64, kBytesPerStage = int64_t{4} << 20;
 struct Plan {
   int channels;                     // of a gradient's tile
   int64_t words, pieces;            // of a piece
@@ -822,7 +823,8 @@ Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   for (int64_t s = 1; s <= kMaxSplits; ++s) {
     const int64_t share = up(ceil_div(p.words, s), kStep), splits = ceil_div(p.words, share);
     if (splits < s) continue;
-    const int64_t hidden_time = share / kStep * parts + kOverhead, moved = splits * rows * p.pitch * 8 / kBytesPerStage;
+    const int64_t hidden_time = share / kStep * parts + kOverhead;
+    const int64_t moved = (splits > 1 ? kLaunch : 0) + splits * rows * p.pitch * 8 / kBytesPerStage;
     if (moved >= least) break;
     const int64_t time = moved + (hidden_time > weight_time ? finish(hidden_tiles * splits, hidden_time, weight_tiles, weight_time)
                                                             : finish(weight_tiles, weight_time, hidden_tiles * splits, hidden_time));

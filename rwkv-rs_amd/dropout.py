@@ -29,12 +29,14 @@ def _check(x: torch.Tensor, p: float, rng: torch.Tensor, site: int) -> None:
         raise ValueError(f"site must be 0 to 2^32 - 1, got {site}")
 
 
-def _run(x, residual, rng, site, p, out_dtype):
-    out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    with _on(x.device):
+def _run(x, residual, rng, site, p, code, out_dtype, out_code):
+    """Of contiguous operands. The codes are the dtypes'."""
+    dev = x.device
+    out = torch.empty_like(x, dtype=out_dtype)
+    with _on(dev):
         _native.check(_native.lib().rwkv_dropout(
-            x.data_ptr(), _ptr(residual), rng.data_ptr(), site, p, x.numel(), _code(x.dtype),
-            _code(out_dtype), out.data_ptr(), _stream(x.device)))
+            x.data_ptr(), _ptr(residual), rng.data_ptr(), site, p, x.numel(), code, out_code,
+            out.data_ptr(), _stream(dev)))
     return out
 
 
@@ -42,34 +44,33 @@ class _Dropout(torch.autograd.Function):
     """x to ``out_dtype``. Its backward is itself, the other way round."""
 
     @staticmethod
-    def forward(ctx, x, rng, site, p, out_dtype):
+    def forward(ctx, x, rng, site, p, code, out_dtype, out_code):
         ctx.save_for_backward(rng)
-        ctx.args = site, p, x.dtype
-        return _run(x.contiguous(), None, rng, site, p, out_dtype)
+        ctx.args = site, p, out_code, x.dtype, code
+        return _run(x, None, rng, site, p, code, out_dtype, out_code)
 
     @staticmethod
     def backward(ctx, grad):
-        return _backward(ctx, grad), None, None, None, None
+        return _backward(ctx, grad), None, None, None, None, None, None
 
 
 def _backward(ctx, grad):
     rng, = ctx.saved_tensors
     if torch.is_grad_enabled():        # a gradient of the gradient is wanted
-        return _Dropout.apply(grad, rng, *ctx.args)
-    site, p, dtype = ctx.args
-    return _run(grad.contiguous(), None, rng, site, p, dtype)
+        return _Dropout.apply(grad.contiguous(), rng, *ctx.args)
+    return _run(grad if grad.is_contiguous() else grad.contiguous(), None, rng, *ctx.args)
 
 
 class _DropoutAdd(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, residual, x, rng, site, p):
+    def forward(ctx, residual, x, rng, site, p, code, out_code):
         ctx.save_for_backward(rng)
-        ctx.args = site, p, x.dtype
-        return _run(x, residual, rng, site, p, residual.dtype)
+        ctx.args = site, p, out_code, x.dtype, code
+        return _run(x, residual, rng, site, p, code, residual.dtype, out_code)
 
     @staticmethod
     def backward(ctx, grad):
-        return grad, _backward(ctx, grad) if ctx.needs_input_grad[1] else None, None, None, None
+        return grad, _backward(ctx, grad) if ctx.needs_input_grad[1] else None, None, None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, site: int = 0) -> torch.Tensor:
@@ -78,9 +79,9 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, site: int = 0) -> torc
     in ``x``. A dropped element is 0 even where x is NaN or infinite."""
     if not x.is_cuda:
         raise ValueError("x must be a GPU tensor")
-    _code(x.dtype)
+    code = _code(x.dtype)
     _check(x, p, rng, site)
-    return _Dropout.apply(x, rng.contiguous(), int(site), float(p), x.dtype)
+    return _Dropout.apply(x.contiguous(), rng.contiguous(), int(site), float(p), code, x.dtype, code)
 
 
 def dropout_add(residual: torch.Tensor, x: torch.Tensor, p: float, rng: torch.Tensor,
@@ -92,9 +93,10 @@ def dropout_add(residual: torch.Tensor, x: torch.Tensor, p: float, rng: torch.Te
         raise ValueError("residual and x must be on the same GPU")
     if residual.shape != x.shape:
         raise ValueError(f"residual and x must have one shape, got {tuple(residual.shape)} and {tuple(x.shape)}")
-    _code(x.dtype), _code(residual.dtype)
+    code, out_code = _code(x.dtype), _code(residual.dtype)
     _check(x, p, rng, site)
-    return _DropoutAdd.apply(residual.contiguous(), x.contiguous(), rng.contiguous(), int(site), float(p))
+    return _DropoutAdd.apply(residual.contiguous(), x.contiguous(), rng.contiguous(), int(site), float(p),
+                             code, out_code)
 
 
 def keep_probability(p: float) -> float:

@@ -73,24 +73,24 @@ def cross_entropy_l2wrap(logits: torch.Tensor, targets: torch.Tensor) -> torch.T
 
 
 # ------------------------------------------- from hidden states and unembedding
-def _workspace(which: str, rows: int, vocab: int, c: int, code: int, device) -> tuple:
-    nbytes = getattr(_native.lib(), f"rwkv_linear_loss_{which}_workspace_bytes")(rows, vocab, c, code)
+def _workspace(nbytes: int, device) -> torch.Tensor:
     if nbytes < 0:
-        raise ValueError(f"hidden [{rows}, {c}] and weight [{vocab}, {c}] are not supported")
-    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+        raise ValueError("hidden states or an unembedding of this size are not supported")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def _linear_forward(hidden, weight, targets, ignore_index):
     """Every row's loss, and what the backward needs of it: a [3, rows] tensor of its
     log-sum-exp, its maximum and (as int32) its argmax."""
     (rows, c), vocab, dev = hidden.shape, weight.shape[0], hidden.device
-    code = _code(hidden.dtype)
+    code, lib = _code(hidden.dtype), _native.lib()
+    nbytes = lib.rwkv_linear_loss_forward_workspace_bytes(rows, vocab, c, code)
+    ws = _workspace(nbytes, dev)
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
     kept = torch.empty(3, rows, dtype=torch.float32, device=dev)
     at = kept.data_ptr()
-    ws, nbytes = _workspace("forward", rows, vocab, c, code, dev)
     with _on(dev):
-        _native.check(_native.lib().rwkv_linear_loss_forward(
+        _native.check(lib.rwkv_linear_loss_forward(
             hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), rows, vocab, c, code, ignore_index,
             loss.data_ptr(), at, at + 4 * rows, at + 8 * rows, ws.data_ptr(), nbytes, _stream(dev)))
     return loss, kept
@@ -110,13 +110,15 @@ class _LinearCrossEntropyL2Wrap(torch.autograd.Function):
     def backward(ctx, dloss):
         hidden, weight, targets, kept = ctx.saved_tensors
         (rows, c), vocab, dev = hidden.shape, weight.shape[0], hidden.device
-        code, at = _code(hidden.dtype), kept.data_ptr()
-        g = dloss.to(torch.float32).contiguous()
-        dhidden, dweight = (torch.empty_like(t) if need else None
-                            for t, need in zip((hidden, weight), ctx.needs_input_grad))
-        ws, nbytes = _workspace("backward", rows, vocab, c, code, dev)
+        code, at, lib = _code(hidden.dtype), kept.data_ptr(), _native.lib()
+        g = dloss if dloss.is_contiguous() else dloss.contiguous()
+        need = ctx.needs_input_grad
+        dhidden = torch.empty_like(hidden) if need[0] else None
+        dweight = torch.empty_like(weight) if need[1] else None
+        nbytes = lib.rwkv_linear_loss_backward_workspace_bytes(rows, vocab, c, code)
+        ws = _workspace(nbytes, dev)
         with _on(dev):
-            _native.check(_native.lib().rwkv_linear_loss_backward(
+            _native.check(lib.rwkv_linear_loss_backward(
                 hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), at, at + 4 * rows, at + 8 * rows,
                 g.data_ptr(), ctx.scale, rows, vocab, c, code, ctx.ignore_index, _ptr(dhidden), _ptr(dweight),
                 ws.data_ptr(), nbytes, _stream(dev)))
