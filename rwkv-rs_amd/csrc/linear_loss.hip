@@ -27,8 +27,19 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWords = 256, kRowsTile = 256;   // a tile of logits
-constexpr int kWavesP = 2, kWavesQ = 4, kThreads = 512;
+// A tile of logits: words by rows, on waves by waves. Two smaller ones, of which a
+// compute unit has two and four at a time, for few rows or words.
+struct Big {
+  static constexpr int kWords = 256, kRows = 256, kWavesP = 2, kWavesQ = 4, kEach = 1;
+};
+struct Middle {
+  static constexpr int kWords = 128, kRows = 128, kWavesP = 2, kWavesQ = 2, kEach = 2;
+};
+struct Small {
+  static constexpr int kWords = 64, kRows = 64, kWavesP = 2, kWavesQ = 2, kEach = 4;
+};
+constexpr int kWholeWords = 256;               // a piece of the vocabulary is whole tiles of any size
+constexpr int kWavesP = 2, kWavesQ = 4, kThreads = 512;   // of a gradient's tile
 constexpr int kUnits = 256;                    // compute units; a tile's LDS leaves room for one workgroup on each
 constexpr int kXcds = 8;
 constexpr int kMaxBlocks = 256;                // of a maximum over an operand
@@ -307,12 +318,16 @@ __device__ __forceinline__ float as_read(float v) {
 
 // A run of words whose rows of w stay in an XCD's L2 while the rows of x pass by.
 constexpr int kWordTiles = 8;
-template <bool BF, bool kBackward>
-__global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c) {
+template <bool BF, bool kBackward, typename Shape>
+__global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, Shape::kWavesP* Shape::kWavesQ* Shape::kEach / 4) void logits_kernel(
+    const LogitsCall c) {
+  constexpr int kWords = Shape::kWords, kRowsTile = Shape::kRows, kWavesP = Shape::kWavesP, kWavesQ = Shape::kWavesQ;
   using T = Tile<kRows, kRows, kWords, kRowsTile, kWavesP, kWavesQ, true, true, BF ? kBf16 : kHalves>;
   __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
   const int rows = c.count ? *c.count : c.rows;
-  const int row_tiles = (rows + kRowsTile - 1) / kRowsTile, word_tiles = c.words / kWords, tiles = row_tiles * word_tiles;
+  // the backward's D is made up to whole pieces, of zeros past the vocabulary
+  const int words = kBackward ? c.words : min(c.words, c.vocab - c.first);
+  const int row_tiles = (rows + kRowsTile - 1) / kRowsTile, word_tiles = (words + kWords - 1) / kWords, tiles = row_tiles * word_tiles;
   // each XCD has a run of tiles, and its workgroups take them in turn
   const int xcd = blockIdx.x % kXcds, local = blockIdx.x / kXcds, locals = (static_cast<int>(gridDim.x) - xcd + kXcds - 1) / kXcds;
   const int each = tiles / kXcds, rest = tiles % kXcds;
@@ -326,7 +341,7 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
     const int run_words = min(kWordTiles, word_tiles - run * kWordTiles);
     v0 = c.first + (run * kWordTiles + in_run % run_words) * kWords;
     r0 = in_run / run_words * kRowsTile;
-    T::begin(work, lds, Operand{c.w.data + int64_t{v0} * c.w.pitch, c.w.pitch, c.vocab - v0, c.steps},
+    T::begin(work, lds, Operand{c.w.data + int64_t{min(v0, c.vocab - 1)} * c.w.pitch, c.w.pitch, max(c.vocab - v0, 1), c.steps},
              Operand{c.x.data + int64_t{r0} * c.x.pitch, c.x.pitch, rows - r0, c.steps}, c.w.plane, c.x.plane, 0, c.steps);
   };
   if (at < last) begin(at);
@@ -336,8 +351,8 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
     if (at + locals < last) begin(at + locals);   // its loads run under what follows
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
-    // lane's words: this + 64 (i / 4) + 4 (i % 4) + element
-    const int word0 = v + wp * T::kWaveP + 16 * g;
+    // lane's words: this + 32 (i / 2) + 4 (i % 2) + element
+    const int word0 = v + wp * T::kWaveP + 8 * g;
     if constexpr (!BF) {
       const int exponent = -(c.scalars->exponent[0] + c.scalars->exponent[1]);
 #pragma unroll
@@ -353,7 +368,7 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
         for (int i = 0; i < T::kTilesP; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (word0 + 64 * (i / 4) + 4 * (i % 4) + e >= c.vocab) {
+            if (word0 + 32 * (i / 2) + 4 * (i % 2) + e >= c.vocab) {
 #pragma unroll
               for (int j = 0; j < T::kTilesQ; ++j) t.acc[i][j][e] = -INFINITY;
             }
@@ -380,9 +395,9 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
           for (int e = 3; e >= 0; --e) {
             const float z = t.acc[i][j][e];
             sum += __expf(z - most);
-            first = z == most ? 64 * (i / 4) + 4 * (i % 4) + e : first;
+            first = z == most ? 32 * (i / 2) + 4 * (i % 2) + e : first;
           }
-        if (first != INT_MAX) first += wp * T::kWaveP + 16 * g;
+        if (first != INT_MAX) first += wp * T::kWaveP + 8 * g;
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         first = min(first, __shfl_xor(first, 16));
@@ -395,12 +410,12 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
         if (row < rows) {
           const int64_t target = c.targets[c.index ? c.index[row] : row];
           const int own = target >= 0 && target < c.vocab ? static_cast<int>(target) - word0 : -1;
-          if (own >= 0 && own < T::kWaveP && (own & 63) < 16) {
+          if (own >= 0 && own < T::kWaveP && (own & 31) < 8) {
 #pragma unroll
             for (int i = 0; i < T::kTilesP; ++i)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (own == 64 * (i / 4) + 4 * (i % 4) + e) c.row_target[row] = t.acc[i][j][e];
+                if (own == 32 * (i / 2) + 4 * (i % 2) + e) c.row_target[row] = t.acc[i][j][e];
           }
         }
       }
@@ -442,15 +457,15 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
         const int own = of[j].own, top = of[j].top;
         const bool dead = of[j].dead;
 #pragma unroll
-        for (int half = 0; half < T::kTilesP / 4; ++half) {
-          float d[16];
+        for (int pair = 0; pair < T::kTilesP / 2; ++pair) {
+          float d[8];
 #pragma unroll
-          for (int n = 0; n < 16; ++n) d[n] = h * __expf(t.acc[4 * half + n / 4][j][n % 4] - lse);
-          const bool has_own = own >= 64 * half && own < 64 * half + 16, has_top = top >= 64 * half && top < 64 * half + 16;
+          for (int n = 0; n < 8; ++n) d[n] = h * __expf(t.acc[2 * pair + n / 4][j][n % 4] - lse);
+          const bool has_own = own >= 32 * pair && own < 32 * pair + 8, has_top = top >= 32 * pair && top < 32 * pair + 8;
           if (has_own || has_top) {
 #pragma unroll
-            for (int n = 0; n < 16; ++n) {
-              const bool is_own = own == 64 * half + n, is_top = top == 64 * half + n;
+            for (int n = 0; n < 8; ++n) {
+              const bool is_own = own == 32 * pair + n, is_top = top == 32 * pair + n;
               if (is_own) d[n] -= h;
               if (is_top) d[n] += wrap;
               if constexpr (BF) {
@@ -459,25 +474,22 @@ __global__ __launch_bounds__(kThreads, 2) void logits_kernel(const LogitsCall c)
               }
             }
           }
-          const int word = word0 + 64 * half;
-          if (dead || word + 16 > c.vocab) {
+          const int word = word0 + 32 * pair;
+          if (dead || word + 8 > c.vocab) {
 #pragma unroll
-            for (int n = 0; n < 16; ++n)
+            for (int n = 0; n < 8; ++n)
               if (dead || word + n >= c.vocab) d[n] = 0.f;
           }
           char* const to = c.d + (static_cast<int64_t>(row) * c.words + word - c.first) * 2;
+          f16x8 hi;
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            f16x8 hi;
+          for (int n = 0; n < 8; ++n) hi[n] = static_cast<_Float16>(d[n]);
+          *reinterpret_cast<f16x8*>(to) = hi;
+          if constexpr (!BF) {
+            f16x8 lo;
 #pragma unroll
-            for (int n = 0; n < 8; ++n) hi[n] = static_cast<_Float16>(d[8 * q + n]);
-            reinterpret_cast<f16x8*>(to)[q] = hi;
-            if constexpr (!BF) {
-              f16x8 lo;
-#pragma unroll
-              for (int n = 0; n < 8; ++n) lo[n] = static_cast<_Float16>(d[8 * q + n] - static_cast<float>(hi[n]));
-              reinterpret_cast<f16x8*>(to + c.d_plane)[q] = lo;
-            }
+            for (int n = 0; n < 8; ++n) lo[n] = static_cast<_Float16>(d[n] - static_cast<float>(hi[n]));
+            *reinterpret_cast<f16x8*>(to + c.d_plane) = lo;
           }
         }
       }
@@ -492,6 +504,7 @@ struct JoinCall {
   const int64_t* targets;
   const int* place;          // of each row among the parts' rows; null: as it is
   int64_t rows, vocab, ignore_index;
+  int words;                 // of a tile
   float *row_loss, *row_lse, *row_max;
   int32_t* row_argmax;
 };
@@ -510,7 +523,7 @@ __device__ __forceinline__ Run combine(const Run& a, const Run& b) {
 __global__ __launch_bounds__(256) void join_kernel(const JoinCall c) {
   __shared__ Run part[16][17];
   const int own = threadIdx.x & 15, share = threadIdx.x >> 4;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + own, tiles = (c.vocab + kWords - 1) / kWords;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + own, tiles = (c.vocab + c.words - 1) / c.words;
   Run run{-INFINITY, 0.f, INT_MAX};
   const int64_t part_row = row >= c.rows ? -1 : c.place ? c.place[row] : row;
   if (part_row >= 0) {
@@ -570,10 +583,18 @@ struct HiddenCall {
   const int32_t* row_argmax;
   const __bf16* weight;
 };
+// What the sums are multiplied with.
+struct Factor {
+  float reference;
+  int exponent;
+};
+__device__ __forceinline__ Factor weight_factor(const Scalars* s) { return Factor{s->reference, -(kHalfExponent + s->exponent[0])}; }
 template <bool BF>
-__device__ __forceinline__ void finish_hidden(const HiddenCall& c, const Scalars* scalars, int64_t row, int64_t part_row, int64_t channel, f32x4 v) {
-  const float reference = scalars->reference;
-  const int exponent = -(kHalfExponent + (BF ? 0 : scalars->exponent[1]));
+__device__ __forceinline__ Factor hidden_factor(const Scalars* s) {
+  return Factor{s->reference, -(kHalfExponent + (BF ? 0 : s->exponent[1]))};
+}
+template <bool BF>
+__device__ __forceinline__ void finish_hidden(const HiddenCall& c, Factor f, int64_t row, int64_t part_row, int64_t channel, f32x4 v) {
   const bool whole = c.c % 4 == 0;
   if constexpr (BF) {
 #pragma unroll
@@ -593,7 +614,7 @@ __device__ __forceinline__ void finish_hidden(const HiddenCall& c, const Scalars
     }
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], exponent) * reference;
+  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], f.exponent) * f.reference;
   store4<BF>(c.grad, row * c.c + channel, v, c.c - channel, whole);
 }
 
@@ -609,6 +630,8 @@ struct GradientsCall {
   int hidden_blocks;                 // dx's, likewise
   bool hidden_first;
   void* weight_grad;
+  int row_share;             // rows of a workgroup of dw
+  float* weight_sums;        // [row shares, vocab, pitch]; null: one share, dw itself is stored
   int share;                 // words of a workgroup of dx
   bool begin;                // the first piece: no sums to add to
   float* sums;               // [splits, rows, pitch]; null: dx itself is stored
@@ -626,42 +649,55 @@ __device__ __forceinline__ void place(int at, int channel_tiles, int others, int
   other = in_run / width;
 }
 
-// A tile of dw, of the piece's words: steps are rows; those past the last have D = 0.
+// dw of four channels from its sum, in the operands' type.
+template <bool BF>
+__device__ __forceinline__ void finish_weight(void* grad, Factor f, int64_t word, int64_t channel, int64_t c, f32x4 v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], f.exponent) * f.reference;
+  store4<BF>(grad, word * c + channel, v, c - channel, c % 4 == 0);
+}
+
+// A tile of dw, of the piece's words over a share of the rows: steps are rows; those past
+// the last have D = 0.
 template <bool BF, int kChannels>
-__device__ __forceinline__ void weight_tile(const GradientsCall& c, char* lds, int at) {
+__device__ __forceinline__ void weight_tile(const GradientsCall& c, char* lds, int tile) {
   using T = Tile<kSteps, kSteps, kChannels, kGradTile, kWavesP, kWavesQ, false, false, BF ? kHalf : kHalves>;
+  const int channel_tiles = (c.c + kChannels - 1) / kChannels, word_tiles = c.words / kGradTile;
+  const int split = tile / (channel_tiles * word_tiles);
   int channel_tile, word_tile;
-  place(at, (c.c + kChannels - 1) / kChannels, c.words / kGradTile, channel_tile, word_tile);
+  place(tile % (channel_tiles * word_tiles), channel_tiles, word_tiles, channel_tile, word_tile);
   const int c0 = channel_tile * kChannels, w0 = word_tile * kGradTile;
   const int rows = c.count ? *c.count : c.rows;
+  const Factor factor = weight_factor(c.scalars);
+  const int k0 = split * c.row_share, k1 = min(k0 + c.row_share, (rows + kStep - 1) / kStep * kStep);
   T t;
-  if (rows == 0) {
+  if (k0 >= k1) {
     t.clear();
   } else {
     typename T::Work work;
     T::begin(work, lds, Operand{c.x.data + c0 * 2, c.x.pitch, c.c - c0, rows},
-             Operand{c.d + w0 * 2, int64_t{c.words} * 2, c.words - w0, c.padded_rows}, c.x.plane, c.d_plane, 0,
-             (rows + kStep - 1) / kStep * kStep);
+             Operand{c.d + w0 * 2, int64_t{c.words} * 2, c.words - w0, c.padded_rows}, c.x.plane, c.d_plane, k0, k1);
     t.run(work, lds);
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
-  const float reference = c.scalars->reference;
-  const int exponent = -(kHalfExponent + c.scalars->exponent[0]);
-  const bool whole = c.c % 4 == 0;
+  auto all_of = [&](auto store) {
 #pragma unroll
-  for (int j = 0; j < T::kTilesQ; ++j) {
-    const int word = c.first + w0 + wq * T::kWaveQ + 16 * j + m;
-    if (word >= c.vocab) continue;
+    for (int j = 0; j < T::kTilesQ; ++j) {
+      const int word = c.first + w0 + wq * T::kWaveQ + 16 * j + m;
+      if (word >= c.vocab) continue;
 #pragma unroll
-    for (int i = 0; i < T::kTilesP; ++i) {
-      const int channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
-      if (channel >= c.c) continue;
-      f32x4 v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = ldexpf(t.acc[i][j][e], exponent) * reference;
-      store4<BF>(c.weight_grad, int64_t{word} * c.c + channel, v, c.c - channel, whole);
+      for (int i = 0; i < T::kTilesP; ++i) {
+        const int channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
+        if (channel < c.c) store(word, channel, t.acc[i][j]);
+      }
     }
+  };
+  if (c.weight_sums) {
+    float* const sums = c.weight_sums + int64_t{split} * c.vocab * c.pitch;
+    all_of([&](int word, int channel, f32x4 v) { *reinterpret_cast<f32x4*>(sums + int64_t{word} * c.pitch + channel) = v; });
+  } else {
+    all_of([&](int word, int channel, f32x4 v) { finish_weight<BF>(c.weight_grad, factor, word, channel, c.c, v); });
   }
 }
 
@@ -679,28 +715,34 @@ __device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, i
   place(at % each, channel_tiles, row_tiles, channel_tile, row_tile);
   const int c0 = channel_tile * kChannels, r0 = row_tile * kGradTile;
   const int k0 = split * c.share, k1 = min(k0 + c.share, c.words);
+  const Factor factor = hidden_factor<BF>(c.scalars);
   T t;
   typename T::Work work;
   T::begin(work, lds, Operand{c.w.data + int64_t{c.first} * c.w.pitch + c0 * 2, c.w.pitch, c.c - c0, c.vocab - c.first},
-           Operand{c.d + int64_t{r0} * c.words * 2, int64_t{c.words} * 2, kGradTile, c.words}, c.w.plane, c.d_plane, k0, k1);
+           Operand{c.d + int64_t{r0} * c.words * 2, int64_t{c.words} * 2, (rows + kStep - 1) / kStep * kStep - r0, c.words}, c.w.plane, c.d_plane, k0, k1);
   t.run(work, lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
+  auto all_of = [&](auto store) {
 #pragma unroll
-  for (int j = 0; j < T::kTilesQ; ++j) {
-    const int row = r0 + wq * T::kWaveQ + 16 * j + m;
-    if (row >= rows) continue;
+    for (int j = 0; j < T::kTilesQ; ++j) {
+      const int row = r0 + wq * T::kWaveQ + 16 * j + m;
+      if (row >= rows) continue;
 #pragma unroll
-    for (int i = 0; i < T::kTilesP; ++i) {
-      const int channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
-      if (channel >= c.pitch) continue;
-      if (!c.sums) {
-        finish_hidden<BF>(c.hidden, c.scalars, row, row, channel, t.acc[i][j]);
-        continue;
+      for (int i = 0; i < T::kTilesP; ++i) {
+        const int channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
+        if (channel < c.pitch) store(row, channel, t.acc[i][j]);
       }
-      f32x4* const to = reinterpret_cast<f32x4*>(c.sums + (int64_t{split} * c.rows + row) * c.pitch + channel);
-      *to = c.begin ? t.acc[i][j] : *to + t.acc[i][j];
     }
+  };
+  if (c.sums) {
+    float* const sums = c.sums + int64_t{split} * c.rows * c.pitch;
+    all_of([&](int row, int channel, f32x4 v) {
+      f32x4* const to = reinterpret_cast<f32x4*>(sums + int64_t{row} * c.pitch + channel);
+      *to = c.begin ? v : *to + v;
+    });
+  } else {
+    all_of([&](int row, int channel, f32x4 v) { finish_hidden<BF>(c.hidden, factor, row, row, channel, v); });
   }
 }
 
@@ -720,28 +762,39 @@ __global__ __launch_bounds__(kThreads, 2) void gradients_kernel(const GradientsC
   }
 }
 
-// The splits' sums of dx in order.
-struct HiddenSumCall {
-  const float* sums;
-  int64_t rows, pitch;
-  int splits;
+// The shares' sums of dx and of dw, in order.
+struct SumCall {
+  const float *hidden_sums, *weight_sums;   // null: nothing to add
+  int64_t rows, vocab, pitch;
+  int splits, row_splits;
   const int* place;          // of each row among the sums' rows; null: as it is
   const Scalars* scalars;
   HiddenCall hidden;
+  void* weight_grad;
 };
-template <bool BF>
-__global__ __launch_bounds__(256) void hidden_sum_kernel(const HiddenSumCall c) {
-  const int64_t fours = c.pitch / 4, n = c.rows * fours;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = i / fours, four = i % fours, part_row = c.place ? c.place[row] : row;
-    f32x4 v{0.f, 0.f, 0.f, 0.f};
-    if (part_row < 0) {
-      store4<BF>(c.hidden.grad, row * c.hidden.c + 4 * four, v, c.hidden.c - 4 * four, c.hidden.c % 4 == 0);
-      continue;
-    }
+__device__ __forceinline__ f32x4 sum_of(const float* sums, int64_t n, int64_t at, int splits) {
+  f32x4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int s = 0; s < c.splits; ++s) v += reinterpret_cast<const f32x4*>(c.sums)[s * n + part_row * fours + four];
-    finish_hidden<BF>(c.hidden, c.scalars, row, part_row, 4 * four, v);
+  for (int s = 0; s < splits; ++s) v += reinterpret_cast<const f32x4*>(sums)[s * n + at];
+  return v;
+}
+template <bool BF>
+__global__ __launch_bounds__(256) void sum_kernel(const SumCall c) {
+  const int64_t fours = c.pitch / 4, step = static_cast<int64_t>(gridDim.x) * 256;
+  int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (blockIdx.y == 0 && c.hidden_sums) {
+    const int64_t n = c.rows * fours;
+    const Factor factor = hidden_factor<BF>(c.scalars);
+    for (; i < n; i += step) {
+      const int64_t row = i / fours, four = i % fours, part_row = c.place ? c.place[row] : row;
+      if (part_row < 0) store4<BF>(c.hidden.grad, row * c.hidden.c + 4 * four, f32x4{0.f, 0.f, 0.f, 0.f}, c.hidden.c - 4 * four, c.hidden.c % 4 == 0);
+      else finish_hidden<BF>(c.hidden, factor, row, part_row, 4 * four, sum_of(c.hidden_sums, n, part_row * fours + four, c.splits));
+    }
+  } else if (blockIdx.y == 1 && c.weight_sums) {
+    const int64_t n = c.vocab * fours;
+    const Factor factor = weight_factor(c.scalars);
+    for (; i < n; i += step)
+      finish_weight<BF>(c.weight_grad, factor, i / fours, i % fours * 4, c.hidden.c, sum_of(c.weight_sums, n, i, c.row_splits));
   }
 }
 
@@ -786,16 +839,18 @@ Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward
   return p;
 }
 
-// D of a piece takes at most kMaxD bytes, of which the least is a tile of words. dx's
-// shares: those with which the two gradients' tiles, handed to the compute units in turn,
-// the longer ones first, are done first, in stages; a tile's first loads and its stores
-// count as kOverhead stages, the launch that adds shares up as kLaunch, and the sums' way
-// to memory and back as kBytesPerStage has it.
-constexpr int64_t kMaxD = int64_t{512} << 20, kOverhead = 4, kLaunch = 4, kMaxSplits = 64, kBytesPerStage = int64_t{4} << 20;
+// D of a piece takes at most kMaxD bytes, of which the least is a tile of words. The
+// gradients' shares, of dx over the words and, of a vocabulary in one piece, of dw over
+// the rows: those with which the tiles, handed to the compute units in turn, the longer
+// ones first, are done first, in stages. A tile's first loads and its stores count as
+// kOverhead stages, the launch that adds shares up as kLaunch, and the sums' way to memory
+// and back as kBytesPerStage has it.
+constexpr int64_t kMaxD = int64_t{512} << 20, kOverhead = 4, kLaunch = 4, kMaxSplits = 64, kBytesPerStage = int64_t{8} << 20;
 struct Plan {
   int channels;                     // of a gradient's tile
   int64_t words, pieces;            // of a piece
-  int64_t padded_rows, splits, share, pitch;
+  int64_t padded_rows, pitch;
+  int64_t splits, share, row_splits, row_share;
   bool hidden_first;
 };
 // when `more` tiles of `more_each` are done behind `tiles` longer ones of `each`
@@ -809,30 +864,38 @@ int64_t finish(int64_t tiles, int64_t each, int64_t more, int64_t more_each) {
 Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   Plan p{};
   p.channels = (c - 1) % 256 < 128 ? 128 : 256;
-  p.padded_rows = up(rows, kRowsTile);
+  p.padded_rows = up(rows, kGradTile);
   p.pitch = up(c, 4);
   const int64_t channel_tiles = ceil_div(c, p.channels), planes = bf16 ? 1 : 2;
-  const int64_t all = up(vocab, kWords);
-  const int64_t most = std::max<int64_t>(kWords, kMaxD / (p.padded_rows * 2 * planes) / kWords * kWords);
+  const int64_t all = up(vocab, kWholeWords);
+  const int64_t most = std::max<int64_t>(kWholeWords, kMaxD / (p.padded_rows * 2 * planes) / kWholeWords * kWholeWords);
   p.pieces = ceil_div(all, most);
-  p.words = up(ceil_div(all, p.pieces), kWords);
+  p.words = up(ceil_div(all, p.pieces), kWholeWords);
   p.pieces = ceil_div(all, p.words);
   const int64_t weight_tiles = channel_tiles * ceil_div(p.words, kGradTile), hidden_tiles = channel_tiles * p.padded_rows / kGradTile;
-  const int64_t parts = bf16 ? 1 : 3, weight_time = ceil_div(rows, kStep) * parts + kOverhead;
+  const int64_t parts = bf16 ? 1 : 3;
   int64_t least = INT64_MAX;
-  for (int64_t s = 1; s <= kMaxSplits; ++s) {
-    const int64_t share = up(ceil_div(p.words, s), kStep), splits = ceil_div(p.words, share);
-    if (splits < s) continue;
-    const int64_t hidden_time = share / kStep * parts + kOverhead;
-    const int64_t moved = (splits > 1 ? kLaunch : 0) + splits * rows * p.pitch * 8 / kBytesPerStage;
-    if (moved >= least) break;
-    const int64_t time = moved + (hidden_time > weight_time ? finish(hidden_tiles * splits, hidden_time, weight_tiles, weight_time)
-                                                            : finish(weight_tiles, weight_time, hidden_tiles * splits, hidden_time));
-    if (time >= least) continue;
-    least = time;
-    p.splits = splits;
-    p.share = share;
-    p.hidden_first = hidden_time > weight_time;
+  for (int64_t r = 1; r <= (p.pieces == 1 ? kMaxSplits : 1); r *= 2) {
+    const int64_t row_share = up(ceil_div(rows, r), kStep), row_splits = ceil_div(rows, row_share);
+    if (row_splits < r) break;
+    const int64_t weight_time = row_share / kStep * parts + kOverhead;
+    const int64_t weight_moved = row_splits > 1 ? kLaunch + row_splits * vocab * p.pitch * 8 / kBytesPerStage : 0;
+    for (int64_t s = 1; s <= kMaxSplits; ++s) {
+      const int64_t share = up(ceil_div(p.words, s), kStep), splits = ceil_div(p.words, share);
+      if (splits < s) continue;
+      const int64_t hidden_time = share / kStep * parts + kOverhead;
+      const int64_t moved = (splits > 1 ? kLaunch + splits * rows * p.pitch * 8 / kBytesPerStage : 0) + weight_moved;
+      if (moved >= least) break;
+      const int64_t time = moved + (hidden_time > weight_time ? finish(hidden_tiles * splits, hidden_time, weight_tiles * row_splits, weight_time)
+                                                              : finish(weight_tiles * row_splits, weight_time, hidden_tiles * splits, hidden_time));
+      if (time >= least) continue;
+      least = time;
+      p.splits = splits;
+      p.share = share;
+      p.row_splits = row_splits;
+      p.row_share = row_share;
+      p.hidden_first = hidden_time > weight_time;
+    }
   }
   return p;
 }
@@ -841,7 +904,7 @@ Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
 bool needs_sums(const Plan& p, int64_t rows) { return p.splits > 1 || p.pieces > 1 || numbered(rows); }
 struct BackwardPlaces {
   Places operands;
-  int64_t d, d_plane, sums, residuals, end;
+  int64_t d, d_plane, sums, weight_sums, residuals, end;
 };
 BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   BackwardPlaces b{};
@@ -850,9 +913,36 @@ BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64
   b.d_plane = p.padded_rows * p.words * 2;
   b.d = take(b.end, b.d_plane * (bf16 ? 1 : 2));
   b.sums = !needs_sums(p, rows) ? 0 : take(b.end, p.splits * rows * p.pitch * 4);
+  b.weight_sums = p.row_splits == 1 ? 0 : take(b.end, p.row_splits * vocab * p.pitch * 4);
   b.residuals = take(b.end, 2 * rows * 4);
   return b;
 }
+
+// The tile with which the logits are done first: as many workgroups as there are places
+// for them take the tiles in turn, each `first` and `stage` times the steps of a tile, in
+// ns.
+enum { kBig, kMiddle, kSmall };
+struct Shape {
+  int words, rows, places;
+  int64_t first, stage;
+};
+constexpr Shape kShapes[] = {{Big::kWords, Big::kRows, kUnits * Big::kEach, 6000, 1200},
+                             {Middle::kWords, Middle::kRows, kUnits * Middle::kEach, 4000, 900},
+                             {Small::kWords, Small::kRows, kUnits * Small::kEach, 3000, 700}};
+int shape_of(int64_t rows, int64_t words, int64_t c, bool bf16) {
+  int best = kBig;
+  int64_t least = INT64_MAX;
+  for (int i = kBig; i <= kSmall; ++i) {
+    const Shape& t = kShapes[i];
+    const int64_t tiles = ceil_div(words, t.words) * ceil_div(rows, t.rows);
+    const int64_t time = ceil_div(tiles, t.places) * (t.first + t.stage * ceil_div(c, kStep) * (bf16 ? 1 : 3));
+    if (time >= least) continue;
+    least = time;
+    best = i;
+  }
+  return best;
+}
+int shape_words(int shape) { return kShapes[shape].words; }
 
 struct ForwardPlaces {
   Places operands;
@@ -862,7 +952,7 @@ ForwardPlaces forward_places(int64_t rows, int64_t vocab, int64_t c, bool bf16) 
   ForwardPlaces f{};
   f.operands = operands(rows, vocab, c, bf16, false);
   f.end = f.operands.end;
-  const int64_t parts = ceil_div(vocab, kWords) * rows * 4;
+  const int64_t parts = ceil_div(vocab, shape_words(shape_of(rows, vocab, c, bf16))) * rows * 4;
   f.part_max = take(f.end, parts);
   f.part_sum = take(f.end, parts);
   f.part_argmax = take(f.end, parts);
@@ -935,10 +1025,17 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
 // workgroups of 256 for n threads; a launch has fewer than 2^32 of these
 dim3 grid_of(int64_t n) { return dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n, 256), 1 << 22))); }
 
+template <bool BF, bool kBackward, typename Shape>
+void logits(const LogitsCall& l, hipStream_t s) {
+  const int64_t tiles = l.words / Shape::kWords * ceil_div(l.rows, Shape::kRows);
+  hipLaunchKernelGGL((logits_kernel<BF, kBackward, Shape>), dim3(static_cast<unsigned>(std::min<int64_t>(tiles, kUnits * Shape::kEach))),
+                     dim3(64 * Shape::kWavesP * Shape::kWavesQ), 0, s, l);
+}
 template <bool BF, bool kBackward>
-void logits(LogitsCall& l, hipStream_t s) {
-  const int64_t tiles = l.words / kWords * ceil_div(l.rows, kRowsTile);
-  hipLaunchKernelGGL((logits_kernel<BF, kBackward>), dim3(static_cast<unsigned>(std::min<int64_t>(tiles, kUnits))), dim3(kThreads), 0, s, l);
+void logits(const LogitsCall& l, int shape, hipStream_t s) {
+  if (shape == kBig) logits<BF, kBackward, Big>(l, s);
+  else if (shape == kMiddle) logits<BF, kBackward, Middle>(l, s);
+  else logits<BF, kBackward, Small>(l, s);
 }
 
 template <bool BF>
@@ -953,15 +1050,16 @@ void forward(const ForwardCall& c, hipStream_t s) {
   l.rows = static_cast<int>(c.rows);
   l.vocab = static_cast<int>(c.vocab);
   l.steps = static_cast<int>(up(c.c, kStep));
-  l.words = static_cast<int>(up(c.vocab, kWords));
+  l.words = static_cast<int>(up(c.vocab, kWholeWords));
   l.scalars = reinterpret_cast<const Scalars*>(c.workspace + f.operands.scalars);
   l.targets = c.targets;
   l.part_max = reinterpret_cast<float*>(c.workspace + f.part_max);
   l.part_sum = reinterpret_cast<float*>(c.workspace + f.part_sum);
   l.part_argmax = reinterpret_cast<int*>(c.workspace + f.part_argmax);
   l.row_target = reinterpret_cast<float*>(c.workspace + f.row_target);
-  logits<BF, false>(l, s);
-  const JoinCall j{l.part_max, l.part_sum, l.row_target, l.part_argmax, c.targets, o.place, c.rows, c.vocab, c.ignore_index,
+  const int shape = shape_of(c.rows, c.vocab, c.c, BF);
+  logits<BF, false>(l, shape, s);
+  const JoinCall j{l.part_max, l.part_sum, l.row_target, l.part_argmax, c.targets, o.place, c.rows, c.vocab, c.ignore_index, shape_words(shape),
                    c.row_loss, c.row_lse, c.row_max, c.row_argmax};
   hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>(ceil_div(c.rows, 16))), dim3(256), 0, s, j);
 }
@@ -1004,6 +1102,8 @@ void backward(const BackwardCall& c, hipStream_t s) {
   g.c = static_cast<int>(c.c);
   g.scalars = scalars;
   g.weight_grad = c.weight_grad;
+  g.row_share = static_cast<int>(p.row_share);
+  g.weight_sums = p.row_splits == 1 ? nullptr : reinterpret_cast<float*>(c.workspace + b.weight_sums);
   g.share = static_cast<int>(p.share);
   const bool direct = !needs_sums(p, c.rows);
   g.sums = direct ? nullptr : reinterpret_cast<float*>(c.workspace + b.sums);
@@ -1013,10 +1113,10 @@ void backward(const BackwardCall& c, hipStream_t s) {
   const int64_t channel_tiles = ceil_div(c.c, p.channels);
   for (int64_t first = 0; first < c.vocab; first += p.words) {
     g.first = l.first = static_cast<int>(first);
-    g.words = l.words = static_cast<int>(std::min(p.words, up(c.vocab - first, kWords)));
-    logits<BF, true>(l, s);
+    g.words = l.words = static_cast<int>(std::min(p.words, up(c.vocab - first, kWholeWords)));
+    logits<BF, true>(l, shape_of(c.rows, l.words, c.c, BF), s);
     g.begin = first == 0;
-    g.weight_tiles = c.weight_grad ? static_cast<int>(channel_tiles * (l.words / kGradTile)) : 0;
+    g.weight_tiles = c.weight_grad ? static_cast<int>(channel_tiles * (l.words / kGradTile) * p.row_splits) : 0;
     g.weight_blocks = static_cast<int>(up(g.weight_tiles, kXcds));
     g.hidden_blocks = c.hidden_grad ? static_cast<int>(up(channel_tiles * (p.padded_rows / kGradTile) * ceil_div(l.words, p.share), kXcds)) : 0;
     g.hidden_first = p.hidden_first;
@@ -1024,9 +1124,22 @@ void backward(const BackwardCall& c, hipStream_t s) {
     if (p.channels == 128) hipLaunchKernelGGL((gradients_kernel<BF, 128>), grid, dim3(kThreads), 0, s, g);
     else hipLaunchKernelGGL((gradients_kernel<BF, 256>), grid, dim3(kThreads), 0, s, g);
   }
-  if (c.hidden_grad && !direct) {
-    const HiddenSumCall h{g.sums, c.rows, p.pitch, static_cast<int>(p.splits), o.place, scalars, g.hidden};
-    hipLaunchKernelGGL(hidden_sum_kernel<BF>, grid_of(c.rows * p.pitch / 4), dim3(256), 0, s, h);
+  SumCall u{};
+  u.hidden_sums = c.hidden_grad ? g.sums : nullptr;
+  u.weight_sums = c.weight_grad ? g.weight_sums : nullptr;
+  if (u.hidden_sums || u.weight_sums) {
+    u.rows = c.rows;
+    u.vocab = c.vocab;
+    u.pitch = p.pitch;
+    u.splits = static_cast<int>(p.splits);
+    u.row_splits = static_cast<int>(p.row_splits);
+    u.place = o.place;
+    u.scalars = scalars;
+    u.hidden = g.hidden;
+    u.weight_grad = c.weight_grad;
+    dim3 grid = grid_of(std::max(u.hidden_sums ? c.rows : 0, u.weight_sums ? c.vocab : 0) * p.pitch / 4);
+    grid.y = u.weight_sums ? 2 : 1;
+    hipLaunchKernelGGL(sum_kernel<BF>, grid, dim3(256), 0, s, u);
   }
 }
 

@@ -77,10 +77,10 @@ struct Operand {
 
 enum Layout { kRows, kSteps };
 // Where the 16-byte pieces of a row lie, so that the lanes of a read touch different
-// banks. kSpread: tile i's lane m reads row 64 (i / 4) + 16 (m / 4) + 4 (i % 4) + m %
-// 4 instead of 16 i + m, which leaves a lane with 16 consecutive p.
+// banks. kSpread: tile i's lane m reads row 32 (i / 2) + 8 (m / 4) + 4 (i % 2) + m %
+// 4 instead of 16 i + m, which leaves a lane with 8 consecutive p of two tiles.
 template <bool kSpread>
-__device__ __forceinline__ int row_swizzle(int row) { return ((-(row >> (kSpread ? 4 : 2))) & 3) + 2 * (row & 2); }
+__device__ __forceinline__ int row_swizzle(int row) { return ((-(row >> (kSpread ? 3 : 2))) & 3) + 2 * (row & 2); }
 __device__ __forceinline__ int step_swizzle(int k) { return (k & 3) | ((k >> 1) & 4); }
 
 // How a workgroup's lanes bring an operand of kItems to LDS and read it back.
@@ -142,7 +142,7 @@ struct Side {
   // over half a stage's steps
   __device__ __forceinline__ s16x8 read(const char* lds, int half, int first, int i, int m, int g) const {
     if constexpr (kLayout == kRows) {
-      const int row = first + (kSpread ? 64 * (i / 4) + 16 * (m >> 2) + 4 * (i % 4) + (m & 3) : 16 * i + m);
+      const int row = first + (kSpread ? 32 * (i / 2) + 8 * (m >> 2) + 4 * (i % 2) + (m & 3) : 16 * i + m);
       return *reinterpret_cast<const s16x8*>(lds + row * kStepBytes + 16 * ((4 * half + g) ^ row_swizzle<kSpread>(row)));
     } else {
       typedef __attribute__((address_space(3))) s16x4* Local;
@@ -171,7 +171,7 @@ struct Tile {
   static constexpr int kWaves = kWavesP * kWavesQ, kThreads = 64 * kWaves;
   static constexpr int kWaveP = kP / kWavesP, kWaveQ = kQ / kWavesQ;
   static constexpr int kTilesP = kWaveP / 16, kTilesQ = kWaveQ / 16;
-  static_assert(!kSpread || kWaveP % 64 == 0);
+  static_assert(!kSpread || kWaveP % 32 == 0);
   using SideP = Side<kLayoutP, kP, kWaves, kSpread>;
   using SideQ = Side<kLayoutQ, kQ, kWaves, false>;
   static constexpr int kSlotsP = kDeepP ? 3 : 2, kSlotsQ = kDeepP ? 2 : 3;
