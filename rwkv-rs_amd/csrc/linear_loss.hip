@@ -38,6 +38,23 @@ struct Middle {
 struct Small {
   static constexpr int kWords = 64, kRows = 64, kWavesP = 2, kWavesQ = 2, kEach = 4;
 };
+// Of fp32 operands where there are few rows: w is split on its way to the products.
+struct Few {
+  static constexpr int kWords = 256, kRows = 64, kWavesP = 4, kWavesQ = 1, kEach = 1, kSlots = 3;
+};
+struct FewSmall {
+  static constexpr int kWords = 64, kRows = 64, kWavesP = 2, kWavesQ = 1, kEach = 1, kSlots = 5;
+};
+template <typename Shape>
+constexpr bool kIsFew = std::is_same<Shape, Few>::value || std::is_same<Shape, FewSmall>::value;
+template <typename Shape, Kind kKind, bool kFew = kIsFew<Shape>>
+struct LogitsTile {
+  using T = Tile<kRows, kRows, Shape::kWords, Shape::kRows, Shape::kWavesP, Shape::kWavesQ, true, true, kKind>;
+};
+template <typename Shape, Kind kKind>
+struct LogitsTile<Shape, kKind, true> {
+  using T = FewTile<kRows, Shape::kWords, Shape::kRows, Shape::kWavesP, true, Shape::kSlots>;
+};
 constexpr int kWholeWords = 256;               // a piece of the vocabulary is whole tiles of any size
 constexpr int kWavesP = 2, kWavesQ = 4, kThreads = 512;   // of a gradient's tile
 constexpr int kUnits = 256;                    // compute units; a tile's LDS leaves room for one workgroup on each
@@ -193,7 +210,8 @@ __global__ __launch_bounds__(kWide) void survey_kernel(const SurveyCall c) {
 }
 
 // One array made of another: rows of `padded` elements, zeros behind the c there are.
-enum PackKind { kCopy, kToHalf, kToHalves };   // bf16 as it is; bf16 to fp16; fp32 to two of fp16
+// bf16 as it is; bf16 to fp16; fp32 to two of fp16, or to three of bf16
+enum PackKind { kCopy, kToHalf, kToHalves, kToThirds };
 struct PackJob {
   const void* from;
   char* to;
@@ -228,7 +246,9 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
     if (writes) c.scalars->reference = most ? __builtin_bit_cast(float, most) : 1.f;
   }
   if (static_cast<int>(blockIdx.y) >= c.jobs) return;
-  if (job.kind != kCopy) {
+  if (job.kind == kToThirds) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) c.scalars->exponent[0] = c.scalars->exponent[1] = 0;
+  } else if (job.kind != kCopy) {
     exponent = exponent_of(block_max<4>(c.largest[job.which * kMaxBlocks + threadIdx.x]));
     if (blockIdx.x == 0 && threadIdx.x == 0) c.scalars->exponent[job.which] = exponent;
   }
@@ -245,8 +265,9 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
       if (ignored) {
         char* const to = job.to + (row * c.padded + 8 * i) * 2;
         *reinterpret_cast<u32x4*>(to) = u32x4{0, 0, 0, 0};
-        if (job.kind == kToHalves) *reinterpret_cast<u32x4*>(to + plane * 2) = u32x4{0, 0, 0, 0};
-      } else if (job.kind == kToHalves) {
+        if (job.kind == kToHalves || job.kind == kToThirds) *reinterpret_cast<u32x4*>(to + plane * 2) = u32x4{0, 0, 0, 0};
+        if (job.kind == kToThirds) *reinterpret_cast<u32x4*>(to + plane * 4) = u32x4{0, 0, 0, 0};
+      } else if (job.kind == kToHalves || job.kind == kToThirds) {
         float v[8];
         const float* const from = static_cast<const float*>(job.from) + at;
         if (whole && 8 * i < c.c) {
@@ -256,6 +277,13 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = 8 * i + e < c.c ? from[e] : 0.f;
+        }
+        if (job.kind == kToThirds) {
+          s16x8 part[3];
+          thirds(v, part);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) *reinterpret_cast<s16x8*>(job.to + (row * c.padded + 8 * i + k * plane) * 2) = part[k];
+          continue;
         }
         f16x8 hi, lo;
 #pragma unroll
@@ -293,7 +321,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
 // ------------------------------------------------------------------------- logits
 struct LogitsCall {
   Matrix x, w;
-  int rows, vocab, steps;        // steps: c up to a whole step
+  int rows, vocab, c, steps;     // steps: c up to whole stages
   int first, words;              // the piece of the vocabulary, whole tiles
   const int *index, *count;      // the rows that x's are, and how many; null: all as they are
   const Scalars* scalars;
@@ -306,7 +334,7 @@ struct LogitsCall {
   const float *row_lse, *row_max, *row_grad;
   const int32_t* row_argmax;
   float l2wrap_scale;
-  char* d;                       // [rows up to whole tiles, words] fp16; for fp32 two of them
+  char* d;                       // [rows up to whole tiles, words] fp16; for fp32 two of them, or three of bf16
   int64_t d_plane;
   float* residuals;              // [2, rows], bf16 operands: what rounding took from D at the target and at the argmax
 };
@@ -319,10 +347,11 @@ __device__ __forceinline__ float as_read(float v) {
 // A run of words whose rows of w stay in an XCD's L2 while the rows of x pass by.
 constexpr int kWordTiles = 8;
 template <bool BF, bool kBackward, typename Shape>
-__global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, Shape::kWavesP* Shape::kWavesQ* Shape::kEach / 4) void logits_kernel(
+__global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, std::max(Shape::kWavesP* Shape::kWavesQ* Shape::kEach / 4, 1)) void logits_kernel(
     const LogitsCall c) {
-  constexpr int kWords = Shape::kWords, kRowsTile = Shape::kRows, kWavesP = Shape::kWavesP, kWavesQ = Shape::kWavesQ;
-  using T = Tile<kRows, kRows, kWords, kRowsTile, kWavesP, kWavesQ, true, true, BF ? kBf16 : kHalves>;
+  constexpr int kWords = Shape::kWords, kRowsTile = Shape::kRows, kWavesP = Shape::kWavesP;
+  constexpr bool kFew = kIsFew<Shape>;
+  using T = typename LogitsTile<Shape, BF ? kBf16 : kHalves>::T;
   __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
   const int rows = c.count ? *c.count : c.rows;
   // the backward's D is made up to whole pieces, of zeros past the vocabulary
@@ -341,7 +370,7 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, Shape::kWaves
     const int run_words = min(kWordTiles, word_tiles - run * kWordTiles);
     v0 = c.first + (run * kWordTiles + in_run % run_words) * kWords;
     r0 = in_run / run_words * kRowsTile;
-    T::begin(work, lds, Operand{c.w.data + int64_t{min(v0, c.vocab - 1)} * c.w.pitch, c.w.pitch, max(c.vocab - v0, 1), c.steps},
+    T::begin(work, lds, Operand{c.w.data + int64_t{min(v0, c.vocab - 1)} * c.w.pitch, c.w.pitch, max(c.vocab - v0, 1), kFew ? c.c : c.steps},
              Operand{c.x.data + int64_t{r0} * c.x.pitch, c.x.pitch, rows - r0, c.steps}, c.w.plane, c.x.plane, 0, c.steps);
   };
   if (at < last) begin(at);
@@ -353,7 +382,7 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, Shape::kWaves
     const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
     // lane's words: this + 32 (i / 2) + 4 (i % 2) + element
     const int word0 = v + wp * T::kWaveP + 8 * g;
-    if constexpr (!BF) {
+    if constexpr (!BF && !kFew) {
       const int exponent = -(c.scalars->exponent[0] + c.scalars->exponent[1]);
 #pragma unroll
       for (int i = 0; i < T::kTilesP; ++i)
@@ -422,14 +451,21 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, Shape::kWaves
       __syncthreads();
       if (threadIdx.x < kRowsTile && r + static_cast<int>(threadIdx.x) < rows) {
         const int q = threadIdx.x;
-        const float a = maxima[q], b = maxima[kRowsTile + q];
-        const float most = fmaxf(a, b), sa = sums[q], sb = sums[kRowsTile + q];
+        float most = maxima[q];
+#pragma unroll
+        for (int w = 1; w < kWavesP; ++w) most = fmaxf(most, maxima[w * kRowsTile + q]);
+        float sum = 0.f;
+        int f = INT_MAX;
+#pragma unroll
+        for (int w = kWavesP - 1; w >= 0; --w) {
+          const float own = maxima[w * kRowsTile + q];
+          // a wave without a word (or all of minus infinity) has a NaN for a sum
+          sum += own == -INFINITY ? 0.f : sums[w * kRowsTile + q] * __expf(own - most);
+          if (own == most) f = firsts[w * kRowsTile + q];
+        }
         const int64_t to = int64_t{v / kWords} * c.rows + r + q;
-        const int fa = firsts[q], fb = firsts[kRowsTile + q];
         c.part_max[to] = most;
-        // a half without a word (or all of minus infinity) has a NaN for a sum
-        c.part_sum[to] = (a == -INFINITY ? 0.f : sa * __expf(a - most)) + (b == -INFINITY ? 0.f : sb * __expf(b - most));
-        const int f = a >= b ? fa : fb;
+        c.part_sum[to] = sum;
         c.part_argmax[to] = f == INT_MAX ? INT_MAX : v + f;
       }
     } else {
@@ -481,6 +517,13 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, Shape::kWaves
               if (dead || word + n >= c.vocab) d[n] = 0.f;
           }
           char* const to = c.d + (static_cast<int64_t>(row) * c.words + word - c.first) * 2;
+          if constexpr (kFew) {
+            s16x8 part[3];
+            thirds(d, part);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) *reinterpret_cast<s16x8*>(to + k * c.d_plane) = part[k];
+            continue;
+          }
           f16x8 hi;
 #pragma unroll
           for (int n = 0; n < 8; ++n) hi[n] = static_cast<_Float16>(d[n]);
@@ -595,7 +638,7 @@ __device__ __forceinline__ Factor hidden_factor(const Scalars* s) {
 }
 template <bool BF>
 __device__ __forceinline__ void finish_hidden(const HiddenCall& c, Factor f, int64_t row, int64_t part_row, int64_t channel, f32x4 v) {
-  const bool whole = c.c % 4 == 0;
+  const bool whole = c.c % 8 == 0;
   if constexpr (BF) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -654,14 +697,14 @@ template <bool BF>
 __device__ __forceinline__ void finish_weight(void* grad, Factor f, int64_t word, int64_t channel, int64_t c, f32x4 v) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], f.exponent) * f.reference;
-  store4<BF>(grad, word * c + channel, v, c - channel, c % 4 == 0);
+  store4<BF>(grad, word * c + channel, v, c - channel, c % 8 == 0);
 }
 
 // A tile of dw, of the piece's words over a share of the rows: steps are rows; those past
 // the last have D = 0.
-template <bool BF, int kChannels>
+template <bool BF, int kChannels, bool kFew>
 __device__ __forceinline__ void weight_tile(const GradientsCall& c, char* lds, int tile) {
-  using T = Tile<kSteps, kSteps, kChannels, kGradTile, kWavesP, kWavesQ, false, false, BF ? kHalf : kHalves>;
+  using T = Tile<kSteps, kSteps, kChannels, kGradTile, kWavesP, kWavesQ, false, false, BF ? kHalf : kFew ? kThirds : kHalves>;
   const int channel_tiles = (c.c + kChannels - 1) / kChannels, word_tiles = c.words / kGradTile;
   const int split = tile / (channel_tiles * word_tiles);
   int channel_tile, word_tile;
@@ -701,24 +744,34 @@ __device__ __forceinline__ void weight_tile(const GradientsCall& c, char* lds, i
   }
 }
 
+template <bool BF, int kChannels, bool kFew>
+struct HiddenTile {
+  using T = Tile<kSteps, kRows, kChannels, kGradTile, kWavesP, kWavesQ, false, true, BF ? kHalfQ : kHalves>;
+};
+template <int kChannels>
+struct HiddenTile<false, kChannels, true> {
+  using T = FewTile<kSteps, kChannels, Few::kRows, Few::kWavesP, false>;
+};
+
 // A tile of dx, over a share of the piece's words; the words past the vocabulary have D =
 // 0. There are as many workgroups as all rows would need.
-template <bool BF, int kChannels>
+template <bool BF, int kChannels, bool kFew>
 __device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, int block) {
-  using T = Tile<kSteps, kRows, kChannels, kGradTile, kWavesP, kWavesQ, false, true, BF ? kHalfQ : kHalves>;
+  using T = typename HiddenTile<BF, kChannels, kFew>::T;
+  constexpr int kTileRows = T::kItemsQ, kWavesP = T::kAcross;
   const int rows = c.count ? *c.count : c.rows;
-  const int channel_tiles = (c.c + kChannels - 1) / kChannels, row_tiles = (rows + kGradTile - 1) / kGradTile;
+  const int channel_tiles = (c.c + kChannels - 1) / kChannels, row_tiles = (rows + kTileRows - 1) / kTileRows;
   const int each = channel_tiles * row_tiles, all = each * ((c.words + c.share - 1) / c.share);
   if (block >= all) return;
   const int at = tile_of_block(block, all), split = at / each;
   int channel_tile, row_tile;
   place(at % each, channel_tiles, row_tiles, channel_tile, row_tile);
-  const int c0 = channel_tile * kChannels, r0 = row_tile * kGradTile;
+  const int c0 = channel_tile * kChannels, r0 = row_tile * kTileRows;
   const int k0 = split * c.share, k1 = min(k0 + c.share, c.words);
   const Factor factor = hidden_factor<BF>(c.scalars);
   T t;
   typename T::Work work;
-  T::begin(work, lds, Operand{c.w.data + int64_t{c.first} * c.w.pitch + c0 * 2, c.w.pitch, c.c - c0, c.vocab - c.first},
+  T::begin(work, lds, Operand{c.w.data + int64_t{c.first} * c.w.pitch + c0 * (kFew ? 4 : 2), c.w.pitch, c.c - c0, c.vocab - c.first},
            Operand{c.d + int64_t{r0} * c.words * 2, int64_t{c.words} * 2, (rows + kStep - 1) / kStep * kStep - r0, c.words}, c.w.plane, c.d_plane, k0, k1);
   t.run(work, lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -748,18 +801,31 @@ __device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, i
 
 // Both gradients of a piece side by side: first the longer tiles, then the shorter ones,
 // which fill the compute units that have none of the last of those.
+template <int kChannels>
+constexpr int kWeightLds = Tile<kSteps, kSteps, kChannels, kGradTile, kWavesP, kWavesQ, false, false, kHalves>::kLdsBytes;
 template <bool BF, int kChannels>
 __global__ __launch_bounds__(kThreads, 2) void gradients_kernel(const GradientsCall c) {
-  using T = Tile<kSteps, kRows, kChannels, kGradTile, kWavesP, kWavesQ, false, true, kHalves>;
-  using U = Tile<kSteps, kSteps, kChannels, kGradTile, kWavesP, kWavesQ, false, false, kHalves>;
-  __shared__ __attribute__((aligned(16))) char lds[std::max(T::kLdsBytes, U::kLdsBytes)];
+  __shared__ __attribute__((aligned(16))) char lds[std::max(HiddenTile<BF, kChannels, false>::T::kLdsBytes, kWeightLds<kChannels>)];
   const int weight = static_cast<int>(blockIdx.x) - (c.hidden_first ? c.hidden_blocks : 0);
   if (weight >= 0 && weight < c.weight_blocks) {
     const int at = tile_of_block(weight, c.weight_blocks);
-    if (at < c.weight_tiles) weight_tile<BF, kChannels>(c, lds, at);
+    if (at < c.weight_tiles) weight_tile<BF, kChannels, false>(c, lds, at);
   } else {
-    hidden_tile<BF, kChannels>(c, lds, c.hidden_first ? static_cast<int>(blockIdx.x) : weight - c.weight_blocks);
+    hidden_tile<BF, kChannels, false>(c, lds, c.hidden_first ? static_cast<int>(blockIdx.x) : weight - c.weight_blocks);
   }
+}
+
+// Of few rows, one after the other: memory bounds both.
+template <int kChannels>
+__global__ __launch_bounds__(kThreads, 2) void few_weight_kernel(const GradientsCall c) {
+  __shared__ __attribute__((aligned(16))) char lds[kWeightLds<kChannels>];
+  const int at = tile_of_block(blockIdx.x, c.weight_blocks);
+  if (at < c.weight_tiles) weight_tile<false, kChannels, true>(c, lds, at);
+}
+template <int kChannels>
+__global__ __launch_bounds__(64 * Few::kWavesP, 1) void few_hidden_kernel(const GradientsCall c) {
+  __shared__ __attribute__((aligned(16))) char lds[HiddenTile<false, kChannels, true>::T::kLdsBytes];
+  hidden_tile<false, kChannels, true>(c, lds, blockIdx.x);
 }
 
 // The shares' sums of dx and of dw, in order.
@@ -787,7 +853,7 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumCall c) {
     const Factor factor = hidden_factor<BF>(c.scalars);
     for (; i < n; i += step) {
       const int64_t row = i / fours, four = i % fours, part_row = c.place ? c.place[row] : row;
-      if (part_row < 0) store4<BF>(c.hidden.grad, row * c.hidden.c + 4 * four, f32x4{0.f, 0.f, 0.f, 0.f}, c.hidden.c - 4 * four, c.hidden.c % 4 == 0);
+      if (part_row < 0) store4<BF>(c.hidden.grad, row * c.hidden.c + 4 * four, f32x4{0.f, 0.f, 0.f, 0.f}, c.hidden.c - 4 * four, c.hidden.c % 8 == 0);
       else finish_hidden<BF>(c.hidden, factor, row, part_row, 4 * four, sum_of(c.hidden_sums, n, part_row * fours + four, c.splits));
     }
   } else if (blockIdx.y == 1 && c.weight_sums) {
@@ -811,6 +877,18 @@ bool numbered(int64_t rows) { return rows >= kManyRows; }
 // bf16 operands whose rows are whole steps are read where they are.
 bool packed(int64_t c, bool bf16) { return !bf16 || c % kStep != 0; }
 
+// fp32 operands with few rows and a w that is nearly all there is to read: w is read where
+// it is, three times in the two calls, where packing it to fp16 reads or writes it eleven
+// times in all. Against the packed form, us for both calls: 1 to 64 rows of 768 with 65536
+// words 230 and 480, 128 rows 352 and 514, 192 rows 490 and 531, 256 rows 634 and 571; 64 of
+// 2048 with 8000 words 163 and 202, 192 rows 271 and 212; 64 of 512 with 2000 words, whose
+// launches are what counts, 78 and 64. Rows of w that begin at whole 16 bytes.
+constexpr int64_t kFewRows = 128, kLargeWeight = int64_t{1} << 22;
+bool few(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
+  return !bf16 && rows <= kFewRows && vocab * c >= kLargeWeight && c % 8 == 0;
+}
+int64_t planes_of(int64_t rows, int64_t vocab, int64_t c, bool bf16) { return bf16 ? 1 : few(rows, vocab, c, bf16) ? 3 : 2; }
+
 int64_t take(int64_t& end, int64_t bytes) {
   const int64_t at = end;
   end += up(bytes, 256);
@@ -823,7 +901,7 @@ struct Places {
 };
 Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward) {
   Places p{};
-  const int64_t pitch = up(c, kStep) * 2, planes = bf16 ? 1 : 2;
+  const int64_t pitch = up(c, kStep) * 2, planes = planes_of(rows, vocab, c, bf16);
   p.scalars = take(p.end, sizeof(Scalars));
   p.largest = take(p.end, 3 * kMaxBlocks * 4);
   p.x_plane = rows * pitch;
@@ -834,7 +912,7 @@ Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward
     p.count = take(p.end, 4);
   }
   if (packed(c, bf16) || numbered(rows)) p.x = take(p.end, planes * p.x_plane);
-  if (packed(c, bf16)) p.w = take(p.end, planes * p.w_plane);
+  if (packed(c, bf16) && !few(rows, vocab, c, bf16)) p.w = take(p.end, planes * p.w_plane);
   if (bf16 && backward) p.x_half = take(p.end, p.x_plane);
   return p;
 }
@@ -866,12 +944,20 @@ Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   p.channels = (c - 1) % 256 < 128 ? 128 : 256;
   p.padded_rows = up(rows, kGradTile);
   p.pitch = up(c, 4);
-  const int64_t channel_tiles = ceil_div(c, p.channels), planes = bf16 ? 1 : 2;
+  const int64_t channel_tiles = ceil_div(c, p.channels), planes = planes_of(rows, vocab, c, bf16);
   const int64_t all = up(vocab, kWholeWords);
   const int64_t most = std::max<int64_t>(kWholeWords, kMaxD / (p.padded_rows * 2 * planes) / kWholeWords * kWholeWords);
   p.pieces = ceil_div(all, most);
   p.words = up(ceil_div(all, p.pieces), kWholeWords);
   p.pieces = ceil_div(all, p.words);
+  if (few(rows, vocab, c, bf16)) {
+    const int64_t splits = std::max<int64_t>(kUnits / (channel_tiles * ceil_div(rows, Few::kRows)), 1);
+    p.share = up(ceil_div(p.words, splits), kStep);
+    p.splits = ceil_div(p.words, p.share);
+    p.row_splits = 1;
+    p.row_share = up(rows, kStep);
+    return p;
+  }
   const int64_t weight_tiles = channel_tiles * ceil_div(p.words, kGradTile), hidden_tiles = channel_tiles * p.padded_rows / kGradTile;
   const int64_t parts = bf16 ? 1 : 3;
   int64_t least = INT64_MAX;
@@ -911,7 +997,7 @@ BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64
   b.operands = operands(rows, vocab, c, bf16, true);
   b.end = b.operands.end;
   b.d_plane = p.padded_rows * p.words * 2;
-  b.d = take(b.end, b.d_plane * (bf16 ? 1 : 2));
+  b.d = take(b.end, b.d_plane * planes_of(rows, vocab, c, bf16));
   b.sums = !needs_sums(p, rows) ? 0 : take(b.end, p.splits * rows * p.pitch * 4);
   b.weight_sums = p.row_splits == 1 ? 0 : take(b.end, p.row_splits * vocab * p.pitch * 4);
   b.residuals = take(b.end, 2 * rows * 4);
@@ -921,21 +1007,24 @@ BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64
 // The tile with which the logits are done first: as many workgroups as there are places
 // for them take the tiles in turn, each `first` and `stage` times the steps of a tile, in
 // ns.
-enum { kBig, kMiddle, kSmall };
+enum { kBig, kMiddle, kSmall, kFew, kFewSmall };
 struct Shape {
   int words, rows, places;
   int64_t first, stage;
 };
 constexpr Shape kShapes[] = {{Big::kWords, Big::kRows, kUnits * Big::kEach, 6000, 1200},
                              {Middle::kWords, Middle::kRows, kUnits * Middle::kEach, 4000, 900},
-                             {Small::kWords, Small::kRows, kUnits * Small::kEach, 3000, 700}};
-int shape_of(int64_t rows, int64_t words, int64_t c, bool bf16) {
-  int best = kBig;
+                             {Small::kWords, Small::kRows, kUnits * Small::kEach, 3000, 700},
+                             {Few::kWords, Few::kRows, kUnits * Few::kEach, 2000, 1300},
+                             {FewSmall::kWords, FewSmall::kRows, kUnits * FewSmall::kEach, 2000, 700}};
+int shape_of(int64_t rows, int64_t words, int64_t c, bool bf16, bool split) {
+  int best = 0;
   int64_t least = INT64_MAX;
-  for (int i = kBig; i <= kSmall; ++i) {
+  for (int i = split ? kFew : kBig; i <= (split ? kFewSmall : kSmall); ++i) {
     const Shape& t = kShapes[i];
     const int64_t tiles = ceil_div(words, t.words) * ceil_div(rows, t.rows);
-    const int64_t time = ceil_div(tiles, t.places) * (t.first + t.stage * ceil_div(c, kStep) * (bf16 ? 1 : 3));
+    const int64_t stages = split ? ceil_div(c, kFewStep) : ceil_div(c, kStep) * (bf16 ? 1 : 3);
+    const int64_t time = ceil_div(tiles, t.places) * (t.first + t.stage * stages);
     if (time >= least) continue;
     least = time;
     best = i;
@@ -952,7 +1041,7 @@ ForwardPlaces forward_places(int64_t rows, int64_t vocab, int64_t c, bool bf16) 
   ForwardPlaces f{};
   f.operands = operands(rows, vocab, c, bf16, false);
   f.end = f.operands.end;
-  const int64_t parts = ceil_div(vocab, shape_words(shape_of(rows, vocab, c, bf16))) * rows * 4;
+  const int64_t parts = ceil_div(vocab, shape_words(shape_of(rows, vocab, c, bf16, few(rows, vocab, c, bf16)))) * rows * 4;
   f.part_max = take(f.end, parts);
   f.part_sum = take(f.end, parts);
   f.part_argmax = take(f.end, parts);
@@ -971,7 +1060,8 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
   const int64_t padded = up(c.c, kStep);
   Operands o{};
   o.x = Matrix{static_cast<const char*>(c.hidden), c.c * 2, 0};
-  o.w = Matrix{static_cast<const char*>(c.weight), c.c * 2, 0};
+  o.w = Matrix{static_cast<const char*>(c.weight), c.c * (BF ? 2 : 4), 0};
+  const bool split = few(c.rows, c.vocab, c.c, BF);
   RowsCall r{c.targets, c.ignore_index, static_cast<int>(c.rows), nullptr, nullptr, nullptr};
   if (numbered(c.rows)) {
     o.index = r.index = reinterpret_cast<int*>(c.workspace + p.index);
@@ -983,8 +1073,8 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
     k.job[k.jobs++] = PackJob{from, c.workspace + to, rows, kind, which};
     return Matrix{c.workspace + to, padded * 2, plane};
   };
-  if (packed(c.c, BF) || r.index) o.x = pack(c.hidden, p.x, c.rows, BF ? kCopy : kToHalves, 0, p.x_plane);
-  if (packed(c.c, BF)) o.w = pack(c.weight, p.w, c.vocab, BF ? kCopy : kToHalves, 1, p.w_plane);
+  if (packed(c.c, BF) || r.index) o.x = pack(c.hidden, p.x, c.rows, BF ? kCopy : split ? kToThirds : kToHalves, 0, p.x_plane);
+  if (packed(c.c, BF) && !split) o.w = pack(c.weight, p.w, c.vocab, BF ? kCopy : kToHalves, 1, p.w_plane);
   o.x_half = o.x;
   if (BF && b && b->weight_grad) o.x_half = pack(c.hidden, p.x_half, c.rows, kToHalf, 0, 0);
   if (k.jobs == 0 && !b) return o;
@@ -997,8 +1087,8 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
   k.largest = largest;
   k.scalars = reinterpret_cast<Scalars*>(c.workspace + p.scalars);
   SurveyCall v{};
-  if (!BF || (b && b->weight_grad)) v.from[0] = c.hidden;
-  if (!BF) v.from[1] = c.weight;
+  if ((!BF && !split) || (b && BF && b->weight_grad)) v.from[0] = c.hidden;
+  if (!BF && !split) v.from[1] = c.weight;
   v.n[0] = c.rows;
   v.n[1] = c.vocab;
   v.c = c.c;
@@ -1033,6 +1123,10 @@ void logits(const LogitsCall& l, hipStream_t s) {
 }
 template <bool BF, bool kBackward>
 void logits(const LogitsCall& l, int shape, hipStream_t s) {
+  if constexpr (!BF) {
+    if (shape == kFew) return logits<BF, kBackward, Few>(l, s);
+    if (shape == kFewSmall) return logits<BF, kBackward, FewSmall>(l, s);
+  }
   if (shape == kBig) logits<BF, kBackward, Big>(l, s);
   else if (shape == kMiddle) logits<BF, kBackward, Middle>(l, s);
   else logits<BF, kBackward, Small>(l, s);
@@ -1049,7 +1143,8 @@ void forward(const ForwardCall& c, hipStream_t s) {
   l.count = o.count;
   l.rows = static_cast<int>(c.rows);
   l.vocab = static_cast<int>(c.vocab);
-  l.steps = static_cast<int>(up(c.c, kStep));
+  l.c = static_cast<int>(c.c);
+  l.steps = static_cast<int>(up(c.c, few(c.rows, c.vocab, c.c, BF) ? kFewStep : kStep));
   l.words = static_cast<int>(up(c.vocab, kWholeWords));
   l.scalars = reinterpret_cast<const Scalars*>(c.workspace + f.operands.scalars);
   l.targets = c.targets;
@@ -1057,11 +1152,17 @@ void forward(const ForwardCall& c, hipStream_t s) {
   l.part_sum = reinterpret_cast<float*>(c.workspace + f.part_sum);
   l.part_argmax = reinterpret_cast<int*>(c.workspace + f.part_argmax);
   l.row_target = reinterpret_cast<float*>(c.workspace + f.row_target);
-  const int shape = shape_of(c.rows, c.vocab, c.c, BF);
+  const int shape = shape_of(c.rows, c.vocab, c.c, BF, few(c.rows, c.vocab, c.c, BF));
   logits<BF, false>(l, shape, s);
   const JoinCall j{l.part_max, l.part_sum, l.row_target, l.part_argmax, c.targets, o.place, c.rows, c.vocab, c.ignore_index, shape_words(shape),
                    c.row_loss, c.row_lse, c.row_max, c.row_argmax};
   hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>(ceil_div(c.rows, 16))), dim3(256), 0, s, j);
+}
+
+template <int kChannels>
+void few_gradients(const GradientsCall& g, hipStream_t s) {
+  if (g.weight_blocks) hipLaunchKernelGGL(few_weight_kernel<kChannels>, dim3(static_cast<unsigned>(g.weight_blocks)), dim3(kThreads), 0, s, g);
+  if (g.hidden_blocks) hipLaunchKernelGGL(few_hidden_kernel<kChannels>, dim3(static_cast<unsigned>(g.hidden_blocks)), dim3(64 * Few::kWavesP), 0, s, g);
 }
 
 template <bool BF>
@@ -1078,7 +1179,8 @@ void backward(const BackwardCall& c, hipStream_t s) {
   l.count = o.count;
   l.rows = static_cast<int>(c.rows);
   l.vocab = static_cast<int>(c.vocab);
-  l.steps = static_cast<int>(up(c.c, kStep));
+  l.c = static_cast<int>(c.c);
+  l.steps = static_cast<int>(up(c.c, few(c.rows, c.vocab, c.c, BF) ? kFewStep : kStep));
   l.scalars = scalars;
   l.targets = c.targets;
   l.ignore_index = c.ignore_index;
@@ -1114,13 +1216,20 @@ void backward(const BackwardCall& c, hipStream_t s) {
   for (int64_t first = 0; first < c.vocab; first += p.words) {
     g.first = l.first = static_cast<int>(first);
     g.words = l.words = static_cast<int>(std::min(p.words, up(c.vocab - first, kWholeWords)));
-    logits<BF, true>(l, shape_of(c.rows, l.words, c.c, BF), s);
+    logits<BF, true>(l, shape_of(c.rows, l.words, c.c, BF, few(c.rows, c.vocab, c.c, BF)), s);
     g.begin = first == 0;
     g.weight_tiles = c.weight_grad ? static_cast<int>(channel_tiles * (l.words / kGradTile) * p.row_splits) : 0;
     g.weight_blocks = static_cast<int>(up(g.weight_tiles, kXcds));
-    g.hidden_blocks = c.hidden_grad ? static_cast<int>(up(channel_tiles * (p.padded_rows / kGradTile) * ceil_div(l.words, p.share), kXcds)) : 0;
+    g.hidden_blocks = c.hidden_grad ? static_cast<int>(up(channel_tiles * ceil_div(c.rows, few(c.rows, c.vocab, c.c, BF) ? Few::kRows : kGradTile) * ceil_div(l.words, p.share), kXcds)) : 0;
     g.hidden_first = p.hidden_first;
     const dim3 grid(static_cast<unsigned>(g.weight_blocks + g.hidden_blocks));
+    if constexpr (!BF) {
+      if (few(c.rows, c.vocab, c.c, BF)) {
+        if (p.channels == 128) few_gradients<128>(g, s);
+        else few_gradients<256>(g, s);
+        continue;
+      }
+    }
     if (p.channels == 128) hipLaunchKernelGGL((gradients_kernel<BF, 128>), grid, dim3(kThreads), 0, s, g);
     else hipLaunchKernelGGL((gradients_kernel<BF, 256>), grid, dim3(kThreads), 0, s, g);
   }

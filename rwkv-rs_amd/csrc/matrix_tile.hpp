@@ -28,8 +28,6 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = 64;              // steps of k a stage: whole cache lines of an operand that lies by rows
-constexpr int kStepBytes = kStep * 2;
-constexpr int kPieces = kStepBytes / 16;
 
 template <bool kFp16>   // or bf16
 __device__ __forceinline__ f32x4 multiply(s16x8 p, s16x8 q, f32x4 c) {
@@ -83,14 +81,16 @@ template <bool kSpread>
 __device__ __forceinline__ int row_swizzle(int row) { return ((-(row >> (kSpread ? 3 : 2))) & 3) + 2 * (row & 2); }
 __device__ __forceinline__ int step_swizzle(int k) { return (k & 3) | ((k >> 1) & 4); }
 
-// How a workgroup's lanes bring an operand of kItems to LDS and read it back.
-template <Layout kLayout, int kItems, int kWaves, bool kSpread>
+// How a workgroup's lanes bring an operand of kItems to LDS and read it back: kSize bytes
+// an element, kSteps of them a stage.
+template <Layout kLayout, int kItems, int kWaves, bool kSpread, int kSteps = kStep, int kSize = 2>
 struct Side {
-  static constexpr int kBytes = kItems * kStepBytes;
+  static constexpr int kBytes = kItems * kSteps * kSize;
   static constexpr int kLoads = kBytes / (kWaves * 1024);   // a wave's instructions a stage
   static_assert(kBytes % (kWaves * 1024) == 0);
-  static_assert(kLayout == kRows || kItems >= 128);         // a step's pieces are swapped within sixteen
-  static constexpr int kPerStep = kItems / 8;               // pieces of a step (steps' form)
+  static_assert(kLayout == kRows || kItems * kSize >= 256); // a step's pieces are swapped within sixteen
+  static constexpr int kRowBytes = kSteps * kSize, kPieces = kRowBytes / 16;   // of a row (rows' form)
+  static constexpr int kPerStep = kItems * kSize / 16;      // pieces of a step (steps' form)
   uint32_t at[kLoads];     // byte offset of a lane's piece from the stage's first element
   const char* base;
   int64_t pitch;
@@ -101,12 +101,15 @@ struct Side {
     const int place = (j * kWaves + wave) * 64 + lane;
     return kLayout == kRows ? place / kPieces : place / kPerStep;
   }
+  // where a line's pieces lie in LDS: swapped, so that the lanes of a read touch different banks
+  __device__ __forceinline__ static int swap(int line) {
+    if constexpr (kLayout == kRows) return kPieces == 8 ? row_swizzle<kSpread>(line) : row_swizzle<kSpread>(line) & 3;
+    else return kSize == 2 ? 2 * step_swizzle(line) : 4 * ((line >> 3) & 3);
+  }
   // bytes from the line's first element on
   __device__ __forceinline__ int within(int j, int wave, int lane) const {
-    const int place = (j * kWaves + wave) * 64 + lane, l = line(j, wave, lane);
-    if constexpr (kLayout == kRows) return 16 * ((place % kPieces) ^ row_swizzle<kSpread>(l));
-    const int c = place % kPerStep;
-    return 16 * (c ^ (2 * step_swizzle(l)));
+    const int place = (j * kWaves + wave) * 64 + lane;
+    return 16 * (place % (kLayout == kRows ? kPieces : kPerStep) ^ swap(line(j, wave, lane)));
   }
   __device__ __forceinline__ void init(const Operand& o, int wave, int lane) {
     base = reinterpret_cast<const char*>(uniform(reinterpret_cast<int64_t>(o.base)));
@@ -118,7 +121,7 @@ struct Side {
       if constexpr (kLayout == kRows) {
         at[j] = static_cast<uint32_t>(min(l, o.items - 1) * pitch) + within(j, wave, lane);
       } else {
-        const int last = min(o.items - 1, kItems - 1) / 8 * 16;
+        const int last = min(o.items - 1, kItems - 1) / (16 / kSize) * 16;
         at[j] = static_cast<uint32_t>(l * pitch) + min(within(j, wave, lane), last);
       }
     }
@@ -126,32 +129,52 @@ struct Side {
   // The buffer of the steps k .. k + kStep - 1 of the operand's array at `offset` bytes
   // from the first one, and its load j.
   __device__ __forceinline__ Buffer stage(int64_t offset, int k) const {
-    return buffer(base + offset + (kLayout == kRows ? 2 * k : min(k, steps - 1) * pitch));
+    return buffer(base + offset + (kLayout == kRows ? kSize * k : min(k, steps - 1) * pitch));
   }
   __device__ __forceinline__ void load(int j, char* lds, Buffer from, int k, int wave, int lane) const {
     uint32_t offset = at[j];
-    if constexpr (kLayout == kSteps) {
-      if (k + kStep > steps) {
+    if constexpr (kLayout == Layout::kSteps) {
+      if (k + kSteps > steps) {
         const int last = max(steps - 1 - k, 0);
         offset -= static_cast<uint32_t>(max(line(j, wave, lane) - last, 0)) * static_cast<uint32_t>(pitch);
       }
+    } else if constexpr (kSize == 4) {   // rows of 16-bit elements are whole stages; k < steps
+      if (k + kSteps > steps) offset -= static_cast<uint32_t>(max(within(j, wave, lane) - (steps - 1 - k) / 4 * 16, 0));
     }
     bring(from, offset, 0, lds + (j * kWaves + wave) * 1024);
   }
   // what lane (m, g) of a wave whose items begin at `first` gives to tile i's instruction
   // over half a stage's steps
   __device__ __forceinline__ s16x8 read(const char* lds, int half, int first, int i, int m, int g) const {
+    static_assert(kSize == 2);
     if constexpr (kLayout == kRows) {
       const int row = first + (kSpread ? 32 * (i / 2) + 8 * (m >> 2) + 4 * (i % 2) + (m & 3) : 16 * i + m);
-      return *reinterpret_cast<const s16x8*>(lds + row * kStepBytes + 16 * ((4 * half + g) ^ row_swizzle<kSpread>(row)));
+      return *reinterpret_cast<const s16x8*>(lds + row * kRowBytes + 16 * ((4 * half + g) ^ swap(row)));
     } else {
       typedef __attribute__((address_space(3))) s16x4* Local;
       const int k = 32 * half + 8 * g + (m >> 2);          // and k + 4, whose pieces lie alike
-      const int piece = (first / 8 + 2 * i + ((m & 3) >> 1)) ^ (2 * step_swizzle(k));
+      const int piece = (first / 8 + 2 * i + ((m & 3) >> 1)) ^ swap(k);
       const char* from = lds + k * (kItems * 2) + 16 * piece + 8 * (m & 1);
       const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Local)(from));
       const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Local)(from + 4 * kItems * 2));
       return s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+  }
+  // the same of fp32 elements
+  __device__ __forceinline__ void read(const char* lds, int first, int i, int m, int g, float (&v)[8]) const {
+    static_assert(kSize == 4 && kSteps == 32);
+    if constexpr (kLayout == kRows) {
+      const int row = first + (kSpread ? 32 * (i / 2) + 8 * (m >> 2) + 4 * (i % 2) + (m & 3) : 16 * i + m);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 p = *reinterpret_cast<const f32x4*>(lds + row * kRowBytes + 16 * ((2 * g + h) ^ swap(row)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * h + e] = p[e];
+      }
+    } else {
+      const char* const from = lds + 16 * ((first / 4 + 4 * i + (m >> 2)) ^ swap(8 * g)) + 4 * (m & 3);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const float*>(from + (8 * g + e) * (kItems * kSize));
     }
   }
 };
@@ -159,8 +182,12 @@ struct Side {
 // What the operands are: kBf16; kHalf, both fp16; kHalfQ, P bf16 and Q fp16, which is
 // rounded to bf16 on its way to the products; kHalves, each two fp16 arrays, the second
 // (`plane` bytes behind the first) holding what rounding took from the first: the
-// product is hi hi + hi lo + lo hi.
-enum Kind { kBf16, kHalf, kHalfQ, kHalves };
+// product is hi hi + hi lo + lo hi; kThirds, each three bf16 arrays that add up to an
+// fp32 number: the six products down to 2^-16 of the first.
+enum Kind { kBf16, kHalf, kHalfQ, kHalves, kThirds };
+constexpr int kThirdsParts = 6;
+__device__ __forceinline__ int third_p(int part) { return part == 2 || part == 3 ? 1 : part == 5 ? 2 : 0; }
+__device__ __forceinline__ int third_q(int part) { return part == 1 || part == 3 ? 1 : part == 4 ? 2 : 0; }
 
 // LDS holds three stages of one operand and two of the other (kDeepP: three of P). The
 // loop's barrier lies kTail groups of products before a stage's end, when all of the
@@ -168,7 +195,7 @@ enum Kind { kBf16, kHalf, kHalfQ, kHalves };
 // overwrite this one are issued under the products that are left.
 template <Layout kLayoutP, Layout kLayoutQ, int kP, int kQ, int kWavesP, int kWavesQ, bool kSpread, bool kDeepP, Kind kKind>
 struct Tile {
-  static constexpr int kWaves = kWavesP * kWavesQ, kThreads = 64 * kWaves;
+  static constexpr int kWaves = kWavesP * kWavesQ, kItemsQ = kQ, kAcross = kWavesP;
   static constexpr int kWaveP = kP / kWavesP, kWaveQ = kQ / kWavesQ;
   static constexpr int kTilesP = kWaveP / 16, kTilesQ = kWaveQ / 16;
   static_assert(!kSpread || kWaveP % 32 == 0);
@@ -178,7 +205,7 @@ struct Tile {
   static constexpr int kPlaceQ = kSlotsP * SideP::kBytes;
   static constexpr int kLdsBytes = kPlaceQ + kSlotsQ * SideQ::kBytes;
   static constexpr int kDeepLoads = kDeepP ? SideP::kLoads : SideQ::kLoads;
-  static constexpr int kParts = kKind == kHalves ? 3 : 1;
+  static constexpr int kParts = kKind == kHalves ? 3 : kKind == kThirds ? kThirdsParts : 1;
   static constexpr int kTail = kTilesP / 2, kBody = 2 * kTilesP - kTail;   // groups of kTilesQ products
   static constexpr int kHeldP = 2;
 
@@ -211,8 +238,12 @@ struct Tile {
     SideQ q;
     int64_t plane_p, plane_q;
     int wave, lane;
-    __device__ __forceinline__ Buffer from(const Next<kSlotsP>& n) const { return p.stage(kKind == kHalves && n.part == 2 ? plane_p : 0, n.k); }
-    __device__ __forceinline__ Buffer from(const Next<kSlotsQ>& n, int) const { return q.stage(kKind == kHalves && n.part == 1 ? plane_q : 0, n.k); }
+    __device__ __forceinline__ Buffer from(const Next<kSlotsP>& n) const {
+      return p.stage(kKind == kHalves ? (n.part == 2 ? plane_p : 0) : kKind == kThirds ? third_p(n.part) * plane_p : 0, n.k);
+    }
+    __device__ __forceinline__ Buffer from(const Next<kSlotsQ>& n, int) const {
+      return q.stage(kKind == kHalves ? (n.part == 1 ? plane_q : 0) : kKind == kThirds ? third_q(n.part) * plane_q : 0, n.k);
+    }
     __device__ __forceinline__ s16x8 read_p(const char* lds, int half, int i) const {
       return p.read(lds, half, wave % kWavesP * kWaveP, i, lane & 15, lane >> 4);
     }
@@ -376,6 +407,112 @@ struct Tile {
     for (int i = 0; i < kTail; ++i) products(kTilesP - kTail + i, held.last_p[i], held.last_q);
     // the loads that were brought for no product, and everyone's reads
     arrive<0>();
+  }
+};
+
+// Eight fp32 numbers as three bf16 each that add up to them: cut off, not rounded, so that
+// the largest do not overflow.
+__device__ __forceinline__ void thirds(const float (&x)[8], s16x8 (&part)[3]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float hi = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[e]) & 0xffff0000u), rest = x[e] - hi;
+    const float mid = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, rest) & 0xffff0000u), lo = rest - mid;
+    part[0][e] = static_cast<short>(__builtin_bit_cast(uint32_t, hi) >> 16);
+    part[1][e] = static_cast<short>(__builtin_bit_cast(uint32_t, mid) >> 16);
+    part[2][e] = static_cast<short>(__builtin_bit_cast(uint32_t, lo) >> 16);
+  }
+}
+
+// The same for few q, where P is large, fp32, and read once: it is made three bf16 arrays
+// on its way from LDS to the products, not in memory before. Q is three bf16 arrays in
+// memory, by rows, `plane` bytes apart. Each wave has all of the tile's q.
+constexpr int kFewStep = 32;
+template <Layout kLayoutP, int kP, int kQ, int kWaves, bool kSpread, int kSlots = 3>
+struct FewTile {
+  static constexpr int kSteps = kFewStep, kItemsQ = kQ, kAcross = kWaves;
+  static constexpr int kWaveP = kP / kWaves, kWaveQ = kQ, kTilesP = kWaveP / 16, kTilesQ = kQ / 16;
+  static_assert(!kSpread || kWaveP % 32 == 0);
+  using SideP = Side<kLayoutP, kP, kWaves, kSpread, kSteps, 4>;
+  using SideQ = Side<kRows, kQ, kWaves, false, kSteps, 2>;
+  static constexpr int kSlotBytes = SideP::kBytes + 3 * SideQ::kBytes, kLdsBytes = kSlots * kSlotBytes;
+  static constexpr int kLoads = SideP::kLoads + 3 * SideQ::kLoads;
+  static constexpr int kFree = (kSlots - 1) * kSlotBytes;
+
+  f32x4 acc[kTilesP][kTilesQ];
+
+  struct Work {
+    SideP p;
+    SideQ q;
+    int64_t plane_q;
+    int k0, k1, wave, lane;
+  };
+  __device__ __forceinline__ static void load(const Work& w, char* to, int stage) {
+    const int k = min(w.k0 + stage * kSteps, w.k1 - kSteps);   // past the last stage that one again
+    const Buffer from = w.p.stage(0, k);
+#pragma unroll
+    for (int n = 0; n < SideP::kLoads; ++n) w.p.load(n, to, from, k, w.wave, w.lane);
+#pragma unroll
+    for (int plane = 0; plane < 3; ++plane) {
+      const Buffer of = w.q.stage(plane * w.plane_q, k);
+#pragma unroll
+      for (int n = 0; n < SideQ::kLoads; ++n) w.q.load(n, to + SideP::kBytes + plane * SideQ::kBytes, of, k, w.wave, w.lane);
+    }
+  }
+  __device__ __forceinline__ static void begin(Work& w, char* lds, const Operand& p, const Operand& q, int64_t, int64_t plane_q,
+                                               int k0, int k1) {
+    w.lane = threadIdx.x & 63;
+    w.wave = uniform(static_cast<int>(threadIdx.x >> 6));
+    w.p.init(p, w.wave, w.lane);
+    w.q.init(q, w.wave, w.lane);
+    w.plane_q = plane_q;
+    w.k0 = k0;
+    w.k1 = k1;
+#pragma unroll
+    for (int s = 0; s < kSlots - 1; ++s) load(w, lds + s * kSlotBytes, s);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kTilesP; ++i)
+#pragma unroll
+      for (int j = 0; j < kTilesQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ void step(char* __restrict to, const char* __restrict from, const Work& w, int stage) {
+    const int m = w.lane & 15, g = w.lane >> 4;
+    load(w, to, stage);
+    s16x8 q[kTilesQ][3];
+#pragma unroll
+    for (int j = 0; j < kTilesQ; ++j)
+#pragma unroll
+      for (int plane = 0; plane < 3; ++plane) q[j][plane] = w.q.read(from + SideP::kBytes + plane * SideQ::kBytes, 0, 0, j, m, g);
+#pragma unroll
+    for (int i = 0; i < kTilesP; ++i) {
+      float v[8];
+      w.p.read(from, w.wave * kWaveP, i, m, g, v);
+      s16x8 p[3];
+      thirds(v, p);
+#pragma unroll
+      for (int part = 0; part < kThirdsParts; ++part)
+#pragma unroll
+        for (int j = 0; j < kTilesQ; ++j) acc[i][j] = multiply<false>(p[third_p(part)], q[j][third_q(part)], acc[i][j]);
+    }
+  }
+  __device__ __forceinline__ void run(Work& w, char* lds) {
+    clear();
+    const int stages = (w.k1 - w.k0) / kSteps;
+    int now = 0, free = kSlots - 1;
+    for (int s = 0; s < stages; ++s) {
+      // this wave's loads of stage s are here, and behind the barrier everyone's; and
+      // everyone has read the stage that is overwritten next
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kSlots - 2) * kLoads) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      step(lds + free * kSlotBytes, lds + now * kSlotBytes, w, s + kSlots - 1);
+      now = now == kSlots - 1 ? 0 : now + 1;
+      free = free == kSlots - 1 ? 0 : free + 1;
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   }
 };
 
