@@ -27,14 +27,17 @@
  * most 512 MiB of D in memory (or a tile of 256 words). D is held in fp16, over the
  * call's largest |g_r| or |l2wrap_scale max_r| and with what the power of two 2^13
  * makes of it: 11 bits of each element, but never finer than 2^-38 of that largest
- * factor; for fp32 operands in two such numbers, 22 bits. The hidden gradient's
+ * factor; for fp32 operands in two such numbers, 22 bits (or whole, in three bf16
+ * ones). The hidden gradient's
  * products round it to bf16 for bf16 operands, but for the target and the argmax,
  * whose error is put back; the weight gradient's are fp16, of hidden states scaled by
  * a power of two (exact but below 2^-27 of the largest magnitude).
  *
  * fp32 operands are multiplied as two fp16 numbers each, after a power of two that
  * brings the operand's largest magnitude to 2^13 .. 2^14: 22 bits of each element, but
- * never finer than 2^-38 of that largest magnitude, three products, fp32 sums.
+ * never finer than 2^-38 of that largest magnitude, three products, fp32 sums. Where
+ * there are few rows and many weights, as three bf16 numbers each that hold an element
+ * whole, of nine products the six of 2^-15 and more.
  *
  * Operands are aligned to their elements, and where c is a multiple of 8, hidden,
  * weight and their gradients to 16 bytes. What a call writes may not overlap

@@ -938,7 +938,7 @@ struct Plan {
 // when `more` tiles of `more_each` are done behind `tiles` longer ones of `each`
 int64_t finish(int64_t tiles, int64_t each, int64_t more, int64_t more_each) {
   const int64_t whole = tiles / kUnits * each, late = tiles % kUnits, at = whole + (late ? each : 0);
-  for (int64_t k = (at - whole) / more_each;; ++k) {
+  for (int64_t k = std::max((at - whole) / more_each, more / kUnits);; ++k) {   // before, too few are done
     const int64_t t = std::max(at, whole + k * more_each);
     if ((kUnits - late) * ((t - whole) / more_each) + late * ((t - at) / more_each) >= more) return t;
   }

@@ -119,6 +119,7 @@ def _philox(c0, c1, c2, c3, seed):
 def keep_mask(shape, p: float, rng: torch.Tensor, site: int = 0) -> torch.Tensor:
     """The elements that ``dropout`` of a tensor of this shape keeps, as a bool tensor
     on ``rng``'s device, in plain torch."""
+    _check(rng, p, rng, site)
     n = torch.Size(shape).numel()
     q = torch.arange(-(-n // 8), device=rng.device)
     step = (rng[1] & LOW32).expand_as(q)

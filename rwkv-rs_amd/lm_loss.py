@@ -164,4 +164,5 @@ def linear_cross_entropy_l2wrap(hidden: torch.Tensor, weight: torch.Tensor, targ
     mean over the rows that are not ignored (0 when all are), l2wrap counting every
     row as a token."""
     rows = linear_cross_entropy_l2wrap_rows(hidden, weight, targets, hidden.shape[0], ignore_index)
-    return rows.sum() / (targets != ignore_index).sum().clamp(min=1)
+    # in 64 bits: a narrow type would be compared with ignore_index cut off to it
+    return rows.sum() / (targets.to(torch.int64) != ignore_index).sum().clamp(min=1)

@@ -576,12 +576,15 @@ class AutoRegressiveModel(nn.Module):
     ``dropout``: in training mode each mixer's output is dropped with this
     probability where it joins the residual stream (``dropout.dropout_add``). The
     masks follow from ``dropout_rng``, an int64 buffer [seed, step] that is no part of the
-    state dict: each forward that draws takes the step it finds and counts it up.
+    state dict: each forward that draws takes the step it finds and counts it up. Ranks
+    that train on data of their own want seeds of their own, and a wrapper that does not
+    broadcast buffers.
 
     ``loss``: "logits" forms them for the loss; "pieces" does not keep them
     (``lm_loss.linear_cross_entropy_l2wrap``), needs the "hip" neighbour ops, and
     leaves out targets of ``lm_loss.IGNORE_INDEX``. An unembedding that is no plain
-    linear layer any more (4-bit weights) has its logits formed all the same."""
+    linear layer without a bias any more (4-bit weights) has its logits formed all the
+    same; that of one is not called, so a hook on it does not run."""
 
     def __init__(self, vocab_size: int, num_cells: int, embedded_dim: int, num_heads: int,
                  head_size: int = 64, wkv7_dtype: torch.dtype = torch.bfloat16,
@@ -733,7 +736,7 @@ class AutoRegressiveModel(nn.Module):
         x, _, _, _ = self.cells(x, batch_ids, kernel, dropout_rng=self._draw())
         n = B * T
         x = self.layer_norm_for_unembed(x)
-        if self.loss == "pieces" and type(self.unembed) is nn.Linear:
+        if self.loss == "pieces" and type(self.unembed) is nn.Linear and self.unembed.bias is None:
             weight = self.unembed.weight
             dtype = _matmul_dtype(weight)
             hidden = x.reshape(n, x.shape[-1]).to(dtype)

@@ -438,3 +438,18 @@ def test_refusals():
         for args in ((dual, w), (x.detach(), fw.make_dual(w, torch.ones_like(w)))):
             with pytest.raises(NotImplementedError):
                 f(*args, t, 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32])
+def test_targets_of_narrow_types(dtype):
+    """The mean counts rows by the targets' own values: 156 in eight bits without a sign
+    is not -100."""
+    announce("linear loss, narrow targets", dtype)
+    x, w, t = make(40, 120 if dtype == torch.int8 else 200, 64, torch.float32, seed=51)
+    if dtype == torch.uint8:
+        t[::2] = 156
+    else:
+        t[::3] = -100
+    assert torch.equal(ll.linear_cross_entropy_l2wrap(x, w, t.to(dtype)), ll.linear_cross_entropy_l2wrap(x, w, t))
+    rows = ll.linear_cross_entropy_l2wrap_rows(x, w, t.to(dtype), 40)
+    assert torch.equal(ll.linear_cross_entropy_l2wrap(x, w, t.to(dtype)), rows.sum() / (t != -100).sum())

@@ -155,3 +155,20 @@ def test_quantized_model_forms_its_logits():
         with torch.no_grad(), torch.autocast(DEV, dtype=torch.bfloat16):
             got.append(model(inputs, targets, wk.KernelPretrain))
     assert torch.equal(*got)
+
+
+def test_unembedding_with_a_bias_forms_its_logits():
+    announce("unembedding with a bias, with the loss in pieces")
+    wk = _wkv7_mod()
+    inputs, targets = (t.to(DEV) for t in tokens(2, 32, 160))
+    got = []
+    for loss in ("logits", "pieces"):
+        model = build(vocab=160, loss=loss)
+        plain = model.unembed
+        model.unembed = torch.nn.Linear(plain.in_features, 160, device=DEV)
+        with torch.no_grad():
+            model.unembed.weight.copy_(plain.weight)
+            model.unembed.bias.copy_(torch.linspace(-2, 2, 160))
+            with torch.autocast(DEV, dtype=torch.bfloat16):
+                got.append(model(inputs, targets, wk.KernelPretrain))
+    assert torch.equal(*got)

@@ -178,3 +178,24 @@ def test_model_drops_in_training_alone():
     assert model.dropout_rng.tolist() == [5, 11]
     plain.train()
     assert float(plain(inputs, targets, TorchKernel)) == float(model(inputs, targets, TorchKernel))
+
+
+def test_keep_mask_refuses():
+    d = load_pkg().dropout
+    rng = torch.tensor([1, 2])
+    for bad in (lambda: d.keep_mask((3,), 1.5, rng), lambda: d.keep_mask((3,), float("nan"), rng),
+                lambda: d.keep_mask((3,), 0.5, rng, -1), lambda: d.keep_mask((3,), 0.5, rng, 1 << 32),
+                lambda: d.keep_mask((3,), 0.5, torch.tensor([1, 2, 3])), lambda: d.keep_mask((3,), 0.5, rng.int())):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_workspaces_of_the_largest_sizes_are_planned_at_once(native):
+    """Planned anew for each call: a size of many tiles takes the host no longer."""
+    import time
+    size = native.lib().rwkv_linear_loss_backward_workspace_bytes
+    for rows, vocab, c in ((1 << 22, 1 << 22, 2048), (1 << 22, 1, 2048), (1, 1 << 22, 2048), (1 << 22, 256, 2048), (1 << 17, 1 << 17, 1 << 16)):
+        for dtype in (0, 1):
+            start = time.perf_counter()
+            assert size(rows, vocab, c, dtype) > 0
+            assert time.perf_counter() - start < 0.05
