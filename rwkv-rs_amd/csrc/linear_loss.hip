@@ -344,6 +344,9 @@ __device__ __forceinline__ float as_read(float v) {
   return static_cast<float>(static_cast<__bf16>(static_cast<float>(static_cast<_Float16>(v))));
 }
 
+// What a sum of exponentials over the maximum `own` counts among ones over `most`.
+__device__ __forceinline__ float share_of(float own, float most) { return own == most ? 1.f : __expf(own - most); }
+
 // A run of words whose rows of w stay in an XCD's L2 while the rows of x pass by.
 constexpr int kWordTiles = 8;
 template <bool BF, bool kBackward, typename Shape>
@@ -416,6 +419,7 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, std::max(Shap
           for (int e = 0; e < 4; ++e) most = fmaxf(most, t.acc[i][j][e]);
         most = fmaxf(most, __shfl_xor(most, 16));
         most = fmaxf(most, __shfl_xor(most, 32));
+        const float base = most == -INFINITY ? 0.f : most;   // words of minus infinity alone: nothing, but a NaN among them
         float sum = 0.f;
         int first = INT_MAX;
 #pragma unroll
@@ -423,7 +427,7 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, std::max(Shap
 #pragma unroll
           for (int e = 3; e >= 0; --e) {
             const float z = t.acc[i][j][e];
-            sum += __expf(z - most);
+            sum += __expf(z - base);
             first = z == most ? 32 * (i / 2) + 4 * (i % 2) + e : first;
           }
         if (first != INT_MAX) first += wp * T::kWaveP + 8 * g;
@@ -459,8 +463,7 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, std::max(Shap
 #pragma unroll
         for (int w = kWavesP - 1; w >= 0; --w) {
           const float own = maxima[w * kRowsTile + q];
-          // a wave without a word (or all of minus infinity) has a NaN for a sum
-          sum += own == -INFINITY ? 0.f : sums[w * kRowsTile + q] * __expf(own - most);
+          sum += sums[w * kRowsTile + q] * share_of(own, most);
           if (own == most) f = firsts[w * kRowsTile + q];
         }
         const int64_t to = int64_t{v / kWords} * c.rows + r + q;
@@ -560,8 +563,7 @@ struct Run {
 __device__ __forceinline__ Run combine(const Run& a, const Run& b) {
   Run r;
   r.most = fmaxf(a.most, b.most);
-  r.sum = (a.most == -INFINITY && a.sum == 0.f ? 0.f : a.sum * __expf(a.most - r.most)) +
-          (b.most == -INFINITY && b.sum == 0.f ? 0.f : b.sum * __expf(b.most - r.most));
+  r.sum = a.sum * share_of(a.most, r.most) + b.sum * share_of(b.most, r.most);
   r.first = a.most > b.most ? a.first : b.most > a.most ? b.first : min(a.first, b.first);
   return r;
 }
@@ -590,11 +592,12 @@ __global__ __launch_bounds__(kJoinRows * kJoinShares) void join_kernel(const Joi
   c.row_lse[row] = lse;
   c.row_max[row] = run.most;
   c.row_argmax[row] = run.first;
-  // a logit is at most the sum's logarithm: no rounding makes a loss negative
-  c.row_loss[row] = target == c.ignore_index ? 0.f
-                    : target < 0 || target >= c.vocab ? NAN
-                    : lse != lse ? NAN
-                                 : fmaxf(lse - c.row_target[part_row], 0.f);
+  float loss = target == c.ignore_index ? 0.f : NAN;
+  if (target != c.ignore_index && target >= 0 && target < c.vocab && lse == lse) {
+    loss = lse - c.row_target[part_row];
+    loss = loss < 0.f ? 0.f : loss;   // a logit is at most the sum's logarithm: no rounding makes a loss negative
+  }
+  c.row_loss[row] = loss;
 }
 
 // ---------------------------------------------------------------------- gradients

@@ -453,3 +453,24 @@ def test_targets_of_narrow_types(dtype):
     assert torch.equal(ll.linear_cross_entropy_l2wrap(x, w, t.to(dtype)), ll.linear_cross_entropy_l2wrap(x, w, t))
     rows = ll.linear_cross_entropy_l2wrap_rows(x, w, t.to(dtype), 40)
     assert torch.equal(ll.linear_cross_entropy_l2wrap(x, w, t.to(dtype)), rows.sum() / (t != -100).sum())
+
+
+@pytest.mark.parametrize("vocab", [1, 40, 700])
+def test_logits_of_minus_infinity(vocab):
+    """Words of bf16 whose logit is minus infinity: probability 0; where there is no other
+    word no loss, and a NaN among them is not lost."""
+    announce("linear loss, minus infinity", vocab)
+    x, w, t = make(9, vocab, 64, torch.bfloat16, seed=53)
+    x[:, 0] = 1.0
+    inf = w.clone()
+    inf[:, 0] = -math.inf
+    assert ll.linear_cross_entropy_l2wrap_rows(x, inf, t, 9).isnan().all()
+    last = torch.full_like(t, vocab - 1)
+    one = inf.clone()
+    one[vocab - 1] = w[vocab - 1]
+    loss = ll.linear_cross_entropy_l2wrap_rows(x, one, last, 9)
+    assert (loss.abs() <= 2.0 ** -20 + 64 * U * (x.double() @ w[vocab - 1].double()).abs().max()).all()
+    if vocab > 1:
+        assert (ll.linear_cross_entropy_l2wrap_rows(x, one, last - 1, 9) == math.inf).all()
+        one[0, 3] = math.nan                      # a NaN in a tile of minus infinities
+        assert ll.linear_cross_entropy_l2wrap_rows(x, one, last, 9).isnan().all()
