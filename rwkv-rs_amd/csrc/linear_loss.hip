@@ -380,6 +380,8 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, std::max(Shap
   for (; at < last; at += locals) {
     t.run(work, lds);
     const int v = v0, r = r0;
+    // a wave whose rows are all behind the last one, and behind the steps of D's other product
+    const bool idle = T::kWaveQ % kStep == 0 && r + uniform(static_cast<int>(threadIdx.x >> 6)) / kWavesP * T::kWaveQ >= rows;
     if (at + locals < last) begin(at + locals);   // its loads run under what follows
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
@@ -408,47 +410,49 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, std::max(Shap
       float* const maxima = reinterpret_cast<float*>(lds + T::kFree);      // [kWavesP][kRowsTile] each
       float* const sums = maxima + kWavesP * kRowsTile;
       int* const firsts = reinterpret_cast<int*>(sums + kWavesP * kRowsTile);
+      if (!idle) {
 #pragma unroll
-      for (int j = 0; j < T::kTilesQ; ++j) {
-        const int in_tile = wq * T::kWaveQ + 16 * j + m;
-        const int row = r + in_tile;
-        float most = t.acc[0][j][0];
+        for (int j = 0; j < T::kTilesQ; ++j) {
+          const int in_tile = wq * T::kWaveQ + 16 * j + m;
+          const int row = r + in_tile;
+          float most = t.acc[0][j][0];
 #pragma unroll
-        for (int i = 0; i < T::kTilesP; ++i)
+          for (int i = 0; i < T::kTilesP; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) most = fmaxf(most, t.acc[i][j][e]);
-        most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
-        const float base = most == -INFINITY ? 0.f : most;   // words of minus infinity alone: nothing, but a NaN among them
-        float sum = 0.f;
-        int first = INT_MAX;
+            for (int e = 0; e < 4; ++e) most = fmaxf(most, t.acc[i][j][e]);
+          most = fmaxf(most, __shfl_xor(most, 16));
+          most = fmaxf(most, __shfl_xor(most, 32));
+          const float base = most == -INFINITY ? 0.f : most;   // words of minus infinity alone: nothing, but a NaN among them
+          float sum = 0.f;
+          int first = INT_MAX;
 #pragma unroll
-        for (int i = T::kTilesP - 1; i >= 0; --i)
+          for (int i = T::kTilesP - 1; i >= 0; --i)
 #pragma unroll
-          for (int e = 3; e >= 0; --e) {
-            const float z = t.acc[i][j][e];
-            sum += __expf(z - base);
-            first = z == most ? 32 * (i / 2) + 4 * (i % 2) + e : first;
+            for (int e = 3; e >= 0; --e) {
+              const float z = t.acc[i][j][e];
+              sum += __expf(z - base);
+              first = z == most ? 32 * (i / 2) + 4 * (i % 2) + e : first;
+            }
+          if (first != INT_MAX) first += wp * T::kWaveP + 8 * g;
+          sum += __shfl_xor(sum, 16);
+          sum += __shfl_xor(sum, 32);
+          first = min(first, __shfl_xor(first, 16));
+          first = min(first, __shfl_xor(first, 32));
+          if (g == 0) {
+            maxima[wp * kRowsTile + in_tile] = most;
+            sums[wp * kRowsTile + in_tile] = sum;
+            firsts[wp * kRowsTile + in_tile] = first;
           }
-        if (first != INT_MAX) first += wp * T::kWaveP + 8 * g;
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        first = min(first, __shfl_xor(first, 16));
-        first = min(first, __shfl_xor(first, 32));
-        if (g == 0) {
-          maxima[wp * kRowsTile + in_tile] = most;
-          sums[wp * kRowsTile + in_tile] = sum;
-          firsts[wp * kRowsTile + in_tile] = first;
-        }
-        if (row < rows) {
-          const int64_t target = c.targets[c.index ? c.index[row] : row];
-          const int own = target >= 0 && target < c.vocab ? static_cast<int>(target) - word0 : -1;
-          if (own >= 0 && own < T::kWaveP && (own & 31) < 8) {
+          if (row < rows) {
+            const int64_t target = c.targets[c.index ? c.index[row] : row];
+            const int own = target >= 0 && target < c.vocab ? static_cast<int>(target) - word0 : -1;
+            if (own >= 0 && own < T::kWaveP && (own & 31) < 8) {
 #pragma unroll
-            for (int i = 0; i < T::kTilesP; ++i)
+              for (int i = 0; i < T::kTilesP; ++i)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (own == 32 * (i / 2) + 4 * (i % 2) + e) c.row_target[row] = t.acc[i][j][e];
+                for (int e = 0; e < 4; ++e)
+                  if (own == 32 * (i / 2) + 4 * (i % 2) + e) c.row_target[row] = t.acc[i][j][e];
+            }
           }
         }
       }
@@ -471,7 +475,7 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, std::max(Shap
         c.part_sum[to] = sum;
         c.part_argmax[to] = f == INT_MAX ? INT_MAX : v + f;
       }
-    } else {
+    } else if (!idle) {
       const float reference = c.scalars->reference;
       struct Row {
         float lse, h, wrap;

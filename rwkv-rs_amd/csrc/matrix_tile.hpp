@@ -348,6 +348,7 @@ struct Tile {
   struct Work {
     Place a;
     int k0, k1;
+    bool busy;               // the wave has items of Q; one that has none leaves its share of a SIMD to another
     Next<kSlotsP> next_p;
     Next<kSlotsQ> next_q;
   };
@@ -361,6 +362,7 @@ struct Tile {
     w.a.plane_q = plane_q;
     w.k0 = k0;
     w.k1 = k1;
+    w.busy = w.a.wave / kWavesP * kWaveQ < uniform(q.items);
     w.next_p = {k0, 0, 0};
     w.next_q = {k0, 0, 0};
     auto all_p = [&] {
@@ -385,24 +387,47 @@ struct Tile {
 #pragma unroll
       for (int j = 0; j < kTilesQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // The workgroup may use `lds` again once all of its waves have come back.
+  // The workgroup may use `lds` again once all of its waves have come back. A wave that is
+  // not busy has no sums.
   __device__ __forceinline__ void run(Work& w, char* lds) {
-    clear();
     const int stages = (w.k1 - w.k0) / kStep * kParts;
     int slot_p = 0, slot_q = 0;
     Held held;
-    auto one = [&](auto first) {
-      arrive<kDeepLoads>();
-      step<decltype(first)::value>(lds + w.next_p.slot * SideP::kBytes, lds + kPlaceQ + w.next_q.slot * SideQ::kBytes,
-                                   lds + slot_p * SideP::kBytes, lds + kPlaceQ + slot_q * SideQ::kBytes, held, w.a, w.next_p,
-                                   w.next_q);
+    auto next = [&] {
       w.next_p.advance(w.k0, w.k1);
       w.next_q.advance(w.k0, w.k1);
       slot_p = slot_p == kSlotsP - 1 ? 0 : slot_p + 1;
       slot_q = slot_q == kSlotsQ - 1 ? 0 : slot_q + 1;
     };
-    one(std::true_type());
-    for (int s = 1; s < stages; ++s) one(std::false_type());
+    auto one = [&](auto first) {
+      arrive<kDeepLoads>();
+      step<decltype(first)::value>(lds + w.next_p.slot * SideP::kBytes, lds + kPlaceQ + w.next_q.slot * SideQ::kBytes,
+                                   lds + slot_p * SideP::kBytes, lds + kPlaceQ + slot_q * SideQ::kBytes, held, w.a, w.next_p,
+                                   w.next_q);
+      next();
+    };
+    if (w.busy) {
+      clear();
+      one(std::true_type());
+      for (int s = 1; s < stages; ++s) one(std::false_type());
+    } else {
+      for (int s = 0; s < stages; ++s) {   // the same loads in the same order, and the same barriers
+        arrive<kDeepLoads>();
+        const Buffer from_p = w.a.from(w.next_p), from_q = w.a.from(w.next_q, 0);
+        auto all_p = [&] {
+#pragma unroll
+          for (int n = 0; n < SideP::kLoads; ++n) bring_p(n, lds, w.a, from_p, w.next_p);
+        };
+        auto all_q = [&] {
+#pragma unroll
+          for (int n = 0; n < SideQ::kLoads; ++n) bring_q(n, lds, w.a, from_q, w.next_q);
+        };
+        if constexpr (kDeepP) all_q(), all_p();
+        else all_p(), all_q();
+        next();
+      }
+    }
+    // by idle waves too, of nothing: in one block with what follows, which runs under them
 #pragma unroll
     for (int i = 0; i < kTail; ++i) products(kTilesP - kTail + i, held.last_p[i], held.last_q);
     // the loads that were brought for no product, and everyone's reads
