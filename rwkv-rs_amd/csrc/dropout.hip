@@ -4,6 +4,10 @@
 // A thread draws one Philox4x32-10 block, eight 16-bit numbers, for eight consecutive
 // elements: sixteen bits decide as well as 32 do (p is a multiple of 2^-16, and what
 // is kept is scaled by the probability in use), for half the multiplications.
+//
+// Memory bounds it: 16384 x 4096 bf16 with a residual 73 us, 5.5 TB/s (part of it from the
+// last level's cache; a copy from memory reaches 4.96); without one 48, 5.6; 8192 x 768
+// bf16 onto an fp32 residual 12 us, 5.2. Small calls are a launch (127 x 768: 2.4 us).
 #include <algorithm>
 
 #include "dropout_launch.hpp"

@@ -2,15 +2,22 @@
 // its unembedding w [vocab, c], without the logits z = x w^T (include/
 // rwkv_linear_loss.h). Three products, each by way of matrix_tile.hpp:
 //
-//   logits  z's tiles of 256 words by 128 rows; the forward reduces a tile to each
-//           row's maximum, sum of exponentials and first index of the maximum
-//           (join_kernel joins the tiles), the backward makes it D;
+//   logits  tiles of z; the forward reduces a tile to each row's maximum, sum of
+//           exponentials and first index of the maximum (join_kernel joins the tiles),
+//           the backward makes it D;
 //   dw      = D^T x, of a piece of the vocabulary;
 //   dx      = D w, summed over the pieces in fp32, the words of a piece shared
 //           among `splits` workgroups that each keep a sum of their own.
 //
 // The backward forms z a second time instead of keeping it: 8 rows vocab c products
-// and sums in all, where 6 would do with the logits in memory.
+// and sums in all, where 6 would do with the logits in memory. The matrix cores, and the
+// power that they take, bound all three for many rows. For 7168 learned rows of 8192, c =
+// 768, 65536 words in bf16 (us, PFLOP/s; torch's own products of 8192 rows in brackets):
+// logits 623 to 690, 1.05 to 1.16 (812, 1.02); D 762 to 800, 0.9 (as the logits, and 1
+// GiB written); dw and dx together 1280 to 1380, 1.05 to 1.13 (858 and 848, 0.97).
+// A product of 8192 cubed reaches 1.49 here, one of 16384 cubed 1.65.
+// For few rows it is memory: 64 rows of the same, 26 us for the loss, of which 20 are
+// w's bytes at a copy's rate.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -27,8 +34,11 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
-// A tile of logits: words by rows, on waves by waves. Two smaller ones, of which a
-// compute unit has two and four at a time, for few rows or words.
+// A tile of logits: words by rows, on waves by waves. 256 by 256 reads each operand's
+// element once for 256 products, which the matrix cores need to be fed from L2: tiles of
+// 128 by 128 took a third longer for 8192 rows. Two smaller ones, of which a compute unit
+// has two and four at a time, for few rows or words, where large ones leave units idle:
+// 64 rows of 768 with 65536 words 26 us on the small one, 45 on the large one.
 struct Big {
   static constexpr int kWords = 256, kRows = 256, kWavesP = 2, kWavesQ = 4, kEach = 1;
 };
@@ -38,7 +48,10 @@ struct Middle {
 struct Small {
   static constexpr int kWords = 64, kRows = 64, kWavesP = 2, kWavesQ = 2, kEach = 4;
 };
-// Of fp32 operands where there are few rows: w is split on its way to the products.
+// Of fp32 operands where there are few rows: w is split on its way to the products. 256
+// words a workgroup keep 64 KiB of w on their way to each compute unit; the small one is
+// for few words, of which the large one makes too few workgroups (8 rows of 2048 with 8000
+// words: 57 us for 92).
 struct Few {
   static constexpr int kWords = 256, kRows = 64, kWavesP = 4, kWavesQ = 1, kEach = 1, kSlots = 3;
 };
@@ -347,7 +360,14 @@ __device__ __forceinline__ float as_read(float v) {
 // What a sum of exponentials over the maximum `own` counts among ones over `most`.
 __device__ __forceinline__ float share_of(float own, float most) { return own == most ? 1.f : __expf(own - most); }
 
-// A run of words whose rows of w stay in an XCD's L2 while the rows of x pass by.
+// A run of words whose rows of w stay in an XCD's L2 while the rows of x pass by: eight
+// tiles of 256 words of c = 768 are 3 MiB of its 4.
+//
+// Persistent: as many workgroups as fit take the tiles in turn, and ask for a tile's first
+// operands before they are done with the one before, so that only the first tile's loads
+// are waited for. What follows the products bounds a tile of few channels beside them: of
+// 256 by 256 logits, c = 768, 14 of 23 us are products, the rest the maximum, the
+// exponentials and the first index (ten instructions' time an element).
 constexpr int kWordTiles = 8;
 template <bool BF, bool kBackward, typename Shape>
 __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, std::max(Shape::kWavesP* Shape::kWavesQ* Shape::kEach / 4, 1)) void logits_kernel(
@@ -647,24 +667,40 @@ template <bool BF>
 __device__ __forceinline__ Factor hidden_factor(const Scalars* s) {
   return Factor{s->reference, -(kHalfExponent + (BF ? 0 : s->exponent[1]))};
 }
+// What goes back to a row: r[k] times w's row at w[k]. Asked for before its channels are,
+// so that all rows' loads are on their way at once, and read whether it is wanted or not.
+struct PutBack {
+  float r[2];
+  const __bf16* w[2];
+};
 template <bool BF>
-__device__ __forceinline__ void finish_hidden(const HiddenCall& c, Factor f, int64_t row, int64_t part_row, int64_t channel, f32x4 v) {
+__device__ __forceinline__ PutBack put_back(const HiddenCall& c, int64_t row, int64_t part_row) {
+  PutBack b{};
+  if constexpr (BF) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) b.r[k] = c.residuals[k * c.rows + part_row];
+    const int64_t target = c.targets[row], top = c.row_argmax[row];
+    // no residual: there may be no such word
+    b.w[0] = c.weight + (b.r[0] != 0.f ? target : 0) * c.c;
+    b.w[1] = c.weight + (b.r[1] != 0.f ? top : 0) * c.c;
+  }
+  return b;
+}
+template <bool BF>
+__device__ __forceinline__ void finish_hidden(const HiddenCall& c, Factor f, int64_t row, const PutBack& b, int64_t channel, f32x4 v) {
   const bool whole = c.c % 8 == 0;
   if constexpr (BF) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const float r = c.residuals[k * c.rows + part_row];
-      if (r == 0.f) continue;                      // and so where there is no such word
-      const __bf16* const w = c.weight + (k ? c.row_argmax[row] : c.targets[row]) * c.c + channel;
+      bf16x4 w;
       if (whole) {
-        const bf16x4 b = *reinterpret_cast<const bf16x4*>(w);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += r * static_cast<float>(b[e]);
+        w = *reinterpret_cast<const bf16x4*>(b.w[k] + channel);
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (channel + e < c.c) v[e] += r * static_cast<float>(w[e]);
+        for (int e = 0; e < 4; ++e) w[e] = b.w[k][min(channel + e, c.c - 1)];
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += b.r[k] != 0.f ? b.r[k] * static_cast<float>(w[e]) : 0.f;
     }
   }
 #pragma unroll
@@ -693,6 +729,10 @@ struct GradientsCall {
   HiddenCall hidden;
 };
 
+// Tiles of 256 by 256 (or 128 channels) as the logits' are. Workgroups of both gradients in
+// one launch: either alone would leave units idle in its last round, dx's of 768 channels
+// and 8192 rows has 84 tiles a share. In turn they took 3% longer.
+//
 // The tiles of a gradient in an order in which those that an XCD has at a time share
 // both operands: runs of up to five tiles of channels, in each the other tiles.
 constexpr int kMaxRun = 5;
@@ -795,18 +835,24 @@ __device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, i
 #pragma unroll
       for (int i = 0; i < T::kTilesP; ++i) {
         const int channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
-        if (channel < c.pitch) store(row, channel, t.acc[i][j]);
+        if (channel < c.pitch) store(j, row, channel, t.acc[i][j]);
       }
     }
   };
   if (c.sums) {
     float* const sums = c.sums + int64_t{split} * c.rows * c.pitch;
-    all_of([&](int row, int channel, f32x4 v) {
+    all_of([&](int, int row, int channel, f32x4 v) {
       f32x4* const to = reinterpret_cast<f32x4*>(sums + int64_t{row} * c.pitch + channel);
       *to = c.begin ? v : *to + v;
     });
   } else {
-    all_of([&](int row, int channel, f32x4 v) { finish_hidden<BF>(c.hidden, factor, row, row, channel, v); });
+    PutBack back[T::kTilesQ];
+#pragma unroll
+    for (int j = 0; j < T::kTilesQ; ++j) {
+      const int row = min(r0 + wq * T::kWaveQ + 16 * j + m, rows - 1);
+      back[j] = put_back<BF>(c.hidden, row, row);
+    }
+    all_of([&](int j, int row, int channel, f32x4 v) { finish_hidden<BF>(c.hidden, factor, row, back[j], channel, v); });
   }
 }
 
@@ -865,7 +911,7 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumCall c) {
     for (; i < n; i += step) {
       const int64_t row = i / fours, four = i % fours, part_row = c.place ? c.place[row] : row;
       if (part_row < 0) store4<BF>(c.hidden.grad, row * c.hidden.c + 4 * four, f32x4{0.f, 0.f, 0.f, 0.f}, c.hidden.c - 4 * four, c.hidden.c % 8 == 0);
-      else finish_hidden<BF>(c.hidden, factor, row, part_row, 4 * four, sum_of(c.hidden_sums, n, part_row * fours + four, c.splits));
+      else finish_hidden<BF>(c.hidden, factor, row, put_back<BF>(c.hidden, row, part_row), 4 * four, sum_of(c.hidden_sums, n, part_row * fours + four, c.splits));
     }
   } else if (blockIdx.y == 1 && c.weight_sums) {
     const int64_t n = c.vocab * fours;
@@ -881,13 +927,6 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t* to, int64_t words,
 }
 
 // ------------------------------------------------------------------ plan, workspace
-// The rows that are not ignored are numbered, and x's brought together, where that is a
-// small part of the work.
-constexpr int64_t kManyRows = 1024;
-bool numbered(int64_t rows) { return rows >= kManyRows; }
-// bf16 operands whose rows are whole steps are read where they are.
-bool packed(int64_t c, bool bf16) { return !bf16 || c % kStep != 0; }
-
 // fp32 operands with few rows and a w that is nearly all there is to read: w is read where
 // it is, three times in the two calls, where packing it to fp16 reads or writes it eleven
 // times in all. Against the packed form, us for both calls: 1 to 64 rows of 768 with 65536
@@ -899,6 +938,19 @@ bool few(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   return !bf16 && rows <= kFewRows && vocab * c >= kLargeWeight && c % 8 == 0;
 }
 int64_t planes_of(int64_t rows, int64_t vocab, int64_t c, bool bf16) { return bf16 ? 1 : few(rows, vocab, c, bf16) ? 3 : 2; }
+
+// The rows that are not ignored are numbered, and x's brought together, where that is a
+// small part of the work: two launches more for bf16 operands, 10 us; fp32 ones are packed
+// anyhow. With an eighth of the rows ignored, both calls, us, numbered and not: 8192 x 768
+// x 65536 2780 and 3010, 700 x 2048 x 65536 721 and 754, 512 x 768 x 65536 262 and 264, 300
+// rows of that 231 and 222, 2000 x 768 x 8000 146 and 139; fp32 600 x 1024 x 32000 684 and
+// 699.
+constexpr int64_t kLargeWork = int64_t{1} << 36;
+bool numbered(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
+  return rows > kFewRows && rows * c * (bf16 ? 1 : 4) >= kLargeWork / vocab;   // rows c is below 2^34
+}
+// bf16 operands whose rows are whole steps are read where they are.
+bool packed(int64_t c, bool bf16) { return !bf16 || c % kStep != 0; }
 
 int64_t take(int64_t& end, int64_t bytes) {
   const int64_t at = end;
@@ -917,12 +969,12 @@ Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward
   p.largest = take(p.end, 3 * kMaxBlocks * 4);
   p.x_plane = rows * pitch;
   p.w_plane = vocab * pitch;
-  if (numbered(rows)) {
+  if (numbered(rows, vocab, c, bf16)) {
     p.index = take(p.end, rows * 4);
     p.place = take(p.end, rows * 4);
     p.count = take(p.end, 4);
   }
-  if (packed(c, bf16) || numbered(rows)) p.x = take(p.end, planes * p.x_plane);
+  if (packed(c, bf16) || numbered(rows, vocab, c, bf16)) p.x = take(p.end, planes * p.x_plane);
   if (packed(c, bf16) && !few(rows, vocab, c, bf16)) p.w = take(p.end, planes * p.w_plane);
   if (bf16 && backward) p.x_half = take(p.end, p.x_plane);
   return p;
@@ -998,7 +1050,7 @@ Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
 }
 
 // dx goes by way of sums, unless one workgroup has the whole of a row's and no row is left out.
-bool needs_sums(const Plan& p, int64_t rows) { return p.splits > 1 || p.pieces > 1 || numbered(rows); }
+bool needs_sums(const Plan& p, bool numbered) { return p.splits > 1 || p.pieces > 1 || numbered; }
 struct BackwardPlaces {
   Places operands;
   int64_t d, d_plane, sums, weight_sums, residuals, end;
@@ -1009,7 +1061,7 @@ BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64
   b.end = b.operands.end;
   b.d_plane = p.padded_rows * p.words * 2;
   b.d = take(b.end, b.d_plane * planes_of(rows, vocab, c, bf16));
-  b.sums = !needs_sums(p, rows) ? 0 : take(b.end, p.splits * rows * p.pitch * 4);
+  b.sums = !needs_sums(p, numbered(rows, vocab, c, bf16)) ? 0 : take(b.end, p.splits * rows * p.pitch * 4);
   b.weight_sums = p.row_splits == 1 ? 0 : take(b.end, p.row_splits * vocab * p.pitch * 4);
   b.residuals = take(b.end, 2 * rows * 4);
   return b;
@@ -1074,7 +1126,7 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
   o.w = Matrix{static_cast<const char*>(c.weight), c.c * (BF ? 2 : 4), 0};
   const bool split = few(c.rows, c.vocab, c.c, BF);
   RowsCall r{c.targets, c.ignore_index, static_cast<int>(c.rows), nullptr, nullptr, nullptr};
-  if (numbered(c.rows)) {
+  if (numbered(c.rows, c.vocab, c.c, BF)) {
     o.index = r.index = reinterpret_cast<int*>(c.workspace + p.index);
     o.place = r.place = reinterpret_cast<int*>(c.workspace + p.place);
     o.count = r.count = reinterpret_cast<int*>(c.workspace + p.count);
@@ -1218,7 +1270,7 @@ void backward(const BackwardCall& c, hipStream_t s) {
   g.row_share = static_cast<int>(p.row_share);
   g.weight_sums = p.row_splits == 1 ? nullptr : reinterpret_cast<float*>(c.workspace + b.weight_sums);
   g.share = static_cast<int>(p.share);
-  const bool direct = !needs_sums(p, c.rows);
+  const bool direct = !needs_sums(p, o.index != nullptr);
   g.sums = direct ? nullptr : reinterpret_cast<float*>(c.workspace + b.sums);
   g.hidden = HiddenCall{c.hidden_grad, c.c, c.rows, residuals, c.targets, c.row_argmax,
                         BF ? static_cast<const __bf16*>(c.weight) : nullptr};

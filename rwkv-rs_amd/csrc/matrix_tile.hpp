@@ -12,6 +12,15 @@
 // the products, behind one barrier each. Instruction 16x16x32: lane l has
 // element l % 16 of p or q and the steps 8 (l / 16) .. + 7; of the sums, lane l has
 // q = l % 16 and p = 4 (l / 16) .. + 3.
+//
+// Why so: 256 x 256 sums on eight waves take half of the registers (128 of 512 a lane are
+// sums) and 64 steps of both operands 64 KiB, five slots of 32 KiB all of LDS. A stage is
+// 2048 products of 16 x 16 x 32, 256 to a wave... at full rate 0.87 us; it takes 1.1 to 1.2,
+// and over a long c 1.4, where the clock falls (power) and the whole card does 1.49 PFLOP/s.
+// Stages of 32 steps, whose rows are half cache lines, were bound by the L2's requests (a
+// third longer). Three slots for the operand that is read first save a second barrier.
+// Products of 32 x 32 x 16, four waves of 128 x 128 (registers spill) and rows of D at
+// another pitch were 3 to 30% slower.
 #pragma once
 
 #include <hip/hip_runtime.h>

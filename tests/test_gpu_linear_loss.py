@@ -474,3 +474,52 @@ def test_logits_of_minus_infinity(vocab):
         assert (ll.linear_cross_entropy_l2wrap_rows(x, one, last - 1, 9) == math.inf).all()
         one[0, 3] = math.nan                      # a NaN in a tile of minus infinities
         assert ll.linear_cross_entropy_l2wrap_rows(x, one, last, 9).isnan().all()
+
+
+@pytest.mark.parametrize("dtype,rows,vocab,c", [(torch.float32, 129, 65536, 2048), (torch.float32, 1025, 65529, 257),
+                                                (torch.bfloat16, 4097, 65536, 256), (torch.bfloat16, 2500, 20011, 1400)])
+def test_much_work_of_which_some_is_ignored(dtype, rows, vocab, c):
+    """Where there is enough to do, the rows that are learned are brought together first."""
+    announce("linear loss, much work, some ignored", dtype, rows, vocab, c)
+    x, w, t = make(rows, vocab, c, dtype, seed=61)
+    full = t.clone()
+    g = torch.rand(rows, device=DEV) + 0.1
+    r = torch.arange(rows, device=DEV)
+    for dead in (r % 3 != 1, r < rows - 1, r % 8 == 0, (r // 70) % 2 == 0):
+        t = full.masked_fill(dead, -100)
+        y = torch.where(dead[:, None], torch.full_like(x, math.nan), x)
+        loss, dx, dw = check(y, w, t, g, rows)
+        assert not dx[dead].any()
+        del loss, dx, dw
+    a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+    none = ll.linear_cross_entropy_l2wrap_rows(a, b, torch.full_like(t, -100), rows)
+    assert not none.any() and not any(v.any() for v in torch.autograd.grad(none, (a, b), g))
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_in_a_graph_with_much_work(dtype):
+    """The rows are counted on the device: a replay takes other rows than the capture."""
+    rows, vocab, c = 1100, 65536, 1024 if dtype == torch.bfloat16 else 256
+    announce("linear loss, graph, much work", dtype)
+    x, w, t = make(rows, vocab, c, dtype, seed=67)
+    g = torch.rand(rows, device=DEV)
+    a, b = x.detach().clone().requires_grad_(), w.detach().clone().requires_grad_()
+
+    def step():
+        loss = ll.linear_cross_entropy_l2wrap_rows(a, b, t, rows)
+        return (loss.detach(), *torch.autograd.grad(loss, (a, b), g))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    full = t.clone()
+    for k in (1, 2, 5, 1100):
+        t.copy_(full.masked_fill(torch.arange(rows, device=DEV) % k != 0, -100))
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(out, step()):
+            assert torch.equal(p, q)
