@@ -667,40 +667,26 @@ template <bool BF>
 __device__ __forceinline__ Factor hidden_factor(const Scalars* s) {
   return Factor{s->reference, -(kHalfExponent + (BF ? 0 : s->exponent[1]))};
 }
-// What goes back to a row: r[k] times w's row at w[k]. Asked for before its channels are,
-// so that all rows' loads are on their way at once, and read whether it is wanted or not.
-struct PutBack {
-  float r[2];
-  const __bf16* w[2];
-};
 template <bool BF>
-__device__ __forceinline__ PutBack put_back(const HiddenCall& c, int64_t row, int64_t part_row) {
-  PutBack b{};
-  if constexpr (BF) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) b.r[k] = c.residuals[k * c.rows + part_row];
-    const int64_t target = c.targets[row], top = c.row_argmax[row];
-    // no residual: there may be no such word
-    b.w[0] = c.weight + (b.r[0] != 0.f ? target : 0) * c.c;
-    b.w[1] = c.weight + (b.r[1] != 0.f ? top : 0) * c.c;
-  }
-  return b;
-}
-template <bool BF>
-__device__ __forceinline__ void finish_hidden(const HiddenCall& c, Factor f, int64_t row, const PutBack& b, int64_t channel, f32x4 v) {
+__device__ __forceinline__ void finish_hidden(const HiddenCall& c, Factor f, int64_t row, int64_t part_row, int64_t channel, f32x4 v) {
   const bool whole = c.c % 8 == 0;
   if constexpr (BF) {
+    const int64_t words[2] = {c.targets[row], c.row_argmax[row]};
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
+      const float r = c.residuals[k * c.rows + part_row];
+      // read whether it is wanted or not, so that nothing waits for the residual first; where
+      // there is none, there may be no such word
+      const __bf16* const from = c.weight + (r != 0.f ? words[k] : 0) * c.c + channel;
       bf16x4 w;
       if (whole) {
-        w = *reinterpret_cast<const bf16x4*>(b.w[k] + channel);
+        w = *reinterpret_cast<const bf16x4*>(from);
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = b.w[k][min(channel + e, c.c - 1)];
+        for (int e = 0; e < 4; ++e) w[e] = from[min(static_cast<int64_t>(e), c.c - 1 - channel)];
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += b.r[k] != 0.f ? b.r[k] * static_cast<float>(w[e]) : 0.f;
+      for (int e = 0; e < 4; ++e) v[e] += r != 0.f ? r * static_cast<float>(w[e]) : 0.f;
     }
   }
 #pragma unroll
@@ -724,7 +710,7 @@ struct GradientsCall {
   float* weight_sums;        // [row shares, vocab, pitch]; null: one share, dw itself is stored
   int share;                 // words of a workgroup of dx
   bool begin;                // the first piece: no sums to add to
-  float* sums;               // [splits, rows, pitch]; null: dx itself is stored
+  float* sums;               // [splits, rows, pitch]; null (of fp32): dx itself is stored
   int pitch;
   HiddenCall hidden;
 };
@@ -835,24 +821,18 @@ __device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, i
 #pragma unroll
       for (int i = 0; i < T::kTilesP; ++i) {
         const int channel = c0 + wp * T::kWaveP + 16 * i + 4 * g;
-        if (channel < c.pitch) store(j, row, channel, t.acc[i][j]);
+        if (channel < c.pitch) store(row, channel, t.acc[i][j]);
       }
     }
   };
-  if (c.sums) {
+  if (BF || c.sums) {
     float* const sums = c.sums + int64_t{split} * c.rows * c.pitch;
-    all_of([&](int, int row, int channel, f32x4 v) {
+    all_of([&](int row, int channel, f32x4 v) {
       f32x4* const to = reinterpret_cast<f32x4*>(sums + int64_t{row} * c.pitch + channel);
       *to = c.begin ? v : *to + v;
     });
   } else {
-    PutBack back[T::kTilesQ];
-#pragma unroll
-    for (int j = 0; j < T::kTilesQ; ++j) {
-      const int row = min(r0 + wq * T::kWaveQ + 16 * j + m, rows - 1);
-      back[j] = put_back<BF>(c.hidden, row, row);
-    }
-    all_of([&](int j, int row, int channel, f32x4 v) { finish_hidden<BF>(c.hidden, factor, row, back[j], channel, v); });
+    all_of([&](int row, int channel, f32x4 v) { finish_hidden<false>(c.hidden, factor, row, row, channel, v); });
   }
 }
 
@@ -911,7 +891,7 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumCall c) {
     for (; i < n; i += step) {
       const int64_t row = i / fours, four = i % fours, part_row = c.place ? c.place[row] : row;
       if (part_row < 0) store4<BF>(c.hidden.grad, row * c.hidden.c + 4 * four, f32x4{0.f, 0.f, 0.f, 0.f}, c.hidden.c - 4 * four, c.hidden.c % 8 == 0);
-      else finish_hidden<BF>(c.hidden, factor, row, put_back<BF>(c.hidden, row, part_row), 4 * four, sum_of(c.hidden_sums, n, part_row * fours + four, c.splits));
+      else finish_hidden<BF>(c.hidden, factor, row, part_row, 4 * four, sum_of(c.hidden_sums, n, part_row * fours + four, c.splits));
     }
   } else if (blockIdx.y == 1 && c.weight_sums) {
     const int64_t n = c.vocab * fours;
@@ -1033,7 +1013,7 @@ Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
       const int64_t share = up(ceil_div(p.words, s), kStep), splits = ceil_div(p.words, share);
       if (splits < s) continue;
       const int64_t hidden_time = share / kStep * parts + kOverhead;
-      const int64_t moved = (splits > 1 ? kLaunch + splits * rows * p.pitch * 8 / kBytesPerStage : 0) + weight_moved;
+      const int64_t moved = (bf16 || splits > 1 ? kLaunch + splits * rows * p.pitch * 8 / kBytesPerStage : 0) + weight_moved;
       if (moved >= least) break;
       const int64_t time = moved + (hidden_time > weight_time ? finish(hidden_tiles * splits, hidden_time, weight_tiles * row_splits, weight_time)
                                                               : finish(weight_tiles * row_splits, weight_time, hidden_tiles * splits, hidden_time));
@@ -1049,8 +1029,12 @@ Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   return p;
 }
 
-// dx goes by way of sums, unless one workgroup has the whole of a row's and no row is left out.
-bool needs_sums(const Plan& p, bool numbered) { return p.splits > 1 || p.pieces > 1 || numbered; }
+// dx goes by way of sums, unless one workgroup has the whole of a row's, no row is left out
+// and nothing is put back, which a tile's end would wait for (96 x 256 x 256 in bf16 45 us
+// then, 41 with the launch).
+bool needs_sums(const Plan& p, int64_t rows, int64_t vocab, int64_t c, bool bf16) {
+  return bf16 || p.splits > 1 || p.pieces > 1 || numbered(rows, vocab, c, bf16);
+}
 struct BackwardPlaces {
   Places operands;
   int64_t d, d_plane, sums, weight_sums, residuals, end;
@@ -1061,7 +1045,7 @@ BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64
   b.end = b.operands.end;
   b.d_plane = p.padded_rows * p.words * 2;
   b.d = take(b.end, b.d_plane * planes_of(rows, vocab, c, bf16));
-  b.sums = !needs_sums(p, numbered(rows, vocab, c, bf16)) ? 0 : take(b.end, p.splits * rows * p.pitch * 4);
+  b.sums = !needs_sums(p, rows, vocab, c, bf16) ? 0 : take(b.end, p.splits * rows * p.pitch * 4);
   b.weight_sums = p.row_splits == 1 ? 0 : take(b.end, p.row_splits * vocab * p.pitch * 4);
   b.residuals = take(b.end, 2 * rows * 4);
   return b;
@@ -1270,7 +1254,7 @@ void backward(const BackwardCall& c, hipStream_t s) {
   g.row_share = static_cast<int>(p.row_share);
   g.weight_sums = p.row_splits == 1 ? nullptr : reinterpret_cast<float*>(c.workspace + b.weight_sums);
   g.share = static_cast<int>(p.share);
-  const bool direct = !needs_sums(p, o.index != nullptr);
+  const bool direct = !needs_sums(p, c.rows, c.vocab, c.c, BF);
   g.sums = direct ? nullptr : reinterpret_cast<float*>(c.workspace + b.sums);
   g.hidden = HiddenCall{c.hidden_grad, c.c, c.rows, residuals, c.targets, c.row_argmax,
                         BF ? static_cast<const __bf16*>(c.weight) : nullptr};
