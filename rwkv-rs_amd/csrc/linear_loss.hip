@@ -35,10 +35,11 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 // A tile of logits: words by rows, on waves by waves. 256 by 256 reads each operand's
-// element once for 256 products, which the matrix cores need to be fed from L2: tiles of
-// 128 by 128 took a third longer for 8192 rows. Two smaller ones, of which a compute unit
-// has two and four at a time, for few rows or words, where large ones leave units idle:
-// 64 rows of 768 with 65536 words 26 us on the small one, 45 on the large one.
+// element once for 256 products, which the matrix cores need to be fed from L2: on tiles of
+// 128 by 128 the forward of 8192 x 768 x 65536 takes 823 us for 687, of 2048 x 4096 x 65536
+// 1005 for 721. Two smaller ones, of which a compute unit has two and four at a time, for
+// few rows or words, where large ones leave units idle: 30 x 2048 x 8000 19 us on the small
+// one and 31 on the large one, 1000 x 512 x 1000 13 and 26.
 struct Big {
   static constexpr int kWords = 256, kRows = 256, kWavesP = 2, kWavesQ = 4, kEach = 1;
 };
@@ -365,13 +366,13 @@ __device__ __forceinline__ float share_of(float own, float most) { return own ==
 //
 // Persistent: as many workgroups as fit take the tiles in turn, and ask for a tile's first
 // operands before they are done with the one before, so that only the first tile's loads
-// are waited for. What follows the products bounds a tile of few channels beside them: of
-// 256 by 256 logits, c = 768, 14 of 23 us are products, the rest the maximum, the
-// exponentials and the first index (ten instructions' time an element).
+// are waited for. What follows the products bounds a tile of few channels beside them: a
+// tile of 256 by 256 takes 1.5 us for 64 channels and 5 for the maximum, the exponentials and
+// the first index, ten instructions' time an element.
 constexpr int kWordTiles = 8;
 template <bool BF, bool kBackward, typename Shape>
-__global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, std::max(Shape::kWavesP* Shape::kWavesQ* Shape::kEach / 4, 1)) void logits_kernel(
-    const LogitsCall c) {
+__global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ,
+                             std::max(Shape::kWavesP* Shape::kWavesQ* Shape::kEach / 4, 1)) void logits_kernel(const LogitsCall c) {
   constexpr int kWords = Shape::kWords, kRowsTile = Shape::kRows, kWavesP = Shape::kWavesP;
   constexpr bool kFew = kIsFew<Shape>;
   using T = typename LogitsTile<Shape, BF ? kBf16 : kHalves>::T;
@@ -393,7 +394,8 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, std::max(Shap
     const int run_words = min(kWordTiles, word_tiles - run * kWordTiles);
     v0 = c.first + (run * kWordTiles + in_run % run_words) * kWords;
     r0 = in_run / run_words * kRowsTile;
-    T::begin(work, lds, Operand{c.w.data + int64_t{min(v0, c.vocab - 1)} * c.w.pitch, c.w.pitch, max(c.vocab - v0, 1), kFew ? c.c : c.steps},
+    T::begin(work, lds,
+             Operand{c.w.data + int64_t{min(v0, c.vocab - 1)} * c.w.pitch, c.w.pitch, max(c.vocab - v0, 1), kFew ? c.c : c.steps},
              Operand{c.x.data + int64_t{r0} * c.x.pitch, c.x.pitch, rows - r0, c.steps}, c.w.plane, c.x.plane, 0, c.steps);
   };
   if (at < last) begin(at);
@@ -516,7 +518,8 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ, std::max(Shap
 #pragma unroll
       for (int j = 0; j < T::kTilesQ; ++j) {
         const int row = r + wq * T::kWaveQ + 16 * j + m;
-        const float lse = of[j].lse, h = ldexpf(of[j].h / reference, kHalfExponent), wrap = ldexpf(of[j].wrap / reference, kHalfExponent);
+        const float lse = of[j].lse, h = ldexpf(of[j].h / reference, kHalfExponent);
+        const float wrap = ldexpf(of[j].wrap / reference, kHalfExponent);
         const int own = of[j].own, top = of[j].top;
         const bool dead = of[j].dead;
 #pragma unroll
@@ -716,8 +719,9 @@ struct GradientsCall {
 };
 
 // Tiles of 256 by 256 (or 128 channels) as the logits' are. Workgroups of both gradients in
-// one launch: either alone would leave units idle in its last round, dx's of 768 channels
-// and 8192 rows has 84 tiles a share. In turn they took 3% longer.
+// one launch: either alone would leave units idle in its last round. The backward with one
+// after the other: 8192 x 768 x 65536 2377 us for 2090, 512 rows of that 250 for 205,
+// 2048 x 4096 x 65536 2494 for 2479, fp32 1024 x 1024 x 32000 690 for 583.
 //
 // The tiles of a gradient in an order in which those that an XCD has at a time share
 // both operands: runs of up to five tiles of channels, in each the other tiles.
@@ -809,7 +813,8 @@ __device__ __forceinline__ void hidden_tile(const GradientsCall& c, char* lds, i
   T t;
   typename T::Work work;
   T::begin(work, lds, Operand{c.w.data + int64_t{c.first} * c.w.pitch + c0 * (kFew ? 4 : 2), c.w.pitch, c.c - c0, c.vocab - c.first},
-           Operand{c.d + int64_t{r0} * c.words * 2, int64_t{c.words} * 2, (rows + kStep - 1) / kStep * kStep - r0, c.words}, c.w.plane, c.d_plane, k0, k1);
+           Operand{c.d + int64_t{r0} * c.words * 2, int64_t{c.words} * 2, (rows + kStep - 1) / kStep * kStep - r0, c.words},
+           c.w.plane, c.d_plane, k0, k1);
   t.run(work, lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4, wp = wave % kWavesP, wq = wave / kWavesP;
@@ -852,7 +857,8 @@ __global__ __launch_bounds__(kThreads, 2) void gradients_kernel(const GradientsC
   }
 }
 
-// Of few rows, one after the other: memory bounds both.
+// Of few rows of fp32, one after the other: memory bounds both. 64 x 768 x 65536: dw 67 us,
+// of which 41 are what it writes, dx 61, of which 41 are w.
 template <int kChannels>
 __global__ __launch_bounds__(kThreads, 2) void few_weight_kernel(const GradientsCall c) {
   __shared__ __attribute__((aligned(16))) char lds[kWeightLds<kChannels>];
@@ -890,8 +896,10 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumCall c) {
     const Factor factor = hidden_factor<BF>(c.scalars);
     for (; i < n; i += step) {
       const int64_t row = i / fours, four = i % fours, part_row = c.place ? c.place[row] : row;
-      if (part_row < 0) store4<BF>(c.hidden.grad, row * c.hidden.c + 4 * four, f32x4{0.f, 0.f, 0.f, 0.f}, c.hidden.c - 4 * four, c.hidden.c % 8 == 0);
-      else finish_hidden<BF>(c.hidden, factor, row, part_row, 4 * four, sum_of(c.hidden_sums, n, part_row * fours + four, c.splits));
+      if (part_row < 0)
+        store4<BF>(c.hidden.grad, row * c.hidden.c + 4 * four, f32x4{0.f, 0.f, 0.f, 0.f}, c.hidden.c - 4 * four, c.hidden.c % 8 == 0);
+      else
+        finish_hidden<BF>(c.hidden, factor, row, part_row, 4 * four, sum_of(c.hidden_sums, n, part_row * fours + four, c.splits));
     }
   } else if (blockIdx.y == 1 && c.weight_sums) {
     const int64_t n = c.vocab * fours;
@@ -1208,8 +1216,9 @@ void forward(const ForwardCall& c, hipStream_t s) {
 
 template <int kChannels>
 void few_gradients(const GradientsCall& g, hipStream_t s) {
-  if (g.weight_blocks) hipLaunchKernelGGL(few_weight_kernel<kChannels>, dim3(static_cast<unsigned>(g.weight_blocks)), dim3(kThreads), 0, s, g);
-  if (g.hidden_blocks) hipLaunchKernelGGL(few_hidden_kernel<kChannels>, dim3(static_cast<unsigned>(g.hidden_blocks)), dim3(64 * Few::kWavesP), 0, s, g);
+  const dim3 weight(static_cast<unsigned>(g.weight_blocks)), hidden(static_cast<unsigned>(g.hidden_blocks));
+  if (g.weight_blocks) hipLaunchKernelGGL(few_weight_kernel<kChannels>, weight, dim3(kThreads), 0, s, g);
+  if (g.hidden_blocks) hipLaunchKernelGGL(few_hidden_kernel<kChannels>, hidden, dim3(64 * Few::kWavesP), 0, s, g);
 }
 
 template <bool BF>
@@ -1267,7 +1276,8 @@ void backward(const BackwardCall& c, hipStream_t s) {
     g.begin = first == 0;
     g.weight_tiles = c.weight_grad ? static_cast<int>(channel_tiles * (l.words / kGradTile) * p.row_splits) : 0;
     g.weight_blocks = static_cast<int>(up(g.weight_tiles, kXcds));
-    g.hidden_blocks = c.hidden_grad ? static_cast<int>(up(channel_tiles * ceil_div(c.rows, few(c.rows, c.vocab, c.c, BF) ? Few::kRows : kGradTile) * ceil_div(l.words, p.share), kXcds)) : 0;
+    const int64_t row_tiles = ceil_div(c.rows, few(c.rows, c.vocab, c.c, BF) ? Few::kRows : kGradTile);
+    g.hidden_blocks = c.hidden_grad ? static_cast<int>(up(channel_tiles * row_tiles * ceil_div(l.words, p.share), kXcds)) : 0;
     g.hidden_first = p.hidden_first;
     const dim3 grid(static_cast<unsigned>(g.weight_blocks + g.hidden_blocks));
     if constexpr (!BF) {

@@ -13,14 +13,14 @@
 // element l % 16 of p or q and the steps 8 (l / 16) .. + 7; of the sums, lane l has
 // q = l % 16 and p = 4 (l / 16) .. + 3.
 //
-// Why so: 256 x 256 sums on eight waves take half of the registers (128 of 512 a lane are
-// sums) and 64 steps of both operands 64 KiB, five slots of 32 KiB all of LDS. A stage is
-// 2048 products of 16 x 16 x 32, 256 to a wave... at full rate 0.87 us; it takes 1.1 to 1.2,
-// and over a long c 1.4, where the clock falls (power) and the whole card does 1.49 PFLOP/s.
-// Stages of 32 steps, whose rows are half cache lines, were bound by the L2's requests (a
-// third longer). Three slots for the operand that is read first save a second barrier.
-// Products of 32 x 32 x 16, four waves of 128 x 128 (registers spill) and rows of D at
-// another pitch were 3 to 30% slower.
+// Why so: 256 x 256 sums on eight waves of 256 registers a lane (128 of them sums) and five
+// slots of 32 KiB, all of LDS, for 64 steps of the operands. A stage is 512 instructions,
+// 0.86 us at the dense peak; it takes 1.1 to 1.2, and over 4096 channels 1.4, where the
+// matrix cores draw the power that there is and the clock falls (1.49 PFLOP/s; products
+// from registers alone sustain 1.98). Stages of 32 steps, whose rows are half cache lines,
+// were bound by the L2's requests: 2048 x 4096 x 65536 1104 us for 839. Two loops were
+// slower: instructions of 32 x 32 x 16 (1.4 PFLOP/s from registers) and four waves of 128 x
+// 128 (registers spill; 3 to 5%).
 #pragma once
 
 #include <hip/hip_runtime.h>
