@@ -103,7 +103,8 @@ struct Side {
   uint32_t at[kLoads];     // byte offset of a lane's piece from the stage's first element
   const char* base;
   int64_t pitch;
-  int steps;
+  int items, steps;
+  bool ended;              // the places are of the last stage, which is not whole
 
   // the step (steps' form) or row that load j of this lane brings
   __device__ __forceinline__ int line(int j, int wave, int lane) const {
@@ -120,18 +121,35 @@ struct Side {
     const int place = (j * kWaves + wave) * 64 + lane;
     return 16 * (place % (kLayout == kRows ? kPieces : kPerStep) ^ swap(line(j, wave, lane)));
   }
+  // Places of a stage from step k on, of which `steps` are left from k = 0; a whole stage's
+  // do not depend on k.
+  __device__ __forceinline__ void set(int k, int wave, int lane) {
+    const int last = max(steps - 1 - k, 0);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int l = line(j, wave, lane), bytes = within(j, wave, lane);
+      if constexpr (kLayout == kRows) {
+        at[j] = static_cast<uint32_t>(min(l, items - 1) * pitch) + (kSize == 4 ? min(bytes, last / 4 * 16) : bytes);
+      } else {
+        at[j] = static_cast<uint32_t>(min(l, last) * pitch) + min(bytes, min(items - 1, kItems - 1) / (16 / kSize) * 16);
+      }
+    }
+  }
   __device__ __forceinline__ void init(const Operand& o, int wave, int lane) {
     base = reinterpret_cast<const char*>(uniform(reinterpret_cast<int64_t>(o.base)));
     pitch = o.pitch;
+    items = uniform(o.items);
     steps = uniform(o.steps);
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int l = line(j, wave, lane);
-      if constexpr (kLayout == kRows) {
-        at[j] = static_cast<uint32_t>(min(l, o.items - 1) * pitch) + within(j, wave, lane);
-      } else {
-        const int last = min(o.items - 1, kItems - 1) / (16 / kSize) * 16;
-        at[j] = static_cast<uint32_t>(l * pitch) + min(within(j, wave, lane), last);
+    ended = false;
+    set(0, wave, lane);
+  }
+  // Before the loads of the stage from step k on. Rows of 16-bit elements are whole stages.
+  __device__ __forceinline__ void turn(int k, int wave, int lane) {
+    if constexpr (kLayout == Layout::kSteps || kSize == 4) {
+      const bool end = k + kSteps > steps;
+      if (end || ended) {
+        set(k, wave, lane);
+        ended = end;
       }
     }
   }
@@ -140,30 +158,25 @@ struct Side {
   __device__ __forceinline__ Buffer stage(int64_t offset, int k) const {
     return buffer(base + offset + (kLayout == kRows ? kSize * k : min(k, steps - 1) * pitch));
   }
-  __device__ __forceinline__ void load(int j, char* lds, Buffer from, int k, int wave, int lane) const {
-    uint32_t offset = at[j];
-    if constexpr (kLayout == Layout::kSteps) {
-      if (k + kSteps > steps) {
-        const int last = max(steps - 1 - k, 0);
-        offset -= static_cast<uint32_t>(max(line(j, wave, lane) - last, 0)) * static_cast<uint32_t>(pitch);
-      }
-    } else if constexpr (kSize == 4) {   // rows of 16-bit elements are whole stages; k < steps
-      if (k + kSteps > steps) offset -= static_cast<uint32_t>(max(within(j, wave, lane) - (steps - 1 - k) / 4 * 16, 0));
-    }
-    bring(from, offset, 0, lds + (j * kWaves + wave) * 1024);
+  __device__ __forceinline__ void load(int j, char* lds, Buffer from, int wave) const {
+    bring(from, at[j], 0, lds + (j * kWaves + wave) * 1024);
   }
-  // what lane (m, g) of a wave whose items begin at `first` gives to tile i's instruction
-  // over half a stage's steps
-  __device__ __forceinline__ s16x8 read(const char* lds, int half, int first, int i, int m, int g) const {
+  // Of a lane (m, g) of a wave whose items begin at `first`: what read() of the steps' form
+  // begins with. Tile i's place is this with 32 i in exclusive or.
+  __device__ __forceinline__ static uint32_t lane_at(int first, int m, int g) {
+    if constexpr (kLayout == kRows) return 0;
+    const int k = 8 * g + (m >> 2);
+    return k * (kItems * 2) + 16 * ((first / 8 + ((m & 3) >> 1)) ^ swap(k)) + 8 * (m & 1);
+  }
+  // what that lane gives to tile i's instruction over half a stage's steps
+  __device__ __forceinline__ s16x8 read(const char* lds, uint32_t at_lane, int half, int first, int i, int m, int g) const {
     static_assert(kSize == 2);
     if constexpr (kLayout == kRows) {
       const int row = first + (kSpread ? 32 * (i / 2) + 8 * (m >> 2) + 4 * (i % 2) + (m & 3) : 16 * i + m);
       return *reinterpret_cast<const s16x8*>(lds + row * kRowBytes + 16 * ((4 * half + g) ^ swap(row)));
     } else {
       typedef __attribute__((address_space(3))) s16x4* Local;
-      const int k = 32 * half + 8 * g + (m >> 2);          // and k + 4, whose pieces lie alike
-      const int piece = (first / 8 + 2 * i + ((m & 3) >> 1)) ^ swap(k);
-      const char* from = lds + k * (kItems * 2) + 16 * piece + 8 * (m & 1);
+      const char* const from = lds + (at_lane ^ (32 * i)) + 32 * half * (kItems * 2);   // and four steps on, whose pieces lie alike
       const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Local)(from));
       const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Local)(from + 4 * kItems * 2));
       return s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -247,24 +260,25 @@ struct Tile {
     SideQ q;
     int64_t plane_p, plane_q;
     int wave, lane;
+    uint32_t at_p, at_q;
     __device__ __forceinline__ Buffer from(const Next<kSlotsP>& n) const {
       return p.stage(kKind == kHalves ? (n.part == 2 ? plane_p : 0) : kKind == kThirds ? third_p(n.part) * plane_p : 0, n.k);
     }
     __device__ __forceinline__ Buffer from(const Next<kSlotsQ>& n, int) const {
       return q.stage(kKind == kHalves ? (n.part == 1 ? plane_q : 0) : kKind == kThirds ? third_q(n.part) * plane_q : 0, n.k);
     }
-    __device__ __forceinline__ s16x8 read_p(const char* lds, int half, int i) const {
-      return p.read(lds, half, wave % kWavesP * kWaveP, i, lane & 15, lane >> 4);
+    __device__ __forceinline__ s16x8 read_p(const char* lds, uint32_t at, int half, int i) const {
+      return p.read(lds, at, half, wave % kWavesP * kWaveP, i, lane & 15, lane >> 4);
     }
-    __device__ __forceinline__ s16x8 read_q(const char* lds, int half, int j) const {
-      return q.read(lds, half, wave / kWavesP * kWaveQ, j, lane & 15, lane >> 4);
+    __device__ __forceinline__ s16x8 read_q(const char* lds, uint32_t at, int half, int j) const {
+      return q.read(lds, at, half, wave / kWavesP * kWaveQ, j, lane & 15, lane >> 4);
     }
   };
   __device__ __forceinline__ static void bring_p(int n, char* lds, const Place& a, Buffer from, const Next<kSlotsP>& next) {
-    a.p.load(n, lds + next.slot * SideP::kBytes, from, next.k, a.wave, a.lane);
+    a.p.load(n, lds + next.slot * SideP::kBytes, from, a.wave);
   }
   __device__ __forceinline__ static void bring_q(int n, char* lds, const Place& a, Buffer from, const Next<kSlotsQ>& next) {
-    a.q.load(n, lds + kPlaceQ + next.slot * SideQ::kBytes, from, next.k, a.wave, a.lane);
+    a.q.load(n, lds + kPlaceQ + next.slot * SideQ::kBytes, from, a.wave);
   }
   __device__ __forceinline__ void products(int i, s16x8 p, const s16x8 (&q)[kTilesQ]) {
 #pragma unroll
@@ -286,15 +300,20 @@ struct Tile {
     constexpr int kNear = kDeepP ? SideQ::kLoads : SideP::kLoads;       // of the operand with two slots: first
     constexpr int kNearPerGroup = (kNear + kTail - 1) / kTail, kDeepPerGroup = (kDeepLoads + kBody - 1) / kBody;
     const Buffer from_p = a.from(next_p), from_q = a.from(next_q, 0);
+    // Unknown anew for each stage, or the compiler keeps every tile's place in a register of
+    // its own through the loop, of which there are none left.
+    uint32_t at_p = a.at_p, at_q = a.at_q;
+    if constexpr (kLayoutP == kSteps) asm volatile("" : "+v"(at_p));
+    if constexpr (kLayoutQ == kSteps) asm volatile("" : "+v"(at_q));
     auto load_near = [&](int n) {
       if (n >= kNear) return;
-      if constexpr (kDeepP) a.q.load(n, to_q, from_q, next_q.k, a.wave, a.lane);
-      else a.p.load(n, to_p, from_p, next_p.k, a.wave, a.lane);
+      if constexpr (kDeepP) a.q.load(n, to_q, from_q, a.wave);
+      else a.p.load(n, to_p, from_p, a.wave);
     };
     auto load_deep = [&](int n) {
       if (n >= kDeepLoads) return;
-      if constexpr (kDeepP) a.p.load(n, to_p, from_p, next_p.k, a.wave, a.lane);
-      else a.q.load(n, to_q, from_q, next_q.k, a.wave, a.lane);
+      if constexpr (kDeepP) a.p.load(n, to_p, from_p, a.wave);
+      else a.q.load(n, to_q, from_q, a.wave);
     };
 #pragma unroll
     for (int i = 0; i < kTail; ++i) {
@@ -302,8 +321,8 @@ struct Tile {
       for (int n = i * kNearPerGroup; n < (i + 1) * kNearPerGroup; ++n) load_near(n);
 #pragma unroll
       for (int n = i * kHoldsPerGroup; n < (i + 1) * kHoldsPerGroup; ++n) {
-        if (n < kTilesQ) held.q[n] = a.read_q(q, 0, n);
-        else if (n < kHolds) held.p[n - kTilesQ] = a.read_p(p, 0, n - kTilesQ);
+        if (n < kTilesQ) held.q[n] = a.read_q(q, at_q, 0, n);
+        else if (n < kHolds) held.p[n - kTilesQ] = a.read_p(p, at_p, 0, n - kTilesQ);
       }
       if constexpr (!kFirst) products(kTilesP - kTail + i, held.last_p[i], held.last_q);
       if constexpr (kKind == kHalfQ) {
@@ -323,9 +342,9 @@ struct Tile {
       for (int n = i * kDeepPerGroup; n < (i + 1) * kDeepPerGroup; ++n) load_deep(n);
 #pragma unroll
       for (int n = i * kReadsPerGroup; n < (i + 1) * kReadsPerGroup; ++n) {
-        if (n < kTilesP - kHeldP) at[0][n + kHeldP] = a.read_p(p, 0, n + kHeldP);
-        else if (n < kTilesP - kHeldP + kTilesQ) held.last_q[n - (kTilesP - kHeldP)] = a.read_q(q, 1, n - (kTilesP - kHeldP));
-        else if (n < kReads) at[1][n - (kTilesP - kHeldP + kTilesQ)] = a.read_p(p, 1, n - (kTilesP - kHeldP + kTilesQ));
+        if (n < kTilesP - kHeldP) at[0][n + kHeldP] = a.read_p(p, at_p, 0, n + kHeldP);
+        else if (n < kTilesP - kHeldP + kTilesQ) held.last_q[n - (kTilesP - kHeldP)] = a.read_q(q, at_q, 1, n - (kTilesP - kHeldP));
+        else if (n < kReads) at[1][n - (kTilesP - kHeldP + kTilesQ)] = a.read_p(p, at_p, 1, n - (kTilesP - kHeldP + kTilesQ));
       }
       if constexpr (kKind == kHalfQ) {
         // a part of them before each group of products, none left before their own
@@ -367,6 +386,8 @@ struct Tile {
     w.a.wave = uniform(static_cast<int>(threadIdx.x >> 6));
     w.a.p.init(p, w.a.wave, w.a.lane);
     w.a.q.init(q, w.a.wave, w.a.lane);
+    w.a.at_p = SideP::lane_at(w.a.wave % kWavesP * kWaveP, w.a.lane & 15, w.a.lane >> 4);
+    w.a.at_q = SideQ::lane_at(w.a.wave / kWavesP * kWaveQ, w.a.lane & 15, w.a.lane >> 4);
     w.a.plane_p = plane_p;
     w.a.plane_q = plane_q;
     w.k0 = k0;
@@ -375,12 +396,14 @@ struct Tile {
     w.next_p = {k0, 0, 0};
     w.next_q = {k0, 0, 0};
     auto all_p = [&] {
+      w.a.p.turn(w.next_p.k, w.a.wave, w.a.lane);
       const Buffer from = w.a.from(w.next_p);
 #pragma unroll
       for (int n = 0; n < SideP::kLoads; ++n) bring_p(n, lds, w.a, from, w.next_p);
       w.next_p.advance(k0, k1);
     };
     auto all_q = [&] {
+      w.a.q.turn(w.next_q.k, w.a.wave, w.a.lane);
       const Buffer from = w.a.from(w.next_q, 0);
 #pragma unroll
       for (int n = 0; n < SideQ::kLoads; ++n) bring_q(n, lds, w.a, from, w.next_q);
@@ -408,7 +431,12 @@ struct Tile {
       slot_p = slot_p == kSlotsP - 1 ? 0 : slot_p + 1;
       slot_q = slot_q == kSlotsQ - 1 ? 0 : slot_q + 1;
     };
+    auto turn = [&] {
+      w.a.p.turn(w.next_p.k, w.a.wave, w.a.lane);
+      w.a.q.turn(w.next_q.k, w.a.wave, w.a.lane);
+    };
     auto one = [&](auto first) {
+      turn();
       arrive<kDeepLoads>();
       step<decltype(first)::value>(lds + w.next_p.slot * SideP::kBytes, lds + kPlaceQ + w.next_q.slot * SideQ::kBytes,
                                    lds + slot_p * SideP::kBytes, lds + kPlaceQ + slot_q * SideQ::kBytes, held, w.a, w.next_p,
@@ -421,6 +449,7 @@ struct Tile {
       for (int s = 1; s < stages; ++s) one(std::false_type());
     } else {
       for (int s = 0; s < stages; ++s) {   // the same loads in the same order, and the same barriers
+        turn();
         arrive<kDeepLoads>();
         const Buffer from_p = w.a.from(w.next_p), from_q = w.a.from(w.next_q, 0);
         auto all_p = [&] {
@@ -480,16 +509,17 @@ struct FewTile {
     int64_t plane_q;
     int k0, k1, wave, lane;
   };
-  __device__ __forceinline__ static void load(const Work& w, char* to, int stage) {
+  __device__ __forceinline__ static void load(Work& w, char* to, int stage) {
     const int k = min(w.k0 + stage * kSteps, w.k1 - kSteps);   // past the last stage that one again
+    w.p.turn(k, w.wave, w.lane);
     const Buffer from = w.p.stage(0, k);
 #pragma unroll
-    for (int n = 0; n < SideP::kLoads; ++n) w.p.load(n, to, from, k, w.wave, w.lane);
+    for (int n = 0; n < SideP::kLoads; ++n) w.p.load(n, to, from, w.wave);
 #pragma unroll
     for (int plane = 0; plane < 3; ++plane) {
       const Buffer of = w.q.stage(plane * w.plane_q, k);
 #pragma unroll
-      for (int n = 0; n < SideQ::kLoads; ++n) w.q.load(n, to + SideP::kBytes + plane * SideQ::kBytes, of, k, w.wave, w.lane);
+      for (int n = 0; n < SideQ::kLoads; ++n) w.q.load(n, to + SideP::kBytes + plane * SideQ::kBytes, of, w.wave);
     }
   }
   __device__ __forceinline__ static void begin(Work& w, char* lds, const Operand& p, const Operand& q, int64_t, int64_t plane_q,
@@ -510,14 +540,14 @@ struct FewTile {
 #pragma unroll
       for (int j = 0; j < kTilesQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  __device__ __forceinline__ void step(char* __restrict to, const char* __restrict from, const Work& w, int stage) {
+  __device__ __forceinline__ void step(char* __restrict to, const char* __restrict from, Work& w, int stage) {
     const int m = w.lane & 15, g = w.lane >> 4;
     load(w, to, stage);
     s16x8 q[kTilesQ][3];
 #pragma unroll
     for (int j = 0; j < kTilesQ; ++j)
 #pragma unroll
-      for (int plane = 0; plane < 3; ++plane) q[j][plane] = w.q.read(from + SideP::kBytes + plane * SideQ::kBytes, 0, 0, j, m, g);
+      for (int plane = 0; plane < 3; ++plane) q[j][plane] = w.q.read(from + SideP::kBytes + plane * SideQ::kBytes, 0, 0, 0, j, m, g);
 #pragma unroll
     for (int i = 0; i < kTilesP; ++i) {
       float v[8];
