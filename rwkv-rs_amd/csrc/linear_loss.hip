@@ -41,13 +41,18 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 // few rows or words, where large ones leave units idle: 30 x 2048 x 8000 19 us on the small
 // one and 31 on the large one, 1000 x 512 x 1000 13 and 26.
 struct Big {
-  static constexpr int kWords = 256, kRows = 256, kWavesP = 2, kWavesQ = 4, kEach = 1;
+  static constexpr int kWords = 256, kRows = 256, kWavesP = 2, kWavesQ = 4, kEach = 1, kLead = 0;
 };
 struct Middle {
-  static constexpr int kWords = 128, kRows = 128, kWavesP = 2, kWavesQ = 2, kEach = 2;
+  static constexpr int kWords = 128, kRows = 128, kWavesP = 2, kWavesQ = 2, kEach = 2, kLead = 0;
 };
 struct Small {
-  static constexpr int kWords = 64, kRows = 64, kWavesP = 2, kWavesQ = 2, kEach = 4;
+  static constexpr int kWords = 64, kRows = 64, kWavesP = 2, kWavesQ = 2, kEach = 4, kLead = 0;
+};
+// The same with eight stages on their way, one to a compute unit, for few tiles of many
+// channels: 64 x 4096 x 16000 28 us and 34, fp32 7 x 2944 x 70 50 and 59.
+struct Deep {
+  static constexpr int kWords = 64, kRows = 64, kWavesP = 2, kWavesQ = 2, kEach = 1, kLead = 8;
 };
 // Of fp32 operands where there are few rows: w is split on its way to the products. 256
 // words a workgroup keep 64 KiB of w on their way to each compute unit; the small one is
@@ -63,7 +68,7 @@ template <typename Shape>
 constexpr bool kIsFew = std::is_same<Shape, Few>::value || std::is_same<Shape, FewSmall>::value;
 template <typename Shape, Kind kKind, bool kFew = kIsFew<Shape>>
 struct LogitsTile {
-  using T = Tile<kRows, kRows, Shape::kWords, Shape::kRows, Shape::kWavesP, Shape::kWavesQ, true, true, kKind>;
+  using T = Tile<kRows, kRows, Shape::kWords, Shape::kRows, Shape::kWavesP, Shape::kWavesQ, true, true, kKind, Shape::kLead>;
 };
 template <typename Shape, Kind kKind>
 struct LogitsTile<Shape, kKind, true> {
@@ -1062,7 +1067,7 @@ BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64
 // The tile with which the logits are done first: as many workgroups as there are places
 // for them take the tiles in turn, each `first` and `stage` times the steps of a tile, in
 // ns.
-enum { kBig, kMiddle, kSmall, kFew, kFewSmall };
+enum { kBig, kMiddle, kSmall, kDeep, kFew, kFewSmall };
 struct Shape {
   int words, rows, places;
   int64_t first, stage;
@@ -1070,12 +1075,13 @@ struct Shape {
 constexpr Shape kShapes[] = {{Big::kWords, Big::kRows, kUnits * Big::kEach, 6000, 1200},
                              {Middle::kWords, Middle::kRows, kUnits * Middle::kEach, 4000, 900},
                              {Small::kWords, Small::kRows, kUnits * Small::kEach, 3000, 700},
+                             {Deep::kWords, Deep::kRows, kUnits * Deep::kEach, 13000, 200},
                              {Few::kWords, Few::kRows, kUnits * Few::kEach, 2000, 1300},
                              {FewSmall::kWords, FewSmall::kRows, kUnits * FewSmall::kEach, 2000, 700}};
 int shape_of(int64_t rows, int64_t words, int64_t c, bool bf16, bool split) {
   int best = 0;
   int64_t least = INT64_MAX;
-  for (int i = split ? kFew : kBig; i <= (split ? kFewSmall : kSmall); ++i) {
+  for (int i = split ? kFew : kBig; i <= (split ? kFewSmall : kDeep); ++i) {
     const Shape& t = kShapes[i];
     const int64_t tiles = ceil_div(words, t.words) * ceil_div(rows, t.rows);
     const int64_t stages = split ? ceil_div(c, kFewStep) : ceil_div(c, kStep) * (bf16 ? 1 : 3);
@@ -1184,7 +1190,8 @@ void logits(const LogitsCall& l, int shape, hipStream_t s) {
   }
   if (shape == kBig) logits<BF, kBackward, Big>(l, s);
   else if (shape == kMiddle) logits<BF, kBackward, Middle>(l, s);
-  else logits<BF, kBackward, Small>(l, s);
+  else if (shape == kSmall) logits<BF, kBackward, Small>(l, s);
+  else logits<BF, kBackward, Deep>(l, s);
 }
 
 template <bool BF>

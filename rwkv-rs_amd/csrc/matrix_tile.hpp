@@ -214,8 +214,11 @@ __device__ __forceinline__ int third_q(int part) { return part == 1 || part == 3
 // LDS holds three stages of one operand and two of the other (kDeepP: three of P). The
 // loop's barrier lies kTail groups of products before a stage's end, when all of the
 // stage has been read: behind it the next stage's first reads and the loads that
-// overwrite this one are issued under the products that are left.
-template <Layout kLayoutP, Layout kLayoutQ, int kP, int kQ, int kWavesP, int kWavesQ, bool kSpread, bool kDeepP, Kind kKind>
+// overwrite this one are issued under the products that are left. With kLead, LDS holds
+// one stage more than that of both: for small tiles, whose products take less time than a
+// load.
+template <Layout kLayoutP, Layout kLayoutQ, int kP, int kQ, int kWavesP, int kWavesQ, bool kSpread, bool kDeepP, Kind kKind,
+          int kLead = 0>
 struct Tile {
   static constexpr int kWaves = kWavesP * kWavesQ, kItemsQ = kQ, kAcross = kWavesP;
   static constexpr int kWaveP = kP / kWavesP, kWaveQ = kQ / kWavesQ;
@@ -223,10 +226,13 @@ struct Tile {
   static_assert(!kSpread || kWaveP % 32 == 0);
   using SideP = Side<kLayoutP, kP, kWaves, kSpread>;
   using SideQ = Side<kLayoutQ, kQ, kWaves, false>;
-  static constexpr int kSlotsP = kDeepP ? 3 : 2, kSlotsQ = kDeepP ? 2 : 3;
+  static constexpr int kSlotsP = kLead ? kLead + 1 : kDeepP ? 3 : 2, kSlotsQ = kLead ? kLead + 1 : kDeepP ? 2 : 3;
   static constexpr int kPlaceQ = kSlotsP * SideP::kBytes;
   static constexpr int kLdsBytes = kPlaceQ + kSlotsQ * SideQ::kBytes;
   static constexpr int kDeepLoads = kDeepP ? SideP::kLoads : SideQ::kLoads;
+  // a wave's loads behind those of the stage that is waited for
+  static constexpr int kBehind = kLead ? (kLead - 1) * (SideP::kLoads + SideQ::kLoads) : kDeepLoads;
+  static_assert(kBehind < 64);
   static constexpr int kParts = kKind == kHalves ? 3 : kKind == kThirds ? kThirdsParts : 1;
   static constexpr int kTail = kTilesP / 2, kBody = 2 * kTilesP - kTail;   // groups of kTilesQ products
   static constexpr int kHeldP = 2;
@@ -362,17 +368,17 @@ struct Tile {
   }
 
   // Behind it this stage is everyone's, and the stage before has been read by everyone.
-  // kBehind: this wave's loads that may still be on their way.
-  template <int kBehind>
+  // kLeft: this wave's loads that may still be on their way.
+  template <int kLeft>
   __device__ __forceinline__ static void arrive() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kBehind) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLeft) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   }
 
   // A sum over the steps [k0, k1), whole stages: begin() asks for the first ones, run()
   // forms it in acc. Between the two, `lds` is free from kFree on.
-  static constexpr int kFree = kDeepP ? 2 * SideP::kBytes : SideP::kBytes;   // a slot that begin() leaves
+  static constexpr int kFree = (kSlotsP - 1) * SideP::kBytes;   // a slot that begin() leaves
   struct Work {
     Place a;
     int k0, k1;
@@ -409,9 +415,14 @@ struct Tile {
       for (int n = 0; n < SideQ::kLoads; ++n) bring_q(n, lds, w.a, from, w.next_q);
       w.next_q.advance(k0, k1);
     };
-    all_p();
-    all_q();
-    kDeepP ? all_p() : all_q();
+    if constexpr (kLead > 0) {
+#pragma unroll
+      for (int s = 0; s < kLead; ++s) all_p(), all_q();
+    } else {
+      all_p();
+      all_q();
+      kDeepP ? all_p() : all_q();
+    }
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -437,7 +448,7 @@ struct Tile {
     };
     auto one = [&](auto first) {
       turn();
-      arrive<kDeepLoads>();
+      arrive<kBehind>();
       step<decltype(first)::value>(lds + w.next_p.slot * SideP::kBytes, lds + kPlaceQ + w.next_q.slot * SideQ::kBytes,
                                    lds + slot_p * SideP::kBytes, lds + kPlaceQ + slot_q * SideQ::kBytes, held, w.a, w.next_p,
                                    w.next_q);
@@ -450,7 +461,7 @@ struct Tile {
     } else {
       for (int s = 0; s < stages; ++s) {   // the same loads in the same order, and the same barriers
         turn();
-        arrive<kDeepLoads>();
+        arrive<kBehind>();
         const Buffer from_p = w.a.from(w.next_p), from_q = w.a.from(w.next_q, 0);
         auto all_p = [&] {
 #pragma unroll

@@ -523,3 +523,12 @@ def test_in_a_graph_with_much_work(dtype):
         torch.cuda.synchronize()
         for p, q in zip(out, step()):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("rows,vocab,c", [(40, 500, 2048), (65, 130, 4000), (1, 3, 5000), (300, 513, 1472), (7, 70, 2999)])
+def test_few_tiles_of_many_channels(rows, vocab, c, dtype):
+    announce("linear loss, many channels", rows, vocab, c, dtype)
+    x, w, t = make(rows, vocab, c, dtype, seed=71)
+    t[1::5] = -100
+    check(x, w, t, torch.rand(rows, device=DEV) + 0.1, rows)
