@@ -987,12 +987,16 @@ struct Plan {
   int64_t splits, share, row_splits, row_share;
   bool hidden_first;
 };
-// when `more` tiles of `more_each` are done behind `tiles` longer ones of `each`
-int64_t finish(int64_t tiles, int64_t each, int64_t more, int64_t more_each) {
-  const int64_t whole = tiles / kUnits * each, late = tiles % kUnits, at = whole + (late ? each : 0);
-  for (int64_t k = std::max((at - whole) / more_each, more / kUnits);; ++k) {   // before, too few are done
+// When `all_more` tiles of `more_each` are done behind `all` longer ones of `each`. An XCD
+// has an eighth of each, whatever the others do: 102 and 768 tiles of 512 x 768 x 65536 look
+// better than 96 and 768 on 256 units (65 stages and 68), but not on 32 (214 us and 175).
+int64_t finish(int64_t all, int64_t each, int64_t all_more, int64_t more_each) {
+  constexpr int64_t kOwn = kUnits / kXcds;
+  const int64_t tiles = ceil_div(all, kXcds), more = ceil_div(all_more, kXcds);
+  const int64_t whole = tiles / kOwn * each, late = tiles % kOwn, at = whole + (late ? each : 0);
+  for (int64_t k = std::max((at - whole) / more_each, more / kOwn);; ++k) {   // before, too few are done
     const int64_t t = std::max(at, whole + k * more_each);
-    if ((kUnits - late) * ((t - whole) / more_each) + late * ((t - at) / more_each) >= more) return t;
+    if ((kOwn - late) * ((t - whole) / more_each) + late * ((t - at) / more_each) >= more) return t;
   }
 }
 Plan plan(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
