@@ -36,7 +36,7 @@
  * fp32 operands are multiplied as two fp16 numbers each, after a power of two that
  * brings the operand's largest magnitude to 2^13 .. 2^14: 22 bits of each element, but
  * never finer than 2^-38 of that largest magnitude, three products, fp32 sums. Where
- * there are few rows and many weights, as three bf16 numbers each that hold an element
+ * there are few rows and many words, as three bf16 numbers each that hold an element
  * whole, of nine products the six of 2^-15 and more.
  *
  * Operands are aligned to their elements, and where c is a multiple of 8, hidden,

@@ -229,8 +229,9 @@ __global__ __launch_bounds__(kWide) void survey_kernel(const SurveyCall c) {
 }
 
 // One array made of another: rows of `padded` elements, zeros behind the c there are.
-// bf16 as it is; bf16 to fp16; fp32 to two of fp16, or to three of bf16
-enum PackKind { kCopy, kToHalf, kToHalves, kToThirds };
+// bf16 as it is; bf16 to fp16; fp32 to two of fp16, or to three of bf16; fp32 as it is, in
+// rows of whole eights
+enum PackKind { kCopy, kToHalf, kToHalves, kToThirds, kEights };
 struct PackJob {
   const void* from;
   char* to;
@@ -267,11 +268,22 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
   if (static_cast<int>(blockIdx.y) >= c.jobs) return;
   if (job.kind == kToThirds) {
     if (blockIdx.x == 0 && threadIdx.x == 0) c.scalars->exponent[0] = c.scalars->exponent[1] = 0;
-  } else if (job.kind != kCopy) {
+  } else if (job.kind != kCopy && job.kind != kEights) {
     exponent = exponent_of(block_max<4>(c.largest[job.which * kMaxBlocks + threadIdx.x]));
     if (blockIdx.x == 0 && threadIdx.x == 0) c.scalars->exponent[job.which] = exponent;
   }
-  const int lane = threadIdx.x & 63, pieces = c.padded / 8;
+  const int lane = threadIdx.x & 63;
+  if (job.kind == kEights) {
+    const int64_t eights = (c.c + 7) / 8 * 8;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); row < job.rows; row += gridDim.x * int64_t{4}) {
+      const float* const from = static_cast<const float*>(job.from) + row * c.c;
+      float* const to = reinterpret_cast<float*>(job.to) + row * eights;
+#pragma unroll 4
+      for (int i = lane; i < eights; i += 64) to[i] = i < c.c ? from[i] : 0.f;
+    }
+    return;
+  }
+  const int pieces = c.padded / 8;
   const int64_t plane = job.rows * c.padded;
   const bool whole = c.c % 8 == 0;
   const bool some = c.index && job.which == 0;
@@ -340,7 +352,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
 // ------------------------------------------------------------------------- logits
 struct LogitsCall {
   Matrix x, w;
-  int rows, vocab, c, steps;     // steps: c up to whole stages
+  int rows, vocab, c, steps;     // c up to whole eights, and up to whole stages
   int first, words;              // the piece of the vocabulary, whole tiles
   const int *index, *count;      // the rows that x's are, and how many; null: all as they are
   const Scalars* scalars;
@@ -920,15 +932,17 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t* to, int64_t words,
 }
 
 // ------------------------------------------------------------------ plan, workspace
-// fp32 operands with few rows and a w that is nearly all there is to read: w is read where
-// it is, three times in the two calls, where packing it to fp16 reads or writes it eleven
-// times in all. Against the packed form, us for both calls: 1 to 64 rows of 768 with 65536
-// words 230 and 480, 128 rows 352 and 514, 192 rows 490 and 531, 256 rows 634 and 571; 64 of
-// 2048 with 8000 words 163 and 202, 192 rows 271 and 212; 64 of 512 with 2000 words, whose
-// launches are what counts, 78 and 64. Rows of w that begin at whole 16 bytes.
-constexpr int64_t kFewRows = 128, kLargeWeight = int64_t{1} << 22;
+// fp32 operands with few rows and many words, w being nearly all there is to read: w is read
+// where it is, three times in the two calls, where packing it to fp16 reads or writes it
+// eleven times in all. Against the packed form, us for both calls: 1 to 64 rows of 768 with
+// 65536 words 230 and 480, 128 rows 352 and 514, 192 rows 490 and 531, 256 rows 634 and 571;
+// 64 of 768 with 16000 words 107 and 131, with 8000 97 and 91; 64 of 4096 with 4000 242 and
+// 229; 64 of 512 with 2000, whose launches are what counts, 78 and 64. Rows that do not begin
+// at whole 16 bytes are copied to rows of whole eights first: 40 of 333 with 100000 words 396
+// and 517, 64 of 1001 with 65536 777 and 921, with 20000 294 and 276.
+constexpr int64_t kFewRows = 128, kManyWords = 12288, kLargeWeight = int64_t{1} << 22;
 bool few(int64_t rows, int64_t vocab, int64_t c, bool bf16) {
-  return !bf16 && rows <= kFewRows && vocab * c >= kLargeWeight && c % 8 == 0;
+  return !bf16 && rows <= kFewRows && vocab >= kManyWords && vocab * c >= (c % 8 ? 6 : 1) * kLargeWeight;
 }
 int64_t planes_of(int64_t rows, int64_t vocab, int64_t c, bool bf16) { return bf16 ? 1 : few(rows, vocab, c, bf16) ? 3 : 2; }
 
@@ -968,7 +982,11 @@ Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward
     p.count = take(p.end, 4);
   }
   if (packed(c, bf16) || numbered(rows, vocab, c, bf16)) p.x = take(p.end, planes * p.x_plane);
-  if (packed(c, bf16) && !few(rows, vocab, c, bf16)) p.w = take(p.end, planes * p.w_plane);
+  if (few(rows, vocab, c, bf16)) {
+    if (c % 8 != 0) p.w = take(p.end, vocab * up(c, 8) * 4);
+  } else if (packed(c, bf16)) {
+    p.w = take(p.end, planes * p.w_plane);
+  }
   if (bf16 && backward) p.x_half = take(p.end, p.x_plane);
   return p;
 }
@@ -1139,6 +1157,10 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
     return Matrix{c.workspace + to, padded * 2, plane};
   };
   if (packed(c.c, BF) || r.index) o.x = pack(c.hidden, p.x, c.rows, BF ? kCopy : split ? kToThirds : kToHalves, 0, p.x_plane);
+  if (split && c.c % 8 != 0) {
+    k.job[k.jobs++] = PackJob{c.weight, c.workspace + p.w, c.vocab, kEights, 1};
+    o.w = Matrix{c.workspace + p.w, up(c.c, 8) * 4, 0};
+  }
   if (packed(c.c, BF) && !split) o.w = pack(c.weight, p.w, c.vocab, BF ? kCopy : kToHalves, 1, p.w_plane);
   o.x_half = o.x;
   if (BF && b && b->weight_grad) o.x_half = pack(c.hidden, p.x_half, c.rows, kToHalf, 0, 0);
@@ -1209,7 +1231,7 @@ void forward(const ForwardCall& c, hipStream_t s) {
   l.count = o.count;
   l.rows = static_cast<int>(c.rows);
   l.vocab = static_cast<int>(c.vocab);
-  l.c = static_cast<int>(c.c);
+  l.c = static_cast<int>(up(c.c, 8));
   l.steps = static_cast<int>(up(c.c, few(c.rows, c.vocab, c.c, BF) ? kFewStep : kStep));
   l.words = static_cast<int>(up(c.vocab, kWholeWords));
   l.scalars = reinterpret_cast<const Scalars*>(c.workspace + f.operands.scalars);
@@ -1246,7 +1268,7 @@ void backward(const BackwardCall& c, hipStream_t s) {
   l.count = o.count;
   l.rows = static_cast<int>(c.rows);
   l.vocab = static_cast<int>(c.vocab);
-  l.c = static_cast<int>(c.c);
+  l.c = static_cast<int>(up(c.c, 8));
   l.steps = static_cast<int>(up(c.c, few(c.rows, c.vocab, c.c, BF) ? kFewStep : kStep));
   l.scalars = scalars;
   l.targets = c.targets;

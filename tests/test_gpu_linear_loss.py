@@ -532,3 +532,13 @@ def test_few_tiles_of_many_channels(rows, vocab, c, dtype):
     x, w, t = make(rows, vocab, c, dtype, seed=71)
     t[1::5] = -100
     check(x, w, t, torch.rand(rows, device=DEV) + 0.1, rows)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("rows,vocab,c", [(3, 1 << 20, 5), (64, 13000, 333), (20, 33000, 130)])
+def test_many_words_of_few_channels(rows, vocab, c, dtype):
+    """D is far below its floor for most words: 2^-38 of the largest factor."""
+    announce("linear loss, many words", rows, vocab, c, dtype)
+    x, w, t = make(rows, vocab, c, dtype, seed=rows + c)
+    t[1::7] = -100
+    check(x, w, t, torch.rand(rows, device=DEV) + 0.1, rows)

@@ -206,3 +206,51 @@ def test_rows_that_begin_anywhere(rows, vocab, c, dtype):
         results.append((row[0].clone(), fdx[off:off + x.numel()].clone(), fdw[off:off + w.numel()].clone()))
     for p, q in zip(*results):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("rows,vocab,c", [(40, 100000, 333), (64, 5000, 1001), (128, 16500, 514), (1, 66, 65535), (100, 9000, 1260)])
+def test_rows_of_no_whole_eights(rows, vocab, c):
+    announce("linear loss, few rows of no whole eights", rows, vocab, c)
+    x, w, t = make(rows, vocab, c, torch.float32, seed=rows + c)
+    t[1::7] = -100
+    check(x, w, t, torch.rand(rows, device=DEV) + 0.1, rows)
+
+
+@pytest.mark.parametrize("rows,vocab,c", [(40, 75601, 333), (64, 25200, 1001), (1, 1 << 22, 7), (128, 50001, 514), (100, 20011, 1260), (9, 12288, 2051)])
+def test_copied_rows(rows, vocab, c):
+    """Rows that begin anywhere, of words enough to be copied to rows that do not."""
+    announce("linear loss, few rows, copied", rows, vocab, c)
+    x, w, t = make(rows, vocab, c, torch.float32, seed=rows + c)
+    t[1::7] = -100
+    check(x, w, t, torch.rand(rows, device=DEV) + 0.1, rows)
+
+
+@pytest.mark.parametrize("rows,vocab,c", [(17, 12288, 1032), (64, 13000, 1000), (100, 16384, 2056), (3, 12300, 4104), (128, 12289, 344)])
+def test_many_channels(rows, vocab, c):
+    announce("linear loss, few rows, many channels", rows, vocab, c)
+    x, w, t = make(rows, vocab, c, torch.float32, seed=rows + c)
+    t[1::7] = -100
+    check(x, w, t, torch.rand(rows, device=DEV) + 0.1, rows)
+
+
+@pytest.mark.parametrize("c", [512, 1900])
+def test_in_a_graph_of_many_words(c):
+    announce("linear loss, few rows, graph, many words", c)
+    rows, vocab = 70, 14000
+    x, w, t = make(rows, vocab, c, torch.float32, seed=43)
+    g = torch.rand(rows, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(x, w, t, g, rows)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(x, w, t, g, rows)
+    for seed in range(4):
+        x2, w2, t2 = make(rows, vocab, c, torch.float32, seed=200 + seed)
+        x.copy_(x2), w.copy_(w2), t.copy_(t2)
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(out, run(x, w, t, g, rows)):
+            assert torch.equal(p, q)
