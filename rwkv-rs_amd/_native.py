@@ -91,6 +91,10 @@ W4_EXPORTS = ("rwkv_w4_packed_bytes", "rwkv_w4_scales_bytes", "rwkv_w4_quantize"
 DECODE_W4_EXPORTS = ("rwkv_decode_cell_w4", "rwkv_decode_head_w4")
 SCORES_EXPORTS = ("rwkv_token_scores_forward", "rwkv_token_scores_backward")
 
+# and of include/rwkv_lm_loss_ignore.h
+LOSS_IGNORE_EXPORTS = ("rwkv_cross_entropy_l2wrap_ignore_forward",
+                       "rwkv_cross_entropy_l2wrap_ignore_backward")
+
 # and of include/rwkv_linear_loss.h
 LINEAR_LOSS_EXPORTS = ("rwkv_linear_loss_forward_workspace_bytes",
                        "rwkv_linear_loss_backward_workspace_bytes",
@@ -148,6 +152,9 @@ _SIGNATURES = {
     "rwkv_cross_entropy_l2wrap_forward": ([_P] * 2 + [_I64] * 2 + [_INT] + [_P] * 5, _INT),
     "rwkv_cross_entropy_l2wrap_backward": ([_P] * 6 + [ctypes.c_float] + [_I64] * 2 + [_INT]
                                            + [_P] * 2, _INT),
+    "rwkv_cross_entropy_l2wrap_ignore_forward": ([_P] * 2 + [_I64] * 2 + [_INT, _I64] + [_P] * 5, _INT),
+    "rwkv_cross_entropy_l2wrap_ignore_backward": ([_P] * 6 + [ctypes.c_float] + [_I64] * 2 + [_INT, _I64]
+                                                  + [_P] * 2, _INT),
     "rwkv_w4_packed_bytes": ([_I64] * 2, _I64),
     "rwkv_w4_scales_bytes": ([_I64] * 3, _I64),
     "rwkv_w4_quantize": ([_P] + [_I64] * 3 + [_INT] + [_P] * 3, _INT),

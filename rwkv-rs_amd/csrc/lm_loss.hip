@@ -21,6 +21,10 @@
 // by one instead of in pieces, 8192 x 65529 took 545 + 1,271 us in bf16 and 898
 // + 2,070 in fp32; in pieces 189 + 450 and 361 + 916 (its rows' edges share
 // cache lines with their neighbours').
+//
+// Where rows are ignored, a block of such a row reads nothing: its forward writes
+// zeros and ends, its backward only stores (kIgnores: in the backward a form of its
+// own, so that the one without ignored rows has no question more an element).
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -132,6 +136,13 @@ __global__ __launch_bounds__(kWidth) void xent_forward_kernel(XentArgs a) {
   constexpr bool kWhole = kForm == kWholePieces;
   const RowSpan span = kForm == kElements ? RowSpan{0, V, 0} : row_span<BF, kWhole>(a.logits, base, V);
   const int tid = threadIdx.x;
+  if (a.ignores && a.targets[row] == a.ignore_index) {   // the whole block's row
+    if (tid == 0) {
+      a.row_loss[row] = a.row_lse[row] = a.row_max[row] = 0.f;
+      a.row_argmax[row] = 0;
+    }
+    return;
+  }
   Run run{-INFINITY, 0.f, INT_MAX};
   // a logit of -inf adds nothing (and is no maximum), NaN makes the sum NaN
   auto single = [&](int64_t j) {
@@ -192,7 +203,7 @@ __global__ __launch_bounds__(kWidth) void xent_forward_kernel(XentArgs a) {
 // kPieces: the rows of the logits and of their gradient begin alike within 16
 // bytes. kShared: blocks (row, y) take every gridDim.y-th run of kThreads pieces
 // or elements.
-template <bool BF, int kForm, bool kShared>
+template <bool BF, int kForm, bool kShared, bool kIgnores>
 __global__ __launch_bounds__(kThreads) void xent_backward_kernel(XentArgs a) {
   const int64_t row = blockIdx.x;
   const int64_t V = a.vocab, base = row * V;
@@ -201,13 +212,16 @@ __global__ __launch_bounds__(kThreads) void xent_backward_kernel(XentArgs a) {
   const int64_t t = a.targets[row], am = a.argmax[row];
   const int64_t first = (kShared ? static_cast<int64_t>(blockIdx.y) * kThreads : 0) + threadIdx.x;
   const int64_t stride = kShared ? static_cast<int64_t>(gridDim.y) * kThreads : kThreads;
+  const bool dead = kIgnores && t == a.ignore_index;
   auto grad = [&](float x, int64_t j) {
     float d = g * __expf(x - lse);
     if (j == t) d -= g;
     if (j == am) d += l2;
     return d;
   };
-  auto single = [&](int64_t j) { store_one<BF>(a.logits_grad, base + j, grad(load_one<BF>(a.logits, base + j), j)); };
+  auto single = [&](int64_t j) {
+    store_one<BF>(a.logits_grad, base + j, dead ? 0.f : grad(load_one<BF>(a.logits, base + j), j));
+  };
   if constexpr (kForm == kElements) {
     for (int64_t j = first; j < V; j += stride) single(j);
   } else {
@@ -216,9 +230,12 @@ __global__ __launch_bounds__(kThreads) void xent_backward_kernel(XentArgs a) {
     if (!kWhole && first < span.head) single(first);
     for (int64_t q = first; q < span.pieces; q += stride) {
       const int64_t j0 = span.head + q * kPiece;
-      Piece p = load_piece<BF>(a.logits, base + j0);
+      Piece p{};
+      if (!dead) {
+        p = load_piece<BF>(a.logits, base + j0);
 #pragma unroll
-      for (int k = 0; k < kPiece; ++k) p.v[k] = grad(p.v[k], j0 + k);
+        for (int k = 0; k < kPiece; ++k) p.v[k] = grad(p.v[k], j0 + k);
+      }
       store_piece<BF>(a.logits_grad, base + j0, p);
     }
     if (!kWhole && span.tail + first < V) single(span.tail + first);
@@ -274,11 +291,11 @@ hipError_t forward(const XentArgs& a, hipStream_t s) {
 constexpr int64_t kFillBlocks = 2048;
 constexpr int64_t kShareRowsF32 = 256;
 
-template <bool BF, bool kShared>
+template <bool BF, bool kShared, bool kIgnores>
 hipError_t backward(const XentArgs& a, int form, unsigned split, hipStream_t s) {
-  auto* const kernel = form == kElements ? xent_backward_kernel<BF, kElements, kShared>
-                       : form == kPieces ? xent_backward_kernel<BF, kPieces, kShared>
-                                         : xent_backward_kernel<BF, kWholePieces, kShared>;
+  auto* const kernel = form == kElements ? xent_backward_kernel<BF, kElements, kShared, kIgnores>
+                       : form == kPieces ? xent_backward_kernel<BF, kPieces, kShared, kIgnores>
+                                         : xent_backward_kernel<BF, kWholePieces, kShared, kIgnores>;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.rows), split), dim3(kThreads), 0, s, a);
   return hipGetLastError();
 }
@@ -290,8 +307,9 @@ hipError_t backward(const XentArgs& a, hipStream_t s) {
   const int64_t runs = (a.vocab / (form == kElements ? 1 : kPiece) + kThreads - 1) / kThreads;
   const int64_t fill = BF || a.rows <= kShareRowsF32 ? kFillBlocks / a.rows : 1;
   const int64_t split = std::max<int64_t>(1, std::min<int64_t>(fill, runs));
-  if (split > 1) return backward<BF, true>(a, form, static_cast<unsigned>(split), s);
-  return backward<BF, false>(a, form, 1, s);
+  const unsigned y = static_cast<unsigned>(split);
+  if (split > 1) return a.ignores ? backward<BF, true, true>(a, form, y, s) : backward<BF, true, false>(a, form, y, s);
+  return a.ignores ? backward<BF, false, true>(a, form, 1, s) : backward<BF, false, false>(a, form, 1, s);
 }
 
 }  // namespace

@@ -1,6 +1,7 @@
-// C ABI of the fused cross entropy + l2wrap (include/rwkv_lm_loss.h):
+// C ABI of the fused cross entropy + l2wrap (include/rwkv_lm_loss.h, include/
+// rwkv_lm_loss_ignore.h):
 // argument validation on the host, before any HIP call, then dispatch.
-#include "../../include/rwkv_lm_loss.h"
+#include "../../include/rwkv_lm_loss_ignore.h"
 
 #include <hip/hip_runtime.h>
 
@@ -54,13 +55,10 @@ int check_common(const void* logits, const int64_t* targets, int64_t rows, int64
   return WKV7_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-int rwkv_cross_entropy_l2wrap_forward(const void* logits, const int64_t* targets, int64_t rows,
-                                      int64_t vocab, int dtype, float* row_loss, float* row_lse,
-                                      float* row_max, int32_t* row_argmax, void* stream) {
+// ignore_index: null where no row is ignored
+int forward(const void* logits, const int64_t* targets, int64_t rows, int64_t vocab, int dtype,
+            const int64_t* ignore_index, float* row_loss, float* row_lse, float* row_max,
+            int32_t* row_argmax, void* stream) {
   if (int rc = check_common(logits, targets, rows, vocab, dtype)) return rc;
   if (rows > 0 && (!row_loss || !row_lse || !row_max || !row_argmax)) return WKV7_ERR_NULL_POINTER;
   for (const void* p : {static_cast<const void*>(row_loss), static_cast<const void*>(row_lse),
@@ -76,6 +74,8 @@ int rwkv_cross_entropy_l2wrap_forward(const void* logits, const int64_t* targets
   a.rows = rows;
   a.vocab = vocab;
   a.bf16 = dtype == WKV7_DTYPE_BF16;
+  a.ignores = ignore_index != nullptr;
+  a.ignore_index = ignore_index ? *ignore_index : 0;
   a.row_loss = row_loss;
   a.row_lse = row_lse;
   a.row_max = row_max;
@@ -83,11 +83,10 @@ int rwkv_cross_entropy_l2wrap_forward(const void* logits, const int64_t* targets
   return wkv7::hip_status(rwkv_loss::launch_xent_forward(a, static_cast<hipStream_t>(stream)));
 }
 
-int rwkv_cross_entropy_l2wrap_backward(const void* logits, const int64_t* targets,
-                                       const float* row_lse, const float* row_max,
-                                       const int32_t* row_argmax, const float* row_loss_grad,
-                                       float l2wrap_scale, int64_t rows, int64_t vocab, int dtype,
-                                       void* logits_grad, void* stream) {
+int backward(const void* logits, const int64_t* targets, const float* row_lse, const float* row_max,
+             const int32_t* row_argmax, const float* row_loss_grad, float l2wrap_scale,
+             int64_t rows, int64_t vocab, int dtype, const int64_t* ignore_index,
+             void* logits_grad, void* stream) {
   if (int rc = check_common(logits, targets, rows, vocab, dtype)) return rc;
   if (!(l2wrap_scale == l2wrap_scale) || l2wrap_scale == INFINITY || l2wrap_scale == -INFINITY)
     return WKV7_ERR_SHAPE;
@@ -109,6 +108,8 @@ int rwkv_cross_entropy_l2wrap_backward(const void* logits, const int64_t* target
   a.rows = rows;
   a.vocab = vocab;
   a.bf16 = dtype == WKV7_DTYPE_BF16;
+  a.ignores = ignore_index != nullptr;
+  a.ignore_index = ignore_index ? *ignore_index : 0;
   a.lse = row_lse;
   a.max = row_max;
   a.argmax = row_argmax;
@@ -116,6 +117,44 @@ int rwkv_cross_entropy_l2wrap_backward(const void* logits, const int64_t* target
   a.l2wrap_scale = l2wrap_scale;
   a.logits_grad = logits_grad;
   return wkv7::hip_status(rwkv_loss::launch_xent_backward(a, static_cast<hipStream_t>(stream)));
+}
+
+}  // namespace
+
+extern "C" {
+
+int rwkv_cross_entropy_l2wrap_forward(const void* logits, const int64_t* targets, int64_t rows,
+                                      int64_t vocab, int dtype, float* row_loss, float* row_lse,
+                                      float* row_max, int32_t* row_argmax, void* stream) {
+  return forward(logits, targets, rows, vocab, dtype, nullptr, row_loss, row_lse, row_max,
+                 row_argmax, stream);
+}
+
+int rwkv_cross_entropy_l2wrap_backward(const void* logits, const int64_t* targets,
+                                       const float* row_lse, const float* row_max,
+                                       const int32_t* row_argmax, const float* row_loss_grad,
+                                       float l2wrap_scale, int64_t rows, int64_t vocab, int dtype,
+                                       void* logits_grad, void* stream) {
+  return backward(logits, targets, row_lse, row_max, row_argmax, row_loss_grad, l2wrap_scale, rows,
+                  vocab, dtype, nullptr, logits_grad, stream);
+}
+
+int rwkv_cross_entropy_l2wrap_ignore_forward(const void* logits, const int64_t* targets,
+                                             int64_t rows, int64_t vocab, int dtype,
+                                             int64_t ignore_index, float* row_loss, float* row_lse,
+                                             float* row_max, int32_t* row_argmax, void* stream) {
+  return forward(logits, targets, rows, vocab, dtype, &ignore_index, row_loss, row_lse, row_max,
+                 row_argmax, stream);
+}
+
+int rwkv_cross_entropy_l2wrap_ignore_backward(const void* logits, const int64_t* targets,
+                                              const float* row_lse, const float* row_max,
+                                              const int32_t* row_argmax, const float* row_loss_grad,
+                                              float l2wrap_scale, int64_t rows, int64_t vocab,
+                                              int dtype, int64_t ignore_index, void* logits_grad,
+                                              void* stream) {
+  return backward(logits, targets, row_lse, row_max, row_argmax, row_loss_grad, l2wrap_scale, rows,
+                  vocab, dtype, &ignore_index, logits_grad, stream);
 }
 
 }  // extern "C"

@@ -16,6 +16,8 @@ struct XentArgs {
   const int64_t* targets;    // [rows]
   int64_t rows, vocab;
   bool bf16;
+  bool ignores;              // rows whose target is ignore_index have no loss
+  int64_t ignore_index;
   float *row_loss, *row_lse, *row_max;   // forward outputs
   int32_t* row_argmax;
   const float *lse, *max;                // backward inputs (the forward's outputs)

@@ -17,6 +17,8 @@ tiles, twice, and neither they nor their gradient are ever whole in memory.
 
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -29,15 +31,17 @@ IGNORE_INDEX = -100      # a target that is not learned, as torch's cross entrop
 
 class _CrossEntropyL2Wrap(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, targets, num_tokens):
+    def forward(ctx, logits, targets, num_tokens, ignore_index):
         rows, vocab = logits.shape
         dev = logits.device
         loss, lse, mx = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(3))
         arg = torch.empty(rows, dtype=torch.int32, device=dev)
-        _native.call("rwkv_cross_entropy_l2wrap_forward", _ptr(logits), _ptr(targets), rows,
-                     vocab, _code(logits.dtype), _ptr(loss), _ptr(lse), _ptr(mx), _ptr(arg),
+        name, ignore = _form(ignore_index)
+        _native.call(name + "_forward", _ptr(logits), _ptr(targets), rows,
+                     vocab, _code(logits.dtype), *ignore, _ptr(loss), _ptr(lse), _ptr(mx), _ptr(arg),
                      _stream(dev))
         ctx.save_for_backward(logits, targets, lse, mx, arg)
+        ctx.ignore_index = ignore_index
         ctx.scale = L2WRAP_FACTOR / num_tokens if num_tokens > 0 else 0.0
         return loss
 
@@ -47,29 +51,46 @@ class _CrossEntropyL2Wrap(torch.autograd.Function):
         rows, vocab = logits.shape
         g = dloss.to(torch.float32).contiguous()
         dlogits = torch.empty_like(logits)
-        _native.call("rwkv_cross_entropy_l2wrap_backward", _ptr(logits), _ptr(targets), _ptr(lse),
+        name, ignore = _form(ctx.ignore_index)
+        _native.call(name + "_backward", _ptr(logits), _ptr(targets), _ptr(lse),
                      _ptr(mx), _ptr(arg), _ptr(g), float(ctx.scale), rows, vocab,
-                     _code(logits.dtype), _ptr(dlogits), _stream(logits.device))
-        return dlogits, None, None
+                     _code(logits.dtype), *ignore, _ptr(dlogits), _stream(logits.device))
+        return dlogits, None, None, None
+
+
+def _form(ignore_index):
+    """The entry points' name and their further argument."""
+    if ignore_index is None:
+        return "rwkv_cross_entropy_l2wrap", ()
+    return "rwkv_cross_entropy_l2wrap_ignore", (ignore_index,)
 
 
 def cross_entropy_l2wrap_rows(logits: torch.Tensor, targets: torch.Tensor,
-                              num_tokens: int) -> torch.Tensor:
+                              num_tokens: int, ignore_index: Optional[int] = None) -> torch.Tensor:
     """Per-row cross entropy of ``logits`` ([rows, vocab], fp32 or bf16) against ``targets`` ([rows] integer), with l2wrap's
     gradient term for ``num_tokens`` tokens in the backward. A target outside
-    [0, vocab) gives its row a NaN loss."""
+    [0, vocab) gives its row a NaN loss, but for ``ignore_index``, where one is given: such
+    a row has loss 0 and no gradient, whatever its logits are."""
     if not logits.is_cuda or not targets.is_cuda:
         raise ValueError("logits and targets must be GPU tensors")
     if logits.dim() != 2 or targets.shape != (logits.shape[0],):
         raise ValueError("logits must be [rows, vocab] and targets [rows]")
     return _CrossEntropyL2Wrap.apply(logits.contiguous(), targets.to(torch.int64).contiguous(),
-                                     int(num_tokens))
+                                     int(num_tokens), None if ignore_index is None else int(ignore_index))
 
 
-def cross_entropy_l2wrap(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+def cross_entropy_l2wrap(logits: torch.Tensor, targets: torch.Tensor,
+                         ignore_index: Optional[int] = None) -> torch.Tensor:
     """``F.cross_entropy(l2wrap(logits, rows), targets)``: the mean over the
-    rows, l2wrap counting every row as a token (model.rs:161-169)."""
-    return cross_entropy_l2wrap_rows(logits, targets, logits.shape[0]).mean()
+    rows, l2wrap counting every row as a token (model.rs:161-169). With an
+    ``ignore_index`` over those whose target it is not (0 when there is none)."""
+    rows = cross_entropy_l2wrap_rows(logits, targets, logits.shape[0], ignore_index)
+    return rows.mean() if ignore_index is None else _mean_of_learned(rows, targets, ignore_index)
+
+
+def _mean_of_learned(rows, targets, ignore_index):
+    # in 64 bits: a narrow type would be compared with ignore_index cut off to it
+    return rows.sum() / (targets.to(torch.int64) != ignore_index).sum().clamp(min=1)
 
 
 # ------------------------------------------- from hidden states and unembedding
@@ -164,5 +185,4 @@ def linear_cross_entropy_l2wrap(hidden: torch.Tensor, weight: torch.Tensor, targ
     mean over the rows that are not ignored (0 when all are), l2wrap counting every
     row as a token."""
     rows = linear_cross_entropy_l2wrap_rows(hidden, weight, targets, hidden.shape[0], ignore_index)
-    # in 64 bits: a narrow type would be compared with ignore_index cut off to it
-    return rows.sum() / (targets.to(torch.int64) != ignore_index).sum().clamp(min=1)
+    return _mean_of_learned(rows, targets, ignore_index)

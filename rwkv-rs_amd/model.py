@@ -584,7 +584,8 @@ class AutoRegressiveModel(nn.Module):
     (``lm_loss.linear_cross_entropy_l2wrap``), needs the "hip" neighbour ops, and
     leaves out targets of ``lm_loss.IGNORE_INDEX``. An unembedding that is no plain
     linear layer without a bias any more (4-bit weights) has its logits formed all the
-    same; that of one is not called, so a hook on it does not run."""
+    same, with those targets left out too; that of one is not called, so a hook on it does
+    not run."""
 
     def __init__(self, vocab_size: int, num_cells: int, embedded_dim: int, num_heads: int,
                  head_size: int = 64, wkv7_dtype: torch.dtype = torch.bfloat16,
@@ -743,7 +744,8 @@ class AutoRegressiveModel(nn.Module):
             return _loss.linear_cross_entropy_l2wrap(hidden, weight.to(dtype), targets.reshape(n))
         logits = self.unembed(x)
         if self.neighbor_ops == "hip":
-            return _loss.cross_entropy_l2wrap(logits.reshape(n, self.vocab_size), targets.reshape(n))
+            return _loss.cross_entropy_l2wrap(logits.reshape(n, self.vocab_size), targets.reshape(n),
+                                              _loss.IGNORE_INDEX if self.loss == "pieces" else None)
         logits = l2wrap(logits.reshape(n, self.vocab_size), n)
         return F.cross_entropy(logits.float(), targets.reshape(n))
 
