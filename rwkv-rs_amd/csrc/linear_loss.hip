@@ -677,15 +677,25 @@ struct HiddenCall {
   const int32_t* row_argmax;
   const __bf16* weight;
 };
-// What the sums are multiplied with.
+// What the sums are multiplied with: one number from 1 to 2, then one power of two, so that
+// nothing on the way is larger or smaller than the result.
 struct Factor {
-  float reference;
+  float mantissa;
   int exponent;
 };
-__device__ __forceinline__ Factor weight_factor(const Scalars* s) { return Factor{s->reference, -(kHalfExponent + s->exponent[0])}; }
+__device__ __forceinline__ Factor factor_of(float reference, int exponent) {
+  const int scale = ilogbf(reference);
+  return Factor{ldexpf(reference, -scale), scale - kHalfExponent - exponent};
+}
+__device__ __forceinline__ f32x4 times(f32x4 v, Factor f) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e] * f.mantissa, f.exponent);
+  return v;
+}
+__device__ __forceinline__ Factor weight_factor(const Scalars* s) { return factor_of(s->reference, s->exponent[0]); }
 template <bool BF>
 __device__ __forceinline__ Factor hidden_factor(const Scalars* s) {
-  return Factor{s->reference, -(kHalfExponent + (BF ? 0 : s->exponent[1]))};
+  return factor_of(s->reference, BF ? 0 : s->exponent[1]);
 }
 template <bool BF>
 __device__ __forceinline__ void finish_hidden(const HiddenCall& c, Factor f, int64_t row, int64_t part_row, int64_t channel, f32x4 v) {
@@ -709,9 +719,7 @@ __device__ __forceinline__ void finish_hidden(const HiddenCall& c, Factor f, int
       for (int e = 0; e < 4; ++e) v[e] += r != 0.f ? r * static_cast<float>(w[e]) : 0.f;
     }
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], f.exponent) * f.reference;
-  store4<BF>(c.grad, row * c.c + channel, v, c.c - channel, whole);
+  store4<BF>(c.grad, row * c.c + channel, times(v, f), c.c - channel, whole);
 }
 
 constexpr int kGradTile = 256;   // words or rows of a gradient's tile
@@ -753,9 +761,7 @@ __device__ __forceinline__ void place(int at, int channel_tiles, int others, int
 // dw of four channels from its sum, in the operands' type.
 template <bool BF>
 __device__ __forceinline__ void finish_weight(void* grad, Factor f, int64_t word, int64_t channel, int64_t c, f32x4 v) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], f.exponent) * f.reference;
-  store4<BF>(grad, word * c + channel, v, c - channel, c % 8 == 0);
+  store4<BF>(grad, word * c + channel, times(v, f), c - channel, c % 8 == 0);
 }
 
 // A tile of dw, of the piece's words over a share of the rows: steps are rows; those past

@@ -1,0 +1,85 @@
+"""The loss from hidden states at the ends of its ranges: rows of very different weight,
+operands and row gradients near the ends of their types, logits far from zero. Against
+float64 formulas on the GPU.
+
+Errors are bounded element by element as in test_gpu_linear_loss.py, whose docstring
+derives them, but for what is held to a fixed step: with f_r the larger of a row's |g_r|
+and |l2wrap term|, and F the largest of them,
+
+* D is held over 2^e m, e the row's own exponent (2^e <= f_r) and 1 <= m < 2, at 2^13: half
+  of fp16's last step, 2^-25, is 2^-37 f_r or less;
+* what the weight gradient multiplies with D is x 2^(e - E), 2^E <= F, at 2^13 for x's
+  largest: half a step is 2^(E - e) 2^-38 max|x|, and 2^(E - e) <= 2 F / f_r;
+* a result below its type's normal numbers is rounded by half its last step (bf16 2^-134).
+"""
+
+import pytest
+import torch
+
+from conftest import announce, load_pkg
+from test_gpu_linear_loss import DEV, U, logit_error, make
+
+pytestmark = pytest.mark.gpu
+ll = load_pkg().lm_loss
+
+
+def run(x, w, t, g, num_tokens):
+    a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = ll.linear_cross_entropy_l2wrap_rows(a, b, t, num_tokens)
+    return (loss.detach(), *torch.autograd.grad(loss, (a, b), g))
+
+
+def check_gradients(x, w, t, g, num_tokens):
+    """Each row of the hidden gradient within bounds of that row's own size."""
+    (rows, c), vocab = x.shape, w.shape[0]
+    loss, dx, dw = run(x, w, t, g, num_tokens)
+    dead = (t == -100)[:, None]
+    x64, w64 = torch.where(dead, 0.0, x.double()), w.double()
+    z = x64 @ w64.t()
+    m, top = z.max(1, keepdim=True)
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    at = torch.where(dead, 0, t[:, None])
+    ez = logit_error(torch.where(dead, torch.zeros_like(x), x), w)
+    e_lse = ez + (32 + 3 + -(-vocab // 1024) + 17) * 2 * U + 2.0 ** -20 + 2 * U * lse.abs()
+    gd, s = torch.where(dead, 0.0, g.double()[:, None]), 1e-4 / num_tokens if num_tokens else 0.0
+    wrap = torch.where(dead, 0.0, s * m)
+    share = gd * torch.exp(z - lse)
+    d = share.scatter_add(1, at, -gd).scatter_add(1, top, wrap)
+    factor = torch.maximum(gd.abs(), wrap.abs())
+    largest = factor.max()
+    de = share.abs() * (ez + e_lse + 2.0 ** -19) + 4 * U * (share.abs() + d.abs())
+    de = de.scatter_add(1, at, gd.abs() * 4 * U).scatter_add(1, top, wrap.abs() * 8 * U + s * ez)
+    bf = x.dtype == torch.bfloat16
+    held = d.abs() * (2.0 ** -11 if bf else 2.0 ** -22) + factor * 2.0 ** -37
+    again = d.abs() * (2.0 ** -8 if bf else 0.0)
+    again = again.scatter(1, at, 0.0).scatter(1, top, 0.0)
+    out, of = (2.0 ** -8, 0.0) if bf else (2 * U, 2.0 ** -22)
+    last = torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps / 2 + 1e-44
+    size = d.abs() @ w64.abs()
+    exact = d @ w64
+    limit = (de + held + again) @ w64.abs() + of * size + 2.0 ** -38 * w64.abs().max() * d.abs().sum(1, keepdim=True)
+    limit += size * ((3 * vocab + 64) * 2 * U + 2.0 ** -22) + exact.abs() * out + last
+    miss = (dx.double() - exact).abs()
+    assert (miss <= limit).all(), float((miss / limit).max())
+    exact, size = d.t() @ x64, d.abs().t() @ x64.abs()
+    step = (d.abs() / torch.where(factor > 0, factor, 1.0)).sum(0)[:, None] * (largest * 2.0 ** -37 * x64.abs().max())
+    limit = (de + held).t() @ x64.abs() + of * size + step + size * ((3 * rows + 64) * 2 * U + 2.0 ** -22)
+    limit += exact.abs() * out + last
+    miss = (dw.double() - exact).abs()
+    assert (miss <= limit).all(), float((miss / limit).max())
+    return loss, dx, dw
+
+
+@pytest.mark.parametrize("dtype,scale_x,scale_w,size", [
+    (torch.float32, 120, -120, -10), (torch.float32, -120, 120, -10), (torch.float32, 110, -110, 6), (torch.float32, -124, 110, 10),
+    (torch.bfloat16, 120, -120, -10), (torch.bfloat16, -100, 100, -10), (torch.bfloat16, -124, 105, 10)])
+def test_operands_near_the_ends_of_their_type(dtype, scale_x, scale_w, size):
+    """With row gradients that bring the result back: 1024 rows of 2^-10 whose gradient
+    adds up at one word to the size of the operand."""
+    announce("linear loss, operands near the ends", dtype, scale_x, scale_w, size)
+    x, w, t = make(1024, 50, 64, torch.float32, seed=5)
+    t[:] = 7
+    x, w = (x.abs() * 2.0 ** scale_x).to(dtype), (w * 2.0 ** scale_w).to(dtype)
+    g = torch.full((1024,), 2.0 ** size, device=DEV)
+    loss, dx, dw = check_gradients(x, w, t, g, 0)
+    assert loss.isfinite().all() and dx.isfinite().all() and dw.isfinite().all()
