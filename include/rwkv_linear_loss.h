@@ -24,14 +24,16 @@
  * in dtype, each rounded once; either pointer may be NULL (not wanted). A row
  * whose target is ignore_index has D = 0; a target otherwise outside [0, vocab)
  * no target term. z is formed again, a piece of the vocabulary at a time, with at
- * most 512 MiB of D in memory (or a tile of 256 words). D is held in fp16, over the
- * call's largest |g_r| or |l2wrap_scale max_r| and with what the power of two 2^13
- * makes of it: 11 bits of each element, but never finer than 2^-38 of that largest
- * factor; for fp32 operands in two such numbers, 22 bits (or whole, in three bf16
- * ones). The hidden gradient's
+ * most 512 MiB of D in memory (or a tile of 256 words). D is held in fp16, each row
+ * over the size of its own factors, |g_r| or |l2wrap_scale max_r|: 11 bits of each
+ * element, but never finer than 2^-37 of the row's larger factor; for fp32 operands in
+ * two such numbers, 22 bits (or whole, in three bf16 ones). The hidden gradient's
  * products round it to bf16 for bf16 operands, but for the target and the argmax,
- * whose error is put back; the weight gradient's are fp16, of hidden states scaled by
- * a power of two (exact but below 2^-27 of the largest magnitude).
+ * whose error is put back. The weight gradient's are fp16, of hidden states scaled by
+ * a power of two and by their row's factor over the largest row's: each holds 11 bits
+ * (22 for fp32 operands), but never finer than 2^-37 of the largest magnitude and
+ * factor. With bf16 operands the sums of the hidden gradient hold 2^14 of the weights:
+ * these are below 2^112 in magnitude.
  *
  * fp32 operands are multiplied as two fp16 numbers each, after a power of two that
  * brings the operand's largest magnitude to 2^13 .. 2^14: 22 bits of each element, but

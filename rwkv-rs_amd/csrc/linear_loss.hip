@@ -93,7 +93,8 @@ struct Matrix {
 
 // What a call's kernels leave to one another.
 struct Scalars {
-  float reference;     // D is held over this
+  float mantissa;      // of the rows' largest factor, 1 to 2: D is held over this,
+  int scale;           // and over 2^this, or what is less for a row of smaller factors
   int exponent[2];     // the fp16 arrays of x and w are 2^exponent as large
 };
 
@@ -168,6 +169,11 @@ __global__ __launch_bounds__(kWide) void rows_kernel(const RowsCall c) { number_
 // The largest magnitudes: of x but for the rows that are ignored (whatever stands there
 // is nobody's measure), of w, and of the rows' factors of D. Row y of the grid takes
 // array y; each workgroup leaves one number. A fourth row numbers the rows.
+//
+// A row's own power of two: D of each row is held over its own, so that a row of small
+// weight has as many bits of its hidden gradient as any other. The weight gradient, in which
+// the rows meet, takes the powers back on x (pack_kernel).
+constexpr int kLargestScale = INT_MAX;         // a row without a finite factor, or any of fp32 with few rows: as the largest
 struct SurveyCall {
   const void* from[2];       // null: not wanted
   int64_t n[2];              // rows
@@ -177,6 +183,8 @@ struct SurveyCall {
   int64_t rows, ignore_index;
   float l2wrap_scale;
   float* residuals;          // [2, rows], cleared; may be null
+  int* row_scale;            // [rows]
+  bool own_scales;           // or all rows' as the largest
   uint32_t* largest;         // [3, kMaxBlocks]
   RowsCall numbered;
 };
@@ -220,8 +228,9 @@ __global__ __launch_bounds__(kWide) void survey_kernel(const SurveyCall c) {
     if (!c.row_grad) return;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWide + threadIdx.x; r < c.rows; r += kMaxBlocks * kWide) {
       if (c.residuals) c.residuals[r] = c.residuals[c.rows + r] = 0.f;
-      if (c.targets[r] == c.ignore_index) continue;
-      most = max(most, max(finite_magnitude(c.row_grad[r]), finite_magnitude(c.l2wrap_scale * c.row_max[r])));
+      const uint32_t own = c.targets[r] == c.ignore_index ? 0 : max(finite_magnitude(c.row_grad[r]), finite_magnitude(c.l2wrap_scale * c.row_max[r]));
+      c.row_scale[r] = c.own_scales && own ? ilogbf(__builtin_bit_cast(float, own)) : kLargestScale;
+      most = max(most, own);
     }
   }
   most = block_max<kWide / 64>(most);
@@ -237,11 +246,13 @@ struct PackJob {
   char* to;
   int64_t rows;
   int kind, which;           // which: of the largest magnitudes
+  bool weighted;             // rows with the powers of two that D's rows are without
 };
 struct PackCall {
   PackJob job[3];
   int jobs, c, padded;
-  bool factors;              // the backward's reference is wanted
+  bool factors;              // the backward's mantissa and scale are wanted
+  const int* row_scale;
   const int64_t* targets;
   int64_t ignore_index;
   const int *index, *count;  // of x's rows that are taken; null: all
@@ -250,7 +261,9 @@ struct PackCall {
 };
 // fp16 arrays are of x s, s the power of two that brings the largest magnitude to 2^13
 // .. 2^14: bf16 numbers of 2^-27 of it and more are held whole, smaller ones to 2^-38 of
-// it; of fp32 ones the second array holds what is left, rounded to 11 bits or likewise.
+// it; of fp32 ones the second array holds what is left, rounded to 11 bits or likewise. For
+// the weight gradient a row is smaller by the power of two that its weight is below the
+// largest one's: its D is not, and what is lost is below 2^-38 of the largest of both.
 // Ignored rows of x are left out or become zeros: a NaN there does not reach the weight's
 // gradient.
 __device__ __forceinline__ int exponent_of(uint32_t largest) {
@@ -259,11 +272,16 @@ __device__ __forceinline__ int exponent_of(uint32_t largest) {
 __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
   const PackJob job = c.job[blockIdx.y];
   const bool writes = blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0;
-  int exponent = 0;
-  if (c.factors && blockIdx.x == 0 && blockIdx.y == 0) {
+  int exponent = 0, scale = 0;
+  if (c.factors && ((blockIdx.x == 0 && blockIdx.y == 0) || job.weighted)) {
     const uint32_t most = block_max<4>(c.largest[2 * kMaxBlocks + threadIdx.x]);
-    // a gradient that is the same for all rows leaves exactly one, and so its own rounding out of D
-    if (writes) c.scalars->reference = most ? __builtin_bit_cast(float, most) : 1.f;
+    const float largest = most ? __builtin_bit_cast(float, most) : 1.f;
+    scale = ilogbf(largest);
+    // a gradient that is the same for all rows leaves a power of two, and so its own rounding out of D
+    if (writes) {
+      c.scalars->mantissa = ldexpf(largest, -scale);
+      c.scalars->scale = scale;
+    }
   }
   if (static_cast<int>(blockIdx.y) >= c.jobs) return;
   if (job.kind == kToThirds) {
@@ -291,6 +309,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); row < rows; row += gridDim.x * int64_t{4}) {
     const int64_t source = some ? c.index[row] : row;
     const bool ignored = !some && job.kind != kCopy && job.which == 0 && c.targets[row] == c.ignore_index;
+    const int shift = exponent + (job.weighted ? min(c.row_scale[source], scale) - scale : 0);
     for (int i = lane; i < pieces; i += 64) {
       const int64_t at = source * c.c + 8 * i;
       if (ignored) {
@@ -319,7 +338,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
         f16x8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float s = ldexpf(v[e], exponent);
+          const float s = ldexpf(v[e], shift);
           hi[e] = static_cast<_Float16>(s);
           lo[e] = static_cast<_Float16>(s - static_cast<float>(hi[e]));
         }
@@ -341,7 +360,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackCall c) {
         } else {
           f16x8 h;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) h[e] = static_cast<_Float16>(ldexpf(static_cast<float>(raw[e]), exponent));
+          for (int e = 0; e < 8; ++e) h[e] = static_cast<_Float16>(ldexpf(static_cast<float>(raw[e]), shift));
           *reinterpret_cast<f16x8*>(to) = h;
         }
       }
@@ -364,8 +383,11 @@ struct LogitsCall {
   // backward
   const float *row_lse, *row_max, *row_grad;
   const int32_t* row_argmax;
+  const int* row_scale;
   float l2wrap_scale;
-  char* d;                       // [rows up to whole tiles, words] fp16; for fp32 two of them, or three of bf16
+  // [rows up to whole tiles, words] fp16, each row over its own power of two, so 2^15 at most;
+  // for fp32 two of them, or three of bf16
+  char* d;
   int64_t d_plane;
   float* residuals;              // [2, rows], bf16 operands: what rounding took from D at the target and at the argmax
 };
@@ -515,10 +537,11 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ,
         c.part_argmax[to] = f == INT_MAX ? INT_MAX : v + f;
       }
     } else if (!idle) {
-      const float reference = c.scalars->reference;
+      const float mantissa = c.scalars->mantissa;
+      const int scale = c.scalars->scale;
       struct Row {
         float lse, h, wrap;
-        int own, top;
+        int own, top, exponent;
         bool dead;
       } of[T::kTilesQ];
 #pragma unroll
@@ -531,12 +554,13 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ,
         of[j].lse = c.row_lse[known];
         of[j].h = c.row_grad[known];
         of[j].wrap = c.l2wrap_scale * c.row_max[known];
+        of[j].exponent = kHalfExponent - min(c.row_scale[known], scale);
       }
 #pragma unroll
       for (int j = 0; j < T::kTilesQ; ++j) {
         const int row = r + wq * T::kWaveQ + 16 * j + m;
-        const float lse = of[j].lse, h = ldexpf(of[j].h / reference, kHalfExponent);
-        const float wrap = ldexpf(of[j].wrap / reference, kHalfExponent);
+        const float lse = of[j].lse, h = ldexpf(of[j].h, of[j].exponent) / mantissa;
+        const float wrap = ldexpf(of[j].wrap, of[j].exponent) / mantissa;
         const int own = of[j].own, top = of[j].top;
         const bool dead = of[j].dead;
 #pragma unroll
@@ -675,28 +699,27 @@ struct HiddenCall {
   const float* residuals;
   const int64_t* targets;
   const int32_t* row_argmax;
+  const int* row_scale;
   const __bf16* weight;
 };
 // What the sums are multiplied with: one number from 1 to 2, then one power of two, so that
 // nothing on the way is larger or smaller than the result.
 struct Factor {
   float mantissa;
-  int exponent;
+  int exponent, scale;       // of a row of dx of smaller factors: its own scale's
+  __device__ __forceinline__ Factor of_row(int row_scale) const { return Factor{mantissa, exponent + min(row_scale, scale) - scale, scale}; }
 };
-__device__ __forceinline__ Factor factor_of(float reference, int exponent) {
-  const int scale = ilogbf(reference);
-  return Factor{ldexpf(reference, -scale), scale - kHalfExponent - exponent};
-}
 __device__ __forceinline__ f32x4 times(f32x4 v, Factor f) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e] * f.mantissa, f.exponent);
   return v;
 }
-__device__ __forceinline__ Factor weight_factor(const Scalars* s) { return factor_of(s->reference, s->exponent[0]); }
-template <bool BF>
-__device__ __forceinline__ Factor hidden_factor(const Scalars* s) {
-  return factor_of(s->reference, BF ? 0 : s->exponent[1]);
+__device__ __forceinline__ Factor factor_of(const Scalars* s, int exponent) {
+  return Factor{s->mantissa, s->scale - kHalfExponent - exponent, s->scale};
 }
+__device__ __forceinline__ Factor weight_factor(const Scalars* s) { return factor_of(s, s->exponent[0]); }
+template <bool BF>
+__device__ __forceinline__ Factor hidden_factor(const Scalars* s) { return factor_of(s, BF ? 0 : s->exponent[1]); }
 template <bool BF>
 __device__ __forceinline__ void finish_hidden(const HiddenCall& c, Factor f, int64_t row, int64_t part_row, int64_t channel, f32x4 v) {
   const bool whole = c.c % 8 == 0;
@@ -719,12 +742,12 @@ __device__ __forceinline__ void finish_hidden(const HiddenCall& c, Factor f, int
       for (int e = 0; e < 4; ++e) v[e] += r != 0.f ? r * static_cast<float>(w[e]) : 0.f;
     }
   }
-  store4<BF>(c.grad, row * c.c + channel, times(v, f), c.c - channel, whole);
+  store4<BF>(c.grad, row * c.c + channel, times(v, f.of_row(c.row_scale[row])), c.c - channel, whole);
 }
 
 constexpr int kGradTile = 256;   // words or rows of a gradient's tile
 struct GradientsCall {
-  Matrix x, w;               // x: fp16; w: bf16, or fp16 for fp32
+  Matrix x, w;               // x: fp16, weighted; w: bf16, or fp16 for fp32
   const char* d;
   int64_t d_plane;
   int first, words, padded_rows, rows, vocab, c;
@@ -972,7 +995,7 @@ int64_t take(int64_t& end, int64_t bytes) {
 }
 // Byte offsets of the operands in the workspace.
 struct Places {
-  int64_t scalars, largest, index, place, count, x, w, x_half, x_plane, w_plane;
+  int64_t scalars, largest, index, place, count, x, w, x_weighted, x_plane, w_plane;
   int64_t end;
 };
 Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward) {
@@ -993,7 +1016,7 @@ Places operands(int64_t rows, int64_t vocab, int64_t c, bool bf16, bool backward
   } else if (packed(c, bf16)) {
     p.w = take(p.end, planes * p.w_plane);
   }
-  if (bf16 && backward) p.x_half = take(p.end, p.x_plane);
+  if (backward && !few(rows, vocab, c, bf16)) p.x_weighted = take(p.end, planes * p.x_plane);
   return p;
 }
 
@@ -1078,7 +1101,7 @@ bool needs_sums(const Plan& p, int64_t rows, int64_t vocab, int64_t c, bool bf16
 }
 struct BackwardPlaces {
   Places operands;
-  int64_t d, d_plane, sums, weight_sums, residuals, end;
+  int64_t d, d_plane, sums, weight_sums, residuals, row_scale, end;
 };
 BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64_t c, bool bf16) {
   BackwardPlaces b{};
@@ -1089,6 +1112,7 @@ BackwardPlaces backward_places(const Plan& p, int64_t rows, int64_t vocab, int64
   b.sums = !needs_sums(p, rows, vocab, c, bf16) ? 0 : take(b.end, p.splits * rows * p.pitch * 4);
   b.weight_sums = p.row_splits == 1 ? 0 : take(b.end, p.row_splits * vocab * p.pitch * 4);
   b.residuals = take(b.end, 2 * rows * 4);
+  b.row_scale = take(b.end, rows * 4);
   return b;
 }
 
@@ -1138,14 +1162,15 @@ ForwardPlaces forward_places(int64_t rows, int64_t vocab, int64_t c, bool bf16) 
   return f;
 }
 
-// x and w as the tiles read them (and x in fp16 for bf16 operands' weight gradient), made
-// first where they are not so in memory; the rows' numbers; the backward's factors.
+// x and w as the tiles read them, and x as the weight gradient does (in fp16, with the rows'
+// powers of two), made first where they are not so in memory; the rows' numbers; the
+// backward's factors.
 struct Operands {
-  Matrix x, w, x_half;
+  Matrix x, w, x_weighted;
   const int *index, *place, *count;
 };
 template <bool BF>
-Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* residuals, hipStream_t s) {
+Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* residuals, int* row_scale, hipStream_t s) {
   const int64_t padded = up(c.c, kStep);
   Operands o{};
   o.x = Matrix{static_cast<const char*>(c.hidden), c.c * 2, 0};
@@ -1158,22 +1183,23 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
     o.count = r.count = reinterpret_cast<int*>(c.workspace + p.count);
   }
   PackCall k{};
-  auto pack = [&](const void* from, int64_t to, int64_t rows, int kind, int which, int64_t plane) {
-    k.job[k.jobs++] = PackJob{from, c.workspace + to, rows, kind, which};
+  auto pack = [&](const void* from, int64_t to, int64_t rows, int kind, int which, int64_t plane, bool weighted = false) {
+    k.job[k.jobs++] = PackJob{from, c.workspace + to, rows, kind, which, weighted};
     return Matrix{c.workspace + to, padded * 2, plane};
   };
   if (packed(c.c, BF) || r.index) o.x = pack(c.hidden, p.x, c.rows, BF ? kCopy : split ? kToThirds : kToHalves, 0, p.x_plane);
   if (split && c.c % 8 != 0) {
-    k.job[k.jobs++] = PackJob{c.weight, c.workspace + p.w, c.vocab, kEights, 1};
+    k.job[k.jobs++] = PackJob{c.weight, c.workspace + p.w, c.vocab, kEights, 1, false};
     o.w = Matrix{c.workspace + p.w, up(c.c, 8) * 4, 0};
   }
   if (packed(c.c, BF) && !split) o.w = pack(c.weight, p.w, c.vocab, BF ? kCopy : kToHalves, 1, p.w_plane);
-  o.x_half = o.x;
-  if (BF && b && b->weight_grad) o.x_half = pack(c.hidden, p.x_half, c.rows, kToHalf, 0, 0);
+  o.x_weighted = o.x;
+  if (b && b->weight_grad && !split) o.x_weighted = pack(c.hidden, p.x_weighted, c.rows, BF ? kToHalf : kToHalves, 0, BF ? 0 : p.x_plane, true);
   if (k.jobs == 0 && !b) return o;
   k.c = static_cast<int>(c.c);
   k.padded = static_cast<int>(padded);
   k.factors = b != nullptr;
+  k.row_scale = row_scale;
   k.index = o.index;
   k.count = o.count;
   uint32_t* const largest = reinterpret_cast<uint32_t*>(c.workspace + p.largest);
@@ -1195,6 +1221,8 @@ Operands prepare(const Call& c, const Places& p, const BackwardCall* b, float* r
     v.rows = c.rows;
     v.l2wrap_scale = b->l2wrap_scale;
     v.residuals = residuals;
+    v.row_scale = row_scale;
+    v.own_scales = !split;
   }
   if (v.from[0] || b) hipLaunchKernelGGL(survey_kernel<BF>, dim3(kMaxBlocks, r.index ? 4 : b ? 3 : 2), dim3(kWide), 0, s, v);
   else if (r.index) hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(kWide), 0, s, r);
@@ -1229,7 +1257,7 @@ void logits(const LogitsCall& l, int shape, hipStream_t s) {
 template <bool BF>
 void forward(const ForwardCall& c, hipStream_t s) {
   const ForwardPlaces f = forward_places(c.rows, c.vocab, c.c, BF);
-  const Operands o = prepare<BF>(c, f.operands, nullptr, nullptr, s);
+  const Operands o = prepare<BF>(c, f.operands, nullptr, nullptr, nullptr, s);
   LogitsCall l{};
   l.x = o.x;
   l.w = o.w;
@@ -1265,7 +1293,8 @@ void backward(const BackwardCall& c, hipStream_t s) {
   const Plan p = plan(c.rows, c.vocab, c.c, BF);
   const BackwardPlaces b = backward_places(p, c.rows, c.vocab, c.c, BF);
   float* const residuals = BF ? reinterpret_cast<float*>(c.workspace + b.residuals) : nullptr;
-  const Operands o = prepare<BF>(c, b.operands, &c, residuals, s);
+  int* const row_scale = reinterpret_cast<int*>(c.workspace + b.row_scale);
+  const Operands o = prepare<BF>(c, b.operands, &c, residuals, row_scale, s);
   const Scalars* const scalars = reinterpret_cast<const Scalars*>(c.workspace + b.operands.scalars);
   LogitsCall l{};
   l.x = o.x;
@@ -1283,12 +1312,13 @@ void backward(const BackwardCall& c, hipStream_t s) {
   l.row_max = c.row_max;
   l.row_grad = c.row_grad;
   l.row_argmax = c.row_argmax;
+  l.row_scale = row_scale;
   l.l2wrap_scale = c.l2wrap_scale;
   l.d = c.workspace + b.d;
   l.d_plane = b.d_plane;
   l.residuals = residuals;
   GradientsCall g{};
-  g.x = o.x_half;
+  g.x = o.x_weighted;
   g.w = o.w;
   g.count = o.count;
   g.d = l.d;
@@ -1304,7 +1334,7 @@ void backward(const BackwardCall& c, hipStream_t s) {
   g.share = static_cast<int>(p.share);
   const bool direct = !needs_sums(p, c.rows, c.vocab, c.c, BF);
   g.sums = direct ? nullptr : reinterpret_cast<float*>(c.workspace + b.sums);
-  g.hidden = HiddenCall{c.hidden_grad, c.c, c.rows, residuals, c.targets, c.row_argmax,
+  g.hidden = HiddenCall{c.hidden_grad, c.c, c.rows, residuals, c.targets, c.row_argmax, row_scale,
                         BF ? static_cast<const __bf16*>(c.weight) : nullptr};
   g.pitch = static_cast<int>(p.pitch);
   const int64_t channel_tiles = ceil_div(c.c, p.channels);

@@ -13,11 +13,13 @@ and |l2wrap term|, and F the largest of them,
 * a result below its type's normal numbers is rounded by half its last step (bf16 2^-134).
 """
 
+import math
+
 import pytest
 import torch
 
 from conftest import announce, load_pkg
-from test_gpu_linear_loss import DEV, U, logit_error, make
+from test_gpu_linear_loss import BOTH, DEV, U, logit_error, make
 
 pytestmark = pytest.mark.gpu
 ll = load_pkg().lm_loss
@@ -68,6 +70,40 @@ def check_gradients(x, w, t, g, num_tokens):
     miss = (dw.double() - exact).abs()
     assert (miss <= limit).all(), float((miss / limit).max())
     return loss, dx, dw
+
+
+# tiles of every size, sums and none, rows brought together, few rows of fp32, copied operands
+@pytest.mark.parametrize("dtype,rows,vocab,c", [
+    (torch.bfloat16, 40, 600, 64), (torch.float32, 40, 600, 64), (torch.bfloat16, 96, 256, 100), (torch.float32, 96, 256, 100),
+    (torch.float32, 256, 256, 256), (torch.bfloat16, 700, 3000, 192), (torch.float32, 700, 3000, 192),
+    (torch.bfloat16, 1100, 65536, 1024), (torch.float32, 300, 65536, 1024), (torch.float32, 50, 70000, 64)])
+def test_rows_of_any_weight(dtype, rows, vocab, c):
+    announce("linear loss, rows of any weight", dtype, rows, vocab, c)
+    x, w, t = make(rows, vocab, c, dtype, seed=rows, spread=1.0, lift=0.0)
+    t[3::9] = -100
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    weight = (1.0 + torch.rand(rows, generator=gen, device=DEV)) * torch.where(torch.arange(rows, device=DEV) % 2 == 0, 1.0, -1.0)
+    weight *= 2.0 ** -(1.5 * (torch.randperm(rows, generator=gen, device=DEV) % 41))
+    check_gradients(x, w, t, weight, 0)
+    check_gradients(x, w, t, weight, rows)               # l2wrap's term is the larger one for most rows
+    weight[::5] = 0.0
+    check_gradients(x, w, t, weight * 1e-8, 0)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_an_infinite_row_gradient(dtype):
+    """It is that row's alone, but for the weight gradient."""
+    announce("linear loss, an infinite row gradient", dtype)
+    x, w, t = make(30, 300, 64, dtype, seed=3)
+    g = torch.rand(30, device=DEV) + 0.1
+    g[7] = 0.0
+    clean = run(x, w, t, g, 30)
+    others = torch.arange(30, device=DEV) != 7
+    for bad in (math.inf, -math.inf, math.nan):
+        g[7] = bad
+        loss, dx, dw = run(x, w, t, g, 30)
+        assert torch.equal(loss, clean[0]) and torch.equal(dx[others], clean[1][others])
+        assert not dx[7].isfinite().any() and not dw[t[7]].isfinite().any()
 
 
 @pytest.mark.parametrize("dtype,scale_x,scale_w,size", [
