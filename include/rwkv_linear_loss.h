@@ -9,17 +9,20 @@
  *
  * Forward:
  *   z_rj   = sum_k hidden_rk weight_jk      (exact products, fp32 sums)
- *   lse_r  = log sum_j exp(z_rj)
- *   loss_r = lse_r - z_r,t_r
- * to row_loss, row_lse, row_max (fp32 [rows]) and row_argmax (int32 [rows], the
- * first index of the row's maximum); the last three are kept for the backward. A
+ *   max_r     = max_j z_rj
+ *   log_sum_r = log sum_j exp(z_rj - max_r)
+ *   loss_r    = (max_r - z_r,t_r) + log_sum_r
+ * to row_loss, row_log_sum, row_max (fp32 [rows]) and row_argmax (int32 [rows], the
+ * first index of the row's maximum); the last three are kept for the backward. The
+ * maximum and the logarithm stay apart: in one number they would be rounded to a
+ * step of the logits' size. A
  * row whose target is ignore_index has loss 0, and nothing depends on its hidden
  * state; one whose target is otherwise outside [0, vocab) has a NaN loss. A row with a NaN or
  * plus infinity among its logits has a NaN loss; minus infinity is a probability of
  * 0 (bf16 operands; fp32 ones' products make it NaN).
  *
  * Backward, with g_r = row_loss_grad[r] (fp32 [rows]):
- *   D_rj = g_r (exp(z_rj - lse_r) - [j == t_r]) + [j == argmax_r] l2wrap_scale max_r
+ *   D_rj = g_r (exp(z_rj - max_r - log_sum_r) - [j == t_r]) + [j == argmax_r] l2wrap_scale max_r
  *   hidden_grad = D weight,   weight_grad = D^T hidden
  * in dtype, each rounded once; either pointer may be NULL (not wanted). A row
  * whose target is ignore_index has D = 0; a target otherwise outside [0, vocab)
@@ -68,13 +71,13 @@ int64_t rwkv_linear_loss_backward_workspace_bytes(int64_t rows, int64_t vocab, i
 
 int rwkv_linear_loss_forward(const void *hidden, const void *weight, const int64_t *targets,
                              int64_t rows, int64_t vocab, int64_t c, int dtype,
-                             int64_t ignore_index, float *row_loss, float *row_lse,
+                             int64_t ignore_index, float *row_loss, float *row_log_sum,
                              float *row_max, int32_t *row_argmax, void *workspace,
                              int64_t workspace_bytes, void *stream);
 
-/* row_lse, row_max and row_argmax are the forward's of the same operands. */
+/* row_log_sum, row_max and row_argmax are the forward's of the same operands. */
 int rwkv_linear_loss_backward(const void *hidden, const void *weight, const int64_t *targets,
-                              const float *row_lse, const float *row_max,
+                              const float *row_log_sum, const float *row_max,
                               const int32_t *row_argmax, const float *row_loss_grad,
                               float l2wrap_scale, int64_t rows, int64_t vocab, int64_t c,
                               int dtype, int64_t ignore_index, void *hidden_grad,

@@ -381,7 +381,7 @@ struct LogitsCall {
   float *part_max, *part_sum, *row_target;
   int* part_argmax;
   // backward
-  const float *row_lse, *row_max, *row_grad;
+  const float *row_log_sum, *row_max, *row_grad;
   const int32_t* row_argmax;
   const int* row_scale;
   float l2wrap_scale;
@@ -540,7 +540,7 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ,
       const float mantissa = c.scalars->mantissa;
       const int scale = c.scalars->scale;
       struct Row {
-        float lse, h, wrap;
+        float log_sum, h, most;
         int own, top, exponent;
         bool dead;
       } of[T::kTilesQ];
@@ -551,23 +551,25 @@ __global__ __launch_bounds__(64 * Shape::kWavesP * Shape::kWavesQ,
         of[j].dead = row >= rows || target == c.ignore_index;
         of[j].own = target >= 0 && target < c.vocab ? static_cast<int>(target) - word0 : -1;
         of[j].top = c.row_argmax[known] - word0;
-        of[j].lse = c.row_lse[known];
+        of[j].log_sum = c.row_log_sum[known];
         of[j].h = c.row_grad[known];
-        of[j].wrap = c.l2wrap_scale * c.row_max[known];
+        of[j].most = c.row_max[known];
         of[j].exponent = kHalfExponent - min(c.row_scale[known], scale);
       }
 #pragma unroll
       for (int j = 0; j < T::kTilesQ; ++j) {
         const int row = r + wq * T::kWaveQ + 16 * j + m;
-        const float lse = of[j].lse, h = ldexpf(of[j].h, of[j].exponent) / mantissa;
-        const float wrap = ldexpf(of[j].wrap, of[j].exponent) / mantissa;
+        const float most = of[j].most, h = ldexpf(of[j].h, of[j].exponent) / mantissa;
+        const float wrap = ldexpf(c.l2wrap_scale * most, of[j].exponent) / mantissa;
+        // exp(z - max) is as exact as z, however large that is, which max + log_sum in one number would not leave it
+        const float share = h * expf(-of[j].log_sum);
         const int own = of[j].own, top = of[j].top;
         const bool dead = of[j].dead;
 #pragma unroll
         for (int pair = 0; pair < T::kTilesP / 2; ++pair) {
           float d[8];
 #pragma unroll
-          for (int n = 0; n < 8; ++n) d[n] = h * __expf(t.acc[2 * pair + n / 4][j][n % 4] - lse);
+          for (int n = 0; n < 8; ++n) d[n] = share * __expf(t.acc[2 * pair + n / 4][j][n % 4] - most);
           const bool has_own = own >= 32 * pair && own < 32 * pair + 8, has_top = top >= 32 * pair && top < 32 * pair + 8;
           if (has_own || has_top) {
 #pragma unroll
@@ -621,7 +623,7 @@ struct JoinCall {
   const int* place;          // of each row among the parts' rows; null: as it is
   int64_t rows, vocab, ignore_index;
   int words;                 // of a tile
-  float *row_loss, *row_lse, *row_max;
+  float *row_loss, *row_log_sum, *row_max;
   int32_t* row_argmax;
 };
 struct Run {
@@ -655,14 +657,14 @@ __global__ __launch_bounds__(kJoinRows * kJoinShares) void join_kernel(const Joi
     if (share < s) run = combine(run, part[share + s][own]);
   }
   if (share > 0 || row >= c.rows) return;
-  const float lse = run.most + logf(run.sum);
+  const float log_sum = logf(run.sum);
   const int64_t target = c.targets[row];
-  c.row_lse[row] = lse;
+  c.row_log_sum[row] = log_sum;
   c.row_max[row] = run.most;
   c.row_argmax[row] = run.first;
   float loss = target == c.ignore_index ? 0.f : NAN;
-  if (target != c.ignore_index && target >= 0 && target < c.vocab && lse == lse) {
-    loss = lse - c.row_target[part_row];
+  if (target != c.ignore_index && target >= 0 && target < c.vocab && log_sum == log_sum) {
+    loss = run.most - c.row_target[part_row] + log_sum;   // of two large logits the difference first
     loss = loss < 0.f ? 0.f : loss;   // a logit is at most the sum's logarithm: no rounding makes a loss negative
   }
   c.row_loss[row] = loss;
@@ -1277,7 +1279,7 @@ void forward(const ForwardCall& c, hipStream_t s) {
   const int shape = shape_of(c.rows, c.vocab, c.c, BF, few(c.rows, c.vocab, c.c, BF));
   logits<BF, false>(l, shape, s);
   const JoinCall j{l.part_max, l.part_sum, l.row_target, l.part_argmax, c.targets, o.place, c.rows, c.vocab, c.ignore_index, shape_words(shape),
-                   c.row_loss, c.row_lse, c.row_max, c.row_argmax};
+                   c.row_loss, c.row_log_sum, c.row_max, c.row_argmax};
   hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>(ceil_div(c.rows, kJoinRows))), dim3(kJoinRows * kJoinShares), 0, s, j);
 }
 
@@ -1308,7 +1310,7 @@ void backward(const BackwardCall& c, hipStream_t s) {
   l.scalars = scalars;
   l.targets = c.targets;
   l.ignore_index = c.ignore_index;
-  l.row_lse = c.row_lse;
+  l.row_log_sum = c.row_log_sum;
   l.row_max = c.row_max;
   l.row_grad = c.row_grad;
   l.row_argmax = c.row_argmax;

@@ -63,7 +63,7 @@ int64_t rwkv_linear_loss_backward_workspace_bytes(int64_t rows, int64_t vocab, i
 
 int rwkv_linear_loss_forward(const void* hidden, const void* weight, const int64_t* targets, int64_t rows,
                              int64_t vocab, int64_t c, int dtype, int64_t ignore_index, float* row_loss,
-                             float* row_lse, float* row_max, int32_t* row_argmax, void* workspace,
+                             float* row_log_sum, float* row_max, int32_t* row_argmax, void* workspace,
                              int64_t workspace_bytes, void* stream) {
   if (!dtype_ok(dtype)) return WKV7_ERR_DTYPE;
   if (!sizes_ok(rows, vocab, c)) return WKV7_ERR_SHAPE;
@@ -71,14 +71,14 @@ int rwkv_linear_loss_forward(const void* hidden, const void* weight, const int64
   const bool bf16 = dtype == WKV7_DTYPE_BF16;
   const int64_t need = rwkv_linear_loss::forward_workspace_bytes(rows, vocab, c, bf16);
   if (workspace_bytes < need) return WKV7_ERR_SHAPE;
-  if (!hidden || !weight || !targets || !row_loss || !row_lse || !row_max || !row_argmax || !workspace)
+  if (!hidden || !weight || !targets || !row_loss || !row_log_sum || !row_max || !row_argmax || !workspace)
     return WKV7_ERR_NULL_POINTER;
   const uintptr_t a = row_alignment(c, dtype);
   if (!aligned(hidden, a) || !aligned(weight, a) || !aligned(targets, 8) || !aligned(row_loss, 4) ||
-      !aligned(row_lse, 4) || !aligned(row_max, 4) || !aligned(row_argmax, 4) || !aligned(workspace, 16))
+      !aligned(row_log_sum, 4) || !aligned(row_max, 4) || !aligned(row_argmax, 4) || !aligned(workspace, 16))
     return WKV7_ERR_ALIGNMENT;
   const int64_t rb = rows * 4;
-  if (any_overlap({{row_loss, rb}, {row_lse, rb}, {row_max, rb}, {row_argmax, rb}, {workspace, need}},
+  if (any_overlap({{row_loss, rb}, {row_log_sum, rb}, {row_max, rb}, {row_argmax, rb}, {workspace, need}},
                   {{hidden, rows * c * size_of(dtype)}, {weight, vocab * c * size_of(dtype)}, {targets, rows * 8}}))
     return WKV7_ERR_OVERLAP;
   rwkv_linear_loss::ForwardCall f{};
@@ -92,13 +92,13 @@ int rwkv_linear_loss_forward(const void* hidden, const void* weight, const int64
   f.bf16 = bf16;
   f.workspace = static_cast<char*>(workspace);
   f.row_loss = row_loss;
-  f.row_lse = row_lse;
+  f.row_log_sum = row_log_sum;
   f.row_max = row_max;
   f.row_argmax = row_argmax;
   return wkv7::hip_status(rwkv_linear_loss::launch_forward(f, static_cast<hipStream_t>(stream)));
 }
 
-int rwkv_linear_loss_backward(const void* hidden, const void* weight, const int64_t* targets, const float* row_lse,
+int rwkv_linear_loss_backward(const void* hidden, const void* weight, const int64_t* targets, const float* row_log_sum,
                               const float* row_max, const int32_t* row_argmax, const float* row_loss_grad,
                               float l2wrap_scale, int64_t rows, int64_t vocab, int64_t c, int dtype,
                               int64_t ignore_index, void* hidden_grad, void* weight_grad, void* workspace,
@@ -111,15 +111,15 @@ int rwkv_linear_loss_backward(const void* hidden, const void* weight, const int6
   if (rows == 0 && !weight_grad) return WKV7_OK;
   const int64_t need = rwkv_linear_loss::backward_workspace_bytes(rows, vocab, c, bf16);
   if (workspace_bytes < need) return WKV7_ERR_SHAPE;
-  if (rows > 0 && (!hidden || !weight || !targets || !row_lse || !row_max || !row_argmax || !row_loss_grad || !workspace))
+  if (rows > 0 && (!hidden || !weight || !targets || !row_log_sum || !row_max || !row_argmax || !row_loss_grad || !workspace))
     return WKV7_ERR_NULL_POINTER;
   if (!aligned(hidden, a) || !aligned(weight, a) || !aligned(hidden_grad, a) || !aligned(weight_grad, a) ||
-      !aligned(targets, 8) || !aligned(row_lse, 4) || !aligned(row_max, 4) || !aligned(row_argmax, 4) ||
+      !aligned(targets, 8) || !aligned(row_log_sum, 4) || !aligned(row_max, 4) || !aligned(row_argmax, 4) ||
       !aligned(row_loss_grad, 4) || !aligned(workspace, 16))
     return WKV7_ERR_ALIGNMENT;
   const int64_t rb = rows * 4, hb = rows * c * size_of(dtype), wb = vocab * c * size_of(dtype);
   if (any_overlap({{hidden_grad, hb}, {weight_grad, wb}, {workspace, need}},
-                  {{hidden, hb}, {weight, wb}, {targets, rows * 8}, {row_lse, rb}, {row_max, rb}, {row_argmax, rb},
+                  {{hidden, hb}, {weight, wb}, {targets, rows * 8}, {row_log_sum, rb}, {row_max, rb}, {row_argmax, rb},
                    {row_loss_grad, rb}}))
     return WKV7_ERR_OVERLAP;
   rwkv_linear_loss::BackwardCall b{};
@@ -132,7 +132,7 @@ int rwkv_linear_loss_backward(const void* hidden, const void* weight, const int6
   b.ignore_index = ignore_index;
   b.bf16 = bf16;
   b.workspace = static_cast<char*>(workspace);
-  b.row_lse = row_lse;
+  b.row_log_sum = row_log_sum;
   b.row_max = row_max;
   b.row_argmax = row_argmax;
   b.row_grad = row_loss_grad;

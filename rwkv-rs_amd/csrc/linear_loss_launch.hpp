@@ -16,11 +16,11 @@ struct Call {
   char* workspace;
 };
 struct ForwardCall : Call {
-  float *row_loss, *row_lse, *row_max;
+  float *row_loss, *row_log_sum, *row_max;
   int32_t* row_argmax;
 };
 struct BackwardCall : Call {
-  const float *row_lse, *row_max;
+  const float *row_log_sum, *row_max;
   const int32_t* row_argmax;
   const float* row_grad;
   float l2wrap_scale;

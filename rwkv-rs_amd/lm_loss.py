@@ -101,8 +101,8 @@ def _workspace(nbytes: int, device) -> torch.Tensor:
 
 
 def _linear_forward(hidden, weight, targets, ignore_index):
-    """Every row's loss, and what the backward needs of it: a [3, rows] tensor of its
-    log-sum-exp, its maximum and (as int32) its argmax."""
+    """Every row's loss, and what the backward needs of it: a [3, rows] tensor of the logarithm
+    of its exponentials' sum over its maximum, that maximum and (as int32) its argmax."""
     (rows, c), vocab, dev = hidden.shape, weight.shape[0], hidden.device
     code, lib = _code(hidden.dtype), _native.lib()
     nbytes = lib.rwkv_linear_loss_forward_workspace_bytes(rows, vocab, c, code)

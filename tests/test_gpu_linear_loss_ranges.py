@@ -119,3 +119,54 @@ def test_operands_near_the_ends_of_their_type(dtype, scale_x, scale_w, size):
     g = torch.full((1024,), 2.0 ** size, device=DEV)
     loss, dx, dw = check_gradients(x, w, t, g, 0)
     assert loss.isfinite().all() and dx.isfinite().all() and dw.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("vocab", [100, 9000, 70000])
+def test_logits_far_from_zero(vocab, dtype):
+    """Logits of 2^17 and an eighth's multiple up to 8, which both types and fp32 sums hold whole:
+    losses and probabilities are those of the multiples alone. The exponentials' sum is
+    within ``adds`` roundings and an exponential's 2^-20."""
+    announce("linear loss, logits far from zero", vocab, dtype)
+    rows = 20
+    gen = torch.Generator(device=DEV).manual_seed(vocab)
+    x, w = torch.zeros(rows, 64, device=DEV), torch.zeros(vocab, 64, device=DEV)
+    x[:, 0], x[:, 1], w[:, 0] = 2.0 ** 8, 1.0, 2.0 ** 9
+    w[:, 1] = torch.randint(-64, 65, (vocab,), generator=gen, device=DEV) / 8.0
+    t = torch.randint(0, vocab, (rows,), generator=gen, device=DEV)
+    g = torch.rand(rows, generator=gen, device=DEV) + 0.5
+    loss, _, dw = run(x.to(dtype), w.to(dtype), t, g, 0)
+    z = w[:, 1].double()
+    lse = torch.logsumexp(z, 0)
+    adds = (32 + 5 + -(-vocab // 1024) + 17) * 2 * U + 2.0 ** -20
+    want = lse - z[t]
+    assert ((loss.double() - want).abs() <= adds + 4 * U * want).all()
+    d = g.double()[:, None] * torch.exp(z - lse)[None, :]
+    held = d * (adds + 2.0 ** -19 + (2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -22)) + 2.0 ** -37 * g.double()[:, None]
+    d[torch.arange(rows), t] -= g.double()
+    held[torch.arange(rows), t] += (2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -21) * g.double()
+    for channel, of in ((0, 2.0 ** 8), (1, 1.0)):
+        exact, size = of * d.sum(0), of * d.abs().sum(0)
+        limit = of * held.sum(0) + size * (3 * rows + 64) * 2 * U + exact.abs() * (2.0 ** -8 if dtype == torch.bfloat16 else 2 * U)
+        miss = (dw[:, channel].double() - exact).abs()
+        assert (miss <= limit).all(), float((miss / limit).max())
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_two_sure_words(dtype):
+    """Equal words far from zero share the probability; a word 15 below another has
+    exp(-15) of it, which the loss holds to a few steps of the sum, 2^-24 each."""
+    announce("linear loss, two sure words", dtype)
+    x, w = torch.zeros(1, 64, device=DEV), torch.full((300, 64), 0.0, device=DEV)
+    x[:, 0] = 2.0 ** 8
+    w[3, 0] = w[70, 0] = 2.0 ** 9
+    t, one = torch.tensor([70], device=DEV), torch.ones(1, device=DEV)
+    loss, _, dw = run(x.to(dtype), w.to(dtype), t, one, 0)
+    assert abs(float(loss) - math.log(2)) <= 2.0 ** -22
+    # 2^-20 of an exponential, and the results' rounding: 0.5 itself is held whole
+    near = 2.0 ** -8 + 2.0 ** -19 if dtype == torch.bfloat16 else 2.0 ** -18
+    assert abs(float(dw[3, 0]) / 128 - 1) <= near and abs(float(dw[70, 0]) / -128 - 1) <= near
+    x[:, 0], w[:, 0] = 1.0, -40.0
+    w[3, 0], w[70, 0] = 15.0, 30.0
+    loss, _, _ = run(x.to(dtype), w.to(dtype), t, one, 0)
+    assert abs(float(loss) - math.log1p(math.exp(-15.0))) <= 2.0 ** -22
