@@ -576,7 +576,9 @@ class AutoRegressiveModel(nn.Module):
     ``dropout``: in training mode each mixer's output is dropped with this
     probability where it joins the residual stream (``dropout.dropout_add``). The
     masks follow from ``dropout_rng``, an int64 buffer [seed, step] that is no part of the
-    state dict: each forward that draws takes the step it finds and counts it up. Ranks
+    state dict: each forward that draws takes the step it finds and counts it up. A
+    checkpoint may therefore recompute cells, whose masks are an argument, but not the whole
+    forward, which is refused. Ranks
     that train on data of their own want seeds of their own, and a wrapper that does not
     broadcast buffers.
 
@@ -619,6 +621,9 @@ class AutoRegressiveModel(nn.Module):
         """[seed, step] of a forward that drops, or None."""
         if self.dropout == 0.0 or not self.training:
             return None
+        if torch._C._current_graph_task_id() != -1:     # inside of a backward pass
+            raise RuntimeError("a forward that drops would be computed again with another step's masks: "
+                               "checkpoint the cells, which are given theirs, not the model")
         rng = self.dropout_rng.clone()      # the forward's own: the backward reads it again
         self.dropout_rng[1] += 1
         return rng
