@@ -575,12 +575,11 @@ class AutoRegressiveModel(nn.Module):
 
     ``dropout``: in training mode each mixer's output is dropped with this
     probability where it joins the residual stream (``dropout.dropout_add``). The
-    masks follow from ``dropout_rng``, an int64 buffer [seed, step] that is no part of the
-    state dict: each forward that draws takes the step it finds and counts it up. A
-    checkpoint may therefore recompute cells, whose masks are an argument, but not the whole
-    forward, which is refused. Ranks
-    that train on data of their own want seeds of their own, and a wrapper that does not
-    broadcast buffers.
+    masks follow from ``dropout_rng``, an int64 buffer [seed, step] (None without dropout) that
+    is no part of the state dict: each forward that draws takes the step it finds and counts
+    it up. A checkpoint may therefore recompute cells, whose masks are an argument, but not
+    the whole forward, which is refused. Ranks that train on data of their own want seeds of
+    their own, and a wrapper that does not broadcast buffers.
 
     ``loss``: "logits" forms them for the loss; "pieces" does not keep them
     (``lm_loss.linear_cross_entropy_l2wrap``), needs the "hip" neighbour ops, and
@@ -610,11 +609,16 @@ class AutoRegressiveModel(nn.Module):
         self.vocab_size = vocab_size
         self.neighbor_ops = _check_neighbor_ops(neighbor_ops)
         self.dropout, self.loss = dropout, loss
-        self.register_buffer("dropout_rng", torch.zeros(2, dtype=torch.int64), persistent=False)
+        # none without dropout: wrappers broadcast a model's buffers before each forward
+        self.register_buffer("dropout_rng", torch.zeros(2, dtype=torch.int64) if dropout else None,
+                             persistent=False)
+        self._dropout_seed = [0, 0]      # of a model that begins to drop later
 
     def seed_dropout(self, seed: int, step: int = 0):
         """The masks of the forwards to come: those of ``seed`` from ``step`` on."""
-        self.dropout_rng.copy_(torch.tensor([seed, step], dtype=torch.int64))
+        self._dropout_seed = [seed, step]
+        if self.dropout_rng is not None:
+            self.dropout_rng.copy_(torch.tensor(self._dropout_seed, dtype=torch.int64))
         return self
 
     def _draw(self) -> Optional[torch.Tensor]:
@@ -624,6 +628,8 @@ class AutoRegressiveModel(nn.Module):
         if torch._C._current_graph_task_id() != -1:     # inside of a backward pass
             raise RuntimeError("a forward that drops would be computed again with another step's masks: "
                                "checkpoint the cells, which are given theirs, not the model")
+        if self.dropout_rng is None:
+            self.dropout_rng = torch.tensor(self._dropout_seed, dtype=torch.int64, device=self.embed.weight.device)
         rng = self.dropout_rng.clone()      # the forward's own: the backward reads it again
         self.dropout_rng[1] += 1
         return rng

@@ -1,4 +1,4 @@
-"""The model's dropout state on the CPU: what a recomputed forward does."""
+"""The model's dropout state on the CPU: who has one, and what a recomputed forward does."""
 
 import functools
 
@@ -53,3 +53,20 @@ def test_cells_computed_again_take_their_own_masks(reentrant):
     got = grads(model, model(inputs, targets, TorchKernel))
     assert model.dropout_rng.tolist() == [3, 8]
     assert want.keys() == got.keys() and all(torch.equal(want[n], got[n]) for n in want)
+
+
+def test_a_model_that_does_not_drop_has_no_buffer():
+    """Wrappers broadcast a model's buffers before each forward: one that does not drop has
+    none, as before there was dropout."""
+    model = build(0.0)
+    assert not list(model.buffers()) and model.dropout_rng is None
+    assert model.seed_dropout(5, 2) is model and not list(model.buffers())
+    inputs, targets = tokens(2, 32, 97)
+    assert torch.isfinite(model.train()(inputs, targets, TorchKernel))
+    assert [n for n, _ in build().named_buffers()] == ["dropout_rng"]
+    # one that begins to drop later begins where it was told
+    model.dropout = 0.25
+    for cell in model.cells.cells:
+        cell.dropout = 0.25
+    assert torch.equal(model(inputs, targets, TorchKernel), build().seed_dropout(5, 2)(inputs, targets, TorchKernel))
+    assert model.dropout_rng.tolist() == [5, 3]
