@@ -957,9 +957,10 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumCall c) {
   }
 }
 
-__global__ __launch_bounds__(256) void clear_kernel(uint32_t* to, int64_t words, int64_t bytes) {
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < words; i += static_cast<int64_t>(gridDim.x) * 256) to[i] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0 && bytes % 4) *reinterpret_cast<uint16_t*>(to + words) = 0;
+// by elements: where c is no multiple of 8, a gradient may begin at any of them
+template <typename Element>
+__global__ __launch_bounds__(256) void clear_kernel(Element* to, int64_t n) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) to[i] = 0;
 }
 
 // ------------------------------------------------------------------ plan, workspace
@@ -1397,9 +1398,9 @@ hipError_t launch_forward(const ForwardCall& c, hipStream_t s) {
 
 hipError_t launch_backward(const BackwardCall& c, hipStream_t s) {
   if (c.rows == 0) {   // no row: no gradient of the weight
-    const int64_t bytes = c.vocab * c.c * (c.bf16 ? 2 : 4);
-    hipLaunchKernelGGL(clear_kernel, grid_of(bytes / 4 + 1), dim3(256), 0, s,
-                       static_cast<uint32_t*>(c.weight_grad), bytes / 4, bytes);
+    const int64_t n = c.vocab * c.c;
+    if (c.bf16) hipLaunchKernelGGL(clear_kernel<uint16_t>, grid_of(n), dim3(256), 0, s, static_cast<uint16_t*>(c.weight_grad), n);
+    else hipLaunchKernelGGL(clear_kernel<uint32_t>, grid_of(n), dim3(256), 0, s, static_cast<uint32_t*>(c.weight_grad), n);
   } else {
     c.bf16 ? backward<true>(c, s) : backward<false>(c, s);
   }
