@@ -56,8 +56,10 @@ struct Deep {
 };
 // Of fp32 operands where there are few rows: w is split on its way to the products. 256
 // words a workgroup keep 64 KiB of w on their way to each compute unit; the small one is
-// for few words, of which the large one makes too few workgroups (8 rows of 2048 with 8000
-// words: 57 us for 92).
+// for up to 64 rows of 12288 (below, this form does not run) to 16384 words, of which the
+// large one makes a workgroup on a quarter of the units at most: both calls, us, on the large
+// one and on the small, 64 x 344 x 12288 85 and 71, 8 x 768 x 12288 126 and 98, 64 x 2048 x
+// 12288 249 and 178, 64 x 4096 x 16384 518 and 373.
 struct Few {
   static constexpr int kWords = 256, kRows = 64, kWavesP = 4, kWavesQ = 1, kEach = 1, kSlots = 3;
 };
