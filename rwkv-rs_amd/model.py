@@ -569,6 +569,14 @@ class MultiCausalCells(nn.Module):
 LOSSES = ("logits", "pieces")
 
 
+def _is_its_weight(layer: nn.Module) -> bool:
+    """A linear layer that can be had without calling it: of no other kind, without a bias,
+    and with nothing that runs when it is called."""
+    return (type(layer) is nn.Linear and layer.bias is None and "forward" not in vars(layer)
+            and not (layer._forward_pre_hooks or layer._forward_hooks
+                     or layer._backward_pre_hooks or layer._backward_hooks))
+
+
 class AutoRegressiveModel(nn.Module):
     """examples/rwkv-lm/src/model.rs:50-176: embedding, layer norm, the
     cells, layer norm, unembedding, l2wrap and mean cross entropy.
@@ -584,9 +592,8 @@ class AutoRegressiveModel(nn.Module):
     ``loss``: "logits" forms them for the loss; "pieces" does not keep them
     (``lm_loss.linear_cross_entropy_l2wrap``), needs the "hip" neighbour ops, and
     leaves out targets of ``lm_loss.IGNORE_INDEX``. An unembedding that is no plain
-    linear layer without a bias any more (4-bit weights) has its logits formed all the
-    same, with those targets left out too; that of one is not called, so a hook on it does
-    not run."""
+    linear layer any more (4-bit weights, a bias, hooks, which may make its weight anew as
+    pruning does) has its logits formed all the same, with those targets left out too."""
 
     def __init__(self, vocab_size: int, num_cells: int, embedded_dim: int, num_heads: int,
                  head_size: int = 64, wkv7_dtype: torch.dtype = torch.bfloat16,
@@ -748,7 +755,7 @@ class AutoRegressiveModel(nn.Module):
         x, _, _, _ = self.cells(x, batch_ids, kernel, dropout_rng=self._draw())
         n = B * T
         x = self.layer_norm_for_unembed(x)
-        if self.loss == "pieces" and type(self.unembed) is nn.Linear and self.unembed.bias is None:
+        if self.loss == "pieces" and _is_its_weight(self.unembed):
             weight = self.unembed.weight
             dtype = _matmul_dtype(weight)
             hidden = x.reshape(n, x.shape[-1]).to(dtype)
