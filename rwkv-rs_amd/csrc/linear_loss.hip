@@ -13,7 +13,7 @@
 // and sums in all, where 6 would do with the logits in memory. The matrix cores, and the
 // power that they take, bound all three for many rows. For 7168 learned rows of 8192, c =
 // 768, 65536 words in bf16 (us, PFLOP/s; torch's own products of 8192 rows in brackets):
-// logits 623 to 690, 1.05 to 1.16 (812, 1.02); D 762 to 800, 0.9 (as the logits, and 1
+// logits 623 to 690, 1.05 to 1.16 (812, 1.02); D 746 to 802, 0.9 (as the logits, and 1
 // GiB written); dw and dx together 1280 to 1380, 1.05 to 1.13 (858 and 848, 0.97).
 // A product of 8192 cubed reaches 1.49 here, one of 16384 cubed 1.65.
 // For few rows it is memory: 64 rows of the same, 26 us for the loss, of which 20 are
